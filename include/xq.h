@@ -670,6 +670,48 @@ int xq_mlp_fwd_infer(const xq_weight* gate, const xq_weight* up, const xq_weight
                      const void* x, int64_t ldx, int64_t M, void* y, int64_t ldy, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
+/* ---- optimizer step over many tensors ----------------------------------- */
+/* One AdamW step over n tensors (the factors of a model, a trained head): the counterpart of the reference's optimizer
+ * construction (optim/optimizer.py; the update rule is that of torch.optim.AdamW) for the parameters this library produces gradients of.
+ *   m' = b1 m + (1 - b1) g ; v' = b2 v + (1 - b2) g^2 ; t = ++*step
+ *   p' = p - lr wd p - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)
+ * in fp32, rounded once to a bf16 parameter.  Tensors are dense runs of numel elements; types may differ from tensor to tensor.  No two
+ * tensors may share a parameter, a state or a step count.
+ * state_bits 32: exp_avg, exp_avg_sq are fp32[numel].  8: int8[numel] / uint8[numel] codes with fp32[ceil(numel / 256)] scales each,
+ * m = sign(c) (c/127)^2 scale, sqrt(v) = (d/255)^2 scale for 256 consecutive elements; all zero is a valid first state.
+ * norm: device fp32; the 2-norm over all gradients is written there (norm_given: it is read instead, as xq_grad_norm or a sum over
+ * ranks left it) and the gradients are scaled by min(1, max_norm / (norm + 1e-6)).  NULL: no clipping.
+ * lr_device: device fp32 that replaces lr (a schedule under a captured graph), or NULL.  The array of tensors is host memory and may go
+ * when the call returns. */
+typedef struct xq_adamw_tensor {
+    void* param;
+    const void* grad;
+    void* exp_avg;
+    void* exp_avg_sq;
+    float* exp_avg_scale;       /* 8-bit states only */
+    float* exp_avg_sq_scale;
+    float* step;                /* steps taken so far, one float */
+    int64_t numel;
+    int32_t param_dtype, grad_dtype;    /* XQ_DT_* */
+} xq_adamw_tensor;
+
+typedef struct xq_adamw_options {
+    double lr, beta1, beta2, eps, weight_decay, max_norm;
+    const float* lr_device;
+    float* norm;
+    int32_t norm_given;
+    int32_t state_bits;
+} xq_adamw_options;
+
+int64_t xq_adamw_workspace_bytes(int64_t n_tensors);
+int xq_adamw_step(const xq_adamw_tensor* tensors, int64_t n, const xq_adamw_options* options, void* workspace,
+                  int64_t workspace_bytes, void* stream);
+/* The 2-norm over n gradients (grad, grad_dtype and numel are read), summed in 64 bits in an order that the sizes fix. */
+int xq_grad_norm(const xq_adamw_tensor* tensors, int64_t n, float* norm, void* workspace, int64_t workspace_bytes, void* stream);
+/* What 8-bit states stand for: exp_avg and exp_avg_sq (the squares of what the codes hold) as fp32 or bf16 */
+int xq_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale, const float* exp_avg_sq_scale,
+                    int64_t numel, void* exp_avg_out, void* exp_avg_sq_out, int out_dtype, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -79,6 +79,16 @@ class XqMlpGrads(ctypes.Structure):
     _fields_ = [("dA", ctypes.c_void_p * 3), ("dB", ctypes.c_void_p * 3)]
 
 
+class XqAdamwTensor(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step")] + [
+        ("numel", ctypes.c_int64), ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32)]
+
+
+class XqAdamwOptions(ctypes.Structure):
+    _fields_ = [(n, ctypes.c_double) for n in ("lr", "beta1", "beta2", "eps", "weight_decay", "max_norm")] + [
+        ("lr_device", ctypes.c_void_p), ("norm", ctypes.c_void_p), ("norm_given", ctypes.c_int32), ("state_bits", ctypes.c_int32)]
+
+
 class XqError(ValueError):
     """Argument error reported by the library before any launch."""
 
@@ -200,6 +210,13 @@ _SIGNATURES = {
     # gate, up, down, lora, x, ldx, dy, lddy, M, saved, dx, lddx, grads, ws, ws_bytes, stream
     "xq_mlp_bwd": (_INT, [_W, _W, _W, ctypes.POINTER(XqMlpLora), _P, _I64, _P, _I64, _I64, ctypes.POINTER(XqMlpSaved), _P,
                           _I64, ctypes.POINTER(XqMlpGrads), _P, _I64, _P]),
+    "xq_adamw_workspace_bytes": (_I64, [_I64]),
+    # tensors, n, options, ws, ws_bytes, stream
+    "xq_adamw_step": (_INT, [ctypes.POINTER(XqAdamwTensor), _I64, ctypes.POINTER(XqAdamwOptions), _P, _I64, _P]),
+    # tensors, n, norm, ws, ws_bytes, stream
+    "xq_grad_norm": (_INT, [ctypes.POINTER(XqAdamwTensor), _I64, _P, _P, _I64, _P]),
+    # exp_avg, exp_avg_sq, their scales, numel, exp_avg_out, exp_avg_sq_out, out_dtype, stream
+    "xq_adamw_values": (_INT, [_P, _P, _P, _P, _I64, _P, _P, _INT, _P]),
 }
 
 EXPORTS = ("xq_version", "xq_last_error") + tuple(_SIGNATURES)

@@ -1,0 +1,436 @@
+// AdamW over many tensors at once, with 32- or 8-bit states, and the global norm of their gradients.
+//
+//   m' = b1 m + (1 - b1) g        v' = b2 v + (1 - b2) g^2        t = step + 1
+//   p' = p - lr wd p - lr / (1 - b1^t) * m' / (sqrt(v') / sqrt(1 - b2^t) + eps)            g scaled by min(1, max_norm / (|g| + 1e-6))
+//
+// 8-bit states: blocks of 256 consecutive elements of a tensor share a scale each for m and for s = sqrt(v):
+//   m = sign(c) (c / 127)^2 A_m   c in -127 .. 127          s = (d / 255)^2 A_s   d in 0 .. 255          A = the block's largest magnitude
+// The squared codes spend their levels near zero, where most of a block lies: a code's neighbours are 2 / c of its value away, 0.8 % (d) and
+// 1.6 % (c) at the top, and the smallest level is 1.5e-5 (s) of the largest.  s is kept, not v: v would need twice the range, and the
+// update divides by s.  A positive s never takes code 0: the next step would divide its m by eps alone.  The update itself uses m' and s' as
+// computed, before they are rounded to codes.  A NaN or an infinity in a block makes its scale NaN or infinite, so that it shows.
+//
+// Bound by memory: 28 bytes an element (fp32 parameters and gradients, 32-bit states) or 16.06 (8-bit ones).  The factors of a model are
+// hundreds of tensors of 10^4 to 10^6 elements.  Their addresses change from step to step (autograd allocates gradients), so a call takes
+// them by value: adamw_table_kernel's arguments carry up to 52 tensors a launch, and it writes them into a table in the workspace, with the
+// step counts advanced and the bias corrections in 64 bits.  One launch then walks all tensors: chunks of 4096 elements, numbered through,
+// are dealt out to the blocks in ranges; a block looks its first chunk up in the table (two steps of 64 lanes) and goes on from there.
+#include <algorithm>
+
+#include "xq_common.h"
+
+namespace xq {
+namespace {
+
+constexpr int kBlock = 256;                 // elements that share a scale: a wave's four a lane
+constexpr int kChunk = 4096;                // of a thread block at a time: four 256-element pieces of each of its waves
+constexpr int kThreads = 256;
+constexpr int kTableArgs = 52;              // tensors by value in one launch: 3744 of the 4096 bytes that arguments may take
+constexpr int kNormBlocks = 1024;
+constexpr int kStepBlocks = 2048;           // eight of a compute unit
+
+struct Row {                                // what the walking kernels read of a tensor
+    void* param;
+    const void* grad;
+    void* m;
+    void* v;
+    float* m_scale;
+    float* v_scale;
+    int64_t numel;
+    int64_t chunk0;                         // its first chunk, counted over all tensors
+    float first, root;                      // lr / (1 - b1^t), 1 / sqrt(1 - b2^t)
+    int32_t param16, grad16;                // bf16 (otherwise fp32)
+};
+
+struct TableArgs {
+    xq_adamw_tensor t[kTableArgs];
+};
+
+struct TableScalars {
+    Row* rows;
+    int64_t chunk0;
+    int32_t n, at, step;                    // step: advance the step counts
+    double lr, beta1, beta2;
+    const float* lr_device;
+};
+
+__global__ void __launch_bounds__(64) adamw_table_kernel(TableArgs a, TableScalars s) {
+    const int i = threadIdx.x;
+    if (i >= s.n) return;
+    const xq_adamw_tensor t = a.t[i];
+    int64_t chunk0 = s.chunk0;
+    for (int k = 0; k < i; ++k) chunk0 += (a.t[k].numel + kChunk - 1) / kChunk;
+    float first = 0.0f, root = 0.0f;
+    if (s.step) {
+        const float step = *t.step + 1.0f;
+        *t.step = step;
+        const double lr = s.lr_device ? (double)*s.lr_device : s.lr;
+        first = (float)(lr / (1.0 - pow(s.beta1, (double)step)));
+        root = (float)(1.0 / sqrt(1.0 - pow(s.beta2, (double)step)));
+    }
+    s.rows[s.at + i] = Row{t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.numel, chunk0, first, root,
+                              t.param_dtype == XQ_DT_BF16, t.grad_dtype == XQ_DT_BF16};
+}
+
+// the last row whose first chunk is not behind `chunk` (rows in order of their first chunks, no row without chunks)
+__device__ __forceinline__ int row_of(const Row* rows, int n, int64_t chunk, int lane) {
+    const int step = (n + 63) >> 6;
+    const int a = min(lane * step, n - 1);
+    const int seg = __builtin_popcountll(__ballot(lane * step < n && rows[a].chunk0 <= chunk)) - 1;
+    int at = seg * step;
+    for (int base = at; base < min(n, at + step); base += 64) {
+        const int k = base + lane;
+        const uint64_t below = __ballot(k < min(n, (seg + 1) * step) && rows[min(k, n - 1)].chunk0 <= chunk);
+        if (!below) break;
+        at = base + __builtin_popcountll(below) - 1;
+    }
+    return __builtin_amdgcn_readfirstlane(at);
+}
+
+template <bool BF16>
+__device__ __forceinline__ float load1(const void* p, int64_t i) {
+    return BF16 ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i];
+}
+// four elements from i on; behind the tensor's end: zeros
+template <bool BF16>
+__device__ __forceinline__ f32x4 load4(const void* p, int64_t i, int64_t n, bool vec) {
+    if (vec && i + 4 <= n) {
+        if constexpr (BF16) {
+            const u32x2 w = *(const u32x2*)((const bf16_t*)p + i);
+            return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+        } else {
+            return *(const f32x4*)((const float*)p + i);
+        }
+    }
+    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (i + k < n) r[k] = load1<BF16>(p, i + k);
+    return r;
+}
+template <bool BF16>
+__device__ __forceinline__ void store4(void* p, int64_t i, int64_t n, bool vec, f32x4 v) {
+    if (vec && i + 4 <= n) {
+        if constexpr (BF16) *(u32x2*)((bf16_t*)p + i) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+        else *(f32x4*)((float*)p + i) = v;
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (i + k < n) {
+            if constexpr (BF16) ((bf16_t*)p)[i + k] = to_bf16(v[k]);
+            else ((float*)p)[i + k] = v[k];
+        }
+}
+__device__ __forceinline__ f32x4 load4(bool bf16, const void* p, int64_t i, int64_t n, bool vec) {
+    return bf16 ? load4<true>(p, i, n, vec) : load4<false>(p, i, n, vec);
+}
+// whether four elements from a multiple of four on can be accessed as one
+__device__ __forceinline__ bool whole(const void* p, bool bf16) { return ((uintptr_t)p & (bf16 ? 7 : 15)) == 0; }
+__device__ __forceinline__ uint32_t load4_codes(const void* p, int64_t i, int64_t n, bool vec) {
+    if (vec && i + 4 <= n) return *(const uint32_t*)((const uint8_t*)p + i);
+    uint32_t r = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (i + k < n) r |= (uint32_t)((const uint8_t*)p)[i + k] << (8 * k);
+    return r;
+}
+__device__ __forceinline__ void store4_codes(void* p, int64_t i, int64_t n, bool vec, uint32_t c) {
+    if (vec && i + 4 <= n) {
+        *(uint32_t*)((uint8_t*)p + i) = c;
+        return;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        if (i + k < n) ((uint8_t*)p)[i + k] = (uint8_t)(c >> (8 * k));
+}
+
+// the largest over a wave of the bits of non-negative floats: NaN lies above infinity, so that neither is lost
+__device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
+    return v;
+}
+__device__ __forceinline__ uint32_t bits_abs(float f) { return __float_as_uint(f) & 0x7fffffffu; }
+
+// what a code stands for, and the code of a value: `inv` is the reciprocal of the block's largest magnitude (0 where that is 0).  The
+// hardware root is off by an ulp at most: it decides between two codes only where the value lies that near the middle.
+__device__ __forceinline__ float m_value(int c, float scale) { return (float)(c * (c < 0 ? -c : c)) * (scale * (1.0f / 16129.0f)); }
+__device__ __forceinline__ float s_value(uint32_t d, float scale) { return (float)(d * d) * (scale * (1.0f / 65025.0f)); }
+__device__ __forceinline__ int m_code(float m, float inv) {
+    const int c = (int)fminf(__builtin_rintf(127.0f * __builtin_amdgcn_sqrtf(fabsf(m) * inv)), 127.0f);
+    return m < 0.0f ? -c : c;
+}
+__device__ __forceinline__ uint32_t s_code(float s, float inv) {
+    const uint32_t d = (uint32_t)fminf(__builtin_rintf(255.0f * __builtin_amdgcn_sqrtf(s * inv)), 255.0f);
+    return s > 0.0f ? max(d, 1u) : 0u;
+}
+__device__ __forceinline__ float reciprocal_or_0(float a) { return a > 0.0f ? 1.0f / a : 0.0f; }
+
+struct StepArgs {
+    const Row* rows;
+    int64_t chunks;
+    const float* norm;                      // of the gradients, or NULL
+    int32_t n;
+    float max_norm, beta1, beta2, one_minus_beta1, one_minus_beta2, eps, lr, weight_decay;
+    const float* lr_device;
+};
+
+template <bool EIGHT>
+__global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs a) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t c = a.chunks * blockIdx.x / gridDim.x;
+    const int64_t c1 = a.chunks * (blockIdx.x + 1) / gridDim.x;
+    if (c >= c1) return;
+    const float decay = (a.lr_device ? *a.lr_device : a.lr) * a.weight_decay;
+    // (written so that a NaN norm makes the gradients NaN)
+    float clip = 1.0f;
+    if (a.norm) {
+        clip = a.max_norm / (*a.norm + 1e-6f);
+        clip = clip > 1.0f ? 1.0f : clip;
+    }
+    int t = row_of(a.rows, a.n, c, lane);
+    Row r = a.rows[t];
+    for (; c < c1; ++c) {
+        while (t + 1 < a.n && a.rows[t + 1].chunk0 <= c) r = a.rows[++t];
+        const int64_t n = r.numel, base = (c - r.chunk0) * kChunk + wave * kBlock + lane * 4;
+        const bool vec = whole(r.param, r.param16) && whole(r.grad, r.grad16) && (((uintptr_t)r.m | (uintptr_t)r.v) & (EIGHT ? 3 : 15)) == 0;
+#pragma unroll 1
+        for (int u = 0; u < 4; ++u) {
+            const int64_t i = base + u * (kThreads * 4);
+            if (i - lane * 4 >= n) break;                       // (the whole wave's piece lies behind the end)
+            f32x4 p = load4(r.param16, r.param, i, n, vec);
+            const f32x4 g = load4(r.grad16, r.grad, i, n, vec) * clip;
+            f32x4 m, v;
+            const int64_t blk = i >> 8;
+            if constexpr (EIGHT) {
+                const uint32_t mc = load4_codes(r.m, i, n, vec), vc = load4_codes(r.v, i, n, vec);
+                const float ms = r.m_scale[blk], vs = r.v_scale[blk];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    m[k] = m_value((int)(int8_t)(mc >> (8 * k)), ms);
+                    const float s = s_value((vc >> (8 * k)) & 0xffu, vs);
+                    v[k] = s * s;
+                }
+            } else {
+                m = load4<false>(r.m, i, n, vec);
+                v = load4<false>(r.v, i, n, vec);
+            }
+            f32x4 s;
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                m[k] = a.beta1 * m[k] + a.one_minus_beta1 * g[k];
+                v[k] = a.beta2 * v[k] + a.one_minus_beta2 * (g[k] * g[k]);
+                s[k] = sqrtf(v[k]);
+                p[k] = p[k] - p[k] * decay - m[k] * r.first / (s[k] * r.root + a.eps);
+            }
+            if (r.param16) store4<true>(r.param, i, n, vec, p);
+            else store4<false>(r.param, i, n, vec, p);
+            if constexpr (EIGHT) {
+                uint32_t mb = 0, sb = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    mb = max(mb, bits_abs(m[k]));
+                    sb = max(sb, bits_abs(s[k]));
+                }
+                const float ms = __uint_as_float(wave_max_bits(mb)), ss = __uint_as_float(wave_max_bits(sb));
+                const float mi = reciprocal_or_0(ms), si = reciprocal_or_0(ss);
+                uint32_t mc = 0, sc = 0;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    mc |= ((uint32_t)m_code(m[k], mi) & 0xffu) << (8 * k);
+                    sc |= s_code(s[k], si) << (8 * k);
+                }
+                store4_codes(r.m, i, n, vec, mc);
+                store4_codes(r.v, i, n, vec, sc);
+                if (lane == 0) {
+                    r.m_scale[blk] = ms;
+                    r.v_scale[blk] = ss;
+                }
+            } else {
+                store4<false>(r.m, i, n, vec, m);
+                store4<false>(r.v, i, n, vec, v);
+            }
+        }
+    }
+}
+
+// ---------------------------------------------------------------- the norm of all gradients
+// Squares and sums in 64 bits, in an order fixed by the sizes alone: partial sums of the blocks, then one block over them.
+__device__ __forceinline__ double block_sum(double v, double* lds) {
+#pragma unroll
+    for (int d = 32; d; d >>= 1) v += __shfl_xor(v, d);
+    __syncthreads();
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = v;
+    __syncthreads();
+    v = 0.0;
+    for (int w = 0; w < (int)(blockDim.x >> 6); ++w) v += lds[w];
+    return v;
+}
+
+__global__ void __launch_bounds__(kThreads) grad_norm_kernel(const Row* rows, int n_rows, int64_t chunks, double* partial) {
+    __shared__ double lds[kThreads / 64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    int64_t c = chunks * blockIdx.x / gridDim.x;
+    const int64_t c1 = chunks * (blockIdx.x + 1) / gridDim.x;
+    double sum = 0.0;
+    if (c < c1) {
+        int t = row_of(rows, n_rows, c, lane);
+        Row r = rows[t];
+        for (; c < c1; ++c) {
+            while (t + 1 < n_rows && rows[t + 1].chunk0 <= c) r = rows[++t];
+            const int64_t base = (c - r.chunk0) * kChunk + wave * kBlock + lane * 4;
+            const bool vec = whole(r.grad, r.grad16);
+            f32x4 g[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u) g[u] = load4(r.grad16, r.grad, base + u * (kThreads * 4), r.numel, vec);
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+#pragma unroll
+                for (int k = 0; k < 4; ++k) sum += (double)g[u][k] * (double)g[u][k];
+        }
+    }
+    sum = block_sum(sum, lds);
+    if (threadIdx.x == 0) partial[blockIdx.x] = sum;
+}
+
+__global__ void __launch_bounds__(kThreads) grad_norm_finish_kernel(const double* partial, int n, float* out) {
+    __shared__ double lds[kThreads / 64];
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < n; i += kThreads) sum += partial[i];
+    sum = block_sum(sum, lds);
+    if (threadIdx.x == 0) *out = (float)sqrt(sum);
+}
+
+// ---------------------------------------------------------------- what 8-bit states stand for
+template <bool OUT16>
+__global__ void __launch_bounds__(kThreads) adamw_values_kernel(const uint8_t* mc, const uint8_t* vc, const float* ms, const float* vs,
+                                                                int64_t n, void* m_out, void* v_out, bool vec) {
+    const int64_t stride = (int64_t)gridDim.x * kThreads * 4;
+    for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; i < n; i += stride) {
+        const uint32_t a = load4_codes(mc, i, n, vec), b = load4_codes(vc, i, n, vec);
+        const float sm = ms[i >> 8], sv = vs[i >> 8];
+        f32x4 m, v;
+#pragma unroll
+        for (int k = 0; k < 4; ++k) {
+            m[k] = m_value((int)(int8_t)(a >> (8 * k)), sm);
+            const float s = s_value((b >> (8 * k)) & 0xffu, sv);
+            v[k] = s * s;
+        }
+        store4<OUT16>(m_out, i, n, vec, m);
+        store4<OUT16>(v_out, i, n, vec, v);
+    }
+}
+
+int check_tensors(const char* who, const xq_adamw_tensor* t, int64_t n, int state_bits, bool grads_only, int64_t* chunks) {
+    XQ_REQUIRE(n >= 0 && n < (1 << 24), "%s: bad number of tensors %lld", who, (long long)n);
+    XQ_REQUIRE(n == 0 || t, "%s: tensors are NULL", who);
+    *chunks = 0;
+    for (int64_t i = 0; i < n; ++i) {
+        const xq_adamw_tensor& a = t[i];
+        XQ_REQUIRE(a.numel > 0, "%s: tensor %lld has %lld elements", who, (long long)i, (long long)a.numel);
+        XQ_REQUIRE(a.grad_dtype == XQ_DT_BF16 || a.grad_dtype == XQ_DT_F32, "%s: gradient %lld is neither fp32 nor bf16", who, (long long)i);
+        XQ_REQUIRE(a.grad && xq_aligned(a.grad, a.grad_dtype == XQ_DT_BF16 ? 2 : 4), "%s: gradient %lld is NULL or misaligned", who, (long long)i);
+        *chunks += xq_cdiv(a.numel, kChunk);
+        if (grads_only) continue;
+        XQ_REQUIRE(a.param_dtype == XQ_DT_BF16 || a.param_dtype == XQ_DT_F32, "%s: parameter %lld is neither fp32 nor bf16", who, (long long)i);
+        XQ_REQUIRE(a.param && xq_aligned(a.param, a.param_dtype == XQ_DT_BF16 ? 2 : 4), "%s: parameter %lld is NULL or misaligned", who, (long long)i);
+        XQ_REQUIRE(a.exp_avg && a.exp_avg_sq && a.step && xq_aligned(a.step, 4), "%s: a state of tensor %lld is NULL or misaligned", who, (long long)i);
+        if (state_bits == 8)
+            XQ_REQUIRE(a.exp_avg_scale && a.exp_avg_sq_scale && xq_aligned(a.exp_avg_scale, 4) && xq_aligned(a.exp_avg_sq_scale, 4),
+                       "%s: 8-bit states of tensor %lld have no scales, or misaligned ones", who, (long long)i);
+        else
+            XQ_REQUIRE(xq_aligned(a.exp_avg, 4) && xq_aligned(a.exp_avg_sq, 4), "%s: a state of tensor %lld is misaligned", who, (long long)i);
+    }
+    return XQ_OK;
+}
+
+int64_t table_bytes(int64_t n) { return xq_cdiv(n * (int64_t)sizeof(Row), 256) * 256; }
+
+int check_workspace(const char* who, int64_t n, const void* workspace, int64_t bytes) {
+    XQ_REQUIRE(workspace && xq_aligned(workspace, 256) && bytes >= xq_adamw_workspace_bytes(n), "%s: a workspace of %lld bytes, 256-byte aligned, is needed", who,
+               (long long)xq_adamw_workspace_bytes(n));
+    return XQ_OK;
+}
+
+void write_table(const xq_adamw_tensor* t, int64_t n, void* workspace, const xq_adamw_options* o, hipStream_t s) {
+    int64_t chunk0 = 0;
+    for (int64_t at = 0; at < n; at += kTableArgs) {
+        TableArgs a;
+        const int k = (int)std::min<int64_t>(kTableArgs, n - at);
+        std::copy(t + at, t + at + k, a.t);
+        adamw_table_kernel<<<dim3(1), 64, 0, s>>>(a, TableScalars{(Row*)workspace, chunk0, k, (int32_t)at, o != nullptr, o ? o->lr : 0.0, o ? o->beta1 : 0.0,
+                                                                  o ? o->beta2 : 0.0, o ? o->lr_device : nullptr});
+        for (int i = 0; i < k; ++i) chunk0 += xq_cdiv(t[at + i].numel, kChunk);
+    }
+}
+
+void norm_of(int64_t n, int64_t chunks, void* workspace, float* norm, hipStream_t s) {
+    double* partial = (double*)((uint8_t*)workspace + table_bytes(n));
+    const int blocks = (int)std::min<int64_t>(chunks, kNormBlocks);
+    if (blocks) grad_norm_kernel<<<dim3(blocks), kThreads, 0, s>>>((const Row*)workspace, (int)n, chunks, partial);
+    grad_norm_finish_kernel<<<dim3(1), kThreads, 0, s>>>(partial, blocks, norm);
+}
+
+}  // namespace
+}  // namespace xq
+
+using namespace xq;
+
+extern "C" int64_t xq_adamw_workspace_bytes(int64_t n_tensors) { return n_tensors < 0 ? -1 : table_bytes(n_tensors) + kNormBlocks * 8; }
+
+extern "C" int xq_grad_norm(const xq_adamw_tensor* tensors, int64_t n, float* norm, void* workspace, int64_t workspace_bytes, void* stream) {
+    int64_t chunks;
+    int rc = check_tensors("xq_grad_norm", tensors, n, 32, true, &chunks);
+    if (rc == XQ_OK) rc = check_workspace("xq_grad_norm", n, workspace, workspace_bytes);
+    if (rc != XQ_OK) return rc;
+    XQ_REQUIRE(norm && xq_aligned(norm, 4), "xq_grad_norm: norm is NULL or misaligned");
+    write_table(tensors, n, workspace, nullptr, (hipStream_t)stream);
+    norm_of(n, chunks, workspace, norm, (hipStream_t)stream);
+    XQ_CHECK_LAUNCH("xq_grad_norm");
+    return XQ_OK;
+}
+
+extern "C" int xq_adamw_step(const xq_adamw_tensor* tensors, int64_t n, const xq_adamw_options* o, void* workspace, int64_t workspace_bytes, void* stream) {
+    XQ_REQUIRE(o, "xq_adamw_step: options are NULL");
+    XQ_REQUIRE(o->state_bits == 8 || o->state_bits == 32, "xq_adamw_step: states of 8 or 32 bits, got %d", o->state_bits);
+    XQ_REQUIRE(o->lr >= 0.0 && o->beta1 >= 0.0 && o->beta1 < 1.0 && o->beta2 >= 0.0 && o->beta2 < 1.0 && o->eps >= 0.0 && o->weight_decay >= 0.0,
+               "xq_adamw_step: lr %g, betas %g and %g, eps %g, weight_decay %g", o->lr, o->beta1, o->beta2, o->eps, o->weight_decay);
+    XQ_REQUIRE(!o->norm || (o->max_norm > 0.0 && xq_aligned(o->norm, 4)), "xq_adamw_step: a norm needs max_norm > 0 (got %g) and 4-byte alignment", o->max_norm);
+    XQ_REQUIRE(!o->norm_given || o->norm, "xq_adamw_step: norm_given without a norm");
+    XQ_REQUIRE(!o->lr_device || xq_aligned(o->lr_device, 4), "xq_adamw_step: lr_device is misaligned");
+    int64_t chunks;
+    int rc = check_tensors("xq_adamw_step", tensors, n, o->state_bits, false, &chunks);
+    if (rc == XQ_OK) rc = check_workspace("xq_adamw_step", n, workspace, workspace_bytes);
+    if (rc != XQ_OK) return rc;
+    hipStream_t s = (hipStream_t)stream;
+    write_table(tensors, n, workspace, o, s);
+    if (o->norm && !o->norm_given) norm_of(n, chunks, workspace, o->norm, s);
+    if (n) {
+        const StepArgs a = {(const Row*)workspace, chunks, o->norm, (int32_t)n, (float)o->max_norm, (float)o->beta1, (float)o->beta2,
+                            (float)(1.0 - o->beta1), (float)(1.0 - o->beta2), (float)o->eps, (float)o->lr, (float)o->weight_decay, o->lr_device};
+        const dim3 grid((unsigned)std::min<int64_t>(chunks, kStepBlocks));
+        if (o->state_bits == 8) adamw_kernel<true><<<grid, kThreads, 0, s>>>(a);
+        else adamw_kernel<false><<<grid, kThreads, 0, s>>>(a);
+    }
+    XQ_CHECK_LAUNCH("xq_adamw_step");
+    return XQ_OK;
+}
+
+extern "C" int xq_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale, const float* exp_avg_sq_scale, int64_t numel,
+                               void* exp_avg_out, void* exp_avg_sq_out, int out_dtype, void* stream) {
+    XQ_REQUIRE(numel >= 0, "xq_adamw_values: %lld elements", (long long)numel);
+    XQ_REQUIRE(out_dtype == XQ_DT_BF16 || out_dtype == XQ_DT_F32, "xq_adamw_values: the outputs are fp32 or bf16");
+    if (numel == 0) return XQ_OK;
+    XQ_REQUIRE(exp_avg && exp_avg_sq && exp_avg_scale && exp_avg_sq_scale && exp_avg_out && exp_avg_sq_out, "xq_adamw_values: NULL buffer");
+    const size_t e = out_dtype == XQ_DT_BF16 ? 2 : 4;
+    XQ_REQUIRE(xq_aligned(exp_avg_scale, 4) && xq_aligned(exp_avg_sq_scale, 4) && xq_aligned(exp_avg_out, e) && xq_aligned(exp_avg_sq_out, e),
+               "xq_adamw_values: misaligned buffer");
+    const bool vec = xq_aligned(exp_avg, 4) && xq_aligned(exp_avg_sq, 4) && xq_aligned(exp_avg_out, 4 * e) && xq_aligned(exp_avg_sq_out, 4 * e);
+    const dim3 grid((unsigned)std::min<int64_t>(xq_cdiv(numel, 4 * kThreads), kStepBlocks));
+    const auto *m = (const uint8_t*)exp_avg, *v = (const uint8_t*)exp_avg_sq;
+    if (e == 2) adamw_values_kernel<true><<<grid, kThreads, 0, (hipStream_t)stream>>>(m, v, exp_avg_scale, exp_avg_sq_scale, numel, exp_avg_out, exp_avg_sq_out, vec);
+    else adamw_values_kernel<false><<<grid, kThreads, 0, (hipStream_t)stream>>>(m, v, exp_avg_scale, exp_avg_sq_scale, numel, exp_avg_out, exp_avg_sq_out, vec);
+    XQ_CHECK_LAUNCH("xq_adamw_values");
+    return XQ_OK;
+}

@@ -28,6 +28,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
 
+#include <algorithm>
 #include <cmath>
 #include <optional>
 #include <string>
@@ -811,6 +812,155 @@ PyObject* moe(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// ---- the optimizer step: its arguments are hundreds of tensors, whose addresses and checks are a matter of tens of microseconds here
+struct TensorList {
+    const char* name;
+    PyObject* seq = nullptr;
+    TensorList(const char* n, PyObject* o) : name(n) {
+        if (o == Py_None) return;
+        seq = PySequence_Fast(o, "");
+        if (!seq) { PyErr_Clear(); throw ArgError(std::string("adamw_step: ") + n + " must be a list of tensors"); }
+    }
+    ~TensorList() { Py_XDECREF(seq); }
+    TensorList(const TensorList&) = delete;
+    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(seq); }
+    std::string at(Py_ssize_t i) const { return std::string("adamw_step: ") + name + "[" + std::to_string(i) + "]"; }
+    const Tensor& operator[](Py_ssize_t i) const {
+        PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
+        if (!THPVariable_Check(o)) throw ArgError(at(i) + " is not a tensor");
+        const Tensor& t = THPVariable_Unpack(o);
+        if (!t.defined() || t.layout() != at::kStrided || at::isTensorSubclassLike(t)) throw ArgError(at(i) + " is not a plain dense tensor");
+        if (!t.is_cuda()) throw std::runtime_error(at(i) + ": xorl_amd kernels run on a HIP device only; got a tensor on " + t.device().str() + " (there is no CPU fallback)");
+        return t;
+    }
+};
+
+int float_code(const Tensor& t, const TensorList& l, Py_ssize_t i) {
+    if (t.scalar_type() == at::kFloat) return XQ_DT_F32;
+    if (t.scalar_type() == at::kBFloat16) return XQ_DT_BF16;
+    throw ArgError(l.at(i) + " must be fp32 or bf16, got " + toString(t.scalar_type()));
+}
+
+// adamw(params, grads, exp_avgs, exp_avg_sqs, steps, exp_avg_scales or None, exp_avg_sq_scales or None, (lr, beta1, beta2, eps, weight_decay),
+//       lr tensor or None, max_norm or None, norm or None) -> the norm, or None.  params None: the norm of grads alone.
+PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
+    return guarded([&]() -> PyObject* {
+        if (n_args != 11) { PyErr_SetString(PyExc_TypeError, "adamw(11 arguments)"); return nullptr; }
+        const TensorList p("params", args[0]), g("grads", args[1]), m("exp_avgs", args[2]), v("exp_avg_sqs", args[3]), t("steps", args[4]),
+            ms("exp_avg_scales", args[5]), vs("exp_avg_sq_scales", args[6]);
+        const bool norm_only = !p.seq, eight = ms.seq || vs.seq;
+        if (!g.seq) throw ArgError("adamw_step: grads must be a list of tensors");
+        const Py_ssize_t n = g.size();
+        if (!norm_only) {
+            for (const TensorList* l : {&p, &m, &v, &t})
+                if (!l->seq || l->size() != n) throw ArgError(std::string("adamw_step: ") + l->name + " and grads differ in length");
+            if (eight && (!ms.seq || !vs.seq || ms.size() != n || vs.size() != n))
+                throw ArgError("adamw_step: 8-bit states need exp_avg_scales and exp_avg_sq_scales, one for each tensor");
+        }
+        xq_adamw_options o{};
+        if (!norm_only && !PyArg_ParseTuple(args[7], "ddddd", &o.lr, &o.beta1, &o.beta2, &o.eps, &o.weight_decay)) return nullptr;
+        o.state_bits = eight ? 8 : 32;
+        std::optional<at::Device> device;
+        auto same_device = [&](const Tensor& a, const std::string& what) {
+            if (!device) device = a.device();
+            else if (a.device() != *device) throw ArgError(what + " is on " + a.device().str() + ", others on " + device->str());
+        };
+        std::vector<xq_adamw_tensor> q;
+        std::vector<Tensor> keep, written;
+        std::vector<const void*> once;            // what the step writes: named twice it would be written by two blocks at a time
+        q.reserve(n);
+        for (Py_ssize_t i = 0; i < n; ++i) {
+            const Tensor& gr = g[i];
+            xq_adamw_tensor a{};
+            a.numel = gr.numel();
+            a.grad_dtype = float_code(gr, g, i);
+            same_device(gr, g.at(i));
+            Tensor gc = gr;
+            if (!gr.is_contiguous() || gr.is_neg()) {
+                gc = gr.detach().resolve_neg().contiguous();
+                keep.push_back(gc);
+            }
+            a.grad = gc.data_ptr();
+            if (!norm_only) {
+                const Tensor &pt = p[i], &mt = m[i], &vt = v[i], &st = t[i];
+                a.param_dtype = float_code(pt, p, i);
+                if (pt.sizes() != gr.sizes()) throw ArgError(g.at(i) + " has another shape than its parameter");
+                struct { const Tensor& t; const TensorList& l; at::ScalarType dt; int64_t n; } all[] = {
+                    {pt, p, pt.scalar_type(), a.numel}, {mt, m, eight ? at::kChar : at::kFloat, a.numel},
+                    {vt, v, eight ? at::kByte : at::kFloat, a.numel}, {st, t, at::kFloat, 1}};
+                for (const auto& c : all) {
+                    same_device(c.t, c.l.at(i));
+                    if (c.t.scalar_type() != c.dt) throw ArgError(c.l.at(i) + " must be " + toString(c.dt) + ", got " + toString(c.t.scalar_type()));
+                    if (c.t.numel() != c.n) throw ArgError(c.l.at(i) + " holds " + std::to_string(c.t.numel()) + " elements, expected " + std::to_string(c.n));
+                    if (!c.t.is_contiguous() || c.t.is_neg()) throw ArgError(c.l.at(i) + " must be contiguous");
+                }
+                a.param = pt.data_ptr(); a.exp_avg = mt.data_ptr(); a.exp_avg_sq = vt.data_ptr(); a.step = (float*)st.data_ptr();
+                if (eight) {
+                    float** to[] = {&a.exp_avg_scale, &a.exp_avg_sq_scale};
+                    const TensorList* from[] = {&ms, &vs};
+                    for (int k = 0; k < 2; ++k) {
+                        const Tensor& sc = (*from[k])[i];
+                        same_device(sc, from[k]->at(i));
+                        if (sc.scalar_type() != at::kFloat || !sc.is_contiguous() || sc.numel() != (a.numel + 255) / 256)
+                            throw ArgError(from[k]->at(i) + " must be contiguous fp32 with " + std::to_string((a.numel + 255) / 256) + " element(s)");
+                        *to[k] = (float*)sc.data_ptr();
+                        written.push_back(sc);
+                        if (a.numel) once.push_back(sc.data_ptr());
+                    }
+                }
+                for (const Tensor* w : {&pt, &mt, &vt}) {
+                    written.push_back(*w);
+                    if (a.numel) once.push_back(w->data_ptr());
+                }
+                written.push_back(st);
+                once.push_back(st.data_ptr());
+            }
+            if (a.numel) q.push_back(a);
+        }
+        std::sort(once.begin(), once.end());
+        if (std::adjacent_find(once.begin(), once.end()) != once.end())
+            throw ArgError("adamw_step: two tensors share a parameter, a state or a step count");
+        if (args[8] != Py_None) {
+            const Tensor* lr = plain(args[8]);
+            if (!lr || lr->scalar_type() != at::kFloat || lr->numel() != 1) throw ArgError("adamw_step: an lr tensor must be one fp32 element on the device");
+            same_device(*lr, "adamw_step: lr");
+            o.lr_device = (const float*)lr->data_ptr();
+        }
+        Tensor norm;
+        if (args[10] != Py_None) {
+            const Tensor* given = plain(args[10]);
+            if (!given || given->scalar_type() != at::kFloat || given->numel() != 1) throw ArgError("adamw_step: grad_norm must be one fp32 element on the device");
+            same_device(*given, "adamw_step: grad_norm");
+            norm = *given;
+            o.norm_given = 1;
+        }
+        if (args[9] != Py_None) {
+            o.max_norm = PyFloat_AsDouble(args[9]);
+            if (o.max_norm == -1.0 && PyErr_Occurred()) return nullptr;
+        } else if (o.norm_given) {
+            throw ArgError("adamw_step: grad_norm without max_norm");
+        }
+        if (!device) {
+            if (norm_only || args[9] != Py_None) throw ArgError("adamw_step: a norm over no gradients has no device");
+            Py_RETURN_NONE;
+        }
+        c10::DeviceGuard guard(*device);
+        if (!norm.defined() && (norm_only || args[9] != Py_None)) norm = empty_f32({});
+        if (norm.defined()) o.norm = (float*)norm.data_ptr();
+        void* stream = (void*)c10::hip::getCurrentHIPStream(device->index()).stream();
+        Scratch ws(xq_adamw_workspace_bytes((int64_t)q.size()));
+        {
+            ReleaseGil nogil;
+            check(norm_only ? xq_grad_norm(q.data(), (int64_t)q.size(), o.norm, ws.get(), ws.bytes, stream)
+                            : xq_adamw_step(q.data(), (int64_t)q.size(), &o, ws.get(), ws.bytes, stream));
+        }
+        for (const Tensor& w : written)
+            if (!w.is_inference()) w.unsafeGetTensorImpl()->bump_version();
+        if (!norm.defined()) Py_RETURN_NONE;
+        return THPVariable_Wrap(std::move(norm));
+    });
+}
+
 // {format: (class, ((method name, method), ...))} -> programs by format
 bool fill_programs(PyObject* table, Program* out) {
     PyObject *key, *entry;
@@ -857,6 +1007,7 @@ PyMethodDef methods[] = {
     {"linears", (PyCFunction)(void (*)())linears, METH_FASTCALL, nullptr},
     {"mlp", (PyCFunction)(void (*)())mlp, METH_FASTCALL, nullptr},
     {"moe", (PyCFunction)(void (*)())moe, METH_FASTCALL, nullptr},
+    {"adamw", (PyCFunction)(void (*)())adamw, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };
 
