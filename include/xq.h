@@ -670,6 +670,43 @@ int xq_mlp_fwd_infer(const xq_weight* gate, const xq_weight* up, const xq_weight
                      const void* x, int64_t ldx, int64_t M, void* y, int64_t ldy, void* workspace,
                      int64_t workspace_bytes, void* stream);
 
+/* ---- cross entropy over an output head ---------------------------------- */
+/* loss_i = log sum_v exp(c x_i . w_v) - c x_i . w_label(i) for x [M, H] and a head w [V, H], both bf16, without the logits ever
+ * being written (the reference: ops/loss, the fused linear cross entropy).  Rows whose label is ignore_index have loss 0, gradient 0 and
+ * no cost; a label outside [0, V) makes its row's loss and gradient NaN (and with them the head's gradient).
+ * reduction: XQ_LCE_NONE, loss[M]; XQ_LCE_MEAN (over the rows that count; NaN if there are none) and XQ_LCE_SUM, loss[1].
+ * keep: what a backward will ask for: KEEP_NONE nothing, KEEP_HEAD the head's gradient alone, KEEP_DX the input gradient and maybe the
+ * head's.  saved: xq_lce_saved_bytes(M, V, H, keep) bytes, 256-byte aligned, needed in every case; the backward reads it and leaves it.
+ * workspace: xq_lce_workspace_bytes(M, V, H, keep), for a backward with dw XQ_LCE_KEEP_HEAD_BWD in place of keep; without dw none.
+ * xq_lce_bwd: grad fp32[M] or [1] by the reduction, of the loss; dx [M, H] and dw [V, H] bf16, NULL where not wanted; problem, and
+ * what it points at, as in the forward.  H % 64 == 0; rows of x, w, dx, dw at multiples of 16 bytes. */
+#define XQ_LCE_NONE 0
+#define XQ_LCE_MEAN 1
+#define XQ_LCE_SUM 2
+#define XQ_LCE_KEEP_NONE 0
+#define XQ_LCE_KEEP_HEAD 1
+#define XQ_LCE_KEEP_DX 2
+#define XQ_LCE_KEEP_HEAD_BWD 3
+
+typedef struct xq_lce_problem {
+    const void* x;
+    int64_t ldx;
+    const void* w;
+    int64_t ldw;
+    const void* labels;         /* int32 or int64 [M] */
+    int64_t M, V, H, ignore_index;
+    float logit_scale;          /* c */
+    int32_t label_bytes;        /* 4 or 8 */
+    int32_t reduction;
+    int32_t reserved;
+} xq_lce_problem;
+
+int64_t xq_lce_saved_bytes(int64_t M, int64_t V, int64_t H, int keep);
+int64_t xq_lce_workspace_bytes(int64_t M, int64_t V, int64_t H, int pass);
+int xq_lce_fwd(const xq_lce_problem* problem, float* loss, void* saved, int keep, void* workspace, int64_t workspace_bytes, void* stream);
+int xq_lce_bwd(const xq_lce_problem* problem, const float* grad, const void* saved, int keep, void* dx, int64_t lddx, void* dw, int64_t lddw,
+               void* workspace, int64_t workspace_bytes, void* stream);
+
 /* ---- optimizer step over many tensors ----------------------------------- */
 /* One AdamW step over n tensors (the factors of a model, a trained head): the counterpart of the reference's optimizer
  * construction (optim/optimizer.py; the update rule is that of torch.optim.AdamW) for the parameters this library produces gradients of.

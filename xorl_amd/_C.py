@@ -79,6 +79,17 @@ class XqMlpGrads(ctypes.Structure):
     _fields_ = [("dA", ctypes.c_void_p * 3), ("dB", ctypes.c_void_p * 3)]
 
 
+class XqLceProblem(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("w", ctypes.c_void_p), ("ldw", ctypes.c_int64),
+                ("labels", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("M", "V", "H", "ignore_index")] + [
+                    ("logit_scale", ctypes.c_float), ("label_bytes", ctypes.c_int32), ("reduction", ctypes.c_int32),
+                    ("reserved", ctypes.c_int32)]
+
+
+XQ_LCE_KEEP_NONE, XQ_LCE_KEEP_HEAD, XQ_LCE_KEEP_DX, XQ_LCE_KEEP_HEAD_BWD = 0, 1, 2, 3
+LCE_REDUCTIONS = {"none": 0, "mean": 1, "sum": 2}
+
+
 class XqAdamwTensor(ctypes.Structure):
     _fields_ = [(n, ctypes.c_void_p) for n in ("param", "grad", "exp_avg", "exp_avg_sq", "exp_avg_scale", "exp_avg_sq_scale", "step")] + [
         ("numel", ctypes.c_int64), ("param_dtype", ctypes.c_int32), ("grad_dtype", ctypes.c_int32)]
@@ -210,6 +221,13 @@ _SIGNATURES = {
     # gate, up, down, lora, x, ldx, dy, lddy, M, saved, dx, lddx, grads, ws, ws_bytes, stream
     "xq_mlp_bwd": (_INT, [_W, _W, _W, ctypes.POINTER(XqMlpLora), _P, _I64, _P, _I64, _I64, ctypes.POINTER(XqMlpSaved), _P,
                           _I64, ctypes.POINTER(XqMlpGrads), _P, _I64, _P]),
+    # M, V, H, keep (saved) or pass (workspace)
+    "xq_lce_saved_bytes": (_I64, [_I64, _I64, _I64, _INT]),
+    "xq_lce_workspace_bytes": (_I64, [_I64, _I64, _I64, _INT]),
+    # problem, loss, saved, keep, ws, ws_bytes, stream
+    "xq_lce_fwd": (_INT, [ctypes.POINTER(XqLceProblem), _P, _P, _INT, _P, _I64, _P]),
+    # problem, grad, saved, keep, dx, lddx, dw, lddw, ws, ws_bytes, stream
+    "xq_lce_bwd": (_INT, [ctypes.POINTER(XqLceProblem), _P, _P, _INT, _P, _I64, _P, _I64, _P, _I64, _P]),
     "xq_adamw_workspace_bytes": (_I64, [_I64]),
     # tensors, n, options, ws, ws_bytes, stream
     "xq_adamw_step": (_INT, [ctypes.POINTER(XqAdamwTensor), _I64, ctypes.POINTER(XqAdamwOptions), _P, _I64, _P]),

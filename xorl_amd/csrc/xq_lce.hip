@@ -1,0 +1,510 @@
+// Cross entropy over an output head, in pieces of the vocabulary, with its gradients; no logits are kept.
+//
+//   l_iv = c x_i . w_v        loss_i = log sum_v exp(l_iv) - l_it        t = label of row i
+//   dx_i = g_i c (sum_v p_iv w_v - w_t)        dw_v = c sum_i g_i (p_iv - [v = t_i]) x_i
+//
+// Rows whose label is ignore_index are taken out first (prepare_kernel lists the others in order), so that they cost nothing: every launch
+// covers the most rows there can be and blocks behind the last one end at once.  The label's column is left out of all sums and joined
+// at the end: with Z' = sum_{v != t} exp(l_v - ref), e_t = exp(l_t - ref),
+//   loss = log(Z' + e_t) + ref - l_t        (log1p(Z') where ref is the label's own logit)
+//   dx_i = g_i c (O_i - Z' w_t) / (Z' + e_t),        O_i = sum_{v != t} exp(l_v - ref) w_v
+// which keeps what a confident row has left of its loss and gradient, where p_t - 1 would cancel.
+//
+//  * Scores (no gradient wanted): one product whose ends are the largest logit and the sum of exponentials of 256 columns; one joining pass.
+//  * Training: E = exp(l - ref) of a piece goes to the workspace as bf16, and E . W is added to O in fp32: the forward leaves
+//    the whole input gradient but its factor, in two products, where forming the logits again in the backward would take three.  E needs
+//    a reference before the row's largest logit is known: the label's own logit (target_kernel).  E is right as long as no logit is more
+//    than 2^64 times e above it; a piece that finds one takes the largest as the new reference (O and Z' are scaled to it) and is done
+//    again for the row tiles concerned.  bf16 keeps E to half a step (2^-9 of each term, of either sign).
+//  * A trained head: the backward forms the logits again with the roles exchanged, G = g (p - [v = t]) as bf16 with the tokens along the
+//    contraction, and multiplies it with the rows that count.
+#include <algorithm>
+
+#include "xq_lce.h"
+
+namespace xq {
+namespace {
+
+constexpr int64_t kPieceBytes = 1ll << 30;          // of E or G at a time
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+constexpr float kFar = 64.0f;                       // a logit this far (log2) above its reference: the piece is done again
+
+inline int64_t up256(int64_t n) { return (n + 255) & ~255ll; }
+
+// the rows that count, in order; arrays as long as whole tiles (behind the last row: no label)
+struct Prep {
+    const void* labels;
+    int32_t label_bytes;
+    int64_t M, M_pad, V, ignore;
+    int32_t *count, *row, *label, *place;           // place: of a row of x among those that count, or -1
+    float* at_label;
+};
+
+__global__ void __launch_bounds__(1024) lce_prepare_kernel(Prep a) {
+    __shared__ int wave_n[16], base_s;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    if (threadIdx.x == 0) base_s = 0;
+    __syncthreads();
+    for (int64_t at = 0; at < a.M; at += 1024) {
+        const int64_t i = at + threadIdx.x;
+        int64_t label = a.ignore;
+        if (i < a.M) label = a.label_bytes == 8 ? ((const int64_t*)a.labels)[i] : (int64_t)((const int32_t*)a.labels)[i];
+        const bool in = i < a.M && label != a.ignore;
+        const uint64_t mask = __ballot(in);
+        if (lane == 0) wave_n[wave] = __builtin_popcountll(mask);
+        __syncthreads();
+        int before = base_s;
+        for (int w = 0; w < wave; ++w) before += wave_n[w];
+        const int c = before + __builtin_popcountll(mask & ((1ull << lane) - 1));
+        if (in) {
+            a.row[c] = (int)i;
+            a.label[c] = label >= 0 && label < a.V ? (int)label : -1;
+            a.at_label[c] = __builtin_nanf("");
+        }
+        if (i < a.M) a.place[i] = in ? c : -1;
+        __syncthreads();
+        if (threadIdx.x == 1023) base_s = c + in;
+        __syncthreads();
+    }
+    const int n = base_s;
+    if (threadIdx.x == 0) *a.count = n;
+    for (int64_t c = n + threadIdx.x; c < a.M_pad; c += 1024) {
+        a.row[c] = 0;
+        a.label[c] = -1;
+    }
+}
+
+__device__ __forceinline__ f32x4 bf16x4_f32(u32x2 w) {
+    return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+}
+
+// the label's logit of every row (log2 units): the first reference
+__global__ void __launch_bounds__(256) lce_target_kernel(LceRows rows, const bf16_t* x, int64_t ldx, const bf16_t* w, int64_t ldw, int H, float scale2,
+                                                         float* at_label, float* ref, float* z) {
+    const int lane = threadIdx.x & 63;
+    const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
+    if (c >= *rows.count) return;
+    const int label = rows.label[c];
+    float sum = 0.0f;
+    if (label >= 0) {
+        const bf16_t *xr = x + rows.row[c] * ldx, *wr = w + label * ldw;
+        for (int k = lane * 8; k < H; k += 512) {
+            const u32x4 a = *(const u32x4*)(xr + k), b = *(const u32x4*)(wr + k);
+#pragma unroll
+            for (int q = 0; q < 4; ++q)
+                sum += __uint_as_float(a[q] << 16) * __uint_as_float(b[q] << 16) + __uint_as_float(a[q] & 0xffff0000u) * __uint_as_float(b[q] & 0xffff0000u);
+        }
+    }
+#pragma unroll
+    for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
+    if (lane == 0) {
+        const float t = label >= 0 ? sum * scale2 : __builtin_nanf("");
+        at_label[c] = t;
+        ref[c] = t;
+        z[c] = 0.0f;
+    }
+}
+
+// ---- joins over the column tiles of a piece: 64 rows a block, 16 waves over the tiles
+struct Join {
+    const int32_t* count;
+    const f32x2* part;
+    int64_t rows_pad;
+    int32_t tiles, tile_rows;
+    float *ref, *z, *alpha;
+    int32_t* redo;                      // by row tile
+};
+
+template <typename F>
+__device__ __forceinline__ bool join_rows(const Join& a, f32x2 (*lds)[64], f32x2 start, F fold, f32x2* out, int64_t* row) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t r = (int64_t)blockIdx.x * 64 + lane;
+    f32x2 v = start;
+    if (r < *a.count) {
+#pragma unroll 8
+        for (int t = wave; t < a.tiles; t += 16) v = fold(v, a.part[t * a.rows_pad + r]);
+    }
+    lds[wave][lane] = v;
+    __syncthreads();
+    if (wave != 0 || r >= *a.count) return false;
+    for (int w = 1; w < 16; ++w) v = fold(v, lds[w][lane]);
+    *out = v;
+    *row = r;
+    return true;
+}
+
+// EXP, before the second try: rows whose largest logit is too far above the reference get it as their new one
+__global__ void __launch_bounds__(1024) lce_far_kernel(Join a) {
+    __shared__ f32x2 lds[16][64];
+    f32x2 v;
+    int64_t r;
+    if (!join_rows(a, lds, f32x2{-INFINITY, 0.0f}, [](f32x2 p, f32x2 q) { return f32x2{fmaxf(p[0], q[0]), 0.0f}; }, &v, &r)) return;
+    const float ref = a.ref[r];
+    const bool far = v[0] - ref > kFar;
+    a.alpha[r] = far ? __builtin_amdgcn_exp2f(ref - v[0]) : 1.0f;
+    if (far) {
+        a.ref[r] = v[0];
+        a.redo[r / a.tile_rows] = 1;             // (set by several rows, to the same)
+    }
+}
+
+__global__ void __launch_bounds__(1024) lce_sum_kernel(Join a) {
+    __shared__ f32x2 lds[16][64];
+    f32x2 v;
+    int64_t r;
+    if (!join_rows(a, lds, f32x2{0.0f, 0.0f}, [](f32x2 p, f32x2 q) { return f32x2{0.0f, p[1] + q[1]}; }, &v, &r)) return;
+    a.z[r] = a.z[r] * a.alpha[r] + v[1];
+}
+
+__global__ void __launch_bounds__(256) lce_clear_kernel(int32_t* p, int n) {
+    for (int i = threadIdx.x; i < n; i += 256) p[i] = 0;
+}
+
+// what is kept of a row: 1 / Z, Z' / Z, log2 of the sum of exponentials
+struct RowEnd {
+    float *inv, *rest, *lse2, *loss;
+};
+__device__ __forceinline__ void end_row(const RowEnd& e, int64_t c, float z, float ref, float t) {
+    const float et = __builtin_amdgcn_exp2f(t - ref), sum = z + et;
+    e.loss[c] = ref == t ? log1pf(z) : logf(sum) + (ref - t) * kLn2;
+    e.inv[c] = 1.0f / sum;
+    e.rest[c] = z / sum;
+    e.lse2[c] = ref == t ? log1pf(z) * kLog2e + t : log2f(sum) + ref;
+}
+
+// STATS: joins and ends
+__global__ void __launch_bounds__(1024) lce_score_kernel(Join a, const float* at_label, RowEnd e) {
+    __shared__ f32x2 lds[16][64];
+    f32x2 v;
+    int64_t r;
+    auto fold = [](f32x2 p, f32x2 q) {
+        const float top = fmaxf(p[0], q[0]);
+        if (top == -INFINITY) return f32x2{top, p[1] + q[1]};
+        return f32x2{top, p[1] * __builtin_amdgcn_exp2f(p[0] - top) + q[1] * __builtin_amdgcn_exp2f(q[0] - top)};
+    };
+    if (!join_rows(a, lds, f32x2{-INFINITY, 0.0f}, fold, &v, &r)) return;
+    const float t = at_label[r];
+    const float ref = v[0] > t ? v[0] : t;
+    end_row(e, r, v[1] * __builtin_amdgcn_exp2f(v[0] - ref), ref, t);
+}
+
+__global__ void __launch_bounds__(256) lce_end_kernel(const int32_t* count, const float* z, const float* ref, const float* at_label, RowEnd e) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c < *count) end_row(e, c, z[c], ref[c], at_label[c]);
+}
+
+// losses to where their rows are, or their sum or mean: one block, in an order that the sizes fix
+__global__ void __launch_bounds__(1024) lce_reduce_kernel(const int32_t* count, const float* loss, int mean, float* out) {
+    __shared__ double lds[16];
+    const int n = *count;
+    double s = 0.0;
+    for (int c = threadIdx.x; c < n; c += 1024) s += (double)loss[c];
+#pragma unroll
+    for (int d = 32; d; d >>= 1) s += __shfl_xor(s, d);
+    if ((threadIdx.x & 63) == 0) lds[threadIdx.x >> 6] = s;
+    __syncthreads();
+    if (threadIdx.x) return;
+    for (int w = 1; w < 16; ++w) s += lds[w];
+    *out = (float)(mean ? s / n : s);
+}
+__global__ void __launch_bounds__(256) lce_place_kernel(const int32_t* place, int64_t M, const float* loss, float* out) {
+    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (i >= M) return;
+    const int c = place[i];
+    out[i] = c < 0 ? 0.0f : loss[c];
+}
+
+// ---- backward
+struct Upstream {
+    const float* grad;
+    int32_t reduction;
+    const int32_t* count;
+    float scale;
+};
+__device__ __forceinline__ float upstream(const Upstream& u, int64_t row) {
+    const float g = u.grad[u.reduction == XQ_LCE_NONE ? row : 0] * u.scale;
+    return u.reduction == XQ_LCE_MEAN ? g / (float)*u.count : g;
+}
+
+// dx: a block has rows of x, a thread 8 columns at a time
+__global__ void __launch_bounds__(256) lce_dx_kernel(const int32_t* place, const int32_t* label, int64_t M, int H, const float* o, int splits, int64_t split_stride,
+                                                     const float* inv, const float* rest, const bf16_t* w, int64_t ldw, Upstream u, bf16_t* dx, int64_t lddx) {
+    const int64_t i = blockIdx.x;
+    const int c = place[i];
+    bf16_t* out = dx + i * lddx;
+    if (c < 0) {
+        for (int k = threadIdx.x * 8; k < H; k += 2048) *(u32x4*)(out + k) = u32x4{0, 0, 0, 0};
+        return;
+    }
+    const float g = upstream(u, i);
+    const float a = g * inv[c], b = label[c] < 0 ? __builtin_nanf("") : g * rest[c];
+    const bf16_t* wr = w + max(label[c], 0) * ldw;
+    const float* oc = o + (int64_t)c * H;
+    for (int k = threadIdx.x * 8; k < H; k += 2048) {
+        const u32x4 t = *(const u32x4*)(wr + k);
+        f32x4 lo = *(const f32x4*)(oc + k), hi = *(const f32x4*)(oc + k + 4);
+        for (int s = 1; s < splits; ++s) {
+            lo += *(const f32x4*)(oc + s * split_stride + k);
+            hi += *(const f32x4*)(oc + s * split_stride + k + 4);
+        }
+        const f32x4 tl = bf16x4_f32(u32x2{t[0], t[1]}), th = bf16x4_f32(u32x2{t[2], t[3]});
+        lo = lo * a - tl * b;
+        hi = hi * a - th * b;
+        *(u32x4*)(out + k) = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
+    }
+}
+
+// the factors of the head's gradient by row, and the rows of x that count in order
+__global__ void __launch_bounds__(256) lce_factors_kernel(LceRows rows, int64_t M_pad, const float* lse2, const float* rest, Upstream u, float* lse_out, float* up_out,
+                                                          float* rest_out) {
+    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
+    if (c >= M_pad) return;
+    const bool in = c < *rows.count;
+    lse_out[c] = in ? lse2[c] : INFINITY;
+    up_out[c] = in ? upstream(u, rows.row[c]) : 0.0f;
+    rest_out[c] = in ? rest[c] : 0.0f;
+}
+__global__ void __launch_bounds__(256) lce_gather_kernel(LceRows rows, const bf16_t* x, int64_t ldx, int H, bf16_t* out) {
+    const int64_t c = blockIdx.x;
+    if (c >= *rows.count) return;
+    const bf16_t* xr = x + rows.row[c] * ldx;
+    for (int k = threadIdx.x * 8; k < H; k += 2048) *(u32x4*)(out + c * H + k) = *(const u32x4*)(xr + k);
+}
+
+// ---------------------------------------------------------------- host side
+struct Plan {
+    int tm;                             // rows of a tile: 32 tm
+    int64_t rows_pad, piece, pieces;    // columns of the vocabulary at a time (a multiple of 256), and how many times
+    int splits;                         // of the product E . W
+};
+
+int tile_for(int64_t rows) { return rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }
+
+Plan plan_tokens(int64_t M, int64_t V, int64_t H) {
+    Plan p;
+    p.tm = tile_for(M);
+    p.rows_pad = up256(std::max<int64_t>(M, 1));
+    const int64_t most = std::max<int64_t>(256, kPieceBytes / (p.rows_pad * 2) / 256 * 256);
+    p.pieces = xq_cdiv(up256(V), most);
+    p.piece = up256(xq_cdiv(up256(V), p.pieces));
+    p.pieces = xq_cdiv(V, p.piece);
+    const int64_t tiles = xq_cdiv(std::max<int64_t>(M, 1), 32 * p.tm) * xq_cdiv(H, 256);
+    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, p.piece / 512));
+    return p;
+}
+
+Plan plan_head(int64_t M, int64_t V) {       // G: rows of the vocabulary, tokens along the contraction
+    Plan p;
+    p.tm = 8;
+    p.rows_pad = up256(std::max<int64_t>(M, 1));
+    const int64_t most = std::max<int64_t>(256, kPieceBytes / (p.rows_pad * 2) / 256 * 256);
+    p.pieces = xq_cdiv(up256(V), most);
+    p.piece = up256(xq_cdiv(up256(V), p.pieces));
+    p.pieces = xq_cdiv(V, p.piece);
+    p.splits = 1;
+    return p;
+}
+
+// what a forward leaves for the backward
+struct Saved {
+    int32_t *count, *row, *label, *place;
+    float *at_label, *inv, *rest, *lse2, *loss, *o;
+    int64_t bytes;
+};
+Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
+    const Plan p = plan_tokens(M, V, H);
+    uint8_t* at = (uint8_t*)base;
+    auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
+    Saved s;
+    s.count = (int32_t*)take(4);
+    s.row = (int32_t*)take(4 * p.rows_pad);
+    s.label = (int32_t*)take(4 * p.rows_pad);
+    s.place = (int32_t*)take(4 * p.rows_pad);
+    s.at_label = (float*)take(4 * p.rows_pad);
+    s.inv = (float*)take(4 * p.rows_pad);
+    s.rest = (float*)take(4 * p.rows_pad);
+    s.lse2 = (float*)take(4 * p.rows_pad);
+    s.loss = (float*)take(4 * p.rows_pad);
+    s.o = keep == XQ_LCE_KEEP_DX ? (float*)take(4 * p.splits * M * H) : nullptr;
+    s.bytes = at - (uint8_t*)base;
+    return s;
+}
+
+struct Scratch {
+    float *ref, *z, *alpha, *up;
+    int32_t* redo;
+    f32x2* part;
+    bf16_t *image, *x;
+    int64_t bytes;
+};
+Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
+    const Plan p = pass == XQ_LCE_KEEP_HEAD_BWD ? plan_head(M, V) : plan_tokens(M, V, H);
+    uint8_t* at = (uint8_t*)base;
+    auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
+    Scratch s = {};
+    s.ref = (float*)take(4 * p.rows_pad);
+    s.z = (float*)take(4 * p.rows_pad);
+    s.alpha = (float*)take(4 * p.rows_pad);
+    s.up = (float*)take(4 * p.rows_pad);
+    s.redo = (int32_t*)take(4 * (p.rows_pad / 64));
+    if (pass == XQ_LCE_KEEP_HEAD_BWD) {
+        s.x = (bf16_t*)take(2 * M * H);
+        s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
+    } else {
+        const int64_t columns = pass == XQ_LCE_KEEP_DX ? p.piece : up256(V);
+        s.part = (f32x2*)take(8 * p.rows_pad * (columns / 256));
+        if (pass == XQ_LCE_KEEP_DX) s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
+    }
+    s.bytes = at - (uint8_t*)base;
+    return s;
+}
+
+template <int TM, int MODE>
+int launch_logits(const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_t s) {
+    using T = LceTile<TM>;
+    auto k = lce_logits_kernel<TM, MODE>;
+    static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
+    if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
+    k<<<dim3((unsigned)(xq_cdiv(rows, T::ROWS) * xq_cdiv(cols, 256))), 512, T::LDS_BYTES, s>>>(a);
+    return XQ_OK;
+}
+template <int MODE>
+int launch_logits(int tm, const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_t s) {
+    return tm == 2 ? launch_logits<2, MODE>(a, rows, cols, s) : tm == 4 ? launch_logits<4, MODE>(a, rows, cols, s) : launch_logits<8, MODE>(a, rows, cols, s);
+}
+template <int TM>
+int launch_product(const LceProductArgs& a, int64_t rows, hipStream_t s) {
+    using T = LceTile<TM>;
+    auto k = lce_product_kernel<TM>;
+    static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
+    if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
+    k<<<dim3((unsigned)(xq_cdiv(rows, T::ROWS) * xq_cdiv(a.H, 256)), a.splits), 512, T::LDS_BYTES, s>>>(a);
+    return XQ_OK;
+}
+int launch_product(int tm, const LceProductArgs& a, int64_t rows, hipStream_t s) {
+    return tm == 2 ? launch_product<2>(a, rows, s) : tm == 4 ? launch_product<4>(a, rows, s) : launch_product<8>(a, rows, s);
+}
+
+int check_problem(const char* who, const xq_lce_problem* q, const void* ws, int64_t ws_bytes, int64_t need, const void* saved, int64_t saved_need) {
+    XQ_REQUIRE(q, "%s: the problem is NULL", who);
+    XQ_REQUIRE(q->M >= 0 && q->M < (1 << 30) && q->V >= 1 && q->V < (1 << 30), "%s: %lld rows, %lld columns of logits", who, (long long)q->M, (long long)q->V);
+    XQ_REQUIRE(q->H >= 64 && q->H % 64 == 0 && q->H < (1 << 24), "%s: the hidden size must be a multiple of 64, got %lld", who, (long long)q->H);
+    XQ_REQUIRE(q->reduction >= XQ_LCE_NONE && q->reduction <= XQ_LCE_SUM, "%s: unknown reduction %d", who, q->reduction);
+    XQ_REQUIRE(q->label_bytes == 4 || q->label_bytes == 8, "%s: labels are int32 or int64, got %d bytes", who, q->label_bytes);
+    XQ_REQUIRE(q->logit_scale > 0.0f && q->logit_scale < INFINITY, "%s: logit_scale must be positive and finite, got %g", who, (double)q->logit_scale);
+    XQ_REQUIRE(q->w && xq_aligned(q->w, 16) && q->ldw >= q->H && q->ldw % 8 == 0, "%s: the head must be 16-byte aligned with a row stride that is a multiple of 8 elements", who);
+    XQ_REQUIRE(q->M == 0 || (q->x && xq_aligned(q->x, 16) && q->ldx >= q->H && q->ldx % 8 == 0),
+               "%s: x must be 16-byte aligned with a row stride that is a multiple of 8 elements", who);
+    XQ_REQUIRE(q->M == 0 || (q->labels && xq_aligned(q->labels, q->label_bytes)), "%s: labels are NULL or misaligned", who);
+    XQ_REQUIRE(ws && xq_aligned(ws, 256) && ws_bytes >= need, "%s: a workspace of %lld bytes, 256-byte aligned, is needed", who, (long long)need);
+    XQ_REQUIRE(saved_need == 0 || (saved && xq_aligned(saved, 256)), "%s: the saved buffer is NULL or not 256-byte aligned", who);
+    return XQ_OK;
+}
+
+}  // namespace
+}  // namespace xq
+
+using namespace xq;
+
+extern "C" int64_t xq_lce_saved_bytes(int64_t M, int64_t V, int64_t H, int keep) {
+    if (M < 0 || V < 1 || H < 1) return -1;
+    return saved_of(nullptr, M, V, H, keep).bytes;
+}
+
+extern "C" int64_t xq_lce_workspace_bytes(int64_t M, int64_t V, int64_t H, int pass) {
+    if (M < 0 || V < 1 || H < 1) return -1;
+    return scratch_of(nullptr, M, V, H, pass).bytes;
+}
+
+extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int keep, void* workspace, int64_t workspace_bytes, void* stream) {
+    XQ_REQUIRE(q && keep >= XQ_LCE_KEEP_NONE && keep <= XQ_LCE_KEEP_DX, "xq_lce_fwd: the problem is NULL or keep is unknown");
+    int rc = check_problem("xq_lce_fwd", q, workspace, workspace_bytes, xq_lce_workspace_bytes(q->M, q->V, q->H, keep), saved, 1);
+    if (rc != XQ_OK) return rc;
+    XQ_REQUIRE((loss && xq_aligned(loss, 4)) || (q->M == 0 && q->reduction == XQ_LCE_NONE), "xq_lce_fwd: loss is NULL or misaligned");
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t M = q->M, V = q->V, H = q->H;
+    const Plan p = plan_tokens(M, V, H);
+    const Saved s = saved_of(saved, M, V, H, keep);
+    const Scratch c = scratch_of(workspace, M, V, H, keep);
+    const LceRows rows = {s.count, s.row, s.label};
+    const RowEnd end = {s.inv, s.rest, s.lse2, s.loss};
+    const float scale2 = q->logit_scale * kLog2e;
+    lce_prepare_kernel<<<dim3(1), 1024, 0, st>>>(Prep{q->labels, q->label_bytes, M, p.rows_pad, V, q->ignore_index, s.count, s.row, s.label, s.place, s.at_label});
+    const dim3 by64((unsigned)xq_cdiv(M, 64)), by256((unsigned)xq_cdiv(M, 256));
+    LceLogitsArgs a = {};
+    a.A = (const bf16_t*)q->x; a.lda = q->ldx; a.B = (const bf16_t*)q->w; a.ldb = q->ldw;
+    a.H = (int32_t)H; a.rows = rows; a.scale2 = scale2; a.part = c.part; a.at_label = s.at_label; a.rows_pad = p.rows_pad;
+    if (M > 0 && keep != XQ_LCE_KEEP_DX) {
+        a.first_v = 0; a.n_v = (int32_t)V;
+        if ((rc = launch_logits<kLceStats>(p.tm, a, M, V, st)) != XQ_OK) return rc;
+        lce_score_kernel<<<by64, 1024, 0, st>>>(Join{s.count, c.part, p.rows_pad, (int32_t)xq_cdiv(V, 256), 0, nullptr, nullptr, nullptr, nullptr}, s.at_label, end);
+    } else if (M > 0) {
+        lce_target_kernel<<<dim3((unsigned)xq_cdiv(M, 4)), 256, 0, st>>>(rows, a.A, a.lda, a.B, a.ldb, (int)H, scale2, s.at_label, c.ref, c.z);
+        const int row_tiles = (int)xq_cdiv(M, 32 * p.tm);
+        for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+            const int64_t n = std::min(p.piece, V - v0);
+            a.first_v = (int32_t)v0; a.n_v = (int32_t)n; a.ref = c.ref; a.image = c.image; a.image_steps = (int32_t)(p.piece / 32); a.redo = nullptr;
+            if ((rc = launch_logits<kLceExp>(p.tm, a, M, n, st)) != XQ_OK) return rc;
+            lce_clear_kernel<<<dim3(1), 256, 0, st>>>(c.redo, row_tiles);
+            const Join j = {s.count, c.part, p.rows_pad, (int32_t)xq_cdiv(n, 256), 32 * p.tm, c.ref, c.z, c.alpha, c.redo};
+            lce_far_kernel<<<by64, 1024, 0, st>>>(j);
+            a.redo = c.redo;
+            if ((rc = launch_logits<kLceExp>(p.tm, a, M, n, st)) != XQ_OK) return rc;
+            lce_sum_kernel<<<by64, 1024, 0, st>>>(j);
+            LceProductArgs o = {};
+            o.image = c.image; o.image_steps = a.image_steps; o.rows = -1; o.k = (int32_t)n; o.count = s.count;
+            o.B = a.B + v0 * a.ldb; o.ldb = a.ldb; o.H = (int32_t)H; o.splits = p.splits;
+            o.out = s.o; o.split_stride = M * H; o.alpha = c.alpha; o.add = v0 > 0;
+            if ((rc = launch_product(p.tm, o, M, st)) != XQ_OK) return rc;
+        }
+        lce_end_kernel<<<by256, 256, 0, st>>>(s.count, c.z, c.ref, s.at_label, end);
+    }
+    if (q->reduction != XQ_LCE_NONE) lce_reduce_kernel<<<dim3(1), 1024, 0, st>>>(s.count, s.loss, q->reduction == XQ_LCE_MEAN, loss);
+    else if (M > 0) lce_place_kernel<<<by256, 256, 0, st>>>(s.place, M, s.loss, loss);
+    XQ_CHECK_LAUNCH("xq_lce_fwd");
+    return XQ_OK;
+}
+
+extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void* saved, int keep, void* dx, int64_t lddx, void* dw, int64_t lddw,
+                          void* workspace, int64_t workspace_bytes, void* stream) {
+    XQ_REQUIRE(q && (keep == XQ_LCE_KEEP_HEAD || keep == XQ_LCE_KEEP_DX), "xq_lce_bwd: the problem is NULL, or its forward kept nothing");
+    int rc = check_problem("xq_lce_bwd", q, dw ? workspace : (const void*)256, dw ? workspace_bytes : 0, dw ? xq_lce_workspace_bytes(q->M, q->V, q->H, XQ_LCE_KEEP_HEAD_BWD) : 0,
+                           saved, 1);
+    if (rc != XQ_OK) return rc;
+    XQ_REQUIRE((grad && xq_aligned(grad, 4)) || q->M == 0, "xq_lce_bwd: the upstream gradient is NULL or misaligned");
+    XQ_REQUIRE(!dx || keep == XQ_LCE_KEEP_DX, "xq_lce_bwd: the forward was not asked to keep what dx needs");
+    XQ_REQUIRE(!dx || (xq_aligned(dx, 16) && lddx >= q->H && lddx % 8 == 0), "xq_lce_bwd: dx must be 16-byte aligned with a row stride that is a multiple of 8 elements");
+    XQ_REQUIRE(!dw || (xq_aligned(dw, 16) && lddw >= q->H && lddw % 8 == 0), "xq_lce_bwd: dw must be 16-byte aligned with a row stride that is a multiple of 8 elements");
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t M = q->M, V = q->V, H = q->H;
+    const Plan p = plan_tokens(M, V, H);
+    const Saved s = saved_of((void*)saved, M, V, H, keep);
+    const LceRows rows = {s.count, s.row, s.label};
+    const Upstream u = {grad, q->reduction, s.count, q->logit_scale};
+    if (dx && M > 0)
+        lce_dx_kernel<<<dim3((unsigned)M), 256, 0, st>>>(s.place, s.label, M, (int)H, s.o, p.splits, M * H, s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
+    if (dw) {
+        const Plan h = plan_head(M, V);
+        const Scratch c = scratch_of(workspace, M, V, H, XQ_LCE_KEEP_HEAD_BWD);
+        if (M > 0) {
+            lce_factors_kernel<<<dim3((unsigned)(h.rows_pad / 256)), 256, 0, st>>>(rows, h.rows_pad, s.lse2, s.rest, u, c.ref, c.up, c.z);
+            lce_gather_kernel<<<dim3((unsigned)M), 256, 0, st>>>(rows, (const bf16_t*)q->x, q->ldx, (int)H, c.x);
+        }
+        LceLogitsArgs a = {};
+        a.A = (const bf16_t*)q->w; a.lda = q->ldw; a.B = (const bf16_t*)q->x; a.ldb = q->ldx;
+        a.H = (int32_t)H; a.rows = rows; a.scale2 = q->logit_scale * kLog2e; a.ref = c.ref; a.grad = c.up; a.rest = c.z; a.rows_pad = h.rows_pad;
+        a.image = c.image; a.image_steps = (int32_t)(h.rows_pad / 32);
+        for (int64_t v0 = 0; v0 < V; v0 += h.piece) {
+            const int64_t n = std::min(h.piece, V - v0);
+            a.first_v = (int32_t)v0; a.n_v = (int32_t)n;
+            if (M > 0 && (rc = launch_logits<kLceGrad>(h.tm, a, n, M, st)) != XQ_OK) return rc;
+            LceProductArgs o = {};
+            o.image = c.image; o.image_steps = a.image_steps; o.rows = (int32_t)n; o.k = -1; o.count = s.count;
+            o.B = c.x; o.ldb = H; o.H = (int32_t)H; o.splits = 1;
+            o.out16 = (bf16_t*)dw + v0 * lddw; o.ld16 = lddw;
+            if ((rc = launch_product(h.tm, o, n, st)) != XQ_OK) return rc;
+        }
+    }
+    XQ_CHECK_LAUNCH("xq_lce_bwd");
+    return XQ_OK;
+}
