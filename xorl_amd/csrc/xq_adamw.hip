@@ -16,6 +16,8 @@
 // step counts advanced and the bias corrections in 64 bits.  One launch then walks all tensors: chunks of 4096 elements, numbered through,
 // are dealt out to the blocks in ranges; a block looks its first chunk up in the table (two steps of 64 lanes) and goes on from there.
 #include <algorithm>
+#include <cmath>
+#include <type_traits>
 
 #include "xq_common.h"
 
@@ -26,7 +28,7 @@ constexpr int kBlock = 256;                 // elements that share a scale: a wa
 constexpr int kChunk = 4096;                // of a thread block at a time: four 256-element pieces of each of its waves
 constexpr int kThreads = 256;
 constexpr int kTableArgs = 52;              // tensors by value in one launch: 3744 of the 4096 bytes that arguments may take
-constexpr int kNormBlocks = 1024;
+constexpr int kNormBlocks = 2048;
 constexpr int kStepBlocks = 2048;           // eight of a compute unit
 
 struct Row {                                // what the walking kernels read of a tensor
@@ -50,26 +52,30 @@ struct TableScalars {
     Row* rows;
     int64_t chunk0;
     int32_t n, at, step;                    // step: advance the step counts
-    double lr, beta1, beta2;
+    double lr, log_beta1, log_beta2;
     const float* lr_device;
 };
 
 __global__ void __launch_bounds__(64) adamw_table_kernel(TableArgs a, TableScalars s) {
     const int i = threadIdx.x;
+    const xq_adamw_tensor t = a.t[min(i, s.n - 1)];
+    int64_t end = i < s.n ? (t.numel + kChunk - 1) / kChunk : 0;
+    const int64_t own = end;
+    for (int d = 1; d < 64; d <<= 1) {
+        const int64_t before = __shfl_up(end, d);
+        if (i >= d) end += before;
+    }
     if (i >= s.n) return;
-    const xq_adamw_tensor t = a.t[i];
-    int64_t chunk0 = s.chunk0;
-    for (int k = 0; k < i; ++k) chunk0 += (a.t[k].numel + kChunk - 1) / kChunk;
     float first = 0.0f, root = 0.0f;
     if (s.step) {
         const float step = *t.step + 1.0f;
         *t.step = step;
         const double lr = s.lr_device ? (double)*s.lr_device : s.lr;
-        first = (float)(lr / (1.0 - pow(s.beta1, (double)step)));
-        root = (float)(1.0 / sqrt(1.0 - pow(s.beta2, (double)step)));
+        first = (float)(lr / (1.0 - exp(step * s.log_beta1)));             // b^t; a beta of 0 has the logarithm -inf
+        root = (float)(1.0 / sqrt(1.0 - exp(step * s.log_beta2)));
     }
-    s.rows[s.at + i] = Row{t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.numel, chunk0, first, root,
-                              t.param_dtype == XQ_DT_BF16, t.grad_dtype == XQ_DT_BF16};
+    s.rows[s.at + i] = Row{t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.numel, s.chunk0 + end - own, first, root,
+                           t.param_dtype == XQ_DT_BF16, t.grad_dtype == XQ_DT_BF16};
 }
 
 // the last row whose first chunk is not behind `chunk` (rows in order of their first chunks, no row without chunks)
@@ -91,81 +97,104 @@ template <bool BF16>
 __device__ __forceinline__ float load1(const void* p, int64_t i) {
     return BF16 ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i];
 }
-// four elements from i on; behind the tensor's end: zeros
-template <bool BF16>
-__device__ __forceinline__ f32x4 load4(const void* p, int64_t i, int64_t n, bool vec) {
-    if (vec && i + 4 <= n) {
-        if constexpr (BF16) {
-            const u32x2 w = *(const u32x2*)((const bf16_t*)p + i);
-            return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
-        } else {
-            return *(const f32x4*)((const float*)p + i);
-        }
-    }
-    f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
+// four elements from i on.  WHOLE: all there, at an address for one access; otherwise one by one, zeros behind the tensor's end
+template <bool WHOLE>
+__device__ __forceinline__ f32x4 load4(bool bf16, const void* p, int64_t i, int64_t n) {
+    if constexpr (WHOLE) {
+        if (!bf16) return *(const f32x4*)((const float*)p + i);
+        const u32x2 w = *(const u32x2*)((const bf16_t*)p + i);
+        return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
+    } else {
+        f32x4 r = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (i + k < n) r[k] = load1<BF16>(p, i + k);
-    return r;
+        for (int k = 0; k < 4; ++k)
+            if (i + k < n) r[k] = bf16 ? load1<true>(p, i + k) : load1<false>(p, i + k);
+        return r;
+    }
 }
-template <bool BF16>
-__device__ __forceinline__ void store4(void* p, int64_t i, int64_t n, bool vec, f32x4 v) {
-    if (vec && i + 4 <= n) {
-        if constexpr (BF16) *(u32x2*)((bf16_t*)p + i) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+template <bool WHOLE>
+__device__ __forceinline__ void store4(bool bf16, void* p, int64_t i, int64_t n, f32x4 v) {
+    if constexpr (WHOLE) {
+        if (bf16) *(u32x2*)((bf16_t*)p + i) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
         else *(f32x4*)((float*)p + i) = v;
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (i + k < n) {
-            if constexpr (BF16) ((bf16_t*)p)[i + k] = to_bf16(v[k]);
-            else ((float*)p)[i + k] = v[k];
-        }
+        for (int k = 0; k < 4; ++k)
+            if (i + k < n) {
+                if (bf16) ((bf16_t*)p)[i + k] = to_bf16(v[k]);
+                else ((float*)p)[i + k] = v[k];
+            }
+    }
 }
-__device__ __forceinline__ f32x4 load4(bool bf16, const void* p, int64_t i, int64_t n, bool vec) {
-    return bf16 ? load4<true>(p, i, n, vec) : load4<false>(p, i, n, vec);
-}
-// whether four elements from a multiple of four on can be accessed as one
-__device__ __forceinline__ bool whole(const void* p, bool bf16) { return ((uintptr_t)p & (bf16 ? 7 : 15)) == 0; }
-__device__ __forceinline__ uint32_t load4_codes(const void* p, int64_t i, int64_t n, bool vec) {
-    if (vec && i + 4 <= n) return *(const uint32_t*)((const uint8_t*)p + i);
+template <bool WHOLE>
+__device__ __forceinline__ uint32_t load4_codes(const void* p, int64_t i, int64_t n) {
+    if constexpr (WHOLE) return *(const uint32_t*)((const uint8_t*)p + i);
     uint32_t r = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k)
         if (i + k < n) r |= (uint32_t)((const uint8_t*)p)[i + k] << (8 * k);
     return r;
 }
-__device__ __forceinline__ void store4_codes(void* p, int64_t i, int64_t n, bool vec, uint32_t c) {
-    if (vec && i + 4 <= n) {
+template <bool WHOLE>
+__device__ __forceinline__ void store4_codes(void* p, int64_t i, int64_t n, uint32_t c) {
+    if constexpr (WHOLE) {
         *(uint32_t*)((uint8_t*)p + i) = c;
-        return;
-    }
+    } else {
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        if (i + k < n) ((uint8_t*)p)[i + k] = (uint8_t)(c >> (8 * k));
+        for (int k = 0; k < 4; ++k)
+            if (i + k < n) ((uint8_t*)p)[i + k] = (uint8_t)(c >> (8 * k));
+    }
 }
+// whether four elements from a multiple of four on can be accessed as one
+__device__ __forceinline__ bool whole4(const void* p, bool bf16) { return ((uintptr_t)p & (bf16 ? 7 : 15)) == 0; }
 
 // the largest over a wave of the bits of non-negative floats: NaN lies above infinity, so that neither is lost
 __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
-#pragma unroll
-    for (int d = 1; d < 64; d <<= 1) v = max(v, (uint32_t)__shfl_xor((int)v, d));
-    return v;
+    // (0 for the lanes that get nothing: the identity, with which each step is one instruction)
+    auto from = [](uint32_t x, auto ctrl, auto rows) {
+        return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, decltype(ctrl)::value, decltype(rows)::value, 0xf, false);
+    };
+    using All = std::integral_constant<int, 0xf>;
+    v = max(v, from(v, std::integral_constant<int, 0xb1>{}, All{}));       // lanes 1, 0, 3, 2 of four
+    v = max(v, from(v, std::integral_constant<int, 0x4e>{}, All{}));       // 2, 3, 0, 1
+    v = max(v, from(v, std::integral_constant<int, 0x141>{}, All{}));      // mirrored within eight
+    v = max(v, from(v, std::integral_constant<int, 0x140>{}, All{}));      // within sixteen
+    v = max(v, from(v, std::integral_constant<int, 0x142>{}, std::integral_constant<int, 0xa>{}));     // lane 15 of a row of sixteen to the next
+    v = max(v, from(v, std::integral_constant<int, 0x143>{}, std::integral_constant<int, 0xc>{}));     // lane 31 to the upper half
+    return (uint32_t)__builtin_amdgcn_readlane((int)v, 63);
 }
 __device__ __forceinline__ uint32_t bits_abs(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-// what a code stands for, and the code of a value: `inv` is the reciprocal of the block's largest magnitude (0 where that is 0).  The
-// hardware root is off by an ulp at most: it decides between two codes only where the value lies that near the middle.
-__device__ __forceinline__ float m_value(int c, float scale) { return (float)(c * (c < 0 ? -c : c)) * (scale * (1.0f / 16129.0f)); }
-__device__ __forceinline__ float s_value(uint32_t d, float scale) { return (float)(d * d) * (scale * (1.0f / 65025.0f)); }
-__device__ __forceinline__ int m_code(float m, float inv) {
-    const int c = (int)fminf(__builtin_rintf(127.0f * __builtin_amdgcn_sqrtf(fabsf(m) * inv)), 127.0f);
-    return m < 0.0f ? -c : c;
+// Codes of four elements.  The instruction that packs a byte rounds to nearest even and saturates, so that a code takes a product, a
+// root and a packing; m goes in as 128 + c, whose top bit is flipped afterwards.  The hardware root and reciprocal are off by an ulp at
+// most: it decides between two codes only where the value lies that near the middle.  inv: top code squared over the block's largest.
+__device__ __forceinline__ uint32_t m_codes(f32x4 m, float inv) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k)
+        c = __builtin_amdgcn_cvt_pk_u8_f32(128.0f + __builtin_copysignf(__builtin_amdgcn_sqrtf(fabsf(m[k]) * inv), m[k]), k, c);
+    return c ^ 0x80808080u;
 }
-__device__ __forceinline__ uint32_t s_code(float s, float inv) {
-    const uint32_t d = (uint32_t)fminf(__builtin_rintf(255.0f * __builtin_amdgcn_sqrtf(s * inv)), 255.0f);
-    return s > 0.0f ? max(d, 1u) : 0u;
+__device__ __forceinline__ uint32_t s_codes(f32x4 s, float inv) {
+    uint32_t c = 0;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        const float least = __builtin_amdgcn_fmed3f(s[k] * 0x1p120f, 0.0f, 1.0f);      // 1, or 0 for 0
+        c = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(__builtin_amdgcn_sqrtf(s[k] * inv), least), k, c);
+    }
+    return c;
 }
-__device__ __forceinline__ float reciprocal_or_0(float a) { return a > 0.0f ? 1.0f / a : 0.0f; }
+// what they stand for: scale is the block's largest magnitude over the top code squared
+__device__ __forceinline__ float m_value(uint32_t codes, int k, float scale) {
+    const float c = (float)(int8_t)(codes >> (8 * k));
+    return c * fabsf(c) * scale;
+}
+__device__ __forceinline__ float s_value(uint32_t codes, int k, float scale) {
+    const float d = (float)((codes >> (8 * k)) & 0xffu);
+    return d * d * scale;
+}
+constexpr float kM2 = 127.0f * 127.0f, kS2 = 255.0f * 255.0f;
+constexpr float kSmallest = 1e-30f;         // blocks below it take the lowest codes: the quotient stays finite
 
 struct StepArgs {
     const Row* rows;
@@ -176,82 +205,114 @@ struct StepArgs {
     const float* lr_device;
 };
 
+// constants of a call
+struct Call {
+    float clip, keep;                       // of the gradients; minus the decay
+    float g, g_root, m_value, s_value;      // 8 bits: what g counts in m' and, squared, in v'; what a squared code counts in either
+};
+
+// a wave's four pieces of a chunk, from element base on (lane 0's) 1024 apart; everything is read before anything is computed
+// (types known to the compiler where the pieces are whole: a branch on them between the loads would wait for each)
+template <bool EIGHT, bool WHOLE, bool P16, bool G16>
+__device__ __forceinline__ void step_chunk(const StepArgs& a, const Row& r, int64_t base, int lane, const Call& c) {
+    constexpr int N = WHOLE ? 4 : 1;
+    const bool p16 = WHOLE ? P16 : r.param16, g16 = WHOLE ? G16 : r.grad16;
+    const int64_t n = r.numel;
+#pragma unroll 1
+    for (int u0 = 0; u0 < 4; u0 += N) {
+        if (!WHOLE && base + u0 * (kThreads * 4) >= n) break;                // (the whole wave's piece lies behind the end)
+        f32x4 p[N], g[N], m[N], v[N];
+        uint32_t mc[N], vc[N];
+        float ms[N], vs[N];
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int64_t i = base + (u0 + u) * (kThreads * 4) + lane * 4;
+            g[u] = load4<WHOLE>(g16, r.grad, i, n);
+            if constexpr (EIGHT) {
+                mc[u] = load4_codes<WHOLE>(r.m, i, n);
+                vc[u] = load4_codes<WHOLE>(r.v, i, n);
+                ms[u] = r.m_scale[i >> 8];
+                vs[u] = r.v_scale[i >> 8];
+            } else {
+                m[u] = load4<WHOLE>(false, r.m, i, n);
+                v[u] = load4<WHOLE>(false, r.v, i, n);
+            }
+            p[u] = load4<WHOLE>(p16, r.param, i, n);
+        }
+#pragma unroll
+        for (int u = 0; u < N; ++u) {
+            const int64_t i = base + (u0 + u) * (kThreads * 4) + lane * 4;
+            f32x4 s;
+            uint32_t mb = 0, sb = 0;
+            if constexpr (EIGHT) {
+                // bound by instructions: what is constant over a block or a call is multiplied together first, and root and reciprocal are the
+                // hardware's (an ulp each)
+                const float mk = ms[u] * c.m_value, sk = vs[u] * c.s_value;
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float h = g[u][k] * c.g_root, q = (float)((vc[u] >> (8 * k)) & 0xffu), old = q * q * sk, e = (float)(int8_t)(mc[u] >> (8 * k));
+                    m[u][k] = fmaf(e * fabsf(e), mk, g[u][k] * c.g);
+                    s[k] = __builtin_amdgcn_sqrtf(fmaf(old, old, h * h));
+                    p[u][k] = fmaf(p[u][k], c.keep, p[u][k]) - m[u][k] * r.first * __builtin_amdgcn_rcpf(fmaf(s[k], r.root, a.eps));
+                    mb = max(mb, bits_abs(m[u][k]));
+                    sb = max(sb, __float_as_uint(s[k]));
+                }
+            } else {
+#pragma unroll
+                for (int k = 0; k < 4; ++k) {
+                    const float gk = g[u][k] * c.clip;
+                    m[u][k] = fmaf(a.beta1, m[u][k], a.one_minus_beta1 * gk);
+                    v[u][k] = fmaf(a.beta2, v[u][k], a.one_minus_beta2 * (gk * gk));
+                    p[u][k] = fmaf(p[u][k], c.keep, p[u][k]) - m[u][k] * r.first / fmaf(sqrtf(v[u][k]), r.root, a.eps);
+                }
+            }
+            store4<WHOLE>(p16, r.param, i, n, p[u]);
+            if constexpr (EIGHT) {
+                const float mt = __uint_as_float(wave_max_bits(mb)), st = __uint_as_float(wave_max_bits(sb) & 0x7fffffffu);
+                store4_codes<WHOLE>(r.m, i, n, m_codes(m[u], mt > kSmallest ? kM2 * __builtin_amdgcn_rcpf(mt) : 0.0f));
+                store4_codes<WHOLE>(r.v, i, n, s_codes(s, st > kSmallest ? kS2 * __builtin_amdgcn_rcpf(st) : 0.0f));
+                if (lane == 0) {
+                    r.m_scale[i >> 8] = mt;
+                    r.v_scale[i >> 8] = st;
+                }
+            } else {
+                store4<WHOLE>(false, r.m, i, n, m[u]);
+                store4<WHOLE>(false, r.v, i, n, v[u]);
+            }
+        }
+    }
+}
+
 template <bool EIGHT>
 __global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs a) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     int64_t c = a.chunks * blockIdx.x / gridDim.x;
     const int64_t c1 = a.chunks * (blockIdx.x + 1) / gridDim.x;
     if (c >= c1) return;
-    const float decay = (a.lr_device ? *a.lr_device : a.lr) * a.weight_decay;
+    Call k;
+    k.keep = -(a.lr_device ? *a.lr_device : a.lr) * a.weight_decay;
     // (written so that a NaN norm makes the gradients NaN)
     float clip = 1.0f;
     if (a.norm) {
         clip = a.max_norm / (*a.norm + 1e-6f);
         clip = clip > 1.0f ? 1.0f : clip;
     }
+    k.clip = clip;
+    k.g = a.one_minus_beta1 * clip;
+    k.g_root = sqrtf(a.one_minus_beta2) * clip;
+    k.m_value = a.beta1 / kM2;
+    k.s_value = sqrtf(a.beta2) / kS2;
     int t = row_of(a.rows, a.n, c, lane);
     Row r = a.rows[t];
     for (; c < c1; ++c) {
         while (t + 1 < a.n && a.rows[t + 1].chunk0 <= c) r = a.rows[++t];
-        const int64_t n = r.numel, base = (c - r.chunk0) * kChunk + wave * kBlock + lane * 4;
-        const bool vec = whole(r.param, r.param16) && whole(r.grad, r.grad16) && (((uintptr_t)r.m | (uintptr_t)r.v) & (EIGHT ? 3 : 15)) == 0;
-#pragma unroll 1
-        for (int u = 0; u < 4; ++u) {
-            const int64_t i = base + u * (kThreads * 4);
-            if (i - lane * 4 >= n) break;                       // (the whole wave's piece lies behind the end)
-            f32x4 p = load4(r.param16, r.param, i, n, vec);
-            const f32x4 g = load4(r.grad16, r.grad, i, n, vec) * clip;
-            f32x4 m, v;
-            const int64_t blk = i >> 8;
-            if constexpr (EIGHT) {
-                const uint32_t mc = load4_codes(r.m, i, n, vec), vc = load4_codes(r.v, i, n, vec);
-                const float ms = r.m_scale[blk], vs = r.v_scale[blk];
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    m[k] = m_value((int)(int8_t)(mc >> (8 * k)), ms);
-                    const float s = s_value((vc >> (8 * k)) & 0xffu, vs);
-                    v[k] = s * s;
-                }
-            } else {
-                m = load4<false>(r.m, i, n, vec);
-                v = load4<false>(r.v, i, n, vec);
-            }
-            f32x4 s;
-#pragma unroll
-            for (int k = 0; k < 4; ++k) {
-                m[k] = a.beta1 * m[k] + a.one_minus_beta1 * g[k];
-                v[k] = a.beta2 * v[k] + a.one_minus_beta2 * (g[k] * g[k]);
-                s[k] = sqrtf(v[k]);
-                p[k] = p[k] - p[k] * decay - m[k] * r.first / (s[k] * r.root + a.eps);
-            }
-            if (r.param16) store4<true>(r.param, i, n, vec, p);
-            else store4<false>(r.param, i, n, vec, p);
-            if constexpr (EIGHT) {
-                uint32_t mb = 0, sb = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    mb = max(mb, bits_abs(m[k]));
-                    sb = max(sb, bits_abs(s[k]));
-                }
-                const float ms = __uint_as_float(wave_max_bits(mb)), ss = __uint_as_float(wave_max_bits(sb));
-                const float mi = reciprocal_or_0(ms), si = reciprocal_or_0(ss);
-                uint32_t mc = 0, sc = 0;
-#pragma unroll
-                for (int k = 0; k < 4; ++k) {
-                    mc |= ((uint32_t)m_code(m[k], mi) & 0xffu) << (8 * k);
-                    sc |= s_code(s[k], si) << (8 * k);
-                }
-                store4_codes(r.m, i, n, vec, mc);
-                store4_codes(r.v, i, n, vec, sc);
-                if (lane == 0) {
-                    r.m_scale[blk] = ms;
-                    r.v_scale[blk] = ss;
-                }
-            } else {
-                store4<false>(r.m, i, n, vec, m);
-                store4<false>(r.v, i, n, vec, v);
-            }
-        }
+        const int64_t at = (c - r.chunk0) * kChunk;
+        const bool whole = at + kChunk <= r.numel && whole4(r.param, r.param16) && whole4(r.grad, r.grad16) &&
+                           (((uintptr_t)r.m | (uintptr_t)r.v) & (EIGHT ? 3 : 15)) == 0;
+        const int64_t base = at + wave * kBlock;
+        if (!whole) step_chunk<EIGHT, false, false, false>(a, r, base, lane, k);
+        else if (r.param16) r.grad16 ? step_chunk<EIGHT, true, true, true>(a, r, base, lane, k) : step_chunk<EIGHT, true, true, false>(a, r, base, lane, k);
+        else r.grad16 ? step_chunk<EIGHT, true, false, true>(a, r, base, lane, k) : step_chunk<EIGHT, true, false, false>(a, r, base, lane, k);
     }
 }
 
@@ -280,10 +341,18 @@ __global__ void __launch_bounds__(kThreads) grad_norm_kernel(const Row* rows, in
         for (; c < c1; ++c) {
             while (t + 1 < n_rows && rows[t + 1].chunk0 <= c) r = rows[++t];
             const int64_t base = (c - r.chunk0) * kChunk + wave * kBlock + lane * 4;
-            const bool vec = whole(r.grad, r.grad16);
             f32x4 g[4];
+            const bool whole = (c - r.chunk0 + 1) * kChunk <= r.numel && whole4(r.grad, r.grad16);
+            if (whole && r.grad16) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) g[u] = load4(r.grad16, r.grad, base + u * (kThreads * 4), r.numel, vec);
+                for (int u = 0; u < 4; ++u) g[u] = load4<true>(true, r.grad, base + u * (kThreads * 4), r.numel);
+            } else if (whole) {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) g[u] = load4<true>(false, r.grad, base + u * (kThreads * 4), r.numel);
+            } else {
+#pragma unroll
+                for (int u = 0; u < 4; ++u) g[u] = load4<false>(r.grad16, r.grad, base + u * (kThreads * 4), r.numel);
+            }
 #pragma unroll
             for (int u = 0; u < 4; ++u)
 #pragma unroll
@@ -303,22 +372,28 @@ __global__ void __launch_bounds__(kThreads) grad_norm_finish_kernel(const double
 }
 
 // ---------------------------------------------------------------- what 8-bit states stand for
+template <bool WHOLE>
+__device__ __forceinline__ void values4(const uint8_t* mc, const uint8_t* vc, const float* ms, const float* vs, int64_t i, int64_t n, void* m_out, void* v_out,
+                                        bool out16) {
+    const uint32_t a = load4_codes<WHOLE>(mc, i, n), b = load4_codes<WHOLE>(vc, i, n);
+    const float sm = ms[i >> 8] * (1.0f / kM2), sv = vs[i >> 8] * (1.0f / kS2);
+    f32x4 m, v;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        m[k] = m_value(a, k, sm);
+        const float s = s_value(b, k, sv);
+        v[k] = s * s;
+    }
+    store4<WHOLE>(out16, m_out, i, n, m);
+    store4<WHOLE>(out16, v_out, i, n, v);
+}
 template <bool OUT16>
-__global__ void __launch_bounds__(kThreads) adamw_values_kernel(const uint8_t* mc, const uint8_t* vc, const float* ms, const float* vs,
-                                                                int64_t n, void* m_out, void* v_out, bool vec) {
+__global__ void __launch_bounds__(kThreads) adamw_values_kernel(const uint8_t* mc, const uint8_t* vc, const float* ms, const float* vs, int64_t n, void* m_out,
+                                                                void* v_out, bool vec) {
     const int64_t stride = (int64_t)gridDim.x * kThreads * 4;
     for (int64_t i = ((int64_t)blockIdx.x * kThreads + threadIdx.x) * 4; i < n; i += stride) {
-        const uint32_t a = load4_codes(mc, i, n, vec), b = load4_codes(vc, i, n, vec);
-        const float sm = ms[i >> 8], sv = vs[i >> 8];
-        f32x4 m, v;
-#pragma unroll
-        for (int k = 0; k < 4; ++k) {
-            m[k] = m_value((int)(int8_t)(a >> (8 * k)), sm);
-            const float s = s_value((b >> (8 * k)) & 0xffu, sv);
-            v[k] = s * s;
-        }
-        store4<OUT16>(m_out, i, n, vec, m);
-        store4<OUT16>(v_out, i, n, vec, v);
+        if (vec && i + 4 <= n) values4<true>(mc, vc, ms, vs, i, n, m_out, v_out, OUT16);
+        else values4<false>(mc, vc, ms, vs, i, n, m_out, v_out, OUT16);
     }
 }
 
@@ -359,8 +434,8 @@ void write_table(const xq_adamw_tensor* t, int64_t n, void* workspace, const xq_
         TableArgs a;
         const int k = (int)std::min<int64_t>(kTableArgs, n - at);
         std::copy(t + at, t + at + k, a.t);
-        adamw_table_kernel<<<dim3(1), 64, 0, s>>>(a, TableScalars{(Row*)workspace, chunk0, k, (int32_t)at, o != nullptr, o ? o->lr : 0.0, o ? o->beta1 : 0.0,
-                                                                  o ? o->beta2 : 0.0, o ? o->lr_device : nullptr});
+        adamw_table_kernel<<<dim3(1), 64, 0, s>>>(a, TableScalars{(Row*)workspace, chunk0, k, (int32_t)at, o != nullptr, o ? o->lr : 0.0, o ? log(o->beta1) : 0.0,
+                                                                  o ? log(o->beta2) : 0.0, o ? o->lr_device : nullptr});
         for (int i = 0; i < k; ++i) chunk0 += xq_cdiv(t[at + i].numel, kChunk);
     }
 }

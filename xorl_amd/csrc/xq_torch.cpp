@@ -861,26 +861,28 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         if (!norm_only && !PyArg_ParseTuple(args[7], "ddddd", &o.lr, &o.beta1, &o.beta2, &o.eps, &o.weight_decay)) return nullptr;
         o.state_bits = eight ? 8 : 32;
         std::optional<at::Device> device;
-        auto same_device = [&](const Tensor& a, const std::string& what) {
+        auto same_device = [&](const Tensor& a, auto&& what) {
             if (!device) device = a.device();
-            else if (a.device() != *device) throw ArgError(what + " is on " + a.device().str() + ", others on " + device->str());
+            else if (a.device() != *device) throw ArgError(what() + " is on " + a.device().str() + ", others on " + device->str());
         };
         std::vector<xq_adamw_tensor> q;
-        std::vector<Tensor> keep, written;
+        std::vector<Tensor> keep;
+        std::vector<at::TensorImpl*> written;     // (the lists hold them)
         std::vector<const void*> once;            // what the step writes: named twice it would be written by two blocks at a time
         q.reserve(n);
+        written.reserve(6 * n);
+        once.reserve(6 * n);
         for (Py_ssize_t i = 0; i < n; ++i) {
             const Tensor& gr = g[i];
             xq_adamw_tensor a{};
             a.numel = gr.numel();
             a.grad_dtype = float_code(gr, g, i);
-            same_device(gr, g.at(i));
-            Tensor gc = gr;
+            same_device(gr, [&] { return g.at(i); });
+            a.grad = gr.data_ptr();
             if (!gr.is_contiguous() || gr.is_neg()) {
-                gc = gr.detach().resolve_neg().contiguous();
-                keep.push_back(gc);
+                keep.push_back(gr.detach().resolve_neg().contiguous());
+                a.grad = keep.back().data_ptr();
             }
-            a.grad = gc.data_ptr();
             if (!norm_only) {
                 const Tensor &pt = p[i], &mt = m[i], &vt = v[i], &st = t[i];
                 a.param_dtype = float_code(pt, p, i);
@@ -889,7 +891,7 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                     {pt, p, pt.scalar_type(), a.numel}, {mt, m, eight ? at::kChar : at::kFloat, a.numel},
                     {vt, v, eight ? at::kByte : at::kFloat, a.numel}, {st, t, at::kFloat, 1}};
                 for (const auto& c : all) {
-                    same_device(c.t, c.l.at(i));
+                    same_device(c.t, [&] { return c.l.at(i); });
                     if (c.t.scalar_type() != c.dt) throw ArgError(c.l.at(i) + " must be " + toString(c.dt) + ", got " + toString(c.t.scalar_type()));
                     if (c.t.numel() != c.n) throw ArgError(c.l.at(i) + " holds " + std::to_string(c.t.numel()) + " elements, expected " + std::to_string(c.n));
                     if (!c.t.is_contiguous() || c.t.is_neg()) throw ArgError(c.l.at(i) + " must be contiguous");
@@ -900,19 +902,19 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                     const TensorList* from[] = {&ms, &vs};
                     for (int k = 0; k < 2; ++k) {
                         const Tensor& sc = (*from[k])[i];
-                        same_device(sc, from[k]->at(i));
+                        same_device(sc, [&] { return from[k]->at(i); });
                         if (sc.scalar_type() != at::kFloat || !sc.is_contiguous() || sc.numel() != (a.numel + 255) / 256)
                             throw ArgError(from[k]->at(i) + " must be contiguous fp32 with " + std::to_string((a.numel + 255) / 256) + " element(s)");
                         *to[k] = (float*)sc.data_ptr();
-                        written.push_back(sc);
+                        written.push_back(sc.unsafeGetTensorImpl());
                         if (a.numel) once.push_back(sc.data_ptr());
                     }
                 }
                 for (const Tensor* w : {&pt, &mt, &vt}) {
-                    written.push_back(*w);
+                    written.push_back(w->unsafeGetTensorImpl());
                     if (a.numel) once.push_back(w->data_ptr());
                 }
-                written.push_back(st);
+                written.push_back(st.unsafeGetTensorImpl());
                 once.push_back(st.data_ptr());
             }
             if (a.numel) q.push_back(a);
@@ -923,14 +925,14 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         if (args[8] != Py_None) {
             const Tensor* lr = plain(args[8]);
             if (!lr || lr->scalar_type() != at::kFloat || lr->numel() != 1) throw ArgError("adamw_step: an lr tensor must be one fp32 element on the device");
-            same_device(*lr, "adamw_step: lr");
+            same_device(*lr, [] { return std::string("adamw_step: lr"); });
             o.lr_device = (const float*)lr->data_ptr();
         }
         Tensor norm;
         if (args[10] != Py_None) {
             const Tensor* given = plain(args[10]);
             if (!given || given->scalar_type() != at::kFloat || given->numel() != 1) throw ArgError("adamw_step: grad_norm must be one fp32 element on the device");
-            same_device(*given, "adamw_step: grad_norm");
+            same_device(*given, [] { return std::string("adamw_step: grad_norm"); });
             norm = *given;
             o.norm_given = 1;
         }
@@ -954,8 +956,8 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
             check(norm_only ? xq_grad_norm(q.data(), (int64_t)q.size(), o.norm, ws.get(), ws.bytes, stream)
                             : xq_adamw_step(q.data(), (int64_t)q.size(), &o, ws.get(), ws.bytes, stream));
         }
-        for (const Tensor& w : written)
-            if (!w.is_inference()) w.unsafeGetTensorImpl()->bump_version();
+        for (at::TensorImpl* w : written)
+            if (!w->is_inference()) w->bump_version();
         if (!norm.defined()) Py_RETURN_NONE;
         return THPVariable_Wrap(std::move(norm));
     });
