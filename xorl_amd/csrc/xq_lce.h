@@ -29,7 +29,12 @@ struct LceTile {
     static constexpr int ROWS = 32 * TM, COLS = 256, BK = 32, STAGES = 4;
     static constexpr int A_BYTES = ROWS * 64, B_BYTES = COLS * 64, STAGE_BYTES = A_BYTES + B_BYTES;
     static constexpr int AP = (ROWS / 8 + 15) / 16, BP = 2, NP = AP + BP;        // direct loads of a wave and K-step: 16 rows of 64 bytes each
-    static constexpr int LDS_BYTES = STAGES * STAGE_BYTES;
+    // a block goes on to its next tile, whose first K-steps are on their way while the ends of this one are computed; 64 rows: two blocks
+    // of one tile each share a compute unit instead
+    static constexpr bool AHEAD = TM >= 4;
+    static constexpr int END_BYTES = ROWS * 32 + 1024 * 4;      // of the ends: sums by row and wave; four numbers by row or column
+    static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + (AHEAD ? END_BYTES : 0);
+    static_assert(AHEAD || END_BYTES <= STAGES * STAGE_BYTES, "the ends reuse the stages");
 };
 
 struct LceRows {                        // what is kept of the labels: the rows that count, in order
@@ -53,12 +58,33 @@ struct LceLogitsArgs {
     int64_t rows_pad;
     bf16_t* image;
     int32_t image_steps;                // K-steps of the image's rows
-    const int32_t* redo;                // EXP: row tiles to do again, or NULL
+    int32_t* redo;                      // EXP: row tiles that found a logit too far above its reference
+    int32_t again;                      // do those again, and those only, with the row's largest logit as its reference
+    float* new_ref;                     // of the rows done again, and what their sums so far count by
+    float* alpha;
 };
+constexpr float kLceFar = 64.0f;        // log2
 
-// C[r, n] over the tile's K-steps; issue(kt, part, dst): one of NP direct loads of K-step kt
-template <int TM, bool BT, typename Issue>
-__device__ __forceinline__ void lce_core(f32x4 (&acc)[TM][4], unsigned char* dsm, int nk, int wave, int lane, Issue issue) {
+// The first three of a stream of K-steps: K-step k of it goes to stage k & 3.  issue(at, part, stage): one of NP direct loads of a K-step.
+template <int TM, typename Advance, typename Issue>
+__device__ __forceinline__ void lce_begin(unsigned char* dsm, Advance advance, Issue issue) {
+    using T = LceTile<TM>;
+    const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)dsm;
+#pragma unroll
+    for (int kt = 0; kt < 3; ++kt) {
+        const int at = advance(kt);
+#pragma unroll
+        for (int part = 0; part < T::NP; ++part) issue(at, part, lds0 + kt * T::STAGE_BYTES);
+    }
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(T::NP) : "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+}
+
+// C[r, n] over the stream's K-steps first .. first + nk - 1 (an even number, not 0), the first two of which have landed; the same holds of the
+// two behind them in the end.  advance(k): what issue is to be told for the tile's K-step k, which goes on behind the last.
+template <int TM, bool BT, typename Advance, typename Issue>
+__device__ __forceinline__ void lce_run(f32x4 (&acc)[TM][4], unsigned char* dsm, int first, int nk, int wave, int lane, Advance advance, Issue issue) {
     using T = LceTile<TM>;
     constexpr int NC = TM, LA = NC < 3 ? NC : 3, FB = NC < 4 ? 4 / NC : 1;
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
@@ -91,27 +117,21 @@ __device__ __forceinline__ void lce_core(f32x4 (&acc)[TM][4], unsigned char* dsm
     for (int i = 0; i < TM; ++i)
 #pragma unroll
         for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    if (nk <= 0) return;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)dsm;
-#pragma unroll
-    for (int kt = 0; kt < 3; ++kt)
-#pragma unroll
-        for (int part = 0; part < T::NP; ++part) issue(min(kt, nk - 1), part, lds0 + kt * T::STAGE_BYTES);
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(T::NP) : "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-
     bf16x8 fa[4], fb[2][4];
+    {
+        const unsigned char* stage = dsm + (first & 3) * T::STAGE_BYTES;
 #pragma unroll
-    for (int j = 0; j < 4; ++j) fb[0][j] = read_b(dsm, j);
+        for (int j = 0; j < 4; ++j) fb[0][j] = read_b(stage, j);
 #pragma unroll
-    for (int c = 0; c < LA; ++c) fa[c] = read_a(dsm, c);
+        for (int c = 0; c < LA; ++c) fa[c] = read_a(stage, c);
+    }
     auto iteration = [&](int kt, auto P_) {
         constexpr int P = decltype(P_)::value;
-        const unsigned char* here = dsm + (kt & 3) * T::STAGE_BYTES;
-        const unsigned char* next = dsm + ((kt + 1) & 3) * T::STAGE_BYTES;
-        const uint32_t fill = lds0 + ((kt + 3) & 3) * T::STAGE_BYTES;
-        const int kf = min(kt + 3, nk - 1);
+        const unsigned char* here = dsm + ((first + kt) & 3) * T::STAGE_BYTES;
+        const unsigned char* next = dsm + ((first + kt + 1) & 3) * T::STAGE_BYTES;
+        const uint32_t fill = lds0 + ((first + kt + 3) & 3) * T::STAGE_BYTES;
+        const int ahead = advance(kt + 3);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int at = (P * NC + c) & 3;
@@ -122,181 +142,293 @@ __device__ __forceinline__ void lce_core(f32x4 (&acc)[TM][4], unsigned char* dsm
             for (int q = 0; q < FB; ++q)
                 if (c * FB + q < 4) fb[P ^ 1][c * FB + q] = read_b(next, c * FB + q);
 #pragma unroll
-            for (int part = c * T::NP / NC; part < (c + 1) * T::NP / NC; ++part) issue(kf, part, fill);
+            for (int part = c * T::NP / NC; part < (c + 1) * T::NP / NC; ++part) issue(ahead, part, fill);
             __builtin_amdgcn_sched_barrier(0);
         }
+        // K-step kt + 2 has landed
         asm volatile("s_waitcnt vmcnt(%0)" :: "n"(T::NP) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
     };
-    int kt = 0;
-    for (; kt + 1 < nk; kt += 2) {
+    // (one loop and one exit: with several the sums met with no register to spare)
+    for (int kt = 0; kt < nk; kt += 2) {
         iteration(kt, std::integral_constant<int, 0>{});
         iteration(kt + 1, std::integral_constant<int, 1>{});
     }
-    if (kt < nk) iteration(kt, std::integral_constant<int, 0>{});
-    // nothing is on its way into LDS, and nobody reads it, from here on
-    asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
 }
+// before LDS is used for something else, or given back
+__device__ __forceinline__ void lce_loads_done() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 __device__ __forceinline__ void lce_load_lds(uint32_t dst, const void* src) {
-    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(dst), "v"(src) : "memory");
+    asm volatile("s_mov_b32 m0, %0\n\ts_nop 0\n\tglobal_load_lds_dwordx4 %1, off" :: "s"(__builtin_amdgcn_readfirstlane(dst)), "v"(src) : "memory");
 }
 
-// blocks to tiles: neighbours in time on one XCD share rows of A and B; blocks behind the last tile have none
-__device__ __forceinline__ bool lce_tile(int tiles_a, int tiles_b, int* ta, int* tb) {
-    const int nb = tiles_a * tiles_b, b = blockIdx.x, per = nb >> 3;
-    if (b >= nb) return false;
-    const int logical = b < per * 8 ? (b & 7) * per + (b >> 3) : b;
+// What a block works on.  XCD x (blocks are dealt to the eight of them in turn) has an eighth of the tiles, in order; its blocks take them one
+// after the other, so that what it works on at a time shares rows of A (4 tiles) and of B (8).
+struct LceWalk {
+    int at, end, step;
+    __device__ LceWalk(int tiles) {
+        const int x = blockIdx.x & 7, slots = gridDim.x >> 3;
+        if (gridDim.x & 7) {                    // (fewer than eight, or an odd number: in turn)
+            at = blockIdx.x; end = tiles; step = gridDim.x;
+        } else {
+            const int first = (int)((int64_t)tiles * x >> 3);
+            at = first + (int)(blockIdx.x >> 3); end = (int)((int64_t)tiles * (x + 1) >> 3); step = slots;
+        }
+    }
+    __device__ bool more() const { return at < end; }
+};
+__device__ __forceinline__ void lce_tile(int logical, int tiles_a, int tiles_b, int* ta, int* tb) {
     constexpr int GM = 4;
     const int width = GM * tiles_b, grp = logical / width, first = grp * GM, gsz = min(tiles_a - first, GM), in = logical - grp * width;
     *ta = first + in % gsz;
     *tb = in / gsz;
-    return true;
+}
+
+// (as fmaxf twice it is four instructions: the compiler makes its arguments quiet first)
+__device__ __forceinline__ float max3(float a, float b, float c) {
+    float r;
+    asm("v_max3_f32 %0, %1, %2, %3" : "=v"(r) : "v"(a), "v"(b), "v"(c));
+    return r;
+}
+__device__ __forceinline__ float over_groups_max(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return fmaxf(__uint_as_float(b[0]), __uint_as_float(b[1]));
+}
+__device__ __forceinline__ float over_groups_sum(float v) {
+    const auto a = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    v = __uint_as_float(a[0]) + __uint_as_float(a[1]);
+    const auto b = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
 template <int TM, int MODE>
 __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLogitsArgs g) {
     using T = LceTile<TM>;
     extern __shared__ __attribute__((aligned(16))) unsigned char dsm[];
+    unsigned char* const ends = T::AHEAD ? dsm + T::STAGES * T::STAGE_BYTES : dsm;
+    f32x2* const sums = (f32x2*)ends;                       // [row][wave column]
+    float* const info = (float*)(ends + T::ROWS * 32);      // EXP, STATS: label and reference by row;  GRAD: label, lse, up, rest by column
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
-    const int count = *g.rows.count;
+    const int count = __builtin_amdgcn_readfirstlane(*g.rows.count);
     const int n_a = MODE == kLceGrad ? g.n_v : count, n_b = MODE == kLceGrad ? count : g.n_v;
-    int ta, tb;
-    if (!lce_tile((n_a + T::ROWS - 1) / T::ROWS, (n_b + 255) >> 8, &ta, &tb)) return;
-    if (MODE == kLceExp && g.redo && !g.redo[ta]) return;
-    const int r0 = ta * T::ROWS, c0 = tb * 256;
+    const int tiles_a = (n_a + T::ROWS - 1) / T::ROWS, tiles_b = (n_b + 255) >> 8, nk = g.H / T::BK;
 
-    // ---- sources of the direct loads: a wave brings in an eighth of either side's rows, 64 bytes of each, 16 rows to a load
-    const bf16_t* src[T::NP];
+    LceWalk walk(tiles_a * tiles_b);
+    int ta, tb;
+    auto find = [&]() -> bool {                             // the block's next tile
+        for (; walk.more(); walk.at += walk.step) {
+            lce_tile(walk.at, tiles_a, tiles_b, &ta, &tb);
+            if (MODE != kLceExp || !g.again || __builtin_amdgcn_readfirstlane(g.redo[ta])) return true;
+        }
+        return false;
+    };
+    // ---- sources of the direct loads: a wave brings in an eighth of either side's rows, 64 bytes of each, 16 rows to a load; and what
+    // the ends want to know of the rows (EXP, STATS) or columns (GRAD) that are tokens
+    constexpr int N_INFO = MODE == kLceGrad ? 256 : T::ROWS;
+    auto sources = [&](const bf16_t* (&src)[T::NP], float (&about)[4]) {
 #pragma unroll
-    for (int p = 0; p < T::NP; ++p) {
-        const bool of_a = p < T::AP;
-        const int rt = of_a ? wave * (T::ROWS / 8) + p * 16 + (lane >> 2) : wave * 32 + (p - T::AP) * 16 + (lane >> 2);
-        const int n = min(of_a ? r0 + rt : c0 + rt, (of_a ? n_a : n_b) - 1);
-        const bool tokens = of_a != (MODE == kLceGrad);
-        const int64_t row = tokens ? g.rows.row[n] : g.first_v + n;
-        src[p] = (of_a ? g.A + row * g.lda : g.B + row * g.ldb) + (((lane & 3) ^ ((rt >> 2) & 2)) << 3);
-    }
-    f32x4 acc[TM][4];
-    lce_core<TM, false>(acc, dsm, g.H / T::BK, wave, lane, [&](int kt, int part, uint32_t stage) {
+        for (int p = 0; p < T::NP; ++p) {
+            const bool of_a = p < T::AP;
+            const int rt = of_a ? wave * (T::ROWS / 8) + p * 16 + (lane >> 2) : wave * 32 + (p - T::AP) * 16 + (lane >> 2);
+            const int n = min((of_a ? ta * T::ROWS : tb * 256) + rt, (of_a ? n_a : n_b) - 1);
+            const bool tokens = of_a != (MODE == kLceGrad);
+            const int64_t row = tokens ? g.rows.row[n] : g.first_v + n;
+            src[p] = (of_a ? g.A + row * g.lda : g.B + row * g.ldb) + (((lane & 3) ^ ((rt >> 2) & 2)) << 3);
+        }
+        if (tid < N_INFO) {
+            // (GRAD: the arrays are as long as whole tiles; behind the last row up = 0, lse = inf)
+            const int r = MODE == kLceGrad ? tb * 256 + tid : min(ta * T::ROWS + tid, count - 1);
+            about[0] = __int_as_float(g.rows.label[r] - g.first_v);
+            if (MODE != kLceStats) about[1] = g.ref[r];
+            if (MODE == kLceGrad) { about[2] = g.grad[r]; about[3] = g.rest[r]; }
+            if (MODE == kLceExp && g.again) {
+                // done again: the largest logit of the row's tiles is its reference, where that is far from the one it had
+                float top = -INFINITY;
+                for (int t = 0; t < tiles_b; ++t) top = fmaxf(top, g.part[(int64_t)t * g.rows_pad + r][0]);
+                const float old = about[1];
+                const bool far = top - old > kLceFar;
+                if (far) about[1] = top;
+                if (tb == 0 && ta * T::ROWS + tid < count) {
+                    g.new_ref[r] = about[1];
+                    g.alpha[r] = far ? __builtin_amdgcn_exp2f(old - top) : 1.0f;
+                }
+            }
+        }
+    };
+    auto note = [&](const float (&about)[4]) {
+        if (tid < N_INFO) {
+            info[tid] = about[0];
+            if (MODE != kLceStats) info[N_INFO + tid] = about[1];
+            if (MODE == kLceGrad) { info[512 + tid] = about[2]; info[768 + tid] = about[3]; }
+        }
+    };
+    const bf16_t* src[T::NP];
+    const bf16_t* src_next[T::NP];
+    auto issue = [&](int at, int part, uint32_t stage) {
         const bool of_a = part < T::AP;
         const int p = of_a ? part : part - T::AP, rows = of_a ? T::ROWS / 8 : 32;
         const uint32_t dst = stage + (of_a ? 0 : T::A_BYTES) + wave * rows * 64 + p * 1024;
-        if (p * 16 + 16 <= rows || lane < (rows - p * 16) * 4) lce_load_lds(dst, src[part] + kt * T::BK);
-    });
+        if (p * 16 + 16 <= rows || lane < (rows - p * 16) * 4) lce_load_lds(dst, src[part] + at * T::BK);
+    };
+    float about[4];
+    bool more = false;
+    // (behind the tile's last K-step: the next tile's; without one, this one's again, for nothing)
+    auto advance = [&](int kt) -> int {
+        if (kt == nk && more) {
+#pragma unroll
+            for (int p = 0; p < T::NP; ++p) src[p] = src_next[p];
+        }
+        return kt < nk ? kt : kt - nk < nk ? kt - nk : 0;
+    };
+    if (!find()) return;
+    const bool stream = T::AHEAD && nk >= 4;                // (two K-steps: a tile's end is nearer than the loads are ahead)
+    sources(src, about);
+    lce_begin<TM>(dsm, advance, issue);
+    if (T::AHEAD) note(about);
+    int first = 0;
+    do {
+        const int r0 = ta * T::ROWS, c0 = tb * 256, this_a = ta, this_b = tb;
+        if (stream) {
+            walk.at += walk.step;
+            more = find();
+            if (more) sources(src_next, about);
+        }
+        f32x4 acc[TM][4];
+        lce_run<TM, false>(acc, dsm, first, nk, wave, lane, advance, issue);
+        first += nk;
+        if (!stream) {
+            lce_loads_done();
+            __syncthreads();
+            if (!T::AHEAD) note(about);
+            __syncthreads();
+        }
 
-    // ---- lane (l16, lg) holds rows r0 + wm 16 TM + 16 i + l16, columns c0 + 64 wn + 16 j + 4 lg + 0..3
-    const int row_w = wm * 16 * TM + l16, col_w = wn * 64 + 4 * lg;
-    if constexpr (MODE == kLceGrad) {
-        f32x4 lse[4], up[4], rest[4];
-        int label[4][4];
+        // ---- lane (l16, lg) holds rows r0 + wm 16 TM + 16 i + l16, columns c0 + 64 wn + 16 j + 4 lg + 0..3
+        const int row_w = wm * 16 * TM + l16, col_w = wn * 64 + 4 * lg;
+        if constexpr (MODE == kLceGrad) {
 #pragma unroll
-        for (int j = 0; j < 4; ++j) {               // (the arrays are as long as whole tiles: behind the last row up = 0, lse = inf)
-            const int c = c0 + col_w + 16 * j;
-            lse[j] = *(const f32x4*)(g.ref + c);
-            up[j] = *(const f32x4*)(g.grad + c);
-            rest[j] = *(const f32x4*)(g.rest + c);
+            for (int j = 0; j < 4; ++j) {
+                const int c = col_w + 16 * j;
+                const f32x4 label = *(const f32x4*)(info + c), lse = *(const f32x4*)(info + 256 + c), up = *(const f32x4*)(info + 512 + c), rest = *(const f32x4*)(info + 768 + c);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) label[j][e] = g.rows.label[c + e];
-        }
+                for (int i = 0; i < TM; ++i) {
+                    const int v = r0 + row_w + 16 * i;
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int v = g.first_v + r0 + row_w + 16 * i;
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], g.scale2, -lse[j][e]));
-                    acc[i][j][e] = up[j][e] * (label[j][e] == v ? -rest[j][e] : p);
+                    for (int e = 0; e < 4; ++e) {
+                        const float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], g.scale2, -lse[e]));
+                        acc[i][j][e] = up[e] * (__float_as_int(label[e]) == v ? -rest[e] : p);
+                    }
                 }
-        }
-    } else {
-        // columns that the piece does not have, and the label's, count as -inf
-        const bool tail = c0 + 256 > g.n_v;
-        float ref[TM];
-        int at[TM];                                     // the label's column in the tile, by the lane's own numbering of its 16
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int r = min(r0 + row_w + 16 * i, count - 1);
-            at[i] = g.rows.label[r] - g.first_v - c0 - col_w;
-            if (MODE == kLceExp) ref[i] = g.ref[r];
-        }
-        f32x2* lds = (f32x2*)dsm;                       // [row][wave column]
-#pragma unroll
-        for (int i = 0; i < TM; ++i) {
-#pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) acc[i][j][e] *= g.scale2;
-            if (__any(at[i] >= 0 && at[i] < 52)) {
-#pragma unroll
-                for (int j = 0; j < 4; ++j)
-#pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (at[i] == 16 * j + e) {
-                            if (MODE == kLceStats && r0 + row_w + 16 * i < count) g.at_label[r0 + row_w + 16 * i] = acc[i][j][e];
-                            acc[i][j][e] = -INFINITY;
-                        }
             }
-            if (tail) {
+        } else {
+            // columns that the piece does not have, and the label's, count as -inf
+            if (c0 + 256 > g.n_v) {
 #pragma unroll
-                for (int j = 0; j < 4; ++j)
+                for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int e = 0; e < 4; ++e)
-                        if (c0 + col_w + 16 * j + e >= g.n_v) acc[i][j][e] = -INFINITY;
+                    for (int j = 0; j < 4; ++j)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e)
+                            if (c0 + col_w + 16 * j + e >= g.n_v) acc[i][j][e] = -INFINITY;
             }
-            float top = -INFINITY, sum = 0.0f;
+            float ref[TM], top[TM], sum[TM];
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
+            for (int i = 0; i < TM; ++i) {
+                const int at = __float_as_int(info[row_w + 16 * i]) - c0 - col_w;     // the label's column by the lane's own numbering of its 16
+                if (MODE == kLceExp) ref[i] = info[N_INFO + row_w + 16 * i];
+                if (__any(at >= 0 && at < 52)) {
 #pragma unroll
-                for (int e = 0; e < 4; ++e) top = fmaxf(top, acc[i][j][e]);
-            top = fmaxf(top, __shfl_xor(top, 16));
-            top = fmaxf(top, __shfl_xor(top, 32));
-            const float base = MODE == kLceExp ? ref[i] : (top == -INFINITY ? 0.0f : top);
+                    for (int j = 0; j < 4; ++j)
 #pragma unroll
-            for (int j = 0; j < 4; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e) {
-                    const float x = __builtin_amdgcn_exp2f(acc[i][j][e] - base);
-                    if (MODE == kLceExp) acc[i][j][e] = x;
-                    sum += x;
+                        for (int e = 0; e < 4; ++e)
+                            if (at == 16 * j + e) {
+                                if (MODE == kLceStats && r0 + row_w + 16 * i < count) g.at_label[r0 + row_w + 16 * i] = acc[i][j][e] * g.scale2;
+                                acc[i][j][e] = -INFINITY;
+                            }
                 }
-            sum += __shfl_xor(sum, 16);
-            sum += __shfl_xor(sum, 32);
-            if (lg == 0) lds[(row_w + 16 * i) * 4 + wn] = f32x2{top, sum};
-        }
-        __syncthreads();
-        if (tid < T::ROWS && r0 + tid < count) {
-            f32x2 a = lds[tid * 4], b;
-#pragma unroll
-            for (int w = 1; w < 4; ++w) {
-                b = lds[tid * 4 + w];
-                const float top = fmaxf(a[0], b[0]);
-                if (MODE == kLceExp) a[1] += b[1];
-                else if (top != -INFINITY) a[1] = a[1] * __builtin_amdgcn_exp2f(a[0] - top) + b[1] * __builtin_amdgcn_exp2f(b[0] - top);
-                a[0] = top;
             }
-            g.part[(int64_t)tb * g.rows_pad + r0 + tid] = a;
-        }
-    }
-    if constexpr (MODE != kLceStats) {
-        bf16_t* out = g.image + ((int64_t)ta * g.image_steps + (c0 >> 5) + wn * 2) * (T::ROWS * 32);
 #pragma unroll
-        for (int i = 0; i < TM; ++i) {
-            const int row = row_w + 16 * i;
+            for (int i = 0; i < TM; ++i) {
+                top[i] = acc[i][0][0];
 #pragma unroll
-            for (int q = 0; q < 2; ++q) {
-                const f32x4 a = acc[i][2 * q], b = acc[i][2 * q + 1];
-                *(u32x4*)(out + (q * T::ROWS + row) * 32 + ((lg ^ ((row >> 2) & 2)) << 3)) =
-                    u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
+                for (int j = 0; j < 4; ++j) top[i] = max3(max3(top[i], acc[i][j][0], acc[i][j][1]), acc[i][j][2], acc[i][j][3]);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) top[i] = over_groups_max(top[i]) * g.scale2;
+            bool far = false;
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const float base = MODE == kLceExp ? ref[i] : (top[i] == -INFINITY ? 0.0f : top[i]);
+                if (MODE == kLceExp) far |= top[i] - base > kLceFar;
+                f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int j = 0; j < 4; ++j) {
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], g.scale2, -base));
+                    s += acc[i][j];
+                }
+                sum[i] = (s[0] + s[1]) + (s[2] + s[3]);
+            }
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                sum[i] = over_groups_sum(sum[i]);
+                if (lg == 0) sums[(row_w + 16 * i) * 4 + wn] = f32x2{top[i], sum[i]};
+            }
+            if (MODE == kLceExp && !g.again && __any(far)) {
+                if (lane == 0) g.redo[this_a] = 1;          // (several may say so, all the same)
+            }
+            __syncthreads();
+            if (tid < T::ROWS && r0 + tid < count) {
+                f32x2 a = sums[tid * 4], b;
+#pragma unroll
+                for (int w = 1; w < 4; ++w) {
+                    b = sums[tid * 4 + w];
+                    const float most = fmaxf(a[0], b[0]);
+                    if (MODE == kLceExp) a[1] += b[1];
+                    else if (most != -INFINITY) a[1] = a[1] * __builtin_amdgcn_exp2f(a[0] - most) + b[1] * __builtin_amdgcn_exp2f(b[0] - most);
+                    a[0] = most;
+                }
+                // (done again: the largest stays what it was, the other tiles' blocks read it)
+                if (MODE == kLceExp && g.again) g.part[(int64_t)this_b * g.rows_pad + r0 + tid][1] = a[1];
+                else g.part[(int64_t)this_b * g.rows_pad + r0 + tid] = a;
             }
         }
-    }
+        if constexpr (MODE != kLceStats) {
+            bf16_t* out = g.image + ((int64_t)this_a * g.image_steps + (c0 >> 5) + wn * 2) * (T::ROWS * 32);
+#pragma unroll
+            for (int i = 0; i < TM; ++i) {
+                const int row = row_w + 16 * i;
+#pragma unroll
+                for (int q = 0; q < 2; ++q) {
+                    const f32x4 a = acc[i][2 * q], b = acc[i][2 * q + 1];
+                    *(u32x4*)(out + (q * T::ROWS + row) * 32 + ((lg ^ ((row >> 2) & 2)) << 3)) =
+                        u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
+                }
+            }
+            if (MODE == kLceGrad) __syncthreads();          // (what the ends read of the columns is written anew)
+        }
+        if (stream) {
+            if (more) note(about);
+        } else if (T::AHEAD) {
+            walk.at += walk.step;
+            if (find()) {
+                sources(src, about);
+                __syncthreads();
+                lce_begin<TM>(dsm, advance, issue);
+                note(about);
+                __syncthreads();
+                first = 0;
+                continue;
+            }
+        }
+        if (!more) break;
+    } while (true);
+    lce_loads_done();
 }
 
 struct LceProductArgs {
@@ -306,14 +438,29 @@ struct LceProductArgs {
     const int32_t* count;
     const bf16_t* B;                    // [k, H]
     int64_t ldb;
-    int32_t H, splits;
-    float* out;                         // [split][rows_pad][H]: sums, added to what is there where `add`, that times alpha[row]
-    int64_t split_stride;
-    const float* alpha;
+    int32_t H, cus;                     // cus: compute units to divide the contraction for, or 0: it is not divided
+    float* out;                         // [part of the contraction][row][H]: sums, added to what is there where `add`, that times alpha[row]
+    const float* alpha;                 // (of row tiles that were done again; 1 otherwise)
+    const int32_t* redo;
     int32_t add;
     bf16_t* out16;                      // or [rows, ld16] bf16
     int64_t ld16;
 };
+
+// Parts of a contraction of E . W: as many as leave the least of the chip idle, where tiles alone would (a part costs its sums once more in
+// memory: 2 % a part).  The rows that count are known on the device only, so that every kernel works it out for itself.  Divided, tiles and
+// parts are three rounds of the chip at most, which bounds the sums.
+constexpr int kLceSplitRounds = 3;
+__host__ __device__ inline int lce_parts(int tiles, int steps, int cus) {
+    int best = 1;
+    float least = 1e30f;
+    for (int s = 1; s <= 32; ++s) {
+        if (s > 1 && (tiles * s > kLceSplitRounds * cus || steps < 16 * s)) break;
+        const float cost = (float)((tiles * s + cus - 1) / cus) / (float)s * (1.0f + 0.02f * (float)(s - 1));
+        if (cost < 0.999f * least) { least = cost; best = s; }
+    }
+    return best;
+}
 
 template <int TM>
 __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LceProductArgs g) {
@@ -322,10 +469,16 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
     const int rows = g.rows < 0 ? *g.count : g.rows, k = g.k < 0 ? *g.count : g.k;
+    const int tiles_a = (rows + T::ROWS - 1) / T::ROWS, tiles_b = (g.H + 255) >> 8, tiles = tiles_a * tiles_b, pairs = (k + 63) >> 6;        // of K-steps
+    const int parts = g.cus ? lce_parts(tiles, g.image_steps, g.cus) : 1;
+    // an XCD has an eighth of all tiles and parts, in order of the parts: what it reads of E and W at a time are few rows and the same K-steps
+    const int all = tiles * parts, b = blockIdx.x, per = all >> 3;
+    if (b >= all) return;
+    const int logical = b < per * 8 ? (b & 7) * per + (b >> 3) : b, s = logical / tiles;
     int ta, tb;
-    if (!lce_tile((rows + T::ROWS - 1) / T::ROWS, (g.H + 255) >> 8, &ta, &tb)) return;
-    const int r0 = ta * T::ROWS, c0 = tb * 256, s = blockIdx.y;
-    const int steps = (k + 31) >> 5, kt0 = (int)((int64_t)steps * s / g.splits), nk = (int)((int64_t)steps * (s + 1) / g.splits) - kt0;
+    lce_tile(logical - s * tiles, tiles_a, tiles_b, &ta, &tb);
+    const int r0 = ta * T::ROWS, c0 = tb * 256;
+    const int kt0 = 2 * (int)((int64_t)pairs * s / parts), nk = 2 * (int)((int64_t)pairs * (s + 1) / parts) - kt0;
 
     const bf16_t* const a_src = g.image + ((int64_t)ta * g.image_steps + kt0) * (T::ROWS * 32) + wave * (T::ROWS / 8) * 32 + lane * 8;
     const int kr = wave * 4 + (lane >> 5);             // of a K-step's rows, two more with the second load
@@ -335,8 +488,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
         const int unit = ((lane & 31) >> 1) ^ ((kr + 2 * p) & 7);
         b_col[p] = g.B + min(c0 + unit * 16 + (lane & 1) * 8, g.H - 8);
     }
-    f32x4 acc[TM][4];
-    lce_core<TM, true>(acc, dsm, nk, wave, lane, [&](int kt, int part, uint32_t stage) {
+    auto issue = [&](int kt, int part, uint32_t stage) {
         if (part < T::AP) {
             constexpr int rows8 = T::ROWS / 8;
             if (part * 16 + 16 <= rows8 || lane < (rows8 - part * 16) * 4)
@@ -346,14 +498,27 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
             const int row = min((kt0 + kt) * 32 + kr + 2 * p, k - 1);
             lce_load_lds(stage + T::A_BYTES + wave * 2048 + p * 1024, b_col[p] + row * g.ldb);
         }
-    });
+    };
+    f32x4 acc[TM][4];
+    if (nk > 0) {
+        auto advance = [&](int kt) { return min(kt, nk - 1); };         // (behind the last K-step: that one again, for nothing)
+        lce_begin<TM>(dsm, advance, issue);
+        lce_run<TM, true>(acc, dsm, 0, nk, wave, lane, advance, issue);
+        lce_loads_done();
+    } else {
+#pragma unroll
+        for (int i = 0; i < TM; ++i)
+#pragma unroll
+            for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    }
 
     const int row_w = wm * 16 * TM + l16, col_w = c0 + wn * 64 + 4 * lg;
+    float* const out = g.out + (int64_t)s * rows * g.H;
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
         const int row = r0 + row_w + 16 * i;
         if (row >= rows) continue;
-        const float alpha = g.add ? g.alpha[row] : 0.0f;
+        const float alpha = g.add && g.redo[ta] ? g.alpha[row] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
             const int col = col_w + 16 * j;
@@ -361,7 +526,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
             if (g.out16) {
                 *(u32x2*)(g.out16 + row * g.ld16 + col) = u32x2{pack_bf16x2(acc[i][j][0], acc[i][j][1]), pack_bf16x2(acc[i][j][2], acc[i][j][3])};
             } else {
-                f32x4* o = (f32x4*)(g.out + s * g.split_stride + (int64_t)row * g.H + col);
+                f32x4* o = (f32x4*)(out + (int64_t)row * g.H + col);
                 *o = g.add ? *o * alpha + acc[i][j] : acc[i][j];
             }
         }

@@ -19,6 +19,7 @@
 //  * A trained head: the backward forms the logits again with the roles exchanged, G = g (p - [v = t]) as bf16 with the tokens along the
 //    contraction, and multiplies it with the rows that count.
 #include <algorithm>
+#include <atomic>
 
 #include "xq_lce.h"
 
@@ -27,7 +28,7 @@ namespace {
 
 constexpr int64_t kPieceBytes = 1ll << 30;          // of E or G at a time
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-constexpr float kFar = 64.0f;                       // a logit this far (log2) above its reference: the piece is done again
+constexpr int kBeginRows = 1024;                    // rows whose labels every block of a launch looks through by itself
 
 inline int64_t up256(int64_t n) { return (n + 255) & ~255ll; }
 
@@ -37,136 +38,183 @@ struct Prep {
     int32_t label_bytes;
     int64_t M, M_pad, V, ignore;
     int32_t *count, *row, *label, *place;           // place: of a row of x among those that count, or -1
-    float* at_label;
+    float* at_label;                                // NaN until the scores' tiles find it; or NULL
+    int32_t* redo;                                  // flags to clear
+    int32_t n_redo;
+    float* loss_out;                                // losses by row, 0 for those that do not count; or NULL
 };
-
-__global__ void __launch_bounds__(1024) lce_prepare_kernel(Prep a) {
-    __shared__ int wave_n[16], base_s;
+__device__ __forceinline__ int64_t label_of(const Prep& a, int64_t i) {
+    if (i >= a.M) return a.ignore;
+    return a.label_bytes == 8 ? ((const int64_t*)a.labels)[i] : (int64_t)((const int32_t*)a.labels)[i];
+}
+// a thread's label among 1024: whether it counts, and how many before it do; all: how many of the 1024
+__device__ __forceinline__ bool place_of(bool in, int* before, int* all, int* wave_n) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    if (threadIdx.x == 0) base_s = 0;
+    const uint64_t mask = __ballot(in);
     __syncthreads();
-    for (int64_t at = 0; at < a.M; at += 1024) {
-        const int64_t i = at + threadIdx.x;
-        int64_t label = a.ignore;
-        if (i < a.M) label = a.label_bytes == 8 ? ((const int64_t*)a.labels)[i] : (int64_t)((const int32_t*)a.labels)[i];
-        const bool in = i < a.M && label != a.ignore;
-        const uint64_t mask = __ballot(in);
-        if (lane == 0) wave_n[wave] = __builtin_popcountll(mask);
-        __syncthreads();
-        int before = base_s;
-        for (int w = 0; w < wave; ++w) before += wave_n[w];
-        const int c = before + __builtin_popcountll(mask & ((1ull << lane) - 1));
-        if (in) {
-            a.row[c] = (int)i;
-            a.label[c] = label >= 0 && label < a.V ? (int)label : -1;
-            a.at_label[c] = __builtin_nanf("");
-        }
-        if (i < a.M) a.place[i] = in ? c : -1;
-        __syncthreads();
-        if (threadIdx.x == 1023) base_s = c + in;
-        __syncthreads();
+    if (lane == 0) wave_n[wave] = __builtin_popcountll(mask);
+    __syncthreads();
+    int n = 0, sum = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) {
+        if (w == wave) n = sum;
+        sum += wave_n[w];
     }
-    const int n = base_s;
+    *before = n + __builtin_popcountll(mask & ((1ull << lane) - 1));
+    *all = sum;
+    return in;
+}
+__device__ __forceinline__ void write_row(const Prep& a, int64_t i, int64_t label, bool in, int c) {
+    if (in) {
+        a.row[c] = (int)i;
+        a.label[c] = label >= 0 && label < a.V ? (int)label : -1;
+        if (a.at_label) a.at_label[c] = __builtin_nanf("");
+    }
+    if (i < a.M) {
+        a.place[i] = in ? c : -1;
+        if (!in && a.loss_out) a.loss_out[i] = 0.0f;
+    }
+}
+__device__ __forceinline__ void write_rest(const Prep& a, int n) {
     if (threadIdx.x == 0) *a.count = n;
     for (int64_t c = n + threadIdx.x; c < a.M_pad; c += 1024) {
         a.row[c] = 0;
         a.label[c] = -1;
     }
+    for (int i = threadIdx.x; i < a.n_redo; i += 1024) a.redo[i] = 0;
+}
+
+__global__ void __launch_bounds__(1024) lce_prepare_kernel(Prep a) {
+    __shared__ int wave_n[16];
+    int base = 0;
+    for (int64_t at = 0; at < a.M; at += 1024) {
+        const int64_t i = at + threadIdx.x, label = label_of(a, i);
+        int c, all;
+        const bool in = place_of(label != a.ignore, &c, &all, wave_n);
+        write_row(a, i, label, in, base + c);
+        base += all;
+    }
+    write_rest(a, base);
 }
 
 __device__ __forceinline__ f32x4 bf16x4_f32(u32x2 w) {
     return f32x4{__uint_as_float(w[0] << 16), __uint_as_float(w[0] & 0xffff0000u), __uint_as_float(w[1] << 16), __uint_as_float(w[1] & 0xffff0000u)};
 }
 
-// the label's logit of every row (log2 units): the first reference
-__global__ void __launch_bounds__(256) lce_target_kernel(LceRows rows, const bf16_t* x, int64_t ldx, const bf16_t* w, int64_t ldw, int H, float scale2,
-                                                         float* at_label, float* ref, float* z) {
-    const int lane = threadIdx.x & 63;
-    const int64_t c = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-    if (c >= *rows.count) return;
-    const int label = rows.label[c];
+// The label's logit of every row (log2 units): the first reference.  A wave has a row.  own_rows (up to kBeginRows labels): every block finds
+// its rows by itself, and the first does what lce_prepare_kernel does.
+__global__ void __launch_bounds__(1024) lce_target_kernel(Prep a, int own_rows, const bf16_t* x, int64_t ldx, const bf16_t* w, int64_t ldw, int H, float scale2,
+                                                          float* at_label, float* ref, float* z) {
+    __shared__ int wave_n[16], rows[16], labels[16];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const int64_t first = (int64_t)blockIdx.x * 16, c = first + wave;
+    int count;
+    if (own_rows) {
+        const int64_t i = threadIdx.x, label = label_of(a, i);
+        int at;
+        const bool in = place_of(label != a.ignore, &at, &count, wave_n);
+        if (in && at >= first && at < first + 16) {
+            rows[at - first] = (int)i;
+            labels[at - first] = label >= 0 && label < a.V ? (int)label : -1;
+        }
+        if (blockIdx.x == 0) {
+            write_row(a, i, label, in, at);
+            write_rest(a, count);
+        }
+        __syncthreads();
+    } else {
+        count = *a.count;
+    }
+    if (c >= count) return;
+    const int label = own_rows ? labels[wave] : a.label[c];
+    const int64_t row = own_rows ? rows[wave] : a.row[c];
     float sum = 0.0f;
     if (label >= 0) {
-        const bf16_t *xr = x + rows.row[c] * ldx, *wr = w + label * ldw;
+        const bf16_t *xr = x + row * ldx, *wr = w + label * ldw;
+#pragma unroll 4
         for (int k = lane * 8; k < H; k += 512) {
-            const u32x4 a = *(const u32x4*)(xr + k), b = *(const u32x4*)(wr + k);
+            const u32x4 p = *(const u32x4*)(xr + k), q = *(const u32x4*)(wr + k);
 #pragma unroll
-            for (int q = 0; q < 4; ++q)
-                sum += __uint_as_float(a[q] << 16) * __uint_as_float(b[q] << 16) + __uint_as_float(a[q] & 0xffff0000u) * __uint_as_float(b[q] & 0xffff0000u);
+            for (int j = 0; j < 4; ++j)
+                sum += __uint_as_float(p[j] << 16) * __uint_as_float(q[j] << 16) + __uint_as_float(p[j] & 0xffff0000u) * __uint_as_float(q[j] & 0xffff0000u);
         }
     }
 #pragma unroll
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) {
-        const float t = label >= 0 ? sum * scale2 : __builtin_nanf("");
-        at_label[c] = t;
-        ref[c] = t;
+        at_label[c] = ref[c] = label >= 0 ? sum * scale2 : __builtin_nanf("");
         z[c] = 0.0f;
     }
 }
 
-// ---- joins over the column tiles of a piece: 64 rows a block, 16 waves over the tiles
+// ---- joins over the column tiles: 16 rows a block, 64 groups of lanes over the tiles
 struct Join {
     const int32_t* count;
     const f32x2* part;
     int64_t rows_pad;
     int32_t tiles, tile_rows;
-    float *ref, *z, *alpha;
-    int32_t* redo;                      // by row tile
+    float *ref, *z;
+    const float *new_ref, *alpha;       // of row tiles that were done again
+    const int32_t* redo;
 };
 
+// in the first 16 threads of a block, for rows that count: the row's join
 template <typename F>
-__device__ __forceinline__ bool join_rows(const Join& a, f32x2 (*lds)[64], f32x2 start, F fold, f32x2* out, int64_t* row) {
+__device__ __forceinline__ bool join_rows(const Join& a, f32x2 start, F fold, f32x2* out, int64_t* row) {
+    __shared__ f32x2 lds[16][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int64_t r = (int64_t)blockIdx.x * 64 + lane;
+    const int64_t r = (int64_t)blockIdx.x * 16 + (lane & 15);
+    const int count = *a.count;
+    if ((int64_t)blockIdx.x * 16 >= count) return false;
     f32x2 v = start;
-    if (r < *a.count) {
+    const f32x2* p = a.part + min(r, (int64_t)count - 1);
 #pragma unroll 8
-        for (int t = wave; t < a.tiles; t += 16) v = fold(v, a.part[t * a.rows_pad + r]);
-    }
-    lds[wave][lane] = v;
+    for (int t = threadIdx.x >> 4; t < a.tiles; t += 64) v = fold(v, p[t * a.rows_pad]);
+#pragma unroll
+    for (int d = 16; d < 64; d <<= 1) v = fold(v, f32x2{__shfl_xor(v[0], d), __shfl_xor(v[1], d)});
+    if (lane < 16) lds[wave][lane] = v;
     __syncthreads();
-    if (wave != 0 || r >= *a.count) return false;
+    if (threadIdx.x >= 16 || r >= count) return false;
+    v = lds[0][lane];
+#pragma unroll
     for (int w = 1; w < 16; ++w) v = fold(v, lds[w][lane]);
     *out = v;
     *row = r;
     return true;
 }
+__device__ __forceinline__ f32x2 fold_sum(f32x2 p, f32x2 q) { return f32x2{0.0f, p[1] + q[1]}; }
 
-// EXP, before the second try: rows whose largest logit is too far above the reference get it as their new one
-__global__ void __launch_bounds__(1024) lce_far_kernel(Join a) {
-    __shared__ f32x2 lds[16][64];
-    f32x2 v;
-    int64_t r;
-    if (!join_rows(a, lds, f32x2{-INFINITY, 0.0f}, [](f32x2 p, f32x2 q) { return f32x2{fmaxf(p[0], q[0]), 0.0f}; }, &v, &r)) return;
-    const float ref = a.ref[r];
-    const bool far = v[0] - ref > kFar;
-    a.alpha[r] = far ? __builtin_amdgcn_exp2f(ref - v[0]) : 1.0f;
-    if (far) {
-        a.ref[r] = v[0];
-        a.redo[r / a.tile_rows] = 1;             // (set by several rows, to the same)
+// a row's Z' and reference with those of a piece
+__device__ __forceinline__ void add_piece(const Join& a, int64_t r, float sum, float* z, float* ref) {
+    *z = a.z[r];
+    *ref = a.ref[r];
+    if (a.redo[r / a.tile_rows]) {
+        *z *= a.alpha[r];
+        *ref = a.new_ref[r];
     }
+    *z += sum;
 }
-
 __global__ void __launch_bounds__(1024) lce_sum_kernel(Join a) {
-    __shared__ f32x2 lds[16][64];
     f32x2 v;
     int64_t r;
-    if (!join_rows(a, lds, f32x2{0.0f, 0.0f}, [](f32x2 p, f32x2 q) { return f32x2{0.0f, p[1] + q[1]}; }, &v, &r)) return;
-    a.z[r] = a.z[r] * a.alpha[r] + v[1];
-}
-
-__global__ void __launch_bounds__(256) lce_clear_kernel(int32_t* p, int n) {
-    for (int i = threadIdx.x; i < n; i += 256) p[i] = 0;
+    if (!join_rows(a, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
+    float z, ref;
+    add_piece(a, r, v[1], &z, &ref);
+    a.z[r] = z;
+    a.ref[r] = ref;
 }
 
 // what is kept of a row: 1 / Z, Z' / Z, log2 of the sum of exponentials
 struct RowEnd {
     float *inv, *rest, *lse2, *loss;
+    const int32_t* row;
+    float* out;                         // losses by row of x, or NULL
 };
 __device__ __forceinline__ void end_row(const RowEnd& e, int64_t c, float z, float ref, float t) {
     const float et = __builtin_amdgcn_exp2f(t - ref), sum = z + et;
-    e.loss[c] = ref == t ? log1pf(z) : logf(sum) + (ref - t) * kLn2;
+    const float loss = ref == t ? log1pf(z) : logf(sum) + (ref - t) * kLn2;
+    e.loss[c] = loss;
+    if (e.out) e.out[e.row[c]] = loss;
     e.inv[c] = 1.0f / sum;
     e.rest[c] = z / sum;
     e.lse2[c] = ref == t ? log1pf(z) * kLog2e + t : log2f(sum) + ref;
@@ -174,7 +222,6 @@ __device__ __forceinline__ void end_row(const RowEnd& e, int64_t c, float z, flo
 
 // STATS: joins and ends
 __global__ void __launch_bounds__(1024) lce_score_kernel(Join a, const float* at_label, RowEnd e) {
-    __shared__ f32x2 lds[16][64];
     f32x2 v;
     int64_t r;
     auto fold = [](f32x2 p, f32x2 q) {
@@ -182,18 +229,22 @@ __global__ void __launch_bounds__(1024) lce_score_kernel(Join a, const float* at
         if (top == -INFINITY) return f32x2{top, p[1] + q[1]};
         return f32x2{top, p[1] * __builtin_amdgcn_exp2f(p[0] - top) + q[1] * __builtin_amdgcn_exp2f(q[0] - top)};
     };
-    if (!join_rows(a, lds, f32x2{-INFINITY, 0.0f}, fold, &v, &r)) return;
+    if (!join_rows(a, f32x2{-INFINITY, 0.0f}, fold, &v, &r)) return;
     const float t = at_label[r];
     const float ref = v[0] > t ? v[0] : t;
     end_row(e, r, v[1] * __builtin_amdgcn_exp2f(v[0] - ref), ref, t);
 }
-
-__global__ void __launch_bounds__(256) lce_end_kernel(const int32_t* count, const float* z, const float* ref, const float* at_label, RowEnd e) {
-    const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (c < *count) end_row(e, c, z[c], ref[c], at_label[c]);
+// EXP: the last piece's sums, and ends; the label's logit is the first reference
+__global__ void __launch_bounds__(1024) lce_end_kernel(Join a, const float* at_label, RowEnd e) {
+    f32x2 v;
+    int64_t r;
+    if (!join_rows(a, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
+    float z, ref;
+    add_piece(a, r, v[1], &z, &ref);
+    end_row(e, r, z, ref, at_label[r]);
 }
 
-// losses to where their rows are, or their sum or mean: one block, in an order that the sizes fix
+// sum or mean of the losses: one block, in an order that the sizes fix
 __global__ void __launch_bounds__(1024) lce_reduce_kernel(const int32_t* count, const float* loss, int mean, float* out) {
     __shared__ double lds[16];
     const int n = *count;
@@ -206,12 +257,6 @@ __global__ void __launch_bounds__(1024) lce_reduce_kernel(const int32_t* count, 
     if (threadIdx.x) return;
     for (int w = 1; w < 16; ++w) s += lds[w];
     *out = (float)(mean ? s / n : s);
-}
-__global__ void __launch_bounds__(256) lce_place_kernel(const int32_t* place, int64_t M, const float* loss, float* out) {
-    const int64_t i = (int64_t)blockIdx.x * 256 + threadIdx.x;
-    if (i >= M) return;
-    const int c = place[i];
-    out[i] = c < 0 ? 0.0f : loss[c];
 }
 
 // ---- backward
@@ -227,7 +272,7 @@ __device__ __forceinline__ float upstream(const Upstream& u, int64_t row) {
 }
 
 // dx: a block has rows of x, a thread 8 columns at a time
-__global__ void __launch_bounds__(256) lce_dx_kernel(const int32_t* place, const int32_t* label, int64_t M, int H, const float* o, int splits, int64_t split_stride,
+__global__ void __launch_bounds__(256) lce_dx_kernel(const int32_t* place, const int32_t* label, int64_t M, int H, const float* o, int tile_rows, int steps, int cus,
                                                      const float* inv, const float* rest, const bf16_t* w, int64_t ldw, Upstream u, bf16_t* dx, int64_t lddx) {
     const int64_t i = blockIdx.x;
     const int c = place[i];
@@ -240,10 +285,12 @@ __global__ void __launch_bounds__(256) lce_dx_kernel(const int32_t* place, const
     const float a = g * inv[c], b = label[c] < 0 ? __builtin_nanf("") : g * rest[c];
     const bf16_t* wr = w + max(label[c], 0) * ldw;
     const float* oc = o + (int64_t)c * H;
+    const int count = *u.count, parts = lce_parts((count + tile_rows - 1) / tile_rows * ((H + 255) >> 8), steps, cus);
+    const int64_t split_stride = (int64_t)count * H;
     for (int k = threadIdx.x * 8; k < H; k += 2048) {
         const u32x4 t = *(const u32x4*)(wr + k);
         f32x4 lo = *(const f32x4*)(oc + k), hi = *(const f32x4*)(oc + k + 4);
-        for (int s = 1; s < splits; ++s) {
+        for (int s = 1; s < parts; ++s) {
             lo += *(const f32x4*)(oc + s * split_stride + k);
             hi += *(const f32x4*)(oc + s * split_stride + k + 4);
         }
@@ -272,37 +319,39 @@ __global__ void __launch_bounds__(256) lce_gather_kernel(LceRows rows, const bf1
 }
 
 // ---------------------------------------------------------------- host side
+int compute_units() {
+    static std::atomic<int> cached{0};
+    int n = cached.load(std::memory_order_relaxed), dev = 0;
+    if (n > 0) return n;
+    if (hipGetDevice(&dev) != hipSuccess || hipDeviceGetAttribute(&n, hipDeviceAttributeMultiprocessorCount, dev) != hipSuccess || n <= 0) n = 256;
+    cached.store(n, std::memory_order_relaxed);
+    return n;
+}
+
 struct Plan {
     int tm;                             // rows of a tile: 32 tm
     int64_t rows_pad, piece, pieces;    // columns of the vocabulary at a time (a multiple of 256), and how many times
-    int splits;                         // of the product E . W
 };
 
 int tile_for(int64_t rows) { return rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }
 
-Plan plan_tokens(int64_t M, int64_t V, int64_t H) {
+// tm 0: by the rows
+Plan plan_for(int64_t M, int64_t V, int tm) {
     Plan p;
-    p.tm = tile_for(M);
+    p.tm = tm ? tm : tile_for(M);
     p.rows_pad = up256(std::max<int64_t>(M, 1));
     const int64_t most = std::max<int64_t>(256, kPieceBytes / (p.rows_pad * 2) / 256 * 256);
     p.pieces = xq_cdiv(up256(V), most);
     p.piece = up256(xq_cdiv(up256(V), p.pieces));
     p.pieces = xq_cdiv(V, p.piece);
-    const int64_t tiles = xq_cdiv(std::max<int64_t>(M, 1), 32 * p.tm) * xq_cdiv(H, 256);
-    p.splits = (int)std::max<int64_t>(1, std::min<int64_t>(256 / tiles, p.piece / 512));
     return p;
 }
+Plan plan_tokens(int64_t M, int64_t V) { return plan_for(M, V, 0); }
+Plan plan_head(int64_t M, int64_t V) { return plan_for(M, V, 8); }          // G: rows of the vocabulary, tokens along the contraction
 
-Plan plan_head(int64_t M, int64_t V) {       // G: rows of the vocabulary, tokens along the contraction
-    Plan p;
-    p.tm = 8;
-    p.rows_pad = up256(std::max<int64_t>(M, 1));
-    const int64_t most = std::max<int64_t>(256, kPieceBytes / (p.rows_pad * 2) / 256 * 256);
-    p.pieces = xq_cdiv(up256(V), most);
-    p.piece = up256(xq_cdiv(up256(V), p.pieces));
-    p.pieces = xq_cdiv(V, p.piece);
-    p.splits = 1;
-    return p;
+// fp32 sums of E . W over the parts of the contraction, whatever the rows that count (lce_parts)
+int64_t sums_bytes(const Plan& p, int64_t M, int64_t H) {
+    return 4 * std::max<int64_t>(M * H, (int64_t)kLceSplitRounds * compute_units() * 32 * p.tm * 256);
 }
 
 // what a forward leaves for the backward
@@ -312,7 +361,7 @@ struct Saved {
     int64_t bytes;
 };
 Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
-    const Plan p = plan_tokens(M, V, H);
+    const Plan p = plan_tokens(M, V);
     uint8_t* at = (uint8_t*)base;
     auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
     Saved s;
@@ -325,20 +374,20 @@ Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
     s.rest = (float*)take(4 * p.rows_pad);
     s.lse2 = (float*)take(4 * p.rows_pad);
     s.loss = (float*)take(4 * p.rows_pad);
-    s.o = keep == XQ_LCE_KEEP_DX ? (float*)take(4 * p.splits * M * H) : nullptr;
+    s.o = keep == XQ_LCE_KEEP_DX ? (float*)take(sums_bytes(p, M, H)) : nullptr;
     s.bytes = at - (uint8_t*)base;
     return s;
 }
 
 struct Scratch {
-    float *ref, *z, *alpha, *up;
+    float *ref, *z, *alpha, *up, *new_ref;
     int32_t* redo;
     f32x2* part;
     bf16_t *image, *x;
     int64_t bytes;
 };
 Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
-    const Plan p = pass == XQ_LCE_KEEP_HEAD_BWD ? plan_head(M, V) : plan_tokens(M, V, H);
+    const Plan p = pass == XQ_LCE_KEEP_HEAD_BWD ? plan_head(M, V) : plan_tokens(M, V);
     uint8_t* at = (uint8_t*)base;
     auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
     Scratch s = {};
@@ -346,7 +395,8 @@ Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
     s.z = (float*)take(4 * p.rows_pad);
     s.alpha = (float*)take(4 * p.rows_pad);
     s.up = (float*)take(4 * p.rows_pad);
-    s.redo = (int32_t*)take(4 * (p.rows_pad / 64));
+    s.new_ref = (float*)take(4 * p.rows_pad);
+    s.redo = (int32_t*)take(4 * p.pieces * (p.rows_pad / 64));
     if (pass == XQ_LCE_KEEP_HEAD_BWD) {
         s.x = (bf16_t*)take(2 * M * H);
         s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
@@ -365,7 +415,9 @@ int launch_logits(const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_
     auto k = lce_logits_kernel<TM, MODE>;
     static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
     if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
-    k<<<dim3((unsigned)(xq_cdiv(rows, T::ROWS) * xq_cdiv(cols, 256))), 512, T::LDS_BYTES, s>>>(a);
+    int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(cols, 256);
+    if (T::AHEAD) blocks = std::min<int64_t>(blocks, compute_units());
+    k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
     return XQ_OK;
 }
 template <int MODE>
@@ -378,7 +430,9 @@ int launch_product(const LceProductArgs& a, int64_t rows, hipStream_t s) {
     auto k = lce_product_kernel<TM>;
     static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
     if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
-    k<<<dim3((unsigned)(xq_cdiv(rows, T::ROWS) * xq_cdiv(a.H, 256)), a.splits), 512, T::LDS_BYTES, s>>>(a);
+    int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(a.H, 256);
+    if (a.cus) blocks = std::max<int64_t>(blocks, std::min<int64_t>(32 * blocks, (int64_t)kLceSplitRounds * a.cus));
+    k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
     return XQ_OK;
 }
 int launch_product(int tm, const LceProductArgs& a, int64_t rows, hipStream_t s) {
@@ -423,44 +477,47 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
     XQ_REQUIRE((loss && xq_aligned(loss, 4)) || (q->M == 0 && q->reduction == XQ_LCE_NONE), "xq_lce_fwd: loss is NULL or misaligned");
     hipStream_t st = (hipStream_t)stream;
     const int64_t M = q->M, V = q->V, H = q->H;
-    const Plan p = plan_tokens(M, V, H);
+    const Plan p = plan_tokens(M, V);
     const Saved s = saved_of(saved, M, V, H, keep);
     const Scratch c = scratch_of(workspace, M, V, H, keep);
-    const LceRows rows = {s.count, s.row, s.label};
-    const RowEnd end = {s.inv, s.rest, s.lse2, s.loss};
     const float scale2 = q->logit_scale * kLog2e;
-    lce_prepare_kernel<<<dim3(1), 1024, 0, st>>>(Prep{q->labels, q->label_bytes, M, p.rows_pad, V, q->ignore_index, s.count, s.row, s.label, s.place, s.at_label});
-    const dim3 by64((unsigned)xq_cdiv(M, 64)), by256((unsigned)xq_cdiv(M, 256));
+    const bool none = q->reduction == XQ_LCE_NONE;
+    const int row_tiles = (int)xq_cdiv(M, 32 * p.tm);
+    const RowEnd end = {s.inv, s.rest, s.lse2, s.loss, s.row, none ? loss : nullptr};
+    const Prep prep = {q->labels, q->label_bytes, M, p.rows_pad, V, q->ignore_index, s.count, s.row, s.label, s.place,
+                       keep == XQ_LCE_KEEP_DX ? nullptr : s.at_label, c.redo,
+                       keep == XQ_LCE_KEEP_DX ? (int32_t)(p.pieces * row_tiles) : 0, none ? loss : nullptr};
+    const dim3 by16((unsigned)xq_cdiv(M, 16));
+    Join join = {s.count, c.part, p.rows_pad, 0, 32 * p.tm, c.ref, c.z, c.new_ref, c.alpha, nullptr};
     LceLogitsArgs a = {};
     a.A = (const bf16_t*)q->x; a.lda = q->ldx; a.B = (const bf16_t*)q->w; a.ldb = q->ldw;
-    a.H = (int32_t)H; a.rows = rows; a.scale2 = scale2; a.part = c.part; a.at_label = s.at_label; a.rows_pad = p.rows_pad;
+    a.H = (int32_t)H; a.rows = {s.count, s.row, s.label}; a.scale2 = scale2; a.part = c.part; a.rows_pad = p.rows_pad;
+    const bool own_rows = keep == XQ_LCE_KEEP_DX && M > 0 && M <= kBeginRows;
+    if (!own_rows) lce_prepare_kernel<<<dim3(1), 1024, 0, st>>>(prep);
     if (M > 0 && keep != XQ_LCE_KEEP_DX) {
-        a.first_v = 0; a.n_v = (int32_t)V;
+        a.n_v = (int32_t)V; a.at_label = s.at_label;
         if ((rc = launch_logits<kLceStats>(p.tm, a, M, V, st)) != XQ_OK) return rc;
-        lce_score_kernel<<<by64, 1024, 0, st>>>(Join{s.count, c.part, p.rows_pad, (int32_t)xq_cdiv(V, 256), 0, nullptr, nullptr, nullptr, nullptr}, s.at_label, end);
+        join.tiles = (int32_t)xq_cdiv(V, 256);
+        lce_score_kernel<<<by16, 1024, 0, st>>>(join, s.at_label, end);
     } else if (M > 0) {
-        lce_target_kernel<<<dim3((unsigned)xq_cdiv(M, 4)), 256, 0, st>>>(rows, a.A, a.lda, a.B, a.ldb, (int)H, scale2, s.at_label, c.ref, c.z);
-        const int row_tiles = (int)xq_cdiv(M, 32 * p.tm);
-        for (int64_t v0 = 0; v0 < V; v0 += p.piece) {
+        lce_target_kernel<<<by16, 1024, 0, st>>>(prep, own_rows, a.A, a.lda, a.B, a.ldb, (int)H, scale2, s.at_label, c.ref, c.z);
+        a.ref = c.ref; a.new_ref = c.new_ref; a.alpha = c.alpha; a.image = c.image; a.image_steps = (int32_t)(p.piece / 32); a.redo = c.redo;
+        for (int64_t v0 = 0; v0 < V; v0 += p.piece, a.redo += row_tiles) {
             const int64_t n = std::min(p.piece, V - v0);
-            a.first_v = (int32_t)v0; a.n_v = (int32_t)n; a.ref = c.ref; a.image = c.image; a.image_steps = (int32_t)(p.piece / 32); a.redo = nullptr;
-            if ((rc = launch_logits<kLceExp>(p.tm, a, M, n, st)) != XQ_OK) return rc;
-            lce_clear_kernel<<<dim3(1), 256, 0, st>>>(c.redo, row_tiles);
-            const Join j = {s.count, c.part, p.rows_pad, (int32_t)xq_cdiv(n, 256), 32 * p.tm, c.ref, c.z, c.alpha, c.redo};
-            lce_far_kernel<<<by64, 1024, 0, st>>>(j);
-            a.redo = c.redo;
-            if ((rc = launch_logits<kLceExp>(p.tm, a, M, n, st)) != XQ_OK) return rc;
-            lce_sum_kernel<<<by64, 1024, 0, st>>>(j);
+            a.first_v = (int32_t)v0; a.n_v = (int32_t)n;
+            for (a.again = 0; a.again < 2; ++a.again)
+                if ((rc = launch_logits<kLceExp>(p.tm, a, M, n, st)) != XQ_OK) return rc;
+            join.tiles = (int32_t)xq_cdiv(n, 256); join.redo = a.redo;
+            if (v0 + n < V) lce_sum_kernel<<<by16, 1024, 0, st>>>(join);
+            else lce_end_kernel<<<by16, 1024, 0, st>>>(join, s.at_label, end);
             LceProductArgs o = {};
             o.image = c.image; o.image_steps = a.image_steps; o.rows = -1; o.k = (int32_t)n; o.count = s.count;
-            o.B = a.B + v0 * a.ldb; o.ldb = a.ldb; o.H = (int32_t)H; o.splits = p.splits;
-            o.out = s.o; o.split_stride = M * H; o.alpha = c.alpha; o.add = v0 > 0;
+            o.B = a.B + v0 * a.ldb; o.ldb = a.ldb; o.H = (int32_t)H; o.cus = compute_units();
+            o.out = s.o; o.alpha = c.alpha; o.redo = a.redo; o.add = v0 > 0;
             if ((rc = launch_product(p.tm, o, M, st)) != XQ_OK) return rc;
         }
-        lce_end_kernel<<<by256, 256, 0, st>>>(s.count, c.z, c.ref, s.at_label, end);
     }
-    if (q->reduction != XQ_LCE_NONE) lce_reduce_kernel<<<dim3(1), 1024, 0, st>>>(s.count, s.loss, q->reduction == XQ_LCE_MEAN, loss);
-    else if (M > 0) lce_place_kernel<<<by256, 256, 0, st>>>(s.place, M, s.loss, loss);
+    if (!none) lce_reduce_kernel<<<dim3(1), 1024, 0, st>>>(s.count, s.loss, q->reduction == XQ_LCE_MEAN, loss);
     XQ_CHECK_LAUNCH("xq_lce_fwd");
     return XQ_OK;
 }
@@ -477,12 +534,12 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
     XQ_REQUIRE(!dw || (xq_aligned(dw, 16) && lddw >= q->H && lddw % 8 == 0), "xq_lce_bwd: dw must be 16-byte aligned with a row stride that is a multiple of 8 elements");
     hipStream_t st = (hipStream_t)stream;
     const int64_t M = q->M, V = q->V, H = q->H;
-    const Plan p = plan_tokens(M, V, H);
+    const Plan p = plan_tokens(M, V);
     const Saved s = saved_of((void*)saved, M, V, H, keep);
     const LceRows rows = {s.count, s.row, s.label};
     const Upstream u = {grad, q->reduction, s.count, q->logit_scale};
     if (dx && M > 0)
-        lce_dx_kernel<<<dim3((unsigned)M), 256, 0, st>>>(s.place, s.label, M, (int)H, s.o, p.splits, M * H, s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
+        lce_dx_kernel<<<dim3((unsigned)M), 256, 0, st>>>(s.place, s.label, M, (int)H, s.o, 32 * p.tm, (int)(p.piece / 32), compute_units(), s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
     if (dw) {
         const Plan h = plan_head(M, V);
         const Scratch c = scratch_of(workspace, M, V, H, XQ_LCE_KEEP_HEAD_BWD);
@@ -500,7 +557,7 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
             if (M > 0 && (rc = launch_logits<kLceGrad>(h.tm, a, n, M, st)) != XQ_OK) return rc;
             LceProductArgs o = {};
             o.image = c.image; o.image_steps = a.image_steps; o.rows = (int32_t)n; o.k = -1; o.count = s.count;
-            o.B = c.x; o.ldb = H; o.H = (int32_t)H; o.splits = 1;
+            o.B = c.x; o.ldb = H; o.H = (int32_t)H;
             o.out16 = (bf16_t*)dw + v0 * lddw; o.ld16 = lddw;
             if ((rc = launch_product(h.tm, o, n, st)) != XQ_OK) return rc;
         }
