@@ -48,6 +48,7 @@ struct LceLogitsArgs {
     const bf16_t* B;
     int64_t lda, ldb;
     int32_t H, first_v, n_v;            // the piece of the vocabulary: its first row of the head and how many
+    int32_t cols;                       // of a tile, up to 256 (GRAD, and above 128 rows: 256)
     LceRows rows;
     float scale2;                       // of the logits, times log2(e)
     const float* ref;                   // EXP: reference of a row, in log2 units;  GRAD: log2 of the row's sum of exponentials
@@ -216,7 +217,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
     const int count = __builtin_amdgcn_readfirstlane(*g.rows.count);
     const int n_a = MODE == kLceGrad ? g.n_v : count, n_b = MODE == kLceGrad ? count : g.n_v;
-    const int tiles_a = (n_a + T::ROWS - 1) / T::ROWS, tiles_b = (n_b + 255) >> 8, nk = g.H / T::BK;
+    const int tiles_a = (n_a + T::ROWS - 1) / T::ROWS, cols = MODE == kLceGrad || TM > 4 ? 256 : g.cols, tiles_b = (n_b + cols - 1) / cols, nk = g.H / T::BK;
 
     LceWalk walk(tiles_a * tiles_b);
     int ta, tb;
@@ -235,7 +236,8 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
         for (int p = 0; p < T::NP; ++p) {
             const bool of_a = p < T::AP;
             const int rt = of_a ? wave * (T::ROWS / 8) + p * 16 + (lane >> 2) : wave * 32 + (p - T::AP) * 16 + (lane >> 2);
-            const int n = min((of_a ? ta * T::ROWS : tb * 256) + rt, (of_a ? n_a : n_b) - 1);
+            // (rows behind the last, of either side or of the tile's columns: that one again, for nothing)
+            const int n = of_a ? min(ta * T::ROWS + rt, n_a - 1) : min(tb * cols + min(rt, cols - 1), n_b - 1);
             const bool tokens = of_a != (MODE == kLceGrad);
             const int64_t row = tokens ? g.rows.row[n] : g.first_v + n;
             src[p] = (of_a ? g.A + row * g.lda : g.B + row * g.ldb) + (((lane & 3) ^ ((rt >> 2) & 2)) << 3);
@@ -277,26 +279,37 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     };
     float about[4];
     bool more = false;
+    // Few rows: the head is all that is read, by all blocks at the same pace.  Starting each column tile at another K-step (and going round)
+    // spreads what they read at a time over the memory channels: rows of the head are often a power of two apart (65536 x 4096 under one row:
+    // 138 us in step, 110 so).
+    auto turn = [&](int tile) -> int { return TM <= 4 ? (int)((uint32_t)tile * 37u % (uint32_t)nk) : 0; };
+    int turned = 0, turned_next = 0;
     // (behind the tile's last K-step: the next tile's; without one, this one's again, for nothing)
     auto advance = [&](int kt) -> int {
         if (kt == nk && more) {
 #pragma unroll
             for (int p = 0; p < T::NP; ++p) src[p] = src_next[p];
+            turned = turned_next;
         }
-        return kt < nk ? kt : kt - nk < nk ? kt - nk : 0;
+        const int k = (kt < nk ? kt : kt - nk < nk ? kt - nk : 0) + turned;
+        return k < nk ? k : k - nk;
     };
     if (!find()) return;
     const bool stream = T::AHEAD && nk >= 4;                // (two K-steps: a tile's end is nearer than the loads are ahead)
     sources(src, about);
+    turned = turn(tb);
     lce_begin<TM>(dsm, advance, issue);
     if (T::AHEAD) note(about);
     int first = 0;
     do {
-        const int r0 = ta * T::ROWS, c0 = tb * 256, this_a = ta, this_b = tb;
+        const int r0 = ta * T::ROWS, c0 = tb * cols, this_a = ta, this_b = tb;
         if (stream) {
             walk.at += walk.step;
             more = find();
-            if (more) sources(src_next, about);
+            if (more) {
+                sources(src_next, about);
+                turned_next = turn(tb);
+            }
         }
         f32x4 acc[TM][4];
         lce_run<TM, false>(acc, dsm, first, nk, wave, lane, advance, issue);
@@ -327,19 +340,21 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             }
         } else {
             // columns that the piece does not have, and the label's, count as -inf
-            if (c0 + 256 > g.n_v) {
+            const int end = min(cols, g.n_v - c0);
+            if (end < 256) {
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
                     for (int j = 0; j < 4; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
-                            if (c0 + col_w + 16 * j + e >= g.n_v) acc[i][j][e] = -INFINITY;
+                            if (col_w + 16 * j + e >= end) acc[i][j][e] = -INFINITY;
             }
             float ref[TM], top[TM], sum[TM];
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                const int at = __float_as_int(info[row_w + 16 * i]) - c0 - col_w;     // the label's column by the lane's own numbering of its 16
+                int at = __float_as_int(info[row_w + 16 * i]) - c0 - col_w;           // the label's column by the lane's own numbering of its 16
+                if (col_w + at >= end) at = -1;
                 if (MODE == kLceExp) ref[i] = info[N_INFO + row_w + 16 * i];
                 if (__any(at >= 0 && at < 52)) {
 #pragma unroll
@@ -405,6 +420,11 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                 const int row = row_w + 16 * i;
 #pragma unroll
                 for (int q = 0; q < 2; ++q) {
+                    if (TM <= 4) {
+                        // the next tile's;  (the last tile goes on to the end of the image: the product takes K-steps in pairs)
+                        const int step = wn * 2 + q;
+                        if ((step * 32 >= cols && this_b + 1 < tiles_b) || (c0 >> 5) + step >= g.image_steps) continue;
+                    }
                     const f32x4 a = acc[i][2 * q], b = acc[i][2 * q + 1];
                     *(u32x4*)(out + (q * T::ROWS + row) * 32 + ((lg ^ ((row >> 2) & 2)) << 3)) =
                         u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
@@ -418,6 +438,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             walk.at += walk.step;
             if (find()) {
                 sources(src, about);
+                turned = turn(tb);
                 __syncthreads();
                 lce_begin<TM>(dsm, advance, issue);
                 note(about);
@@ -450,11 +471,11 @@ struct LceProductArgs {
 // Parts of a contraction of E . W: as many as leave the least of the chip idle, where tiles alone would (a part costs its sums once more in
 // memory: 2 % a part).  The rows that count are known on the device only, so that every kernel works it out for itself.  Divided, tiles and
 // parts are three rounds of the chip at most, which bounds the sums.
-constexpr int kLceSplitRounds = 3;
+constexpr int kLceSplitRounds = 3, kLceMostParts = 64;
 __host__ __device__ inline int lce_parts(int tiles, int steps, int cus) {
     int best = 1;
     float least = 1e30f;
-    for (int s = 1; s <= 32; ++s) {
+    for (int s = 1; s <= kLceMostParts; ++s) {
         if (s > 1 && (tiles * s > kLceSplitRounds * cus || steps < 16 * s)) break;
         const float cost = (float)((tiles * s + cus - 1) / cus) / (float)s * (1.0f + 0.02f * (float)(s - 1));
         if (cost < 0.999f * least) { least = cost; best = s; }

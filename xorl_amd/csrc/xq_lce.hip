@@ -328,15 +328,32 @@ int compute_units() {
     return n;
 }
 
+// blocks of a product that run at a time, for lce_parts
+int slots(int tm) { return (tm == 2 ? 2 : 1) * compute_units(); }
+
 struct Plan {
-    int tm;                             // rows of a tile: 32 tm
+    int tm, cols;                       // rows of a logits tile: 32 tm, and its columns
     int64_t rows_pad, piece, pieces;    // columns of the vocabulary at a time (a multiple of 256), and how many times
 };
 
 int tile_for(int64_t rows) { return rows <= 64 ? 2 : rows <= 128 ? 4 : 8; }
 
-// tm 0: by the rows
-Plan plan_for(int64_t M, int64_t V, int tm) {
+// Columns of a tile.  Up to 128 rows reading the head is what counts, and a compute unit reads at a rate of its own: as many columns as leave
+// the busiest the least to read (100003 columns: 481 tiles of 208 and not 391 of 256, of which some units have two and some one).
+// A tile costs what 16 columns do beside.  E: whole K-steps of 32.
+int columns_for(int tm, int64_t V, bool steps) {
+    if (tm > 4) return 256;
+    int best = 256;
+    int64_t least = INT64_MAX;
+    for (int c = 256; c >= 64; c -= steps ? 32 : 16) {
+        const int64_t cost = xq_cdiv(xq_cdiv(V, c), compute_units()) * (c + 16);
+        if (cost < least) { least = cost; best = c; }
+    }
+    return best;
+}
+
+// tm 0: by the rows;  steps: E is wanted
+Plan plan_for(int64_t M, int64_t V, int tm, bool steps) {
     Plan p;
     p.tm = tm ? tm : tile_for(M);
     p.rows_pad = up256(std::max<int64_t>(M, 1));
@@ -344,14 +361,15 @@ Plan plan_for(int64_t M, int64_t V, int tm) {
     p.pieces = xq_cdiv(up256(V), most);
     p.piece = up256(xq_cdiv(up256(V), p.pieces));
     p.pieces = xq_cdiv(V, p.piece);
+    p.cols = columns_for(p.tm, steps ? std::min(V, p.piece) : V, steps);
     return p;
 }
-Plan plan_tokens(int64_t M, int64_t V) { return plan_for(M, V, 0); }
-Plan plan_head(int64_t M, int64_t V) { return plan_for(M, V, 8); }          // G: rows of the vocabulary, tokens along the contraction
+Plan plan_tokens(int64_t M, int64_t V, int keep) { return plan_for(M, V, 0, keep == XQ_LCE_KEEP_DX); }
+Plan plan_head(int64_t M, int64_t V) { return plan_for(M, V, 8, true); }          // G: rows of the vocabulary, tokens along the contraction
 
 // fp32 sums of E . W over the parts of the contraction, whatever the rows that count (lce_parts)
 int64_t sums_bytes(const Plan& p, int64_t M, int64_t H) {
-    return 4 * std::max<int64_t>(M * H, (int64_t)kLceSplitRounds * compute_units() * 32 * p.tm * 256);
+    return 4 * std::max<int64_t>(M * H, (int64_t)kLceSplitRounds * slots(p.tm) * 32 * p.tm * 256);
 }
 
 // what a forward leaves for the backward
@@ -361,7 +379,7 @@ struct Saved {
     int64_t bytes;
 };
 Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
-    const Plan p = plan_tokens(M, V);
+    const Plan p = plan_tokens(M, V, keep);
     uint8_t* at = (uint8_t*)base;
     auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
     Saved s;
@@ -387,7 +405,7 @@ struct Scratch {
     int64_t bytes;
 };
 Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
-    const Plan p = pass == XQ_LCE_KEEP_HEAD_BWD ? plan_head(M, V) : plan_tokens(M, V);
+    const Plan p = pass == XQ_LCE_KEEP_HEAD_BWD ? plan_head(M, V) : plan_tokens(M, V, pass);
     uint8_t* at = (uint8_t*)base;
     auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
     Scratch s = {};
@@ -401,8 +419,7 @@ Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
         s.x = (bf16_t*)take(2 * M * H);
         s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
     } else {
-        const int64_t columns = pass == XQ_LCE_KEEP_DX ? p.piece : up256(V);
-        s.part = (f32x2*)take(8 * p.rows_pad * (columns / 256));
+        s.part = (f32x2*)take(8 * p.rows_pad * xq_cdiv(pass == XQ_LCE_KEEP_DX ? p.piece : V, p.cols));
         if (pass == XQ_LCE_KEEP_DX) s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
     }
     s.bytes = at - (uint8_t*)base;
@@ -415,7 +432,7 @@ int launch_logits(const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_
     auto k = lce_logits_kernel<TM, MODE>;
     static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
     if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
-    int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(cols, 256);
+    int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(cols, a.cols);
     if (T::AHEAD) blocks = std::min<int64_t>(blocks, compute_units());
     k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
     return XQ_OK;
@@ -431,7 +448,7 @@ int launch_product(const LceProductArgs& a, int64_t rows, hipStream_t s) {
     static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
     if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
     int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(a.H, 256);
-    if (a.cus) blocks = std::max<int64_t>(blocks, std::min<int64_t>(32 * blocks, (int64_t)kLceSplitRounds * a.cus));
+    if (a.cus) blocks = std::max<int64_t>(blocks, std::min<int64_t>(kLceMostParts * blocks, (int64_t)kLceSplitRounds * a.cus));
     k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
     return XQ_OK;
 }
@@ -477,7 +494,7 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
     XQ_REQUIRE((loss && xq_aligned(loss, 4)) || (q->M == 0 && q->reduction == XQ_LCE_NONE), "xq_lce_fwd: loss is NULL or misaligned");
     hipStream_t st = (hipStream_t)stream;
     const int64_t M = q->M, V = q->V, H = q->H;
-    const Plan p = plan_tokens(M, V);
+    const Plan p = plan_tokens(M, V, keep);
     const Saved s = saved_of(saved, M, V, H, keep);
     const Scratch c = scratch_of(workspace, M, V, H, keep);
     const float scale2 = q->logit_scale * kLog2e;
@@ -491,13 +508,13 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
     Join join = {s.count, c.part, p.rows_pad, 0, 32 * p.tm, c.ref, c.z, c.new_ref, c.alpha, nullptr};
     LceLogitsArgs a = {};
     a.A = (const bf16_t*)q->x; a.lda = q->ldx; a.B = (const bf16_t*)q->w; a.ldb = q->ldw;
-    a.H = (int32_t)H; a.rows = {s.count, s.row, s.label}; a.scale2 = scale2; a.part = c.part; a.rows_pad = p.rows_pad;
+    a.H = (int32_t)H; a.cols = p.cols; a.rows = {s.count, s.row, s.label}; a.scale2 = scale2; a.part = c.part; a.rows_pad = p.rows_pad;
     const bool own_rows = keep == XQ_LCE_KEEP_DX && M > 0 && M <= kBeginRows;
     if (!own_rows) lce_prepare_kernel<<<dim3(1), 1024, 0, st>>>(prep);
     if (M > 0 && keep != XQ_LCE_KEEP_DX) {
         a.n_v = (int32_t)V; a.at_label = s.at_label;
         if ((rc = launch_logits<kLceStats>(p.tm, a, M, V, st)) != XQ_OK) return rc;
-        join.tiles = (int32_t)xq_cdiv(V, 256);
+        join.tiles = (int32_t)xq_cdiv(V, p.cols);
         lce_score_kernel<<<by16, 1024, 0, st>>>(join, s.at_label, end);
     } else if (M > 0) {
         lce_target_kernel<<<by16, 1024, 0, st>>>(prep, own_rows, a.A, a.lda, a.B, a.ldb, (int)H, scale2, s.at_label, c.ref, c.z);
@@ -507,12 +524,12 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
             a.first_v = (int32_t)v0; a.n_v = (int32_t)n;
             for (a.again = 0; a.again < 2; ++a.again)
                 if ((rc = launch_logits<kLceExp>(p.tm, a, M, n, st)) != XQ_OK) return rc;
-            join.tiles = (int32_t)xq_cdiv(n, 256); join.redo = a.redo;
+            join.tiles = (int32_t)xq_cdiv(n, p.cols); join.redo = a.redo;
             if (v0 + n < V) lce_sum_kernel<<<by16, 1024, 0, st>>>(join);
             else lce_end_kernel<<<by16, 1024, 0, st>>>(join, s.at_label, end);
             LceProductArgs o = {};
             o.image = c.image; o.image_steps = a.image_steps; o.rows = -1; o.k = (int32_t)n; o.count = s.count;
-            o.B = a.B + v0 * a.ldb; o.ldb = a.ldb; o.H = (int32_t)H; o.cus = compute_units();
+            o.B = a.B + v0 * a.ldb; o.ldb = a.ldb; o.H = (int32_t)H; o.cus = slots(p.tm);
             o.out = s.o; o.alpha = c.alpha; o.redo = a.redo; o.add = v0 > 0;
             if ((rc = launch_product(p.tm, o, M, st)) != XQ_OK) return rc;
         }
@@ -534,12 +551,12 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
     XQ_REQUIRE(!dw || (xq_aligned(dw, 16) && lddw >= q->H && lddw % 8 == 0), "xq_lce_bwd: dw must be 16-byte aligned with a row stride that is a multiple of 8 elements");
     hipStream_t st = (hipStream_t)stream;
     const int64_t M = q->M, V = q->V, H = q->H;
-    const Plan p = plan_tokens(M, V);
+    const Plan p = plan_tokens(M, V, keep);
     const Saved s = saved_of((void*)saved, M, V, H, keep);
     const LceRows rows = {s.count, s.row, s.label};
     const Upstream u = {grad, q->reduction, s.count, q->logit_scale};
     if (dx && M > 0)
-        lce_dx_kernel<<<dim3((unsigned)M), 256, 0, st>>>(s.place, s.label, M, (int)H, s.o, 32 * p.tm, (int)(p.piece / 32), compute_units(), s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
+        lce_dx_kernel<<<dim3((unsigned)M), 256, 0, st>>>(s.place, s.label, M, (int)H, s.o, 32 * p.tm, (int)(p.piece / 32), slots(p.tm), s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
     if (dw) {
         const Plan h = plan_head(M, V);
         const Scratch c = scratch_of(workspace, M, V, H, XQ_LCE_KEEP_HEAD_BWD);
@@ -549,12 +566,12 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
         }
         LceLogitsArgs a = {};
         a.A = (const bf16_t*)q->w; a.lda = q->ldw; a.B = (const bf16_t*)q->x; a.ldb = q->ldx;
-        a.H = (int32_t)H; a.rows = rows; a.scale2 = q->logit_scale * kLog2e; a.ref = c.ref; a.grad = c.up; a.rest = c.z; a.rows_pad = h.rows_pad;
+        a.H = (int32_t)H; a.cols = 256; a.rows = rows; a.scale2 = q->logit_scale * kLog2e; a.ref = c.ref; a.grad = c.up; a.rest = c.z; a.rows_pad = h.rows_pad;
         a.image = c.image; a.image_steps = (int32_t)(h.rows_pad / 32);
         for (int64_t v0 = 0; v0 < V; v0 += h.piece) {
             const int64_t n = std::min(h.piece, V - v0);
             a.first_v = (int32_t)v0; a.n_v = (int32_t)n;
-            if (M > 0 && (rc = launch_logits<kLceGrad>(h.tm, a, n, M, st)) != XQ_OK) return rc;
+            if (M > 0 && (rc = launch_logits<8, kLceGrad>(a, n, M, st)) != XQ_OK) return rc;
             LceProductArgs o = {};
             o.image = c.image; o.image_steps = a.image_steps; o.rows = (int32_t)n; o.k = -1; o.count = s.count;
             o.B = c.x; o.ldb = H; o.H = (int32_t)H;

@@ -24,6 +24,7 @@
 #include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/functions/utils.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/autograd/saved_variable.h>
@@ -448,6 +449,71 @@ struct QLoRAMLPBackward : public Node {
     }
 };
 
+// what a cross entropy over a head is about: tensors, checked, as the library takes them
+struct HeadLoss {
+    xq_lce_problem q{};
+    Tensor keep_labels;
+    Rows xr;
+
+    HeadLoss(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore, int reduction, double scale) : xr(x, x.size(-1)) {
+        keep_labels = labels.is_contiguous() ? labels : labels.contiguous();
+        q.x = xr.ptr; q.ldx = xr.ld; q.M = xr.M;
+        q.w = w.data_ptr(); q.V = w.size(0); q.H = w.size(1); q.ldw = q.V > 1 ? w.stride(0) : q.H;
+        q.labels = keep_labels.data_ptr(); q.label_bytes = (int32_t)keep_labels.element_size();
+        q.ignore_index = ignore; q.reduction = reduction; q.logit_scale = (float)scale;
+    }
+    static bool takes(const Tensor& x, const Tensor& w, const Tensor& labels) {
+        if (x.scalar_type() != at::kBFloat16 || w.scalar_type() != at::kBFloat16 || w.dim() != 2 || x.dim() < 1 || labels.dim() != x.dim() - 1) return false;
+        if (labels.scalar_type() != at::kLong && labels.scalar_type() != at::kInt) return false;
+        if (x.sizes().slice(0, x.dim() - 1) != labels.sizes() || x.size(-1) != w.size(1) || w.size(1) < 64 || w.size(1) % 64 || w.size(0) < 1) return false;
+        if (x.device() != w.device() || x.device() != labels.device() || x.is_neg() || w.is_neg() || labels.is_neg()) return false;
+        return w.stride(1) == 1 && (w.size(0) == 1 || (w.stride(0) >= w.size(1) && w.stride(0) % 8 == 0)) && (uintptr_t)w.data_ptr() % 16 == 0;
+    }
+};
+
+struct LinearCrossEntropyBackward : public Node {
+    SavedVariable x_, w_, labels_, saved_;
+    int64_t ignore = 0;
+    int reduction = 0, keep = 0;
+    double scale = 1;
+
+    std::string name() const override { return "LinearCrossEntropyBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        x_.reset_data();
+        w_.reset_data();
+        labels_.reset_data();
+        saved_.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(2);
+        if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
+        const Tensor x = x_.unpack(), w = w_.unpack(), labels = labels_.unpack(), saved = saved_.unpack(shared_from_this());
+        c10::DeviceGuard guard(x.device());
+        const bool again = at::GradMode::is_enabled();
+        {
+            at::NoGradGuard no_grad;
+            const Tensor g = cast_to(grads[0], at::kFloat).contiguous();
+            const HeadLoss h(x, w, labels, ignore, reduction, scale);
+            const bool need_dx = task_should_compute_output(0), need_dw = task_should_compute_output(1);
+            if (need_dx) out[0] = empty_bf(x.sizes());
+            if (need_dw) out[1] = empty_bf(w.sizes());
+            Scratch ws(need_dw ? xq_lce_workspace_bytes(h.q.M, h.q.V, h.q.H, XQ_LCE_KEEP_HEAD_BWD) : 0);
+            check(xq_lce_bwd(&h.q, (const float*)g.data_ptr(), saved.data_ptr(), keep, need_dx ? out[0].data_ptr() : nullptr, h.q.H,
+                             need_dw ? out[1].data_ptr() : nullptr, h.q.H, need_dw ? ws.get() : nullptr, ws.bytes, stream_of(x)));
+        }
+        // a graph of the backward is being recorded: what comes out of it here cannot be differentiated, and says so if it is
+        if (again)
+            for (Tensor& t : out)
+                if (t.defined()) {
+                    auto error = std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy is differentiable once", 1);
+                    t = (*error)({t.detach().requires_grad_(true)})[0];
+                }
+        return out;
+    }
+};
+
 // the eleven buffers of xq_grouped_saved that a forward fills, in its order
 constexpr int kGroupedKept = 11;
 void grouped_saved(xq_grouped_saved* S, const Tensor* kept, const Rows* x) {
@@ -812,6 +878,48 @@ PyObject* moe(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// cross_entropy(x, weight, labels, ignore_index, reduction, logit_scale)
+PyObject* cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 6) { PyErr_SetString(PyExc_TypeError, "cross_entropy(x, weight, labels, ignore_index, reduction, logit_scale)"); return nullptr; }
+        const Tensor *x = plain(args[0]), *w = plain(args[1]), *labels = plain(args[2]);
+        if (under_transform() || !x || !w || !labels || !HeadLoss::takes(*x, *w, *labels)) XQ_NONE;
+        const int64_t ignore = PyLong_AsLongLong(args[3]);
+        if (ignore == -1 && PyErr_Occurred()) { PyErr_Clear(); XQ_NONE; }
+        const long reduction = PyLong_AsLong(args[4]);
+        const double scale = PyFloat_AsDouble(args[5]);
+        if (PyErr_Occurred()) { PyErr_Clear(); XQ_NONE; }
+        if (!(scale > 0.0) || !std::isfinite(scale)) XQ_NONE;
+        const bool grad = at::GradMode::is_enabled(), want_x = grad && x->requires_grad(), want_w = grad && w->requires_grad();
+        const int keep = want_x ? XQ_LCE_KEEP_DX : want_w ? XQ_LCE_KEEP_HEAD : XQ_LCE_KEEP_NONE;
+        c10::DeviceGuard guard(x->device());
+        Tensor loss, saved;
+        {
+            at::NoGradGuard no_grad;
+            const HeadLoss h(*x, *w, *labels, ignore, (int)reduction, scale);
+            loss = reduction == XQ_LCE_NONE ? empty_f32(labels->sizes()) : empty_f32({});
+            saved = empty({xq_lce_saved_bytes(h.q.M, h.q.V, h.q.H, keep)}, at::kByte);
+            Scratch ws(xq_lce_workspace_bytes(h.q.M, h.q.V, h.q.H, keep));
+            void* stream = stream_of(*x);
+            ReleaseGil nogil;
+            check(xq_lce_fwd(&h.q, (float*)loss.data_ptr(), saved.data_ptr(), keep, ws.get(), ws.bytes, stream));
+        }
+        if (!keep) return THPVariable_Wrap(std::move(loss));
+        auto node = std::shared_ptr<LinearCrossEntropyBackward>(new LinearCrossEntropyBackward(), torch::autograd::deleteNode);
+        node->set_next_edges(torch::autograd::collect_next_edges(*x, *w));
+        node->x_ = SavedVariable(*x, false);
+        node->w_ = SavedVariable(*w, false);
+        node->labels_ = SavedVariable(*labels, false);
+        node->saved_ = SavedVariable(saved, false);
+        node->ignore = ignore;
+        node->reduction = (int)reduction;
+        node->keep = keep;
+        node->scale = scale;
+        torch::autograd::set_history(loss, node);
+        return THPVariable_Wrap(std::move(loss));
+    });
+}
+
 // ---- the optimizer step: its arguments are hundreds of tensors, whose addresses and checks are a matter of tens of microseconds here
 struct TensorList {
     const char* name;
@@ -1009,6 +1117,7 @@ PyMethodDef methods[] = {
     {"linears", (PyCFunction)(void (*)())linears, METH_FASTCALL, nullptr},
     {"mlp", (PyCFunction)(void (*)())mlp, METH_FASTCALL, nullptr},
     {"moe", (PyCFunction)(void (*)())moe, METH_FASTCALL, nullptr},
+    {"cross_entropy", (PyCFunction)(void (*)())cross_entropy, METH_FASTCALL, nullptr},
     {"adamw", (PyCFunction)(void (*)())adamw, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

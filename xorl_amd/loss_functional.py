@@ -14,6 +14,7 @@ import torch
 from torch import Tensor
 
 from . import _C
+from ._native import native
 from .functional import _as_2d, _ld
 
 
@@ -118,6 +119,11 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
     Products accumulate in fp32, sums of exponentials in fp32 relative to the label's logit or the largest.  Gradients come in bf16; the
     probabilities in them are rounded to bf16 once (half a step, 2^-8, each), all but the label's.  H must be a multiple of 64.  First
     derivatives only."""
+    if not torch.compiler.is_compiling() and reduction in _C.LCE_REDUCTIONS:
+        loss = native().cross_entropy(x, weight, labels, ignore_index, _C.LCE_REDUCTIONS[reduction], logit_scale)
+        if loss is not None:
+            return loss
+    # what the native path leaves: copies of heads that are laid out otherwise, traced calls, and the errors
     if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise _C.XqError(f"linear_cross_entropy: x and weight must be bf16, got {x.dtype} and {weight.dtype}")
     if labels.dtype not in (torch.int64, torch.int32):
