@@ -459,7 +459,8 @@ struct LceProductArgs {
     const int32_t* count;
     const bf16_t* B;                    // [k, H]
     int64_t ldb;
-    int32_t H, cus;                     // cus: compute units to divide the contraction for, or 0: it is not divided
+    int32_t H;
+    const int32_t* parts;               // of the contraction, or NULL: it is not divided
     float* out;                         // [part of the contraction][row][H]: sums, added to what is there where `add`, that times alpha[row]
     const float* alpha;                 // (of row tiles that were done again; 1 otherwise)
     const int32_t* redo;
@@ -469,18 +470,17 @@ struct LceProductArgs {
 };
 
 // Parts of a contraction of E . W: as many as leave the least of the chip idle, where tiles alone would (a part costs its sums once more in
-// memory: 2 % a part).  The rows that count are known on the device only, so that every kernel works it out for itself.  Divided, tiles and
-// parts are three rounds of the chip at most, which bounds the sums.
+// memory: 2 % a part).  The rows that count are known on the device only, so that the kernel that counts them works it out, a wave with
+// a number of parts in each lane.  Divided, tiles and parts are three rounds of the chip at most, which bounds the sums.
 constexpr int kLceSplitRounds = 3, kLceMostParts = 64;
-__host__ __device__ inline int lce_parts(int tiles, int steps, int cus) {
-    int best = 1;
-    float least = 1e30f;
-    for (int s = 1; s <= kLceMostParts; ++s) {
-        if (s > 1 && (tiles * s > kLceSplitRounds * cus || steps < 16 * s)) break;
-        const float cost = (float)((tiles * s + cus - 1) / cus) / (float)s * (1.0f + 0.02f * (float)(s - 1));
-        if (cost < 0.999f * least) { least = cost; best = s; }
-    }
-    return best;
+__device__ __forceinline__ int lce_parts(int tiles, int steps, int slots, int lane) {
+    const int s = lane + 1, all = tiles * s;
+    const bool may = s == 1 || (all <= kLceSplitRounds * slots && steps >= 16 * s);
+    const float cost = may ? (float)((all + slots - 1) / slots) / (float)s * (1.0f + 0.02f * (float)(s - 1)) : INFINITY;
+    float least = cost;
+#pragma unroll
+    for (int d = 1; d < 64; d <<= 1) least = fminf(least, __shfl_xor(least, d));
+    return __builtin_ctzll(__ballot(cost <= least * 1.001f)) + 1;
 }
 
 template <int TM>
@@ -489,9 +489,9 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
     extern __shared__ __attribute__((aligned(16))) unsigned char dsm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
-    const int rows = g.rows < 0 ? *g.count : g.rows, k = g.k < 0 ? *g.count : g.k;
+    const int count = __builtin_amdgcn_readfirstlane(*g.count), rows = g.rows < 0 ? count : g.rows, k = g.k < 0 ? count : g.k;
     const int tiles_a = (rows + T::ROWS - 1) / T::ROWS, tiles_b = (g.H + 255) >> 8, tiles = tiles_a * tiles_b, pairs = (k + 63) >> 6;        // of K-steps
-    const int parts = g.cus ? lce_parts(tiles, g.image_steps, g.cus) : 1;
+    const int parts = g.parts ? __builtin_amdgcn_readfirstlane(*g.parts) : 1;
     // an XCD has an eighth of all tiles and parts, in order of the parts: what it reads of E and W at a time are few rows and the same K-steps
     const int all = tiles * parts, b = blockIdx.x, per = all >> 3;
     if (b >= all) return;

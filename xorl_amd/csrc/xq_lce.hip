@@ -42,6 +42,7 @@ struct Prep {
     int32_t* redo;                                  // flags to clear
     int32_t n_redo;
     float* loss_out;                                // losses by row, 0 for those that do not count; or NULL
+    int32_t tile_rows, tiles_h, steps, slots;       // of E . W, for the parts of its contraction (count[1])
 };
 __device__ __forceinline__ int64_t label_of(const Prep& a, int64_t i) {
     if (i >= a.M) return a.ignore;
@@ -76,7 +77,13 @@ __device__ __forceinline__ void write_row(const Prep& a, int64_t i, int64_t labe
     }
 }
 __device__ __forceinline__ void write_rest(const Prep& a, int n) {
-    if (threadIdx.x == 0) *a.count = n;
+    if (threadIdx.x < 64) {
+        const int parts = lce_parts((n + a.tile_rows - 1) / a.tile_rows * a.tiles_h, a.steps, a.slots, threadIdx.x);
+        if (threadIdx.x == 0) {
+            a.count[0] = n;
+            a.count[1] = parts;
+        }
+    }
     for (int64_t c = n + threadIdx.x; c < a.M_pad; c += 1024) {
         a.row[c] = 0;
         a.label[c] = -1;
@@ -271,34 +278,32 @@ __device__ __forceinline__ float upstream(const Upstream& u, int64_t row) {
     return u.reduction == XQ_LCE_MEAN ? g / (float)*u.count : g;
 }
 
-// dx: a block has rows of x, a thread 8 columns at a time
-__global__ void __launch_bounds__(256) lce_dx_kernel(const int32_t* place, const int32_t* label, int64_t M, int H, const float* o, int tile_rows, int steps, int cus,
-                                                     const float* inv, const float* rest, const bf16_t* w, int64_t ldw, Upstream u, bf16_t* dx, int64_t lddx) {
+// dx: a block has 512 columns of a row of x, a thread 8 of them
+__global__ void __launch_bounds__(64) lce_dx_kernel(const int32_t* place, const int32_t* label, int H, const float* o,
+                                                    const float* inv, const float* rest, const bf16_t* w, int64_t ldw, Upstream u, bf16_t* dx, int64_t lddx) {
     const int64_t i = blockIdx.x;
+    const int k = blockIdx.y * 512 + threadIdx.x * 8;
+    if (k >= H) return;
     const int c = place[i];
-    bf16_t* out = dx + i * lddx;
+    u32x4* out = (u32x4*)(dx + i * lddx + k);
     if (c < 0) {
-        for (int k = threadIdx.x * 8; k < H; k += 2048) *(u32x4*)(out + k) = u32x4{0, 0, 0, 0};
+        *out = u32x4{0, 0, 0, 0};
         return;
     }
+    const int t = label[c], count = u.count[0], parts = u.count[1];
+    const u32x4 wt = *(const u32x4*)(w + max(t, 0) * ldw + k);
     const float g = upstream(u, i);
-    const float a = g * inv[c], b = label[c] < 0 ? __builtin_nanf("") : g * rest[c];
-    const bf16_t* wr = w + max(label[c], 0) * ldw;
-    const float* oc = o + (int64_t)c * H;
-    const int count = *u.count, parts = lce_parts((count + tile_rows - 1) / tile_rows * ((H + 255) >> 8), steps, cus);
-    const int64_t split_stride = (int64_t)count * H;
-    for (int k = threadIdx.x * 8; k < H; k += 2048) {
-        const u32x4 t = *(const u32x4*)(wr + k);
-        f32x4 lo = *(const f32x4*)(oc + k), hi = *(const f32x4*)(oc + k + 4);
-        for (int s = 1; s < parts; ++s) {
-            lo += *(const f32x4*)(oc + s * split_stride + k);
-            hi += *(const f32x4*)(oc + s * split_stride + k + 4);
-        }
-        const f32x4 tl = bf16x4_f32(u32x2{t[0], t[1]}), th = bf16x4_f32(u32x2{t[2], t[3]});
-        lo = lo * a - tl * b;
-        hi = hi * a - th * b;
-        *(u32x4*)(out + k) = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
+    const float a = g * inv[c], b = t < 0 ? __builtin_nanf("") : g * rest[c];
+    const float* oc = o + (int64_t)c * H + k;
+    f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
+#pragma unroll 4
+    for (int s = 0; s < parts; ++s) {
+        lo += *(const f32x4*)(oc + s * (int64_t)count * H);
+        hi += *(const f32x4*)(oc + s * (int64_t)count * H + 4);
     }
+    lo = lo * a - bf16x4_f32(u32x2{wt[0], wt[1]}) * b;
+    hi = hi * a - bf16x4_f32(u32x2{wt[2], wt[3]}) * b;
+    *out = u32x4{pack_bf16x2(lo[0], lo[1]), pack_bf16x2(lo[2], lo[3]), pack_bf16x2(hi[0], hi[1]), pack_bf16x2(hi[2], hi[3])};
 }
 
 // the factors of the head's gradient by row, and the rows of x that count in order
@@ -374,7 +379,7 @@ int64_t sums_bytes(const Plan& p, int64_t M, int64_t H) {
 
 // what a forward leaves for the backward
 struct Saved {
-    int32_t *count, *row, *label, *place;
+    int32_t *count, *row, *label, *place;       // count[1]: parts of the contraction of E . W
     float *at_label, *inv, *rest, *lse2, *loss, *o;
     int64_t bytes;
 };
@@ -383,7 +388,7 @@ Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
     uint8_t* at = (uint8_t*)base;
     auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
     Saved s;
-    s.count = (int32_t*)take(4);
+    s.count = (int32_t*)take(8);
     s.row = (int32_t*)take(4 * p.rows_pad);
     s.label = (int32_t*)take(4 * p.rows_pad);
     s.place = (int32_t*)take(4 * p.rows_pad);
@@ -448,7 +453,7 @@ int launch_product(const LceProductArgs& a, int64_t rows, hipStream_t s) {
     static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
     if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
     int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(a.H, 256);
-    if (a.cus) blocks = std::max<int64_t>(blocks, std::min<int64_t>(kLceMostParts * blocks, (int64_t)kLceSplitRounds * a.cus));
+    if (a.parts) blocks = std::max<int64_t>(blocks, std::min<int64_t>(kLceMostParts * blocks, (int64_t)kLceSplitRounds * slots(TM)));
     k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
     return XQ_OK;
 }
@@ -503,7 +508,8 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
     const RowEnd end = {s.inv, s.rest, s.lse2, s.loss, s.row, none ? loss : nullptr};
     const Prep prep = {q->labels, q->label_bytes, M, p.rows_pad, V, q->ignore_index, s.count, s.row, s.label, s.place,
                        keep == XQ_LCE_KEEP_DX ? nullptr : s.at_label, c.redo,
-                       keep == XQ_LCE_KEEP_DX ? (int32_t)(p.pieces * row_tiles) : 0, none ? loss : nullptr};
+                       keep == XQ_LCE_KEEP_DX ? (int32_t)(p.pieces * row_tiles) : 0, none ? loss : nullptr,
+                       32 * p.tm, (int32_t)xq_cdiv(H, 256), (int32_t)(p.piece / 32), slots(p.tm)};
     const dim3 by16((unsigned)xq_cdiv(M, 16));
     Join join = {s.count, c.part, p.rows_pad, 0, 32 * p.tm, c.ref, c.z, c.new_ref, c.alpha, nullptr};
     LceLogitsArgs a = {};
@@ -529,7 +535,7 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
             else lce_end_kernel<<<by16, 1024, 0, st>>>(join, s.at_label, end);
             LceProductArgs o = {};
             o.image = c.image; o.image_steps = a.image_steps; o.rows = -1; o.k = (int32_t)n; o.count = s.count;
-            o.B = a.B + v0 * a.ldb; o.ldb = a.ldb; o.H = (int32_t)H; o.cus = slots(p.tm);
+            o.B = a.B + v0 * a.ldb; o.ldb = a.ldb; o.H = (int32_t)H; o.parts = s.count + 1;
             o.out = s.o; o.alpha = c.alpha; o.redo = a.redo; o.add = v0 > 0;
             if ((rc = launch_product(p.tm, o, M, st)) != XQ_OK) return rc;
         }
@@ -551,12 +557,11 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
     XQ_REQUIRE(!dw || (xq_aligned(dw, 16) && lddw >= q->H && lddw % 8 == 0), "xq_lce_bwd: dw must be 16-byte aligned with a row stride that is a multiple of 8 elements");
     hipStream_t st = (hipStream_t)stream;
     const int64_t M = q->M, V = q->V, H = q->H;
-    const Plan p = plan_tokens(M, V, keep);
     const Saved s = saved_of((void*)saved, M, V, H, keep);
     const LceRows rows = {s.count, s.row, s.label};
     const Upstream u = {grad, q->reduction, s.count, q->logit_scale};
     if (dx && M > 0)
-        lce_dx_kernel<<<dim3((unsigned)M), 256, 0, st>>>(s.place, s.label, M, (int)H, s.o, 32 * p.tm, (int)(p.piece / 32), slots(p.tm), s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
+        lce_dx_kernel<<<dim3((unsigned)M, (unsigned)xq_cdiv(H, 512)), 64, 0, st>>>(s.place, s.label, (int)H, s.o, s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
     if (dw) {
         const Plan h = plan_head(M, V);
         const Scratch c = scratch_of(workspace, M, V, H, XQ_LCE_KEEP_HEAD_BWD);
