@@ -6,9 +6,9 @@
 //   GRAD    A the head, B the tokens: G = g_i (p_iv - [v = t_i]) as a bf16 image with the tokens along the contraction
 // lce_product_kernel  C = image . B, B with the contraction across its rows: E . W (input gradients), G . X (the head's)
 //
-//  * Tiles of 32 TM x 256, K-steps of 32, four LDS stages filled by direct-to-LDS loads, eight waves of 16 TM x 64 on
-//    v_mfma_f32_16x16x32_bf16.  In iteration kt every wave reads stages kt and kt + 1 and fills stage kt + 3; the loads of kt + 2 are waited
-//    for at its end.  A K-step is TM chunks of four MFMAs; a chunk's fragment of A is read three chunks ahead, the fragments of B a
+//  * Tiles of 32 TM x 64 TN, K-steps of 32, LDS stages (four or eight) filled by direct-to-LDS loads, eight waves of 16 TM x 16 TN on
+//    v_mfma_f32_16x16x32_bf16.  In iteration kt every wave reads stages kt and kt + 1 and fills stage kt + 3 (or kt + 7); the loads of
+//    kt + 2 are waited for at its end.  A K-step is TM chunks of TN MFMAs; a chunk's fragment of A is read three chunks ahead, the fragments of B a
 //    K-step ahead (two register sets).  Loads behind the last K-step repeat it, so that every iteration is the same.
 //  * Stage.  A: [row][32 k], the 16-byte chunk c of a row at c ^ ((row >> 2) & 2): 16 rows x 4 chunks meet no bank twice.  B of
 //    the logits the same.  B of the product: [32 k][256 columns], the 32-byte unit u of row k at u ^ (k & 7); fragments come out by
@@ -24,17 +24,18 @@ namespace xq {
 
 enum { kLceStats = 0, kLceExp = 1, kLceGrad = 2 };
 
-template <int TM>
+template <int TM, int TN = 4, int ST = 4>
 struct LceTile {
-    static constexpr int ROWS = 32 * TM, COLS = 256, BK = 32, STAGES = 4;
+    static constexpr int ROWS = 32 * TM, COLS = 64 * TN, BK = 32, STAGES = ST;
     static constexpr int A_BYTES = ROWS * 64, B_BYTES = COLS * 64, STAGE_BYTES = A_BYTES + B_BYTES;
-    static constexpr int AP = (ROWS / 8 + 15) / 16, BP = 2, NP = AP + BP;        // direct loads of a wave and K-step: 16 rows of 64 bytes each
+    static constexpr int AP = (ROWS / 8 + 15) / 16, BP = COLS / 128, NP = AP + BP;       // direct loads of a wave and K-step: 16 rows of 64 bytes each
     // a block goes on to its next tile, whose first K-steps are on their way while the ends of this one are computed; 64 rows: two blocks
     // of one tile each share a compute unit instead
     static constexpr bool AHEAD = TM >= 4;
     static constexpr int END_BYTES = ROWS * 32 + 1024 * 4;      // of the ends: sums by row and wave; four numbers by row or column
     static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + (AHEAD ? END_BYTES : 0);
     static_assert(AHEAD || END_BYTES <= STAGES * STAGE_BYTES, "the ends reuse the stages");
+    static_assert((STAGES & (STAGES - 1)) == 0 && LDS_BYTES <= 160 * 1024, "stages are taken in turn");
 };
 
 struct LceRows {                        // what is kept of the labels: the rows that count, in order
@@ -66,39 +67,39 @@ struct LceLogitsArgs {
 };
 constexpr float kLceFar = 64.0f;        // log2
 
-// The first three of a stream of K-steps: K-step k of it goes to stage k & 3.  issue(at, part, stage): one of NP direct loads of a K-step.
-template <int TM, typename Advance, typename Issue>
+// The first of a stream of K-steps, all stages but one: K-step k of it goes to stage k % STAGES.  issue(at, part, stage): one of NP direct loads of a K-step.
+template <typename T, typename Advance, typename Issue>
 __device__ __forceinline__ void lce_begin(unsigned char* dsm, Advance advance, Issue issue) {
-    using T = LceTile<TM>;
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)dsm;
 #pragma unroll
-    for (int kt = 0; kt < 3; ++kt) {
+    for (int kt = 0; kt < T::STAGES - 1; ++kt) {
         const int at = advance(kt);
 #pragma unroll
         for (int part = 0; part < T::NP; ++part) issue(at, part, lds0 + kt * T::STAGE_BYTES);
     }
-    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(T::NP) : "memory");
+    asm volatile("s_waitcnt vmcnt(%0)" :: "n"(T::NP * (T::STAGES - 3)) : "memory");
     __builtin_amdgcn_s_barrier();
     asm volatile("" ::: "memory");
 }
 
 // C[r, n] over the stream's K-steps first .. first + nk - 1 (an even number, not 0), the first two of which have landed; the same holds of the
 // two behind them in the end.  advance(k): what issue is to be told for the tile's K-step k, which goes on behind the last.
-template <int TM, bool BT, typename Advance, typename Issue>
-__device__ __forceinline__ void lce_run(f32x4 (&acc)[TM][4], unsigned char* dsm, int first, int nk, int wave, int lane, Advance advance, Issue issue) {
-    using T = LceTile<TM>;
-    constexpr int NC = TM, LA = NC < 3 ? NC : 3, FB = NC < 4 ? 4 / NC : 1;
+template <int TM, int TN, int ST, bool BT, typename Advance, typename Issue>
+__device__ __forceinline__ void lce_run(f32x4 (&acc)[TM][TN], unsigned char* dsm, int first, int nk, int wave, int lane, Advance advance, Issue issue) {
+    using T = LceTile<TM, TN, ST>;
+    constexpr int NC = TM, LA = NC < 3 ? NC : 3, FB = (TN + NC - 1) / NC, D = ST - 1;
+    static_assert(!BT || TN == 4, "the transposed stage is 256 columns wide");
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
     const int sw = (l16 >> 2) & 2;
     const int a_at = (wm * 16 * TM + l16) * 64 + ((lg ^ sw) << 4);
-    int b_at[4];
+    int b_at[TN];
 #pragma unroll
-    for (int j = 0; j < 4; ++j) {
+    for (int j = 0; j < TN; ++j) {
         if constexpr (BT) {
             const int k = 4 * lg + (l16 >> 2);
             b_at[j] = T::A_BYTES + k * 512 + (((wn * 4 + j) ^ (k & 7)) << 5) + (l16 & 3) * 8;
         } else {
-            b_at[j] = T::A_BYTES + (wn * 64 + j * 16 + l16) * 64 + ((lg ^ sw) << 4);
+            b_at[j] = T::A_BYTES + (wn * 16 * TN + j * 16 + l16) * 64 + ((lg ^ sw) << 4);
         }
     }
     auto read_a = [&](const unsigned char* stage, int c) -> bf16x8 { return *(const bf16x8*)(stage + a_at + c * 1024); };
@@ -117,37 +118,37 @@ __device__ __forceinline__ void lce_run(f32x4 (&acc)[TM][4], unsigned char* dsm,
 #pragma unroll
     for (int i = 0; i < TM; ++i)
 #pragma unroll
-        for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < TN; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     const uint32_t lds0 = (uint32_t)(uintptr_t)(__attribute__((address_space(3))) unsigned char*)dsm;
-    bf16x8 fa[4], fb[2][4];
+    bf16x8 fa[4], fb[2][TN];
     {
-        const unsigned char* stage = dsm + (first & 3) * T::STAGE_BYTES;
+        const unsigned char* stage = dsm + (first & D) * T::STAGE_BYTES;
 #pragma unroll
-        for (int j = 0; j < 4; ++j) fb[0][j] = read_b(stage, j);
+        for (int j = 0; j < TN; ++j) fb[0][j] = read_b(stage, j);
 #pragma unroll
         for (int c = 0; c < LA; ++c) fa[c] = read_a(stage, c);
     }
     auto iteration = [&](int kt, auto P_) {
         constexpr int P = decltype(P_)::value;
-        const unsigned char* here = dsm + ((first + kt) & 3) * T::STAGE_BYTES;
-        const unsigned char* next = dsm + ((first + kt + 1) & 3) * T::STAGE_BYTES;
-        const uint32_t fill = lds0 + ((first + kt + 3) & 3) * T::STAGE_BYTES;
-        const int ahead = advance(kt + 3);
+        const unsigned char* here = dsm + ((first + kt) & D) * T::STAGE_BYTES;
+        const unsigned char* next = dsm + ((first + kt + 1) & D) * T::STAGE_BYTES;
+        const uint32_t fill = lds0 + ((first + kt + D) & D) * T::STAGE_BYTES;
+        const int ahead = advance(kt + D);
 #pragma unroll
         for (int c = 0; c < NC; ++c) {
             const int at = (P * NC + c) & 3;
 #pragma unroll
-            for (int j = 0; j < 4; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[P][j], fa[at], acc[c][j], 0, 0, 0);
+            for (int j = 0; j < TN; ++j) acc[c][j] = __builtin_amdgcn_mfma_f32_16x16x32_bf16(fb[P][j], fa[at], acc[c][j], 0, 0, 0);
             fa[(at + LA) & 3] = c + LA < NC ? read_a(here, c + LA) : read_a(next, c + LA - NC);
 #pragma unroll
             for (int q = 0; q < FB; ++q)
-                if (c * FB + q < 4) fb[P ^ 1][c * FB + q] = read_b(next, c * FB + q);
+                if (c * FB + q < TN) fb[P ^ 1][c * FB + q] = read_b(next, c * FB + q);
 #pragma unroll
             for (int part = c * T::NP / NC; part < (c + 1) * T::NP / NC; ++part) issue(ahead, part, fill);
             __builtin_amdgcn_sched_barrier(0);
         }
         // K-step kt + 2 has landed
-        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(T::NP) : "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" :: "n"(T::NP * (ST - 3)) : "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
         __builtin_amdgcn_sched_barrier(0);
@@ -206,9 +207,10 @@ __device__ __forceinline__ float over_groups_sum(float v) {
     return __uint_as_float(b[0]) + __uint_as_float(b[1]);
 }
 
-template <int TM, int MODE>
+template <int TM, int TN, int ST, int MODE>
 __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLogitsArgs g) {
-    using T = LceTile<TM>;
+    using T = LceTile<TM, TN, ST>;
+    static_assert(MODE != kLceGrad || TN == 4, "what the ends keep of 256 columns");
     extern __shared__ __attribute__((aligned(16))) unsigned char dsm[];
     unsigned char* const ends = T::AHEAD ? dsm + T::STAGES * T::STAGE_BYTES : dsm;
     f32x2* const sums = (f32x2*)ends;                       // [row][wave column]
@@ -217,7 +219,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
     const int count = __builtin_amdgcn_readfirstlane(*g.rows.count);
     const int n_a = MODE == kLceGrad ? g.n_v : count, n_b = MODE == kLceGrad ? count : g.n_v;
-    const int tiles_a = (n_a + T::ROWS - 1) / T::ROWS, cols = MODE == kLceGrad || TM > 4 ? 256 : g.cols, tiles_b = (n_b + cols - 1) / cols, nk = g.H / T::BK;
+    const int tiles_a = (n_a + T::ROWS - 1) / T::ROWS, cols = MODE == kLceGrad || TM > 4 ? 256 : min(g.cols, T::COLS), tiles_b = (n_b + cols - 1) / cols, nk = g.H / T::BK;
 
     LceWalk walk(tiles_a * tiles_b);
     int ta, tb;
@@ -235,7 +237,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
 #pragma unroll
         for (int p = 0; p < T::NP; ++p) {
             const bool of_a = p < T::AP;
-            const int rt = of_a ? wave * (T::ROWS / 8) + p * 16 + (lane >> 2) : wave * 32 + (p - T::AP) * 16 + (lane >> 2);
+            const int rt = of_a ? wave * (T::ROWS / 8) + p * 16 + (lane >> 2) : wave * (T::COLS / 8) + (p - T::AP) * 16 + (lane >> 2);
             // (rows behind the last, of either side or of the tile's columns: that one again, for nothing)
             const int n = of_a ? min(ta * T::ROWS + rt, n_a - 1) : min(tb * cols + min(rt, cols - 1), n_b - 1);
             const bool tokens = of_a != (MODE == kLceGrad);
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     const bf16_t* src_next[T::NP];
     auto issue = [&](int at, int part, uint32_t stage) {
         const bool of_a = part < T::AP;
-        const int p = of_a ? part : part - T::AP, rows = of_a ? T::ROWS / 8 : 32;
+        const int p = of_a ? part : part - T::AP, rows = (of_a ? T::ROWS : T::COLS) / 8;
         const uint32_t dst = stage + (of_a ? 0 : T::A_BYTES) + wave * rows * 64 + p * 1024;
         if (p * 16 + 16 <= rows || lane < (rows - p * 16) * 4) lce_load_lds(dst, src[part] + at * T::BK);
     };
@@ -295,10 +297,10 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
         return k < nk ? k : k - nk;
     };
     if (!find()) return;
-    const bool stream = T::AHEAD && nk >= 4;                // (two K-steps: a tile's end is nearer than the loads are ahead)
+    const bool stream = T::AHEAD && nk >= ST;               // (fewer: a tile's end is nearer than the loads are ahead)
     sources(src, about);
     turned = turn(tb);
-    lce_begin<TM>(dsm, advance, issue);
+    lce_begin<T>(dsm, advance, issue);
     if (T::AHEAD) note(about);
     int first = 0;
     do {
@@ -311,8 +313,8 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                 turned_next = turn(tb);
             }
         }
-        f32x4 acc[TM][4];
-        lce_run<TM, false>(acc, dsm, first, nk, wave, lane, advance, issue);
+        f32x4 acc[TM][TN];
+        lce_run<TM, TN, ST, false>(acc, dsm, first, nk, wave, lane, advance, issue);
         first += nk;
         if (!stream) {
             lce_loads_done();
@@ -321,11 +323,11 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             __syncthreads();
         }
 
-        // ---- lane (l16, lg) holds rows r0 + wm 16 TM + 16 i + l16, columns c0 + 64 wn + 16 j + 4 lg + 0..3
-        const int row_w = wm * 16 * TM + l16, col_w = wn * 64 + 4 * lg;
+        // ---- lane (l16, lg) holds rows r0 + wm 16 TM + 16 i + l16, columns c0 + 16 TN wn + 16 j + 4 lg + 0..3
+        const int row_w = wm * 16 * TM + l16, col_w = wn * 16 * TN + 4 * lg;
         if constexpr (MODE == kLceGrad) {
 #pragma unroll
-            for (int j = 0; j < 4; ++j) {
+            for (int j = 0; j < TN; ++j) {
                 const int c = col_w + 16 * j;
                 const f32x4 label = *(const f32x4*)(info + c), lse = *(const f32x4*)(info + 256 + c), up = *(const f32x4*)(info + 512 + c), rest = *(const f32x4*)(info + 768 + c);
 #pragma unroll
@@ -341,11 +343,11 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
         } else {
             // columns that the piece does not have, and the label's, count as -inf
             const int end = min(cols, g.n_v - c0);
-            if (end < 256) {
+            if (end < T::COLS) {
 #pragma unroll
                 for (int i = 0; i < TM; ++i)
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < TN; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (col_w + 16 * j + e >= end) acc[i][j][e] = -INFINITY;
@@ -353,12 +355,12 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             float ref[TM], top[TM], sum[TM];
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
-                int at = __float_as_int(info[row_w + 16 * i]) - c0 - col_w;           // the label's column by the lane's own numbering of its 16
+                int at = __float_as_int(info[row_w + 16 * i]) - c0 - col_w;           // the label's column by the lane's own numbering of its 4 TN
                 if (col_w + at >= end) at = -1;
                 if (MODE == kLceExp) ref[i] = info[N_INFO + row_w + 16 * i];
-                if (__any(at >= 0 && at < 52)) {
+                if (__any(at >= 0 && at < 16 * TN - 12)) {
 #pragma unroll
-                    for (int j = 0; j < 4; ++j)
+                    for (int j = 0; j < TN; ++j)
 #pragma unroll
                         for (int e = 0; e < 4; ++e)
                             if (at == 16 * j + e) {
@@ -371,7 +373,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             for (int i = 0; i < TM; ++i) {
                 top[i] = acc[i][0][0];
 #pragma unroll
-                for (int j = 0; j < 4; ++j) top[i] = max3(max3(top[i], acc[i][j][0], acc[i][j][1]), acc[i][j][2], acc[i][j][3]);
+                for (int j = 0; j < TN; ++j) top[i] = max3(max3(top[i], acc[i][j][0], acc[i][j][1]), acc[i][j][2], acc[i][j][3]);
             }
 #pragma unroll
             for (int i = 0; i < TM; ++i) top[i] = over_groups_max(top[i]) * g.scale2;
@@ -382,7 +384,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                 if (MODE == kLceExp) far |= top[i] - base > kLceFar;
                 f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-                for (int j = 0; j < 4; ++j) {
+                for (int j = 0; j < TN; ++j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], g.scale2, -base));
                     s += acc[i][j];
@@ -414,15 +416,15 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             }
         }
         if constexpr (MODE != kLceStats) {
-            bf16_t* out = g.image + ((int64_t)this_a * g.image_steps + (c0 >> 5) + wn * 2) * (T::ROWS * 32);
+            bf16_t* out = g.image + ((int64_t)this_a * g.image_steps + (c0 >> 5) + wn * (TN / 2)) * (T::ROWS * 32);
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 const int row = row_w + 16 * i;
 #pragma unroll
-                for (int q = 0; q < 2; ++q) {
+                for (int q = 0; q < TN / 2; ++q) {
                     if (TM <= 4) {
                         // the next tile's;  (the last tile goes on to the end of the image: the product takes K-steps in pairs)
-                        const int step = wn * 2 + q;
+                        const int step = wn * (TN / 2) + q;
                         if ((step * 32 >= cols && this_b + 1 < tiles_b) || (c0 >> 5) + step >= g.image_steps) continue;
                     }
                     const f32x4 a = acc[i][2 * q], b = acc[i][2 * q + 1];
@@ -440,7 +442,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                 sources(src, about);
                 turned = turn(tb);
                 __syncthreads();
-                lce_begin<TM>(dsm, advance, issue);
+                lce_begin<T>(dsm, advance, issue);
                 note(about);
                 __syncthreads();
                 first = 0;
@@ -523,8 +525,8 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
     f32x4 acc[TM][4];
     if (nk > 0) {
         auto advance = [&](int kt) { return min(kt, nk - 1); };         // (behind the last K-step: that one again, for nothing)
-        lce_begin<TM>(dsm, advance, issue);
-        lce_run<TM, true>(acc, dsm, 0, nk, wave, lane, advance, issue);
+        lce_begin<T>(dsm, advance, issue);
+        lce_run<TM, 4, 4, true>(acc, dsm, 0, nk, wave, lane, advance, issue);
         lce_loads_done();
     } else {
 #pragma unroll

@@ -431,10 +431,10 @@ Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
     return s;
 }
 
-template <int TM, int MODE>
+template <int TM, int TN, int ST, int MODE>
 int launch_logits(const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_t s) {
-    using T = LceTile<TM>;
-    auto k = lce_logits_kernel<TM, MODE>;
+    using T = LceTile<TM, TN, ST>;
+    auto k = lce_logits_kernel<TM, TN, ST, MODE>;
     static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
     if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
     int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(cols, a.cols);
@@ -442,9 +442,12 @@ int launch_logits(const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_
     k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
     return XQ_OK;
 }
+// tokens as rows.  Up to 128 columns a tile: eight stages, as a unit with one block reads no faster than its loads in flight allow
 template <int MODE>
 int launch_logits(int tm, const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_t s) {
-    return tm == 2 ? launch_logits<2, MODE>(a, rows, cols, s) : tm == 4 ? launch_logits<4, MODE>(a, rows, cols, s) : launch_logits<8, MODE>(a, rows, cols, s);
+    if (tm == 2) return a.cols <= 128 ? launch_logits<2, 2, 8, MODE>(a, rows, cols, s) : launch_logits<2, 4, 4, MODE>(a, rows, cols, s);
+    if (tm == 4) return a.cols <= 128 ? launch_logits<4, 2, 8, MODE>(a, rows, cols, s) : launch_logits<4, 4, 4, MODE>(a, rows, cols, s);
+    return launch_logits<8, 4, 4, MODE>(a, rows, cols, s);
 }
 template <int TM>
 int launch_product(const LceProductArgs& a, int64_t rows, hipStream_t s) {
@@ -576,7 +579,7 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
         for (int64_t v0 = 0; v0 < V; v0 += h.piece) {
             const int64_t n = std::min(h.piece, V - v0);
             a.first_v = (int32_t)v0; a.n_v = (int32_t)n;
-            if (M > 0 && (rc = launch_logits<8, kLceGrad>(a, n, M, st)) != XQ_OK) return rc;
+            if (M > 0 && (rc = launch_logits<8, 4, 4, kLceGrad>(a, n, M, st)) != XQ_OK) return rc;
             LceProductArgs o = {};
             o.image = c.image; o.image_steps = a.image_steps; o.rows = (int32_t)n; o.k = -1; o.count = s.count;
             o.B = c.x; o.ldb = H; o.H = (int32_t)H;
