@@ -128,7 +128,7 @@ def test_step_by_type_and_alignment(hip_device, bits, pdt, gdt, offset):
 
 
 @pytest.mark.parametrize("bits", [32, 8])
-@pytest.mark.parametrize("count", [52, 53, 64, 65, 200, 4200])
+@pytest.mark.parametrize("count", [63, 64, 65, 84, 85, 200, 4200])
 def test_step_over_many_tensors(hip_device, bits, count):
     shapes = [((i * 37) % 300 + 1,) if i % 50 else (9001,) for i in range(count)]
     prob = _problem(shapes, bits, torch.float32, torch.float32, 5, hip_device)
@@ -171,6 +171,14 @@ def test_grad_norm(hip_device, gdt):
     big = [torch.full((5000,), 1e30, device=hip_device)]
     assert abs(float(grad_norm(big)) / (1e30 * 5000 ** 0.5) - 1) < 1e-6           # squares beyond fp32
     assert float(grad_norm([torch.zeros(0, device=hip_device)])) == 0.0
+
+
+@pytest.mark.parametrize("count", [1, 251, 252, 253, 3000])
+def test_grad_norm_over_many_tensors(hip_device, count):
+    g = torch.Generator(device=hip_device).manual_seed(count)
+    grads = [torch.randn((i * 53) % 9000 + 1, device=hip_device, generator=g).to(torch.bfloat16 if i % 3 == 0 else torch.float32) for i in range(count)]
+    want = sum(float(x.double().square().sum()) for x in grads) ** 0.5
+    assert abs(float(grad_norm(grads)) - want) <= (U + 1e-10) * want
 
 
 @pytest.mark.parametrize("bits", [32, 8])

@@ -12,7 +12,7 @@
 //
 // Bound by memory: 28 bytes an element (fp32 parameters and gradients, 32-bit states) or 16.06 (8-bit ones).  The factors of a model are
 // hundreds of tensors of 10^4 to 10^6 elements.  Their addresses change from step to step (autograd allocates gradients), so a call takes
-// them by value: adamw_table_kernel's arguments carry up to 52 tensors a launch, and it writes them into a table in the workspace, with the
+// them by value: adamw_table_kernel's arguments carry 63 to 252 tensors a launch, and it writes them into a table in the workspace, with the
 // step counts advanced and the bias corrections in 64 bits.  One launch then walks all tensors: chunks of 4096 elements, numbered through,
 // are dealt out to the blocks in ranges; a block looks its first chunk up in the table (two steps of 64 lanes) and goes on from there.
 #include <algorithm>
@@ -27,7 +27,7 @@ namespace {
 constexpr int kBlock = 256;                 // elements that share a scale: a wave's four a lane
 constexpr int kChunk = 4096;                // of a thread block at a time: four 256-element pieces of each of its waves
 constexpr int kThreads = 256;
-constexpr int kTableArgs = 52;              // tensors by value in one launch: 3744 of the 4096 bytes that arguments may take
+constexpr int kTableWords = 504;            // of tensors by value in one launch: 4032 bytes, of the 4096 that arguments may take
 constexpr int kNormBlocks = 2048;
 constexpr int kStepBlocks = 2048;           // eight of a compute unit
 
@@ -44,38 +44,54 @@ struct Row {                                // what the walking kernels read of 
     int32_t param16, grad16;                // bf16 (otherwise fp32)
 };
 
+// A tensor in 2 words (its gradient alone), 6 (with 32-bit states) or 8: gradient, elements with the types in the top bits; parameter, states
+// and step count; scales.
 struct TableArgs {
-    xq_adamw_tensor t[kTableArgs];
-};
-
-struct TableScalars {
+    uint64_t word[kTableWords];
     Row* rows;
-    int64_t chunk0;
-    int32_t n, at, step;                    // step: advance the step counts
+    int32_t chunk0, n;
+};
+struct TableScalars {
     double lr, log_beta1, log_beta2;
     const float* lr_device;
 };
+static_assert(sizeof(TableArgs) + sizeof(TableScalars) <= 4096, "kernel arguments");
+constexpr int table_tensors(int words) { return kTableWords / words; }
 
-__global__ void __launch_bounds__(64) adamw_table_kernel(TableArgs a, TableScalars s) {
-    const int i = threadIdx.x;
-    const xq_adamw_tensor t = a.t[min(i, s.n - 1)];
-    int64_t end = i < s.n ? (t.numel + kChunk - 1) / kChunk : 0;
-    const int64_t own = end;
+template <int WORDS>
+__global__ void __launch_bounds__(256) adamw_table_kernel(TableArgs a, TableScalars s) {
+    __shared__ int wave_end[4];
+    const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
+    const uint64_t* w = a.word + min(i, a.n - 1) * WORDS;
+    const int64_t numel = (int64_t)(w[1] & ~(3ull << 62));
+    const int own = i < a.n ? (int)((numel + kChunk - 1) / kChunk) : 0;
+    int end = own;
+#pragma unroll
     for (int d = 1; d < 64; d <<= 1) {
-        const int64_t before = __shfl_up(end, d);
-        if (i >= d) end += before;
+        const int before = __shfl_up(end, d);
+        if (lane >= d) end += before;
     }
-    if (i >= s.n) return;
-    float first = 0.0f, root = 0.0f;
-    if (s.step) {
-        const float step = *t.step + 1.0f;
-        *t.step = step;
+    if (lane == 63) wave_end[wave] = end;
+    __syncthreads();
+    if (i >= a.n) return;
+    for (int k = 0; k < wave; ++k) end += wave_end[k];
+    Row r = {};
+    r.grad = (const void*)w[0];
+    r.numel = numel;
+    r.chunk0 = a.chunk0 + end - own;
+    r.grad16 = (int)(w[1] >> 62 & 1);
+    if constexpr (WORDS >= 6) {
+        r.param16 = (int)(w[1] >> 63);
+        r.param = (void*)w[2]; r.m = (void*)w[3]; r.v = (void*)w[4];
+        float* const count = (float*)w[5];
+        const float step = *count + 1.0f;
+        *count = step;
         const double lr = s.lr_device ? (double)*s.lr_device : s.lr;
-        first = (float)(lr / (1.0 - exp(step * s.log_beta1)));             // b^t; a beta of 0 has the logarithm -inf
-        root = (float)(1.0 / sqrt(1.0 - exp(step * s.log_beta2)));
+        r.first = (float)(lr / (1.0 - exp(step * s.log_beta1)));           // b^t; a beta of 0 has the logarithm -inf
+        r.root = (float)(1.0 / sqrt(1.0 - exp(step * s.log_beta2)));
     }
-    s.rows[s.at + i] = Row{t.param, t.grad, t.exp_avg, t.exp_avg_sq, t.exp_avg_scale, t.exp_avg_sq_scale, t.numel, s.chunk0 + end - own, first, root,
-                           t.param_dtype == XQ_DT_BF16, t.grad_dtype == XQ_DT_BF16};
+    if constexpr (WORDS == 8) { r.m_scale = (float*)w[6]; r.v_scale = (float*)w[7]; }
+    a.rows[i] = r;
 }
 
 // the last row whose first chunk is not behind `chunk` (rows in order of their first chunks, no row without chunks)
@@ -407,6 +423,7 @@ int check_tensors(const char* who, const xq_adamw_tensor* t, int64_t n, int stat
         XQ_REQUIRE(a.grad_dtype == XQ_DT_BF16 || a.grad_dtype == XQ_DT_F32, "%s: gradient %lld is neither fp32 nor bf16", who, (long long)i);
         XQ_REQUIRE(a.grad && xq_aligned(a.grad, a.grad_dtype == XQ_DT_BF16 ? 2 : 4), "%s: gradient %lld is NULL or misaligned", who, (long long)i);
         *chunks += xq_cdiv(a.numel, kChunk);
+        XQ_REQUIRE(*chunks < (1ll << 31), "%s: more than %lld elements", who, (long long)kChunk << 31);
         if (grads_only) continue;
         XQ_REQUIRE(a.param_dtype == XQ_DT_BF16 || a.param_dtype == XQ_DT_F32, "%s: parameter %lld is neither fp32 nor bf16", who, (long long)i);
         XQ_REQUIRE(a.param && xq_aligned(a.param, a.param_dtype == XQ_DT_BF16 ? 2 : 4), "%s: parameter %lld is NULL or misaligned", who, (long long)i);
@@ -428,15 +445,30 @@ int check_workspace(const char* who, int64_t n, const void* workspace, int64_t b
     return XQ_OK;
 }
 
+// words 2: for the norm alone
+template <int WORDS>
 void write_table(const xq_adamw_tensor* t, int64_t n, void* workspace, const xq_adamw_options* o, hipStream_t s) {
+    TableScalars c = {};
+    if (o) c = TableScalars{o->lr, std::log(o->beta1), std::log(o->beta2), o->lr_device};
     int64_t chunk0 = 0;
-    for (int64_t at = 0; at < n; at += kTableArgs) {
+    for (int64_t at = 0; at < n; at += table_tensors(WORDS)) {
         TableArgs a;
-        const int k = (int)std::min<int64_t>(kTableArgs, n - at);
-        std::copy(t + at, t + at + k, a.t);
-        adamw_table_kernel<<<dim3(1), 64, 0, s>>>(a, TableScalars{(Row*)workspace, chunk0, k, (int32_t)at, o != nullptr, o ? o->lr : 0.0, o ? log(o->beta1) : 0.0,
-                                                                  o ? log(o->beta2) : 0.0, o ? o->lr_device : nullptr});
-        for (int i = 0; i < k; ++i) chunk0 += xq_cdiv(t[at + i].numel, kChunk);
+        a.rows = (Row*)workspace + at;
+        a.chunk0 = (int32_t)chunk0;
+        a.n = (int32_t)std::min<int64_t>(table_tensors(WORDS), n - at);
+        for (int i = 0; i < a.n; ++i) {
+            const xq_adamw_tensor& q = t[at + i];
+            uint64_t* w = a.word + i * WORDS;
+            w[0] = (uint64_t)q.grad;
+            w[1] = (uint64_t)q.numel | (uint64_t)(q.grad_dtype == XQ_DT_BF16) << 62;
+            if (WORDS >= 6) {
+                w[1] |= (uint64_t)(q.param_dtype == XQ_DT_BF16) << 63;
+                w[2] = (uint64_t)q.param; w[3] = (uint64_t)q.exp_avg; w[4] = (uint64_t)q.exp_avg_sq; w[5] = (uint64_t)q.step;
+            }
+            if (WORDS == 8) { w[6] = (uint64_t)q.exp_avg_scale; w[7] = (uint64_t)q.exp_avg_sq_scale; }
+            chunk0 += xq_cdiv(q.numel, kChunk);
+        }
+        adamw_table_kernel<WORDS><<<dim3(1), 256, 0, s>>>(a, c);
     }
 }
 
@@ -460,7 +492,7 @@ extern "C" int xq_grad_norm(const xq_adamw_tensor* tensors, int64_t n, float* no
     if (rc == XQ_OK) rc = check_workspace("xq_grad_norm", n, workspace, workspace_bytes);
     if (rc != XQ_OK) return rc;
     XQ_REQUIRE(norm && xq_aligned(norm, 4), "xq_grad_norm: norm is NULL or misaligned");
-    write_table(tensors, n, workspace, nullptr, (hipStream_t)stream);
+    write_table<2>(tensors, n, workspace, nullptr, (hipStream_t)stream);
     norm_of(n, chunks, workspace, norm, (hipStream_t)stream);
     XQ_CHECK_LAUNCH("xq_grad_norm");
     return XQ_OK;
@@ -479,7 +511,8 @@ extern "C" int xq_adamw_step(const xq_adamw_tensor* tensors, int64_t n, const xq
     if (rc == XQ_OK) rc = check_workspace("xq_adamw_step", n, workspace, workspace_bytes);
     if (rc != XQ_OK) return rc;
     hipStream_t s = (hipStream_t)stream;
-    write_table(tensors, n, workspace, o, s);
+    if (o->state_bits == 8) write_table<8>(tensors, n, workspace, o, s);
+    else write_table<6>(tensors, n, workspace, o, s);
     if (o->norm && !o->norm_given) norm_of(n, chunks, workspace, o->norm, s);
     if (n) {
         const StepArgs a = {(const Row*)workspace, chunks, o->norm, (int32_t)n, (float)o->max_norm, (float)o->beta1, (float)o->beta2,
