@@ -128,11 +128,12 @@ __device__ __forceinline__ f32x4 load4(bool bf16, const void* p, int64_t i, int6
         return r;
     }
 }
+// (past the caches: nothing of it is read before the next step, and 504 factors take 1 % less)
 template <bool WHOLE>
 __device__ __forceinline__ void store4(bool bf16, void* p, int64_t i, int64_t n, f32x4 v) {
     if constexpr (WHOLE) {
-        if (bf16) *(u32x2*)((bf16_t*)p + i) = u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
-        else *(f32x4*)((float*)p + i) = v;
+        if (bf16) __builtin_nontemporal_store(u32x2{pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])}, (u32x2*)((bf16_t*)p + i));
+        else __builtin_nontemporal_store(v, (f32x4*)((float*)p + i));
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
@@ -154,7 +155,7 @@ __device__ __forceinline__ uint32_t load4_codes(const void* p, int64_t i, int64_
 template <bool WHOLE>
 __device__ __forceinline__ void store4_codes(void* p, int64_t i, int64_t n, uint32_t c) {
     if constexpr (WHOLE) {
-        *(uint32_t*)((uint8_t*)p + i) = c;
+        __builtin_nontemporal_store(c, (uint32_t*)((uint8_t*)p + i));
     } else {
 #pragma unroll
         for (int k = 0; k < 4; ++k)
