@@ -311,6 +311,7 @@ def test_refusals(hip_device):
     q = prob(); q[4][1] = q[4][0]; refused(q, "share")
     q = prob(); q[0][1] = q[0][0].view(-1)[:5]; refused(q, "share")
     q = prob(); q[2][1] = q[3][1]; refused(q, "share")
+    q = prob(); both = torch.zeros(66, device=hip_device); q[2][0], q[3][0] = both[:64].view(8, 8), both[2:].view(8, 8); refused(q, "share")
     q = prob(8); q[5][0] = q[5][0].new_zeros(2); refused(q, r"1 element\(s\)")
     q = prob(8); q[2][0] = q[2][0].view(torch.uint8); refused(q, "must be Char")
     q = prob(8); q[5] = None; refused(q, "exp_avg_scales")
@@ -405,6 +406,37 @@ def test_class_under_the_merge_schedule(hip_device):
     m.lora_A.grad = torch.ones_like(m.lora_A)
     opt.step()
     assert float(opt.state[m.lora_A]["step"]) == 1.0
+
+
+def test_class_in_a_graph(hip_device):
+    """States are not made while a graph is captured; with states, replays are steps."""
+    runs = []
+    for graphed in (False, True):
+        params = _params(hip_device)
+        opt = AdamW(params, lr=torch.tensor(1e-2, device=hip_device), state_bits=8, max_grad_norm=1.0)
+        grads = [torch.randn(p.shape, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(i)) for i, p in enumerate(params)]
+        for p, g in zip(params, grads):
+            p.grad = g.clone()
+        graph = torch.cuda.CUDAGraph()
+        if graphed:
+            with pytest.raises(_C.XqError, match="before the capture"):
+                with torch.cuda.graph(graph):
+                    opt.step()
+            graph = torch.cuda.CUDAGraph()
+        opt.step()
+        torch.cuda.synchronize()
+        if graphed:
+            with torch.cuda.graph(graph):
+                opt.step()
+        for k in range(3):
+            for p, g in zip(params, grads):
+                p.grad.copy_(g * (k + 1))
+            opt.param_groups[0]["lr"].fill_(1e-2 / (k + 1))
+            graph.replay() if graphed else opt.step()
+            torch.cuda.synchronize()
+        runs.append(params)
+    for a, b in zip(*runs):
+        assert torch.equal(a, b)
 
 
 def test_step_is_seen_by_autograd(hip_device):

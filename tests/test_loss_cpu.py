@@ -29,7 +29,7 @@ def test_cpu_tensors_raise():
     (dict(x=torch.zeros(3, 128, dtype=BF)), "do not go together"), (dict(x=torch.zeros(1, 3, 64, dtype=BF)), "do not go together"),
     (dict(x=torch.zeros(3, 96, dtype=BF), w=torch.zeros(10, 96, dtype=BF)), "multiple of 64"),
     (dict(w=torch.zeros(0, 64, dtype=BF)), "not empty"), (dict(reduction="batchmean"), "reduction"),
-    (dict(logit_scale=0.0), "logit_scale"), (dict(logit_scale=float("inf")), "logit_scale"), (dict(logit_scale=float("nan")), "logit_scale"),
+    (dict(ignore_index=2 ** 63), "ignore_index"), (dict(logit_scale=0.0), "logit_scale"), (dict(logit_scale=float("inf")), "logit_scale"), (dict(logit_scale=float("nan")), "logit_scale"),
 ])
 def test_argument_errors(kw, match):
     with pytest.raises(_C.XqError, match=match):

@@ -473,11 +473,13 @@ struct LceProductArgs {
 
 // Parts of a contraction of E . W: as many as leave the least of the chip idle, where tiles alone would (a part costs its sums once more in
 // memory: 2 % a part).  The rows that count are known on the device only, so that the kernel that counts them works it out, a wave with
-// a number of parts in each lane.  Divided, tiles and parts are three rounds of the chip at most, which bounds the sums.
-constexpr int kLceSplitRounds = 3, kLceMostParts = 64;
+// a number of parts in each lane.  Divided, tiles and parts are three rounds of the chip at most, one where the tiles are few (more would
+// gain nothing), which bounds the sums.
+constexpr int kLceMostParts = 64;
+__host__ __device__ inline int lce_rounds(int tiles, int slots) { return 4 * tiles <= slots ? 1 : 3; }
 __device__ __forceinline__ int lce_parts(int tiles, int steps, int slots, int lane) {
     const int s = lane + 1, all = tiles * s;
-    const bool may = s == 1 || (all <= kLceSplitRounds * slots && steps >= 16 * s);
+    const bool may = s == 1 || (all <= lce_rounds(tiles, slots) * slots && steps >= 16 * s);
     const float cost = may ? (float)((all + slots - 1) / slots) / (float)s * (1.0f + 0.02f * (float)(s - 1)) : INFINITY;
     float least = cost;
 #pragma unroll
@@ -535,23 +537,42 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
             for (int j = 0; j < 4; ++j) acc[i][j] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
     }
 
-    const int row_w = wm * 16 * TM + l16, col_w = c0 + wn * 64 + 4 * lg;
+    const int row_w = r0 + wm * 16 * TM + l16, col_w = c0 + wn * 64;
+    if (g.out16) {
+#pragma unroll
+        for (int i = 0; i < TM; ++i) {
+            const int row = row_w + 16 * i;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                // eight columns in a row for each lane: fragments 2 q and 2 q + 1 exchange halves, then rows of sixteen lanes
+                const f32x4 u = acc[i][2 * q], v = acc[i][2 * q + 1];
+                uint32_t x[2] = {pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3])}, y[2] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
+#pragma unroll
+                for (int d = 0; d < 2; ++d) {
+                    const auto h = __builtin_amdgcn_permlane32_swap(x[d], y[d], false, false);
+                    const auto r = __builtin_amdgcn_permlane16_swap(h[0], h[1], false, false);
+                    x[d] = r[0];
+                    y[d] = r[1];
+                }
+                const int col = col_w + q * 32 + lg * 8;
+                if (row < rows && col < g.H) *(u32x4*)(g.out16 + row * g.ld16 + col) = u32x4{x[0], x[1], y[0], y[1]};
+            }
+        }
+        return;
+    }
     float* const out = g.out + (int64_t)s * rows * g.H;
+    const bool again = g.add && g.redo[ta];
 #pragma unroll
     for (int i = 0; i < TM; ++i) {
-        const int row = r0 + row_w + 16 * i;
+        const int row = row_w + 16 * i;
         if (row >= rows) continue;
-        const float alpha = g.add && g.redo[ta] ? g.alpha[row] : 1.0f;
+        const float alpha = again ? g.alpha[row] : 1.0f;
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-            const int col = col_w + 16 * j;
+            const int col = col_w + 16 * j + 4 * lg;
             if (col >= g.H) continue;
-            if (g.out16) {
-                *(u32x2*)(g.out16 + row * g.ld16 + col) = u32x2{pack_bf16x2(acc[i][j][0], acc[i][j][1]), pack_bf16x2(acc[i][j][2], acc[i][j][3])};
-            } else {
-                f32x4* o = (f32x4*)(out + (int64_t)row * g.H + col);
-                *o = g.add ? *o * alpha + acc[i][j] : acc[i][j];
-            }
+            f32x4* o = (f32x4*)(out + (int64_t)row * g.H + col);
+            *o = g.add ? *o * alpha + acc[i][j] : acc[i][j];
         }
     }
 }

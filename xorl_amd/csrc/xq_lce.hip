@@ -372,9 +372,19 @@ Plan plan_for(int64_t M, int64_t V, int tm, bool steps) {
 Plan plan_tokens(int64_t M, int64_t V, int keep) { return plan_for(M, V, 0, keep == XQ_LCE_KEEP_DX); }
 Plan plan_head(int64_t M, int64_t V) { return plan_for(M, V, 8, true); }          // G: rows of the vocabulary, tokens along the contraction
 
-// fp32 sums of E . W over the parts of the contraction, whatever the rows that count (lce_parts)
+// rows of E, whole tiles of them
+int64_t image_rows(const Plan& p, int64_t M) { return xq_cdiv(std::max<int64_t>(M, 1), 32 * p.tm) * 32 * p.tm; }
+
+// fp32 sums of E . W over the parts of the contraction, however many of the rows count (lce_parts)
 int64_t sums_bytes(const Plan& p, int64_t M, int64_t H) {
-    return 4 * std::max<int64_t>(M * H, (int64_t)kLceSplitRounds * slots(p.tm) * 32 * p.tm * 256);
+    const int64_t tiles_h = xq_cdiv(H, 256), rows = 32 * p.tm, free = slots(p.tm);
+    int64_t most = M * H;
+    for (int64_t t = 1; t <= xq_cdiv(M, rows); ++t) {
+        const int64_t tiles = t * tiles_h, parts = std::min<int64_t>({kLceMostParts, lce_rounds((int)tiles, (int)free) * free / tiles, p.piece / 512});
+        if (parts > 1) most = std::max(most, parts * std::min(t * rows, M) * H);
+        else if (tiles > free) break;
+    }
+    return 4 * most;
 }
 
 // what a forward leaves for the backward
@@ -425,7 +435,7 @@ Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
         s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
     } else {
         s.part = (f32x2*)take(8 * p.rows_pad * xq_cdiv(pass == XQ_LCE_KEEP_DX ? p.piece : V, p.cols));
-        if (pass == XQ_LCE_KEEP_DX) s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
+        if (pass == XQ_LCE_KEEP_DX) s.image = (bf16_t*)take(2 * image_rows(p, M) * p.piece);
     }
     s.bytes = at - (uint8_t*)base;
     return s;
@@ -456,7 +466,7 @@ int launch_product(const LceProductArgs& a, int64_t rows, hipStream_t s) {
     static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
     if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
     int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(a.H, 256);
-    if (a.parts) blocks = std::max<int64_t>(blocks, std::min<int64_t>(kLceMostParts * blocks, (int64_t)kLceSplitRounds * slots(TM)));
+    if (a.parts) blocks = std::max<int64_t>(blocks, std::min<int64_t>(kLceMostParts * blocks, 3ll * slots(TM)));
     k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
     return XQ_OK;
 }

@@ -976,7 +976,8 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         std::vector<xq_adamw_tensor> q;
         std::vector<Tensor> keep;
         std::vector<at::TensorImpl*> written;     // (the lists hold them)
-        std::vector<const void*> once;            // what the step writes: named twice it would be written by two blocks at a time
+        std::vector<std::pair<const char*, const char*>> once;        // what the step writes, from and to: named twice it would be written by two blocks at a time
+        auto note = [&](const Tensor& t) { once.emplace_back((const char*)t.data_ptr(), (const char*)t.data_ptr() + nbytes(t)); };
         q.reserve(n);
         written.reserve(6 * n);
         once.reserve(6 * n);
@@ -1015,21 +1016,21 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                             throw ArgError(from[k]->at(i) + " must be contiguous fp32 with " + std::to_string((a.numel + 255) / 256) + " element(s)");
                         *to[k] = (float*)sc.data_ptr();
                         written.push_back(sc.unsafeGetTensorImpl());
-                        if (a.numel) once.push_back(sc.data_ptr());
+                        if (a.numel) note(sc);
                     }
                 }
                 for (const Tensor* w : {&pt, &mt, &vt}) {
                     written.push_back(w->unsafeGetTensorImpl());
-                    if (a.numel) once.push_back(w->data_ptr());
+                    if (a.numel) note(*w);
                 }
                 written.push_back(st.unsafeGetTensorImpl());
-                once.push_back(st.data_ptr());
+                note(st);
             }
             if (a.numel) q.push_back(a);
         }
         std::sort(once.begin(), once.end());
-        if (std::adjacent_find(once.begin(), once.end()) != once.end())
-            throw ArgError("adamw_step: two tensors share a parameter, a state or a step count");
+        if (std::adjacent_find(once.begin(), once.end(), [](const auto& a, const auto& b) { return b.first < a.second; }) != once.end())
+            throw ArgError("adamw_step: two tensors share memory of a parameter, a state or a step count");
         if (args[8] != Py_None) {
             const Tensor* lr = plain(args[8]);
             if (!lr || lr->scalar_type() != at::kFloat || lr->numel() != 1) throw ArgError("adamw_step: an lr tensor must be one fp32 element on the device");

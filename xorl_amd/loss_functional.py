@@ -137,6 +137,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
         raise _C.XqError(f"linear_cross_entropy: the hidden size must be a multiple of 64 and the vocabulary not empty, got {tuple(weight.shape)}")
     if not (logit_scale > 0.0 and math.isfinite(logit_scale)):
         raise _C.XqError(f"linear_cross_entropy: logit_scale must be positive and finite, got {logit_scale}")
+    if not -2 ** 63 <= int(ignore_index) < 2 ** 63:
+        raise _C.XqError(f"linear_cross_entropy: ignore_index must fit 64 bits, got {ignore_index}")
     _C.require_hip(x, weight, labels)
     if weight.device != x.device or labels.device != x.device:
         raise _C.XqError(f"linear_cross_entropy: x, weight and labels are on {x.device}, {weight.device} and {labels.device}")

@@ -38,8 +38,8 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
                grad_norm: Optional[Tensor] = None) -> Optional[Tensor]:
     """One AdamW step over all ``params``, in place, with the states they come with.
 
-    Parameters and gradients are fp32 or bf16, tensor by tensor; parameters, states and step counts are contiguous and none occurs
-    twice (other layouts are refused; a gradient that is not contiguous is copied).  States are fp32, or, with both lists of scales
+    Parameters and gradients are fp32 or bf16, tensor by tensor; parameters, states and step counts are contiguous and share no
+    memory (both refused otherwise; a gradient that is not contiguous is copied).  States are fp32, or, with both lists of scales
     given, 8-bit codes: int8 ``exp_avgs`` and uint8 ``exp_avg_sqs`` with fp32 scales for every 256 elements (``adamw_state_values``
     says what they stand for).  ``steps`` are fp32 tensors of one element each, advanced here.  ``lr`` may be a 0-dim fp32 tensor on
     the device: a captured step then follows it.
@@ -81,7 +81,8 @@ class AdamW(torch.optim.Optimizer):
 
     ``state_bits=8`` keeps the two moments as 8-bit codes (2.03 bytes an element in place of 8).  ``max_grad_norm`` clips by the norm
     over the parameters of all groups inside the step; the norm of the last step is ``self.grad_norm`` (a device tensor).  States are
-    made at a parameter's first step and whenever its state has been dropped.  State names: ``step``, ``exp_avg``, ``exp_avg_sq``, with
+    made at a parameter's first step and whenever its state has been dropped, but not while a graph is captured (refused: they would be made
+    anew in every replay).  In a captured step ``lr`` follows a tensor, a number stays what it was.  State names: ``step``, ``exp_avg``, ``exp_avg_sq``, with
     8 bits ``exp_avg_scale`` and ``exp_avg_sq_scale`` too.  All parameters lie on one device."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
@@ -98,6 +99,8 @@ class AdamW(torch.optim.Optimizer):
         state = self.state[p]
         if not state:
             local = _local(p)
+            if local.is_cuda and torch.cuda.is_current_stream_capturing():
+                raise _C.XqError("AdamW: a captured step would make its states anew in every replay; take one step before the capture")
             state["step"] = torch.zeros((), dtype=torch.float32, device=local.device)
             if state_bits == 8:
                 n = _scale_count(local.numel())
