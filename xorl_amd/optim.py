@@ -30,7 +30,6 @@ def grad_norm(grads: Iterable[Tensor]) -> Tensor:
     return native().adamw(None, list(grads), None, None, None, None, None, None, None, None, None)
 
 
-@torch.no_grad()
 def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequence[Tensor], exp_avg_sqs: Sequence[Tensor],
                steps: Sequence[Tensor], *, exp_avg_scales: Optional[Sequence[Tensor]] = None,
                exp_avg_sq_scales: Optional[Sequence[Tensor]] = None, lr: Union[float, Tensor], betas: Tuple[float, float] = (0.9, 0.999),
