@@ -141,6 +141,27 @@ def test_step_over_many_tensors(hip_device, bits, count):
     _check(prob, exp, bits, torch.float32, DECODED if bits == 8 else 0.0)
 
 
+@pytest.mark.parametrize("clip", [None, 0.02])
+@pytest.mark.parametrize("n", [256 * 4000, 256 * 33 + 77])
+def test_codes_are_the_nearest_ones(hip_device, n, clip):
+    """8-bit codes against the nearest ones of m' and s', both formed by the formula's operations in fp32: equal, whatever lies in the middle"""
+    prob = _problem([(n,)], 8, torch.float32, torch.float32, 41, hip_device)
+    m, v = _blocks(prob[2][0].float()), _blocks(prob[3][0].float())
+    g = _blocks(prob[1][0])
+    if clip is not None:
+        norm = g.double().square().sum().sqrt().float()
+        g = g * ((norm + 1e-6).reciprocal() * clip).clamp(max=1.0)
+    m = m * m.abs() * (prob[5][0] * (1 / 16129))[:, None] * B1 + g * (1 - B1)
+    old = v * v * (prob[6][0] * (1 / 65025))[:, None]
+    s = (old * old * B2 + g * g * (1 - B2)).sqrt()
+    adamw_step(*prob[:5], exp_avg_scales=prob[5], exp_avg_sq_scales=prob[6], lr=1e-3, max_norm=clip)
+    ma, sa = m.abs().amax(1), s.amax(1)
+    assert torch.equal(prob[5][0], ma) and torch.equal(prob[6][0], sa)
+    c = (m.double().abs() / ma.double()[:, None]).sqrt().mul(127).round() * m.sign()
+    d = (s.double() / sa.double()[:, None]).sqrt().mul(255).round().clamp(min=1) * (s > 0)
+    assert torch.equal(c.view(-1)[:n].to(torch.int8), prob[2][0]) and torch.equal(d.view(-1)[:n].to(torch.uint8), prob[3][0])
+
+
 def test_elements_outside_stay(hip_device):
     """What lies around a tensor's elements is left alone: the last pieces are stored one by one."""
     for bits in (32, 8):

@@ -114,7 +114,7 @@ __device__ __forceinline__ float load1(const void* p, int64_t i) {
     return BF16 ? bf16_to_f32(((const bf16_t*)p)[i]) : ((const float*)p)[i];
 }
 // What a step reads and writes goes past the caches, but for the gradients: nothing else of it is read again before the next step, and the
-// gradients that the norm read last are still there (504 factors, 87 M elements: 595 -> 545 us, with 8-bit states 496 -> 451).
+// gradients that the norm read last are still there (504 factors, 87 M elements: 595 us otherwise, 545 so).
 template <bool PAST, typename V>
 __device__ __forceinline__ V load_as(const void* p) {
     if constexpr (PAST) return __builtin_nontemporal_load((const V*)p);
@@ -188,22 +188,51 @@ __device__ __forceinline__ uint32_t wave_max_bits(uint32_t v) {
 }
 __device__ __forceinline__ uint32_t bits_abs(float f) { return __float_as_uint(f) & 0x7fffffffu; }
 
-// Codes of four elements.  The instruction that packs a byte rounds to nearest even and saturates, so that a code takes a product, a
-// root and a packing; m goes in as 128 + c, whose top bit is flipped afterwards.  The hardware root and reciprocal are off by an ulp at
-// most: it decides between two codes only where the value lies that near the middle.  inv: top code squared over the block's largest.
-__device__ __forceinline__ uint32_t m_codes(f32x4 m, float inv) {
+// Codes of four elements: the nearest to 127 sqrt(|m| / A) and 255 sqrt(s / A), exactly.  A product, the hardware's root and the instruction
+// that packs a byte (to nearest even, saturating; m goes in as 128 + c, whose top bit is flipped afterwards) decide all but the elements
+// that come near the middle between two codes: the errors of reciprocal, product and root together are below 2e-7 (m) and 3e-7 (s, a root
+// itself) of the code.  A wave with such an element, 7 % of them, compares |m| 127^2 with (c + 1/2)^2 A in 64 bits, where both sides
+// are exact.  That a code does not hang on an ulp matters a step later: the neighbour of a small s is several per cent away.
+__device__ __forceinline__ bool near_middle(float f, float by) { return fabsf(__builtin_amdgcn_fractf(f) - 0.5f) < by; }
+__device__ __forceinline__ int exact_code(float x, float f, double top2, float amax) {
+    const int c = (int)f;
+    const double half = (double)c + 0.5, at = (double)x * top2, middle = half * half * (double)amax;
+    return at > middle || (at == middle && (c & 1)) ? c + 1 : c;               // (in the middle: the even one)
+}
+__device__ __forceinline__ uint32_t m_codes(f32x4 m, float amax, float inv) {
+    f32x4 f;
+    bool near = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        f[k] = __builtin_amdgcn_sqrtf(fabsf(m[k]) * inv);
+        near |= near_middle(f[k], 4e-5f);
+    }
+    if (__any(near)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = f[k] <= 127.0f ? (float)exact_code(fabsf(m[k]), f[k], 127.0 * 127.0, amax) : f[k];
+    }
     uint32_t c = 0;
 #pragma unroll
-    for (int k = 0; k < 4; ++k)
-        c = __builtin_amdgcn_cvt_pk_u8_f32(128.0f + __builtin_copysignf(__builtin_amdgcn_sqrtf(fabsf(m[k]) * inv), m[k]), k, c);
+    for (int k = 0; k < 4; ++k) c = __builtin_amdgcn_cvt_pk_u8_f32(128.0f + __builtin_copysignf(f[k], m[k]), k, c);
     return c ^ 0x80808080u;
 }
-__device__ __forceinline__ uint32_t s_codes(f32x4 s, float inv) {
+__device__ __forceinline__ uint32_t s_codes(f32x4 s, f32x4 v, float amax, float inv) {
+    f32x4 f;
+    bool near = false;
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        f[k] = __builtin_amdgcn_sqrtf(s[k] * inv);
+        near |= near_middle(f[k], 1e-4f);
+    }
+    if (__any(near)) {
+#pragma unroll
+        for (int k = 0; k < 4; ++k) f[k] = f[k] <= 255.0f ? (float)exact_code(sqrtf(v[k]), f[k], 255.0 * 255.0, amax) : f[k];
+    }
     uint32_t c = 0;
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
         const float least = __builtin_amdgcn_fmed3f(s[k] * 0x1p120f, 0.0f, 1.0f);      // 1, or 0 for 0
-        c = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(__builtin_amdgcn_sqrtf(s[k] * inv), least), k, c);
+        c = __builtin_amdgcn_cvt_pk_u8_f32(fmaxf(f[k], least), k, c);
     }
     return c;
 }
@@ -231,7 +260,6 @@ struct StepArgs {
 // constants of a call
 struct Call {
     float clip, keep;                       // of the gradients; minus the decay
-    float g, g_root, m_value, s_value;      // 8 bits: what g counts in m' and, squared, in v'; what a squared code counts in either
 };
 
 // a wave's four pieces of a chunk, from element base on (lane 0's) 1024 apart; everything is read before anything is computed
@@ -268,17 +296,18 @@ __device__ __forceinline__ void step_chunk(const StepArgs& a, const Row& r, int6
             f32x4 s;
             uint32_t mb = 0, sb = 0;
             if constexpr (EIGHT) {
-                // bound by instructions: what is constant over a block or a call is multiplied together first, and root and reciprocal are the
-                // hardware's (an ulp each)
-                const float mk = ms[u] * c.m_value, sk = vs[u] * c.s_value;
+                // m' and v' by the formula's products and sums, each rounded as it stands: the codes are of these numbers.  For the update root and
+                // reciprocal are the hardware's (an ulp each)
+                const float mk = ms[u] * (1.0f / kM2), sk = vs[u] * (1.0f / kS2);
 #pragma unroll
                 for (int k = 0; k < 4; ++k) {
-                    const float h = g[u][k] * c.g_root, q = (float)((vc[u] >> (8 * k)) & 0xffu), old = q * q * sk, e = (float)(int8_t)(mc[u] >> (8 * k));
-                    m[u][k] = fmaf(e * fabsf(e), mk, g[u][k] * c.g);
-                    s[k] = __builtin_amdgcn_sqrtf(fmaf(old, old, h * h));
+                    const float gk = g[u][k] * c.clip, old = s_value(vc[u], k, sk);
+                    m[u][k] = m_value(mc[u], k, mk) * a.beta1 + gk * a.one_minus_beta1;
+                    v[u][k] = old * old * a.beta2 + gk * gk * a.one_minus_beta2;
+                    s[k] = __builtin_amdgcn_sqrtf(v[u][k]);
                     p[u][k] = fmaf(p[u][k], c.keep, p[u][k]) - m[u][k] * r.first * __builtin_amdgcn_rcpf(fmaf(s[k], r.root, a.eps));
                     mb = max(mb, bits_abs(m[u][k]));
-                    sb = max(sb, __float_as_uint(s[k]));
+                    sb = max(sb, __float_as_uint(v[u][k]));
                 }
             } else {
 #pragma unroll
@@ -291,9 +320,9 @@ __device__ __forceinline__ void step_chunk(const StepArgs& a, const Row& r, int6
             }
             store4<WHOLE>(p16, r.param, i, n, p[u]);
             if constexpr (EIGHT) {
-                const float mt = __uint_as_float(wave_max_bits(mb)), st = __uint_as_float(wave_max_bits(sb) & 0x7fffffffu);
-                store4_codes<WHOLE>(r.m, i, n, m_codes(m[u], mt > kSmallest ? kM2 * __builtin_amdgcn_rcpf(mt) : 0.0f));
-                store4_codes<WHOLE>(r.v, i, n, s_codes(s, st > kSmallest ? kS2 * __builtin_amdgcn_rcpf(st) : 0.0f));
+                const float mt = __uint_as_float(wave_max_bits(mb)), st = sqrtf(__uint_as_float(wave_max_bits(sb) & 0x7fffffffu));
+                store4_codes<WHOLE>(r.m, i, n, m_codes(m[u], mt, mt > kSmallest ? kM2 * __builtin_amdgcn_rcpf(mt) : 0.0f));
+                store4_codes<WHOLE>(r.v, i, n, s_codes(s, v[u], st, st > kSmallest ? kS2 * __builtin_amdgcn_rcpf(st) : 0.0f));
                 if (lane == 0) {
                     r.m_scale[i >> 8] = mt;
                     r.v_scale[i >> 8] = st;
@@ -318,14 +347,10 @@ __global__ void __launch_bounds__(kThreads) adamw_kernel(StepArgs a) {
     // (written so that a NaN norm makes the gradients NaN)
     float clip = 1.0f;
     if (a.norm) {
-        clip = a.max_norm / (*a.norm + 1e-6f);
+        clip = 1.0f / (*a.norm + 1e-6f) * a.max_norm;
         clip = clip > 1.0f ? 1.0f : clip;
     }
     k.clip = clip;
-    k.g = a.one_minus_beta1 * clip;
-    k.g_root = sqrtf(a.one_minus_beta2) * clip;
-    k.m_value = a.beta1 / kM2;
-    k.s_value = sqrtf(a.beta2) / kS2;
     int t = row_of(a.rows, a.n, c, lane);
     Row r = a.rows[t];
     for (; c >= c0; --c) {
