@@ -118,6 +118,20 @@ def test_hidden_sizes(hip_device, M, H):
     _case(*_inputs(M, 777, H, H, hip_device))
 
 
+@pytest.mark.parametrize("M,V,H", [(40, 70001, 128), (100, 70001, 128), (100, 70001, 64), (128, 40000, 192), (64, 140001, 64), (1, 66000, 320), (1100, 3000, 128),
+                                   (300, 66000, 64), (513, 20000, 192), (90, 9000, 256), (33, 9000, 256)])
+@pytest.mark.parametrize("far", [False, True])
+def test_tiles_of_every_kind(hip_device, M, V, H, far):
+    """Several tiles a block, narrow and wide ones, contractions shorter than the loads are ahead; and done again for logits far apart"""
+    x, w, labels = _inputs(M, V, H, M + V + H, hip_device, std=0.05, ignored=0.1)
+    if far:
+        w[V // 2:V // 2 + 40] = (w[V // 2:V // 2 + 40].float() * 300).to(BF)
+        w[V - 3:] = (w[V - 3:].float() * 500).to(BF)
+    if M == 1:
+        labels.clamp_(min=0)
+    _case(x, w, labels, "none")
+
+
 @pytest.mark.parametrize("reduction", ["none", "mean", "sum"])
 @pytest.mark.parametrize("scale", [1.0, 0.3, 2.5])
 @pytest.mark.parametrize("label_dtype", [torch.int64, torch.int32])
@@ -380,6 +394,22 @@ def test_captured_step_with_changing_inputs(hip_device, M):
         want = step()
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want)), k
+
+
+def test_graph_captured_without_a_first_call(hip_device):
+    """Shapes that no other call here has: nothing is left to be set up by a first call outside the graph"""
+    x, w, labels = _inputs(77, 2345, 448, 71, hip_device)
+    x.requires_grad_(True)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        loss = linear_cross_entropy(x, w, labels)
+        dx, = torch.autograd.grad(loss, x)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = linear_cross_entropy(x, w, labels)
+        assert torch.equal(loss.detach(), want.detach()) and torch.equal(dx, torch.autograd.grad(want, x)[0])
 
 
 def test_two_calls_at_once(hip_device):

@@ -9,7 +9,12 @@
 //  * Tiles of 32 TM x 64 TN, K-steps of 32, LDS stages (four or eight) filled by direct-to-LDS loads, eight waves of 16 TM x 16 TN on
 //    v_mfma_f32_16x16x32_bf16.  In iteration kt every wave reads stages kt and kt + 1 and fills stage kt + 3 (or kt + 7); the loads of
 //    kt + 2 are waited for at its end.  A K-step is TM chunks of TN MFMAs; a chunk's fragment of A is read three chunks ahead, the fragments of B a
-//    K-step ahead (two register sets).  Loads behind the last K-step repeat it, so that every iteration is the same.
+//    K-step ahead (two register sets).  Every iteration is the same: behind a tile's last K-step the logits kernel loads the next tile's, the product
+//    the last one again (a branch around the loads cost both 5 %).
+//  * What bounds it.  Many rows: the matrix units, two thirds (logits) to three quarters (product) busy, and the power they draw: 1.36 PFLOP/s of
+//    STATS at 8192 rows under [131072, 4096], 1.28 of EXP (its 1 GiB pieces of E are 5 % of it, the other ends 3 %, reading 64-byte pieces of
+//    rows and not whole lines 5 %), 1.36 of E . W; a library product of the same operands 1.41.  Up to 128 rows: reading the head, 1 GiB of it in 180 us
+//    (6.0 TB/s) under one row, 174 us for E . W.
 //  * Stage.  A: [row][32 k], the 16-byte chunk c of a row at c ^ ((row >> 2) & 2): 16 rows x 4 chunks meet no bank twice.  B of
 //    the logits the same.  B of the product: [32 k][256 columns], the 32-byte unit u of row k at u ^ (k & 7); fragments come out by
 //    the transposing read, which takes 4 rows x 16 columns for 16 lanes: eight rows of a half wave lie in eight bank groups.
@@ -35,7 +40,7 @@ struct LceTile {
     static constexpr int END_BYTES = ROWS * 32 + 1024 * 4;      // of the ends: sums by row and wave; four numbers by row or column
     static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + (AHEAD ? END_BYTES : 0);
     static_assert(AHEAD || END_BYTES <= STAGES * STAGE_BYTES, "the ends reuse the stages");
-    static_assert((STAGES & (STAGES - 1)) == 0 && LDS_BYTES <= 160 * 1024, "stages are taken in turn");
+    static_assert((STAGES & (STAGES - 1)) == 0 && LDS_BYTES <= 160 * 1024, "stages are counted by a mask, and fit");
 };
 
 struct LceRows {                        // what is kept of the labels: the rows that count, in order

@@ -18,6 +18,10 @@
 //    again for the row tiles concerned.  bf16 keeps E to half a step (2^-9 of each term, of either sign).
 //  * A trained head: the backward forms the logits again with the roles exchanged, G = g (p - [v = t]) as bf16 with the tokens along the
 //    contraction, and multiplies it with the rows that count.
+//
+// 8192 rows, 5735 of which count, under [131072, 4096], forward and backward: 10.1 ms, in two pieces of 2.5 (logits) and 2.45 ms (product) each, 0.1 ms of
+// everything else.  One row, scored: 192 us.  96 rows under [32003, 2048], forward and backward: 82 us, of which 28 and 27 are the products and the rest
+// six small launches.
 #include <algorithm>
 #include <atomic>
 
