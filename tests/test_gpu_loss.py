@@ -412,6 +412,27 @@ def test_graph_captured_without_a_first_call(hip_device):
         assert torch.equal(loss.detach(), want.detach()) and torch.equal(dx, torch.autograd.grad(want, x)[0])
 
 
+def test_capture_beside_a_living_loss_is_refused(hip_device):
+    """Nothing is handed to the stream of the loss outside; what went before and comes after is as it was"""
+    x, w, labels = _inputs(40, 1000, 128, 72, hip_device)
+    x.requires_grad_(True)
+    eager = linear_cross_entropy(x, w, labels)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(linear_cross_entropy(x, w, labels), x)
+    torch.cuda.synchronize()
+    want, = torch.autograd.grad(eager, x)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx, = torch.autograd.grad(linear_cross_entropy(x, w, labels), x)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want)
+
+
 def test_two_calls_at_once(hip_device):
     problems = [_inputs(M, 6000, 256, 80 + M, hip_device) for M in (400, 30)]
     want = []

@@ -383,6 +383,55 @@ def test_class_matches_torch_over_steps(hip_device):
         assert float((a - b).abs().max()) <= 6 * lr * 1.1 * 2e-5 + 6 * 4 * U * float(b.abs().max())
 
 
+def test_gradients_that_share_memory(hip_device):
+    """With each other they may; with what the step writes they may not: a block would read what another has written"""
+    def prob():
+        return list(_problem([(8, 8), (8, 8)], 32, torch.float32, torch.float32, 30, hip_device))
+
+    q = prob()
+    both = torch.randn(72, device=hip_device)
+    q[1][0], q[1][1] = both[:64].view(8, 8), both[8:].view(8, 8)
+    other = [[t.clone() for t in l] for l in q[:5]]
+    adamw_step(*q[:5], lr=1e-2)
+    adamw_step(*other, lr=1e-2)
+    assert all(torch.equal(a, b) for a, b in zip(q[0], other[0]))
+    for k in (0, 2, 3):
+        q = prob()
+        whole = torch.zeros(128, device=hip_device)
+        q[k][1], q[1][0] = whole[:64].view(8, 8), whole[4:68].view(8, 8)
+        with pytest.raises(_C.XqError, match="share"):
+            adamw_step(*q[:5], lr=1e-2)
+        q[1][0], q[1][1] = q[1][1], whole[60:124].view(8, 8)
+        with pytest.raises(_C.XqError, match="share"):
+            adamw_step(*q[:5], lr=1e-2)
+        q[1][0], q[1][1], q[k][1] = q[1][0], whole[:64].view(8, 8), whole[4:68].view(8, 8)
+        with pytest.raises(_C.XqError, match="share"):
+            adamw_step(*q[:5], lr=1e-2)
+        assert not whole.any()
+
+
+def test_class_goes_on_from_torch(hip_device):
+    """Two steps of torch.optim.AdamW, then two here, against four of it"""
+    ours, theirs = _params(hip_device), _params(hip_device)
+    first = torch.optim.AdamW(ours, lr=1e-2)
+    all_theirs = torch.optim.AdamW(theirs, lr=1e-2)
+    g = torch.Generator(device=hip_device).manual_seed(5)
+    opt = first
+    for k in range(4):
+        if k == 2:
+            opt = AdamW(ours)
+            opt.load_state_dict(first.state_dict())
+        for p, q in zip(ours, theirs):
+            p.grad = torch.randn(p.shape, device=hip_device, generator=g)
+            q.grad = p.grad.clone()
+        opt.step()
+        all_theirs.step()
+    # two steps of either side: 2 roundings of the parameter each, and 16 of an update that is at most 1.1 lr after so few steps (the moments' own
+    # roundings reach it enlarged by 1 / (1 - 0.9^3), hence twice the 8 operations)
+    for p, q in zip(ours, theirs):
+        assert (p - q).abs().max() <= 4 * 2.0 ** -24 * (2 * float(q.abs().max()) + 16 * 1.1e-2)
+
+
 @pytest.mark.parametrize("bits", [32, 8])
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_class_state_dict_round_trip(hip_device, bits, dtype):

@@ -1,5 +1,6 @@
 """Host side of the optimizer step: what adamw_step, grad_norm, AdamW and the C entry points refuse before anything runs."""
 
+import copy
 import ctypes
 
 import pytest
@@ -95,3 +96,33 @@ def test_norm_and_values_refuse():
 
 def test_struct_layout():
     assert ctypes.sizeof(_C.XqAdamwTensor) == 72 and ctypes.sizeof(_C.XqAdamwOptions) == 72
+
+
+def test_states_of_torch_adamw_are_taken():
+    """A dictionary of torch.optim.AdamW, with a bf16 parameter's bf16 moments and a step count that is a number, goes on in fp32 with 32 bits"""
+    a, b = torch.nn.Parameter(torch.ones(8)), torch.nn.Parameter(torch.ones(8, dtype=torch.bfloat16))
+    theirs = torch.optim.AdamW([a, b], lr=0.5, betas=(0.8, 0.9))
+    a.grad, b.grad = torch.ones(8), torch.ones(8, dtype=torch.bfloat16)
+    theirs.step()
+    d = theirs.state_dict()
+    d["state"][1]["step"] = 1
+    opt = AdamW([a, b], state_bits=8)
+    opt.load_state_dict(d)
+    g = opt.param_groups[0]
+    assert (g["lr"], g["betas"], g["state_bits"]) == (0.5, (0.8, 0.9), 32)
+    for p in (a, b):
+        s = opt.state[p]
+        assert all(s[k].dtype == torch.float32 for k in ("step", "exp_avg", "exp_avg_sq")) and float(s["step"]) == 1.0
+        assert torch.equal(s["exp_avg"], theirs.state[p]["exp_avg"].float())
+    for variant in ("amsgrad", "maximize"):
+        with pytest.raises(_C.XqError, match="amsgrad and maximize"):
+            opt.load_state_dict(torch.optim.AdamW([a, b], **{variant: True}).state_dict())
+
+
+def test_copies_and_groups_keep_the_options():
+    q = torch.nn.Parameter(torch.zeros(4))
+    opt = AdamW([q], state_bits=8, max_grad_norm=0.5)
+    assert copy.deepcopy(opt).max_grad_norm == 0.5 and copy.deepcopy(opt).param_groups[0]["state_bits"] == 8
+    for bits in (16, None):
+        with pytest.raises(_C.XqError, match="state_bits"):
+            opt.add_param_group({"params": [torch.nn.Parameter(torch.zeros(2))], "state_bits": bits})

@@ -492,6 +492,19 @@ struct LinearCrossEntropyBackward : public Node {
         const Tensor x = x_.unpack(), w = w_.unpack(), labels = labels_.unpack(), saved = saved_.unpack(shared_from_this());
         c10::DeviceGuard guard(x.device());
         const bool again = at::GradMode::is_enabled();
+        // Gradients that go on to another stream make that stream wait for this one; under capture that ends the process.  A leaf's stream is that of
+        // the oldest graph which still holds it, so an eager loss that lives is enough.
+        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+        if (hipStreamIsCapturing((hipStream_t)stream_of(x), &capture) == hipSuccess && capture != hipStreamCaptureStatusNone) {
+            const c10::StreamId here = c10::hip::getCurrentHIPStream(x.device().index()).unwrap().id();
+            for (uint32_t i = 0; i < num_outputs(); ++i) {
+                const auto& edge = next_edge(i);
+                const auto there = edge.function ? edge.function->stream() : std::nullopt;
+                if (task_should_compute_output(i) && there && there->id() != here)
+                    throw std::runtime_error("linear_cross_entropy: a captured backward would hand its gradients to another stream; free the losses that were made "
+                                             "from the same tensors outside the capture, and make x inside it or let it be a leaf");
+            }
+        }
         {
             at::NoGradGuard no_grad;
             const Tensor g = cast_to(grads[0], at::kFloat).contiguous();
@@ -976,11 +989,12 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         std::vector<xq_adamw_tensor> q;
         std::vector<Tensor> keep;
         std::vector<at::TensorImpl*> written;     // (the lists hold them)
-        std::vector<std::pair<const char*, const char*>> once;        // what the step writes, from and to: named twice it would be written by two blocks at a time
-        auto note = [&](const Tensor& t) { once.emplace_back((const char*)t.data_ptr(), (const char*)t.data_ptr() + nbytes(t)); };
+        struct Span { const char *from, *to; bool write; };
+        std::vector<Span> once;        // what the step writes and the gradients: written twice, or read where another block writes, the result would hang on the order
+        auto note = [&](const Tensor& t, bool write = true) { once.push_back({(const char*)t.data_ptr(), (const char*)t.data_ptr() + nbytes(t), write}); };
         q.reserve(n);
         written.reserve(6 * n);
-        once.reserve(6 * n);
+        once.reserve(7 * n);
         for (Py_ssize_t i = 0; i < n; ++i) {
             const Tensor& gr = g[i];
             xq_adamw_tensor a{};
@@ -1025,12 +1039,17 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                 }
                 written.push_back(st.unsafeGetTensorImpl());
                 note(st);
+                if (a.numel && a.grad == gr.data_ptr()) note(gr, false);
             }
             if (a.numel) q.push_back(a);
         }
-        std::sort(once.begin(), once.end());
-        if (std::adjacent_find(once.begin(), once.end(), [](const auto& a, const auto& b) { return b.first < a.second; }) != once.end())
-            throw ArgError("adamw_step: two tensors share memory of a parameter, a state or a step count");
+        std::sort(once.begin(), once.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+        const char *read_to = nullptr, *written_to = nullptr;         // the ends of what came before
+        for (const Span& a : once) {
+            if (a.from < written_to || (a.write && a.from < read_to)) throw ArgError("adamw_step: two tensors share memory of a parameter, a state or a step count");
+            const char*& to = a.write ? written_to : read_to;
+            to = std::max(to, a.to);
+        }
         if (args[8] != Py_None) {
             const Tensor* lr = plain(args[8]);
             if (!lr || lr->scalar_type() != at::kFloat || lr->numel() != 1) throw ArgError("adamw_step: an lr tensor must be one fp32 element on the device");

@@ -118,7 +118,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
 
     Products accumulate in fp32, sums of exponentials in fp32 relative to the label's logit or the largest.  Gradients come in bf16; the
     probabilities in them are rounded to bf16 once (half a step, 2^-8, each), all but the label's.  H must be a multiple of 64.  First
-    derivatives only."""
+    derivatives only.  Under graph capture forward and backward go into the same graph, and no loss made outside it from the same x or weight may
+    still be alive (refused, for a weight whose rows need no copy)."""
     if not torch.compiler.is_compiling() and reduction in _C.LCE_REDUCTIONS:
         loss = native().cross_entropy(x, weight, labels, ignore_index, _C.LCE_REDUCTIONS[reduction], logit_scale)
         if loss is not None:

@@ -38,7 +38,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     """One AdamW step over all ``params``, in place, with the states they come with.
 
     Parameters and gradients are fp32 or bf16, tensor by tensor; parameters, states and step counts are contiguous and share no
-    memory (both refused otherwise; a gradient that is not contiguous is copied).  States are fp32, or, with both lists of scales
+    memory, with gradients neither (both refused otherwise; a gradient that is not contiguous is copied).  States are fp32, or, with both lists of scales
     given, 8-bit codes: int8 ``exp_avgs`` and uint8 ``exp_avg_sqs`` with fp32 scales for every 256 elements (``adamw_state_values``
     says what they stand for).  ``steps`` are fp32 tensors of one element each, advanced here.  ``lr`` may be a 0-dim fp32 tensor on
     the device: a captured step then follows it.
@@ -94,6 +94,15 @@ class AdamW(torch.optim.Optimizer):
         self.grad_norm: Optional[Tensor] = None
         super().__init__(params, dict(lr=lr, betas=betas, eps=eps, weight_decay=weight_decay, state_bits=state_bits))
 
+    def __getstate__(self) -> dict:
+        return {**super().__getstate__(), "max_grad_norm": self.max_grad_norm, "grad_norm": None}
+
+    def add_param_group(self, param_group: dict) -> None:
+        bits = param_group.get("state_bits", self.defaults["state_bits"])
+        if bits not in (8, 32):
+            raise _C.XqError(f"state_bits must be 8 or 32, got {bits}")
+        super().add_param_group(param_group)
+
     def _init_state(self, p: Tensor, state_bits: int) -> dict:
         state = self.state[p]
         if not state:
@@ -142,14 +151,26 @@ class AdamW(torch.optim.Optimizer):
         return loss
 
     def load_state_dict(self, state_dict) -> None:
+        """States of this class or of ``torch.optim.AdamW`` (a group of the latter goes on with 32 bits; its variants are refused)."""
+        for g in state_dict["param_groups"]:
+            if g.get("amsgrad") or g.get("maximize"):
+                raise _C.XqError("AdamW: amsgrad and maximize have no counterpart here")
         # the base class casts floating-point state, and codes with it, to the parameter's type
         super().load_state_dict(state_dict)
+        for g in self.param_groups:
+            g.setdefault("state_bits", 32)
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, own):
             if i in state_dict["state"]:
-                self.state[p] = {k: v.detach().to(_local(p).device, copy=True) if isinstance(v, Tensor) else v
-                                 for k, v in state_dict["state"][i].items()}
+                self.state[p] = {k: _state(v, _local(p).device) for k, v in state_dict["state"][i].items()}
+
+
+def _state(v, device):
+    """A copy of a loaded state on ``device``: codes as they are, all else (moments in bf16, a step count that is a number) in fp32"""
+    if isinstance(v, Tensor):
+        return v.detach().to(device, torch.float32 if v.is_floating_point() else v.dtype, copy=True)
+    return torch.tensor(float(v), device=device) if isinstance(v, (int, float)) else v
 
 
 def _local(t: Tensor) -> Tensor:
