@@ -79,3 +79,18 @@ def test_sizes():
         for p in (2, 3):
             ws = L.xq_lce_workspace_bytes(M, V, 4096, p)
             assert ws <= max(1 << 30, rows * 512) + rows * 64 + rows * 8 * (V // 256 + 1) + (2 * M * 4096 if p == 3 else 0) + (1 << 20)
+
+
+@pytest.mark.parametrize("M,V,H", [(1 << 24, 10, 64), (3, 1 << 28, 64), (3, 10, 1 << 24), (2 ** 63 - 1, 10, 64), (1, 2 ** 63 - 1, 64), (1 << 62, 1 << 62, 1 << 62)])
+def test_sizes_out_of_range(M, V, H):
+    """Launches that would have 2^32 threads and more, and sizes whose products pass 64 bits"""
+    L = _C.lib()
+    assert L.xq_lce_saved_bytes(M, V, H, 2) == -1 and L.xq_lce_workspace_bytes(M, V, H, 3) == -1
+    assert _fwd(M=M, V=V, H=H, ldx=H, ldw=H) == -1 and _bwd(M=M, V=V, H=H, ldx=H, ldw=H) == -1
+
+
+def test_largest_sizes():
+    L = _C.lib()
+    for M, V, H in (((1 << 24) - 1, 1000, 64), (1, (1 << 28) - 1, 64), (1, 1000, (1 << 24) - 64)):
+        for p in (0, 1, 2, 3):
+            assert L.xq_lce_workspace_bytes(M, V, H, p) > 0

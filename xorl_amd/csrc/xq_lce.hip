@@ -340,6 +340,18 @@ int compute_units() {
 // blocks of a product that run at a time, for lce_parts
 int slots(int tm) { return (tm == 2 ? 2 : 1) * compute_units(); }
 
+// a kernel may have as much LDS as it asks for on the current device; raised: by device (a race only repeats the call)
+int raise_lds(const void* kernel, int bytes, std::atomic<uint64_t>& raised) {
+    int dev = 0;
+    hipError_t e = hipGetDevice(&dev);
+    const uint64_t bit = 1ull << (dev & 63);
+    if (e == hipSuccess && dev < 64 && (raised.load(std::memory_order_relaxed) & bit)) return XQ_OK;
+    if (e == hipSuccess) e = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, bytes);
+    if (e != hipSuccess) { xq_set_error("xq_lce: cannot raise the dynamic LDS limit: %s", hipGetErrorString(e)); return XQ_ERR_LAUNCH; }
+    raised.fetch_or(bit, std::memory_order_relaxed);
+    return XQ_OK;
+}
+
 struct Plan {
     int tm, cols;                       // rows of a logits tile: 32 tm, and its columns
     int64_t rows_pad, piece, pieces;    // columns of the vocabulary at a time (a multiple of 256), and how many times
@@ -449,8 +461,9 @@ template <int TM, int TN, int ST, int MODE>
 int launch_logits(const LceLogitsArgs& a, int64_t rows, int64_t cols, hipStream_t s) {
     using T = LceTile<TM, TN, ST>;
     auto k = lce_logits_kernel<TM, TN, ST, MODE>;
-    static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
-    if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
+    static std::atomic<uint64_t> raised{0};
+    const int rc = raise_lds((const void*)k, T::LDS_BYTES, raised);
+    if (rc != XQ_OK) return rc;
     int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(cols, a.cols);
     if (T::AHEAD) blocks = std::min<int64_t>(blocks, compute_units());
     k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
@@ -467,8 +480,9 @@ template <int TM>
 int launch_product(const LceProductArgs& a, int64_t rows, hipStream_t s) {
     using T = LceTile<TM>;
     auto k = lce_product_kernel<TM>;
-    static const hipError_t once = hipFuncSetAttribute((const void*)k, hipFuncAttributeMaxDynamicSharedMemorySize, T::LDS_BYTES);
-    if (once != hipSuccess) { xq_set_error("xq_lce: %s", hipGetErrorString(once)); return XQ_ERR_LAUNCH; }
+    static std::atomic<uint64_t> raised{0};
+    const int rc = raise_lds((const void*)k, T::LDS_BYTES, raised);
+    if (rc != XQ_OK) return rc;
     int64_t blocks = xq_cdiv(rows, T::ROWS) * xq_cdiv(a.H, 256);
     if (a.parts) blocks = std::max<int64_t>(blocks, std::min<int64_t>(kLceMostParts * blocks, 3ll * slots(TM)));
     k<<<dim3((unsigned)blocks), 512, T::LDS_BYTES, s>>>(a);
@@ -478,10 +492,13 @@ int launch_product(int tm, const LceProductArgs& a, int64_t rows, hipStream_t s)
     return tm == 2 ? launch_product<2>(a, rows, s) : tm == 4 ? launch_product<4>(a, rows, s) : launch_product<8>(a, rows, s);
 }
 
+// (a launch has fewer than 2^32 threads: 256 a row in the gather, 512 for 64 columns of few rows)
+bool sizes_fit(int64_t M, int64_t V, int64_t H) { return M >= 0 && M < (1 << 24) && V >= 1 && V < (1 << 28) && H >= 1 && H < (1 << 24); }
+
 int check_problem(const char* who, const xq_lce_problem* q, const void* ws, int64_t ws_bytes, int64_t need, const void* saved, int64_t saved_need) {
     XQ_REQUIRE(q, "%s: the problem is NULL", who);
-    XQ_REQUIRE(q->M >= 0 && q->M < (1 << 30) && q->V >= 1 && q->V < (1 << 30), "%s: %lld rows, %lld columns of logits", who, (long long)q->M, (long long)q->V);
-    XQ_REQUIRE(q->H >= 64 && q->H % 64 == 0 && q->H < (1 << 24), "%s: the hidden size must be a multiple of 64, got %lld", who, (long long)q->H);
+    XQ_REQUIRE(sizes_fit(q->M, q->V, q->H), "%s: %lld rows, %lld columns of logits, hidden size %lld", who, (long long)q->M, (long long)q->V, (long long)q->H);
+    XQ_REQUIRE(q->H >= 64 && q->H % 64 == 0, "%s: the hidden size must be a multiple of 64, got %lld", who, (long long)q->H);
     XQ_REQUIRE(q->reduction >= XQ_LCE_NONE && q->reduction <= XQ_LCE_SUM, "%s: unknown reduction %d", who, q->reduction);
     XQ_REQUIRE(q->label_bytes == 4 || q->label_bytes == 8, "%s: labels are int32 or int64, got %d bytes", who, q->label_bytes);
     XQ_REQUIRE(q->logit_scale > 0.0f && q->logit_scale < INFINITY, "%s: logit_scale must be positive and finite, got %g", who, (double)q->logit_scale);
@@ -500,12 +517,12 @@ int check_problem(const char* who, const xq_lce_problem* q, const void* ws, int6
 using namespace xq;
 
 extern "C" int64_t xq_lce_saved_bytes(int64_t M, int64_t V, int64_t H, int keep) {
-    if (M < 0 || V < 1 || H < 1) return -1;
+    if (!sizes_fit(M, V, H)) return -1;
     return saved_of(nullptr, M, V, H, keep).bytes;
 }
 
 extern "C" int64_t xq_lce_workspace_bytes(int64_t M, int64_t V, int64_t H, int pass) {
-    if (M < 0 || V < 1 || H < 1) return -1;
+    if (!sizes_fit(M, V, H)) return -1;
     return scratch_of(nullptr, M, V, H, pass).bytes;
 }
 
