@@ -340,6 +340,46 @@ def test_gradients_against_differences(hip_device):
     assert abs(got - slope) <= float((bx * vx.abs()).sum() + (bw * vw.abs()).sum()) + 1e-6 * abs(slope)
 
 
+def _exact_head_gradient(x, w, labels, up):
+    """The head's gradient in 64 bits, and the sum of its terms' magnitudes"""
+    xd, wd = x.double(), w.double()
+    p = torch.softmax(xd @ wd.t(), -1)
+    p[torch.arange(len(labels), device=x.device), labels] -= 1
+    p *= up.double()[:, None]
+    return p.t() @ xd, p.abs().t() @ xd.abs()
+
+
+@pytest.mark.parametrize("M", [1, 2, 31, 32, 33, 64, 65, 96, 97, 128])
+def test_head_gradient_of_few_tokens_is_rounded_once(hip_device, M):
+    """Half a step of the result (2^-8); G in two bf16 numbers (2^-16 of each term), products in fp32 (at most 256 sums of 2^-24 each), p to the
+    logits' own error: 192 sums of 2^-24 of the magnitudes of a logit's terms, in numerator and denominator, and ten roundings of the exponential"""
+    x, w, labels = _inputs(M, 1500, 192, 300 + M, hip_device, std=0.05)
+    labels[M // 2] = labels[0]                                # (two tokens of one row)
+    w.requires_grad_(True)
+    up = torch.randn(M, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(M))
+    dw, = torch.autograd.grad(linear_cross_entropy(x, w, labels, reduction="none"), w, up)
+    want, terms = _exact_head_gradient(x, w.detach(), labels, up)
+    logit_terms = float((x.double().abs() @ w.detach().double().abs().t()).max())
+    near = 2.0 ** -16 + 256 * U + 2 * (192 * logit_terms + 10) * U
+    assert bool(((dw.double() - want).abs() <= 2.0 ** -8 * want.abs() + 1.01 * near * terms + 1e-37).all())
+
+
+@pytest.mark.parametrize("reduction,M,grad", [("mean", 255, 1.0), ("mean", 100, 1.0), ("sum", 255, 257 / 256), ("sum", 300, 1.0)])
+def test_what_all_rows_share_is_not_rounded(hip_device, reduction, M, grad):
+    """1 / 255 and 257 / 256 lie in the middle between two bf16 numbers: rounded, the whole gradient would be off by 2^-8.  What may stay of that is the label's
+    1 - p, off by the largest p where it rounds to 1 (upstream gradients by row are rounded with it)"""
+    x, w, labels = _inputs(M, 4096, 128, 400 + M, hip_device, std=0.01, lift=0.0)
+    w.requires_grad_(True)
+    dw, = torch.autograd.grad(linear_cross_entropy(x, w, labels, reduction=reduction), w, torch.tensor(grad, device=hip_device))
+    up = torch.full((M,), grad / (M if reduction == "mean" else 1), dtype=torch.float64, device=hip_device)
+    want, _ = _exact_head_gradient(x, w.detach(), labels, up)
+    p = float(torch.softmax(x.double() @ w.detach().double().t(), -1).max())
+    assert p < 2.0 ** -10
+    off = float((dw.double() * want).sum() / (want * want).sum()) - 1
+    # the result's own roundings are of either sign: 2^-8 / sqrt of half a million elements
+    assert abs(off) <= p + 2.0 ** -8 / 128
+
+
 def test_backward_twice_and_expanded_upstream(hip_device):
     x, w, labels = _inputs(100, 800, 128, 59, hip_device)
     x.requires_grad_(True)

@@ -58,7 +58,7 @@ struct LceLogitsArgs {
     LceRows rows;
     float scale2;                       // of the logits, times log2(e)
     const float* ref;                   // EXP: reference of a row, in log2 units;  GRAD: log2 of the row's sum of exponentials
-    const float* grad;                  // GRAD: upstream gradient of a row times the logit scale
+    const float* grad;                  // GRAD: upstream gradient of a row, but for what all rows share
     const float* rest;                  // GRAD: 1 - p of the label
     f32x2* part;                        // STATS, EXP: [column tile][rows_pad] (largest, sum)
     float* at_label;                    // STATS: the label's logit
@@ -71,6 +71,13 @@ struct LceLogitsArgs {
     float* alpha;
 };
 constexpr float kLceFar = 64.0f;        // log2
+
+// G of few tokens is kept as two bf16 numbers, the value and what its rounding left, in two runs of columns (K-steps of the product) of this length
+// each: a row of the head's gradient is often one token's, whose rounded G would be a second error of half a step beside the result's own.  With
+// many tokens the errors of G are as many and no larger, and the product would be twice the work; for 128 it is still level with writing the
+// gradient (512 FLOP an element against 2 bytes).
+constexpr int kLceSplit = 128;
+__device__ __forceinline__ int lce_half(int count) { return count <= kLceSplit ? (count + 31) & ~31 : 1 << 30; }
 
 // The first of a stream of K-steps, all stages but one: K-step k of it goes to stage k % STAGES.  issue(at, part, stage): one of NP direct loads of a K-step.
 template <typename T, typename Advance, typename Issue>
@@ -226,6 +233,10 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     const int n_a = MODE == kLceGrad ? g.n_v : count, n_b = MODE == kLceGrad ? count : g.n_v;
     const int tiles_a = (n_a + T::ROWS - 1) / T::ROWS, cols = MODE == kLceGrad || TM > 4 ? 256 : min(g.cols, T::COLS), tiles_b = (n_b + cols - 1) / cols, nk = g.H / T::BK;
 
+    const int half = MODE == kLceGrad ? lce_half(count) : 0;
+    // a column of the tile to a token of it
+    auto token = [&](int c) -> int { return c >= half ? c - half : c; };
+
     LceWalk walk(tiles_a * tiles_b);
     int ta, tb;
     auto find = [&]() -> bool {                             // the block's next tile
@@ -244,14 +255,14 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             const bool of_a = p < T::AP;
             const int rt = of_a ? wave * (T::ROWS / 8) + p * 16 + (lane >> 2) : wave * (T::COLS / 8) + (p - T::AP) * 16 + (lane >> 2);
             // (rows behind the last, of either side or of the tile's columns: that one again, for nothing)
-            const int n = of_a ? min(ta * T::ROWS + rt, n_a - 1) : min(tb * cols + min(rt, cols - 1), n_b - 1);
+            const int n = of_a ? min(ta * T::ROWS + rt, n_a - 1) : min(tb * cols + (MODE == kLceGrad ? token(rt) : min(rt, cols - 1)), n_b - 1);
             const bool tokens = of_a != (MODE == kLceGrad);
             const int64_t row = tokens ? g.rows.row[n] : g.first_v + n;
             src[p] = (of_a ? g.A + row * g.lda : g.B + row * g.ldb) + (((lane & 3) ^ ((rt >> 2) & 2)) << 3);
         }
         if (tid < N_INFO) {
             // (GRAD: the arrays are as long as whole tiles; behind the last row up = 0, lse = inf)
-            const int r = MODE == kLceGrad ? tb * 256 + tid : min(ta * T::ROWS + tid, count - 1);
+            const int r = MODE == kLceGrad ? tb * 256 + token(tid) : min(ta * T::ROWS + tid, count - 1);
             about[0] = __int_as_float(g.rows.label[r] - g.first_v);
             if (MODE != kLceStats) about[1] = g.ref[r];
             if (MODE == kLceGrad) { about[2] = g.grad[r]; about[3] = g.rest[r]; }
@@ -343,6 +354,15 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                         const float p = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], g.scale2, -lse[e]));
                         acc[i][j][e] = up[e] * (__float_as_int(label[e]) == v ? -rest[e] : p);
                     }
+                }
+                if (wn * 64 + 16 * j >= half) {             // what the rounding of the same token's value left (nothing of an infinity)
+#pragma unroll
+                    for (int i = 0; i < TM; ++i)
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const float hi = bf16_to_f32(to_bf16(acc[i][j][e]));
+                            acc[i][j][e] = fabsf(hi) == INFINITY ? 0.0f : acc[i][j][e] - hi;
+                        }
                 }
             }
         } else {
@@ -472,8 +492,9 @@ struct LceProductArgs {
     const float* alpha;                 // (of row tiles that were done again; 1 otherwise)
     const int32_t* redo;
     int32_t add;
-    bf16_t* out16;                      // or [rows, ld16] bf16
+    bf16_t* out16;                      // or [rows, ld16] bf16: times *scale (NULL: 1)
     int64_t ld16;
+    const float* scale;
 };
 
 // Parts of a contraction of E . W: as many as leave the least of the chip idle, where tiles alone would (a part costs its sums once more in
@@ -498,7 +519,8 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
     extern __shared__ __attribute__((aligned(16))) unsigned char dsm[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
-    const int count = __builtin_amdgcn_readfirstlane(*g.count), rows = g.rows < 0 ? count : g.rows, k = g.k < 0 ? count : g.k;
+    const int count = __builtin_amdgcn_readfirstlane(*g.count), rows = g.rows < 0 ? count : g.rows;
+    const int half = g.k < 0 ? lce_half(count) : 1 << 30, k = g.k >= 0 ? g.k : half <= kLceSplit ? 2 * half : count, last = (g.k < 0 ? count : k) - 1;
     const int tiles_a = (rows + T::ROWS - 1) / T::ROWS, tiles_b = (g.H + 255) >> 8, tiles = tiles_a * tiles_b, pairs = (k + 63) >> 6;        // of K-steps
     const int parts = g.parts ? __builtin_amdgcn_readfirstlane(*g.parts) : 1;
     // an XCD has an eighth of all tiles and parts, in order of the parts: what it reads of E and W at a time are few rows and the same K-steps
@@ -525,7 +547,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
                 lce_load_lds(stage + wave * rows8 * 64 + part * 1024, a_src + (int64_t)kt * (T::ROWS * 32) + part * 512);
         } else {
             const int p = part - T::AP;
-            const int row = min((kt0 + kt) * 32 + kr + 2 * p, k - 1);
+            const int at = (kt0 + kt) * 32, row = min((at >= half ? at - half : at) + kr + 2 * p, last);
             lce_load_lds(stage + T::A_BYTES + wave * 2048 + p * 1024, b_col[p] + row * g.ldb);
         }
     };
@@ -544,13 +566,14 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_product_kernel(LcePr
 
     const int row_w = r0 + wm * 16 * TM + l16, col_w = c0 + wn * 64;
     if (g.out16) {
+        const float scale = g.scale ? *g.scale : 1.0f;
 #pragma unroll
         for (int i = 0; i < TM; ++i) {
             const int row = row_w + 16 * i;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
                 // eight columns in a row for each lane: fragments 2 q and 2 q + 1 exchange halves, then rows of sixteen lanes
-                const f32x4 u = acc[i][2 * q], v = acc[i][2 * q + 1];
+                const f32x4 u = acc[i][2 * q] * scale, v = acc[i][2 * q + 1] * scale;
                 uint32_t x[2] = {pack_bf16x2(u[0], u[1]), pack_bf16x2(u[2], u[3])}, y[2] = {pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3])};
 #pragma unroll
                 for (int d = 0; d < 2; ++d) {

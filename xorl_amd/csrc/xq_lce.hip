@@ -17,7 +17,8 @@
 //    than 2^64 times e above it; a piece that finds one takes the largest as the new reference (O and Z' are scaled to it) and is done
 //    again for the row tiles concerned.  bf16 keeps E to half a step (2^-9 of each term, of either sign).
 //  * A trained head: the backward forms the logits again with the roles exchanged, G = g (p - [v = t]) as bf16 with the tokens along the
-//    contraction, and multiplies it with the rows that count.
+//    contraction, and multiplies it with the rows that count.  What all rows share of g (the mean's 1 / count, the logit scale) is left to the
+//    result in 32 bits: in G it would be one and the same rounding error, up to half a step, of the whole gradient.
 //
 // 8192 rows, 5735 of which count, under [131072, 4096], forward and backward: 10.1 ms, in two pieces of 2.5 (logits) and 2.45 ms (product) each, 0.1 ms of
 // everything else.  One row, scored: 192 us.  96 rows under [32003, 2048], forward and backward: 82 us, of which 28 and 27 are the products and the rest
@@ -277,6 +278,13 @@ struct Upstream {
     const int32_t* count;
     float scale;
 };
+// (upstream is the product of the two behind it)
+__device__ __forceinline__ float upstream_of_row(const Upstream& u, int64_t row) { return u.reduction == XQ_LCE_NONE ? u.grad[row] : 1.0f; }
+__device__ __forceinline__ float upstream_of_all(const Upstream& u) {
+    const int count = *u.count;
+    if (u.reduction == XQ_LCE_NONE || count == 0) return u.scale;
+    return u.reduction == XQ_LCE_MEAN ? *u.grad * u.scale / (float)count : *u.grad * u.scale;
+}
 __device__ __forceinline__ float upstream(const Upstream& u, int64_t row) {
     const float g = u.grad[u.reduction == XQ_LCE_NONE ? row : 0] * u.scale;
     return u.reduction == XQ_LCE_MEAN ? g / (float)*u.count : g;
@@ -312,12 +320,13 @@ __global__ void __launch_bounds__(64) lce_dx_kernel(const int32_t* place, const 
 
 // the factors of the head's gradient by row, and the rows of x that count in order
 __global__ void __launch_bounds__(256) lce_factors_kernel(LceRows rows, int64_t M_pad, const float* lse2, const float* rest, Upstream u, float* lse_out, float* up_out,
-                                                          float* rest_out) {
+                                                          float* rest_out, float* all_out) {
     const int64_t c = (int64_t)blockIdx.x * 256 + threadIdx.x;
     if (c >= M_pad) return;
     const bool in = c < *rows.count;
     lse_out[c] = in ? lse2[c] : INFINITY;
-    up_out[c] = in ? upstream(u, rows.row[c]) : 0.0f;
+    up_out[c] = in ? upstream_of_row(u, rows.row[c]) : 0.0f;
+    if (c == 0) *all_out = upstream_of_all(u);
     rest_out[c] = in ? rest[c] : 0.0f;
 }
 __global__ void __launch_bounds__(256) lce_gather_kernel(LceRows rows, const bf16_t* x, int64_t ldx, int H, bf16_t* out) {
@@ -600,7 +609,7 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
         const Plan h = plan_head(M, V);
         const Scratch c = scratch_of(workspace, M, V, H, XQ_LCE_KEEP_HEAD_BWD);
         if (M > 0) {
-            lce_factors_kernel<<<dim3((unsigned)(h.rows_pad / 256)), 256, 0, st>>>(rows, h.rows_pad, s.lse2, s.rest, u, c.ref, c.up, c.z);
+            lce_factors_kernel<<<dim3((unsigned)(h.rows_pad / 256)), 256, 0, st>>>(rows, h.rows_pad, s.lse2, s.rest, u, c.ref, c.up, c.z, c.alpha);
             lce_gather_kernel<<<dim3((unsigned)M), 256, 0, st>>>(rows, (const bf16_t*)q->x, q->ldx, (int)H, c.x);
         }
         LceLogitsArgs a = {};
@@ -614,7 +623,7 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
             LceProductArgs o = {};
             o.image = c.image; o.image_steps = a.image_steps; o.rows = (int32_t)n; o.k = -1; o.count = s.count;
             o.B = c.x; o.ldb = H; o.H = (int32_t)H;
-            o.out16 = (bf16_t*)dw + v0 * lddw; o.ld16 = lddw;
+            o.out16 = (bf16_t*)dw + v0 * lddw; o.ld16 = lddw; o.scale = M > 0 ? c.alpha : nullptr;
             if ((rc = launch_product(h.tm, o, n, st)) != XQ_OK) return rc;
         }
     }

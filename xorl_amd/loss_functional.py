@@ -116,9 +116,10 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
     (minus the label's log-probability), 0 where the label is ``ignore_index``.  Such rows get zero gradients and cost nothing.  A label outside
     [0, V) gives its row NaN, in the loss and in the gradients, the weight's with it.
 
-    Products accumulate in fp32, sums of exponentials in fp32 relative to the label's logit or the largest.  Gradients come in bf16; the
-    probabilities in them are rounded to bf16 once (half a step, 2^-8, each), all but the label's.  H must be a multiple of 64.  First
-    derivatives only.  Under graph capture forward and backward go into the same graph, and no loss made outside it from the same x or weight may
+    Products accumulate in fp32, sums of exponentials in fp32 relative to the label's logit or the largest.  Gradients come in bf16. For x, the
+    probabilities in them are rounded to bf16 once (half a step, 2^-8, each), all but the label's; for the weight, probabilities and the label's
+    1 - p times the row's upstream gradient are, unless at most 128 rows count (then 2^-16).  H must be a multiple of 64.  First derivatives
+    only.  Under graph capture forward and backward go into the same graph, and no loss made outside it from the same x or weight may
     still be alive (refused, for a weight whose rows need no copy)."""
     if not torch.compiler.is_compiling() and reduction in _C.LCE_REDUCTIONS:
         loss = native().cross_entropy(x, weight, labels, ignore_index, _C.LCE_REDUCTIONS[reduction], logit_scale)
