@@ -49,6 +49,17 @@ struct LceRows {                        // what is kept of the labels: the rows 
     const int32_t* label;               // -1: out of range
 };
 
+// Up to kLceOwnRows labels: every wave of a STATS launch finds the rows that count by itself, a lane each
+constexpr int kLceOwnRows = 64;
+struct LceLabels {
+    const void* label;                  // NULL: LceRows has them
+    int32_t bytes, M;
+    int64_t ignore, V;
+};
+__device__ __forceinline__ int64_t lce_label(const void* labels, int bytes, int64_t i) {
+    return bytes == 8 ? ((const int64_t*)labels)[i] : (int64_t)((const int32_t*)labels)[i];
+}
+
 struct LceLogitsArgs {
     const bf16_t* A;
     const bf16_t* B;
@@ -56,6 +67,7 @@ struct LceLogitsArgs {
     int32_t H, first_v, n_v;            // the piece of the vocabulary: its first row of the head and how many
     int32_t cols;                       // of a tile, up to 256 (GRAD, and above 128 rows: 256)
     LceRows rows;
+    LceLabels labels;                   // STATS
     float scale2;                       // of the logits, times log2(e)
     const float* ref;                   // EXP: reference of a row, in log2 units;  GRAD: log2 of the row's sum of exponentials
     const float* grad;                  // GRAD: upstream gradient of a row, but for what all rows share
@@ -229,7 +241,18 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     float* const info = (float*)(ends + T::ROWS * 32);      // EXP, STATS: label and reference by row;  GRAD: label, lse, up, rest by column
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
-    const int count = __builtin_amdgcn_readfirstlane(*g.rows.count);
+    constexpr bool OWN = MODE == kLceStats && 32 * TM <= kLceOwnRows;
+    int count, own_row = 0, own_label = -1;                 // (a lane's of the rows that count)
+    if (OWN && g.labels.label) {
+        const int64_t label = lane < g.labels.M ? lce_label(g.labels.label, g.labels.bytes, lane) : g.labels.ignore;
+        const uint64_t in = __ballot(label != g.labels.ignore), below = (1ull << lane) - 1;
+        count = __builtin_popcountll(in);
+        const int to = 4 * (in >> lane & 1 ? __builtin_popcountll(in & below) : count + __builtin_popcountll(~in & below));
+        own_row = __builtin_amdgcn_ds_permute(to, lane);
+        own_label = __builtin_amdgcn_ds_permute(to, label >= 0 && label < g.labels.V ? (int)label : -1);
+    } else {
+        count = __builtin_amdgcn_readfirstlane(*g.rows.count);
+    }
     const int n_a = MODE == kLceGrad ? g.n_v : count, n_b = MODE == kLceGrad ? count : g.n_v;
     const int tiles_a = (n_a + T::ROWS - 1) / T::ROWS, cols = MODE == kLceGrad || TM > 4 ? 256 : min(g.cols, T::COLS), tiles_b = (n_b + cols - 1) / cols, nk = g.H / T::BK;
 
@@ -249,6 +272,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     // ---- sources of the direct loads: a wave brings in an eighth of either side's rows, 64 bytes of each, 16 rows to a load; and what
     // the ends want to know of the rows (EXP, STATS) or columns (GRAD) that are tokens
     constexpr int N_INFO = MODE == kLceGrad ? 256 : T::ROWS;
+    auto own_label_of = [&](int r) -> int { return __shfl(own_label, r); };         // (N_INFO threads: whole waves)
     auto sources = [&](const bf16_t* (&src)[T::NP], float (&about)[4]) {
 #pragma unroll
         for (int p = 0; p < T::NP; ++p) {
@@ -257,13 +281,13 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             // (rows behind the last, of either side or of the tile's columns: that one again, for nothing)
             const int n = of_a ? min(ta * T::ROWS + rt, n_a - 1) : min(tb * cols + (MODE == kLceGrad ? token(rt) : min(rt, cols - 1)), n_b - 1);
             const bool tokens = of_a != (MODE == kLceGrad);
-            const int64_t row = tokens ? g.rows.row[n] : g.first_v + n;
+            const int64_t row = !tokens ? g.first_v + n : OWN && g.labels.label ? __shfl(own_row, n) : g.rows.row[n];
             src[p] = (of_a ? g.A + row * g.lda : g.B + row * g.ldb) + (((lane & 3) ^ ((rt >> 2) & 2)) << 3);
         }
         if (tid < N_INFO) {
             // (GRAD: the arrays are as long as whole tiles; behind the last row up = 0, lse = inf)
             const int r = MODE == kLceGrad ? tb * 256 + token(tid) : min(ta * T::ROWS + tid, count - 1);
-            about[0] = __int_as_float(g.rows.label[r] - g.first_v);
+            about[0] = __int_as_float((OWN && g.labels.label ? own_label_of(r) : g.rows.label[r]) - g.first_v);
             if (MODE != kLceStats) about[1] = g.ref[r];
             if (MODE == kLceGrad) { about[2] = g.grad[r]; about[3] = g.rest[r]; }
             if (MODE == kLceExp && g.again) {

@@ -21,8 +21,8 @@
 //    result in 32 bits: in G it would be one and the same rounding error, up to half a step, of the whole gradient.
 //
 // 8192 rows, 5735 of which count, under [131072, 4096], forward and backward: 10.1 ms, in two pieces of 2.5 (logits) and 2.45 ms (product) each, 0.1 ms of
-// everything else.  One row, scored: 192 us.  96 rows under [32003, 2048], forward and backward: 82 us, of which 28 and 27 are the products and the rest
-// six small launches.
+// everything else.  One row, scored: 188 us (192 with a launch of its own that lists the rows, as above 64 rows).  96 rows under [32003, 2048], forward and
+// backward: 82 us, of which 27 and 27 are the products and the rest four small launches.
 #include <algorithm>
 #include <atomic>
 
@@ -43,16 +43,12 @@ struct Prep {
     int32_t label_bytes;
     int64_t M, M_pad, V, ignore;
     int32_t *count, *row, *label, *place;           // place: of a row of x among those that count, or -1
-    float* at_label;                                // NaN until the scores' tiles find it; or NULL
     int32_t* redo;                                  // flags to clear
     int32_t n_redo;
     float* loss_out;                                // losses by row, 0 for those that do not count; or NULL
     int32_t tile_rows, tiles_h, steps, slots;       // of E . W, for the parts of its contraction (count[1])
 };
-__device__ __forceinline__ int64_t label_of(const Prep& a, int64_t i) {
-    if (i >= a.M) return a.ignore;
-    return a.label_bytes == 8 ? ((const int64_t*)a.labels)[i] : (int64_t)((const int32_t*)a.labels)[i];
-}
+__device__ __forceinline__ int64_t label_of(const Prep& a, int64_t i) { return i < a.M ? lce_label(a.labels, a.label_bytes, i) : a.ignore; }
 // a thread's label among 1024: whether it counts, and how many before it do; all: how many of the 1024
 __device__ __forceinline__ bool place_of(bool in, int* before, int* all, int* wave_n) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -74,7 +70,6 @@ __device__ __forceinline__ void write_row(const Prep& a, int64_t i, int64_t labe
     if (in) {
         a.row[c] = (int)i;
         a.label[c] = label >= 0 && label < a.V ? (int)label : -1;
-        if (a.at_label) a.at_label[c] = __builtin_nanf("");
     }
     if (i < a.M) {
         a.place[i] = in ? c : -1;
@@ -94,6 +89,23 @@ __device__ __forceinline__ void write_rest(const Prep& a, int n) {
         a.label[c] = -1;
     }
     for (int i = threadIdx.x; i < a.n_redo; i += 1024) a.redo[i] = 0;
+}
+
+// A block of 1024 threads finds the rows that count, of up to kBeginRows labels, and notes the sixteen from first on; the first block does what
+// lce_prepare_kernel does
+__device__ __forceinline__ void own_rows_of(const Prep& a, int64_t first, int* count, int* wave_n, int* rows, int* labels) {
+    const int64_t i = threadIdx.x, label = label_of(a, i);
+    int at;
+    const bool in = place_of(label != a.ignore, &at, count, wave_n);
+    if (in && at >= first && at < first + 16) {
+        rows[at - first] = (int)i;
+        labels[at - first] = label >= 0 && label < a.V ? (int)label : -1;
+    }
+    if (blockIdx.x == 0) {
+        write_row(a, i, label, in, at);
+        write_rest(a, *count);
+    }
+    __syncthreads();
 }
 
 __global__ void __launch_bounds__(1024) lce_prepare_kernel(Prep a) {
@@ -122,18 +134,7 @@ __global__ void __launch_bounds__(1024) lce_target_kernel(Prep a, int own_rows, 
     const int64_t first = (int64_t)blockIdx.x * 16, c = first + wave;
     int count;
     if (own_rows) {
-        const int64_t i = threadIdx.x, label = label_of(a, i);
-        int at;
-        const bool in = place_of(label != a.ignore, &at, &count, wave_n);
-        if (in && at >= first && at < first + 16) {
-            rows[at - first] = (int)i;
-            labels[at - first] = label >= 0 && label < a.V ? (int)label : -1;
-        }
-        if (blockIdx.x == 0) {
-            write_row(a, i, label, in, at);
-            write_rest(a, count);
-        }
-        __syncthreads();
+        own_rows_of(a, first, &count, wave_n, rows, labels);
     } else {
         count = *a.count;
     }
@@ -172,14 +173,13 @@ struct Join {
 
 // in the first 16 threads of a block, for rows that count: the row's join
 template <typename F>
-__device__ __forceinline__ bool join_rows(const Join& a, f32x2 start, F fold, f32x2* out, int64_t* row) {
+__device__ __forceinline__ bool join_rows(const Join& a, int count, f32x2 start, F fold, f32x2* out, int64_t* row) {
     __shared__ f32x2 lds[16][16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t r = (int64_t)blockIdx.x * 16 + (lane & 15);
-    const int count = *a.count;
     if ((int64_t)blockIdx.x * 16 >= count) return false;
     f32x2 v = start;
-    const f32x2* p = a.part + min(r, (int64_t)count - 1);
+    const f32x2* p = a.part + r;                            // (behind the last row: whatever is there, for nothing)
 #pragma unroll 8
     for (int t = threadIdx.x >> 4; t < a.tiles; t += 64) v = fold(v, p[t * a.rows_pad]);
 #pragma unroll
@@ -209,7 +209,7 @@ __device__ __forceinline__ void add_piece(const Join& a, int64_t r, float sum, f
 __global__ void __launch_bounds__(1024) lce_sum_kernel(Join a) {
     f32x2 v;
     int64_t r;
-    if (!join_rows(a, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
+    if (!join_rows(a, *a.count, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
     float z, ref;
     add_piece(a, r, v[1], &z, &ref);
     a.z[r] = z;
@@ -222,38 +222,51 @@ struct RowEnd {
     const int32_t* row;
     float* out;                         // losses by row of x, or NULL
 };
-__device__ __forceinline__ void end_row(const RowEnd& e, int64_t c, float z, float ref, float t) {
+__device__ __forceinline__ void end_row(const RowEnd& e, int64_t c, int row, float z, float ref, float t) {
     const float et = __builtin_amdgcn_exp2f(t - ref), sum = z + et;
     const float loss = ref == t ? log1pf(z) : logf(sum) + (ref - t) * kLn2;
     e.loss[c] = loss;
-    if (e.out) e.out[e.row[c]] = loss;
+    if (e.out) e.out[row] = loss;
     e.inv[c] = 1.0f / sum;
     e.rest[c] = z / sum;
     e.lse2[c] = ref == t ? log1pf(z) * kLog2e + t : log2f(sum) + ref;
 }
 
-// STATS: joins and ends
-__global__ void __launch_bounds__(1024) lce_score_kernel(Join a, const float* at_label, RowEnd e) {
+// STATS: joins and ends.  own_rows: as the logits kernel, every block finds the rows that count by itself, and the first notes them
+__global__ void __launch_bounds__(1024) lce_score_kernel(Join a, Prep p, int own_rows, const float* at_label, RowEnd e) {
+    __shared__ int wave_n[16], rows[16], labels[16];
+    const int64_t first = (int64_t)blockIdx.x * 16, c = first + (threadIdx.x & 15);
+    int count, row = 0, label = -1;
+    // (read before the count is known: arrays as long as whole tiles)
+    const float found = at_label[c];
+    if (own_rows) {
+        own_rows_of(p, first, &count, wave_n, rows, labels);
+        row = rows[threadIdx.x & 15];
+        label = labels[threadIdx.x & 15];
+    } else {
+        row = p.row[c];
+        label = p.label[c];
+        count = *a.count;
+    }
     f32x2 v;
     int64_t r;
     auto fold = [](f32x2 p, f32x2 q) {
-        const float top = fmaxf(p[0], q[0]);
-        if (top == -INFINITY) return f32x2{top, p[1] + q[1]};
-        return f32x2{top, p[1] * __builtin_amdgcn_exp2f(p[0] - top) + q[1] * __builtin_amdgcn_exp2f(q[0] - top)};
+        const float top = fmaxf(p[0], q[0]), by = top == -INFINITY ? 0.0f : top;
+        return f32x2{top, p[1] * __builtin_amdgcn_exp2f(p[0] - by) + q[1] * __builtin_amdgcn_exp2f(q[0] - by)};
     };
-    if (!join_rows(a, f32x2{-INFINITY, 0.0f}, fold, &v, &r)) return;
-    const float t = at_label[r];
+    if (!join_rows(a, count, f32x2{-INFINITY, 0.0f}, fold, &v, &r)) return;
+    const float t = label >= 0 ? found : __builtin_nanf("");
     const float ref = v[0] > t ? v[0] : t;
-    end_row(e, r, v[1] * __builtin_amdgcn_exp2f(v[0] - ref), ref, t);
+    end_row(e, r, row, v[1] * __builtin_amdgcn_exp2f(v[0] - ref), ref, t);
 }
 // EXP: the last piece's sums, and ends; the label's logit is the first reference
 __global__ void __launch_bounds__(1024) lce_end_kernel(Join a, const float* at_label, RowEnd e) {
     f32x2 v;
     int64_t r;
-    if (!join_rows(a, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
+    if (!join_rows(a, *a.count, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
     float z, ref;
     add_piece(a, r, v[1], &z, &ref);
-    end_row(e, r, z, ref, at_label[r]);
+    end_row(e, r, e.row[r], z, ref, at_label[r]);
 }
 
 // sum or mean of the losses: one block, in an order that the sizes fix
@@ -549,8 +562,7 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
     const bool none = q->reduction == XQ_LCE_NONE;
     const int row_tiles = (int)xq_cdiv(M, 32 * p.tm);
     const RowEnd end = {s.inv, s.rest, s.lse2, s.loss, s.row, none ? loss : nullptr};
-    const Prep prep = {q->labels, q->label_bytes, M, p.rows_pad, V, q->ignore_index, s.count, s.row, s.label, s.place,
-                       keep == XQ_LCE_KEEP_DX ? nullptr : s.at_label, c.redo,
+    const Prep prep = {q->labels, q->label_bytes, M, p.rows_pad, V, q->ignore_index, s.count, s.row, s.label, s.place, c.redo,
                        keep == XQ_LCE_KEEP_DX ? (int32_t)(p.pieces * row_tiles) : 0, none ? loss : nullptr,
                        32 * p.tm, (int32_t)xq_cdiv(H, 256), (int32_t)(p.piece / 32), slots(p.tm)};
     const dim3 by16((unsigned)xq_cdiv(M, 16));
@@ -558,13 +570,15 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
     LceLogitsArgs a = {};
     a.A = (const bf16_t*)q->x; a.lda = q->ldx; a.B = (const bf16_t*)q->w; a.ldb = q->ldw;
     a.H = (int32_t)H; a.cols = p.cols; a.rows = {s.count, s.row, s.label}; a.scale2 = scale2; a.part = c.part; a.rows_pad = p.rows_pad;
-    const bool own_rows = keep == XQ_LCE_KEEP_DX && M > 0 && M <= kBeginRows;
+    // few rows: no launch before the others that finds those that count
+    const bool own_rows = M > 0 && M <= (keep == XQ_LCE_KEEP_DX ? kBeginRows : kLceOwnRows);
     if (!own_rows) lce_prepare_kernel<<<dim3(1), 1024, 0, st>>>(prep);
     if (M > 0 && keep != XQ_LCE_KEEP_DX) {
         a.n_v = (int32_t)V; a.at_label = s.at_label;
+        if (own_rows) a.labels = {q->labels, q->label_bytes, (int32_t)M, q->ignore_index, V};
         if ((rc = launch_logits<kLceStats>(p.tm, a, M, V, st)) != XQ_OK) return rc;
         join.tiles = (int32_t)xq_cdiv(V, p.cols);
-        lce_score_kernel<<<by16, 1024, 0, st>>>(join, s.at_label, end);
+        lce_score_kernel<<<by16, 1024, 0, st>>>(join, prep, own_rows, s.at_label, end);
     } else if (M > 0) {
         lce_target_kernel<<<by16, 1024, 0, st>>>(prep, own_rows, a.A, a.lda, a.B, a.ldb, (int)H, scale2, s.at_label, c.ref, c.z);
         a.ref = c.ref; a.new_ref = c.new_ref; a.alpha = c.alpha; a.image = c.image; a.image_steps = (int32_t)(p.piece / 32); a.redo = c.redo;
