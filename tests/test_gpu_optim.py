@@ -141,6 +141,22 @@ def test_step_over_many_tensors(hip_device, bits, count):
     _check(prob, exp, bits, torch.float32, DECODED if bits == 8 else 0.0)
 
 
+@pytest.mark.parametrize("bits,count", [(8, 83), (8, 168), (8, 169), (32, 111), (32, 112), (32, 113), (32, 225)])
+@pytest.mark.parametrize("pdt,gdt", [(torch.bfloat16, torch.float32), (torch.float32, torch.bfloat16)])
+def test_step_where_a_table_launch_ends(hip_device, bits, count, pdt, gdt):
+    prob = _problem([(300 * (i % 7) + i + 1,) for i in range(count)], bits, pdt, gdt, 6, hip_device)
+    exp = _expected(prob, bits, 2e-4, 0.0)
+    adamw_step(*prob[:5], exp_avg_scales=prob[5], exp_avg_sq_scales=prob[6], lr=2e-4, weight_decay=0.0)
+    _check(prob, exp, bits, pdt, DECODED if bits == 8 else 0.0)
+
+
+@pytest.mark.parametrize("count", [255, 256, 257, 512, 513])
+def test_grad_norm_where_a_table_launch_ends(hip_device, count):
+    grads = [torch.full((i + 1,), 0.5, device=hip_device, dtype=torch.bfloat16 if i % 2 else torch.float32) for i in range(count)]
+    want = (0.25 * count * (count + 1) / 2) ** 0.5
+    assert abs(float(grad_norm(grads)) - want) <= (U + 1e-10) * want
+
+
 @pytest.mark.parametrize("clip", [None, 0.02])
 @pytest.mark.parametrize("n", [256 * 4000, 256 * 33 + 77])
 def test_codes_are_the_nearest_ones(hip_device, n, clip):

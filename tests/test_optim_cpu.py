@@ -61,7 +61,7 @@ def _step(tensor, n=1, ws=1 << 20, ws_bytes=1 << 20, **over):
 
 
 @pytest.mark.parametrize("over", [dict(numel=0), dict(numel=-1), dict(param=None), dict(grad=None), dict(exp_avg=None), dict(exp_avg_sq=None), dict(step=None),
-                                  dict(param=4098), dict(grad=8193, grad_dtype=_C.XQ_DT_BF16), dict(exp_avg=12290), dict(param_dtype=7), dict(grad_dtype=-1)])
+                                  dict(param=4098), dict(grad=8193, grad_dtype=_C.XQ_DT_BF16), dict(exp_avg=12290), dict(param_dtype=7), dict(grad_dtype=-1)] + [{k: 1 << 48} for k in ("param", "grad", "exp_avg", "exp_avg_sq", "step")])
 def test_step_refuses_tensor(over):
     assert _step(_tensor(**over)) == -1
     assert b"xq_adamw_step" in _C.lib().xq_last_error()

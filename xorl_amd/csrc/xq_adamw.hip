@@ -12,7 +12,7 @@
 //
 // Bound by memory: 28 bytes an element (fp32 parameters and gradients, 32-bit states) or 16.06 (8-bit ones).  The factors of a model are
 // hundreds of tensors of 10^4 to 10^6 elements.  Their addresses change from step to step (autograd allocates gradients), so a call takes
-// them by value: adamw_table_kernel's arguments carry 63 to 252 tensors a launch, and it writes them into a table in the workspace, with the
+// them by value: adamw_table_kernel's arguments carry 84 to 256 tensors a launch, and it writes them into a table in the workspace, with the
 // step counts advanced and the bias corrections in 64 bits.  One launch then walks all tensors: chunks of 4096 elements, numbered through,
 // are dealt out to the blocks in ranges; a block looks a chunk up in the table (two steps of 64 lanes) and goes on from there.
 //
@@ -30,7 +30,7 @@ namespace {
 constexpr int kBlock = 256;                 // elements that share a scale: a wave's four a lane
 constexpr int kChunk = 4096;                // of a thread block at a time: four 256-element pieces of each of its waves
 constexpr int kThreads = 256;
-constexpr int kTableWords = 504;            // of tensors by value in one launch: 4032 bytes, of the 4096 that arguments may take
+constexpr int kTableWords = 1008;           // of tensors by value in one launch: 4032 bytes, of the 4096 that arguments may take
 constexpr int kNormBlocks = 2048;
 constexpr int kStepBlocks = 2048;           // eight of a compute unit
 
@@ -47,10 +47,11 @@ struct Row {                                // what the walking kernels read of 
     int32_t param16, grad16;                // bf16 (otherwise fp32)
 };
 
-// A tensor in 2 words (its gradient alone), 6 (with 32-bit states) or 8: gradient, elements with the types in the top bits; parameter, states
-// and step count; scales.
+// A tensor in 3 words of 32 bits (its gradient alone), 9 (with 32-bit states) or 12: 504 factors are 5 or 6 launches of 2 to 5 us.
+//   0  elements, low      1  elements, high (11 bits), bf16 parameter (bit 14), bf16 gradient (bit 15), gradient's top 16 bits      2  gradient
+//   3 .. 6  parameter, states, step count; 7, 8  their top 16 bits, two a word      9 .. 11  scales, and theirs
 struct TableArgs {
-    uint64_t word[kTableWords];
+    uint32_t word[kTableWords];
     Row* rows;
     int32_t chunk0, n;
 };
@@ -59,14 +60,17 @@ struct TableScalars {
     const float* lr_device;
 };
 static_assert(sizeof(TableArgs) + sizeof(TableScalars) <= 4096, "kernel arguments");
-constexpr int table_tensors(int words) { return kTableWords / words; }
+constexpr int table_tensors(int words) { return kTableWords / words < 256 ? kTableWords / words : 256; }
+constexpr int kAddressBits = 48;
+template <typename P>
+__device__ __forceinline__ P* address(uint32_t low, uint32_t high16) { return (P*)((uint64_t)(high16 & 0xffffu) << 32 | low); }
 
 template <int WORDS>
 __global__ void __launch_bounds__(256) adamw_table_kernel(TableArgs a, TableScalars s) {
     __shared__ int wave_end[4];
     const int i = threadIdx.x, lane = i & 63, wave = i >> 6;
-    const uint64_t* w = a.word + min(i, a.n - 1) * WORDS;
-    const int64_t numel = (int64_t)(w[1] & ~(3ull << 62));
+    const uint32_t* w = a.word + min(i, a.n - 1) * WORDS;
+    const int64_t numel = (int64_t)(w[1] & 0x7ffu) << 32 | w[0];
     const int own = i < a.n ? (int)((numel + kChunk - 1) / kChunk) : 0;
     int end = own;
 #pragma unroll
@@ -79,21 +83,21 @@ __global__ void __launch_bounds__(256) adamw_table_kernel(TableArgs a, TableScal
     if (i >= a.n) return;
     for (int k = 0; k < wave; ++k) end += wave_end[k];
     Row r = {};
-    r.grad = (const void*)w[0];
+    r.grad = address<const void>(w[2], w[1] >> 16);
     r.numel = numel;
     r.chunk0 = a.chunk0 + end - own;
-    r.grad16 = (int)(w[1] >> 62 & 1);
-    if constexpr (WORDS >= 6) {
-        r.param16 = (int)(w[1] >> 63);
-        r.param = (void*)w[2]; r.m = (void*)w[3]; r.v = (void*)w[4];
-        float* const count = (float*)w[5];
+    r.grad16 = (int)(w[1] >> 15 & 1);
+    if constexpr (WORDS >= 9) {
+        r.param16 = (int)(w[1] >> 14 & 1);
+        r.param = address<void>(w[3], w[7]); r.m = address<void>(w[4], w[7] >> 16); r.v = address<void>(w[5], w[8]);
+        float* const count = address<float>(w[6], w[8] >> 16);
         const float step = *count + 1.0f;
         *count = step;
         const double lr = s.lr_device ? (double)*s.lr_device : s.lr;
         r.first = (float)(lr / (1.0 - exp(step * s.log_beta1)));           // b^t; a beta of 0 has the logarithm -inf
         r.root = (float)(1.0 / sqrt(1.0 - exp(step * s.log_beta2)));
     }
-    if constexpr (WORDS == 8) { r.m_scale = (float*)w[6]; r.v_scale = (float*)w[7]; }
+    if constexpr (WORDS == 12) { r.m_scale = address<float>(w[9], w[11]); r.v_scale = address<float>(w[10], w[11] >> 16); }
     a.rows[i] = r;
 }
 
@@ -455,6 +459,12 @@ int check_tensors(const char* who, const xq_adamw_tensor* t, int64_t n, int stat
     *chunks = 0;
     for (int64_t i = 0; i < n; ++i) {
         const xq_adamw_tensor& a = t[i];
+        uintptr_t bits = (uintptr_t)a.grad;
+        if (!grads_only) {
+            bits |= (uintptr_t)a.param | (uintptr_t)a.exp_avg | (uintptr_t)a.exp_avg_sq | (uintptr_t)a.step;
+            if (state_bits == 8) bits |= (uintptr_t)a.exp_avg_scale | (uintptr_t)a.exp_avg_sq_scale;
+        }
+        XQ_REQUIRE(bits >> kAddressBits == 0, "%s: an address of tensor %lld has more than %d bits", who, (long long)i, kAddressBits);
         XQ_REQUIRE(a.numel > 0, "%s: tensor %lld has %lld elements", who, (long long)i, (long long)a.numel);
         XQ_REQUIRE(a.grad_dtype == XQ_DT_BF16 || a.grad_dtype == XQ_DT_F32, "%s: gradient %lld is neither fp32 nor bf16", who, (long long)i);
         XQ_REQUIRE(a.grad && xq_aligned(a.grad, a.grad_dtype == XQ_DT_BF16 ? 2 : 4), "%s: gradient %lld is NULL or misaligned", who, (long long)i);
@@ -481,7 +491,7 @@ int check_workspace(const char* who, int64_t n, const void* workspace, int64_t b
     return XQ_OK;
 }
 
-// words 2: for the norm alone
+// words 3: for the norm alone
 template <int WORDS>
 void write_table(const xq_adamw_tensor* t, int64_t n, void* workspace, const xq_adamw_options* o, hipStream_t s) {
     TableScalars c = {};
@@ -494,14 +504,18 @@ void write_table(const xq_adamw_tensor* t, int64_t n, void* workspace, const xq_
         a.n = (int32_t)std::min<int64_t>(table_tensors(WORDS), n - at);
         for (int i = 0; i < a.n; ++i) {
             const xq_adamw_tensor& q = t[at + i];
-            uint64_t* w = a.word + i * WORDS;
-            w[0] = (uint64_t)q.grad;
-            w[1] = (uint64_t)q.numel | (uint64_t)(q.grad_dtype == XQ_DT_BF16) << 62;
-            if (WORDS >= 6) {
-                w[1] |= (uint64_t)(q.param_dtype == XQ_DT_BF16) << 63;
-                w[2] = (uint64_t)q.param; w[3] = (uint64_t)q.exp_avg; w[4] = (uint64_t)q.exp_avg_sq; w[5] = (uint64_t)q.step;
+            uint32_t* w = a.word + i * WORDS;
+            auto low = [](const void* p) { return (uint32_t)(uintptr_t)p; };
+            auto high = [](const void* p) { return (uint32_t)((uintptr_t)p >> 32); };
+            w[0] = (uint32_t)q.numel;
+            w[1] = (uint32_t)(q.numel >> 32) | (uint32_t)(q.grad_dtype == XQ_DT_BF16) << 15 | high(q.grad) << 16;
+            w[2] = low(q.grad);
+            if (WORDS >= 9) {
+                w[1] |= (uint32_t)(q.param_dtype == XQ_DT_BF16) << 14;
+                w[3] = low(q.param); w[4] = low(q.exp_avg); w[5] = low(q.exp_avg_sq); w[6] = low(q.step);
+                w[7] = high(q.param) | high(q.exp_avg) << 16; w[8] = high(q.exp_avg_sq) | high(q.step) << 16;
             }
-            if (WORDS == 8) { w[6] = (uint64_t)q.exp_avg_scale; w[7] = (uint64_t)q.exp_avg_sq_scale; }
+            if (WORDS == 12) { w[9] = low(q.exp_avg_scale); w[10] = low(q.exp_avg_sq_scale); w[11] = high(q.exp_avg_scale) | high(q.exp_avg_sq_scale) << 16; }
             chunk0 += xq_cdiv(q.numel, kChunk);
         }
         adamw_table_kernel<WORDS><<<dim3(1), 256, 0, s>>>(a, c);
@@ -528,7 +542,7 @@ extern "C" int xq_grad_norm(const xq_adamw_tensor* tensors, int64_t n, float* no
     if (rc == XQ_OK) rc = check_workspace("xq_grad_norm", n, workspace, workspace_bytes);
     if (rc != XQ_OK) return rc;
     XQ_REQUIRE(norm && xq_aligned(norm, 4), "xq_grad_norm: norm is NULL or misaligned");
-    write_table<2>(tensors, n, workspace, nullptr, (hipStream_t)stream);
+    write_table<3>(tensors, n, workspace, nullptr, (hipStream_t)stream);
     norm_of(n, chunks, workspace, norm, (hipStream_t)stream);
     XQ_CHECK_LAUNCH("xq_grad_norm");
     return XQ_OK;
@@ -547,8 +561,8 @@ extern "C" int xq_adamw_step(const xq_adamw_tensor* tensors, int64_t n, const xq
     if (rc == XQ_OK) rc = check_workspace("xq_adamw_step", n, workspace, workspace_bytes);
     if (rc != XQ_OK) return rc;
     hipStream_t s = (hipStream_t)stream;
-    if (o->state_bits == 8) write_table<8>(tensors, n, workspace, o, s);
-    else write_table<6>(tensors, n, workspace, o, s);
+    if (o->state_bits == 8) write_table<12>(tensors, n, workspace, o, s);
+    else write_table<9>(tensors, n, workspace, o, s);
     if (o->norm && !o->norm_given) norm_of(n, chunks, workspace, o->norm, s);
     if (n) {
         const StepArgs a = {(const Row*)workspace, chunks, o->norm, (int32_t)n, (float)o->max_norm, (float)o->beta1, (float)o->beta2,
