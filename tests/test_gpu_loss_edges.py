@@ -1,0 +1,67 @@
+"""GPU: linear_cross_entropy where the plain bounds of its other tests let a mistake through, and the calls at the edge of what it takes.
+
+U = 2^-24, half a step of fp32; B = 2^-8, half a step of bf16; `_reference` has the bounds of loss and gradients that are derived there."""
+
+import pytest
+import torch
+
+from tests.test_gpu_loss import B, BF, U, _inputs, _reference, _within
+from xorl_amd.loss_functional import linear_cross_entropy
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------- the input gradient of a head whose rows have something in common
+def _shared_head(M, V, H, seed, device, share, lift):
+    """A head whose rows are a common vector of `share` times their own spread and rows of their own; every token leans to a wrong one"""
+    g = torch.Generator(device=device).manual_seed(seed)
+    own = torch.randn(V, H, device=device, generator=g) * 0.02
+    w = (own + 0.02 * share * torch.randn(H, device=device, generator=g)).to(BF)
+    labels, wrong = torch.randint(0, V // 2, (M,), device=device, generator=g), torch.randint(V // 2, V, (M,), device=device, generator=g)
+    x = torch.randn(M, H, device=device, generator=g) + lift * own[wrong] / (0.0004 * H)
+    return x.to(BF), w, labels
+
+
+def _dx_of_differences(x, w, labels, up):
+    """dx by row in 64 bits, and its bound where what the rows have in common cancels.  dx = g sum_v q_v (w_v - w_t), q = p without the label's: E is off by
+    the logit's error and rounded to bf16 (B), in O = sum E w and Y = sum E alike, so that both count on |w_v - w_t|; the sums in fp32 count on
+    the magnitudes ((V / 32 + 64) U for O, 300 U for Y, four roundings behind them), Z on the result, which is rounded to bf16 in the end."""
+    V, H = w.shape
+    xd, wd = x.double(), w.double()
+    l = xd @ wd.t()
+    q = torch.softmax(l, 1)
+    rows = torch.arange(len(labels), device=x.device)
+    S = (xd.abs() @ wd.abs().t()).amax(1)
+    logit = 2 * (H / 32 + 36) * U * S + 300 * U + 8 * U * (l.abs().amax(1) + l[rows, labels].abs())
+    q[rows, labels] = 0.0
+    want, bound = torch.empty_like(xd), torch.empty_like(xd)
+    for i in range(len(labels)):
+        apart = wd - wd[labels[i]]
+        dx = up[i].double() * (q[i] @ apart)
+        own = (B + logit[i]) * (q[i] @ apart.abs()) + (V / 32 + 368) * U * (q[i] @ wd.abs() + q[i].sum() * wd[labels[i]].abs())
+        want[i] = dx
+        bound[i] = 1.01 * (up[i].double().abs() * own + logit[i] * dx.abs()) + B * dx.abs() + 1e-30
+    return want, bound
+
+
+@pytest.mark.parametrize("M", [3, 20, 100, 300])
+@pytest.mark.parametrize("lift", [6.0, 80.0])                 # 80: beyond the label's logit as the reference, so that the tiles are done again
+@pytest.mark.parametrize("share", [0.0, 16.0])
+def test_what_the_heads_rows_share_cancels(hip_device, M, lift, share):
+    x, w, labels = _shared_head(M, 2500, 128, M, hip_device, share, lift)
+    x.requires_grad_(True)
+    up = torch.randn(M, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(M))
+    dx, = torch.autograd.grad(linear_cross_entropy(x, w, labels, reduction="none"), x, up)
+    _within(dx, _dx_of_differences(x.detach(), w, labels, up), "dx")
+
+
+@pytest.mark.parametrize("lift", [6.0, 80.0])
+def test_what_the_heads_rows_share_cancels_over_pieces(hip_device, lift):
+    M, V = 4096, 140000
+    assert 2 * M * V > 1 << 30
+    x, w, labels = _shared_head(M, V, 64, 5, hip_device, 16.0, lift)
+    x.requires_grad_(True)
+    up = torch.linspace(-1, 1, M, device=hip_device)
+    dx, = torch.autograd.grad(linear_cross_entropy(x, w, labels, reduction="none"), x, up)
+    some = torch.arange(7, M, 371, device=hip_device)
+    _within(dx[some], _dx_of_differences(x.detach()[some], w, labels[some], up[some]), "dx")

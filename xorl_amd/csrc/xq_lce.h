@@ -2,7 +2,7 @@
 //
 // lce_logits_kernel   S = A . B^T, both with the contraction along their rows (hidden states and head), and one of three ends:
 //   STATS   a row's largest logit and its sum of exponentials, by column tile (nothing else is written)
-//   EXP     the same sums relative to a reference logit of the row, and E = exp(l - reference) as a bf16 image
+//   EXP     the same sums relative to a reference logit of the row, E = exp(l - reference) as a bf16 image, and the sum of what the image holds
 //   GRAD    A the head, B the tokens: G = g_i (p_iv - [v = t_i]) as a bf16 image with the tokens along the contraction
 // lce_product_kernel  C = image . B, B with the contraction across its rows: E . W (input gradients), G . X (the head's)
 //
@@ -37,7 +37,7 @@ struct LceTile {
     // a block goes on to its next tile, whose first K-steps are on their way while the ends of this one are computed; 64 rows: two blocks
     // of one tile each share a compute unit instead
     static constexpr bool AHEAD = TM >= 4;
-    static constexpr int END_BYTES = ROWS * 32 + 1024 * 4;      // of the ends: sums by row and wave; four numbers by row or column
+    static constexpr int END_BYTES = ROWS * 64 + 1024 * 4;      // of the ends: up to four numbers by row and wave; four by row or column
     static constexpr int LDS_BYTES = STAGES * STAGE_BYTES + (AHEAD ? END_BYTES : 0);
     static_assert(AHEAD || END_BYTES <= STAGES * STAGE_BYTES, "the ends reuse the stages");
     static_assert((STAGES & (STAGES - 1)) == 0 && LDS_BYTES <= 160 * 1024, "stages are counted by a mask, and fit");
@@ -72,7 +72,8 @@ struct LceLogitsArgs {
     const float* ref;                   // EXP: reference of a row, in log2 units;  GRAD: log2 of the row's sum of exponentials
     const float* grad;                  // GRAD: upstream gradient of a row, but for what all rows share
     const float* rest;                  // GRAD: 1 - p of the label
-    f32x2* part;                        // STATS, EXP: [column tile][rows_pad] (largest, sum)
+    f32x2* part;                        // [column tile][rows_pad], STATS: a row's (largest, sum);  EXP: (sum of E as the image holds it, sum)
+    float* top;                         // EXP: [column tile][rows_pad] the largest
     float* at_label;                    // STATS: the label's logit
     int64_t rows_pad;
     bf16_t* image;
@@ -237,8 +238,8 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
     static_assert(MODE != kLceGrad || TN == 4, "what the ends keep of 256 columns");
     extern __shared__ __attribute__((aligned(16))) unsigned char dsm[];
     unsigned char* const ends = T::AHEAD ? dsm + T::STAGES * T::STAGE_BYTES : dsm;
-    f32x2* const sums = (f32x2*)ends;                       // [row][wave column]
-    float* const info = (float*)(ends + T::ROWS * 32);      // EXP, STATS: label and reference by row;  GRAD: label, lse, up, rest by column
+    f32x4* const sums = (f32x4*)ends;                       // [row][wave column], STATS: largest, sum;  EXP: sum of the image's E, sum, largest
+    float* const info = (float*)(ends + T::ROWS * 64);      // EXP, STATS: label and reference by row;  GRAD: label, lse, up, rest by column
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 2, wn = wave & 3, l16 = lane & 15, lg = lane >> 4;
     constexpr bool OWN = MODE == kLceStats && 32 * TM <= kLceOwnRows;
@@ -293,7 +294,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
             if (MODE == kLceExp && g.again) {
                 // done again: the largest logit of the row's tiles is its reference, where that is far from the one it had
                 float top = -INFINITY;
-                for (int t = 0; t < tiles_b; ++t) top = fmaxf(top, g.part[(int64_t)t * g.rows_pad + r][0]);
+                for (int t = 0; t < tiles_b; ++t) top = fmaxf(top, g.top[(int64_t)t * g.rows_pad + r]);
                 const float old = about[1];
                 const bool far = top - old > kLceFar;
                 if (far) about[1] = top;
@@ -401,7 +402,7 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                         for (int e = 0; e < 4; ++e)
                             if (col_w + 16 * j + e >= end) acc[i][j][e] = -INFINITY;
             }
-            float ref[TM], top[TM], sum[TM];
+            float ref[TM], top[TM], sum[TM], kept[TM];
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 int at = __float_as_int(info[row_w + 16 * i]) - c0 - col_w;           // the label's column by the lane's own numbering of its 4 TN
@@ -432,36 +433,50 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                 const float base = MODE == kLceExp ? ref[i] : (top[i] == -INFINITY ? 0.0f : top[i]);
                 if (MODE == kLceExp) far |= top[i] - base > kLceFar;
                 f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+                f32x2 k = {0.0f, 0.0f};
 #pragma unroll
                 for (int j = 0; j < TN; ++j) {
 #pragma unroll
                     for (int e = 0; e < 4; ++e) acc[i][j][e] = __builtin_amdgcn_exp2f(fmaf(acc[i][j][e], g.scale2, -base));
                     s += acc[i][j];
+                    if (MODE == kLceExp) {                  // as the image is to have it, and what that stands for
+                        const uint32_t lo = pack_bf16x2(acc[i][j][0], acc[i][j][1]), hi = pack_bf16x2(acc[i][j][2], acc[i][j][3]);
+                        k += f32x2{__uint_as_float(lo << 16), __uint_as_float(lo & 0xffff0000u)};
+                        k += f32x2{__uint_as_float(hi << 16), __uint_as_float(hi & 0xffff0000u)};
+                        acc[i][j][0] = __uint_as_float(lo);
+                        acc[i][j][1] = __uint_as_float(hi);
+                    }
                 }
                 sum[i] = (s[0] + s[1]) + (s[2] + s[3]);
+                kept[i] = k[0] + k[1];
             }
 #pragma unroll
             for (int i = 0; i < TM; ++i) {
                 sum[i] = over_groups_sum(sum[i]);
-                if (lg == 0) sums[(row_w + 16 * i) * 4 + wn] = f32x2{top[i], sum[i]};
+                if (MODE == kLceExp) kept[i] = over_groups_sum(kept[i]);
+                if (lg == 0) sums[(row_w + 16 * i) * 4 + wn] = MODE == kLceExp ? f32x4{kept[i], sum[i], top[i], 0.0f} : f32x4{top[i], sum[i], 0.0f, 0.0f};
             }
             if (MODE == kLceExp && !g.again && __any(far)) {
                 if (lane == 0) g.redo[this_a] = 1;          // (several may say so, all the same)
             }
             __syncthreads();
             if (tid < T::ROWS && r0 + tid < count) {
-                f32x2 a = sums[tid * 4], b;
+                f32x4 a = sums[tid * 4], b;
 #pragma unroll
                 for (int w = 1; w < 4; ++w) {
                     b = sums[tid * 4 + w];
+                    if (MODE == kLceExp) {
+                        a = f32x4{a[0] + b[0], a[1] + b[1], fmaxf(a[2], b[2]), 0.0f};
+                        continue;
+                    }
                     const float most = fmaxf(a[0], b[0]);
-                    if (MODE == kLceExp) a[1] += b[1];
-                    else if (most != -INFINITY) a[1] = a[1] * __builtin_amdgcn_exp2f(a[0] - most) + b[1] * __builtin_amdgcn_exp2f(b[0] - most);
+                    if (most != -INFINITY) a[1] = a[1] * __builtin_amdgcn_exp2f(a[0] - most) + b[1] * __builtin_amdgcn_exp2f(b[0] - most);
                     a[0] = most;
                 }
+                const int64_t at = (int64_t)this_b * g.rows_pad + r0 + tid;
+                g.part[at] = f32x2{a[0], a[1]};
                 // (done again: the largest stays what it was, the other tiles' blocks read it)
-                if (MODE == kLceExp && g.again) g.part[(int64_t)this_b * g.rows_pad + r0 + tid][1] = a[1];
-                else g.part[(int64_t)this_b * g.rows_pad + r0 + tid] = a;
+                if (MODE == kLceExp && !g.again) g.top[at] = a[2];
             }
         }
         if constexpr (MODE != kLceStats) {
@@ -477,8 +492,9 @@ __global__ void __launch_bounds__(512, TM <= 2 ? 4 : 2) lce_logits_kernel(LceLog
                         if ((step * 32 >= cols && this_b + 1 < tiles_b) || (c0 >> 5) + step >= g.image_steps) continue;
                     }
                     const f32x4 a = acc[i][2 * q], b = acc[i][2 * q + 1];
-                    *(u32x4*)(out + (q * T::ROWS + row) * 32 + ((lg ^ ((row >> 2) & 2)) << 3)) =
-                        u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
+                    u32x4* const to = (u32x4*)(out + (q * T::ROWS + row) * 32 + ((lg ^ ((row >> 2) & 2)) << 3));
+                    if (MODE == kLceExp) *to = u32x4{__float_as_uint(a[0]), __float_as_uint(a[1]), __float_as_uint(b[0]), __float_as_uint(b[1])};
+                    else *to = u32x4{pack_bf16x2(a[0], a[1]), pack_bf16x2(a[2], a[3]), pack_bf16x2(b[0], b[1]), pack_bf16x2(b[2], b[3])};
                 }
             }
             if (MODE == kLceGrad) __syncthreads();          // (what the ends read of the columns is written anew)

@@ -7,15 +7,17 @@
 // covers the most rows there can be and blocks behind the last one end at once.  The label's column is left out of all sums and joined
 // at the end: with Z' = sum_{v != t} exp(l_v - ref), e_t = exp(l_t - ref),
 //   loss = log(Z' + e_t) + ref - l_t        (log1p(Z') where ref is the label's own logit)
-//   dx_i = g_i c (O_i - Z' w_t) / (Z' + e_t),        O_i = sum_{v != t} exp(l_v - ref) w_v
-// which keeps what a confident row has left of its loss and gradient, where p_t - 1 would cancel.
+//   dx_i = g_i c (O_i - Y w_t) / (Z' + e_t),        O_i = sum_{v != t} E_v w_v,        Y = sum_{v != t} E_v,        E_v = exp(l_v - ref) as bf16
+// which keeps what a confident row has left of its loss and gradient, where p_t - 1 would cancel.  Y, and not Z', is taken off: the roundings of
+// E then count on differences w_v - w_t, and what the rows of the head have in common cancels (300 tokens under rows whose common part is 16 times
+// their spread, [4096, 256]: the gradient is off by 0.0017 of it, 0.0022 at worst, which is the result's own rounding; 0.0029 and 0.0152 with Z').
 //
 //  * Scores (no gradient wanted): one product whose ends are the largest logit and the sum of exponentials of 256 columns; one joining pass.
 //  * Training: E = exp(l - ref) of a piece goes to the workspace as bf16, and E . W is added to O in fp32: the forward leaves
 //    the whole input gradient but its factor, in two products, where forming the logits again in the backward would take three.  E needs
-//    a reference before the row's largest logit is known: the label's own logit (target_kernel).  E is right as long as no logit is more
+//    a reference before the row's largest logit is known: the label's own logit (lce_target_kernel).  E is right as long as no logit is more
 //    than 2^64 times e above it; a piece that finds one takes the largest as the new reference (O and Z' are scaled to it) and is done
-//    again for the row tiles concerned.  bf16 keeps E to half a step (2^-9 of each term, of either sign).
+//    again for the row tiles concerned.  bf16 keeps E to half a step (up to 2^-8 of each term, of either sign).
 //  * A trained head: the backward forms the logits again with the roles exchanged, G = g (p - [v = t]) as bf16 with the tokens along the
 //    contraction, and multiplies it with the rows that count.  What all rows share of g (the mean's 1 / count, the logit scale) is left to the
 //    result in 32 bits: in G it would be one and the same rounding error, up to half a step, of the whole gradient.
@@ -128,7 +130,7 @@ __device__ __forceinline__ f32x4 bf16x4_f32(u32x2 w) {
 // The label's logit of every row (log2 units): the first reference.  A wave has a row.  own_rows (up to kBeginRows labels): every block finds
 // its rows by itself, and the first does what lce_prepare_kernel does.
 __global__ void __launch_bounds__(1024) lce_target_kernel(Prep a, int own_rows, const bf16_t* x, int64_t ldx, const bf16_t* w, int64_t ldw, int H, float scale2,
-                                                          float* at_label, float* ref, float* z) {
+                                                          float* at_label, float* ref, f32x2* z) {
     __shared__ int wave_n[16], rows[16], labels[16];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int64_t first = (int64_t)blockIdx.x * 16, c = first + wave;
@@ -156,7 +158,7 @@ __global__ void __launch_bounds__(1024) lce_target_kernel(Prep a, int own_rows, 
     for (int d = 32; d; d >>= 1) sum += __shfl_xor(sum, d);
     if (lane == 0) {
         at_label[c] = ref[c] = label >= 0 ? sum * scale2 : __builtin_nanf("");
-        z[c] = 0.0f;
+        z[c] = f32x2{0.0f, 0.0f};
     }
 }
 
@@ -166,7 +168,8 @@ struct Join {
     const f32x2* part;
     int64_t rows_pad;
     int32_t tiles, tile_rows;
-    float *ref, *z;
+    float* ref;
+    f32x2* z;                           // (Y, Z') so far
     const float *new_ref, *alpha;       // of row tiles that were done again
     const int32_t* redo;
 };
@@ -194,10 +197,10 @@ __device__ __forceinline__ bool join_rows(const Join& a, int count, f32x2 start,
     *row = r;
     return true;
 }
-__device__ __forceinline__ f32x2 fold_sum(f32x2 p, f32x2 q) { return f32x2{0.0f, p[1] + q[1]}; }
+__device__ __forceinline__ f32x2 fold_sum(f32x2 p, f32x2 q) { return p + q; }
 
-// a row's Z' and reference with those of a piece
-__device__ __forceinline__ void add_piece(const Join& a, int64_t r, float sum, float* z, float* ref) {
+// a row's sums and reference with those of a piece
+__device__ __forceinline__ void add_piece(const Join& a, int64_t r, f32x2 sum, f32x2* z, float* ref) {
     *z = a.z[r];
     *ref = a.ref[r];
     if (a.redo[r / a.tile_rows]) {
@@ -210,26 +213,29 @@ __global__ void __launch_bounds__(1024) lce_sum_kernel(Join a) {
     f32x2 v;
     int64_t r;
     if (!join_rows(a, *a.count, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
-    float z, ref;
-    add_piece(a, r, v[1], &z, &ref);
+    f32x2 z;
+    float ref;
+    add_piece(a, r, v, &z, &ref);
     a.z[r] = z;
     a.ref[r] = ref;
 }
 
-// what is kept of a row: 1 / Z, Z' / Z, log2 of the sum of exponentials
+// what is kept of a row: 1 / Z, Z' / Z, Y / Z (EXP), log2 of the sum of exponentials
 struct RowEnd {
-    float *inv, *rest, *lse2, *loss;
+    float *inv, *rest, *off, *lse2, *loss;
     const int32_t* row;
     float* out;                         // losses by row of x, or NULL
 };
-__device__ __forceinline__ void end_row(const RowEnd& e, int64_t c, int row, float z, float ref, float t) {
+__device__ __forceinline__ float end_row(const RowEnd& e, int64_t c, int row, float z, float ref, float t) {
     const float et = __builtin_amdgcn_exp2f(t - ref), sum = z + et;
     const float loss = ref == t ? log1pf(z) : logf(sum) + (ref - t) * kLn2;
     e.loss[c] = loss;
     if (e.out) e.out[row] = loss;
-    e.inv[c] = 1.0f / sum;
+    const float inv = 1.0f / sum;
+    e.inv[c] = inv;
     e.rest[c] = z / sum;
     e.lse2[c] = ref == t ? log1pf(z) * kLog2e + t : log2f(sum) + ref;
+    return inv;
 }
 
 // STATS: joins and ends.  own_rows: as the logits kernel, every block finds the rows that count by itself, and the first notes them
@@ -264,9 +270,10 @@ __global__ void __launch_bounds__(1024) lce_end_kernel(Join a, const float* at_l
     f32x2 v;
     int64_t r;
     if (!join_rows(a, *a.count, f32x2{0.0f, 0.0f}, fold_sum, &v, &r)) return;
-    float z, ref;
-    add_piece(a, r, v[1], &z, &ref);
-    end_row(e, r, e.row[r], z, ref, at_label[r]);
+    f32x2 z;
+    float ref;
+    add_piece(a, r, v, &z, &ref);
+    e.off[r] = z[0] * end_row(e, r, e.row[r], z[1], ref, at_label[r]);
 }
 
 // sum or mean of the losses: one block, in an order that the sizes fix
@@ -305,7 +312,7 @@ __device__ __forceinline__ float upstream(const Upstream& u, int64_t row) {
 
 // dx: a block has 512 columns of a row of x, a thread 8 of them
 __global__ void __launch_bounds__(64) lce_dx_kernel(const int32_t* place, const int32_t* label, int H, const float* o,
-                                                    const float* inv, const float* rest, const bf16_t* w, int64_t ldw, Upstream u, bf16_t* dx, int64_t lddx) {
+                                                    const float* inv, const float* off, const bf16_t* w, int64_t ldw, Upstream u, bf16_t* dx, int64_t lddx) {
     const int64_t i = blockIdx.x;
     const int k = blockIdx.y * 512 + threadIdx.x * 8;
     if (k >= H) return;
@@ -318,7 +325,7 @@ __global__ void __launch_bounds__(64) lce_dx_kernel(const int32_t* place, const 
     const int t = label[c], count = u.count[0], parts = u.count[1];
     const u32x4 wt = *(const u32x4*)(w + max(t, 0) * ldw + k);
     const float g = upstream(u, i);
-    const float a = g * inv[c], b = t < 0 ? __builtin_nanf("") : g * rest[c];
+    const float a = g * inv[c], b = t < 0 ? __builtin_nanf("") : g * off[c];
     const float* oc = o + (int64_t)c * H + k;
     f32x4 lo = {0.0f, 0.0f, 0.0f, 0.0f}, hi = lo;
 #pragma unroll 4
@@ -428,7 +435,7 @@ int64_t sums_bytes(const Plan& p, int64_t M, int64_t H) {
 // what a forward leaves for the backward
 struct Saved {
     int32_t *count, *row, *label, *place;       // count[1]: parts of the contraction of E . W
-    float *at_label, *inv, *rest, *lse2, *loss, *o;
+    float *at_label, *inv, *rest, *off, *lse2, *loss, *o;
     int64_t bytes;
 };
 Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
@@ -443,6 +450,7 @@ Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
     s.at_label = (float*)take(4 * p.rows_pad);
     s.inv = (float*)take(4 * p.rows_pad);
     s.rest = (float*)take(4 * p.rows_pad);
+    s.off = keep == XQ_LCE_KEEP_DX ? (float*)take(4 * p.rows_pad) : nullptr;
     s.lse2 = (float*)take(4 * p.rows_pad);
     s.loss = (float*)take(4 * p.rows_pad);
     s.o = keep == XQ_LCE_KEEP_DX ? (float*)take(sums_bytes(p, M, H)) : nullptr;
@@ -451,9 +459,9 @@ Saved saved_of(void* base, int64_t M, int64_t V, int64_t H, int keep) {
 }
 
 struct Scratch {
-    float *ref, *z, *alpha, *up, *new_ref;
+    float *ref, *rest, *alpha, *up, *new_ref, *top;
     int32_t* redo;
-    f32x2* part;
+    f32x2 *part, *z;
     bf16_t *image, *x;
     int64_t bytes;
 };
@@ -463,17 +471,22 @@ Scratch scratch_of(void* base, int64_t M, int64_t V, int64_t H, int pass) {
     auto take = [&](int64_t n) { uint8_t* r = at; at += up256(n); return r; };
     Scratch s = {};
     s.ref = (float*)take(4 * p.rows_pad);
-    s.z = (float*)take(4 * p.rows_pad);
     s.alpha = (float*)take(4 * p.rows_pad);
     s.up = (float*)take(4 * p.rows_pad);
     s.new_ref = (float*)take(4 * p.rows_pad);
     s.redo = (int32_t*)take(4 * p.pieces * (p.rows_pad / 64));
     if (pass == XQ_LCE_KEEP_HEAD_BWD) {
+        s.rest = (float*)take(4 * p.rows_pad);
         s.x = (bf16_t*)take(2 * M * H);
         s.image = (bf16_t*)take(2 * p.rows_pad * p.piece);
     } else {
-        s.part = (f32x2*)take(8 * p.rows_pad * xq_cdiv(pass == XQ_LCE_KEEP_DX ? p.piece : V, p.cols));
-        if (pass == XQ_LCE_KEEP_DX) s.image = (bf16_t*)take(2 * image_rows(p, M) * p.piece);
+        const int64_t tiles = xq_cdiv(pass == XQ_LCE_KEEP_DX ? p.piece : V, p.cols);
+        s.part = (f32x2*)take(8 * p.rows_pad * tiles);
+        if (pass == XQ_LCE_KEEP_DX) {
+            s.z = (f32x2*)take(8 * p.rows_pad);
+            s.top = (float*)take(4 * p.rows_pad * tiles);
+            s.image = (bf16_t*)take(2 * image_rows(p, M) * p.piece);
+        }
     }
     s.bytes = at - (uint8_t*)base;
     return s;
@@ -561,7 +574,7 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
     const float scale2 = q->logit_scale * kLog2e;
     const bool none = q->reduction == XQ_LCE_NONE;
     const int row_tiles = (int)xq_cdiv(M, 32 * p.tm);
-    const RowEnd end = {s.inv, s.rest, s.lse2, s.loss, s.row, none ? loss : nullptr};
+    const RowEnd end = {s.inv, s.rest, s.off, s.lse2, s.loss, s.row, none ? loss : nullptr};
     const Prep prep = {q->labels, q->label_bytes, M, p.rows_pad, V, q->ignore_index, s.count, s.row, s.label, s.place, c.redo,
                        keep == XQ_LCE_KEEP_DX ? (int32_t)(p.pieces * row_tiles) : 0, none ? loss : nullptr,
                        32 * p.tm, (int32_t)xq_cdiv(H, 256), (int32_t)(p.piece / 32), slots(p.tm)};
@@ -581,7 +594,7 @@ extern "C" int xq_lce_fwd(const xq_lce_problem* q, float* loss, void* saved, int
         lce_score_kernel<<<by16, 1024, 0, st>>>(join, prep, own_rows, s.at_label, end);
     } else if (M > 0) {
         lce_target_kernel<<<by16, 1024, 0, st>>>(prep, own_rows, a.A, a.lda, a.B, a.ldb, (int)H, scale2, s.at_label, c.ref, c.z);
-        a.ref = c.ref; a.new_ref = c.new_ref; a.alpha = c.alpha; a.image = c.image; a.image_steps = (int32_t)(p.piece / 32); a.redo = c.redo;
+        a.ref = c.ref; a.new_ref = c.new_ref; a.alpha = c.alpha; a.top = c.top; a.image = c.image; a.image_steps = (int32_t)(p.piece / 32); a.redo = c.redo;
         for (int64_t v0 = 0; v0 < V; v0 += p.piece, a.redo += row_tiles) {
             const int64_t n = std::min(p.piece, V - v0);
             a.first_v = (int32_t)v0; a.n_v = (int32_t)n;
@@ -618,17 +631,17 @@ extern "C" int xq_lce_bwd(const xq_lce_problem* q, const float* grad, const void
     const LceRows rows = {s.count, s.row, s.label};
     const Upstream u = {grad, q->reduction, s.count, q->logit_scale};
     if (dx && M > 0)
-        lce_dx_kernel<<<dim3((unsigned)M, (unsigned)xq_cdiv(H, 512)), 64, 0, st>>>(s.place, s.label, (int)H, s.o, s.inv, s.rest, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
+        lce_dx_kernel<<<dim3((unsigned)M, (unsigned)xq_cdiv(H, 512)), 64, 0, st>>>(s.place, s.label, (int)H, s.o, s.inv, s.off, (const bf16_t*)q->w, q->ldw, u, (bf16_t*)dx, lddx);
     if (dw) {
         const Plan h = plan_head(M, V);
         const Scratch c = scratch_of(workspace, M, V, H, XQ_LCE_KEEP_HEAD_BWD);
         if (M > 0) {
-            lce_factors_kernel<<<dim3((unsigned)(h.rows_pad / 256)), 256, 0, st>>>(rows, h.rows_pad, s.lse2, s.rest, u, c.ref, c.up, c.z, c.alpha);
+            lce_factors_kernel<<<dim3((unsigned)(h.rows_pad / 256)), 256, 0, st>>>(rows, h.rows_pad, s.lse2, s.rest, u, c.ref, c.up, c.rest, c.alpha);
             lce_gather_kernel<<<dim3((unsigned)M), 256, 0, st>>>(rows, (const bf16_t*)q->x, q->ldx, (int)H, c.x);
         }
         LceLogitsArgs a = {};
         a.A = (const bf16_t*)q->w; a.lda = q->ldw; a.B = (const bf16_t*)q->x; a.ldb = q->ldx;
-        a.H = (int32_t)H; a.cols = 256; a.rows = rows; a.scale2 = q->logit_scale * kLog2e; a.ref = c.ref; a.grad = c.up; a.rest = c.z; a.rows_pad = h.rows_pad;
+        a.H = (int32_t)H; a.cols = 256; a.rows = rows; a.scale2 = q->logit_scale * kLog2e; a.ref = c.ref; a.grad = c.up; a.rest = c.rest; a.rows_pad = h.rows_pad;
         a.image = c.image; a.image_steps = (int32_t)(h.rows_pad / 32);
         for (int64_t v0 = 0; v0 < V; v0 += h.piece) {
             const int64_t n = std::min(h.piece, V - v0);
