@@ -65,3 +65,66 @@ def test_what_the_heads_rows_share_cancels_over_pieces(hip_device, lift):
     dx, = torch.autograd.grad(linear_cross_entropy(x, w, labels, reduction="none"), x, up)
     some = torch.arange(7, M, 371, device=hip_device)
     _within(dx[some], _dx_of_differences(x.detach()[some], w, labels[some], up[some]), "dx")
+
+
+# ---------------------------------------------------------------- heads that are laid out otherwise
+def _laid_out(w, kind):
+    """The head's values where its rows cannot be read in place"""
+    V, H = w.shape
+    if kind == "transposed":
+        return w.t().contiguous().t()
+    if kind == "odd pitch":
+        return torch.zeros(V, H + 3, dtype=BF, device=w.device).index_copy_(1, torch.arange(H, device=w.device), w)[:, :H]
+    return torch.cat([w.new_zeros(1), w.reshape(-1)])[1:].view(V, H)          # (contiguous, two bytes behind an aligned address)
+
+
+@pytest.mark.parametrize("kind", ["transposed", "odd pitch", "off by one"])
+def test_layouts_that_are_copied(hip_device, kind):
+    x, w, labels = _inputs(150, 700, 128, 37, hip_device)
+    up = torch.randn(150, device=hip_device)
+    xl, wl = _laid_out(x, kind).requires_grad_(True), _laid_out(w, kind).requires_grad_(True)
+    assert torch.equal(wl, w)
+    loss = linear_cross_entropy(xl, wl, labels, reduction="none")
+    grads = torch.autograd.grad(loss, (xl, wl), up)
+    xp, wp = x.requires_grad_(True), w.requires_grad_(True)
+    want = linear_cross_entropy(xp, wp, labels, reduction="none")
+    assert torch.equal(loss, want) and all(torch.equal(a, b) for a, b in zip(grads, torch.autograd.grad(want, (xp, wp), up)))
+
+
+@pytest.mark.parametrize("kind", ["transposed", "odd pitch", "off by one"])
+def test_capture_beside_a_living_loss_over_a_copied_head_is_refused(hip_device, kind):
+    x, w, labels = _inputs(40, 1000, 128, 72, hip_device)
+    w = _laid_out(w, kind)
+    x.requires_grad_(True)
+    eager = linear_cross_entropy(x, w, labels)
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="another stream"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(linear_cross_entropy(x, w, labels), x)
+    torch.cuda.synchronize()
+    want, = torch.autograd.grad(eager, x)
+    del eager
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        dx, = torch.autograd.grad(linear_cross_entropy(x, w, labels), x)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(dx, want)
+
+
+class _Head(torch.nn.Parameter):
+    pass
+
+
+def test_captured_backward_of_a_subclass_is_refused(hip_device):
+    """A subclass goes by the Python function, which cannot see whom torch hands its gradients to; outside a capture it has the plain one's"""
+    x, w, labels = _inputs(40, 1000, 128, 73, hip_device)
+    x.requires_grad_(True)
+    head = _Head(w, requires_grad=False)
+    with pytest.raises(RuntimeError, match="no subclasses"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(linear_cross_entropy(x, head, labels), x)
+    torch.cuda.synchronize()
+    got, = torch.autograd.grad(linear_cross_entropy(x, head, labels), x)
+    assert torch.equal(got, torch.autograd.grad(linear_cross_entropy(x, w, labels), x)[0])

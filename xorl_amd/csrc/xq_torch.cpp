@@ -449,16 +449,18 @@ struct QLoRAMLPBackward : public Node {
     }
 };
 
-// what a cross entropy over a head is about: tensors, checked, as the library takes them
+// what a cross entropy over a head is about: tensors, checked, as the library takes them.  A head whose rows do not lie a multiple of 16 bytes
+// apart is copied by the call, in the forward and in the backward again: kept in between it would be held twice
 struct HeadLoss {
     xq_lce_problem q{};
-    Tensor keep_labels;
+    Tensor keep_w, keep_labels;
     Rows xr;
 
-    HeadLoss(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore, int reduction, double scale) : xr(x, x.size(-1)) {
+    HeadLoss(const Tensor& x, const Tensor& w, const Tensor& labels, int64_t ignore, int reduction, double scale) : xr(aligned(x), x.size(-1)) {
+        keep_w = in_rows(w) ? w : aligned(w.contiguous());
         keep_labels = labels.is_contiguous() ? labels : labels.contiguous();
         q.x = xr.ptr; q.ldx = xr.ld; q.M = xr.M;
-        q.w = w.data_ptr(); q.V = w.size(0); q.H = w.size(1); q.ldw = q.V > 1 ? w.stride(0) : q.H;
+        q.w = keep_w.data_ptr(); q.V = w.size(0); q.H = w.size(1); q.ldw = q.V > 1 ? keep_w.stride(0) : q.H;
         q.labels = keep_labels.data_ptr(); q.label_bytes = (int32_t)keep_labels.element_size();
         q.ignore_index = ignore; q.reduction = reduction; q.logit_scale = (float)scale;
     }
@@ -467,8 +469,12 @@ struct HeadLoss {
         if (labels.scalar_type() != at::kLong && labels.scalar_type() != at::kInt) return false;
         if (x.sizes().slice(0, x.dim() - 1) != labels.sizes() || x.size(-1) != w.size(1) || w.size(1) < 64 || w.size(1) % 64 || w.size(0) < 1) return false;
         if (x.device() != w.device() || x.device() != labels.device() || x.is_neg() || w.is_neg() || labels.is_neg()) return false;
+        return true;
+    }
+    static bool in_rows(const Tensor& w) {
         return w.stride(1) == 1 && (w.size(0) == 1 || (w.stride(0) >= w.size(1) && w.stride(0) % 8 == 0)) && (uintptr_t)w.data_ptr() % 16 == 0;
     }
+    static Tensor aligned(const Tensor& t) { return t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 != 0 ? t.clone() : t; }
 };
 
 struct LinearCrossEntropyBackward : public Node {

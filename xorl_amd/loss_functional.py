@@ -102,6 +102,9 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, grad):
+        if not torch.compiler.is_compiling() and torch.cuda.is_current_stream_capturing():
+            # (torch may hand the gradients to another stream, which ends the process under capture; the native node looks at whose)
+            raise RuntimeError("linear_cross_entropy: a captured backward takes plain tensors, no subclasses of them")
         x, weight, labels, saved = ctx.saved_tensors
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         bwd = _bwd_op if torch.compiler.is_compiling() else _bwd_impl
@@ -120,12 +123,12 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
     probabilities in them are rounded to bf16 once (half a step, 2^-8, each), all but the label's; for the weight, probabilities and the label's
     1 - p times the row's upstream gradient are, unless at most 128 rows count (then 2^-16).  H must be a multiple of 64.  First derivatives
     only.  Under graph capture forward and backward go into the same graph, and no loss made outside it from the same x or weight may
-    still be alive (refused, for a weight whose rows need no copy)."""
+    still be alive (refused; in a compiled call torch ends the process).  Rows of x and weight at multiples of 16 bytes are read in place; other layouts are copied, in both passes."""
     if not torch.compiler.is_compiling() and reduction in _C.LCE_REDUCTIONS:
         loss = native().cross_entropy(x, weight, labels, ignore_index, _C.LCE_REDUCTIONS[reduction], logit_scale)
         if loss is not None:
             return loss
-    # what the native path leaves: copies of heads that are laid out otherwise, traced calls, and the errors
+    # what the native path leaves: traced calls, tensor subclasses, and the errors
     if x.dtype != torch.bfloat16 or weight.dtype != torch.bfloat16:
         raise _C.XqError(f"linear_cross_entropy: x and weight must be bf16, got {x.dtype} and {weight.dtype}")
     if labels.dtype not in (torch.int64, torch.int32):
