@@ -940,20 +940,22 @@ PyObject* cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
 }
 
 // ---- the optimizer step: its arguments are hundreds of tensors, whose addresses and checks are a matter of tens of microseconds here
+// (a tuple of its own: the caller's list may change while this call converts a number of a user's class or has let go of the GIL, and with it go
+// the tensors)
 struct TensorList {
     const char* name;
     PyObject* seq = nullptr;
     TensorList(const char* n, PyObject* o) : name(n) {
         if (o == Py_None) return;
-        seq = PySequence_Fast(o, "");
+        seq = PySequence_Tuple(o);
         if (!seq) { PyErr_Clear(); throw ArgError(std::string("adamw_step: ") + n + " must be a list of tensors"); }
     }
     ~TensorList() { Py_XDECREF(seq); }
     TensorList(const TensorList&) = delete;
-    Py_ssize_t size() const { return PySequence_Fast_GET_SIZE(seq); }
+    Py_ssize_t size() const { return PyTuple_GET_SIZE(seq); }
     std::string at(Py_ssize_t i) const { return std::string("adamw_step: ") + name + "[" + std::to_string(i) + "]"; }
     const Tensor& operator[](Py_ssize_t i) const {
-        PyObject* o = PySequence_Fast_GET_ITEM(seq, i);
+        PyObject* o = PyTuple_GET_ITEM(seq, i);
         if (!THPVariable_Check(o)) throw ArgError(at(i) + " is not a tensor");
         const Tensor& t = THPVariable_Unpack(o);
         if (!t.defined() || t.layout() != at::kStrided || at::isTensorSubclassLike(t)) throw ArgError(at(i) + " is not a plain dense tensor");
@@ -987,6 +989,10 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         xq_adamw_options o{};
         if (!norm_only && !PyArg_ParseTuple(args[7], "ddddd", &o.lr, &o.beta1, &o.beta2, &o.eps, &o.weight_decay)) return nullptr;
         o.state_bits = eight ? 8 : 32;
+        if (args[9] != Py_None) {          // (before an address is taken: this may run Python)
+            o.max_norm = PyFloat_AsDouble(args[9]);
+            if (o.max_norm == -1.0 && PyErr_Occurred()) return nullptr;
+        }
         std::optional<at::Device> device;
         auto same_device = [&](const Tensor& a, auto&& what) {
             if (!device) device = a.device();
@@ -994,7 +1000,7 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         };
         std::vector<xq_adamw_tensor> q;
         std::vector<Tensor> keep;
-        std::vector<at::TensorImpl*> written;     // (the lists hold them)
+        std::vector<at::TensorImpl*> written;     // (the tuples hold them)
         struct Span { const char *from, *to; bool write; };
         std::vector<Span> once;        // what the step writes and the gradients: written twice, or read where another block writes, the result would hang on the order
         auto note = [&](const Tensor& t, bool write = true) { once.push_back({(const char*)t.data_ptr(), (const char*)t.data_ptr() + nbytes(t), write}); };
@@ -1070,12 +1076,7 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
             norm = *given;
             o.norm_given = 1;
         }
-        if (args[9] != Py_None) {
-            o.max_norm = PyFloat_AsDouble(args[9]);
-            if (o.max_norm == -1.0 && PyErr_Occurred()) return nullptr;
-        } else if (o.norm_given) {
-            throw ArgError("adamw_step: grad_norm without max_norm");
-        }
+        if (args[9] == Py_None && o.norm_given) throw ArgError("adamw_step: grad_norm without max_norm");
         if (!device) {
             if (norm_only || args[9] != Py_None) throw ArgError("adamw_step: a norm over no gradients has no device");
             Py_RETURN_NONE;
