@@ -128,3 +128,22 @@ def test_captured_backward_of_a_subclass_is_refused(hip_device):
     torch.cuda.synchronize()
     got, = torch.autograd.grad(linear_cross_entropy(x, head, labels), x)
     assert torch.equal(got, torch.autograd.grad(linear_cross_entropy(x, w, labels), x)[0])
+
+
+@pytest.mark.parametrize("head_grad", [False, True])
+@pytest.mark.parametrize("which", [0, 1])
+def test_tangents_and_transforms_are_refused(hip_device, which, head_grad):
+    import torch.autograd.forward_ad as fwAD
+
+    x, w, labels = _inputs(20, 300, 64, 74, hip_device)
+    t = [x, w.requires_grad_(head_grad)]
+    for grad in (True, False):
+        with fwAD.dual_level(), torch.set_grad_enabled(grad), pytest.raises(NotImplementedError):
+            t[which] = fwAD.make_dual((x, w)[which], torch.ones_like((x, w)[which]))
+            linear_cross_entropy(*t, labels)
+        t = [x, w]
+    for f in (lambda: torch.func.jvp(lambda a: linear_cross_entropy(a, w, labels), (x,), (torch.ones_like(x),)),
+              lambda: torch.func.grad(lambda a: linear_cross_entropy(a, w, labels))(x),
+              lambda: torch.vmap(lambda a: linear_cross_entropy(a, w, labels))(x[None])):
+        with pytest.raises((RuntimeError, NotImplementedError)):
+            f()

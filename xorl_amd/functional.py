@@ -14,6 +14,7 @@ from typing import List, Optional, Tuple
 
 import torch
 from torch import Tensor
+from torch.autograd import forward_ad
 
 from . import _C
 
@@ -49,6 +50,13 @@ class QuantWeight:
             self._cw = _C.make_weight(self.fmt, self.layout, self.packed, self.scales, self.scale_dtype, self.rows,
                                       self.cols, self.group, self.global_scale, self.num_experts)
         return self._cw
+
+
+def refuse_tangents(*tensors: Optional[Tensor]) -> None:
+    """For calls that go past autograd: a tangent of forward-mode differentiation would be dropped there, and the derivative read as
+    zero.  Refused like by the autograd functions, which define no forward mode."""
+    if forward_ad._current_level >= 0 and any(t is not None and forward_ad.unpack_dual(t).tangent is not None for t in tensors):
+        raise NotImplementedError("xorl_amd operators define no forward-mode derivative; got a tensor that carries a tangent")
 
 
 def _r_pad(r: int) -> int:

@@ -15,7 +15,7 @@ from torch import Tensor
 
 from . import _C
 from ._native import native
-from .functional import _as_2d, _ld
+from .functional import _as_2d, _ld, refuse_tangents
 
 
 def _rows_of(w: Tensor) -> Tensor:
@@ -144,6 +144,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
         raise _C.XqError(f"linear_cross_entropy: logit_scale must be positive and finite, got {logit_scale}")
     if not -2 ** 63 <= int(ignore_index) < 2 ** 63:
         raise _C.XqError(f"linear_cross_entropy: ignore_index must fit 64 bits, got {ignore_index}")
+    if not torch.compiler.is_compiling():
+        refuse_tangents(x, weight)
     _C.require_hip(x, weight, labels)
     if weight.device != x.device or labels.device != x.device:
         raise _C.XqError(f"linear_cross_entropy: x, weight and labels are on {x.device}, {weight.device} and {labels.device}")
