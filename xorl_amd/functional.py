@@ -296,6 +296,7 @@ def qlora_linear(x: Tensor, qw: QuantWeight, lora_A: Optional[Tensor], lora_B: O
     if not training and not torch.compiler.is_compiling():
         # decode-regime calls are launch-bound: go straight to the library, skipping the autograd and
         # custom-op dispatch layers (tens of microseconds of host time per call)
+        refuse_tangents(x, lora_A, lora_B, bias)
         A = lora_A.detach()[:r] if lora_A is not None else None
         B = lora_B.detach()[:, :r] if lora_B is not None else None
         return _linear_fwd_impl(x.detach(), qw.packed, qw.scales, qw.global_scale, A, B,
@@ -320,6 +321,7 @@ def qlora_linear_swiglu(x: Tensor, qw: QuantWeight, lora_A: Optional[Tensor], lo
         raise _C.XqError(f"qlora_linear_swiglu: rank {r} exceeds {MAX_FUSED_RANK}")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, lora_A, lora_B, bias)):
         raise _C.XqError("qlora_linear_swiglu is forward-only: call it under torch.no_grad()")
+    refuse_tangents(x, lora_A, lora_B, bias)
     if qw.rows % 2:
         raise _C.XqError(f"qlora_linear_swiglu: the weight must hold gate | up, got {qw.rows} rows")
     _C.require_hip(x)
@@ -357,6 +359,7 @@ def qlora_linear_multi(x: Tensor, jobs) -> list:
         raise _C.XqError(f"activations must be bf16, got {x.dtype}")
     if torch.is_grad_enabled() and any(t is not None and t.requires_grad for j in jobs for t in (x, j[1], j[2], j[5])):
         raise _C.XqError("qlora_linear_multi is forward-only: call it under torch.no_grad()")
+    refuse_tangents(x, *(t for j in jobs for t in (j[1], j[2], j[5])))
     x2 = _as_2d(x)
     M, K = x2.shape
     dev = x.device
@@ -615,6 +618,7 @@ def qlora_mlp_infer(x: Tensor, qw_gate: QuantWeight, qw_up: QuantWeight, qw_down
         raise _C.XqError(f"the fused MLP takes LoRA ranks up to {MAX_FUSED_RANK}, got {r}")
     if x.dtype != torch.bfloat16:
         raise _C.XqError(f"activations must be bf16, got {x.dtype}")
+    refuse_tangents(x, gate_A, gate_B, up_A, up_B, down_A, down_B, bias_gate, bias_up, bias_down)
     _C.require_hip(x)
     x2 = _as_2d(x)
     M, H = x2.shape

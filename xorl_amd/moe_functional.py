@@ -20,7 +20,7 @@ from torch import Tensor
 
 from . import _C
 from ._native import native
-from .functional import _CODE_TO_DT, _DT_TO_CODE, QuantWeight, _as_2d, _r_pad
+from .functional import _CODE_TO_DT, _DT_TO_CODE, QuantWeight, _as_2d, _r_pad, refuse_tangents
 
 
 def _s(dev):
@@ -361,6 +361,7 @@ def _moe_infer(hidden: Tensor, routing_weights: Tensor, selected_experts: Tensor
     are read by the compiled host path."""
     if module is not None:
         return native().moe(module, hidden, routing_weights, selected_experts, True)
+    refuse_tangents(hidden, routing_weights, *factors)
     qg, qu, qd = banks
     H = qg.rows
     if (hidden.dtype != torch.bfloat16 or not hidden.is_cuda or hidden.numel() == 0 or hidden.shape[-1] != H
