@@ -155,10 +155,14 @@ class AdamW(torch.optim.Optimizer):
         for g in state_dict["param_groups"]:
             if g.get("amsgrad") or g.get("maximize"):
                 raise _C.XqError("AdamW: amsgrad and maximize have no counterpart here")
+            if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
+                raise _C.XqError("AdamW: a weight decay that is added to the gradients has no counterpart here")
         # the base class casts floating-point state, and codes with it, to the parameter's type
         super().load_state_dict(state_dict)
         for g in self.param_groups:
             g.setdefault("state_bits", 32)
+            if "decoupled_weight_decay" in g:           # (without a decay it may have come as False)
+                g["decoupled_weight_decay"] = True
         saved = [i for g in state_dict["param_groups"] for i in g["params"]]
         own = [p for g in self.param_groups for p in g["params"]]
         for i, p in zip(saved, own):
