@@ -29,3 +29,31 @@ def test_decay_that_is_added_to_the_gradients_is_refused():
         again = AdamW([p])
         again.load_state_dict(opt.state_dict())
         assert again.param_groups[0]["weight_decay"] == 0.2
+
+
+@pytest.mark.parametrize("step", [3, 3.0, torch.tensor(3), torch.tensor(3, dtype=torch.int32), torch.tensor(3.0, dtype=torch.float64)])
+@pytest.mark.parametrize("default", [torch.float32, torch.bfloat16])
+def test_step_counts_are_taken_in_fp32(step, default):
+    """whatever the dictionary holds, and whatever numbers become tensors of by default"""
+    p = torch.nn.Parameter(torch.ones(8))
+    d = _adam(0.0)
+    d["state"][0]["step"] = step
+    torch.set_default_dtype(default)
+    try:
+        opt = AdamW([p])
+        opt.load_state_dict(d)
+    finally:
+        torch.set_default_dtype(torch.float32)
+    s = opt.state[p]
+    assert s["step"].dtype == torch.float32 and s["step"].shape == () and float(s["step"]) == 3.0 and s["exp_avg"].dtype == torch.float32
+
+
+def test_codes_are_taken_as_they_are():
+    p = torch.nn.Parameter(torch.ones(300))
+    opt = AdamW([p], state_bits=8)
+    codes = {"step": torch.tensor(2.0), "exp_avg": torch.arange(300).to(torch.int8), "exp_avg_sq": torch.arange(300).to(torch.uint8),
+             "exp_avg_scale": torch.rand(2), "exp_avg_sq_scale": torch.rand(2)}
+    d = opt.state_dict()
+    d["state"][0] = codes
+    opt.load_state_dict(d)
+    assert all(opt.state[p][k].dtype == v.dtype and torch.equal(opt.state[p][k], v) and opt.state[p][k] is not v for k, v in codes.items())

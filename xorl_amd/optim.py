@@ -171,10 +171,10 @@ class AdamW(torch.optim.Optimizer):
 
 
 def _state(v, device):
-    """A copy of a loaded state on ``device``: codes as they are, all else (moments in bf16, a step count that is a number) in fp32"""
+    """A copy of a loaded state on ``device``: codes as they are, all else (moments in bf16, a step count that is a number or an integer) in fp32"""
     if isinstance(v, Tensor):
-        return v.detach().to(device, torch.float32 if v.is_floating_point() else v.dtype, copy=True)
-    return torch.tensor(float(v), device=device) if isinstance(v, (int, float)) else v
+        return v.detach().to(device, v.dtype if v.dtype in (torch.int8, torch.uint8) else torch.float32, copy=True)
+    return torch.tensor(float(v), dtype=torch.float32, device=device) if isinstance(v, (int, float)) else v
 
 
 def _local(t: Tensor) -> Tensor:
