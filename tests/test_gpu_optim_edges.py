@@ -56,3 +56,35 @@ def test_lists_that_another_thread_changes(hip_device):
         done.set()
         thread.join()
     assert [float(t) for t in prob[4]] == [103.0 + 7 * (i % 5) for i in range(200)]
+
+
+# ---------------------------------------------------------------- tensors without elements
+@pytest.mark.parametrize("bits", [32, 8])
+@pytest.mark.parametrize("shapes", [[(0,)], [(0, 3), (5,), (0,)], [(300,), (0,), (4097,), (7, 0)]])
+@pytest.mark.parametrize("clip", [None, 0.01])
+def test_tensors_without_elements_count_their_steps(hip_device, bits, shapes, clip):
+    """like the others (a rank's share of a sharded parameter may be empty), and change nothing for them"""
+    prob, want = (_problem(shapes, bits, torch.float32, torch.float32, 53, hip_device) for _ in range(2))
+    before = [float(t) for t in prob[4]]
+    versions = [t._version for t in prob[4]]
+    norm = _step(prob, max_norm=clip)
+    assert [float(t) for t in prob[4]] == [b + 1 for b in before] and all(t._version > v for t, v in zip(prob[4], versions))
+    some = [i for i, s in enumerate(shapes) if 0 not in s]
+    short, full = ([None if l is None else [l[i] for i in some] for l in q] for q in (prob, want))
+    if some:
+        assert clip is None or torch.equal(norm, grad_norm(full[1]))
+        _step(full, max_norm=clip)
+        assert _same(short, full)
+
+
+def test_tensors_without_elements_in_a_graph(hip_device):
+    prob = _problem([(0,), (9,), (0, 4)], 32, torch.float32, torch.float32, 54, hip_device)
+    before = [float(t) for t in prob[4]]
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        _step(prob)
+    for k in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert [float(t) for t in prob[4]] == [b + k + 1 for b in before]

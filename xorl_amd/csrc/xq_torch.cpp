@@ -17,6 +17,7 @@
 #include <ATen/TracerMode.h>
 #include <ATen/core/Tensor.h>
 #include <ATen/EmptyTensor.h>
+#include <ATen/ops/_foreach_add.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
@@ -999,7 +1000,7 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
             else if (a.device() != *device) throw ArgError(what() + " is on " + a.device().str() + ", others on " + device->str());
         };
         std::vector<xq_adamw_tensor> q;
-        std::vector<Tensor> keep;
+        std::vector<Tensor> keep, empty_steps;    // (step counts of tensors without elements, of which the kernels hear nothing)
         std::vector<at::TensorImpl*> written;     // (the tuples hold them)
         struct Span { const char *from, *to; bool write; };
         std::vector<Span> once;        // what the step writes and the gradients: written twice, or read where another block writes, the result would hang on the order
@@ -1052,6 +1053,7 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
                 written.push_back(st.unsafeGetTensorImpl());
                 note(st);
                 if (a.numel && a.grad == gr.data_ptr()) note(gr, false);
+                if (!a.numel) empty_steps.push_back(st);
             }
             if (a.numel) q.push_back(a);
         }
@@ -1090,6 +1092,10 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
             ReleaseGil nogil;
             check(norm_only ? xq_grad_norm(q.data(), (int64_t)q.size(), o.norm, ws.get(), ws.bytes, stream)
                             : xq_adamw_step(q.data(), (int64_t)q.size(), &o, ws.get(), ws.bytes, stream));
+        }
+        if (!empty_steps.empty()) {
+            at::AutoDispatchBelowADInplaceOrView below;
+            at::_foreach_add_(empty_steps, 1);
         }
         for (at::TensorImpl* w : written)
             if (!w->is_inference()) w->bump_version();

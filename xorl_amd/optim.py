@@ -40,7 +40,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     Parameters and gradients are fp32 or bf16, tensor by tensor; parameters, states and step counts are contiguous and share no
     memory, with gradients neither (both refused otherwise; a gradient that is not contiguous is copied).  States are fp32, or, with both lists of scales
     given, 8-bit codes: int8 ``exp_avgs`` and uint8 ``exp_avg_sqs`` with fp32 scales for every 256 elements (``adamw_state_values``
-    says what they stand for).  ``steps`` are fp32 tensors of one element each, advanced here.  ``lr`` may be a 0-dim fp32 tensor on
+    says what they stand for).  ``steps`` are fp32 tensors of one element each, advanced here (of tensors without elements too).  ``lr`` may be a 0-dim fp32 tensor on
     the device: a captured step then follows it.
 
     ``max_norm`` scales the gradients by min(1, max_norm / (norm + 1e-6)) on the way, ``norm`` being the 2-norm over all of them
