@@ -5,7 +5,9 @@ import threading
 import pytest
 import torch
 
+from tests.test_gpu_fsdp2 import one_rank_group  # noqa: F401
 from tests.test_gpu_optim import SIZES, U, _problem
+from tests.util_cases import make_dense_module
 from xorl_amd import _C
 from xorl_amd.optim import AdamW, adamw_step, grad_norm
 
@@ -88,3 +90,40 @@ def test_tensors_without_elements_in_a_graph(hip_device):
         graph.replay()
         torch.cuda.synchronize()
         assert [float(t) for t in prob[4]] == [b + k + 1 for b in before]
+
+
+# ---------------------------------------------------------------- modules under FSDP2, one rank
+@pytest.mark.parametrize("bits", [32, 8])
+def test_factors_under_fsdp2(hip_device, one_rank_group, bits):
+    """The steps of a wrapped module's factors are the plain module's; a distributed checkpoint's state dictionary goes round"""
+    from torch.distributed._composable.fsdp import fully_shard
+    from torch.distributed.checkpoint.state_dict import get_optimizer_state_dict, set_optimizer_state_dict
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor
+
+    plain, wrapped = (make_dense_module("block_fp8", 256, 384, 16, 32, 3, hip_device)[0] for _ in range(2))
+    fully_shard(wrapped, mesh=init_device_mesh("cuda", (1,)), reshard_after_forward=True)
+    runs = [(m, AdamW([m.lora_A, m.lora_B], lr=1e-2, state_bits=bits, max_grad_norm=0.5)) for m in (plain, wrapped)]
+    assert isinstance(wrapped.lora_A, DTensor)
+    for k in range(4):
+        x = torch.randn(70, 384, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(k)).to(torch.bfloat16)
+        if k == 2 and bits == 32:
+            m, opt = runs[1]
+            saved = get_optimizer_state_dict(m, opt)
+            opt = AdamW([m.lora_A, m.lora_B], lr=5.0, max_grad_norm=0.5)
+            set_optimizer_state_dict(m, opt, saved)
+            assert opt.param_groups[0]["lr"] == 1e-2
+            runs[1] = (m, opt)
+        for m, opt in runs:
+            opt.zero_grad()
+            m(x).float().square().mean().backward()
+            opt.step()
+        assert torch.equal(runs[0][1].grad_norm, runs[1][1].grad_norm)
+    for name in ("lora_A", "lora_B"):
+        a, b = getattr(plain, name), getattr(wrapped, name)
+        assert torch.equal(a, b.to_local())
+        s, t = runs[0][1].state[a], runs[1][1].state[b]
+        assert set(s) == set(t) and float(s["step"]) == 4.0
+        for key, value in t.items():
+            sharded = bits == 32 and key in ("exp_avg", "exp_avg_sq")
+            assert isinstance(value, DTensor) == sharded and torch.equal(s[key], value.to_local() if sharded else value)

@@ -57,3 +57,49 @@ def test_codes_are_taken_as_they_are():
     d["state"][0] = codes
     opt.load_state_dict(d)
     assert all(opt.state[p][k].dtype == v.dtype and torch.equal(opt.state[p][k], v) and opt.state[p][k] is not v for k, v in codes.items())
+
+
+# ---------------------------------------------------------------- sharded parameters, two ranks over gloo
+def _two_ranks(rank, path):
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import DTensor, Partial, Replicate, Shard, distribute_tensor
+
+    dist.init_process_group("gloo", init_method=f"file://{path}", rank=rank, world_size=2)
+    mesh = init_device_mesh("cpu", (2,))
+    whole = torch.arange(21.0).view(7, 3)
+
+    def made(placement, grad=None):
+        p = torch.nn.Parameter(distribute_tensor(whole, mesh, [placement]))
+        p.grad = distribute_tensor(torch.ones(7, 3), mesh, [grad or placement])
+        return p
+
+    def refused(match, p, error=_C.XqError, **kw):
+        opt = AdamW([p], **kw)
+        with pytest.raises(error, match=match):
+            opt.step()
+        return opt
+
+    refused("norm over all ranks", made(Shard(0)), max_grad_norm=1.0)
+    assert not any(refused("could not be resharded", made(Shard(0)), state_bits=8).state.values())
+    # (where the norm of what a rank has is that of all, and blocks are of the whole, nothing is refused but the CPU)
+    refused("HIP device only", made(Replicate()), RuntimeError, max_grad_norm=1.0, state_bits=8)
+    # moments like the parameter, so that a checkpoint knows whose they are; a share of 4 and one of 3 rows
+    p = made(Shard(0))
+    opt = refused("HIP device only", p, RuntimeError)
+    state = opt.state[p]
+    for k in ("exp_avg", "exp_avg_sq"):
+        assert isinstance(state[k], DTensor) and state[k].placements == p.placements and state[k].shape == (7, 3) and state[k].dtype == torch.float32
+        assert state[k].to_local().shape == (4 - rank, 3) and not state[k].requires_grad
+    assert type(state["step"]) is torch.Tensor
+    with torch.no_grad():
+        state["exp_avg"].copy_(p)
+    again = AdamW([p], lr=7.0)
+    again.load_state_dict(opt.state_dict())
+    got = again.state[p]["exp_avg"]
+    assert isinstance(got, DTensor) and got.placements == p.placements and torch.equal(got.full_tensor(), whole)
+    dist.destroy_process_group()
+
+
+def test_sharded_parameters(tmp_path):
+    torch.multiprocessing.spawn(_two_ranks, args=(str(tmp_path / "store"),), nprocs=2)

@@ -82,7 +82,11 @@ class AdamW(torch.optim.Optimizer):
     over the parameters of all groups inside the step; the norm of the last step is ``self.grad_norm`` (a device tensor).  States are
     made at a parameter's first step and whenever its state has been dropped, but not while a graph is captured (refused: they would be made
     anew in every replay).  In a captured step ``lr`` follows a tensor, a number stays what it was.  State names: ``step``, ``exp_avg``, ``exp_avg_sq``, with
-    8 bits ``exp_avg_scale`` and ``exp_avg_sq_scale`` too.  All parameters lie on one device."""
+    8 bits ``exp_avg_scale`` and ``exp_avg_sq_scale`` too.  All parameters lie on one device.
+
+    Distributed parameters (DTensor, as FSDP2 makes them): every rank steps its own share, and 32-bit moments are distributed tensors like them, so that a distributed checkpoint can carry them.  Over several ranks
+    ``max_grad_norm`` and 8-bit states of sharded parameters are refused: the norm would be a share's, and the blocks of codes that share a scale are
+    blocks of a share, which no other number of ranks can take up."""
 
     def __init__(self, params, lr: Union[float, Tensor] = 1e-3, betas: Tuple[float, float] = (0.9, 0.999), eps: float = 1e-8,
                  weight_decay: float = 0.01, *, state_bits: int = 32, max_grad_norm: Optional[float] = None):
@@ -109,6 +113,8 @@ class AdamW(torch.optim.Optimizer):
             local = _local(p)
             if local.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise _C.XqError("AdamW: a captured step would make its states anew in every replay; take one step before the capture")
+            if state_bits == 8 and _sharded(p):
+                raise _C.XqError("AdamW: 8-bit states of a parameter that is sharded over ranks could not be resharded; take 32 bits")
             state["step"] = torch.zeros((), dtype=torch.float32, device=local.device)
             if state_bits == 8:
                 n = _scale_count(local.numel())
@@ -117,8 +123,8 @@ class AdamW(torch.optim.Optimizer):
                 state["exp_avg_scale"] = torch.zeros(n, dtype=torch.float32, device=local.device)
                 state["exp_avg_sq_scale"] = torch.zeros(n, dtype=torch.float32, device=local.device)
             else:
-                state["exp_avg"] = torch.zeros(local.shape, dtype=torch.float32, device=local.device)
-                state["exp_avg_sq"] = torch.zeros(local.shape, dtype=torch.float32, device=local.device)
+                state["exp_avg"] = _zeros_fp32(p)
+                state["exp_avg_sq"] = _zeros_fp32(p)
         return state
 
     @torch.no_grad()
@@ -129,20 +135,22 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         groups = [(g, [p for p in g["params"] if p.grad is not None]) for g in self.param_groups]
         groups = [(g, ps) for g, ps in groups if ps]
+        distributed = [p for _, ps in groups for p in ps if hasattr(p, "to_local")]
+        local = _local if distributed else lambda t: t
         norm = None
         if self.max_grad_norm is not None and groups:
-            if any(_sharded(p) for _, ps in groups for p in ps):
+            if any(_sharded(p) for p in distributed):
                 raise _C.XqError("max_grad_norm over sharded parameters: clip them with a norm over all ranks, and leave it out here")
             if len(groups) > 1:
-                norm = grad_norm([_local(p.grad) for _, ps in groups for p in ps])
+                norm = grad_norm([local(p.grad) for _, ps in groups for p in ps])
         for g, ps in groups:
             states = [self._init_state(p, g["state_bits"]) for p in ps]
 
             def of(name):
-                return [s[name] for s in states]
+                return [local(s[name]) for s in states]
 
             eight = g["state_bits"] == 8
-            out = adamw_step([_local(p) for p in ps], [_local(p.grad) for p in ps], of("exp_avg"), of("exp_avg_sq"), of("step"),
+            out = adamw_step([local(p) for p in ps], [local(p.grad) for p in ps], of("exp_avg"), of("exp_avg_sq"), of("step"),
                              exp_avg_scales=of("exp_avg_scale") if eight else None, exp_avg_sq_scales=of("exp_avg_sq_scale") if eight else None,
                              lr=g["lr"], betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], max_norm=self.max_grad_norm,
                              grad_norm=norm)
@@ -178,9 +186,13 @@ def _state(v, device):
 
 
 def _local(t: Tensor) -> Tensor:
-    """The rank's own shard of a distributed tensor (the update is elementwise); other tensors as they are."""
+    """The rank's own share of a distributed tensor (the update is elementwise); other tensors as they are."""
     return t.to_local() if hasattr(t, "to_local") else t
 
 
+def _zeros_fp32(p: Tensor) -> Tensor:
+    return torch.zeros_like(p, dtype=torch.float32, requires_grad=False) if hasattr(p, "to_local") else torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+
+
 def _sharded(p: Tensor) -> bool:
-    return hasattr(p, "to_local") and p.device_mesh.size() > 1
+    return hasattr(p, "to_local") and any(p.device_mesh.size(i) > 1 and not q.is_replicate() for i, q in enumerate(p.placements))
