@@ -84,6 +84,10 @@ def _two_ranks(rank, path):
     assert not any(refused("could not be resharded", made(Shard(0)), state_bits=8).state.values())
     # (where the norm of what a rank has is that of all, and blocks are of the whole, nothing is refused but the CPU)
     refused("HIP device only", made(Replicate()), RuntimeError, max_grad_norm=1.0, state_bits=8)
+    refused("distributed otherwise", made(Shard(0), Replicate()))
+    p = made(Replicate())
+    p.grad = DTensor.from_local(torch.ones(7, 3), mesh, [Partial()])            # (of the local shape that it should have, and a share of the sum)
+    refused("distributed otherwise", p)
     # moments like the parameter, so that a checkpoint knows whose they are; a share of 4 and one of 3 rows
     p = made(Shard(0))
     opt = refused("HIP device only", p, RuntimeError)

@@ -84,7 +84,8 @@ class AdamW(torch.optim.Optimizer):
     anew in every replay).  In a captured step ``lr`` follows a tensor, a number stays what it was.  State names: ``step``, ``exp_avg``, ``exp_avg_sq``, with
     8 bits ``exp_avg_scale`` and ``exp_avg_sq_scale`` too.  All parameters lie on one device.
 
-    Distributed parameters (DTensor, as FSDP2 makes them): every rank steps its own share, and 32-bit moments are distributed tensors like them, so that a distributed checkpoint can carry them.  Over several ranks
+    Distributed parameters (DTensor, as FSDP2 makes them): every rank steps its own share, gradients are to be distributed like their
+    parameters, and 32-bit moments are distributed tensors like them, so that a distributed checkpoint can carry them.  Over several ranks
     ``max_grad_norm`` and 8-bit states of sharded parameters are refused: the norm would be a share's, and the blocks of codes that share a scale are
     blocks of a share, which no other number of ranks can take up."""
 
@@ -136,6 +137,9 @@ class AdamW(torch.optim.Optimizer):
         groups = [(g, [p for p in g["params"] if p.grad is not None]) for g in self.param_groups]
         groups = [(g, ps) for g, ps in groups if ps]
         distributed = [p for _, ps in groups for p in ps if hasattr(p, "to_local")]
+        for p in distributed:
+            if _layout(p) != _layout(p.grad):
+                raise _C.XqError(f"AdamW: a gradient is distributed otherwise than its parameter: {_layout(p.grad)}, {_layout(p)}")
         local = _local if distributed else lambda t: t
         norm = None
         if self.max_grad_norm is not None and groups:
@@ -192,6 +196,10 @@ def _local(t: Tensor) -> Tensor:
 
 def _zeros_fp32(p: Tensor) -> Tensor:
     return torch.zeros_like(p, dtype=torch.float32, requires_grad=False) if hasattr(p, "to_local") else torch.zeros(p.shape, dtype=torch.float32, device=p.device)
+
+
+def _layout(t: Tensor):
+    return (t.device_mesh, tuple(t.placements)) if hasattr(t, "to_local") else None
 
 
 def _sharded(p: Tensor) -> bool:
