@@ -81,7 +81,13 @@ def _two_ranks(rank, path):
         return opt
 
     refused("norm over all ranks", made(Shard(0)), max_grad_norm=1.0)
-    assert not any(refused("could not be resharded", made(Shard(0)), state_bits=8).state.values())
+    p = made(Shard(0))
+    opt = refused("could not be resharded", p, state_bits=8)
+    assert not opt.state
+    # (and where a dictionary has them)
+    opt.load_state_dict({**opt.state_dict(), "state": {0: {"step": 1.0, "exp_avg": torch.zeros(4 - rank, 3, dtype=torch.int8)}}})
+    with pytest.raises(_C.XqError, match="could not be resharded"):
+        opt.step()
     # (where the norm of what a rank has is that of all, and blocks are of the whole, nothing is refused but the CPU)
     refused("HIP device only", made(Replicate()), RuntimeError, max_grad_norm=1.0, state_bits=8)
     refused("distributed otherwise", made(Shard(0), Replicate()))

@@ -114,8 +114,6 @@ class AdamW(torch.optim.Optimizer):
             local = _local(p)
             if local.is_cuda and torch.cuda.is_current_stream_capturing():
                 raise _C.XqError("AdamW: a captured step would make its states anew in every replay; take one step before the capture")
-            if state_bits == 8 and _sharded(p):
-                raise _C.XqError("AdamW: 8-bit states of a parameter that is sharded over ranks could not be resharded; take 32 bits")
             state["step"] = torch.zeros((), dtype=torch.float32, device=local.device)
             if state_bits == 8:
                 n = _scale_count(local.numel())
@@ -136,14 +134,16 @@ class AdamW(torch.optim.Optimizer):
                 loss = closure()
         groups = [(g, [p for p in g["params"] if p.grad is not None]) for g in self.param_groups]
         groups = [(g, ps) for g, ps in groups if ps]
-        distributed = [p for _, ps in groups for p in ps if hasattr(p, "to_local")]
-        for p in distributed:
+        distributed = [(g, p) for g, ps in groups for p in ps if hasattr(p, "to_local")]
+        for g, p in distributed:
+            if g["state_bits"] == 8 and _sharded(p):
+                raise _C.XqError("AdamW: 8-bit states of a parameter that is sharded over ranks could not be resharded; take 32 bits")
             if _layout(p) != _layout(p.grad):
                 raise _C.XqError(f"AdamW: a gradient is distributed otherwise than its parameter: {_layout(p.grad)}, {_layout(p)}")
         local = _local if distributed else lambda t: t
         norm = None
         if self.max_grad_norm is not None and groups:
-            if any(_sharded(p) for p in distributed):
+            if any(_sharded(p) for _, p in distributed):
                 raise _C.XqError("max_grad_norm over sharded parameters: clip them with a norm over all ranks, and leave it out here")
             if len(groups) > 1:
                 norm = grad_norm([local(p.grad) for _, ps in groups for p in ps])
