@@ -127,3 +127,22 @@ def test_factors_under_fsdp2(hip_device, one_rank_group, bits):
         for key, value in t.items():
             sharded = bits == 32 and key in ("exp_avg", "exp_avg_sq")
             assert isinstance(value, DTensor) == sharded and torch.equal(s[key], value.to_local() if sharded else value)
+
+
+# ---------------------------------------------------------------- memory that arguments share
+@pytest.mark.parametrize("bits", [32, 8])
+def test_a_rate_or_norm_that_the_step_writes_is_refused(hip_device, bits):
+    """Every block reads them while others write: a rate that is itself a parameter, a norm that is a step count or one of the scales"""
+    prob = _problem([(1,), (700,)], bits, torch.float32, torch.float32, 55, hip_device)
+    before = [None if l is None else [t.clone() for t in l] for l in prob]
+    written = [prob[0][0], prob[0][1][300:301], prob[4][1]]
+    written += [prob[5][1][2:3], prob[6][0]] if bits == 8 else [prob[2][0], prob[3][1][699:]]
+    for t in written:
+        for kw in (dict(lr=t), dict(max_norm=1.0, grad_norm=t), dict(lr=t, max_norm=1.0, grad_norm=t)):
+            with pytest.raises(_C.XqError, match="share"):
+                _step(prob, **kw)
+    assert _same(prob, before)
+    both = torch.tensor(1e-3, device=hip_device)               # (read by both, and a gradient at that: nothing is written)
+    prob[1][0] = both.view(1)
+    _step(prob, lr=both, max_norm=1.0, grad_norm=both)
+    assert float(both) == torch.tensor(1e-3).item()

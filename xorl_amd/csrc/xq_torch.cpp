@@ -1003,7 +1003,7 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
         std::vector<Tensor> keep, empty_steps;    // (step counts of tensors without elements, of which the kernels hear nothing)
         std::vector<at::TensorImpl*> written;     // (the tuples hold them)
         struct Span { const char *from, *to; bool write; };
-        std::vector<Span> once;        // what the step writes and the gradients: written twice, or read where another block writes, the result would hang on the order
+        std::vector<Span> once;        // what the step writes and what it reads all along: written twice, or read where another block writes, the result would hang on the order
         auto note = [&](const Tensor& t, bool write = true) { once.push_back({(const char*)t.data_ptr(), (const char*)t.data_ptr() + nbytes(t), write}); };
         q.reserve(n);
         written.reserve(6 * n);
@@ -1057,18 +1057,12 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
             }
             if (a.numel) q.push_back(a);
         }
-        std::sort(once.begin(), once.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
-        const char *read_to = nullptr, *written_to = nullptr;         // the ends of what came before
-        for (const Span& a : once) {
-            if (a.from < written_to || (a.write && a.from < read_to)) throw ArgError("adamw_step: two tensors share memory of a parameter, a state or a step count");
-            const char*& to = a.write ? written_to : read_to;
-            to = std::max(to, a.to);
-        }
         if (args[8] != Py_None) {
             const Tensor* lr = plain(args[8]);
             if (!lr || lr->scalar_type() != at::kFloat || lr->numel() != 1) throw ArgError("adamw_step: an lr tensor must be one fp32 element on the device");
             same_device(*lr, [] { return std::string("adamw_step: lr"); });
             o.lr_device = (const float*)lr->data_ptr();
+            note(*lr, false);
         }
         Tensor norm;
         if (args[10] != Py_None) {
@@ -1077,6 +1071,14 @@ PyObject* adamw(PyObject*, PyObject* const* args, Py_ssize_t n_args) {
             same_device(*given, [] { return std::string("adamw_step: grad_norm"); });
             norm = *given;
             o.norm_given = 1;
+            note(norm, false);
+        }
+        std::sort(once.begin(), once.end(), [](const Span& a, const Span& b) { return a.from < b.from; });
+        const char *read_to = nullptr, *written_to = nullptr;         // the ends of what came before
+        for (const Span& a : once) {
+            if (a.from < written_to || (a.write && a.from < read_to)) throw ArgError("adamw_step: two tensors share memory of a parameter, a state or a step count");
+            const char*& to = a.write ? written_to : read_to;
+            to = std::max(to, a.to);
         }
         if (args[9] == Py_None && o.norm_given) throw ArgError("adamw_step: grad_norm without max_norm");
         if (!device) {

@@ -38,7 +38,7 @@ def adamw_step(params: Sequence[Tensor], grads: Sequence[Tensor], exp_avgs: Sequ
     """One AdamW step over all ``params``, in place, with the states they come with.
 
     Parameters and gradients are fp32 or bf16, tensor by tensor; parameters, states and step counts are contiguous and share no
-    memory, with gradients neither (both refused otherwise; a gradient that is not contiguous is copied).  States are fp32, or, with both lists of scales
+    memory, with gradients, ``lr`` and ``grad_norm`` neither (refused otherwise; a gradient that is not contiguous is copied).  States are fp32, or, with both lists of scales
     given, 8-bit codes: int8 ``exp_avgs`` and uint8 ``exp_avg_sqs`` with fp32 scales for every 256 elements (``adamw_state_values``
     says what they stand for).  ``steps`` are fp32 tensors of one element each, advanced here (of tensors without elements too).  ``lr`` may be a 0-dim fp32 tensor on
     the device: a captured step then follows it.
