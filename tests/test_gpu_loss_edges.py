@@ -147,3 +147,26 @@ def test_tangents_and_transforms_are_refused(hip_device, which, head_grad):
               lambda: torch.vmap(lambda a: linear_cross_entropy(a, w, labels))(x[None])):
         with pytest.raises((RuntimeError, NotImplementedError)):
             f()
+
+
+def test_captured_backward_over_two_streams_of_one_capture(hip_device):
+    """What comes before the loss runs on a stream that the same capture has forked: its gradients may go there"""
+    x, w, labels = _inputs(40, 1000, 128, 75, hip_device)
+    x.requires_grad_(True)
+    side, graph = torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        here = torch.cuda.current_stream()
+        side.wait_stream(here)
+        with torch.cuda.stream(side):
+            h = x * 2.0
+        here.wait_stream(side)
+        loss = linear_cross_entropy(h, w, labels)
+        dx, = torch.autograd.grad(loss, x)
+        here.wait_stream(side)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        want = linear_cross_entropy(x * 2.0, w, labels)
+        assert torch.equal(loss.detach(), want.detach()) and torch.equal(dx, torch.autograd.grad(want, x)[0])
+        torch.cuda.synchronize()

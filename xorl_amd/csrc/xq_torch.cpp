@@ -19,6 +19,7 @@
 #include <ATen/EmptyTensor.h>
 #include <ATen/ops/_foreach_add.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
+#include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/core/GradMode.h>
 #include <c10/hip/HIPStream.h>
@@ -478,6 +479,15 @@ struct HeadLoss {
     static Tensor aligned(const Tensor& t) { return t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 != 0 ? t.clone() : t; }
 };
 
+// whether a stream of torch's is part of this capture (the default stream, which has id 0, never is, and may not be asked while one goes on)
+bool in_capture(const c10::Stream& s, unsigned long long id) {
+    if (s.id() == 0) return false;
+    hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+    unsigned long long other = 0;
+    const hipStream_t h = c10::hip::HIPStreamMasqueradingAsCUDA(s).stream();
+    return hipStreamGetCaptureInfo(h, &status, &other) == hipSuccess && status == hipStreamCaptureStatusActive && other == id;
+}
+
 struct LinearCrossEntropyBackward : public Node {
     SavedVariable x_, w_, labels_, saved_;
     int64_t ignore = 0;
@@ -499,15 +509,16 @@ struct LinearCrossEntropyBackward : public Node {
         const Tensor x = x_.unpack(), w = w_.unpack(), labels = labels_.unpack(), saved = saved_.unpack(shared_from_this());
         c10::DeviceGuard guard(x.device());
         const bool again = at::GradMode::is_enabled();
-        // Gradients that go on to another stream make that stream wait for this one; under capture that ends the process.  A leaf's stream is that of
-        // the oldest graph which still holds it, so an eager loss that lives is enough.
+        // Gradients that go on to another stream make that stream wait for this one; under capture that ends the process, unless the stream is in the
+        // same capture.  A leaf's stream is that of the oldest graph which still holds it, so an eager loss that lives is enough.
         hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        if (hipStreamIsCapturing((hipStream_t)stream_of(x), &capture) == hipSuccess && capture != hipStreamCaptureStatusNone) {
+        unsigned long long capture_id = 0;
+        if (hipStreamGetCaptureInfo((hipStream_t)stream_of(x), &capture, &capture_id) == hipSuccess && capture != hipStreamCaptureStatusNone) {
             const c10::StreamId here = c10::hip::getCurrentHIPStream(x.device().index()).unwrap().id();
             for (uint32_t i = 0; i < num_outputs(); ++i) {
                 const auto& edge = next_edge(i);
                 const auto there = edge.function ? edge.function->stream() : std::nullopt;
-                if (task_should_compute_output(i) && there && there->id() != here)
+                if (task_should_compute_output(i) && there && there->id() != here && !in_capture(*there, capture_id))
                     throw std::runtime_error("linear_cross_entropy: a captured backward would hand its gradients to another stream; free the losses that were made "
                                              "from the same tensors outside the capture, and make x inside it or let it be a leaf");
             }
