@@ -170,3 +170,51 @@ def test_captured_backward_over_two_streams_of_one_capture(hip_device):
         want = linear_cross_entropy(x * 2.0, w, labels)
         assert torch.equal(loss.detach(), want.detach()) and torch.equal(dx, torch.autograd.grad(want, x)[0])
         torch.cuda.synchronize()
+
+
+# ---------------------------------------------------------------- labels that name no column, and batches of which nothing counts, by every way to list the rows
+ROWS = [1, 40, 64, 65, 70, 128, 129, 300, 1024, 1025, 1100]
+
+
+@pytest.mark.parametrize("M", ROWS)
+@pytest.mark.parametrize("label_dtype", [torch.int64, torch.int32])
+def test_labels_out_of_range_are_nan_in_their_row(hip_device, M, label_dtype):
+    x, w, labels = _inputs(M, 500, 128, M, hip_device, ignored=0.2 if M > 1 else 0.0, label_dtype=label_dtype)
+    names_none = [500, -1, torch.iinfo(label_dtype).max, torch.iinfo(label_dtype).min, -101]
+    bad = torch.zeros(M, dtype=torch.bool, device=hip_device)
+    for k, name in enumerate(names_none[:M]):
+        labels[k * 13 % M], bad[k * 13 % M] = name, True
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    with torch.no_grad():
+        assert torch.equal(torch.isnan(linear_cross_entropy(x, w, labels, reduction="none")), bad)
+        assert all(bool(torch.isnan(linear_cross_entropy(x, w, labels, reduction=r))) for r in ("mean", "sum"))
+    for leaves in ((x,), (w,), (x, w)):
+        xl, wl = (t if any(t is l for l in leaves) else t.detach() for t in (x, w))
+        loss = linear_cross_entropy(xl, wl, labels, reduction="none")
+        assert torch.equal(torch.isnan(loss), bad)
+        grads = torch.autograd.grad(loss, leaves, torch.ones(M, device=hip_device))
+        if leaves[0] is x:
+            assert torch.equal(torch.isnan(grads[0]).all(1), bad) and torch.equal(torch.isfinite(grads[0]).all(1), ~bad)
+        if leaves[-1] is w:
+            assert bool(torch.isnan(grads[-1]).all())
+
+
+@pytest.mark.parametrize("M", ROWS)
+def test_nothing_counts_in_any_batch(hip_device, M):
+    x, w, labels = _inputs(M, 500, 128, M, hip_device)
+    labels.fill_(-100)
+    x[:] = float("nan")                                       # (nothing of rows that do not count is read)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+    for reduction in ("none", "sum", "mean"):
+        def right(loss):
+            return bool(torch.isnan(loss)) if reduction == "mean" else bool((loss == 0).all())
+
+        with torch.no_grad():
+            assert right(linear_cross_entropy(x, w, labels, reduction=reduction))
+        for leaves in ((x,), (w,), (x, w)):
+            xl, wl = (t if any(t is l for l in leaves) else t.detach() for t in (x, w))
+            loss = linear_cross_entropy(xl, wl, labels, reduction=reduction)
+            assert right(loss.detach())
+            assert all(bool((g == 0).all()) for g in torch.autograd.grad(loss.sum(), leaves))

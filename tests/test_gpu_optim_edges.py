@@ -9,7 +9,7 @@ from tests.test_gpu_fsdp2 import one_rank_group  # noqa: F401
 from tests.test_gpu_optim import SIZES, U, _problem
 from tests.util_cases import make_dense_module
 from xorl_amd import _C
-from xorl_amd.optim import AdamW, adamw_step, grad_norm
+from xorl_amd.optim import AdamW, adamw_state_values, adamw_step, grad_norm
 
 pytestmark = pytest.mark.gpu
 
@@ -146,3 +146,29 @@ def test_a_rate_or_norm_that_the_step_writes_is_refused(hip_device, bits):
     prob[1][0] = both.view(1)
     _step(prob, lr=both, max_norm=1.0, grad_norm=both)
     assert float(both) == torch.tensor(1e-3).item()
+
+
+# ---------------------------------------------------------------- more elements than 32 bits count
+def test_tensors_beyond_32_bits(hip_device):
+    """Gradients that are zero but behind element 2^32: norm, parameters, codes and scales there are those of the end alone, and nothing else moved"""
+    n, tail = (1 << 32) + 4661, 4661 + 512
+    end = torch.randn(tail, device=hip_device).to(torch.bfloat16)
+
+    def made(count):
+        g = torch.zeros(count, dtype=torch.bfloat16, device=hip_device)
+        g[count - tail:] = end
+        return [[torch.zeros_like(g)], [g], [torch.zeros(count, dtype=torch.int8, device=hip_device)], [torch.zeros(count, dtype=torch.uint8, device=hip_device)],
+                [torch.zeros((), device=hip_device)], *([torch.zeros(-(-count // 256), device=hip_device)] for _ in range(2))]
+
+    big, small = made(n), made(tail)                         # (the end begins at a multiple of 256)
+    norm, want = _step(big, lr=1e-2, max_norm=0.5), _step(small, lr=1e-2, max_norm=0.5)
+    assert abs(float(norm) - float(end.double().norm())) <= 2 * U * float(norm) and abs(float(norm) - float(want)) <= 2 * U * float(norm)
+    assert abs(float(grad_norm(big[1])) - float(norm)) == 0.0
+    for a, b in zip(big, small):
+        a, b = a[0].view(-1), b[0].view(-1)
+        k = min(b.numel(), a.numel())
+        assert torch.equal(a[a.numel() - k:], b)
+        assert not bool(a[:a.numel() - k].any())
+    m, v = adamw_state_values(big[2][0], big[3][0], big[5][0], big[6][0], torch.bfloat16)
+    mw, vw = adamw_state_values(small[2][0], small[3][0], small[5][0], small[6][0], torch.bfloat16)
+    assert torch.equal(m[n - tail:], mw) and torch.equal(v[n - tail:], vw) and not bool(m[:n - tail].any()) and not bool(v[:n - tail].any())
