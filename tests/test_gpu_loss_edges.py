@@ -218,3 +218,37 @@ def test_nothing_counts_in_any_batch(hip_device, M):
             loss = linear_cross_entropy(xl, wl, labels, reduction=reduction)
             assert right(loss.detach())
             assert all(bool((g == 0).all()) for g in torch.autograd.grad(loss.sum(), leaves))
+
+
+# ---------------------------------------------------------------- tensors that another takes the place of between forward and backward
+@pytest.mark.parametrize("head", [lambda w: w, _Head])
+def test_tensors_exchanged_before_the_backward_are_refused(hip_device, head):
+    """`.data` and the storage change without a word to autograd; what the forward kept is as long as what it saw"""
+    x, w, labels = _inputs(300, 700, 128, 76, hip_device)
+    wl = head(w.clone()).requires_grad_(True)
+    for which, data in ((0, x[:260]), (0, x.repeat(2, 1)), (0, x[:, :64]), (1, w[:600]), (1, w[:, :64].contiguous())):
+        xl = x.clone().requires_grad_(True)
+        loss = linear_cross_entropy(xl, wl, labels)
+        keep = (xl, wl)[which].data
+        (xl, wl)[which].data = data
+        with pytest.raises(RuntimeError, match="resized between"):
+            torch.autograd.grad(loss, (xl, wl))
+        (xl, wl)[which].data = keep
+    xl = x.clone().requires_grad_(True)
+    loss = linear_cross_entropy(xl, w, labels)
+    xl.untyped_storage().resize_(0)
+    with pytest.raises((RuntimeError, ValueError)):
+        torch.autograd.grad(loss, xl)
+
+
+def test_the_backward_op_checks_what_was_kept(hip_device):
+    x, w, labels = _inputs(300, 700, 128, 77, hip_device)
+    loss, saved = torch.ops.xq.lce_fwd(x, w, labels, -100, 1, 1.0, 1)
+    up = torch.ones((), device=hip_device)
+    args = (x, w, labels)
+    for grad, kept, keep in ((up, saved, 2), (up, saved[:-256], 1), (up.expand(300), saved, 1)):
+        with pytest.raises(ValueError, match="not that of this problem"):
+            torch.ops.xq.lce_bwd(grad, *args, kept, -100, 1, 1.0, keep, keep == 2, True)
+    dw = torch.ops.xq.lce_bwd(up, *args, saved, -100, 1, 1.0, 1, False, True)[1]
+    w.requires_grad_(True)
+    assert torch.equal(dw, torch.autograd.grad(linear_cross_entropy(x, w, labels), w)[0])

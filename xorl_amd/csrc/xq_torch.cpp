@@ -479,6 +479,14 @@ struct HeadLoss {
     static Tensor aligned(const Tensor& t) { return t.is_contiguous() && (uintptr_t)t.data_ptr() % 16 != 0 ? t.clone() : t; }
 };
 
+// whether a tensor's elements lie in its storage
+bool in_storage(const Tensor& t) {
+    if (t.numel() == 0) return true;
+    int64_t last = t.storage_offset();
+    for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+    return (last + 1) * (int64_t)t.element_size() <= (int64_t)t.storage().nbytes();
+}
+
 // whether a stream of torch's is part of this capture (the default stream, which has id 0, never is, and may not be asked while one goes on)
 bool in_capture(const c10::Stream& s, unsigned long long id) {
     if (s.id() == 0) return false;
@@ -493,6 +501,7 @@ struct LinearCrossEntropyBackward : public Node {
     int64_t ignore = 0;
     int reduction = 0, keep = 0;
     double scale = 1;
+    int64_t M = 0, V = 0, H = 0;            // of the forward: what was saved is as long as that
 
     std::string name() const override { return "LinearCrossEntropyBackward"; }
     void release_variables() override {
@@ -526,6 +535,9 @@ struct LinearCrossEntropyBackward : public Node {
         {
             at::NoGradGuard no_grad;
             const Tensor g = cast_to(grads[0], at::kFloat).contiguous();
+            // (`.data` and the storage can be exchanged without a word to autograd)
+            if (!in_storage(x) || !in_storage(w) || x.dim() < 1 || w.dim() != 2 || x.size(-1) != H || w.size(1) != H || w.size(0) != V || x.numel() != M * H)
+                throw std::runtime_error("linear_cross_entropy: x or weight was freed or resized between forward and backward");
             const HeadLoss h(x, w, labels, ignore, reduction, scale);
             const bool need_dx = task_should_compute_output(0), need_dw = task_should_compute_output(1);
             if (need_dx) out[0] = empty_bf(x.sizes());
@@ -946,6 +958,7 @@ PyObject* cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
         node->reduction = (int)reduction;
         node->keep = keep;
         node->scale = scale;
+        node->M = x->numel() / x->size(-1); node->V = w->size(0); node->H = w->size(1);
         torch::autograd::set_history(loss, node);
         return THPVariable_Wrap(std::move(loss));
     });

@@ -53,6 +53,8 @@ def _bwd_impl(grad: Tensor, x: Tensor, weight: Tensor, labels: Tensor, saved: Te
         q = _problem(x2, w2, l1, ignore_index, reduction, logit_scale)
         L = _C.lib()
         g = grad.to(torch.float32).contiguous()
+        if x2.shape[1] != w2.shape[1] or saved.numel() != L.xq_lce_saved_bytes(q.M, q.V, q.H, keep) or g.numel() != (q.M if reduction == 0 else 1):
+            raise _C.XqError("linear_cross_entropy: what the forward kept, or the gradient, is not that of this problem")
         dx = torch.empty(x.shape if need_dx else (0,), dtype=torch.bfloat16, device=dev)
         dw = torch.empty(weight.shape if need_dw else (0,), dtype=torch.bfloat16, device=dev)
         ws_bytes = L.xq_lce_workspace_bytes(q.M, q.V, q.H, _C.XQ_LCE_KEEP_HEAD_BWD) if need_dw else 0
@@ -97,6 +99,7 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
         loss, saved = fwd(x, weight, labels, ignore_index, reduction, logit_scale, keep)
         ctx.save_for_backward(x, weight, labels, saved)
         ctx.args = (ignore_index, reduction, logit_scale, keep)
+        ctx.shapes = (x.shape, weight.shape)
         return loss
 
     @staticmethod
@@ -106,6 +109,8 @@ class LinearCrossEntropyFunction(torch.autograd.Function):
             # (torch may hand the gradients to another stream, which ends the process under capture; the native node looks at whose)
             raise RuntimeError("linear_cross_entropy: a captured backward takes plain tensors, no subclasses of them")
         x, weight, labels, saved = ctx.saved_tensors
+        if (x.shape, weight.shape) != ctx.shapes:
+            raise RuntimeError("linear_cross_entropy: x or weight was resized between forward and backward")
         need_dx, need_dw = ctx.needs_input_grad[0], ctx.needs_input_grad[1]
         bwd = _bwd_op if torch.compiler.is_compiling() else _bwd_impl
         dx, dw = bwd(grad, x, weight, labels, saved, *ctx.args, need_dx, need_dw)
