@@ -252,3 +252,34 @@ def test_the_backward_op_checks_what_was_kept(hip_device):
     dw = torch.ops.xq.lce_bwd(up, *args, saved, -100, 1, 1.0, 1, False, True)[1]
     w.requires_grad_(True)
     assert torch.equal(dw, torch.autograd.grad(linear_cross_entropy(x, w, labels), w)[0])
+
+
+# ---------------------------------------------------------------- infinite logits
+@pytest.mark.parametrize("M", [5, 100, 300, 1100])
+@pytest.mark.parametrize("value", [float("inf"), -float("inf"), 3e38])
+@pytest.mark.parametrize("column", ["label", "another", "last"])
+def test_infinite_logits(hip_device, M, value, column):
+    """A head row that has run away, under tokens that have a 0 there but for some: NaN where the definition has infinity less infinity or 0 times
+    infinity, an infinite loss where the label's logit is minus infinity"""
+    V = 600
+    x, w, labels = _inputs(M, V, 128, M, hip_device, lift=0.0)
+    labels.random_(0, V - 1, generator=torch.Generator(device=hip_device).manual_seed(M))
+    hit = torch.arange(M, device=hip_device) % 3 == 1
+    labels[hit], labels[~hit] = 17, labels[~hit] % 16
+    x[:, 5] = torch.where(hit, 2.0, 0.0).to(BF)
+    w[:, 5] = 0.0
+    w[{"label": 17, "another": 400, "last": V - 1}[column], 5] = value
+    l = x.double() @ w.double().t()
+    # (in fp32 a product beyond its range is infinite)
+    l = torch.where(l.abs() > 3.4028235e38, l.sign() * float("inf"), l)
+    want = torch.nn.functional.cross_entropy(l, labels, reduction="none")
+    x.requires_grad_(True)
+    with torch.no_grad():
+        score = linear_cross_entropy(x, w, labels, reduction="none")
+    loss = linear_cross_entropy(x, w, labels, reduction="none")
+    for got in (score, loss.detach()):
+        assert torch.equal(torch.isnan(got), torch.isnan(want)) and torch.equal(torch.isposinf(got), torch.isposinf(want))
+        fine = torch.isfinite(want)
+        assert bool(((got.double() - want)[fine].abs() <= 1e-4 * want[fine].abs()).all())
+    dx, = torch.autograd.grad(loss.sum(), x)
+    assert bool(torch.isnan(dx[torch.isnan(want)]).all(1).all())

@@ -227,14 +227,15 @@ struct RowEnd {
     float* out;                         // losses by row of x, or NULL
 };
 __device__ __forceinline__ float end_row(const RowEnd& e, int64_t c, int row, float z, float ref, float t) {
-    const float et = __builtin_amdgcn_exp2f(t - ref), sum = z + et;
-    const float loss = ref == t ? log1pf(z) : logf(sum) + (ref - t) * kLn2;
+    // (ref - t is 0 where the label's own logit is the reference, and NaN where that is infinite)
+    const float apart = ref - t, et = __builtin_amdgcn_exp2f(-apart), sum = z + et;
+    const float loss = apart == 0.0f ? log1pf(z) : logf(sum) + apart * kLn2;
     e.loss[c] = loss;
     if (e.out) e.out[row] = loss;
     const float inv = 1.0f / sum;
     e.inv[c] = inv;
     e.rest[c] = z / sum;
-    e.lse2[c] = ref == t ? log1pf(z) * kLog2e + t : log2f(sum) + ref;
+    e.lse2[c] = apart == 0.0f ? log1pf(z) * kLog2e + t : log2f(sum) + ref;
     return inv;
 }
 
