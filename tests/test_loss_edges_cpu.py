@@ -1,10 +1,10 @@
-"""Host side of linear_cross_entropy: tangents of forward-mode differentiation."""
+"""Host side of linear_cross_entropy: what would be left out without a word is refused."""
 
 import pytest
 import torch
 import torch.autograd.forward_ad as fwAD
 
-from xorl_amd import loss_functional
+from xorl_amd import _C, loss_functional
 from xorl_amd.loss_functional import linear_cross_entropy
 
 BF = torch.bfloat16
@@ -31,3 +31,14 @@ def test_tangents_are_refused(monkeypatch, which, head_grad):
             linear_cross_entropy(t["x"], t["weight"], labels)
     with fwAD.dual_level():                               # (a level without tangents refuses nothing)
         assert linear_cross_entropy(torch.zeros(3, 64, dtype=BF), torch.zeros(10, 64, dtype=BF), labels).shape == ()
+
+
+def test_a_trained_scale_is_refused():
+    """It is a number here: the gradient that a tensor waits for would never come"""
+    scale = torch.tensor(2.0, requires_grad=True)
+    x, w, labels = torch.zeros(3, 64, dtype=BF), torch.zeros(10, 64, dtype=BF), torch.zeros(3, dtype=torch.int64)
+    with pytest.raises(_C.XqError, match="logit_scale gets no gradient"):
+        linear_cross_entropy(x, w, labels, logit_scale=scale)
+    for call in (torch.no_grad(), torch.enable_grad()):
+        with call, pytest.raises(RuntimeError, match="HIP device only"):
+            linear_cross_entropy(x, w, labels, logit_scale=scale.detach())

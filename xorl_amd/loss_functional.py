@@ -129,6 +129,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
     1 - p times the row's upstream gradient are, unless at most 128 rows count (then 2^-16).  H must be a multiple of 64.  First derivatives
     only.  Under graph capture forward and backward go into the same graph, and no loss made outside it from the same x or weight may
     still be alive (refused; in a compiled call torch ends the process).  Rows of x and weight at multiples of 16 bytes are read in place; other layouts are copied, in both passes."""
+    if isinstance(logit_scale, Tensor) and logit_scale.requires_grad and torch.is_grad_enabled():
+        raise _C.XqError("linear_cross_entropy: logit_scale gets no gradient; scale x by one that is trained, or detach it")
     if not torch.compiler.is_compiling() and reduction in _C.LCE_REDUCTIONS:
         loss = native().cross_entropy(x, weight, labels, ignore_index, _C.LCE_REDUCTIONS[reduction], logit_scale)
         if loss is not None:
