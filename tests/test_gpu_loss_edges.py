@@ -1,11 +1,12 @@
 """GPU: linear_cross_entropy where the plain bounds of its other tests let a mistake through, and the calls at the edge of what it takes.
 
-U = 2^-24, half a step of fp32; B = 2^-8, half a step of bf16; `_reference` has the bounds of loss and gradients that are derived there."""
+U = 2^-24, half a step of fp32; B = 2^-8, half a step of bf16."""
 
 import pytest
 import torch
 
-from tests.test_gpu_loss import B, BF, U, _inputs, _reference, _within
+from tests.test_gpu_loss import B, BF, U, _inputs, _within
+from xorl_amd import _C
 from xorl_amd.loss_functional import linear_cross_entropy
 
 pytestmark = pytest.mark.gpu
@@ -283,3 +284,16 @@ def test_infinite_logits(hip_device, M, value, column):
         assert bool(((got.double() - want)[fine].abs() <= 1e-4 * want[fine].abs()).all())
     dx, = torch.autograd.grad(loss.sum(), x)
     assert bool(torch.isnan(dx[torch.isnan(want)]).all(1).all())
+
+
+def test_tensors_exchanged_by_a_number_are_looked_at_afterwards(hip_device):
+    x, w, labels = _inputs(300, 700, 128, 78, hip_device)
+    short = x[:, :64].clone()
+
+    class Number:
+        def __float__(self):
+            x.data = short
+            return 1.0
+
+    with pytest.raises(_C.XqError, match="do not go together"):
+        linear_cross_entropy(x, w, labels, logit_scale=Number())

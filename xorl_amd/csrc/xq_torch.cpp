@@ -925,13 +925,14 @@ PyObject* moe(PyObject*, PyObject* const* args, Py_ssize_t n) {
 PyObject* cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
     return guarded([&]() -> PyObject* {
         if (n != 6) { PyErr_SetString(PyExc_TypeError, "cross_entropy(x, weight, labels, ignore_index, reduction, logit_scale)"); return nullptr; }
-        const Tensor *x = plain(args[0]), *w = plain(args[1]), *labels = plain(args[2]);
-        if (under_transform() || !x || !w || !labels || !HeadLoss::takes(*x, *w, *labels)) XQ_NONE;
+        // (numbers first: their conversion may run Python, and with it change the tensors)
         const int64_t ignore = PyLong_AsLongLong(args[3]);
         if (ignore == -1 && PyErr_Occurred()) { PyErr_Clear(); XQ_NONE; }
         const long reduction = PyLong_AsLong(args[4]);
         const double scale = PyFloat_AsDouble(args[5]);
         if (PyErr_Occurred()) { PyErr_Clear(); XQ_NONE; }
+        const Tensor *x = plain(args[0]), *w = plain(args[1]), *labels = plain(args[2]);
+        if (under_transform() || !x || !w || !labels || !HeadLoss::takes(*x, *w, *labels)) XQ_NONE;
         if (!(scale > 0.0) || !std::isfinite(scale)) XQ_NONE;
         const bool grad = at::GradMode::is_enabled(), want_x = grad && x->requires_grad(), want_w = grad && w->requires_grad();
         const int keep = want_x ? XQ_LCE_KEEP_DX : want_w ? XQ_LCE_KEEP_HEAD : XQ_LCE_KEEP_NONE;
