@@ -113,3 +113,23 @@ def _two_ranks(rank, path):
 
 def test_sharded_parameters(tmp_path):
     torch.multiprocessing.spawn(_two_ranks, args=(str(tmp_path / "store"),), nprocs=2)
+
+
+def test_hooks_of_a_load_are_followed():
+    """what a pre-hook puts in the place of the dictionary is loaded, what a post-hook changes stays"""
+    p, q = torch.nn.Parameter(torch.ones(8)), torch.nn.Parameter(torch.ones(8))
+    opt = AdamW([p])
+    d = _adam(0.0)
+    other = {"state": {0: {**d["state"][0], "exp_avg": torch.full((8,), 5.0), "step": 9}}, "param_groups": d["param_groups"]}
+    a = opt.register_load_state_dict_pre_hook(lambda o, s: other)
+    b = opt.register_load_state_dict_post_hook(lambda o: o.state[p].update(exp_avg_sq=torch.full((8,), 6.0)))
+    opt.load_state_dict(d)
+    s = opt.state[p]
+    assert float(s["step"]) == 9.0 and bool((s["exp_avg"] == 5).all()) and bool((s["exp_avg_sq"] == 6).all())
+    a.remove()
+    b.remove()
+    opt.load_state_dict(d)
+    assert float(opt.state[p]["step"]) == 1.0 and torch.equal(opt.state[p]["exp_avg"], d["state"][0]["exp_avg"])
+    assert not opt._optimizer_load_state_dict_pre_hooks and not opt._optimizer_load_state_dict_post_hooks
+    with pytest.raises(ValueError):
+        AdamW([p, q]).load_state_dict(d)

@@ -164,22 +164,35 @@ class AdamW(torch.optim.Optimizer):
 
     def load_state_dict(self, state_dict) -> None:
         """States of this class or of ``torch.optim.AdamW`` (a group of the latter goes on with 32 bits; its variants are refused)."""
-        for g in state_dict["param_groups"]:
-            if g.get("amsgrad") or g.get("maximize"):
-                raise _C.XqError("AdamW: amsgrad and maximize have no counterpart here")
-            if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
-                raise _C.XqError("AdamW: a weight decay that is added to the gradients has no counterpart here")
-        # the base class casts floating-point state, and codes with it, to the parameter's type
-        super().load_state_dict(state_dict)
-        for g in self.param_groups:
-            g.setdefault("state_bits", 32)
-            if "decoupled_weight_decay" in g:           # (without a decay it may have come as False)
-                g["decoupled_weight_decay"] = True
-        saved = [i for g in state_dict["param_groups"] for i in g["params"]]
-        own = [p for g in self.param_groups for p in g["params"]]
-        for i, p in zip(saved, own):
-            if i in state_dict["state"]:
-                self.state[p] = {k: _state(v, _local(p).device) for k, v in state_dict["state"][i].items()}
+        # around what the base class loads, so that hooks of the user's see, and may change, what is loaded and what has been
+        taken: dict = {}
+
+        def check(_, d):
+            for g in d["param_groups"]:
+                if g.get("amsgrad") or g.get("maximize"):
+                    raise _C.XqError("AdamW: amsgrad and maximize have no counterpart here")
+                if g.get("weight_decay") and not g.get("decoupled_weight_decay", True):
+                    raise _C.XqError("AdamW: a weight decay that is added to the gradients has no counterpart here")
+            taken.update(d)
+
+        def finish(_):
+            for g in self.param_groups:
+                g.setdefault("state_bits", 32)
+                if "decoupled_weight_decay" in g:           # (without a decay it may have come as False)
+                    g["decoupled_weight_decay"] = True
+            # (the base class has cast floating-point state, and codes with it, to the parameter's type)
+            saved = [i for g in taken["param_groups"] for i in g["params"]]
+            own = [p for g in self.param_groups for p in g["params"]]
+            for i, p in zip(saved, own):
+                if i in taken["state"]:
+                    self.state[p] = {k: _state(v, _local(p).device) for k, v in taken["state"][i].items()}
+
+        hooks = (self.register_load_state_dict_pre_hook(check), self.register_load_state_dict_post_hook(finish, prepend=True))
+        try:
+            super().load_state_dict(state_dict)
+        finally:
+            for h in hooks:
+                h.remove()
 
 
 def _state(v, device):
