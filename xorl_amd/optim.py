@@ -140,21 +140,21 @@ class AdamW(torch.optim.Optimizer):
                 raise _C.XqError("AdamW: 8-bit states of a parameter that is sharded over ranks could not be resharded; take 32 bits")
             if _layout(p) != _layout(p.grad):
                 raise _C.XqError(f"AdamW: a gradient is distributed otherwise than its parameter: {_layout(p.grad)}, {_layout(p)}")
-        local = _local if distributed else lambda t: t
+        local = (lambda ts: [_local(t) for t in ts]) if distributed else (lambda ts: ts)
         norm = None
         if self.max_grad_norm is not None and groups:
             if any(_sharded(p) for _, p in distributed):
                 raise _C.XqError("max_grad_norm over sharded parameters: clip them with a norm over all ranks, and leave it out here")
             if len(groups) > 1:
-                norm = grad_norm([local(p.grad) for _, ps in groups for p in ps])
+                norm = grad_norm(local([p.grad for _, ps in groups for p in ps]))
         for g, ps in groups:
             states = [self._init_state(p, g["state_bits"]) for p in ps]
 
             def of(name):
-                return [local(s[name]) for s in states]
+                return local([s[name] for s in states])
 
             eight = g["state_bits"] == 8
-            out = adamw_step([local(p) for p in ps], [local(p.grad) for p in ps], of("exp_avg"), of("exp_avg_sq"), of("step"),
+            out = adamw_step(local(ps), local([p.grad for p in ps]), of("exp_avg"), of("exp_avg_sq"), of("step"),
                              exp_avg_scales=of("exp_avg_scale") if eight else None, exp_avg_sq_scales=of("exp_avg_sq_scale") if eight else None,
                              lr=g["lr"], betas=g["betas"], eps=g["eps"], weight_decay=g["weight_decay"], max_norm=self.max_grad_norm,
                              grad_norm=norm)
