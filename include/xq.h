@@ -679,7 +679,7 @@ int xq_mlp_fwd_infer(const xq_weight* gate, const xq_weight* up, const xq_weight
  * head's.  saved: xq_lce_saved_bytes(M, V, H, keep) bytes, 256-byte aligned, needed in every case; the backward reads it and leaves it.
  * workspace: xq_lce_workspace_bytes(M, V, H, keep), for a backward with dw XQ_LCE_KEEP_HEAD_BWD in place of keep; without dw none.
  * xq_lce_bwd: grad fp32[M] or [1] by the reduction, of the loss; dx [M, H] and dw [V, H] bf16, NULL where not wanted; problem, and
- * what it points at, as in the forward.  M < 2^24, V < 2^28, H % 64 == 0; rows of x, w, dx, dw at multiples
+ * what it points at, as in the forward, and keep too: saved is device memory, the host does not look whose it is.  M < 2^24, V < 2^28, H % 64 == 0; rows of x, w, dx, dw at multiples
  * of 16 bytes.  The sizes are -1 for what is out of range. */
 #define XQ_LCE_NONE 0
 #define XQ_LCE_MEAN 1

@@ -125,7 +125,8 @@ def linear_cross_entropy(x: Tensor, weight: Tensor, labels: Tensor, *, ignore_in
     [0, V) gives its row NaN, in the loss and in the gradients, the weight's with it.
 
     Products accumulate in fp32, sums of exponentials in fp32 relative to the label's logit or the largest.  Gradients come in bf16. For x, the
-    probabilities in them are rounded to bf16 once (half a step, 2^-8, each), all but the label's; for the weight, probabilities and the label's
+    probabilities in them are rounded to bf16 once (half a step, 2^-8, each, of the difference between the column's row of the weight and the
+    label's: what all rows have in common cancels), all but the label's; for the weight, probabilities and the label's
     1 - p times the row's upstream gradient are, unless at most 128 rows count (then 2^-16).  H must be a multiple of 64.  First derivatives
     only.  Under graph capture forward and backward go into the same graph, and no loss made outside it from the same x or weight may
     still be alive (refused; in a compiled call torch ends the process).  Rows of x and weight at multiples of 16 bytes are read in place; other layouts are copied, in both passes."""
