@@ -297,3 +297,46 @@ def test_tensors_exchanged_by_a_number_are_looked_at_afterwards(hip_device):
 
     with pytest.raises(_C.XqError, match="do not go together"):
         linear_cross_entropy(x, w, labels, logit_scale=Number())
+
+
+# ---------------------------------------------------------------- what autograd offers around a node
+def test_saved_tensor_hooks(hip_device):
+    """Checkpointing and saving on the CPU give the same gradients; a hook that gives back something shorter is refused"""
+    from torch.utils.checkpoint import checkpoint
+
+    x, w, labels = _inputs(300, 700, 128, 79, hip_device, ignored=0.2)
+    x.requires_grad_(True)
+    w.requires_grad_(True)
+
+    def f(x, w):
+        return linear_cross_entropy(x * 2.0, w, labels)
+
+    loss = f(x, w)
+    want = torch.autograd.grad(loss, (x, w))
+    again = checkpoint(f, x, w, use_reentrant=False)
+    assert torch.equal(again, loss) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, (x, w)), want))
+    with torch.autograd.graph.save_on_cpu():
+        again = f(x, w)
+    assert torch.equal(again, loss) and all(torch.equal(a, b) for a, b in zip(torch.autograd.grad(again, (x, w)), want))
+    for shorten in (lambda t: t[:-256], lambda t: t.cpu()):
+        with torch.autograd.graph.saved_tensors_hooks(lambda t: t, lambda t: shorten(t) if t.dtype == torch.uint8 else t):
+            again = f(x, w)
+        with pytest.raises(RuntimeError, match="hooks of saved tensors"):
+            torch.autograd.grad(again, (x, w))
+
+
+def test_batched_upstream_gradients_are_refused(hip_device):
+    x, w, labels = _inputs(40, 300, 64, 80, hip_device)
+    x.requires_grad_(True)
+    for reduction, shape in (("sum", (2,)), ("none", (2, 40))):
+        loss = linear_cross_entropy(x, w, labels, reduction=reduction)
+        with pytest.raises(RuntimeError):
+            torch.autograd.grad(loss, x, torch.ones(shape, device=hip_device), is_grads_batched=True)
+
+
+def test_fake_tensors_are_refused(hip_device):
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    x, w, labels = _inputs(40, 300, 64, 81, hip_device)
+    with FakeTensorMode() as mode, pytest.raises(Exception):
+        linear_cross_entropy(*(mode.from_tensor(t) for t in (x, w, labels)))

@@ -501,7 +501,7 @@ struct LinearCrossEntropyBackward : public Node {
     int64_t ignore = 0;
     int reduction = 0, keep = 0;
     double scale = 1;
-    int64_t M = 0, V = 0, H = 0;            // of the forward: what was saved is as long as that
+    int64_t M = 0, V = 0, H = 0, saved_bytes = 0;            // of the forward: what was saved is as long as that
 
     std::string name() const override { return "LinearCrossEntropyBackward"; }
     void release_variables() override {
@@ -538,6 +538,8 @@ struct LinearCrossEntropyBackward : public Node {
             // (`.data` and the storage can be exchanged without a word to autograd)
             if (!in_storage(x) || !in_storage(w) || x.dim() < 1 || w.dim() != 2 || x.size(-1) != H || w.size(1) != H || w.size(0) != V || x.numel() != M * H)
                 throw std::runtime_error("linear_cross_entropy: x or weight was freed or resized between forward and backward");
+            if (!saved.is_cuda() || nbytes(saved) != saved_bytes || !saved.is_contiguous() || !in_storage(saved))
+                throw std::runtime_error("linear_cross_entropy: hooks of saved tensors gave back something else than was saved");
             const HeadLoss h(x, w, labels, ignore, reduction, scale);
             const bool need_dx = task_should_compute_output(0), need_dw = task_should_compute_output(1);
             if (need_dx) out[0] = empty_bf(x.sizes());
@@ -959,7 +961,7 @@ PyObject* cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
         node->reduction = (int)reduction;
         node->keep = keep;
         node->scale = scale;
-        node->M = x->numel() / x->size(-1); node->V = w->size(0); node->H = w->size(1);
+        node->saved_bytes = nbytes(saved); node->M = x->numel() / x->size(-1); node->V = w->size(0); node->H = w->size(1);
         torch::autograd::set_history(loss, node);
         return THPVariable_Wrap(std::move(loss));
     });
