@@ -12,7 +12,7 @@
 //    K-step ahead (two register sets).  Every iteration is the same: behind a tile's last K-step the logits kernel loads the next tile's, the product
 //    the last one again (a branch around the loads cost both 5 %).
 //  * What bounds it.  Many rows: the matrix units, two thirds (logits) to three quarters (product) busy, and the power they draw: 1.36 PFLOP/s of
-//    STATS at 8192 rows under [131072, 4096], 1.28 of EXP (its 1 GiB pieces of E are 5 % of it, the sum of what they hold 1.5 %, the other ends 3 %, reading 64-byte pieces of
+//    STATS at 8192 rows under [131072, 4096], 1.25 of EXP (its 1 GiB pieces of E are 5 % of it, the sum of what they hold 1.5 %, the other ends 3 %, reading 64-byte pieces of
 //    rows and not whole lines 5 %), 1.36 of E . W; a library product of the same operands 1.41.  Up to 128 rows: reading the head, 1 GiB of it in 180 us
 //    (6.0 TB/s) under one row, 174 us for E . W.
 //  * Stage.  A: [row][32 k], the 16-byte chunk c of a row at c ^ ((row >> 2) & 2): 16 rows x 4 chunks meet no bank twice.  B of

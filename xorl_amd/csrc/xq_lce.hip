@@ -22,9 +22,9 @@
 //    contraction, and multiplies it with the rows that count.  What all rows share of g (the mean's 1 / count, the logit scale) is left to the
 //    result in 32 bits: in G it would be one and the same rounding error, up to half a step, of the whole gradient.
 //
-// 8192 rows, 5735 of which count, under [131072, 4096], forward and backward: 10.2 ms, in two pieces of 2.55 (logits) and 2.4 ms (product) each, 0.1 ms of
+// 8192 rows, 5735 of which count, under [131072, 4096], forward and backward: 10.3 ms, in two pieces of 2.6 (logits) and 2.45 ms (product) each, 0.1 ms of
 // everything else.  One row, scored: 188 us (192 with a launch of its own that lists the rows, as above 64 rows).  96 rows under [32003, 2048], forward and
-// backward: 82 us, of which 30 and 27 are the products and the rest four small launches.
+// backward: 82 us, of which 32 and 27 are the products and the rest four small launches.
 #include <algorithm>
 #include <atomic>
 
