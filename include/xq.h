@@ -750,6 +750,87 @@ int xq_grad_norm(const xq_adamw_tensor* tensors, int64_t n, float* norm, void* w
 int xq_adamw_values(const void* exp_avg, const void* exp_avg_sq, const float* exp_avg_scale, const float* exp_avg_sq_scale,
                     int64_t numel, void* exp_avg_out, void* exp_avg_sq_out, int out_dtype, void* stream);
 
+/* ---- routing to experts --------------------------------------------------- */
+/* Which experts a token goes to and with what weights: what stands in front of the grouped entry points above (the reference:
+ * models/layers/moe, the routers of its MoE block).
+ *   s = softmax(z) or sigmoid(z) of the row's logits; experts are ordered by s + bias, computed in 64 bits, without a bias by z; equal ones by their index
+ *   num_groups > 1: only experts of the top_groups best groups of equal size; a group is as good as its best expert or the sum of its two best
+ *   weight = scale * s, or scale * s / (sum of s over the chosen) with renormalize
+ * An expert whose logit or bias is -inf is never chosen; places for which none is left get id -1 (which the grouped entry points drop) and weight 0.
+ * A row with a NaN among logits or biases, or under softmax with an infinite logit, gets NaN weights, ids 0 .. top_k - 1 and a NaN gradient.
+ * weights [n_tokens, top_k] fp32 and selected int64, in descending order.  Backward: weights and selected as the forward left them, grad the
+ * gradient of the weights; dlogits in the logits' type.  The bias gets none: the weights do not depend on it but through the choice.
+ * The backward reads logits under sigmoid and without renormalize; renormalized softmax weights are those of the chosen logits alone (NULL will do).
+ * At most 1024 experts, 64 groups, top_k 32, 2^26 - 1 tokens; scale 2^-60 to 2^60. */
+#define XQ_ROUTE_SOFTMAX 0
+#define XQ_ROUTE_SIGMOID 1
+#define XQ_ROUTE_GROUP_MAX 0
+#define XQ_ROUTE_GROUP_SUM2 1
+
+typedef struct xq_moe_route {
+    const void* logits;         /* [n_tokens, num_experts], ld elements from row to row */
+    int64_t ld;
+    const float* bias;          /* [num_experts] or NULL */
+    int64_t n_tokens;
+    int32_t dtype;              /* XQ_DT_* of the logits */
+    int32_t num_experts, top_k, scoring, num_groups, top_groups, group_score, renormalize;
+    float scale;
+    int32_t reserved;
+} xq_moe_route;
+
+int xq_moe_route_fwd(const xq_moe_route* problem, float* weights, int64_t* selected, void* stream);
+int xq_moe_route_bwd(const xq_moe_route* problem, const float* weights, const int64_t* selected, const float* grad, void* dlogits,
+                     int64_t ld_dlogits, void* stream);
+
+/* ---- adapters of many requests ---------------------------------------------- */
+/* out[i] = bf16(base[i] + scaling[a] (x[i] . A[a]^T) . B[a]^T), a = ids[i]: the low-rank updates of the requests of a batch beside one
+ * shared projection, base = what xq_linear_fwd leaves for r = 0.  No counterpart in the reference, which serves one adapter at a time.
+ * A row whose id lies outside [0, n_adapters) has no adapter: out = base.  Products accumulate in fp32, x . A^T is kept to 16 bits and more.
+ * x [M, K], base and out [M, N] bf16, rows at multiples of 16 bytes; out may be base.  A [n_adapters, r, K], B [n_adapters, N, r] dense, in
+ * factor_dtype; an adapter of a smaller rank is padded with zeros.  K % 64 == 0, N % 16 == 0, r 1 to 64, M < 2^24.
+ * workspace: xq_adapters_workspace_bytes(M, N, K, r) bytes, 256-byte aligned. */
+typedef struct xq_adapters {
+    const void* x;
+    int64_t ldx;
+    const void* base;
+    int64_t ld_base;
+    void* out;
+    int64_t ld_out;
+    const void* A;
+    const void* B;
+    const float* scaling;       /* [n_adapters] */
+    const void* ids;            /* int32 or int64 [M] */
+    int64_t M, N, K;
+    int32_t n_adapters, r;
+    int32_t factor_dtype;       /* XQ_DT_* */
+    int32_t id_bytes;           /* 4 or 8 */
+} xq_adapters;
+
+int64_t xq_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r);
+int xq_adapters_add(const xq_adapters* problem, void* workspace, int64_t workspace_bytes, void* stream);
+
+/* ---- embedding ---------------------------------------------------------------- */
+/* out[t] = scale * weight[ids[t]], rounded once; dw[v] = scale * sum of grad[t] over the tokens t with ids[t] = v: summed in fp32 in an order that
+ * the ids alone fix (no atomics: the same bits on every call) and rounded once.  dw is written whole, zeros where no token is.  An id
+ * outside [0, V) gives a row of NaN and no gradient; the gradient of row padding_idx is zero (-1: none).  (The reference: the embedding of
+ * its models, torch's.)  weight, out, grad and dw in one type; the backward reads no weight.
+ * workspace: xq_embedding_workspace_bytes(n_tokens, V, H) bytes, 256-byte aligned. */
+typedef struct xq_embedding {
+    const void* ids;            /* int32 or int64 [n_tokens] */
+    const void* weight;         /* [V, H], ldw elements from row to row */
+    int64_t ldw;
+    int64_t n_tokens, V, H, padding_idx;
+    float scale;
+    int32_t dtype;              /* XQ_DT_* */
+    int32_t id_bytes;           /* 4 or 8 */
+    int32_t reserved;
+} xq_embedding;
+
+int xq_embedding_fwd(const xq_embedding* problem, void* out, int64_t ld_out, void* stream);
+int64_t xq_embedding_workspace_bytes(int64_t n_tokens, int64_t V, int64_t H);
+int xq_embedding_bwd(const xq_embedding* problem, const void* grad, int64_t ld_grad, void* dw, int64_t ld_dw, void* workspace,
+                     int64_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -100,6 +100,27 @@ class XqAdamwOptions(ctypes.Structure):
         ("lr_device", ctypes.c_void_p), ("norm", ctypes.c_void_p), ("norm_given", ctypes.c_int32), ("state_bits", ctypes.c_int32)]
 
 
+class XqMoeRoute(ctypes.Structure):
+    _fields_ = [("logits", ctypes.c_void_p), ("ld", ctypes.c_int64), ("bias", ctypes.c_void_p), ("n_tokens", ctypes.c_int64)] + [
+        (n, ctypes.c_int32) for n in ("dtype", "num_experts", "top_k", "scoring", "num_groups", "top_groups", "group_score", "renormalize")] + [
+            ("scale", ctypes.c_float), ("reserved", ctypes.c_int32)]
+
+
+ROUTE_SCORINGS = {"softmax": 0, "sigmoid": 1}
+ROUTE_GROUP_SCORES = {"max": 0, "sum2": 1}
+
+
+class XqAdapters(ctypes.Structure):
+    _fields_ = [("x", ctypes.c_void_p), ("ldx", ctypes.c_int64), ("base", ctypes.c_void_p), ("ld_base", ctypes.c_int64), ("out", ctypes.c_void_p),
+                ("ld_out", ctypes.c_int64)] + [(n, ctypes.c_void_p) for n in ("A", "B", "scaling", "ids")] + [
+                    (n, ctypes.c_int64) for n in ("M", "N", "K")] + [(n, ctypes.c_int32) for n in ("n_adapters", "r", "factor_dtype", "id_bytes")]
+
+
+class XqEmbedding(ctypes.Structure):
+    _fields_ = [("ids", ctypes.c_void_p), ("weight", ctypes.c_void_p)] + [(n, ctypes.c_int64) for n in ("ldw", "n_tokens", "V", "H", "padding_idx")] + [
+        ("scale", ctypes.c_float), ("dtype", ctypes.c_int32), ("id_bytes", ctypes.c_int32), ("reserved", ctypes.c_int32)]
+
+
 class XqError(ValueError):
     """Argument error reported by the library before any launch."""
 
@@ -235,6 +256,18 @@ _SIGNATURES = {
     "xq_grad_norm": (_INT, [ctypes.POINTER(XqAdamwTensor), _I64, _P, _P, _I64, _P]),
     # exp_avg, exp_avg_sq, their scales, numel, exp_avg_out, exp_avg_sq_out, out_dtype, stream
     "xq_adamw_values": (_INT, [_P, _P, _P, _P, _I64, _P, _P, _INT, _P]),
+    # problem, weights, selected, stream
+    "xq_moe_route_fwd": (_INT, [ctypes.POINTER(XqMoeRoute), _P, _P, _P]),
+    # problem, weights, selected, grad, dlogits, ld_dlogits, stream
+    "xq_moe_route_bwd": (_INT, [ctypes.POINTER(XqMoeRoute), _P, _P, _P, _P, _I64, _P]),
+    "xq_adapters_workspace_bytes": (_I64, [_I64, _I64, _I64, _INT]),
+    # problem, ws, ws_bytes, stream
+    "xq_adapters_add": (_INT, [ctypes.POINTER(XqAdapters), _P, _I64, _P]),
+    # problem, out, ld_out, stream
+    "xq_embedding_fwd": (_INT, [ctypes.POINTER(XqEmbedding), _P, _I64, _P]),
+    "xq_embedding_workspace_bytes": (_I64, [_I64, _I64, _I64]),
+    # problem, grad, ld_grad, dw, ld_dw, ws, ws_bytes, stream
+    "xq_embedding_bwd": (_INT, [ctypes.POINTER(XqEmbedding), _P, _I64, _P, _I64, _P, _I64, _P]),
 }
 
 EXPORTS = ("xq_version", "xq_last_error") + tuple(_SIGNATURES)

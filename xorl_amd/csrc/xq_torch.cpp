@@ -18,6 +18,7 @@
 #include <ATen/core/Tensor.h>
 #include <ATen/EmptyTensor.h>
 #include <ATen/ops/_foreach_add.h>
+#include <ATen/ops/zeros_like.h>
 #include <ATen/hip/impl/HIPCachingAllocatorMasqueradingAsCUDA.h>
 #include <ATen/hip/impl/HIPStreamMasqueradingAsCUDA.h>
 #include <c10/core/DeviceGuard.h>
@@ -264,7 +265,10 @@ struct Rows {
     int64_t ld = 0, M = 0;
 
     static bool pitched(const Tensor& x, int64_t* pitch) {
-        if (x.stride(-1) != 1 || (uintptr_t)x.data_ptr() % 16 != 0) return false;
+        return (uintptr_t)x.data_ptr() % 16 == 0 && any_pitch(x, pitch) && (x.numel() == x.size(-1) || *pitch % 8 == 0);
+    }
+    static bool any_pitch(const Tensor& x, int64_t* pitch) {
+        if (x.stride(-1) != 1) return false;
         int64_t rows = 1;                                          // of the dimensions looked at, the innermost first
         for (int64_t d = x.dim() - 2; d >= 0; --d) {
             if (x.size(d) == 1) continue;
@@ -272,7 +276,7 @@ struct Rows {
             else if (x.stride(d) != *pitch * rows) return false;
             rows *= x.size(d);
         }
-        return rows == 1 || *pitch % 8 == 0;
+        return true;
     }
 
     Rows(const Tensor& x, int64_t width) {
@@ -496,6 +500,32 @@ bool in_capture(const c10::Stream& s, unsigned long long id) {
     return hipStreamGetCaptureInfo(h, &status, &other) == hipSuccess && status == hipStreamCaptureStatusActive && other == id;
 }
 
+// Gradients that go on to another stream make that stream wait for this one; under capture that ends the process, unless the stream is in the
+// same capture.  A leaf's stream is that of the oldest graph which still holds it, so an eager result that lives is enough.
+template <typename F>
+void refuse_other_streams(const Node& node, const Tensor& on, F&& wanted, const char* who, const char* results, const char* input) {
+    hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
+    unsigned long long capture_id = 0;
+    if (hipStreamGetCaptureInfo((hipStream_t)stream_of(on), &capture, &capture_id) != hipSuccess || capture == hipStreamCaptureStatusNone) return;
+    const c10::StreamId here = c10::hip::getCurrentHIPStream(on.device().index()).unwrap().id();
+    for (uint32_t i = 0; i < node.num_outputs(); ++i) {
+        const auto& edge = node.next_edge(i);
+        const auto there = edge.function ? edge.function->stream() : std::nullopt;
+        if (wanted(i) && there && there->id() != here && !in_capture(*there, capture_id))
+            throw std::runtime_error(std::string(who) + ": a captured backward would hand its gradients to another stream; free the " + results +
+                                     " that were made from the same tensors outside the capture, and make " + input + " inside it or let it be a leaf");
+    }
+}
+
+// a graph of the backward is being recorded: what comes out of it cannot be differentiated, and says so if it is
+void differentiable_once(variable_list& out, const char* who) {
+    for (Tensor& t : out)
+        if (t.defined()) {
+            auto error = std::make_shared<torch::autograd::DelayedError>(std::string(who) + " is differentiable once", 1);
+            t = (*error)({t.detach().requires_grad_(true)})[0];
+        }
+}
+
 struct LinearCrossEntropyBackward : public Node {
     SavedVariable x_, w_, labels_, saved_;
     int64_t ignore = 0;
@@ -518,20 +548,7 @@ struct LinearCrossEntropyBackward : public Node {
         const Tensor x = x_.unpack(), w = w_.unpack(), labels = labels_.unpack(), saved = saved_.unpack(shared_from_this());
         c10::DeviceGuard guard(x.device());
         const bool again = at::GradMode::is_enabled();
-        // Gradients that go on to another stream make that stream wait for this one; under capture that ends the process, unless the stream is in the
-        // same capture.  A leaf's stream is that of the oldest graph which still holds it, so an eager loss that lives is enough.
-        hipStreamCaptureStatus capture = hipStreamCaptureStatusNone;
-        unsigned long long capture_id = 0;
-        if (hipStreamGetCaptureInfo((hipStream_t)stream_of(x), &capture, &capture_id) == hipSuccess && capture != hipStreamCaptureStatusNone) {
-            const c10::StreamId here = c10::hip::getCurrentHIPStream(x.device().index()).unwrap().id();
-            for (uint32_t i = 0; i < num_outputs(); ++i) {
-                const auto& edge = next_edge(i);
-                const auto there = edge.function ? edge.function->stream() : std::nullopt;
-                if (task_should_compute_output(i) && there && there->id() != here && !in_capture(*there, capture_id))
-                    throw std::runtime_error("linear_cross_entropy: a captured backward would hand its gradients to another stream; free the losses that were made "
-                                             "from the same tensors outside the capture, and make x inside it or let it be a leaf");
-            }
-        }
+        refuse_other_streams(*this, x, [this](size_t i) { return task_should_compute_output(i); }, "linear_cross_entropy", "losses", "x");
         {
             at::NoGradGuard no_grad;
             const Tensor g = cast_to(grads[0], at::kFloat).contiguous();
@@ -548,13 +565,121 @@ struct LinearCrossEntropyBackward : public Node {
             check(xq_lce_bwd(&h.q, (const float*)g.data_ptr(), saved.data_ptr(), keep, need_dx ? out[0].data_ptr() : nullptr, h.q.H,
                              need_dw ? out[1].data_ptr() : nullptr, h.q.H, need_dw ? ws.get() : nullptr, ws.bytes, stream_of(x)));
         }
-        // a graph of the backward is being recorded: what comes out of it here cannot be differentiated, and says so if it is
-        if (again)
-            for (Tensor& t : out)
-                if (t.defined()) {
-                    auto error = std::make_shared<torch::autograd::DelayedError>("linear_cross_entropy is differentiable once", 1);
-                    t = (*error)({t.detach().requires_grad_(true)})[0];
-                }
+        if (again) differentiable_once(out, "linear_cross_entropy");
+        return out;
+    }
+};
+
+// ---- what a program picks by an index per token
+// rows of any pitch and alignment, not overlapping; other layouts take a packed copy
+struct AnyRows {
+    Tensor keep;
+    void* ptr = nullptr;
+    int64_t ld = 0, M = 0;
+
+    explicit AnyRows(const Tensor& x) : keep(x), ld(x.size(-1)) {
+        M = ld ? x.numel() / ld : 0;
+        const int64_t width = ld;
+        if (!x.is_contiguous() && (!Rows::any_pitch(x, &ld) || ld < width)) {
+            keep = x.contiguous();
+            ld = width;
+        }
+        ptr = keep.data_ptr();
+    }
+};
+
+// a tensor that a node kept, as it was: hooks of saved tensors may give back anything, and storage can be exchanged without a word to autograd
+void check_kept(const char* who, const Tensor& t, const Tensor& on, at::ScalarType dt, int64_t numel) {
+    if (!t.defined() || t.device() != on.device() || t.scalar_type() != dt || t.numel() != numel || !in_storage(t))
+        throw std::runtime_error(std::string(who) + ": what the forward kept was freed, resized or exchanged before the backward");
+}
+
+bool route_keeps_logits(const xq_moe_route& q) { return q.scoring != XQ_ROUTE_SOFTMAX || !q.renormalize; }
+
+struct MoeRouteBackward : public Node {
+    SavedVariable z_, w_, ids_;
+    xq_moe_route q{};                          // without addresses
+    std::vector<int64_t> shape;                // of the logits
+
+    std::string name() const override { return "MoeRouteBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        z_.reset_data();
+        w_.reset_data();
+        ids_.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(1);
+        if (!task_should_compute_output(0)) return out;
+        const Tensor w = w_.unpack(shared_from_this()), ids = ids_.unpack(shared_from_this());
+        const at::ScalarType dt = q.dtype == XQ_DT_F32 ? at::kFloat : at::kBFloat16;
+        const int64_t kept = q.n_tokens * q.top_k;
+        if (!w.defined() || !w.is_cuda()) throw std::runtime_error("moe_route: what the forward kept was freed, resized or exchanged before the backward");
+        c10::DeviceGuard guard(w.device());
+        const bool again = at::GradMode::is_enabled();
+        refuse_other_streams(*this, w, [](size_t) { return true; }, "moe_route", "weights", "the logits");
+        {
+            at::NoGradGuard no_grad;
+            const Tensor g = grads[0].defined() ? cast_to(grads[0], at::kFloat).contiguous() : at::zeros_like(w, at::MemoryFormat::Contiguous);
+            check_kept("moe_route", w, w, at::kFloat, kept);
+            check_kept("moe_route", ids, w, at::kLong, kept);
+            check_kept("moe_route", g, w, at::kFloat, kept);
+            const Tensor wc = w.contiguous(), ic = ids.contiguous();
+            xq_moe_route p = q;
+            p.ld = p.num_experts;
+            std::optional<AnyRows> rows;
+            if (route_keeps_logits(q)) {
+                const Tensor z = z_.unpack();
+                check_kept("moe_route", z, w, dt, q.n_tokens * q.num_experts);
+                rows.emplace(z.view(shape));
+                p.logits = rows->ptr;
+                p.ld = rows->ld;
+            }
+            out[0] = empty(shape, dt);
+            check(xq_moe_route_bwd(&p, (const float*)wc.data_ptr(), (const int64_t*)ic.data_ptr(), (const float*)g.data_ptr(), out[0].data_ptr(), p.num_experts,
+                                   stream_of(w)));
+        }
+        if (again) differentiable_once(out, "moe_route");
+        return out;
+    }
+};
+
+struct EmbeddingBackward : public Node {
+    SavedVariable ids_;
+    xq_embedding q{};                          // without addresses
+    at::ScalarType id_dt = at::kLong;
+    c10::Device device{c10::kCUDA, 0};
+
+    std::string name() const override { return "EmbeddingBackward"; }
+    void release_variables() override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        ids_.reset_data();
+    }
+    variable_list apply(variable_list&& grads) override {
+        std::lock_guard<std::mutex> lock(mutex_);
+        variable_list out(1);
+        if (!task_should_compute_output(0)) return out;
+        const Tensor ids = ids_.unpack();
+        c10::DeviceGuard guard(device);
+        if (!grads[0].defined()) grads[0] = input_metadata(0).zeros_like();
+        const bool again = at::GradMode::is_enabled();
+        refuse_other_streams(*this, grads[0], [](size_t) { return true; }, "embedding", "results", "the weight");
+        {
+            at::NoGradGuard no_grad;
+            const at::ScalarType dt = q.dtype == XQ_DT_F32 ? at::kFloat : at::kBFloat16;
+            const Tensor g = cast_to(grads[0], dt);
+            check_kept("embedding", ids, g, id_dt, q.n_tokens);
+            check_kept("embedding", g, g, dt, q.n_tokens * q.H);
+            const AnyRows rows(g);
+            const Tensor ic = ids.contiguous();
+            xq_embedding p = q;
+            p.ids = ic.data_ptr();
+            out[0] = empty({q.V, q.H}, dt);
+            Scratch ws(xq_embedding_workspace_bytes(q.n_tokens, q.V, q.H));
+            check(xq_embedding_bwd(&p, rows.ptr, rows.ld, out[0].data_ptr(), q.H, ws.get(), ws.bytes, stream_of(g)));
+        }
+        if (again) differentiable_once(out, "embedding");
         return out;
     }
 };
@@ -967,6 +1092,179 @@ PyObject* cross_entropy(PyObject*, PyObject* const* args, Py_ssize_t n) {
     });
 }
 
+// the numbers of a call, which come before its tensors: their conversion may run Python, and with it change those
+bool as_int(PyObject* o, int64_t* v) {
+    if (!PyLong_Check(o)) return false;
+    *v = PyLong_AsLongLong(o);
+    if (*v == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+bool as_number(PyObject* o, double* v) {
+    if (!PyFloat_Check(o) && !PyLong_Check(o)) return false;
+    *v = PyFloat_AsDouble(o);
+    if (*v == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+
+// moe_route(logits, bias or None, top_k, scoring, num_groups, top_groups, group_score, renormalize, scale)
+PyObject* moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 9) { PyErr_SetString(PyExc_TypeError, "moe_route(9 arguments)"); return nullptr; }
+        int64_t k, scoring, groups, top_groups, group_score;
+        double scale;
+        if (!as_int(args[2], &k) || !as_int(args[3], &scoring) || !as_int(args[4], &groups) || !as_int(args[5], &top_groups) || !as_int(args[6], &group_score) ||
+            !as_number(args[8], &scale))
+            XQ_NONE;
+        const Tensor *z = plain(args[0]), *bias = args[1] == Py_None ? nullptr : plain(args[1]);
+        if (under_transform() || !z || (args[1] != Py_None && !bias) || z->dim() < 1 || z->is_neg() || (z->scalar_type() != at::kFloat && z->scalar_type() != at::kBFloat16))
+            XQ_NONE;
+        const int64_t E = z->size(-1);
+        if (E < 1 || E > 1024 || scoring < 0 || group_score < 0 || groups < 1 || groups > 64 || E % groups || top_groups < 1 || top_groups > groups || k < 1 || k > 32 ||
+            k > E / groups * top_groups || !(scale >= 0x1p-60 && scale <= 0x1p60))
+            XQ_NONE;
+        if (bias && (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != E || bias->device() != z->device() || bias->is_neg())) XQ_NONE;
+        const bool grad = at::GradMode::is_enabled() && z->requires_grad();
+        c10::DeviceGuard guard(z->device());
+        Tensor weights, ids;
+        xq_moe_route q{};
+        q.dtype = z->scalar_type() == at::kFloat ? XQ_DT_F32 : XQ_DT_BF16;
+        q.num_experts = (int32_t)E; q.top_k = (int32_t)k; q.scoring = (int32_t)scoring; q.num_groups = (int32_t)groups; q.top_groups = (int32_t)top_groups;
+        q.group_score = (int32_t)group_score; q.renormalize = args[7] == Py_True; q.scale = (float)scale;
+        {
+            at::NoGradGuard no_grad;
+            const AnyRows rows(*z);
+            const Tensor b = bias ? bias->contiguous() : Tensor();
+            weights = empty_f32(with_last(*z, k));
+            ids = empty(with_last(*z, k), at::kLong);
+            q.n_tokens = rows.M;
+            xq_moe_route p = q;
+            p.logits = rows.ptr; p.ld = rows.ld; p.bias = bias ? (const float*)b.data_ptr() : nullptr;
+            void* stream = stream_of(*z);
+            ReleaseGil nogil;
+            check(xq_moe_route_fwd(&p, (float*)weights.data_ptr(), (int64_t*)ids.data_ptr(), stream));
+        }
+        if (grad) {
+            auto node = std::shared_ptr<MoeRouteBackward>(new MoeRouteBackward(), torch::autograd::deleteNode);
+            node->set_next_edges(torch::autograd::collect_next_edges(*z));
+            if (route_keeps_logits(q)) node->z_ = SavedVariable(*z, false);
+            node->ids_ = SavedVariable(ids, false);
+            node->q = q;
+            node->shape.assign(z->sizes().begin(), z->sizes().end());
+            torch::autograd::set_history(weights, node);
+            node->w_ = SavedVariable(weights, true);
+        }
+        PyObject *w = THPVariable_Wrap(std::move(weights)), *i = THPVariable_Wrap(std::move(ids));
+        PyObject* out = w && i ? PyTuple_Pack(2, w, i) : nullptr;
+        Py_XDECREF(w);
+        Py_XDECREF(i);
+        return out;
+    });
+}
+
+// adapters(base, x, A, B, ids, scalings, in place)
+PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 7) { PyErr_SetString(PyExc_TypeError, "adapters(base, x, A, B, ids, scalings, in_place)"); return nullptr; }
+        const Tensor *base = plain(args[0]), *x = plain(args[1]), *A = plain(args[2]), *B = plain(args[3]), *ids = plain(args[4]), *s = plain(args[5]);
+        if (under_transform() || !base || !x || !A || !B || !ids || !s) XQ_NONE;
+        const bool in_place = args[6] == Py_True;
+        for (const Tensor* t : {base, x, A, B, s})
+            if ((at::GradMode::is_enabled() && t->requires_grad()) || t->is_neg()) XQ_NONE;
+        if (base->scalar_type() != at::kBFloat16 || x->scalar_type() != at::kBFloat16 || A->scalar_type() != B->scalar_type() || s->scalar_type() != at::kFloat ||
+            (A->scalar_type() != at::kFloat && A->scalar_type() != at::kBFloat16) || (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || ids->is_neg())
+            XQ_NONE;
+        if (x->dim() < 1 || base->dim() != x->dim() || A->dim() != 3 || B->dim() != 3 || s->dim() != 1 || ids->dim() != x->dim() - 1) XQ_NONE;
+        const int64_t K = x->size(-1), N = base->size(-1), a = A->size(0), r = A->size(1);
+        if (K < 64 || K % 64 || N < 16 || N % 16 || r < 1 || r > 64 || A->size(2) != K || B->size(0) != a || B->size(1) != N || B->size(2) != r || s->size(0) != a ||
+            a >= (1ll << 31))
+            XQ_NONE;
+        const auto lead = x->sizes().slice(0, x->dim() - 1);
+        if (lead != base->sizes().slice(0, base->dim() - 1) || lead != ids->sizes()) XQ_NONE;
+        for (const Tensor* t : {base, A, B, ids, s})
+            if (t->device() != x->device()) XQ_NONE;
+        auto aligned = [](const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0; };
+        // (rows and factors that have to be copied first, and a base that cannot be written, are the Python path's)
+        int64_t ldx = K, ldb = N;
+        if (!A->is_contiguous() || !B->is_contiguous() || !s->is_contiguous() || !ids->is_contiguous() || !aligned(*A) || !aligned(*B) || !aligned(*x) || !aligned(*base) ||
+            (!x->is_contiguous() && (!Rows::pitched(*x, &ldx) || ldx < K)) || (!base->is_contiguous() && (!Rows::pitched(*base, &ldb) || ldb < N)))
+            XQ_NONE;
+        c10::DeviceGuard guard(x->device());
+        xq_adapters q{};
+        q.M = x->numel() / K; q.N = N; q.K = K;
+        q.x = x->data_ptr(); q.ldx = ldx; q.base = base->data_ptr(); q.ld_base = ldb;
+        q.A = A->data_ptr(); q.B = B->data_ptr(); q.scaling = (const float*)s->data_ptr(); q.ids = ids->data_ptr();
+        q.n_adapters = (int32_t)a; q.r = (int32_t)r; q.factor_dtype = A->scalar_type() == at::kFloat ? XQ_DT_F32 : XQ_DT_BF16; q.id_bytes = (int32_t)ids->element_size();
+        Tensor out = in_place ? *base : empty_bf(base->sizes());
+        q.out = out.data_ptr(); q.ld_out = in_place ? ldb : N;
+        if (in_place) {                                     // nothing else that is read may lie in what is written
+            auto end = [](const Tensor& t) {
+                int64_t last = 0;
+                for (int64_t d = 0; d < t.dim(); ++d) last += (t.size(d) - 1) * t.stride(d);
+                return (const char*)t.data_ptr() + (t.numel() ? (last + 1) * (int64_t)t.element_size() : 0);
+            };
+            for (const Tensor* t : {x, A, B, ids, s})
+                if ((const char*)t->data_ptr() < end(out) && (const char*)out.data_ptr() < end(*t)) XQ_NONE;
+        }
+        Scratch ws(xq_adapters_workspace_bytes(q.M, N, K, (int)r));
+        {
+            void* stream = stream_of(*x);
+            ReleaseGil nogil;
+            check(xq_adapters_add(&q, ws.get(), ws.bytes, stream));
+        }
+        if (in_place && !out.is_inference()) out.unsafeGetTensorImpl()->bump_version();
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
+// embedding(ids, weight, scale, padding_idx or None)
+PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
+    return guarded([&]() -> PyObject* {
+        if (n != 4) { PyErr_SetString(PyExc_TypeError, "embedding(ids, weight, scale, padding_idx)"); return nullptr; }
+        double scale;
+        int64_t pad = -1;
+        if (!as_number(args[2], &scale) || (args[3] != Py_None && !as_int(args[3], &pad))) XQ_NONE;
+        const Tensor *ids = plain(args[0]), *w = plain(args[1]);
+        if (under_transform() || !ids || !w || w->dim() != 2 || w->size(0) < 1 || w->size(1) < 1 || (w->scalar_type() != at::kFloat && w->scalar_type() != at::kBFloat16) ||
+            (ids->scalar_type() != at::kInt && ids->scalar_type() != at::kLong) || ids->device() != w->device() || w->is_neg() || ids->is_neg())
+            XQ_NONE;
+        const int64_t V = w->size(0), H = w->size(1);
+        if (args[3] != Py_None) {
+            if (pad < -V || pad >= V) XQ_NONE;
+            if (pad < 0) pad += V;
+        }
+        if (!(std::fabs(scale) <= 3.4e38)) XQ_NONE;
+        const bool grad = at::GradMode::is_enabled() && w->requires_grad();
+        c10::DeviceGuard guard(w->device());
+        Tensor out;
+        xq_embedding q{};
+        q.n_tokens = ids->numel(); q.V = V; q.H = H; q.padding_idx = pad; q.scale = (float)scale;
+        q.dtype = w->scalar_type() == at::kFloat ? XQ_DT_F32 : XQ_DT_BF16; q.id_bytes = (int32_t)ids->element_size();
+        {
+            at::NoGradGuard no_grad;
+            const Tensor i = ids->contiguous();
+            const AnyRows rows(*w);
+            std::vector<int64_t> shape(ids->sizes().begin(), ids->sizes().end());
+            shape.push_back(H);
+            out = empty(shape, w->scalar_type());
+            xq_embedding p = q;
+            p.ids = i.data_ptr(); p.weight = rows.ptr; p.ldw = rows.ld;
+            void* stream = stream_of(*w);
+            ReleaseGil nogil;
+            check(xq_embedding_fwd(&p, out.data_ptr(), H, stream));
+        }
+        if (grad) {
+            auto node = std::shared_ptr<EmbeddingBackward>(new EmbeddingBackward(), torch::autograd::deleteNode);
+            node->set_next_edges(torch::autograd::collect_next_edges(*w));
+            node->ids_ = SavedVariable(*ids, false);
+            node->q = q;
+            node->id_dt = ids->scalar_type();
+            node->device = w->device();
+            torch::autograd::set_history(out, node);
+        }
+        return THPVariable_Wrap(std::move(out));
+    });
+}
+
 // ---- the optimizer step: its arguments are hundreds of tensors, whose addresses and checks are a matter of tens of microseconds here
 // (a tuple of its own: the caller's list may change while this call converts a number of a user's class or has let go of the GIL, and with it go
 // the tensors)
@@ -1180,6 +1478,9 @@ PyMethodDef methods[] = {
     {"mlp", (PyCFunction)(void (*)())mlp, METH_FASTCALL, nullptr},
     {"moe", (PyCFunction)(void (*)())moe, METH_FASTCALL, nullptr},
     {"cross_entropy", (PyCFunction)(void (*)())cross_entropy, METH_FASTCALL, nullptr},
+    {"moe_route", (PyCFunction)(void (*)())moe_route, METH_FASTCALL, nullptr},
+    {"adapters", (PyCFunction)(void (*)())adapters, METH_FASTCALL, nullptr},
+    {"embedding", (PyCFunction)(void (*)())embedding, METH_FASTCALL, nullptr},
     {"adamw", (PyCFunction)(void (*)())adamw, METH_FASTCALL, nullptr},
     {nullptr, nullptr, 0, nullptr},
 };

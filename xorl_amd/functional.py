@@ -17,6 +17,7 @@ from torch import Tensor
 from torch.autograd import forward_ad
 
 from . import _C
+from ._native import native
 
 
 _CODE_TO_DT = {0: torch.float32, 1: torch.bfloat16, 2: torch.float8_e4m3fn}
@@ -392,6 +393,127 @@ def qlora_linear_multi(x: Tensor, jobs) -> list:
                                    ws.data_ptr(), ws_bytes, _C.stream_ptr(dev)))
     _note_decode_forward(dev, M)
     return [y.reshape(*x.shape[:-1], y.shape[1]) for y in ys]
+
+
+# ---------------------------------------------------------------------------
+# adapters of many requests beside one projection (xq_adapters_add)
+# ---------------------------------------------------------------------------
+def _adapters_problem(base2: Tensor, x2: Tensor, A: Tensor, B: Tensor, ids: Tensor, scalings: Tensor, out2: Tensor) -> _C.XqAdapters:
+    q = _C.XqAdapters()
+    q.x, q.ldx, q.base, q.ld_base, q.out, q.ld_out = x2.data_ptr(), _ld(x2), base2.data_ptr(), _ld(base2), out2.data_ptr(), _ld(out2)
+    q.A, q.B, q.scaling, q.ids = A.data_ptr(), B.data_ptr(), scalings.data_ptr(), ids.data_ptr()
+    q.M, q.N, q.K = x2.shape[0], base2.shape[1], x2.shape[1]
+    q.n_adapters, q.r, q.factor_dtype, q.id_bytes = A.shape[0], A.shape[1], _lora_dt(A), ids.element_size()
+    return q
+
+
+def _rows_in_place(x: Tensor) -> Optional[Tensor]:
+    """x as rows at multiples of 16 bytes that share its memory, or None"""
+    x2 = x.flatten(0, -2) if x.dim() > 1 and x.is_contiguous() else x if x.dim() == 2 else x.unsqueeze(0) if x.dim() == 1 else None
+    ok = x2 is not None and x2.stride(1) == 1 and (x2.shape[0] <= 1 or (x2.stride(0) % 8 == 0 and x2.stride(0) >= x2.shape[1])) and x2.data_ptr() % 16 == 0
+    return x2 if ok else None
+
+
+def _adapters_rows(x: Tensor) -> Tensor:
+    x2 = _as_2d(x)
+    if x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:           # (an expanded row)
+        x2 = x2.contiguous()
+    return x2 if x2.data_ptr() % 16 == 0 else x2.clone()
+
+
+def _aligned(t: Tensor) -> Tensor:
+    t = t.contiguous()
+    return t if t.data_ptr() % 16 == 0 else t.clone()
+
+
+def _adapters_impl(base: Tensor, x: Tensor, A: Tensor, B: Tensor, ids: Tensor, scalings: Tensor, out: Optional[Tensor] = None) -> Tensor:
+    dev = x.device
+    with torch.cuda.device(dev):
+        x2, base2, i1 = _adapters_rows(x), _adapters_rows(base), ids.reshape(-1).contiguous()
+        A, B, scalings = _aligned(A), _aligned(B), scalings.contiguous()
+        res = torch.empty(base.shape, dtype=torch.bfloat16, device=dev) if out is None else out
+        out2 = _rows_in_place(res)
+        if out2 is None:
+            raise _C.XqError("lora_adapters: out must have rows at multiples of 16 bytes")
+        q = _adapters_problem(base2, x2, A, B, i1, scalings, out2)
+        L = _C.lib()
+        ws_bytes = L.xq_adapters_workspace_bytes(q.M, q.N, q.K, q.r)
+        ws = torch.empty(max(ws_bytes, 0), dtype=torch.uint8, device=dev)
+        _C.check(L.xq_adapters_add(ctypes.byref(q), ws.data_ptr(), ws_bytes, _C.stream_ptr(dev)))
+    return res
+
+
+@torch.library.custom_op("xq::lora_adapters", mutates_args=(), device_types="cuda")
+def _adapters_op(base: Tensor, x: Tensor, A: Tensor, B: Tensor, ids: Tensor, scalings: Tensor) -> Tensor:
+    return _adapters_impl(base, x, A, B, ids, scalings)
+
+
+@_adapters_op.register_fake
+def _(base, x, A, B, ids, scalings):
+    return base.new_empty(base.shape)
+
+
+def _span(t: Tensor) -> Tuple[int, int]:
+    """the addresses from a tensor's first byte to behind its last"""
+    if t.numel() == 0:
+        return t.data_ptr(), t.data_ptr()
+    return t.data_ptr(), t.data_ptr() + (sum((n - 1) * s for n, s in zip(t.shape, t.stride())) + 1) * t.element_size()
+
+
+def lora_adapters(base: Tensor, x: Tensor, lora_A: Tensor, lora_B: Tensor, adapter_ids: Tensor, scalings: Tensor, *,
+                  out: Optional[Tensor] = None) -> Tensor:
+    """Forward-only: ``base + scalings[a] * (x @ lora_A[a].T) @ lora_B[a].T`` with the adapter ``a = adapter_ids[..]`` of each row: the low-rank updates of
+    the requests of a batch beside one shared projection, whose output without an adapter is ``base`` (``qlora_linear(x, qw, None, None, 0, 0.0)``;
+    :func:`~xorl_amd.qlora.qlora_adapters_forward` does both).  A row whose id is negative or no adapter's has none and gets ``base``.
+
+    base [.., N] and x [.., K] bf16; lora_A [n, r, K] and lora_B [n, N, r] fp32 or bf16, an adapter of a smaller rank padded with zeros; adapter_ids [..] int32
+    or int64; scalings [n] fp32.  K % 64 == 0, N % 16 == 0, r 1 to 64.  Products accumulate in fp32; factors in fp32 and x @ A.T enter them with 16 bits and more; the sum with base is
+    rounded once.  Any mix of adapters is taken; rows of one adapter that follow each other are the fast order above 1024 rows.  The result is a new tensor, or ``out``, which
+    may be base itself and otherwise shares no memory with what is read."""
+    if not torch.compiler.is_compiling() and (out is None or out is base):
+        y = native().adapters(base, x, lora_A, lora_B, adapter_ids, scalings, out is not None)
+        if y is not None:
+            return y
+    # what the native path leaves: traced calls, tensor subclasses, an out of its own, and the errors
+    tensors = (base, x, lora_A, lora_B, scalings)
+    if torch.is_grad_enabled() and any(t.requires_grad for t in (*tensors, *(() if out is None else (out,)))):
+        raise _C.XqError("lora_adapters is forward-only: call it under torch.no_grad()")
+    if base.dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
+        raise _C.XqError(f"lora_adapters: base and x must be bf16, got {base.dtype} and {x.dtype}")
+    if lora_A.dtype != lora_B.dtype or lora_A.dtype not in (torch.float32, torch.bfloat16) or scalings.dtype != torch.float32:
+        raise _C.XqError(f"lora_adapters: the factors must both be fp32 or both bf16 and the scalings fp32, got {lora_A.dtype}, {lora_B.dtype} and {scalings.dtype}")
+    if adapter_ids.dtype not in (torch.int32, torch.int64):
+        raise _C.XqError(f"lora_adapters: adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
+    if (lora_A.dim() != 3 or lora_B.dim() != 3 or x.dim() < 1 or base.dim() < 1 or x.shape[:-1] != base.shape[:-1] or adapter_ids.shape != x.shape[:-1]
+            or tuple(lora_A.shape) != (lora_A.shape[0], lora_B.shape[2], x.shape[-1]) or tuple(lora_B.shape[:2]) != (lora_A.shape[0], base.shape[-1])
+            or tuple(scalings.shape) != (lora_A.shape[0],)):
+        raise _C.XqError(f"lora_adapters: base [.., N], x [.., K], lora_A [n, r, K], lora_B [n, N, r], adapter_ids [..] and scalings [n] do not go together: {tuple(base.shape)}, "
+                         f"{tuple(x.shape)}, {tuple(lora_A.shape)}, {tuple(lora_B.shape)}, {tuple(adapter_ids.shape)}, {tuple(scalings.shape)}")
+    if x.shape[-1] < 64 or x.shape[-1] % 64 or base.shape[-1] < 16 or base.shape[-1] % 16 or not 1 <= lora_A.shape[1] <= MAX_FUSED_RANK:
+        raise _C.XqError(f"lora_adapters: in_features must be a multiple of 64, out_features of 16 and the rank 1 to {MAX_FUSED_RANK}, got {x.shape[-1]}, {base.shape[-1]} "
+                         f"and {lora_A.shape[1]}")
+    if torch.compiler.is_compiling():
+        y = _adapters_op(base.detach(), x.detach(), lora_A.detach(), lora_B.detach(), adapter_ids, scalings.detach())
+        return y if out is None else out.copy_(y)
+    refuse_tangents(*tensors, out)
+    _C.require_hip(*tensors, adapter_ids, out)
+    if len({t.device for t in (*tensors, adapter_ids, *(() if out is None else (out,)))}) > 1:
+        raise _C.XqError("lora_adapters: the tensors are on different devices")
+    if out is not None:
+        if out.dtype != torch.bfloat16 or out.shape != base.shape or _rows_in_place(out) is None:
+            raise _C.XqError(f"lora_adapters: out must be bf16 {tuple(base.shape)} with rows at multiples of 16 bytes, got {out.dtype} {tuple(out.shape)} of strides {out.stride()}")
+        a, b = _span(out)
+        for t in (*tensors, adapter_ids):
+            c, d = _span(t)
+            same = t is base and a == c and out.stride() == base.stride()
+            if a < d and c < b and not same:
+                raise _C.XqError("lora_adapters: out shares memory with what is read (it may be base itself)")
+    y = _adapters_impl(base.detach(), x.detach(), lora_A.detach(), lora_B.detach(), adapter_ids, scalings.detach(), None if out is None else out.detach())
+    if out is None:
+        return y
+    if not out.is_inference():
+        torch.autograd.graph.increment_version(out)
+    return out
 
 
 # ---------------------------------------------------------------------------

@@ -48,6 +48,163 @@ def route_build(selected_experts: Tensor, num_experts: int):
     return counts, offsets, sidx, tile_offsets
 
 
+
+# ---------------------------------------------------------------------------
+# the choice of experts
+# ---------------------------------------------------------------------------
+def _route_rows(z: Tensor) -> Tensor:
+    z2 = z.reshape(-1, z.shape[-1])
+    return z2 if z2.stride(-1) == 1 and (z2.shape[0] <= 1 or z2.stride(0) >= z2.shape[1]) else z2.contiguous()
+
+
+def _route_problem(z2: Optional[Tensor], n_tokens: int, num_experts: int, dtype: torch.dtype, bias: Optional[Tensor], options) -> _C.XqMoeRoute:
+    q = _C.XqMoeRoute()
+    q.logits, q.ld = (None, num_experts) if z2 is None else (z2.data_ptr(), z2.stride(0) if n_tokens > 1 else num_experts)
+    q.bias, q.n_tokens, q.num_experts = _C.ptr(bias), n_tokens, num_experts
+    q.dtype = _C.XQ_DT_F32 if dtype == torch.float32 else _C.XQ_DT_BF16
+    q.top_k, q.scoring, q.num_groups, q.top_groups, q.group_score, q.renormalize, q.scale = options
+    return q
+
+
+def _route_fwd_impl(z: Tensor, bias: Optional[Tensor], options) -> Tuple[Tensor, Tensor]:
+    dev = z.device
+    with torch.cuda.device(dev):
+        z2 = _route_rows(z)
+        b = None if bias is None else bias.contiguous()
+        shape = (*z.shape[:-1], options[0])
+        weights = torch.empty(shape, dtype=torch.float32, device=dev)
+        ids = torch.empty(shape, dtype=torch.int64, device=dev)
+        q = _route_problem(z2, z2.shape[0], z2.shape[1], z.dtype, b, options)
+        _C.check(_C.lib().xq_moe_route_fwd(ctypes.byref(q), weights.data_ptr(), ids.data_ptr(), _s(dev)))
+    return weights, ids
+
+
+def _route_bwd_impl(grad: Tensor, weights: Tensor, ids: Tensor, z: Tensor, num_experts: int, dtype: torch.dtype, options) -> Tensor:
+    """z without elements: a backward that needs no logits"""
+    dev = weights.device
+    with torch.cuda.device(dev):
+        n = weights.numel() // options[0]
+        g, w, i = grad.to(torch.float32).contiguous(), weights.contiguous(), ids.contiguous()
+        z2 = _route_rows(z) if _route_keeps_logits(options) else None
+        if g.numel() != w.numel() or i.numel() != w.numel() or (z2 is not None and (tuple(z2.shape) != (n, num_experts) or z2.dtype != dtype)):
+            raise _C.XqError("moe_route: what the forward kept, or the gradient, is not that of this problem")
+        dz = torch.empty((*weights.shape[:-1], num_experts), dtype=dtype, device=dev)
+        q = _route_problem(z2, n, num_experts, dtype, None, options)
+        _C.check(_C.lib().xq_moe_route_bwd(ctypes.byref(q), w.data_ptr(), i.data_ptr(), g.data_ptr(), dz.data_ptr(), num_experts, _s(dev)))
+    return dz
+
+
+def _route_keeps_logits(options) -> bool:
+    """whether a backward reads the logits: renormalized softmax weights are those of the chosen logits alone"""
+    return not (options[1] == _C.ROUTE_SCORINGS["softmax"] and options[5])
+
+
+@torch.library.custom_op("xq::moe_route_fwd", mutates_args=(), device_types="cuda")
+def _route_fwd_op(z: Tensor, bias: Optional[Tensor], top_k: int, scoring: int, num_groups: int, top_groups: int, group_score: int, renormalize: bool,
+                  scale: float) -> Tuple[Tensor, Tensor]:
+    return _route_fwd_impl(z, bias, (top_k, scoring, num_groups, top_groups, group_score, renormalize, scale))
+
+
+@_route_fwd_op.register_fake
+def _(z, bias, top_k, scoring, num_groups, top_groups, group_score, renormalize, scale):
+    shape = (*z.shape[:-1], top_k)
+    return z.new_empty(shape, dtype=torch.float32), z.new_empty(shape, dtype=torch.int64)
+
+
+@torch.library.custom_op("xq::moe_route_bwd", mutates_args=(), device_types="cuda")
+def _route_bwd_op(grad: Tensor, weights: Tensor, ids: Tensor, z: Tensor, num_experts: int, bf16: bool, top_k: int, scoring: int, num_groups: int,
+                  top_groups: int, group_score: int, renormalize: bool, scale: float) -> Tensor:
+    return _route_bwd_impl(grad, weights, ids, z, num_experts, torch.bfloat16 if bf16 else torch.float32,
+                           (top_k, scoring, num_groups, top_groups, group_score, renormalize, scale))
+
+
+@_route_bwd_op.register_fake
+def _(grad, weights, ids, z, num_experts, bf16, top_k, scoring, num_groups, top_groups, group_score, renormalize, scale):
+    return weights.new_empty((*weights.shape[:-1], num_experts), dtype=torch.bfloat16 if bf16 else torch.float32)
+
+
+class MoeRouteFunction(torch.autograd.Function):
+    """The chosen experts and their weights; the gradient of the logits from the weights' alone."""
+
+    @staticmethod
+    def forward(ctx, z, bias, options):
+        if torch.compiler.is_compiling():
+            weights, ids = _route_fwd_op(z, bias, *options)
+        else:
+            weights, ids = _route_fwd_impl(z, bias, options)
+        ctx.mark_non_differentiable(ids)
+        ctx.options, ctx.num_experts, ctx.dtype = options, z.shape[-1], z.dtype
+        ctx.save_for_backward(weights, ids, *((z,) if _route_keeps_logits(options) else ()))
+        return weights, ids
+
+    @staticmethod
+    @torch.autograd.function.once_differentiable
+    def backward(ctx, grad, _):
+        if not torch.compiler.is_compiling() and torch.cuda.is_current_stream_capturing():
+            # (torch may hand the gradients to another stream, which ends the process under capture; the native node looks at whose)
+            raise RuntimeError("moe_route: a captured backward takes plain tensors, no subclasses of them")
+        weights, ids = ctx.saved_tensors[:2]
+        z = ctx.saved_tensors[2] if len(ctx.saved_tensors) > 2 else weights.new_empty(0)
+        if torch.compiler.is_compiling():
+            return _route_bwd_op(grad, weights, ids, z, ctx.num_experts, ctx.dtype == torch.bfloat16, *ctx.options), None, None
+        return _route_bwd_impl(grad, weights, ids, z, ctx.num_experts, ctx.dtype, ctx.options), None, None
+
+
+def moe_route(router_logits: Tensor, top_k: int, *, scoring: str = "softmax", bias: Optional[Tensor] = None, num_groups: int = 1, top_groups: int = 1,
+              group_score: str = "sum2", renormalize: bool = True, scale: float = 1.0) -> Tuple[Tensor, Tensor]:
+    """``(routing_weights [.., top_k] fp32, selected_experts [.., top_k] int64)`` of ``router_logits [.., E]`` (bf16 or fp32): the arguments that
+    the expert modules and :func:`moe_experts_qlora_forward` take.
+
+    Scores are the softmax over all E logits or their sigmoid.  The top_k experts are chosen in descending order of score + ``bias`` (fp32 [E], for
+    balance; compared in 64 bits), without a bias in that of the logits; equal ones by their index.  With ``num_groups`` > 1 only experts
+    of the ``top_groups`` best groups (runs of E / num_groups experts) can be chosen; a group counts as its best expert (``group_score="max"``) or as the sum of
+    its two best (``"sum2"``).  Weights are the scores without the bias, with ``renormalize`` divided by their sum, times ``scale``.
+
+    An expert whose logit or bias is -inf is never chosen: where fewer than top_k are left, the places behind them hold id -1, which the experts drop, and
+    weight 0.  A row with a NaN (or, under softmax, an infinite logit) gets NaN weights and a NaN gradient.
+
+    Gradients go to the logits, through the weights; the choice itself has none, so the bias gets none.  First derivatives only.  At most 1024 experts, 64
+    groups and top_k 32.  Under graph capture forward and backward go into the same graph, and no weights made outside it from the same logits may
+    still be alive (refused; in a compiled call torch ends the process)."""
+    options = (top_k, _C.ROUTE_SCORINGS.get(scoring, -1), num_groups, top_groups, _C.ROUTE_GROUP_SCORES.get(group_score, -1), bool(renormalize), scale)
+    if not torch.compiler.is_compiling():
+        out = native().moe_route(router_logits, bias, *options)
+        if out is not None:
+            return out
+    # what the native path leaves: traced calls, tensor subclasses, and the errors
+    if isinstance(scale, Tensor) or isinstance(top_k, Tensor):
+        raise _C.XqError("moe_route: scale and top_k are numbers, not tensors")
+    if options[1] < 0:
+        raise _C.XqError(f"moe_route: scoring must be one of {sorted(_C.ROUTE_SCORINGS)}, got {scoring!r}")
+    if options[4] < 0:
+        raise _C.XqError(f"moe_route: group_score must be one of {sorted(_C.ROUTE_GROUP_SCORES)}, got {group_score!r}")
+    if router_logits.dtype not in (torch.bfloat16, torch.float32) or router_logits.dim() < 1:
+        raise _C.XqError(f"moe_route: logits [.., E] must be bf16 or fp32, got {router_logits.dtype} {tuple(router_logits.shape)}")
+    E = router_logits.shape[-1]
+    if not 1 <= E <= 1024:
+        raise _C.XqError(f"moe_route: 1 to 1024 experts, got {E}")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
+        raise _C.XqError(f"moe_route: the bias must be fp32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
+    if not 1 <= num_groups <= 64 or E % num_groups or not 1 <= top_groups <= num_groups:
+        raise _C.XqError(f"moe_route: {E} experts cannot be taken in {num_groups} groups (at most 64, of equal size) of which {top_groups} count")
+    if not 1 <= top_k <= min(32, E // num_groups * top_groups):
+        raise _C.XqError(f"moe_route: top_k must be 1 to 32 and at most the {E // num_groups * top_groups} experts that can be chosen, got {top_k}")
+    if not 2.0 ** -60 <= scale <= 2.0 ** 60:
+        raise _C.XqError(f"moe_route: scale must be from 2^-60 to 2^60, got {scale}")
+    if not torch.compiler.is_compiling():
+        refuse_tangents(router_logits, bias)
+    _C.require_hip(router_logits, bias)
+    if bias is not None and bias.device != router_logits.device:
+        raise _C.XqError(f"moe_route: logits and bias are on {router_logits.device} and {bias.device}")
+    options = (int(top_k), options[1], int(num_groups), int(top_groups), options[4], options[5], float(scale))
+    b = None if bias is None else bias.detach()
+    if torch.is_grad_enabled() and router_logits.requires_grad:
+        return MoeRouteFunction.apply(router_logits, b, options)
+    if torch.compiler.is_compiling():
+        return _route_fwd_op(router_logits.detach(), b, *options)
+    return _route_fwd_impl(router_logits.detach(), b, options)
+
+
 def moe_scatter(x: Tensor, sidx: Tensor, topk: int) -> Tensor:
     x = x.contiguous()
     n, width = sidx.numel(), x.shape[-1]

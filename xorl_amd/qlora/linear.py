@@ -892,6 +892,18 @@ def qlora_linears_forward(modules, x: Tensor) -> list:
                                   for m in mods])
 
 
+def qlora_adapters_forward(module, x: Tensor, lora_A: Tensor, lora_B: Tensor, adapter_ids: Tensor, scalings: Tensor) -> Tensor:
+    """Forward-only: one packed projection for a batch of requests that bring adapters of their own: the module's base weight (and bias) once for all
+    rows, and beside it each row's adapter out of a bank lora_A [n, r, in], lora_B [n, out, r] with its scaling (:func:`~xorl_amd.functional.lora_adapters`).
+    The module's own factors are left out: a request on them takes a bank that holds them."""
+    from ..functional import lora_adapters, qlora_linear
+
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, lora_A, lora_B, scalings, module.bias)):
+        raise _C.XqError("qlora_adapters_forward is forward-only: call it under torch.no_grad()")
+    base = qlora_linear(x, module._forward_quant_weight(), None, None, 0, 0.0, module.bias)
+    return lora_adapters(base, x, lora_A, lora_B, adapter_ids, scalings, out=base)
+
+
 def deregister_qlora_weights_from_fsdp(model: nn.Module, param_names: tuple = ("weight",)) -> int:
     """Drop QLoRALinear parameters from FSDP2 parameter groups so no mixed
     precision cast ever touches the packed bytes; they stay sharded DTensors
