@@ -10,50 +10,263 @@ namespace {
 __device__ __forceinline__ int64_t token_id(const xq_embedding& q, int64_t t) {
     return q.id_bytes == 8 ? ((const int64_t*)q.ids)[t] : (int64_t)((const int32_t*)q.ids)[t];
 }
-__device__ __forceinline__ float load_value(const void* p, int dtype, int64_t at) {
-    return dtype == XQ_DT_F32 ? ((const float*)p)[at] : bf16_to_f32(((const bf16_t*)p)[at]);
-}
-__device__ __forceinline__ void store_value(void* p, int dtype, int64_t at, float v) {
-    if (dtype == XQ_DT_F32) ((float*)p)[at] = v;
-    else ((bf16_t*)p)[at] = to_bf16(v);
-}
 
-__global__ void __launch_bounds__(256) embedding_kernel(xq_embedding q, void* out, int64_t ld_out) {
-    for (int64_t t = blockIdx.x; t < q.n_tokens; t += gridDim.x) {
+// W elements of a row as one access: 16 bytes, or one element where addresses or pitches allow no more
+template <typename T, int W>
+struct Piece {
+    T v[W];
+};
+template <typename T, int W>
+__device__ __forceinline__ Piece<T, W> load_piece(const T* p) {
+    Piece<T, W> r;
+    if constexpr (W > 1) {
+        static_assert(sizeof(r) == 16, "");
+        r = __builtin_bit_cast(Piece<T, W>, *(const u32x4*)p);
+    } else {
+        r.v[0] = *p;
+    }
+    return r;
+}
+template <typename T, int W>
+__device__ __forceinline__ void store_piece(T* p, const Piece<T, W>& r) {
+    if constexpr (W > 1) *(u32x4*)p = __builtin_bit_cast(u32x4, r);
+    else *p = r.v[0];
+}
+__device__ __forceinline__ float value(float v) { return v; }
+__device__ __forceinline__ float value(bf16_t v) { return bf16_to_f32(v); }
+__device__ __forceinline__ void put(float& to, float v) { to = v; }
+__device__ __forceinline__ void put(bf16_t& to, float v) { to = to_bf16(v); }
+
+// out[t] = scale W[id]: `lanes` threads a token
+template <typename T, int W>
+__global__ void __launch_bounds__(256) embedding_kernel(xq_embedding q, T* out, int64_t ld_out, int32_t lanes) {
+    const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1);
+    for (int64_t t = (int64_t)blockIdx.x * per + threadIdx.x / lanes; t < q.n_tokens; t += (int64_t)gridDim.x * per) {
         const int64_t id = token_id(q, t);
         const bool is = id >= 0 && id < q.V;
-        for (int64_t h = threadIdx.x; h < q.H; h += 256)
-            store_value(out, q.dtype, t * ld_out + h, is ? q.scale * load_value(q.weight, q.dtype, id * q.ldw + h) : NAN);
+        const T* from = (const T*)q.weight + (is ? id : 0) * q.ldw;
+        T* to = out + t * ld_out;
+        for (int64_t h = lane * W; h < q.H; h += lanes * W) {
+            Piece<T, W> r = load_piece<T, W>(from + h);
+#pragma unroll
+            for (int i = 0; i < W; ++i) put(r.v[i], is ? q.scale * value(r.v[i]) : NAN);
+            store_piece<T, W>(to + h, r);
+        }
     }
 }
 
-// a block a vocabulary row: it looks through all ids
-__global__ void __launch_bounds__(256) embedding_grad_kernel(xq_embedding q, const void* grad, int64_t ld_grad, void* dw, int64_t ld_dw) {
-    __shared__ int64_t list[256];
-    __shared__ int wave_n[4];
-    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    for (int64_t v = blockIdx.x; v < q.V; v += gridDim.x)
-        for (int64_t h0 = 0; h0 < q.H; h0 += 256) {
-            const int64_t h = h0 + tid;
-            float sum = 0.0f;
-            for (int64_t t0 = 0; t0 < q.n_tokens; t0 += 256) {
-                const bool is = v != q.padding_idx && t0 + tid < q.n_tokens && token_id(q, t0 + tid) == v;
-                const uint64_t mask = __ballot(is);
-                if (lane == 0) wave_n[wave] = __popcll(mask);
-                __syncthreads();
-                int at = __popcll(mask & ((1ull << lane) - 1)), n = 0;
-                for (int w = 0; w < 4; ++w) {
-                    at += w < wave ? wave_n[w] : 0;
-                    n += wave_n[w];
-                }
-                if (is) list[at] = t0 + tid;
-                __syncthreads();
-                if (h < q.H)
-                    for (int i = 0; i < n; ++i) sum += load_value(grad, q.dtype, list[i] * ld_grad + h);
-                __syncthreads();
-            }
-            if (h < q.H) store_value(dw, q.dtype, v * ld_dw + h, q.scale * sum);
+// ---- the gradient: tokens sorted by id (stable), then a pass over the vocabulary that adds each row's tokens or writes its zeros
+// Row v belongs to block v % blocks, as its row v / blocks: ids that come often lie next to each other in a vocabulary, and so go to different blocks.
+struct Sorted {
+    int32_t* start;           // [blocks * rows + 1]: where the tokens of a row begin in token[], by (v % blocks) * rows + v / blocks
+    int32_t* token;           // [n_tokens]: the tokens, row by row, each row's in their order
+    float* part;              // [n_tokens / kChunk, H]: sums over kChunk tokens in that order, where they are all of one row
+    int32_t log_blocks, rows;
+};
+constexpr int kChunk = 64, kSortThreads = 1024, kSortRows = 8192, kSortAtOnce = 4 * kSortThreads;
+
+// Every block looks through all ids: it counts its own rows' and those of the blocks before it, so that no launch is needed that adds
+// counts up, and places its own tokens in a second look.
+__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embedding q, Sorted s) {
+    __shared__ int32_t count[kSortRows], of_wave[16], token[kSortAtOnce];
+    __shared__ uint16_t row[kSortAtOnce];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, block = blockIdx.x;
+    const int64_t mask = (1 << s.log_blocks) - 1;
+    auto real = [&](int64_t id) { return id >= 0 && id < q.V && id != q.padding_idx; };
+    for (int r = tid; r < s.rows; r += kSortThreads) count[r] = 0;
+    __syncthreads();
+    int before = 0;
+    for (int64_t t = tid; t < q.n_tokens; t += kSortThreads) {
+        const int64_t id = token_id(q, t);
+        const int at = (int)(id & mask);
+        before += real(id) && at < block;
+        if (real(id) && at == block) atomicAdd(&count[id >> s.log_blocks], 1);
+    }
+    for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o, 64);
+    if (lane == 0) of_wave[wave] = before;
+    __syncthreads();
+    before = 0;
+    for (int w = 0; w < 16; ++w) before += of_wave[w];
+    __syncthreads();
+    // counts to places: each thread the rows it owns, then the threads before it
+    const int own = (s.rows + kSortThreads - 1) / kSortThreads, first = tid * own, last = min(first + own, s.rows);
+    int mine = 0;
+    for (int r = first; r < last; ++r) mine += count[r];
+    int upto = mine;
+    for (int o = 1; o < 64; o <<= 1) {
+        const int u = __shfl_up(upto, o, 64);
+        if (lane >= o) upto += u;
+    }
+    if (lane == 63) of_wave[wave] = upto;
+    __syncthreads();
+    int at = before + upto - mine, all = 0;
+    for (int w = 0; w < 16; ++w) {
+        at += w < wave ? of_wave[w] : 0;
+        all += of_wave[w];
+    }
+    for (int r = first; r < last; ++r) {
+        const int n = count[r];
+        count[r] = at;
+        s.start[(int64_t)block * s.rows + r] = at;
+        at += n;
+    }
+    if (block == (int)mask && tid == 0) s.start[(int64_t)(block + 1) * s.rows] = before + all;
+    if (all == 0) return;
+    int bits = 0;
+    while ((1 << bits) < s.rows) ++bits;
+    for (int64_t t0 = 0; t0 < q.n_tokens; t0 += kSortAtOnce) {
+        // four tokens a thread, so that the block's come in order
+        int own_row[4], n = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t t = t0 + tid * 4 + i, id = t < q.n_tokens ? token_id(q, t) : -1;
+            own_row[i] = real(id) && (int)(id & mask) == block ? (int)(id >> s.log_blocks) : -1;
+            n += own_row[i] >= 0;
         }
+        int to = n;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(to, o, 64);
+            if (lane >= o) to += u;
+        }
+        __syncthreads();                                   // (the places of the round before have been read)
+        if (lane == 63) of_wave[wave] = to;
+        __syncthreads();
+        to -= n;
+        int found = 0;
+        for (int w = 0; w < 16; ++w) {
+            to += w < wave ? of_wave[w] : 0;
+            found += of_wave[w];
+        }
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (own_row[i] >= 0) {
+                row[to] = (uint16_t)own_row[i];
+                token[to++] = (int)(t0 + tid * 4 + i);
+            }
+        __syncthreads();
+        if (wave == 0)
+            for (int i0 = 0; i0 < found; i0 += 64) {
+                // the tokens of one row among 64: those whose row agrees in every bit
+                const bool is = i0 + lane < found;
+                const int r = is ? row[i0 + lane] : 0;
+                uint64_t same = __ballot(is);
+                for (int b = 0; b < bits; ++b) {
+                    const bool bit = (r >> b) & 1;
+                    const uint64_t m = __ballot(bit);
+                    same &= bit ? m : ~m;
+                }
+                const int rank = __popcll(same & ((1ull << lane) - 1));
+                if (is) {
+                    const int base = count[r];
+                    s.token[base + rank] = token[i0 + lane];
+                    if (rank == __popcll(same) - 1) count[r] = base + rank + 1;
+                }
+            }
+    }
+}
+
+template <typename T, int W>
+__device__ __forceinline__ void add_tokens(const int32_t* token, int from, int to, const T* grad, int64_t ld, int64_t h, float* sum) {
+    int i = from;
+    for (; i + 4 <= to; i += 4) {
+        Piece<T, W> r[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) r[u] = load_piece<T, W>(grad + token[i + u] * ld + h);
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum[j] += value(r[u].v[j]);
+    }
+    for (; i < to; ++i) {
+        const Piece<T, W> r = load_piece<T, W>(grad + token[i] * ld + h);
+#pragma unroll
+        for (int j = 0; j < W; ++j) sum[j] += value(r.v[j]);
+    }
+}
+
+// chunks of kChunk sorted tokens that are all of one row
+template <typename T, int W>
+__global__ void __launch_bounds__(256) embedding_part_kernel(xq_embedding q, Sorted s, const T* grad, int64_t ld) {
+    const int64_t all = s.start[(int64_t)s.rows << s.log_blocks];
+    for (int64_t c = blockIdx.x; (c + 1) * kChunk <= all; c += gridDim.x) {
+        const int32_t* token = s.token + c * kChunk;
+        if (token_id(q, token[0]) != token_id(q, token[kChunk - 1])) continue;
+        for (int64_t h = ((int64_t)blockIdx.y * 256 + threadIdx.x) * W; h < q.H; h += (int64_t)gridDim.y * 256 * W) {
+            float sum[W] = {};
+            add_tokens<T, W>(token, 0, kChunk, grad, ld, h, sum);
+#pragma unroll
+            for (int j = 0; j < W; ++j) s.part[c * q.H + h + j] = sum[j];
+        }
+    }
+}
+
+template <typename T, int W>
+__global__ void __launch_bounds__(256) embedding_grad_kernel(xq_embedding q, Sorted s, const T* grad, int64_t ld, T* dw, int64_t ld_dw, int32_t lanes) {
+    const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1);
+    const int64_t mask = (1 << s.log_blocks) - 1;
+    for (int64_t v = (int64_t)blockIdx.x * per + threadIdx.x / lanes; v < q.V; v += (int64_t)gridDim.x * per) {
+        const int32_t* start = s.start + (v & mask) * s.rows + (v >> s.log_blocks);
+        const int from = start[0], to = start[1];
+        // whole chunks among the row's tokens, and what lies before and behind them
+        const int c0 = (from + kChunk - 1) / kChunk, c1 = max(c0, to / kChunk);
+        for (int64_t h = lane * W; h < q.H; h += lanes * W) {
+            float sum[W] = {};
+            if (c0 < c1) {
+                add_tokens<T, W>(s.token, from, c0 * kChunk, grad, ld, h, sum);
+                for (int c = c0; c < c1; ++c)
+#pragma unroll
+                    for (int j = 0; j < W; ++j) sum[j] += s.part[c * q.H + h + j];
+                add_tokens<T, W>(s.token, c1 * kChunk, to, grad, ld, h, sum);
+            } else {
+                add_tokens<T, W>(s.token, from, to, grad, ld, h, sum);
+            }
+            Piece<T, W> r;
+#pragma unroll
+            for (int j = 0; j < W; ++j) put(r.v[j], q.scale * sum[j]);
+            store_piece<T, W>(dw + v * ld_dw + h, r);
+        }
+    }
+}
+
+// the sorting blocks: 256 of them, more where one would own more rows than fit its counters
+Sorted plan_of(void* base, int64_t n_tokens, int64_t V, int64_t H, int64_t* bytes) {
+    Sorted s = {};
+    s.log_blocks = 8;
+    while (xq_cdiv(V, 1ll << s.log_blocks) > kSortRows) ++s.log_blocks;
+    s.rows = (int32_t)xq_cdiv(V, 1ll << s.log_blocks);
+    uint8_t* at = (uint8_t*)base;
+    auto take = [&](int64_t n) {
+        uint8_t* p = at;
+        at += (n + 255) & ~255ll;
+        return p;
+    };
+    s.start = (int32_t*)take((((int64_t)s.rows << s.log_blocks) + 1) * 4);
+    s.token = (int32_t*)take(n_tokens * 4);
+    s.part = (float*)take(n_tokens / kChunk * H * 4);
+    *bytes = at - (uint8_t*)base;
+    return s;
+}
+
+int32_t lanes_for(int64_t pieces) {
+    int32_t n = 8;
+    while (n < 256 && n < pieces) n <<= 1;
+    return n;
+}
+bool by_16(const void* p, int64_t ld, int64_t rows, int64_t H, int64_t size) { return xq_aligned(p, 16) && H * size % 16 == 0 && (rows <= 1 || ld * size % 16 == 0); }
+
+template <typename T, int W>
+void launch_fwd(const xq_embedding& q, void* out, int64_t ld_out, hipStream_t st) {
+    const int32_t lanes = lanes_for(xq_cdiv(q.H, W));
+    embedding_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(q.n_tokens, 256 / lanes), 1 << 20)), 256, 0, st>>>(q, (T*)out, ld_out, lanes);
+}
+template <typename T, int W>
+void launch_bwd(const xq_embedding& q, const Sorted& s, const void* grad, int64_t ld_grad, void* dw, int64_t ld_dw, hipStream_t st) {
+    embedding_sort_kernel<<<dim3(1u << s.log_blocks), kSortThreads, 0, st>>>(q, s);
+    if (q.n_tokens >= kChunk)
+        embedding_part_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(q.n_tokens / kChunk, 1 << 16), (unsigned)std::min<int64_t>(xq_cdiv(q.H, 256 * W), 16)), 256, 0, st>>>(
+            q, s, (const T*)grad, ld_grad);
+    const int32_t lanes = lanes_for(xq_cdiv(q.H, W));
+    embedding_grad_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(q.V, 256 / lanes), 1 << 20)), 256, 0, st>>>(q, s, (const T*)grad, ld_grad, (T*)dw, ld_dw, lanes);
 }
 
 int check_embedding(const char* who, const xq_embedding* q) {
@@ -80,14 +293,20 @@ extern "C" int xq_embedding_fwd(const xq_embedding* q, void* out, int64_t ld_out
     if (q->n_tokens == 0) return XQ_OK;
     XQ_REQUIRE(rows_ok(q->weight, q->dtype, q->V, q->ldw, q->H), "xq_embedding_fwd: the weight is NULL or misaligned, or its rows overlap");
     XQ_REQUIRE(rows_ok(out, q->dtype, q->n_tokens, ld_out, q->H), "xq_embedding_fwd: out is NULL or misaligned, or its rows overlap");
-    embedding_kernel<<<dim3((unsigned)std::min<int64_t>(q->n_tokens, 1 << 20)), 256, 0, (hipStream_t)stream>>>(*q, out, ld_out);
+    hipStream_t st = (hipStream_t)stream;
+    const int64_t size = q->dtype == XQ_DT_F32 ? 4 : 2;
+    const bool wide = by_16(q->weight, q->ldw, q->V, q->H, size) && by_16(out, ld_out, q->n_tokens, q->H, size);
+    if (size == 4) wide ? launch_fwd<float, 4>(*q, out, ld_out, st) : launch_fwd<float, 1>(*q, out, ld_out, st);
+    else wide ? launch_fwd<bf16_t, 8>(*q, out, ld_out, st) : launch_fwd<bf16_t, 1>(*q, out, ld_out, st);
     XQ_CHECK_LAUNCH("xq_embedding_fwd");
     return XQ_OK;
 }
 
 extern "C" int64_t xq_embedding_workspace_bytes(int64_t n_tokens, int64_t V, int64_t H) {
     if (n_tokens < 0 || n_tokens >= (1ll << 31) || V < 1 || V >= (1ll << 31) || H < 1 || H >= (1ll << 31)) return -1;
-    return 256;
+    int64_t bytes;
+    plan_of(nullptr, n_tokens, V, H, &bytes);
+    return bytes;
 }
 
 extern "C" int xq_embedding_bwd(const xq_embedding* q, const void* grad, int64_t ld_grad, void* dw, int64_t ld_dw, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -97,7 +316,13 @@ extern "C" int xq_embedding_bwd(const xq_embedding* q, const void* grad, int64_t
     XQ_REQUIRE(rows_ok(dw, q->dtype, q->V, ld_dw, q->H), "xq_embedding_bwd: dw is NULL or misaligned, or its rows overlap");
     const int64_t need = xq_embedding_workspace_bytes(q->n_tokens, q->V, q->H);
     XQ_REQUIRE(workspace && xq_aligned(workspace, 256) && workspace_bytes >= need, "xq_embedding_bwd: a workspace of %lld bytes, 256-byte aligned, is needed", (long long)need);
-    embedding_grad_kernel<<<dim3((unsigned)std::min<int64_t>(q->V, 1 << 20)), 256, 0, (hipStream_t)stream>>>(*q, grad, ld_grad, dw, ld_dw);
+    hipStream_t st = (hipStream_t)stream;
+    int64_t bytes;
+    const Sorted s = plan_of(workspace, q->n_tokens, q->V, q->H, &bytes);
+    const int64_t size = q->dtype == XQ_DT_F32 ? 4 : 2;
+    const bool wide = by_16(grad, ld_grad, q->n_tokens, q->H, size) && by_16(dw, ld_dw, q->V, q->H, size);
+    if (size == 4) wide ? launch_bwd<float, 4>(*q, s, grad, ld_grad, dw, ld_dw, st) : launch_bwd<float, 1>(*q, s, grad, ld_grad, dw, ld_dw, st);
+    else wide ? launch_bwd<bf16_t, 8>(*q, s, grad, ld_grad, dw, ld_dw, st) : launch_bwd<bf16_t, 1>(*q, s, grad, ld_grad, dw, ld_dw, st);
     XQ_CHECK_LAUNCH("xq_embedding_bwd");
     return XQ_OK;
 }
