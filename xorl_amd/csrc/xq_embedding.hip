@@ -32,6 +32,12 @@ __device__ __forceinline__ void store_piece(T* p, const Piece<T, W>& r) {
     if constexpr (W > 1) *(u32x4*)p = __builtin_bit_cast(u32x4, r);
     else *p = r.v[0];
 }
+// a result that nothing here reads again: past the caches
+template <typename T, int W>
+__device__ __forceinline__ void store_past(T* p, const Piece<T, W>& r) {
+    if constexpr (W > 1) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, r), (u32x4*)p);
+    else __builtin_nontemporal_store(r.v[0], p);
+}
 __device__ __forceinline__ float value(float v) { return v; }
 __device__ __forceinline__ float value(bf16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ void put(float& to, float v) { to = v; }
@@ -63,7 +69,7 @@ struct Sorted {
     float* part;              // [n_tokens / kChunk, H]: sums over kChunk tokens in that order, where they are all of one row
     int32_t log_blocks, rows;
 };
-constexpr int kChunk = 64, kSortThreads = 1024, kSortRows = 8192, kSortAtOnce = 4 * kSortThreads;
+constexpr int kChunk = 32, kSlots = 8, kSortThreads = 1024, kSortRows = 8192, kSortAtOnce = 4 * kSortThreads;
 
 // Every block looks through all ids: it counts its own rows' and those of the blocks before it, so that no launch is needed that adds
 // counts up, and places its own tokens in a second look.
@@ -165,15 +171,16 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embeddi
     }
 }
 
-template <typename T, int W>
+// `AHEAD` rows on their way at a time
+template <typename T, int W, int AHEAD>
 __device__ __forceinline__ void add_tokens(const int32_t* token, int from, int to, const T* grad, int64_t ld, int64_t h, float* sum) {
     int i = from;
-    for (; i + 4 <= to; i += 4) {
-        Piece<T, W> r[4];
+    for (; i + AHEAD <= to; i += AHEAD) {
+        Piece<T, W> r[AHEAD];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) r[u] = load_piece<T, W>(grad + token[i + u] * ld + h);
+        for (int u = 0; u < AHEAD; ++u) r[u] = load_piece<T, W>(grad + token[i + u] * ld + h);
 #pragma unroll
-        for (int u = 0; u < 4; ++u)
+        for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
             for (int j = 0; j < W; ++j) sum[j] += value(r[u].v[j]);
     }
@@ -193,37 +200,52 @@ __global__ void __launch_bounds__(256) embedding_part_kernel(xq_embedding q, Sor
         if (token_id(q, token[0]) != token_id(q, token[kChunk - 1])) continue;
         for (int64_t h = ((int64_t)blockIdx.y * 256 + threadIdx.x) * W; h < q.H; h += (int64_t)gridDim.y * 256 * W) {
             float sum[W] = {};
-            add_tokens<T, W>(token, 0, kChunk, grad, ld, h, sum);
+            add_tokens<T, W, 16>(token, 0, kChunk, grad, ld, h, sum);
 #pragma unroll
             for (int j = 0; j < W; ++j) s.part[c * q.H + h + j] = sum[j];
         }
     }
 }
 
+// kSlots rows of one sorting block after each other: one look at where their tokens begin
 template <typename T, int W>
 __global__ void __launch_bounds__(256) embedding_grad_kernel(xq_embedding q, Sorted s, const T* grad, int64_t ld, T* dw, int64_t ld_dw, int32_t lanes) {
     const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1);
-    const int64_t mask = (1 << s.log_blocks) - 1;
-    for (int64_t v = (int64_t)blockIdx.x * per + threadIdx.x / lanes; v < q.V; v += (int64_t)gridDim.x * per) {
-        const int32_t* start = s.start + (v & mask) * s.rows + (v >> s.log_blocks);
-        const int from = start[0], to = start[1];
-        // whole chunks among the row's tokens, and what lies before and behind them
-        const int c0 = (from + kChunk - 1) / kChunk, c1 = max(c0, to / kChunk);
-        for (int64_t h = lane * W; h < q.H; h += lanes * W) {
-            float sum[W] = {};
-            if (c0 < c1) {
-                add_tokens<T, W>(s.token, from, c0 * kChunk, grad, ld, h, sum);
-                for (int c = c0; c < c1; ++c)
+    const int64_t slots = (int64_t)s.rows << s.log_blocks;
+    for (int64_t p = ((int64_t)blockIdx.x * per + threadIdx.x / lanes) * kSlots; p < slots; p += (int64_t)gridDim.x * per * kSlots) {
+        int32_t at[kSlots + 1];
 #pragma unroll
-                    for (int j = 0; j < W; ++j) sum[j] += s.part[c * q.H + h + j];
-                add_tokens<T, W>(s.token, c1 * kChunk, to, grad, ld, h, sum);
-            } else {
-                add_tokens<T, W>(s.token, from, to, grad, ld, h, sum);
+        for (int i = 0; i < kSlots; i += 4) {
+            const u32x4 four = *(const u32x4*)(s.start + p + i);
+#pragma unroll
+            for (int j = 0; j < 4; ++j) at[i + j] = (int32_t)four[j];
+        }
+        at[kSlots] = s.start[p + kSlots];
+        int64_t block = p / s.rows, row = p - block * s.rows;
+#pragma unroll
+        for (int i = 0; i < kSlots; ++i, ++row) {
+            if (row == s.rows) { row = 0; ++block; }
+            const int64_t v = (row << s.log_blocks) + block;
+            if (v >= q.V) continue;
+            const int from = at[i], to = at[i + 1];
+            // whole chunks among the row's tokens, and what lies before and behind them
+            const int c0 = (from + kChunk - 1) / kChunk, c1 = max(c0, to / kChunk);
+            for (int64_t h = lane * W; h < q.H; h += lanes * W) {
+                float sum[W] = {};
+                if (from < to) {
+                    add_tokens<T, W, 4>(s.token, from, c0 < c1 ? c0 * kChunk : to, grad, ld, h, sum);
+                    if (c0 < c1) {
+                        for (int c = c0; c < c1; ++c)
+#pragma unroll
+                            for (int j = 0; j < W; ++j) sum[j] += s.part[c * q.H + h + j];
+                        add_tokens<T, W, 4>(s.token, c1 * kChunk, to, grad, ld, h, sum);
+                    }
+                }
+                Piece<T, W> r;
+#pragma unroll
+                for (int j = 0; j < W; ++j) put(r.v[j], q.scale * sum[j]);
+                store_past<T, W>(dw + v * ld_dw + h, r);
             }
-            Piece<T, W> r;
-#pragma unroll
-            for (int j = 0; j < W; ++j) put(r.v[j], q.scale * sum[j]);
-            store_piece<T, W>(dw + v * ld_dw + h, r);
         }
     }
 }
@@ -266,7 +288,7 @@ void launch_bwd(const xq_embedding& q, const Sorted& s, const void* grad, int64_
         embedding_part_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(q.n_tokens / kChunk, 1 << 16), (unsigned)std::min<int64_t>(xq_cdiv(q.H, 256 * W), 16)), 256, 0, st>>>(
             q, s, (const T*)grad, ld_grad);
     const int32_t lanes = lanes_for(xq_cdiv(q.H, W));
-    embedding_grad_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(q.V, 256 / lanes), 1 << 20)), 256, 0, st>>>(q, s, (const T*)grad, ld_grad, (T*)dw, ld_dw, lanes);
+    embedding_grad_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(((int64_t)s.rows << s.log_blocks) / kSlots, 256 / lanes), 1 << 20)), 256, 0, st>>>(q, s, (const T*)grad, ld_grad, (T*)dw, ld_dw, lanes);
 }
 
 int check_embedding(const char* who, const xq_embedding* q) {
