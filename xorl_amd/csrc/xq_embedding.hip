@@ -71,45 +71,88 @@ struct Sorted {
 };
 constexpr int kChunk = 32, kSlots = 8, kSortThreads = 1024, kSortRows = 8192, kSortAtOnce = 4 * kSortThreads;
 
-// Every block looks through all ids: it counts its own rows' and those of the blocks before it, so that no launch is needed that adds
-// counts up, and places its own tokens in a second look.
+// The tokens of a list that belong to one row, among 64 of them: those whose row agrees in every bit.  One wave puts them in their places.
+__device__ __forceinline__ void place_tokens(const uint16_t* row, const int32_t* token, int n, int bits, int32_t* next, int32_t* out) {
+    const int lane = threadIdx.x & 63;
+    for (int i = lane; i - lane < n; i += 64) {
+        const bool is = i < n;
+        const int r = is ? row[i] : 0;
+        uint64_t same = __ballot(is);
+        for (int b = 0; b < bits; ++b) {
+            const bool bit = (r >> b) & 1;
+            const uint64_t m = __ballot(bit);
+            same &= bit ? m : ~m;
+        }
+        const int rank = __popcll(same & ((1ull << lane) - 1));
+        if (is) {
+            const int base = next[r];
+            out[base + rank] = token[i];
+            if (rank == __popcll(same) - 1) next[r] = base + rank + 1;
+        }
+    }
+}
+
+// Every block looks through all ids: it counts its own rows' tokens, and those of the blocks before it, so that no launch is needed that adds counts
+// up, and lists its own.  More of them than the list holds (a token that fills a batch) are found again in a second look.
 __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embedding q, Sorted s) {
-    __shared__ int32_t count[kSortRows], of_wave[16], token[kSortAtOnce];
+    __shared__ int32_t count[kSortRows], of_wave[2][16], token[kSortAtOnce];
     __shared__ uint16_t row[kSortAtOnce];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, block = blockIdx.x;
     const int64_t mask = (1 << s.log_blocks) - 1;
-    auto real = [&](int64_t id) { return id >= 0 && id < q.V && id != q.padding_idx; };
+    auto sum_up = [&](int v, int* all, int turn) {          // the values of the threads before this one, and all threads'; one barrier, two turns
+        int upto = v;
+        for (int o = 1; o < 64; o <<= 1) {
+            const int u = __shfl_up(upto, o, 64);
+            if (lane >= o) upto += u;
+        }
+        if (lane == 63) of_wave[turn][wave] = upto;
+        __syncthreads();
+        int to = upto - v, sum = 0;
+#pragma unroll
+        for (int w = 0; w < 16; ++w) {
+            const int n = of_wave[turn][w];
+            to += w < wave ? n : 0;
+            sum += n;
+        }
+        *all = sum;
+        return to;
+    };
     for (int r = tid; r < s.rows; r += kSortThreads) count[r] = 0;
     __syncthreads();
-    int before = 0;
-    for (int64_t t = tid; t < q.n_tokens; t += kSortThreads) {
-        const int64_t id = token_id(q, t);
-        const int at = (int)(id & mask);
-        before += real(id) && at < block;
-        if (real(id) && at == block) atomicAdd(&count[id >> s.log_blocks], 1);
+    int before = 0, listed = 0, turn = 0;
+    for (int64_t t0 = 0; t0 < q.n_tokens; t0 += kSortAtOnce, turn ^= 1) {
+        // four tokens a thread, so that the block's come in order
+        int own[4], n = 0, found;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const int64_t t = t0 + tid * 4 + i, id = t < q.n_tokens ? token_id(q, t) : -1;
+            const bool real = id >= 0 && id < q.V && id != q.padding_idx;
+            const int at = (int)(id & mask);
+            before += real && at < block;
+            own[i] = real && at == block ? (int)(id >> s.log_blocks) : -1;
+            if (own[i] >= 0) atomicAdd(&count[own[i]], 1);
+            n += own[i] >= 0;
+        }
+        int to = listed + sum_up(n, &found, turn);
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            if (own[i] >= 0) {
+                if (to < kSortAtOnce) {
+                    row[to] = (uint16_t)own[i];
+                    token[to] = (int)(t0 + tid * 4 + i);
+                }
+                ++to;
+            }
+        listed += found;
     }
-    for (int o = 32; o; o >>= 1) before += __shfl_xor(before, o, 64);
-    if (lane == 0) of_wave[wave] = before;
-    __syncthreads();
-    before = 0;
-    for (int w = 0; w < 16; ++w) before += of_wave[w];
-    __syncthreads();
-    // counts to places: each thread the rows it owns, then the threads before it
-    const int own = (s.rows + kSortThreads - 1) / kSortThreads, first = tid * own, last = min(first + own, s.rows);
-    int mine = 0;
+    sum_up(before, &before, turn);
+    turn ^= 1;
+    // counts to places: each thread the rows it owns
+    const int each = (s.rows + kSortThreads - 1) / kSortThreads, first = tid * each, last = min(first + each, s.rows);
+    int mine = 0, all;
     for (int r = first; r < last; ++r) mine += count[r];
-    int upto = mine;
-    for (int o = 1; o < 64; o <<= 1) {
-        const int u = __shfl_up(upto, o, 64);
-        if (lane >= o) upto += u;
-    }
-    if (lane == 63) of_wave[wave] = upto;
-    __syncthreads();
-    int at = before + upto - mine, all = 0;
-    for (int w = 0; w < 16; ++w) {
-        at += w < wave ? of_wave[w] : 0;
-        all += of_wave[w];
-    }
+    int at = before + sum_up(mine, &all, turn);
+    turn ^= 1;
     for (int r = first; r < last; ++r) {
         const int n = count[r];
         count[r] = at;
@@ -117,57 +160,31 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embeddi
         at += n;
     }
     if (block == (int)mask && tid == 0) s.start[(int64_t)(block + 1) * s.rows] = before + all;
-    if (all == 0) return;
+    if (listed == 0) return;
     int bits = 0;
     while ((1 << bits) < s.rows) ++bits;
-    for (int64_t t0 = 0; t0 < q.n_tokens; t0 += kSortAtOnce) {
-        // four tokens a thread, so that the block's come in order
-        int own_row[4], n = 0;
+    __syncthreads();
+    if (listed <= kSortAtOnce) {
+        if (wave == 0) place_tokens(row, token, listed, bits, count, s.token);
+        return;
+    }
+    for (int64_t t0 = 0; t0 < q.n_tokens; t0 += kSortAtOnce, turn ^= 1) {
+        int own[4], n = 0, found;
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             const int64_t t = t0 + tid * 4 + i, id = t < q.n_tokens ? token_id(q, t) : -1;
-            own_row[i] = real(id) && (int)(id & mask) == block ? (int)(id >> s.log_blocks) : -1;
-            n += own_row[i] >= 0;
+            own[i] = id >= 0 && id < q.V && id != q.padding_idx && (int)(id & mask) == block ? (int)(id >> s.log_blocks) : -1;
+            n += own[i] >= 0;
         }
-        int to = n;
-        for (int o = 1; o < 64; o <<= 1) {
-            const int u = __shfl_up(to, o, 64);
-            if (lane >= o) to += u;
-        }
-        __syncthreads();                                   // (the places of the round before have been read)
-        if (lane == 63) of_wave[wave] = to;
-        __syncthreads();
-        to -= n;
-        int found = 0;
-        for (int w = 0; w < 16; ++w) {
-            to += w < wave ? of_wave[w] : 0;
-            found += of_wave[w];
-        }
+        int to = sum_up(n, &found, turn);                  // (behind its barrier the list of the round before has been read)
 #pragma unroll
         for (int i = 0; i < 4; ++i)
-            if (own_row[i] >= 0) {
-                row[to] = (uint16_t)own_row[i];
+            if (own[i] >= 0) {
+                row[to] = (uint16_t)own[i];
                 token[to++] = (int)(t0 + tid * 4 + i);
             }
         __syncthreads();
-        if (wave == 0)
-            for (int i0 = 0; i0 < found; i0 += 64) {
-                // the tokens of one row among 64: those whose row agrees in every bit
-                const bool is = i0 + lane < found;
-                const int r = is ? row[i0 + lane] : 0;
-                uint64_t same = __ballot(is);
-                for (int b = 0; b < bits; ++b) {
-                    const bool bit = (r >> b) & 1;
-                    const uint64_t m = __ballot(bit);
-                    same &= bit ? m : ~m;
-                }
-                const int rank = __popcll(same & ((1ull << lane) - 1));
-                if (is) {
-                    const int base = count[r];
-                    s.token[base + rank] = token[i0 + lane];
-                    if (rank == __popcll(same) - 1) count[r] = base + rank + 1;
-                }
-            }
+        if (wave == 0) place_tokens(row, token, found, bits, count, s.token);
     }
 }
 
