@@ -32,49 +32,57 @@ __device__ __forceinline__ void store_piece(T* p, const Piece<T, W>& r) {
     if constexpr (W > 1) *(u32x4*)p = __builtin_bit_cast(u32x4, r);
     else *p = r.v[0];
 }
-// a result that nothing here reads again: past the caches
-template <typename T, int W>
-__device__ __forceinline__ void store_past(T* p, const Piece<T, W>& r) {
-    if constexpr (W > 1) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, r), (u32x4*)p);
-    else __builtin_nontemporal_store(r.v[0], p);
-}
 __device__ __forceinline__ float value(float v) { return v; }
 __device__ __forceinline__ float value(bf16_t v) { return bf16_to_f32(v); }
 __device__ __forceinline__ void put(float& to, float v) { to = v; }
 __device__ __forceinline__ void put(bf16_t& to, float v) { to = to_bf16(v); }
 
-// out[t] = scale W[id]: `lanes` threads a token
-template <typename T, int W>
+// out[t] = scale W[id]: `lanes` threads U tokens after each other, whose rows are on their way together (16385 rows of 2048 bf16: 25.4 us one by one, 21.0 by four)
+template <typename T, int W, int U>
 __global__ void __launch_bounds__(256) embedding_kernel(xq_embedding q, T* out, int64_t ld_out, int32_t lanes) {
     const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1);
-    for (int64_t t = (int64_t)blockIdx.x * per + threadIdx.x / lanes; t < q.n_tokens; t += (int64_t)gridDim.x * per) {
-        const int64_t id = token_id(q, t);
-        const bool is = id >= 0 && id < q.V;
-        const T* from = (const T*)q.weight + (is ? id : 0) * q.ldw;
-        T* to = out + t * ld_out;
-        for (int64_t h = lane * W; h < q.H; h += lanes * W) {
-            Piece<T, W> r = load_piece<T, W>(from + h);
+    for (int64_t t0 = ((int64_t)blockIdx.x * per + threadIdx.x / lanes) * U; t0 < q.n_tokens; t0 += (int64_t)gridDim.x * per * U) {
+        int64_t id[U];
+        bool is[U];
 #pragma unroll
-            for (int i = 0; i < W; ++i) put(r.v[i], is ? q.scale * value(r.v[i]) : NAN);
-            store_piece<T, W>(to + h, r);
+        for (int u = 0; u < U; ++u) id[u] = token_id(q, min(t0 + u, q.n_tokens - 1));
+#pragma unroll
+        for (int u = 0; u < U; ++u) {
+            is[u] = id[u] >= 0 && id[u] < q.V;
+            if (!is[u]) id[u] = 0;
+        }
+        for (int64_t h = lane * W; h < q.H; h += lanes * W) {
+            Piece<T, W> r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u] = load_piece<T, W>((const T*)q.weight + id[u] * q.ldw + h);
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+#pragma unroll
+                for (int i = 0; i < W; ++i) put(r[u].v[i], is[u] ? q.scale * value(r[u].v[i]) : NAN);
+                if (t0 + u < q.n_tokens) store_piece<T, W>(out + (t0 + u) * ld_out + h, r[u]);
+            }
         }
     }
 }
 
 // ---- the gradient: tokens sorted by id (stable), then a pass over the vocabulary that adds each row's tokens or writes its zeros
 // Row v belongs to block v % blocks, as its row v / blocks: ids that come often lie next to each other in a vocabulary, and so go to different blocks.
+typedef __attribute__((ext_vector_type(2))) int32_t i32x2;
+
 struct Sorted {
     int32_t* start;           // [blocks * rows + 1]: where the tokens of a row begin in token[], by (v % blocks) * rows + v / blocks
-    int32_t* token;           // [n_tokens]: the tokens, row by row, each row's in their order
+    i32x2* token;             // [n_tokens]: the tokens and their ids, row by row, each row's in their order
     float* part;              // [n_tokens / kChunk, H]: sums over kChunk tokens in that order, where they are all of one row
     int32_t log_blocks, rows;
 };
-constexpr int kChunk = 32, kSlots = 8, kSortThreads = 1024, kSortRows = 8192, kSortAtOnce = 4 * kSortThreads;
+constexpr int kChunk = 16, kSlots = 8, kSortRows = 4096, kSortList = 3072, kSortEach = 8, kSortAtOnce = 256 * kSortEach;      // (list and counters: 35 KB, four blocks a unit)
 
-// The tokens of a list that belong to one row, among 64 of them: those whose row agrees in every bit.  One wave puts them in their places.
-__device__ __forceinline__ void place_tokens(const uint16_t* row, const int32_t* token, int n, int bits, int32_t* next, int32_t* out) {
-    const int lane = threadIdx.x & 63;
-    for (int i = lane; i - lane < n; i += 64) {
+// The tokens of a list go to their places, `next` of their row: 256 at a time, each wave's 64 ranked among themselves (those of one row agree in every bit
+// of it), then the waves take their places in turn.
+__device__ __forceinline__ void place_tokens(const uint16_t* row, const int32_t* token, int n, int bits, int32_t* next, const Sorted& s) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int i0 = 0; i0 < n; i0 += 256) {
+        const int i = i0 + threadIdx.x;
         const bool is = i < n;
         const int r = is ? row[i] : 0;
         uint64_t same = __ballot(is);
@@ -84,21 +92,32 @@ __device__ __forceinline__ void place_tokens(const uint16_t* row, const int32_t*
             same &= bit ? m : ~m;
         }
         const int rank = __popcll(same & ((1ull << lane) - 1));
-        if (is) {
-            const int base = next[r];
-            out[base + rank] = token[i];
-            if (rank == __popcll(same) - 1) next[r] = base + rank + 1;
+        int at = 0;
+        for (int w = 0; w < 4 && i0 + w * 64 < n; ++w) {
+            if (wave == w && is) {
+                at = next[r] + rank;
+                if (rank == __popcll(same) - 1) next[r] = at + 1;
+            }
+            __syncthreads();
         }
+        if (is) s.token[at] = i32x2{token[i], (r << s.log_blocks) + (int)blockIdx.x};
     }
 }
 
-// Every block looks through all ids: it counts its own rows' tokens, and those of the blocks before it, so that no launch is needed that adds counts
+// Every sorting block looks through all ids: it counts its own rows' tokens, and those of the blocks before it, so that no launch is needed that adds counts
 // up, and lists its own.  More of them than the list holds (a token that fills a batch) are found again in a second look.
-__global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embedding q, Sorted s) {
-    __shared__ int32_t count[kSortRows], of_wave[2][16], token[kSortAtOnce];
-    __shared__ uint16_t row[kSortAtOnce];
+// Blocks behind the sorting ones write zeros, 16 bytes a thread in the order of addresses: 1 GiB takes 150 us with four blocks on a unit, 175 to 240 in any
+// other order that was tried (several pieces a thread, a share of the rows a block); the sort (8192 ids 9 us by itself) goes on beside them.
+__global__ void __launch_bounds__(256) embedding_sort_kernel(xq_embedding q, Sorted s, u32x4* zeros, int64_t n_zeros) {
+    __shared__ int32_t count[kSortRows], of_wave[2][4], token[kSortList];
+    __shared__ uint16_t row[kSortList];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6, block = blockIdx.x;
     const int64_t mask = (1 << s.log_blocks) - 1;
+    if (block > (int)mask) {
+        const int64_t stride = ((int64_t)gridDim.x - mask - 1) * 256;
+        for (int64_t i = ((int64_t)block - mask - 1) * 256 + tid; i < n_zeros; i += stride) zeros[i] = u32x4{0, 0, 0, 0};
+        return;
+    }
     auto sum_up = [&](int v, int* all, int turn) {          // the values of the threads before this one, and all threads'; one barrier, two turns
         int upto = v;
         for (int o = 1; o < 64; o <<= 1) {
@@ -109,7 +128,7 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embeddi
         __syncthreads();
         int to = upto - v, sum = 0;
 #pragma unroll
-        for (int w = 0; w < 16; ++w) {
+        for (int w = 0; w < 4; ++w) {
             const int n = of_wave[turn][w];
             to += w < wave ? n : 0;
             sum += n;
@@ -117,38 +136,39 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embeddi
         *all = sum;
         return to;
     };
-    for (int r = tid; r < s.rows; r += kSortThreads) count[r] = 0;
+    for (int r = tid; r < s.rows; r += 256) count[r] = 0;
     __syncthreads();
     int before = 0, listed = 0, turn = 0;
     for (int64_t t0 = 0; t0 < q.n_tokens; t0 += kSortAtOnce, turn ^= 1) {
-        // four tokens a thread, so that the block's come in order
-        int own[4], n = 0, found;
+        // consecutive tokens a thread, so that the block's come in order
+        int own[kSortEach], n = 0, found;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t t = t0 + tid * 4 + i, id = t < q.n_tokens ? token_id(q, t) : -1;
+        for (int i = 0; i < kSortEach; ++i) {
+            const int64_t t = t0 + tid * kSortEach + i, id = t < q.n_tokens ? token_id(q, t) : -1;
             const bool real = id >= 0 && id < q.V && id != q.padding_idx;
             const int at = (int)(id & mask);
             before += real && at < block;
             own[i] = real && at == block ? (int)(id >> s.log_blocks) : -1;
-            if (own[i] >= 0) atomicAdd(&count[own[i]], 1);
             n += own[i] >= 0;
         }
         int to = listed + sum_up(n, &found, turn);
+        if (n)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
-            if (own[i] >= 0) {
-                if (to < kSortAtOnce) {
-                    row[to] = (uint16_t)own[i];
-                    token[to] = (int)(t0 + tid * 4 + i);
+            for (int i = 0; i < kSortEach; ++i)
+                if (own[i] >= 0) {
+                    atomicAdd(&count[own[i]], 1);
+                    if (to < kSortList) {
+                        row[to] = (uint16_t)own[i];
+                        token[to] = (int)(t0 + tid * kSortEach + i);
+                    }
+                    ++to;
                 }
-                ++to;
-            }
         listed += found;
     }
     sum_up(before, &before, turn);
     turn ^= 1;
     // counts to places: each thread the rows it owns
-    const int each = (s.rows + kSortThreads - 1) / kSortThreads, first = tid * each, last = min(first + each, s.rows);
+    const int each = (s.rows + 255) / 256, first = tid * each, last = min(first + each, s.rows);
     int mine = 0, all;
     for (int r = first; r < last; ++r) mine += count[r];
     int at = before + sum_up(mine, &all, turn);
@@ -164,45 +184,45 @@ __global__ void __launch_bounds__(kSortThreads) embedding_sort_kernel(xq_embeddi
     int bits = 0;
     while ((1 << bits) < s.rows) ++bits;
     __syncthreads();
-    if (listed <= kSortAtOnce) {
-        if (wave == 0) place_tokens(row, token, listed, bits, count, s.token);
+    if (listed <= kSortList) {
+        place_tokens(row, token, listed, bits, count, s);
         return;
     }
     for (int64_t t0 = 0; t0 < q.n_tokens; t0 += kSortAtOnce, turn ^= 1) {
-        int own[4], n = 0, found;
+        int own[kSortEach], n = 0, found;
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const int64_t t = t0 + tid * 4 + i, id = t < q.n_tokens ? token_id(q, t) : -1;
+        for (int i = 0; i < kSortEach; ++i) {
+            const int64_t t = t0 + tid * kSortEach + i, id = t < q.n_tokens ? token_id(q, t) : -1;
             own[i] = id >= 0 && id < q.V && id != q.padding_idx && (int)(id & mask) == block ? (int)(id >> s.log_blocks) : -1;
             n += own[i] >= 0;
         }
         int to = sum_up(n, &found, turn);                  // (behind its barrier the list of the round before has been read)
 #pragma unroll
-        for (int i = 0; i < 4; ++i)
+        for (int i = 0; i < kSortEach; ++i)
             if (own[i] >= 0) {
                 row[to] = (uint16_t)own[i];
-                token[to++] = (int)(t0 + tid * 4 + i);
+                token[to++] = (int)(t0 + tid * kSortEach + i);
             }
         __syncthreads();
-        if (wave == 0) place_tokens(row, token, found, bits, count, s.token);
+        place_tokens(row, token, found, bits, count, s);
     }
 }
 
 // `AHEAD` rows on their way at a time
 template <typename T, int W, int AHEAD>
-__device__ __forceinline__ void add_tokens(const int32_t* token, int from, int to, const T* grad, int64_t ld, int64_t h, float* sum) {
+__device__ __forceinline__ void add_tokens(const i32x2* token, int from, int to, const T* grad, int64_t ld, int64_t h, float* sum) {
     int i = from;
     for (; i + AHEAD <= to; i += AHEAD) {
         Piece<T, W> r[AHEAD];
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) r[u] = load_piece<T, W>(grad + token[i + u] * ld + h);
+        for (int u = 0; u < AHEAD; ++u) r[u] = load_piece<T, W>(grad + token[i + u][0] * ld + h);
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u)
 #pragma unroll
             for (int j = 0; j < W; ++j) sum[j] += value(r[u].v[j]);
     }
     for (; i < to; ++i) {
-        const Piece<T, W> r = load_piece<T, W>(grad + token[i] * ld + h);
+        const Piece<T, W> r = load_piece<T, W>(grad + token[i][0] * ld + h);
 #pragma unroll
         for (int j = 0; j < W; ++j) sum[j] += value(r.v[j]);
     }
@@ -213,20 +233,89 @@ template <typename T, int W>
 __global__ void __launch_bounds__(256) embedding_part_kernel(xq_embedding q, Sorted s, const T* grad, int64_t ld) {
     const int64_t all = s.start[(int64_t)s.rows << s.log_blocks];
     for (int64_t c = blockIdx.x; (c + 1) * kChunk <= all; c += gridDim.x) {
-        const int32_t* token = s.token + c * kChunk;
-        if (token_id(q, token[0]) != token_id(q, token[kChunk - 1])) continue;
+        const i32x2* token = s.token + c * kChunk;
+        if (token[0][1] != token[kChunk - 1][1]) continue;
         for (int64_t h = ((int64_t)blockIdx.y * 256 + threadIdx.x) * W; h < q.H; h += (int64_t)gridDim.y * 256 * W) {
             float sum[W] = {};
-            add_tokens<T, W, 16>(token, 0, kChunk, grad, ld, h, sum);
+            add_tokens<T, W, kChunk>(token, 0, kChunk, grad, ld, h, sum);
 #pragma unroll
             for (int j = 0; j < W; ++j) s.part[c * q.H + h + j] = sum[j];
         }
     }
 }
 
-// kSlots rows of one sorting block after each other: one look at where their tokens begin
+// the tokens [from, to) of a row: those before its first whole chunk and behind its last one by one
 template <typename T, int W>
+__device__ __forceinline__ void add_row(const Sorted& s, int from, int to, const T* grad, int64_t ld, int64_t H, int64_t h, float* sum) {
+    const int c0 = (from + kChunk - 1) / kChunk, c1 = max(c0, to / kChunk);
+    add_tokens<T, W, 4>(s.token, from, c0 < c1 ? c0 * kChunk : to, grad, ld, h, sum);
+    if (c0 == c1) return;
+    for (int c = c0; c < c1; c += 8) {
+        Piece<float, (W > 1 ? 4 : 1)> r[8][W > 1 ? W / 4 : 1];
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int j = 0; j < (W > 1 ? W / 4 : 1); ++j) r[u][j] = load_piece<float, (W > 1 ? 4 : 1)>(s.part + min(c + u, c1 - 1) * H + h + 4 * j);
+#pragma unroll
+        for (int u = 0; u < 8; ++u)
+#pragma unroll
+            for (int j = 0; j < W; ++j) sum[j] += c + u < c1 ? r[u][j / 4].v[j % 4] : 0.0f;
+    }
+    add_tokens<T, W, 4>(s.token, c1 * kChunk, to, grad, ld, h, sum);
+}
+
+template <typename T, int W, bool PAST = false>
+__device__ __forceinline__ void store_sum(T* to, float scale, const float* sum) {
+    Piece<T, W> r;
+#pragma unroll
+    for (int j = 0; j < W; ++j) put(r.v[j], scale * sum[j]);
+    if constexpr (PAST && W > 1) __builtin_nontemporal_store(__builtin_bit_cast(u32x4, r), (u32x4*)to);
+    else store_piece<T, W>(to, r);
+}
+
+// Rows that have tokens, where the others hold their zeros already: `lanes` threads U sorted tokens after each other, whose gradients are on their way
+// together.  A row is finished where its first token is.
+template <typename T, int W, int U>
 __global__ void __launch_bounds__(256) embedding_grad_kernel(xq_embedding q, Sorted s, const T* grad, int64_t ld, T* dw, int64_t ld_dw, int32_t lanes) {
+    const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1);
+    const int64_t n = s.start[(int64_t)s.rows << s.log_blocks];
+    for (int64_t i0 = ((int64_t)blockIdx.x * per + threadIdx.x / lanes) * U; i0 < n; i0 += (int64_t)gridDim.x * per * U) {
+        i32x2 token[U + 2];                                // one before and one behind (ids are not negative: -1 is no row)
+        token[0] = i0 > 0 ? s.token[i0 - 1] : i32x2{0, -1};
+#pragma unroll
+        for (int u = 1; u < U + 2; ++u) token[u] = i0 + u - 1 < n ? s.token[i0 + u - 1] : i32x2{0, -1};
+        for (int64_t h = lane * W; h < q.H; h += lanes * W) {
+            Piece<T, W> r[U];
+#pragma unroll
+            for (int u = 0; u < U; ++u) r[u] = load_piece<T, W>(grad + token[u + 1][0] * ld + h);
+            float sum[W];
+            bool own = false;                              // whether the row's first token is among these
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+                const int id = token[u + 1][1];
+                if (id < 0) break;
+                if (token[u][1] != id) {
+                    own = true;
+#pragma unroll
+                    for (int j = 0; j < W; ++j) sum[j] = 0.0f;
+                }
+                if (!own) continue;
+#pragma unroll
+                for (int j = 0; j < W; ++j) sum[j] += value(r[u].v[j]);
+                if (token[u + 2][1] == id && u < U - 1) continue;
+                if (token[u + 2][1] == id) {
+                    const int end = s.start[(int64_t)(id & ((1 << s.log_blocks) - 1)) * s.rows + (id >> s.log_blocks) + 1];
+                    add_row<T, W>(s, (int)i0 + U, end, grad, ld, q.H, h, sum);
+                }
+                store_sum<T, W>(dw + id * ld_dw + h, q.scale, sum);
+            }
+        }
+    }
+}
+
+// All rows: `lanes` threads kSlots of one sorting block after each other, whose tokens' places they look up together.
+template <typename T, int W>
+__global__ void __launch_bounds__(256) embedding_grad_rows_kernel(xq_embedding q, Sorted s, const T* grad, int64_t ld, T* dw, int64_t ld_dw, int32_t lanes) {
     const int per = 256 / lanes, lane = threadIdx.x & (lanes - 1);
     const int64_t slots = (int64_t)s.rows << s.log_blocks;
     for (int64_t p = ((int64_t)blockIdx.x * per + threadIdx.x / lanes) * kSlots; p < slots; p += (int64_t)gridDim.x * per * kSlots) {
@@ -244,28 +333,19 @@ __global__ void __launch_bounds__(256) embedding_grad_kernel(xq_embedding q, Sor
             if (row == s.rows) { row = 0; ++block; }
             const int64_t v = (row << s.log_blocks) + block;
             if (v >= q.V) continue;
-            const int from = at[i], to = at[i + 1];
-            // whole chunks among the row's tokens, and what lies before and behind them
-            const int c0 = (from + kChunk - 1) / kChunk, c1 = max(c0, to / kChunk);
             for (int64_t h = lane * W; h < q.H; h += lanes * W) {
                 float sum[W] = {};
-                if (from < to) {
-                    add_tokens<T, W, 4>(s.token, from, c0 < c1 ? c0 * kChunk : to, grad, ld, h, sum);
-                    if (c0 < c1) {
-                        for (int c = c0; c < c1; ++c)
-#pragma unroll
-                            for (int j = 0; j < W; ++j) sum[j] += s.part[c * q.H + h + j];
-                        add_tokens<T, W, 4>(s.token, c1 * kChunk, to, grad, ld, h, sum);
-                    }
-                }
-                Piece<T, W> r;
-#pragma unroll
-                for (int j = 0; j < W; ++j) put(r.v[j], q.scale * sum[j]);
-                store_past<T, W>(dw + v * ld_dw + h, r);
+                if (at[i] < at[i + 1]) add_row<T, W>(s, at[i], at[i + 1], grad, ld, q.H, h, sum);
+                store_sum<T, W, true>(dw + v * ld_dw + h, q.scale, sum);
             }
         }
     }
 }
+
+// Gradients from 256 MiB on (what the memory-side cache holds) whose rows mostly have no token get their zeros first, in the order of addresses beside the sort, at
+// 7 TB/s; others are gone through row by row, at 5.  us with forward, zeros first / row by row: 8192 tokens, [131072, 4096] bf16 231 / 287, [65536, 4096] 159 / 172,
+// [65536, 2048] 83 / 94, 1000 tokens, [131072, 2048] 100 / 119; below: 4000, [60000, 2048] 71 / 71, 4001, [32003, 2048] fp32 90 / 83.
+constexpr int64_t kFillBytes = 256ll << 20;
 
 // the sorting blocks: 256 of them, more where one would own more rows than fit its counters
 Sorted plan_of(void* base, int64_t n_tokens, int64_t V, int64_t H, int64_t* bytes) {
@@ -280,7 +360,7 @@ Sorted plan_of(void* base, int64_t n_tokens, int64_t V, int64_t H, int64_t* byte
         return p;
     };
     s.start = (int32_t*)take((((int64_t)s.rows << s.log_blocks) + 1) * 4);
-    s.token = (int32_t*)take(n_tokens * 4);
+    s.token = (i32x2*)take(n_tokens * 8);
     s.part = (float*)take(n_tokens / kChunk * H * 4);
     *bytes = at - (uint8_t*)base;
     return s;
@@ -293,19 +373,29 @@ int32_t lanes_for(int64_t pieces) {
 }
 bool by_16(const void* p, int64_t ld, int64_t rows, int64_t H, int64_t size) { return xq_aligned(p, 16) && H * size % 16 == 0 && (rows <= 1 || ld * size % 16 == 0); }
 
+// (items of `lanes` threads four at a time where that leaves four blocks and more for every compute unit)
 template <typename T, int W>
 void launch_fwd(const xq_embedding& q, void* out, int64_t ld_out, hipStream_t st) {
     const int32_t lanes = lanes_for(xq_cdiv(q.H, W));
-    embedding_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(q.n_tokens, 256 / lanes), 1 << 20)), 256, 0, st>>>(q, (T*)out, ld_out, lanes);
+    const int64_t blocks = xq_cdiv(q.n_tokens, 256 / lanes);
+    if (blocks >= 4096) embedding_kernel<T, W, 4><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(blocks, 4), 1 << 20)), 256, 0, st>>>(q, (T*)out, ld_out, lanes);
+    else embedding_kernel<T, W, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(q, (T*)out, ld_out, lanes);
 }
 template <typename T, int W>
 void launch_bwd(const xq_embedding& q, const Sorted& s, const void* grad, int64_t ld_grad, void* dw, int64_t ld_dw, hipStream_t st) {
-    embedding_sort_kernel<<<dim3(1u << s.log_blocks), kSortThreads, 0, st>>>(q, s);
+    const int64_t bytes = q.V * q.H * (int64_t)sizeof(T);
+    const bool filled = W > 1 && q.n_tokens < q.V / 2 && bytes >= kFillBytes && (ld_dw == q.H || q.V == 1);
+    const unsigned sorts = 1u << s.log_blocks;
+    embedding_sort_kernel<<<dim3(sorts + (filled ? (unsigned)std::min<int64_t>(xq_cdiv(bytes, 4096), (1 << 23)) : 0u)), 256, 0, st>>>(q, s, (u32x4*)dw, filled ? bytes / 16 : 0);
     if (q.n_tokens >= kChunk)
         embedding_part_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(q.n_tokens / kChunk, 1 << 16), (unsigned)std::min<int64_t>(xq_cdiv(q.H, 256 * W), 16)), 256, 0, st>>>(
             q, s, (const T*)grad, ld_grad);
     const int32_t lanes = lanes_for(xq_cdiv(q.H, W));
-    embedding_grad_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(((int64_t)s.rows << s.log_blocks) / kSlots, 256 / lanes), 1 << 20)), 256, 0, st>>>(q, s, (const T*)grad, ld_grad, (T*)dw, ld_dw, lanes);
+    const int64_t rows = filled ? q.n_tokens : ((int64_t)s.rows << s.log_blocks) / kSlots, blocks = xq_cdiv(rows, 256 / lanes);
+    const T* g = (const T*)grad;
+    if (!filled) embedding_grad_rows_kernel<T, W><<<dim3((unsigned)std::min<int64_t>(blocks, 1 << 20)), 256, 0, st>>>(q, s, g, ld_grad, (T*)dw, ld_dw, lanes);
+    else if (blocks >= 4096) embedding_grad_kernel<T, W, 4><<<dim3((unsigned)std::min<int64_t>(xq_cdiv(blocks, 4), 1 << 20)), 256, 0, st>>>(q, s, g, ld_grad, (T*)dw, ld_dw, lanes);
+    else if (blocks > 0) embedding_grad_kernel<T, W, 1><<<dim3((unsigned)blocks), 256, 0, st>>>(q, s, g, ld_grad, (T*)dw, ld_dw, lanes);
 }
 
 int check_embedding(const char* who, const xq_embedding* q) {
