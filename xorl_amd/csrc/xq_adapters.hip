@@ -7,50 +7,356 @@
 namespace xq {
 namespace {
 
+// Two launches: t = x A_a^T in parts of K, fp32, to the workspace; then out = base + (s t) B_a^T.  Both multiply on 16x16x32 MFMA tiles straight from memory:
+// all four operands have the contraction along their rows, so that a lane's eight elements are one 16-byte load.  t goes into the second product as two bf16
+// numbers (16 bits: one would lose as much of a large update as the result's own rounding), laid out along the contraction: lanes 0-31 hold the high
+// halves of 16 ranks, lanes 32-63 the low ones, and B's 16 ranks stand in both, so that 16 ranks are one MFMA.  fp32 factors are two bf16 numbers in the same way.
+//
+// A tile is rows of one adapter.  Up to kLeaderRows rows in any order: tile b belongs to the row b if that is the first, 17th, 33rd .. of its adapter, and its
+// block finds the rows itself among the ids (no launch that sorts them).  More rows are taken in windows of 16 or 64 that follow each other, and a window once for
+// every adapter in it: of prompts' rows, each window has one or two.
+constexpr int kLeaderRows = 1024;
+constexpr int kMostParts = 16;
+
+struct AdapterPlan {
+    int32_t leaders;      // tiles found by their first row
+    int32_t subs;         // 16-row pieces of a window: 1 or 4
+    int32_t tiles;
+    int32_t parts;        // of K
+    int32_t cols;         // of N a block
+};
 struct AdapterArgs {
     xq_adapters q;
-    float* t;             // [M, r]: x A_a^T
+    AdapterPlan p;
+    float* t;             // [parts][M][r_pad]
+    int32_t r_pad;
 };
 
 // the adapter of a row, or -1
 __device__ __forceinline__ int adapter_of(const xq_adapters& q, int64_t row) {
-    const int64_t id = q.id_bytes == 8 ? ((const int64_t*)q.ids)[row] : ((const int32_t*)q.ids)[row];
+    const int64_t id = q.id_bytes == 8 ? ((const int64_t*)q.ids)[row] : (int64_t)((const int32_t*)q.ids)[row];
     return id >= 0 && id < q.n_adapters ? (int)id : -1;
 }
-__device__ __forceinline__ float load_factor(const void* p, int dtype, int64_t at) {
-    return dtype == XQ_DT_F32 ? ((const float*)p)[at] : bf16_to_f32(((const bf16_t*)p)[at]);
+
+// the rows of a leader's tile, in each wave by itself: lane l gets the row of column l % 16, or -1; false: the row leads no tile
+__device__ __forceinline__ bool leader_rows(const xq_adapters& q, int lead, int* id, int* row) {
+    const int lane = threadIdx.x & 63, M = (int)q.M;
+    const int mine = adapter_of(q, lead);
+    *id = mine;
+    int before = 0, seen = 0, want = lane & 15, found = -1;
+    for (int c = 0; c < M; c += 64) {
+        const int i = c + lane;
+        uint64_t same = __ballot(i < M && adapter_of(q, min(i, M - 1)) == mine);
+        if (lead >= c + 64) { before += __popcll(same); continue; }
+        if (lead > c) {
+            const uint64_t below = (1ull << (lead - c)) - 1;
+            before += __popcll(same & below);
+            same &= ~below;
+        }
+        if (before & 15) return false;
+        const int n = __popcll(same);
+        if (want >= seen && want < seen + n) {
+            uint64_t m = same;
+            for (int k = want - seen; k > 0; --k) m &= m - 1;
+            found = c + __ffsll((unsigned long long)m) - 1;
+        }
+        seen += n;
+        if (seen >= 16) break;
+    }
+    *row = found;
+    return true;
 }
 
-// a wave a value of t
-__global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
-    const xq_adapters& q = a.q;
-    for (int64_t at = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6); at < q.M * q.r; at += (int64_t)gridDim.x * 4) {
-        const int64_t row = at / q.r, j = at - row * q.r;
-        const int id = adapter_of(q, row);
-        float sum = 0.0f;
-        if (id >= 0)
-            for (int64_t k = threadIdx.x & 63; k < q.K; k += 64)
-                sum = fmaf(bf16_to_f32(((const bf16_t*)q.x)[row * q.ldx + k]), load_factor(q.A, q.factor_dtype, ((int64_t)id * q.r + j) * q.K + k), sum);
-        for (int o = 32; o; o >>= 1) sum += __shfl_xor(sum, o, 64);
-        if ((threadIdx.x & 63) == 0) a.t[at] = sum;
+struct Split { bf16x8 hi, lo; };
+__device__ __forceinline__ Split split8(const f32x4& a, const f32x4& b) {
+    Split s;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        const float v = i < 4 ? a[i] : b[i - 4];
+        s.hi[i] = (__bf16)v;
+        s.lo[i] = (__bf16)(v - (float)s.hi[i]);
+    }
+    return s;
+}
+// eight elements of a factor as MFMA operands (bf16 factors have no low halves)
+template <bool F32>
+__device__ __forceinline__ Split load_factor8(const void* p, int64_t at) {
+    if constexpr (F32) return split8(*(const f32x4*)((const float*)p + at), *(const f32x4*)((const float*)p + at + 4));
+    Split s;
+    s.hi = *(const bf16x8*)((const bf16_t*)p + at);
+    s.lo = s.hi;
+    return s;
+}
+// the first n of them, the rest zero, one by one
+template <bool F32>
+__device__ __forceinline__ Split load_factor_n(const void* p, int64_t at, int n) {
+    f32x4 v[2] = {};
+#pragma unroll
+    for (int i = 0; i < 8; ++i)
+        if (i < n) v[i >> 2][i & 3] = F32 ? ((const float*)p)[at + i] : bf16_to_f32(((const bf16_t*)p)[at + i]);
+    return split8(v[0], v[1]);
+}
+__device__ __forceinline__ f32x4 mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+
+// acc[sub][block of 16 ranks] += x A^T over the steps of 32 from `step`, `stride` apart
+template <int SUBS, int RB, bool F32, int AHEAD>
+__device__ __forceinline__ void down_steps(const bf16_t* const (&x)[SUBS], const void* A, const int64_t (&a_at)[RB], int step, int stride, int end, f32x4 (&acc)[SUBS][RB]) {
+    for (; step < end; step += AHEAD * stride) {
+        bf16x8 xv[AHEAD][SUBS];
+        Split av[AHEAD][RB];
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            const int64_t k = (int64_t)min(step + u * stride, end - 1) * 32;
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t) xv[u][t] = *(const bf16x8*)(x[t] + k);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) av[u][b] = load_factor8<F32>(A, a_at[b] + k);
+        }
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (step + u * stride >= end) break;
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int t = 0; t < SUBS; ++t) {
+                    acc[t][b] = mfma(av[u][b].hi, xv[u][t], acc[t][b]);
+                    if (F32) acc[t][b] = mfma(av[u][b].lo, xv[u][t], acc[t][b]);
+                }
+        }
     }
 }
 
-__global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
+// one adapter's part of t for SUBS pieces of 16 rows: row[t] is the row of this lane's column in piece t, or -1
+template <int SUBS, int RB, bool F32>
+__device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int part, float* red) {
     const xq_adapters& q = a.q;
-    const int64_t chunks = (q.N + 255) / 256;
-    for (int64_t at = blockIdx.x; at < q.M * chunks; at += gridDim.x) {
-        const int64_t row = at / chunks, n = (at - row * chunks) * 256 + threadIdx.x;
-        if (n >= q.N) continue;
-        const int id = adapter_of(q, row);
-        const bf16_t base = ((const bf16_t*)q.base)[row * q.ld_base + n];
-        bf16_t out = base;
-        if (id >= 0) {
-            float sum = 0.0f;
-            for (int j = 0; j < q.r; ++j) sum = fmaf(a.t[row * q.r + j], load_factor(q.B, q.factor_dtype, ((int64_t)id * q.N + n) * q.r + j), sum);
-            out = to_bf16(fmaf(q.scaling[id], sum, bf16_to_f32(base)));
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+    const int steps = (int)(q.K / 32), first = (int)((int64_t)steps * part / a.p.parts), last = (int)((int64_t)steps * (part + 1) / a.p.parts);
+    const bf16_t* x[SUBS];
+    int64_t a_at[RB];
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t) x[t] = (const bf16_t*)q.x + (int64_t)max(row[t], 0) * q.ldx + group * 8;
+#pragma unroll
+    for (int b = 0; b < RB; ++b) a_at[b] = ((int64_t)id * q.r + min(b * 16 + col, q.r - 1)) * q.K + group * 8;
+    f32x4 acc[SUBS][RB] = {};
+    down_steps<SUBS, RB, F32, (SUBS * RB > 4 ? 2 : 4)>(x, q.A, a_at, first + wave, 4, last, acc);
+    // the four waves' sums: lane's four ranks of its column
+    __syncthreads();                                       // (what the tile before left in red has been read)
+#pragma unroll
+    for (int half = 2; half; half >>= 1) {
+        if (wave >= half && wave < 2 * half)
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) *(f32x4*)(red + (((wave - half) * SUBS + t) * RB + b) * 256 + lane * 4) = acc[t][b];
+        __syncthreads();
+        if (wave < half)
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) acc[t][b] += *(const f32x4*)(red + ((wave * SUBS + t) * RB + b) * 256 + lane * 4);
+        __syncthreads();
+    }
+    if (wave == 0)
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t)
+            if (row[t] >= 0)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    f32x4 v = acc[t][b];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) v[i] = b * 16 + group * 4 + i < q.r ? v[i] : 0.0f;
+                    *(f32x4*)(a.t + ((int64_t)part * q.M + row[t]) * a.r_pad + b * 16 + group * 4) = v;
+                }
+}
+
+template <int SUBS, int RB, bool F32>
+__global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
+    __shared__ float red[2 * SUBS * RB * 256];
+    const int lane = threadIdx.x & 63;
+    for (int64_t at = blockIdx.x; at < (int64_t)a.p.tiles * a.p.parts; at += gridDim.x) {
+        const int tile = (int)(at / a.p.parts), part = (int)(at - (int64_t)tile * a.p.parts);
+        if (a.p.leaders) {
+            int id, row[1];
+            if (!leader_rows(a.q, tile, &id, &row[0]) || id < 0) continue;
+            down_tile<1, RB, F32>(a, id, row, part, red);
+            continue;
         }
-        ((bf16_t*)q.out)[row * q.ld_out + n] = out;
+        // a window of SUBS * 16 rows: once for every adapter in it
+        const int64_t row0 = (int64_t)tile * (SUBS * 16);
+        const int own = lane < SUBS * 16 && row0 + lane < a.q.M ? adapter_of(a.q, row0 + lane) : -1;
+        uint64_t left = __ballot(own >= 0);
+        while (left) {
+            const int id = __shfl(own, __ffsll((unsigned long long)left) - 1, 64);
+            const uint64_t same = __ballot(own == id) & left;
+            left &= ~same;
+            int row[SUBS], pieces = 0;
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t) {
+                pieces += (same >> (t * 16) & 0xffff) != 0;
+                row[t] = same >> (t * 16 + (lane & 15)) & 1 ? (int)row0 + t * 16 + (lane & 15) : -1;
+            }
+            if (SUBS == 1 || pieces > 2) {
+                down_tile<SUBS, RB, F32>(a, id, row, part, red);
+            } else {
+#pragma unroll
+                for (int t = 0; t < SUBS; ++t) {
+                    const int one[1] = {row[t]};
+                    if (same >> (t * 16) & 0xffff) down_tile<1, RB, F32>(a, id, one, part, red);
+                }
+            }
+        }
+    }
+}
+
+// s t of SUBS pieces of 16 rows as MFMA operands, to LDS: [piece][block of 16 ranks][lane]
+template <int SUBS, int RB>
+__device__ __forceinline__ void up_operands(const AdapterArgs& a, float scale, const int (&row)[SUBS], bf16x8* ts) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            if (((t * RB + b) & 3) != wave) continue;
+            f32x4 v0 = {}, v1 = {};
+            if (row[t] >= 0) {
+                const float* from = a.t + (int64_t)row[t] * a.r_pad + b * 16 + (group & 1) * 8;
+#pragma unroll 4
+                for (int p = 0; p < a.p.parts; ++p) {
+                    v0 += *(const f32x4*)(from + (int64_t)p * a.q.M * a.r_pad);
+                    v1 += *(const f32x4*)(from + (int64_t)p * a.q.M * a.r_pad + 4);
+                }
+            }
+            const Split s = split8(v0 * scale, v1 * scale);
+            ts[(t * RB + b) * 64 + lane] = group < 2 ? s.hi : s.lo;
+        }
+}
+
+// out of one adapter's rows, columns [n0, n1): a wave 32 columns at a time, lane: eight of them of its column's row
+template <int SUBS, int RB, bool F32>
+__device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int64_t n0, int64_t n1, bf16x8* ts) {
+    const xq_adapters& q = a.q;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+    const bool in_place = q.out == q.base && q.ld_out == q.ld_base;
+    if (id >= 0) {
+        __syncthreads();                                   // (what the tile before left in ts has been read)
+        up_operands<SUBS, RB>(a, q.scaling[id], row, ts);
+        __syncthreads();
+    } else if (in_place) {
+        return;
+    }
+    const bool whole = q.r % 8 == 0;                       // ranks in pieces of eight, at multiples of 16 bytes
+    for (int64_t n = n0 + wave * 32; n < n1; n += 128) {
+        Split bv[2][RB];
+        if (id >= 0)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int64_t at = ((int64_t)id * q.N + min(n + (col >> 2) * 8 + j * 4 + (col & 3), q.N - 1)) * q.r;
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    const int k = b * 16 + (group & 1) * 8, real = min(q.r - k, 8);
+                    if (whole && real == 8) bv[j][b] = load_factor8<F32>(q.B, at + k);
+                    else bv[j][b] = load_factor_n<F32>(q.B, at + k, real);
+                }
+            }
+        const int64_t mine = n + group * 8;
+        u32x4 base[SUBS];
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t)
+            if (row[t] >= 0 && mine < q.N) base[t] = *(const u32x4*)((const bf16_t*)q.base + (int64_t)row[t] * q.ld_base + mine);
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t) {
+            f32x4 acc[2] = {};
+            if (id >= 0)
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    const bf16x8 tv = ts[(t * RB + b) * 64 + lane];
+#pragma unroll
+                    for (int j = 0; j < 2; ++j) {
+                        acc[j] = mfma(bv[j][b].hi, tv, acc[j]);
+                        if (F32) acc[j] = mfma(bv[j][b].lo, tv, acc[j]);
+                    }
+                }
+            if (row[t] < 0 || mine >= q.N) continue;
+            u32x4 out = base[t];
+            if (id >= 0)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    const float lo = bf16_to_f32((bf16_t)base[t][i]), hi = bf16_to_f32((bf16_t)(base[t][i] >> 16));
+                    out[i] = pack_bf16x2(lo + acc[i >> 1][(i & 1) * 2], hi + acc[i >> 1][(i & 1) * 2 + 1]);
+                }
+            *(u32x4*)((bf16_t*)q.out + (int64_t)row[t] * q.ld_out + mine) = out;
+        }
+    }
+}
+
+template <int SUBS, int RB, bool F32>
+__global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
+    __shared__ bf16x8 ts[SUBS * RB * 64];
+    const int lane = threadIdx.x & 63;
+    const int64_t chunks = (a.q.N + a.p.cols - 1) / a.p.cols;
+    for (int64_t at = blockIdx.x; at < a.p.tiles * chunks; at += gridDim.x) {
+        const int tile = (int)(at / chunks);
+        const int64_t n0 = (at - tile * chunks) * a.p.cols, n1 = min(n0 + a.p.cols, a.q.N);
+        if (a.p.leaders) {
+            int id, row[1];
+            if (!leader_rows(a.q, tile, &id, &row[0])) continue;
+            up_tile<1, RB, F32>(a, id, row, n0, n1, ts);
+            continue;
+        }
+        const int64_t row0 = (int64_t)tile * (SUBS * 16);
+        const bool real = lane < SUBS * 16 && row0 + lane < a.q.M;
+        const int own = real ? adapter_of(a.q, row0 + lane) : -1;
+        uint64_t left = __ballot(real);
+        while (left) {
+            const int id = __shfl(own, __ffsll((unsigned long long)left) - 1, 64);
+            const uint64_t same = __ballot(own == id) & left;
+            left &= ~same;
+            int row[SUBS], pieces = 0;
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t) {
+                pieces += (same >> (t * 16) & 0xffff) != 0;
+                row[t] = same >> (t * 16 + (lane & 15)) & 1 ? (int)row0 + t * 16 + (lane & 15) : -1;
+            }
+            if (SUBS == 1 || pieces > 2) {
+                up_tile<SUBS, RB, F32>(a, id, row, n0, n1, ts);
+            } else {
+#pragma unroll
+                for (int t = 0; t < SUBS; ++t) {
+                    const int one[1] = {row[t]};
+                    if (same >> (t * 16) & 0xffff) up_tile<1, RB, F32>(a, id, one, n0, n1, ts);
+                }
+            }
+        }
+    }
+}
+
+AdapterPlan plan_adapters(int64_t M, int64_t N, int64_t K) {
+    AdapterPlan p;
+    p.leaders = M <= kLeaderRows;
+    p.subs = p.leaders || M < 8192 ? 1 : 4;
+    p.tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.subs * 16));
+    // parts that bring two blocks to every compute unit where the tiles do not, of at least four steps a wave
+    const int64_t full = xq_cdiv(M, p.subs * 16), steps = K / 32;
+    p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(full, 1), steps / 16, kMostParts}));
+    p.cols = p.leaders ? 128 : 512;
+    return p;
+}
+int r_pad(int r) { return (r + 15) / 16 * 16; }
+
+template <int SUBS, int RB, bool F32>
+void launch_adapters(const AdapterArgs& a, hipStream_t st) {
+    const int64_t most = (1 << 24) - 1;
+    adapter_down_kernel<SUBS, RB, F32><<<dim3((unsigned)std::min((int64_t)a.p.tiles * a.p.parts, most)), 256, 0, st>>>(a);
+    adapter_up_kernel<SUBS, RB, F32><<<dim3((unsigned)std::min(a.p.tiles * xq_cdiv(a.q.N, a.p.cols), most)), 256, 0, st>>>(a);
+}
+template <int SUBS, bool F32>
+void launch_adapters(const AdapterArgs& a, hipStream_t st) {
+    switch (a.r_pad / 16) {
+        case 1: return launch_adapters<SUBS, 1, F32>(a, st);
+        case 2: return launch_adapters<SUBS, 2, F32>(a, st);
+        case 3: return launch_adapters<SUBS, 3, F32>(a, st);
+        default: return launch_adapters<SUBS, 4, F32>(a, st);
     }
 }
 
@@ -65,7 +371,7 @@ using namespace xq;
 
 extern "C" int64_t xq_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r) {
     if (!sizes_fit(M, N, K, r)) return -1;
-    return M * r * 4 + 256;
+    return std::max<int64_t>((int64_t)plan_adapters(M, N, K).parts * M * r_pad(r) * 4, 256);
 }
 
 extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -86,9 +392,10 @@ extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t wo
     XQ_REQUIRE(workspace && xq_aligned(workspace, 256) && workspace_bytes >= xq_adapters_workspace_bytes(q->M, q->N, q->K, q->r),
                "xq_adapters_add: a workspace of %lld bytes, 256-byte aligned, is needed", (long long)xq_adapters_workspace_bytes(q->M, q->N, q->K, q->r));
     hipStream_t st = (hipStream_t)stream;
-    const AdapterArgs a = {*q, (float*)workspace};
-    adapter_down_kernel<<<dim3((unsigned)std::min<int64_t>(xq_cdiv(q->M * q->r, 4), 1 << 22)), 256, 0, st>>>(a);
-    adapter_up_kernel<<<dim3((unsigned)std::min<int64_t>(q->M * xq_cdiv(q->N, 256), 1 << 22)), 256, 0, st>>>(a);
+    const AdapterArgs a = {*q, plan_adapters(q->M, q->N, q->K), (float*)workspace, r_pad(q->r)};
+    const bool f32 = q->factor_dtype == XQ_DT_F32;
+    if (a.p.subs == 1) f32 ? launch_adapters<1, true>(a, st) : launch_adapters<1, false>(a, st);
+    else f32 ? launch_adapters<4, true>(a, st) : launch_adapters<4, false>(a, st);
     XQ_CHECK_LAUNCH("xq_adapters_add");
     return XQ_OK;
 }
