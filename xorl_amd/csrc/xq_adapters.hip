@@ -20,8 +20,8 @@ constexpr int kMostParts = 16;
 
 struct AdapterPlan {
     int32_t leaders;      // tiles found by their first row
-    int32_t subs;         // 16-row pieces of a window: 1 or 4
-    int32_t tiles;
+    int32_t down_subs, up_subs;      // 16-row pieces of a window: 1 or 4
+    int32_t down_tiles, up_tiles;
     int32_t parts;        // of K
     int32_t cols;         // of N a block
 };
@@ -32,6 +32,9 @@ struct AdapterArgs {
     int32_t r_pad;
 };
 
+// MFMA instructions are done whatever lanes are active, so that what decides about them has to be one value a wave, and known as that
+__device__ __forceinline__ int uniform(int v) { return __builtin_amdgcn_readfirstlane(v); }
+
 // the adapter of a row, or -1
 __device__ __forceinline__ int adapter_of(const xq_adapters& q, int64_t row) {
     const int64_t id = q.id_bytes == 8 ? ((const int64_t*)q.ids)[row] : (int64_t)((const int32_t*)q.ids)[row];
@@ -41,7 +44,7 @@ __device__ __forceinline__ int adapter_of(const xq_adapters& q, int64_t row) {
 // the rows of a leader's tile, in each wave by itself: lane l gets the row of column l % 16, or -1; false: the row leads no tile
 __device__ __forceinline__ bool leader_rows(const xq_adapters& q, int lead, int* id, int* row) {
     const int lane = threadIdx.x & 63, M = (int)q.M;
-    const int mine = adapter_of(q, lead);
+    const int mine = uniform(adapter_of(q, lead));
     *id = mine;
     int before = 0, seen = 0, want = lane & 15, found = -1;
     for (int c = 0; c < M; c += 64) {
@@ -78,60 +81,91 @@ __device__ __forceinline__ Split split8(const f32x4& a, const f32x4& b) {
     }
     return s;
 }
-// eight elements of a factor as MFMA operands (bf16 factors have no low halves)
-template <bool F32>
-__device__ __forceinline__ Split load_factor8(const void* p, int64_t at) {
-    if constexpr (F32) return split8(*(const f32x4*)((const float*)p + at), *(const f32x4*)((const float*)p + at + 4));
-    Split s;
-    s.hi = *(const bf16x8*)((const bf16_t*)p + at);
-    s.lo = s.hi;
-    return s;
-}
-// the first n of them, the rest zero, one by one
-template <bool F32>
-__device__ __forceinline__ Split load_factor_n(const void* p, int64_t at, int n) {
-    f32x4 v[2] = {};
-#pragma unroll
-    for (int i = 0; i < 8; ++i)
-        if (i < n) v[i >> 2][i & 3] = F32 ? ((const float*)p)[at + i] : bf16_to_f32(((const bf16_t*)p)[at + i]);
-    return split8(v[0], v[1]);
-}
 __device__ __forceinline__ f32x4 mfma(const bf16x8& a, const bf16x8& b, const f32x4& c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
 
-// acc[sub][block of 16 ranks] += x A^T over the steps of 32 from `step`, `stride` apart
-template <int SUBS, int RB, bool F32, int AHEAD>
-__device__ __forceinline__ void down_steps(const bf16_t* const (&x)[SUBS], const void* A, const int64_t (&a_at)[RB], int step, int stride, int end, f32x4 (&acc)[SUBS][RB]) {
-    for (; step < end; step += AHEAD * stride) {
-        bf16x8 xv[AHEAD][SUBS];
-        Split av[AHEAD][RB];
+// what a factor's eight elements are before they are split
+template <bool F32>
+struct Raw { f32x4 a, b; };
+template <>
+struct Raw<false> { bf16x8 a; };
+template <bool F32>
+__device__ __forceinline__ Raw<F32> load_raw8(const void* p, int64_t at) {
+    if constexpr (F32) return {*(const f32x4*)((const float*)p + at), *(const f32x4*)((const float*)p + at + 4)};
+    else return {*(const bf16x8*)((const bf16_t*)p + at)};
+}
+template <bool F32>
+__device__ __forceinline__ Split split_raw(const Raw<F32>& r) {
+    if constexpr (F32) return split8(r.a, r.b);
+    else return {r.a, r.a};
+}
+
+// the first n of them, the rest zero, one by one
+template <bool F32>
+__device__ __forceinline__ Raw<F32> load_raw_n(const void* p, int64_t at, int n) {
+    Raw<F32> r = {};
 #pragma unroll
-        for (int u = 0; u < AHEAD; ++u) {
-            const int64_t k = (int64_t)min(step + u * stride, end - 1) * 32;
-#pragma unroll
-            for (int t = 0; t < SUBS; ++t) xv[u][t] = *(const bf16x8*)(x[t] + k);
-#pragma unroll
-            for (int b = 0; b < RB; ++b) av[u][b] = load_factor8<F32>(A, a_at[b] + k);
+    for (int i = 0; i < 8; ++i)
+        if (i < n) {
+            if constexpr (F32) {
+                if (i < 4) r.a[i & 3] = ((const float*)p)[at + i];
+                else r.b[i & 3] = ((const float*)p)[at + i];
+            } else {
+                r.a[i] = ((const __bf16*)p)[at + i];
+            }
         }
+    return r;
+}
+
+// acc[sub][block of 16 ranks] += x A^T over n steps of 32, four apart, the first `turn` of them last: AHEAD steps are on their way while the AHEAD before them are multiplied.
+// (Rows lie a power of two apart, or nearly: tiles that all began with their first step would ask the same few memory channels at the same time.)
+template <int SUBS, int RB, bool F32, int AHEAD>
+__device__ __forceinline__ void down_steps(const bf16_t* const (&x)[SUBS], const void* A, const int64_t (&a_at)[RB], int first, int n, int turn, f32x4 (&acc)[SUBS][RB]) {
+    bf16x8 xv[2][AHEAD][SUBS];
+    Raw<F32> av[2][AHEAD][RB];
+    auto load = [&](int buf, int from) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
-            if (step + u * stride >= end) break;
+            if (from + u >= n) break;
+            const int at = from + u + turn;
+            const int64_t k = (int64_t)(first + 4 * (at < n ? at : at - n)) * 32;
 #pragma unroll
-            for (int b = 0; b < RB; ++b)
+            for (int t = 0; t < SUBS; ++t) xv[buf][u][t] = *(const bf16x8*)(x[t] + k);
+#pragma unroll
+            for (int b = 0; b < RB; ++b) av[buf][u][b] = load_raw8<F32>(A, a_at[b] + k);
+        }
+    };
+    auto multiply = [&](int buf, int from) {
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u) {
+            if (from + u >= n) break;
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                const Split s = split_raw<F32>(av[buf][u][b]);
 #pragma unroll
                 for (int t = 0; t < SUBS; ++t) {
-                    acc[t][b] = mfma(av[u][b].hi, xv[u][t], acc[t][b]);
-                    if (F32) acc[t][b] = mfma(av[u][b].lo, xv[u][t], acc[t][b]);
+                    acc[t][b] = mfma(s.hi, xv[buf][u][t], acc[t][b]);
+                    if (F32) acc[t][b] = mfma(s.lo, xv[buf][u][t], acc[t][b]);
                 }
+            }
         }
+    };
+    load(0, 0);
+    for (int i = 0; i < n; i += 2 * AHEAD) {
+        load(1, i + AHEAD);
+        multiply(0, i);
+        load(0, i + 2 * AHEAD);
+        multiply(1, i + AHEAD);
     }
 }
 
 // one adapter's part of t for SUBS pieces of 16 rows: row[t] is the row of this lane's column in piece t, or -1
 template <int SUBS, int RB, bool F32>
-__device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int part, float* red) {
+__device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int part, int turn, float* red) {
     const xq_adapters& q = a.q;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
-    const int steps = (int)(q.K / 32), first = (int)((int64_t)steps * part / a.p.parts), last = (int)((int64_t)steps * (part + 1) / a.p.parts);
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, group = lane >> 4;
+    // this part's steps, the four waves side by side (256 bytes of a row): this wave's are first, first + 4 ..
+    const int steps = (int)(q.K / 32), begin = (int)((int64_t)steps * part / a.p.parts), end = (int)((int64_t)steps * (part + 1) / a.p.parts);
+    const int first = begin + wave, n = (end - first + 3) >> 2;
     const bf16_t* x[SUBS];
     int64_t a_at[RB];
 #pragma unroll
@@ -139,7 +173,7 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const in
 #pragma unroll
     for (int b = 0; b < RB; ++b) a_at[b] = ((int64_t)id * q.r + min(b * 16 + col, q.r - 1)) * q.K + group * 8;
     f32x4 acc[SUBS][RB] = {};
-    down_steps<SUBS, RB, F32, (SUBS * RB > 4 ? 2 : 4)>(x, q.A, a_at, first + wave, 4, last, acc);
+    down_steps<SUBS, RB, F32, (SUBS * RB > 4 ? 1 : RB > 2 ? 2 : 4)>(x, q.A, a_at, first, n, n > 0 ? (int)((uint32_t)turn * 5 % n) : 0, acc);
     // the four waves' sums: lane's four ranks of its column
     __syncthreads();                                       // (what the tile before left in red has been read)
 #pragma unroll
@@ -174,12 +208,12 @@ template <int SUBS, int RB, bool F32>
 __global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
     __shared__ float red[2 * SUBS * RB * 256];
     const int lane = threadIdx.x & 63;
-    for (int64_t at = blockIdx.x; at < (int64_t)a.p.tiles * a.p.parts; at += gridDim.x) {
+    for (int64_t at = blockIdx.x; at < (int64_t)a.p.down_tiles * a.p.parts; at += gridDim.x) {
         const int tile = (int)(at / a.p.parts), part = (int)(at - (int64_t)tile * a.p.parts);
         if (a.p.leaders) {
             int id, row[1];
             if (!leader_rows(a.q, tile, &id, &row[0]) || id < 0) continue;
-            down_tile<1, RB, F32>(a, id, row, part, red);
+            down_tile<1, RB, F32>(a, id, row, part, tile, red);
             continue;
         }
         // a window of SUBS * 16 rows: once for every adapter in it
@@ -187,7 +221,7 @@ __global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
         const int own = lane < SUBS * 16 && row0 + lane < a.q.M ? adapter_of(a.q, row0 + lane) : -1;
         uint64_t left = __ballot(own >= 0);
         while (left) {
-            const int id = __shfl(own, __ffsll((unsigned long long)left) - 1, 64);
+            const int id = __builtin_amdgcn_readlane(own, __ffsll((unsigned long long)left) - 1);
             const uint64_t same = __ballot(own == id) & left;
             left &= ~same;
             int row[SUBS], pieces = 0;
@@ -197,12 +231,12 @@ __global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
                 row[t] = same >> (t * 16 + (lane & 15)) & 1 ? (int)row0 + t * 16 + (lane & 15) : -1;
             }
             if (SUBS == 1 || pieces > 2) {
-                down_tile<SUBS, RB, F32>(a, id, row, part, red);
+                down_tile<SUBS, RB, F32>(a, id, row, part, tile, red);
             } else {
 #pragma unroll
                 for (int t = 0; t < SUBS; ++t) {
                     const int one[1] = {row[t]};
-                    if (same >> (t * 16) & 0xffff) down_tile<1, RB, F32>(a, id, one, part, red);
+                    if (same >> (t * 16) & 0xffff) down_tile<1, RB, F32>(a, id, one, part, tile, red);
                 }
             }
         }
@@ -236,18 +270,13 @@ __device__ __forceinline__ void up_operands(const AdapterArgs& a, float scale, c
 template <int SUBS, int RB, bool F32>
 __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int64_t n0, int64_t n1, bf16x8* ts) {
     const xq_adapters& q = a.q;
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, col = lane & 15, group = lane >> 4;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, group = lane >> 4;
     const bool in_place = q.out == q.base && q.ld_out == q.ld_base;
-    if (id >= 0) {
-        __syncthreads();                                   // (what the tile before left in ts has been read)
-        up_operands<SUBS, RB>(a, q.scaling[id], row, ts);
-        __syncthreads();
-    } else if (in_place) {
-        return;
-    }
+    if (id < 0 && in_place) return;
     const bool whole = q.r % 8 == 0;                       // ranks in pieces of eight, at multiples of 16 bytes
-    for (int64_t n = n0 + wave * 32; n < n1; n += 128) {
-        Split bv[2][RB];
+    Raw<F32> bv[2][2][RB];
+    u32x4 base[2][SUBS];
+    auto load = [&](int buf, int64_t n) {
         if (id >= 0)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
@@ -255,15 +284,22 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int 
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     const int k = b * 16 + (group & 1) * 8, real = min(q.r - k, 8);
-                    if (whole && real == 8) bv[j][b] = load_factor8<F32>(q.B, at + k);
-                    else bv[j][b] = load_factor_n<F32>(q.B, at + k, real);
+                    if (whole && real == 8) bv[buf][j][b] = load_raw8<F32>(q.B, at + k);
+                    else bv[buf][j][b] = load_raw_n<F32>(q.B, at + k, real);
                 }
             }
-        const int64_t mine = n + group * 8;
-        u32x4 base[SUBS];
+        const int64_t mine = min(n + group * 8, q.N - 8);
 #pragma unroll
-        for (int t = 0; t < SUBS; ++t)
-            if (row[t] >= 0 && mine < q.N) base[t] = *(const u32x4*)((const bf16_t*)q.base + (int64_t)row[t] * q.ld_base + mine);
+        for (int t = 0; t < SUBS; ++t) base[buf][t] = *(const u32x4*)((const bf16_t*)q.base + (int64_t)max(row[t], 0) * q.ld_base + mine);
+    };
+    auto finish = [&](int buf, int64_t n) {
+        const int64_t mine = n + group * 8;
+        Split sv[2][RB];
+#pragma unroll
+        for (int b = 0; b < RB; ++b) {
+            sv[0][b] = split_raw<F32>(bv[buf][0][b]);
+            sv[1][b] = split_raw<F32>(bv[buf][1][b]);
+        }
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
             f32x4 acc[2] = {};
@@ -273,20 +309,33 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int 
                     const bf16x8 tv = ts[(t * RB + b) * 64 + lane];
 #pragma unroll
                     for (int j = 0; j < 2; ++j) {
-                        acc[j] = mfma(bv[j][b].hi, tv, acc[j]);
-                        if (F32) acc[j] = mfma(bv[j][b].lo, tv, acc[j]);
+                        acc[j] = mfma(sv[j][b].hi, tv, acc[j]);
+                        if (F32) acc[j] = mfma(sv[j][b].lo, tv, acc[j]);
                     }
                 }
-            if (row[t] < 0 || mine >= q.N) continue;
-            u32x4 out = base[t];
+            if (row[t] < 0 || mine >= n1) continue;
+            u32x4 out = base[buf][t];
             if (id >= 0)
 #pragma unroll
                 for (int i = 0; i < 4; ++i) {
-                    const float lo = bf16_to_f32((bf16_t)base[t][i]), hi = bf16_to_f32((bf16_t)(base[t][i] >> 16));
+                    const float lo = bf16_to_f32((bf16_t)out[i]), hi = bf16_to_f32((bf16_t)(out[i] >> 16));
                     out[i] = pack_bf16x2(lo + acc[i >> 1][(i & 1) * 2], hi + acc[i >> 1][(i & 1) * 2 + 1]);
                 }
             *(u32x4*)((bf16_t*)q.out + (int64_t)row[t] * q.ld_out + mine) = out;
         }
+    };
+    const int64_t from = n0 + wave * 32;                   // (the four waves side by side: 256 bytes of a row)
+    load(0, from);
+    if (id >= 0) {
+        __syncthreads();                                   // (what the tile before left in ts has been read)
+        up_operands<SUBS, RB>(a, q.scaling[id], row, ts);
+        __syncthreads();
+    }
+    for (int64_t n = from; n < n1; n += 256) {
+        load(1, n + 128);
+        finish(0, n);
+        load(0, n + 256);
+        if (n + 128 < n1) finish(1, n + 128);
     }
 }
 
@@ -295,7 +344,7 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
     __shared__ bf16x8 ts[SUBS * RB * 64];
     const int lane = threadIdx.x & 63;
     const int64_t chunks = (a.q.N + a.p.cols - 1) / a.p.cols;
-    for (int64_t at = blockIdx.x; at < a.p.tiles * chunks; at += gridDim.x) {
+    for (int64_t at = blockIdx.x; at < a.p.up_tiles * chunks; at += gridDim.x) {
         const int tile = (int)(at / chunks);
         const int64_t n0 = (at - tile * chunks) * a.p.cols, n1 = min(n0 + a.p.cols, a.q.N);
         if (a.p.leaders) {
@@ -309,7 +358,7 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
         const int own = real ? adapter_of(a.q, row0 + lane) : -1;
         uint64_t left = __ballot(real);
         while (left) {
-            const int id = __shfl(own, __ffsll((unsigned long long)left) - 1, 64);
+            const int id = __builtin_amdgcn_readlane(own, __ffsll((unsigned long long)left) - 1);
             const uint64_t same = __ballot(own == id) & left;
             left &= ~same;
             int row[SUBS], pieces = 0;
@@ -334,29 +383,35 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
 AdapterPlan plan_adapters(int64_t M, int64_t N, int64_t K) {
     AdapterPlan p;
     p.leaders = M <= kLeaderRows;
-    p.subs = p.leaders || M < 8192 ? 1 : 4;
-    p.tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.subs * 16));
+    p.down_subs = p.leaders || M < 8192 ? 1 : 4;
+    p.up_subs = p.leaders ? 1 : 4;
+    p.down_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.down_subs * 16));
+    p.up_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.up_subs * 16));
     // parts that bring two blocks to every compute unit where the tiles do not, of at least four steps a wave
-    const int64_t full = xq_cdiv(M, p.subs * 16), steps = K / 32;
+    const int64_t full = xq_cdiv(M, p.down_subs * 16), steps = K / 32;
     p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(full, 1), steps / 16, kMostParts}));
-    p.cols = p.leaders ? 128 : 512;
+    // columns of a block: fewer blocks repeat the reading of t and its roundings less, as long as there are four of them a compute unit
+    p.cols = p.leaders ? 128 : p.up_tiles * xq_cdiv(N, 1024) >= 1024 ? 1024 : 512;
     return p;
 }
 int r_pad(int r) { return (r + 15) / 16 * 16; }
 
-template <int SUBS, int RB, bool F32>
+template <int RB, bool F32>
 void launch_adapters(const AdapterArgs& a, hipStream_t st) {
     const int64_t most = (1 << 24) - 1;
-    adapter_down_kernel<SUBS, RB, F32><<<dim3((unsigned)std::min((int64_t)a.p.tiles * a.p.parts, most)), 256, 0, st>>>(a);
-    adapter_up_kernel<SUBS, RB, F32><<<dim3((unsigned)std::min(a.p.tiles * xq_cdiv(a.q.N, a.p.cols), most)), 256, 0, st>>>(a);
+    const dim3 down((unsigned)std::min((int64_t)a.p.down_tiles * a.p.parts, most)), up((unsigned)std::min(a.p.up_tiles * xq_cdiv(a.q.N, a.p.cols), most));
+    if (a.p.down_subs == 1) adapter_down_kernel<1, RB, F32><<<down, 256, 0, st>>>(a);
+    else adapter_down_kernel<4, RB, F32><<<down, 256, 0, st>>>(a);
+    if (a.p.up_subs == 1) adapter_up_kernel<1, RB, F32><<<up, 256, 0, st>>>(a);
+    else adapter_up_kernel<4, RB, F32><<<up, 256, 0, st>>>(a);
 }
-template <int SUBS, bool F32>
+template <bool F32>
 void launch_adapters(const AdapterArgs& a, hipStream_t st) {
     switch (a.r_pad / 16) {
-        case 1: return launch_adapters<SUBS, 1, F32>(a, st);
-        case 2: return launch_adapters<SUBS, 2, F32>(a, st);
-        case 3: return launch_adapters<SUBS, 3, F32>(a, st);
-        default: return launch_adapters<SUBS, 4, F32>(a, st);
+        case 1: return launch_adapters<1, F32>(a, st);
+        case 2: return launch_adapters<2, F32>(a, st);
+        case 3: return launch_adapters<3, F32>(a, st);
+        default: return launch_adapters<4, F32>(a, st);
     }
 }
 
@@ -393,9 +448,7 @@ extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t wo
                "xq_adapters_add: a workspace of %lld bytes, 256-byte aligned, is needed", (long long)xq_adapters_workspace_bytes(q->M, q->N, q->K, q->r));
     hipStream_t st = (hipStream_t)stream;
     const AdapterArgs a = {*q, plan_adapters(q->M, q->N, q->K), (float*)workspace, r_pad(q->r)};
-    const bool f32 = q->factor_dtype == XQ_DT_F32;
-    if (a.p.subs == 1) f32 ? launch_adapters<1, true>(a, st) : launch_adapters<1, false>(a, st);
-    else f32 ? launch_adapters<4, true>(a, st) : launch_adapters<4, false>(a, st);
+    q->factor_dtype == XQ_DT_F32 ? launch_adapters<true>(a, st) : launch_adapters<false>(a, st);
     XQ_CHECK_LAUNCH("xq_adapters_add");
     return XQ_OK;
 }
