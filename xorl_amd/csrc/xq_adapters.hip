@@ -116,66 +116,132 @@ __device__ __forceinline__ Raw<F32> load_raw_n(const void* p, int64_t at, int n)
     return r;
 }
 
-// acc[sub][block of 16 ranks] += x A^T over n steps of 32, four apart, the first `turn` of them last: AHEAD steps are on their way while the AHEAD before them are multiplied.
-// (Rows lie a power of two apart, or nearly: tiles that all began with their first step would ask the same few memory channels at the same time.)
+// An MFMA operand has 16 rows in neighbouring lanes; a load that asks for it so touches a cache line a lane.  So rows are loaded whole cache lines at a time, eight
+// lanes on each, and the lanes exchange them through LDS, a wave in a place of its own, pieces of 16 bytes exclusive-ored so that neither side
+// meets a bank twice.  (16384 rows, K 12288, rank 64, us: @DIRECT@)
+__device__ __forceinline__ void wave_fence() {
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+template <int PIECES>
+__device__ __forceinline__ int slot(int row, int piece) { return row * PIECES + (piece ^ (row & 7)); }
+constexpr int kPlaceKb = 8;           // of a wave
+
+// acc[sub][block of 16 ranks] += x A^T over n units of 64 elements (a cache line of x), four apart, the first `turn` of them last: AHEAD units are on their way
+// while the AHEAD before them are multiplied.  (Rows lie a power of two apart, or nearly: tiles that all began with their first unit would ask the same few memory
+// channels at the same time.)  x[t][h], a_at[b][h]: the rows that this lane loads; ex: this wave's place
 template <int SUBS, int RB, bool F32, int AHEAD>
-__device__ __forceinline__ void down_steps(const bf16_t* const (&x)[SUBS], const void* A, const int64_t (&a_at)[RB], int first, int n, int turn, f32x4 (&acc)[SUBS][RB]) {
-    bf16x8 xv[2][AHEAD][SUBS];
-    Raw<F32> av[2][AHEAD][RB];
-    auto load = [&](int buf, int from) {
+__device__ __forceinline__ void down_units(const bf16_t* const (&x)[SUBS][2], const void* A, const uint32_t (&a_at)[RB][F32 ? 4 : 2], int first, int n, int turn, u32x4* ex,
+                                           f32x4 (&acc)[SUBS][RB]) {
+    constexpr int FL = F32 ? 4 : 2, AP = F32 ? 16 : 8;    // loads, and pieces a row, of 16 rows of a factor
+    constexpr int GROUP = kPlaceKb / FL;                   // blocks of ranks that the place holds
+    const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
+    u32x4 xv[AHEAD][SUBS][2], av[AHEAD][RB][FL];
+    auto unit = [&](int i) {
+        const int at = i + turn;
+        return (first + 4 * (at < n ? at : at - n)) * 64;
+    };
+    auto load_x = [&](int from) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (from + u >= n) break;
-            const int at = from + u + turn;
-            const int64_t k = (int64_t)(first + 4 * (at < n ? at : at - n)) * 32;
+            const int64_t k = unit(from + u);
 #pragma unroll
-            for (int t = 0; t < SUBS; ++t) xv[buf][u][t] = *(const bf16x8*)(x[t] + k);
+            for (int t = 0; t < SUBS; ++t)
 #pragma unroll
-            for (int b = 0; b < RB; ++b) av[buf][u][b] = load_raw8<F32>(A, a_at[b] + k);
+                for (int h = 0; h < 2; ++h) xv[u][t][h] = *(const u32x4*)(x[t][h] + k);
         }
     };
-    auto multiply = [&](int buf, int from) {
+    auto load_a = [&](int from) {
 #pragma unroll
         for (int u = 0; u < AHEAD; ++u) {
             if (from + u >= n) break;
+            const char* base = (const char*)A + (int64_t)unit(from + u) * (F32 ? 4 : 2);
 #pragma unroll
-            for (int b = 0; b < RB; ++b) {
-                const Split s = split_raw<F32>(av[buf][u][b]);
+            for (int b = 0; b < RB; ++b)
 #pragma unroll
-                for (int t = 0; t < SUBS; ++t) {
-                    acc[t][b] = mfma(s.hi, xv[buf][u][t], acc[t][b]);
-                    if (F32) acc[t][b] = mfma(s.lo, xv[buf][u][t], acc[t][b]);
+                for (int h = 0; h < FL; ++h) av[u][b][h] = *(const u32x4*)(base + a_at[b][h]);
+        }
+    };
+    load_x(0);
+    load_a(0);
+    for (int i = 0; i < n; i += AHEAD) {
+        bf16x8 xo[AHEAD][SUBS][2];
+        wave_fence();                                      // (what was exchanged before has been read)
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) ex[(u * SUBS + t) * 128 + slot<8>(h * 8 + (lane >> 3), lane & 7)] = xv[u][t][h];
+        wave_fence();
+        load_x(i + AHEAD);
+#pragma unroll
+        for (int u = 0; u < AHEAD; ++u)
+#pragma unroll
+            for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+                for (int h = 0; h < 2; ++h) xo[u][t][h] = __builtin_bit_cast(bf16x8, ex[(u * SUBS + t) * 128 + slot<8>(col, h * 4 + group)]);
+#pragma unroll
+        for (int b0 = 0; b0 < AHEAD * RB; b0 += GROUP) {
+            wave_fence();
+#pragma unroll
+            for (int g = 0; g < GROUP; ++g)
+                if (b0 + g < AHEAD * RB)
+#pragma unroll
+                    for (int h = 0; h < FL; ++h)
+                        ex[g * AP * 16 + slot<AP>(F32 ? h * 4 + (lane >> 4) : h * 8 + (lane >> 3), lane & (AP - 1))] = av[(b0 + g) / RB][(b0 + g) % RB][h];
+            wave_fence();
+            if (b0 + GROUP >= AHEAD * RB) load_a(i + AHEAD);
+#pragma unroll
+            for (int g = 0; g < GROUP; ++g) {
+                const int u = (b0 + g) / RB, b = (b0 + g) % RB;
+                if (b0 + g >= AHEAD * RB || i + u >= n) break;
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    Split s;
+                    const u32x4* from = ex + g * AP * 16;
+                    if constexpr (F32) s = split8(__builtin_bit_cast(f32x4, from[slot<AP>(col, h * 8 + group * 2)]), __builtin_bit_cast(f32x4, from[slot<AP>(col, h * 8 + group * 2 + 1)]));
+                    else s.hi = __builtin_bit_cast(bf16x8, from[slot<AP>(col, h * 4 + group)]);
+#pragma unroll
+                    for (int t = 0; t < SUBS; ++t) {
+                        acc[t][b] = mfma(s.hi, xo[u][t][h], acc[t][b]);
+                        if (F32) acc[t][b] = mfma(s.lo, xo[u][t][h], acc[t][b]);
+                    }
                 }
             }
         }
-    };
-    load(0, 0);
-    for (int i = 0; i < n; i += 2 * AHEAD) {
-        load(1, i + AHEAD);
-        multiply(0, i);
-        load(0, i + 2 * AHEAD);
-        multiply(1, i + AHEAD);
     }
 }
+// units on their way: up to four of x in a wave's place, and 16 loads of factors
+constexpr int ahead_for(int subs, int rb, bool f32) { return subs == 4 ? 1 : std::min(4, std::max(1, 16 / (rb * (f32 ? 8 : 4)))); }
 
 // one adapter's part of t for SUBS pieces of 16 rows: row[t] is the row of this lane's column in piece t, or -1
 template <int SUBS, int RB, bool F32>
 __device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int part, int turn, float* red) {
+    constexpr int FL = F32 ? 4 : 2;
     const xq_adapters& q = a.q;
-    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, group = lane >> 4;
-    // this part's steps, the four waves side by side (256 bytes of a row): this wave's are first, first + 4 ..
-    const int steps = (int)(q.K / 32), begin = (int)((int64_t)steps * part / a.p.parts), end = (int)((int64_t)steps * (part + 1) / a.p.parts);
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), group = lane >> 4;
+    // this part's units, the four waves side by side: this wave's are first, first + 4 ..
+    const int units = (int)(q.K / 64), begin = (int)((int64_t)units * part / a.p.parts), end = (int)((int64_t)units * (part + 1) / a.p.parts);
     const int first = begin + wave, n = (end - first + 3) >> 2;
-    const bf16_t* x[SUBS];
-    int64_t a_at[RB];
+    const bf16_t* x[SUBS][2];
+    uint32_t a_at[RB][FL];                                 // (an adapter's A is below 4 GiB)
 #pragma unroll
-    for (int t = 0; t < SUBS; ++t) x[t] = (const bf16_t*)q.x + (int64_t)max(row[t], 0) * q.ldx + group * 8;
+    for (int t = 0; t < SUBS; ++t)
 #pragma unroll
-    for (int b = 0; b < RB; ++b) a_at[b] = ((int64_t)id * q.r + min(b * 16 + col, q.r - 1)) * q.K + group * 8;
+        for (int h = 0; h < 2; ++h) x[t][h] = (const bf16_t*)q.x + (int64_t)max(__shfl(row[t], h * 8 + (lane >> 3), 64), 0) * q.ldx + (lane & 7) * 8;
+#pragma unroll
+    for (int b = 0; b < RB; ++b)
+#pragma unroll
+        for (int h = 0; h < FL; ++h)
+            a_at[b][h] = (uint32_t)min(b * 16 + (F32 ? h * 4 + (lane >> 4) : h * 8 + (lane >> 3)), q.r - 1) * (uint32_t)q.K * (F32 ? 4 : 2) + (lane & (F32 ? 15 : 7)) * 16;
     f32x4 acc[SUBS][RB] = {};
-    down_steps<SUBS, RB, F32, (SUBS * RB > 4 ? 1 : RB > 2 ? 2 : 4)>(x, q.A, a_at, first, n, n > 0 ? (int)((uint32_t)turn * 5 % n) : 0, acc);
-    // the four waves' sums: lane's four ranks of its column
     __syncthreads();                                       // (what the tile before left in red has been read)
+    const char* A = (const char*)q.A + (int64_t)id * q.r * q.K * (F32 ? 4 : 2);
+    down_units<SUBS, RB, F32, ahead_for(SUBS, RB, F32)>(x, A, a_at, first, n, n > 0 ? (int)((uint32_t)turn * 5 % n) : 0, (u32x4*)red + wave * kPlaceKb * 64, acc);
+    // the four waves' sums: lane's four ranks of its column
+    __syncthreads();
 #pragma unroll
     for (int half = 2; half; half >>= 1) {
         if (wave >= half && wave < 2 * half)
@@ -204,11 +270,21 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const in
                 }
 }
 
+// Blocks go to the eight XCDs in turn: neighbouring items, which are of one adapter as a rule, go to one of them, so that each reads few adapters through its L2
+// (16384 rows of 8 adapters whose A have 1.5 MB each: @XCD@)
+__device__ __forceinline__ int64_t item_of(int64_t at, int64_t n) {
+    const int64_t each = n / 8, rest = n - each * 8, xcd = at & 7, i = at >> 3;
+    return at >= each * 8 + rest ? at : xcd * each + min(xcd, rest) + i;
+}
+
 template <int SUBS, int RB, bool F32>
 __global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
-    __shared__ float red[2 * SUBS * RB * 256];
+    __shared__ __attribute__((aligned(16))) float red[4 * kPlaceKb * 256];       // (and the waves' sums: at most 2 * SUBS * RB KB)
+    static_assert(2 * SUBS * RB <= 4 * kPlaceKb, "");
     const int lane = threadIdx.x & 63;
-    for (int64_t at = blockIdx.x; at < (int64_t)a.p.down_tiles * a.p.parts; at += gridDim.x) {
+    const int64_t items = (int64_t)a.p.down_tiles * a.p.parts;
+    for (int64_t b = blockIdx.x; b < items; b += gridDim.x) {
+        const int64_t at = a.p.leaders ? b : item_of(b, items);
         const int tile = (int)(at / a.p.parts), part = (int)(at - (int64_t)tile * a.p.parts);
         if (a.p.leaders) {
             int id, row[1];
@@ -266,44 +342,84 @@ __device__ __forceinline__ void up_operands(const AdapterArgs& a, float scale, c
         }
 }
 
-// out of one adapter's rows, columns [n0, n1): a wave 32 columns at a time, lane: eight of them of its column's row
+// Where the eight ranks kc of B's row nl (of 32) lie after their exchange, m such pieces a row: exclusive-ored where m is a power of two
+__device__ __forceinline__ int b_slot(int nl, int kc, int m) {
+    const int f = m == 8 ? (nl & 3) | (nl >> 3 & 1) << 2 : m == 4 ? (nl >> 1 & 1) | (nl >> 3 & 1) << 1 : m == 2 ? nl >> 3 & 1 : 0;
+    return nl * m + (kc ^ f);
+}
+
+// out of one adapter's rows, columns [n0, n1): a wave 32 columns at a time.  ex: this wave's place, B's rows and behind them 16 rows of 32 sums.
 template <int SUBS, int RB, bool F32>
-__device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int64_t n0, int64_t n1, bf16x8* ts) {
+__device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int64_t n0, int64_t n1, bf16x8* ts, u32x4* ex) {
+    constexpr int FR = F32 ? 2 : 1, BP = RB * FR;         // KB of B's 32 rows
     const xq_adapters& q = a.q;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, group = lane >> 4;
-    const bool in_place = q.out == q.base && q.ld_out == q.ld_base;
-    if (id < 0 && in_place) return;
+    if (id < 0 && q.out == q.base && q.ld_out == q.ld_base) return;
     const bool whole = q.r % 8 == 0;                       // ranks in pieces of eight, at multiples of 16 bytes
-    Raw<F32> bv[2][2][RB];
-    u32x4 base[2][SUBS];
+    const int m = q.r / 8;
+    // loads and stores: four lanes a row, eight columns each
+    int own[SUBS];
+#pragma unroll
+    for (int t = 0; t < SUBS; ++t) own[t] = __shfl(row[t], lane >> 2, 64);
+    u32x4 base[2][SUBS], braw[BP];
+    int put[BP];                                           // where this lane's pieces of B go
+    if (whole)
+#pragma unroll
+        for (int i = 0; i < BP; ++i) {
+            const int piece = (i * 64 + lane) / FR, nl = piece / m;
+            put[i] = nl < 32 ? b_slot(nl, piece - nl * m, m) * FR + (F32 ? lane & 1 : 0) : -1;
+        }
+    const int64_t b_bytes = F32 ? 4 : 2;
     auto load = [&](int buf, int64_t n) {
+        n = min(n, q.N - 16);
+        if (id >= 0 && whole) {
+            const int64_t last = min(q.N - n, (int64_t)32) * q.r * b_bytes - 16;
+            const char* from = (const char*)q.B + ((int64_t)id * q.N + n) * q.r * b_bytes;
+#pragma unroll
+            for (int i = 0; i < BP; ++i) braw[i] = *(const u32x4*)(from + min((int64_t)(i * 64 + lane) * 16, last));
+        }
+        const int64_t mine = min(n + (lane & 3) * 8, q.N - 8);
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t) base[buf][t] = *(const u32x4*)((const bf16_t*)q.base + (int64_t)max(own[t], 0) * q.ld_base + mine);
+    };
+    auto finish = [&](int buf, int64_t n) {
+        Split sv[2][RB];
+        if (id >= 0) {
+            wave_fence();                                  // (what was exchanged before has been read)
+            if (whole)
+#pragma unroll
+                for (int i = 0; i < BP; ++i)
+                    if (put[i] >= 0) ex[put[i]] = braw[i];
+            wave_fence();
+        }
+        if (SUBS > 1 || n + 128 < n1) load(buf ^ 1, n + 128);
         if (id >= 0)
 #pragma unroll
             for (int j = 0; j < 2; ++j) {
-                const int64_t at = ((int64_t)id * q.N + min(n + (col >> 2) * 8 + j * 4 + (col & 3), q.N - 1)) * q.r;
+                const int nl = (col >> 2) * 8 + j * 4 + (col & 3);
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
-                    const int k = b * 16 + (group & 1) * 8, real = min(q.r - k, 8);
-                    if (whole && real == 8) bv[buf][j][b] = load_raw8<F32>(q.B, at + k);
-                    else bv[buf][j][b] = load_raw_n<F32>(q.B, at + k, real);
+                    const int kc = b * 2 + (group & 1);
+                    Raw<F32> r = {};
+                    if (whole) {
+                        if (kc < m) {
+                            const u32x4* from = ex + b_slot(nl, kc, m) * FR;
+                            r.a = __builtin_bit_cast(decltype(r.a), from[0]);
+                            if constexpr (F32) r.b = __builtin_bit_cast(f32x4, from[1]);
+                        }
+                    } else {
+                        r = load_raw_n<F32>(q.B, ((int64_t)id * q.N + min(n + nl, q.N - 1)) * q.r + kc * 8, min(q.r - kc * 8, 8));
+                    }
+                    sv[j][b] = split_raw<F32>(r);
                 }
             }
-        const int64_t mine = min(n + group * 8, q.N - 8);
-#pragma unroll
-        for (int t = 0; t < SUBS; ++t) base[buf][t] = *(const u32x4*)((const bf16_t*)q.base + (int64_t)max(row[t], 0) * q.ld_base + mine);
-    };
-    auto finish = [&](int buf, int64_t n) {
-        const int64_t mine = n + group * 8;
-        Split sv[2][RB];
-#pragma unroll
-        for (int b = 0; b < RB; ++b) {
-            sv[0][b] = split_raw<F32>(bv[buf][0][b]);
-            sv[1][b] = split_raw<F32>(bv[buf][1][b]);
-        }
+        const int64_t mine = n + (lane & 3) * 8;
+        u32x4* sums = ex + BP * 64;
 #pragma unroll
         for (int t = 0; t < SUBS; ++t) {
-            f32x4 acc[2] = {};
-            if (id >= 0)
+            u32x4 out = base[buf][t];
+            if (id >= 0) {
+                f32x4 acc[2] = {};
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     const bf16x8 tv = ts[(t * RB + b) * 64 + lane];
@@ -313,15 +429,21 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int 
                         if (F32) acc[j] = mfma(sv[j][b].lo, tv, acc[j]);
                     }
                 }
-            if (row[t] < 0 || mine >= n1) continue;
-            u32x4 out = base[buf][t];
-            if (id >= 0)
+                wave_fence();
 #pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    const float lo = bf16_to_f32((bf16_t)out[i]), hi = bf16_to_f32((bf16_t)(out[i] >> 16));
-                    out[i] = pack_bf16x2(lo + acc[i >> 1][(i & 1) * 2], hi + acc[i >> 1][(i & 1) * 2 + 1]);
+                for (int j = 0; j < 2; ++j) sums[slot<8>(col, group * 2 + j)] = __builtin_bit_cast(u32x4, acc[j]);
+                wave_fence();
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const f32x4 d = __builtin_bit_cast(f32x4, sums[slot<8>(lane >> 2, (lane & 3) * 2 + j)]);
+#pragma unroll
+                    for (int i = 0; i < 2; ++i) {
+                        const uint32_t two = out[j * 2 + i];
+                        out[j * 2 + i] = pack_bf16x2(bf16_to_f32((bf16_t)two) + d[i * 2], bf16_to_f32((bf16_t)(two >> 16)) + d[i * 2 + 1]);
+                    }
                 }
-            *(u32x4*)((bf16_t*)q.out + (int64_t)row[t] * q.ld_out + mine) = out;
+            }
+            if (own[t] >= 0 && mine < n1) *(u32x4*)((bf16_t*)q.out + (int64_t)own[t] * q.ld_out + mine) = out;
         }
     };
     const int64_t from = n0 + wave * 32;                   // (the four waves side by side: 256 bytes of a row)
@@ -332,25 +454,28 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int 
         __syncthreads();
     }
     for (int64_t n = from; n < n1; n += 256) {
-        load(1, n + 128);
         finish(0, n);
-        load(0, n + 256);
         if (n + 128 < n1) finish(1, n + 128);
     }
 }
 
 template <int SUBS, int RB, bool F32>
 __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
+    constexpr int kb = RB * (F32 ? 2 : 1) + 2;
     __shared__ bf16x8 ts[SUBS * RB * 64];
+    __shared__ u32x4 exchange[4 * kb * 64];
+    u32x4* ex = exchange + (threadIdx.x >> 6) * kb * 64;
     const int lane = threadIdx.x & 63;
     const int64_t chunks = (a.q.N + a.p.cols - 1) / a.p.cols;
-    for (int64_t at = blockIdx.x; at < a.p.up_tiles * chunks; at += gridDim.x) {
+    const int64_t items = a.p.up_tiles * chunks;
+    for (int64_t b = blockIdx.x; b < items; b += gridDim.x) {
+        const int64_t at = a.p.leaders ? b : item_of(b, items);
         const int tile = (int)(at / chunks);
         const int64_t n0 = (at - tile * chunks) * a.p.cols, n1 = min(n0 + a.p.cols, a.q.N);
         if (a.p.leaders) {
             int id, row[1];
             if (!leader_rows(a.q, tile, &id, &row[0])) continue;
-            up_tile<1, RB, F32>(a, id, row, n0, n1, ts);
+            up_tile<1, RB, F32>(a, id, row, n0, n1, ts, ex);
             continue;
         }
         const int64_t row0 = (int64_t)tile * (SUBS * 16);
@@ -368,12 +493,12 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
                 row[t] = same >> (t * 16 + (lane & 15)) & 1 ? (int)row0 + t * 16 + (lane & 15) : -1;
             }
             if (SUBS == 1 || pieces > 2) {
-                up_tile<SUBS, RB, F32>(a, id, row, n0, n1, ts);
+                up_tile<SUBS, RB, F32>(a, id, row, n0, n1, ts, ex);
             } else {
 #pragma unroll
                 for (int t = 0; t < SUBS; ++t) {
                     const int one[1] = {row[t]};
-                    if (same >> (t * 16) & 0xffff) up_tile<1, RB, F32>(a, id, one, n0, n1, ts);
+                    if (same >> (t * 16) & 0xffff) up_tile<1, RB, F32>(a, id, one, n0, n1, ts, ex);
                 }
             }
         }
@@ -387,9 +512,9 @@ AdapterPlan plan_adapters(int64_t M, int64_t N, int64_t K) {
     p.up_subs = p.leaders ? 1 : 4;
     p.down_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.down_subs * 16));
     p.up_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.up_subs * 16));
-    // parts that bring two blocks to every compute unit where the tiles do not, of at least four steps a wave
-    const int64_t full = xq_cdiv(M, p.down_subs * 16), steps = K / 32;
-    p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(full, 1), steps / 16, kMostParts}));
+    // parts that bring two blocks to every compute unit where the tiles do not, of at least two cache lines of x a wave
+    const int64_t full = xq_cdiv(M, p.down_subs * 16), units = K / 64;
+    p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(full, 1), units / 8, kMostParts}));
     // columns of a block: fewer blocks repeat the reading of t and its roundings less, as long as there are four of them a compute unit
     p.cols = p.leaders ? 128 : p.up_tiles * xq_cdiv(N, 1024) >= 1024 ? 1024 : 512;
     return p;
@@ -416,7 +541,7 @@ void launch_adapters(const AdapterArgs& a, hipStream_t st) {
 }
 
 bool sizes_fit(int64_t M, int64_t N, int64_t K, int r) {
-    return M >= 0 && M < (1 << 24) && N >= 16 && N < (1 << 24) && N % 16 == 0 && K >= 64 && K < (1 << 24) && K % 64 == 0 && r >= 1 && r <= 64;
+    return M >= 0 && M < (1 << 24) && N >= 16 && N < (1 << 24) && N % 16 == 0 && K >= 64 && K < (1 << 23) && K % 64 == 0 && r >= 1 && r <= 64;
 }
 
 }  // namespace
