@@ -322,6 +322,7 @@ __global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
 // s t of SUBS pieces of 16 rows as MFMA operands, to LDS: [piece][block of 16 ranks][lane]
 template <int SUBS, int RB>
 __device__ __forceinline__ void up_operands(const AdapterArgs& a, float scale, const int (&row)[SUBS], bf16x8* ts) {
+    constexpr int AT_ONCE = SUBS > 1 ? 4 : 8;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, group = lane >> 4;
 #pragma unroll
     for (int t = 0; t < SUBS; ++t)
@@ -331,15 +332,91 @@ __device__ __forceinline__ void up_operands(const AdapterArgs& a, float scale, c
             f32x4 v0 = {}, v1 = {};
             if (row[t] >= 0) {
                 const float* from = a.t + (int64_t)row[t] * a.r_pad + b * 16 + (group & 1) * 8;
-#pragma unroll 4
-                for (int p = 0; p < a.p.parts; ++p) {
-                    v0 += *(const f32x4*)(from + (int64_t)p * a.q.M * a.r_pad);
-                    v1 += *(const f32x4*)(from + (int64_t)p * a.q.M * a.r_pad + 4);
+                for (int p0 = 0; p0 < a.p.parts; p0 += AT_ONCE) {
+                    f32x4 r[AT_ONCE][2];
+#pragma unroll
+                    for (int p = 0; p < AT_ONCE; ++p)
+                        if (p0 + p < a.p.parts) {
+                            r[p][0] = *(const f32x4*)(from + (int64_t)(p0 + p) * a.q.M * a.r_pad);
+                            r[p][1] = *(const f32x4*)(from + (int64_t)(p0 + p) * a.q.M * a.r_pad + 4);
+                        }
+#pragma unroll
+                    for (int p = 0; p < AT_ONCE; ++p)
+                        if (p0 + p < a.p.parts) {
+                            v0 += r[p][0];
+                            v1 += r[p][1];
+                        }
                 }
             }
             const Split s = split8(v0 * scale, v1 * scale);
             ts[(t * RB + b) * 64 + lane] = group < 2 ? s.hi : s.lo;
         }
+}
+
+// eight columns of a row: base and the sums, rounded
+__device__ __forceinline__ u32x4 add8(u32x4 base, const f32x4& lo, const f32x4& hi) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const f32x4& d = i < 2 ? lo : hi;
+        base[i] = pack_bf16x2(bf16_to_f32((bf16_t)base[i]) + d[(i & 1) * 2], bf16_to_f32((bf16_t)(base[i] >> 16)) + d[(i & 1) * 2 + 1]);
+    }
+    return base;
+}
+// B's row among 32 that this lane has as the operand of the j-th of two tiles: so that a lane's eight sums are of neighbouring columns
+__device__ __forceinline__ int b_row(int col, int j) { return (col >> 2) * 8 + j * 4 + (col & 3); }
+
+// out of 16 rows of one adapter, columns [n0, n1), a wave 32 at a time, loaded and stored as the operands lie: such blocks have no more than a few loads, and wait for
+// them and not for the cache.  WHOLE: ranks in pieces of eight, at multiples of 16 bytes
+template <int RB, bool F32, bool WHOLE>
+__device__ __forceinline__ void up_piece(const AdapterArgs& a, int id, int row, int64_t n0, int64_t n1, bf16x8* ts) {
+    const xq_adapters& q = a.q;
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, group = lane >> 4;
+    if (id < 0 && q.out == q.base && q.ld_out == q.ld_base) return;
+    Raw<F32> bv[2][RB];
+    u32x4 base;
+    auto load = [&](int64_t n) {
+        if (id >= 0)
+#pragma unroll
+            for (int j = 0; j < 2; ++j) {
+                const int64_t at = ((int64_t)id * q.N + min(n + b_row(col, j), q.N - 1)) * q.r;
+#pragma unroll
+                for (int b = 0; b < RB; ++b) {
+                    const int k = b * 16 + (group & 1) * 8;
+                    if (!WHOLE) bv[j][b] = load_raw_n<F32>(q.B, at + k, min(q.r - k, 8));
+                    else if (b + 1 < RB || k < q.r) bv[j][b] = load_raw8<F32>(q.B, at + k);
+                    else bv[j][b] = {};
+                }
+            }
+        base = *(const u32x4*)((const bf16_t*)q.base + (int64_t)max(row, 0) * q.ld_base + min(n + group * 8, q.N - 8));
+    };
+    const int64_t from = n0 + wave * 32;                   // (the four waves side by side: 256 bytes of a row)
+    load(from);
+    if (id >= 0) {
+        const int rows[1] = {row};
+        __syncthreads();                                   // (what the tile before left in ts has been read)
+        up_operands<1, RB>(a, q.scaling[id], rows, ts);
+        __syncthreads();
+    }
+    for (int64_t n = from; n < n1; n += 128) {
+        u32x4 out = base;
+        if (id >= 0) {
+            f32x4 acc[2] = {};
+#pragma unroll
+            for (int b = 0; b < RB; ++b) {
+                const bf16x8 tv = ts[b * 64 + lane];
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const Split s = split_raw<F32>(bv[j][b]);
+                    acc[j] = mfma(s.hi, tv, acc[j]);
+                    if (F32) acc[j] = mfma(s.lo, tv, acc[j]);
+                }
+            }
+            out = add8(base, acc[0], acc[1]);
+        }
+        const int64_t mine = n + group * 8;
+        if (n + 128 < n1) load(n + 128);
+        if (row >= 0 && mine < n1) *(u32x4*)((bf16_t*)q.out + (int64_t)row * q.ld_out + mine) = out;
+    }
 }
 
 // Where the eight ranks kc of B's row nl (of 32) lie after their exchange, m such pieces a row: exclusive-ored where m is a power of two
@@ -348,75 +425,66 @@ __device__ __forceinline__ int b_slot(int nl, int kc, int m) {
     return nl * m + (kc ^ f);
 }
 
-// out of one adapter's rows, columns [n0, n1): a wave 32 columns at a time.  ex: this wave's place, B's rows and behind them 16 rows of 32 sums.
-template <int SUBS, int RB, bool F32>
-__device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int (&row)[SUBS], int64_t n0, int64_t n1, bf16x8* ts, u32x4* ex) {
+// the same for four pieces, those in `pieces`, ranks in pieces of eight: B's rows, and the sums of each piece, exchange their lanes in ex, this wave's place
+template <int RB, bool F32>
+__device__ __forceinline__ void up_window(const AdapterArgs& a, int id, const int (&row)[4], int pieces, int64_t n0, int64_t n1, bf16x8* ts, u32x4* ex) {
     constexpr int FR = F32 ? 2 : 1, BP = RB * FR;         // KB of B's 32 rows
     const xq_adapters& q = a.q;
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6), col = lane & 15, group = lane >> 4;
     if (id < 0 && q.out == q.base && q.ld_out == q.ld_base) return;
-    const bool whole = q.r % 8 == 0;                       // ranks in pieces of eight, at multiples of 16 bytes
     const int m = q.r / 8;
     // loads and stores: four lanes a row, eight columns each
-    int own[SUBS];
+    int own[4];
 #pragma unroll
-    for (int t = 0; t < SUBS; ++t) own[t] = __shfl(row[t], lane >> 2, 64);
-    u32x4 base[2][SUBS], braw[BP];
+    for (int t = 0; t < 4; ++t) own[t] = __shfl(row[t], lane >> 2, 64);
+    u32x4 base[2][4], braw[BP];
     int put[BP];                                           // where this lane's pieces of B go
-    if (whole)
 #pragma unroll
-        for (int i = 0; i < BP; ++i) {
-            const int piece = (i * 64 + lane) / FR, nl = piece / m;
-            put[i] = nl < 32 ? b_slot(nl, piece - nl * m, m) * FR + (F32 ? lane & 1 : 0) : -1;
-        }
-    const int64_t b_bytes = F32 ? 4 : 2;
+    for (int i = 0; i < BP; ++i) {
+        const int piece = (i * 64 + lane) / FR, nl = piece / m;
+        put[i] = nl < 32 ? b_slot(nl, piece - nl * m, m) * FR + (F32 ? lane & 1 : 0) : -1;
+    }
     auto load = [&](int buf, int64_t n) {
         n = min(n, q.N - 16);
-        if (id >= 0 && whole) {
-            const int64_t last = min(q.N - n, (int64_t)32) * q.r * b_bytes - 16;
-            const char* from = (const char*)q.B + ((int64_t)id * q.N + n) * q.r * b_bytes;
+        if (id >= 0) {
+            const int64_t size = F32 ? 4 : 2, last = min(q.N - n, (int64_t)32) * q.r * size - 16;
+            const char* from = (const char*)q.B + ((int64_t)id * q.N + n) * q.r * size;
 #pragma unroll
             for (int i = 0; i < BP; ++i) braw[i] = *(const u32x4*)(from + min((int64_t)(i * 64 + lane) * 16, last));
         }
         const int64_t mine = min(n + (lane & 3) * 8, q.N - 8);
 #pragma unroll
-        for (int t = 0; t < SUBS; ++t) base[buf][t] = *(const u32x4*)((const bf16_t*)q.base + (int64_t)max(own[t], 0) * q.ld_base + mine);
+        for (int t = 0; t < 4; ++t) base[buf][t] = *(const u32x4*)((const bf16_t*)q.base + (int64_t)max(own[t], 0) * q.ld_base + mine);
     };
     auto finish = [&](int buf, int64_t n) {
         Split sv[2][RB];
         if (id >= 0) {
             wave_fence();                                  // (what was exchanged before has been read)
-            if (whole)
 #pragma unroll
-                for (int i = 0; i < BP; ++i)
-                    if (put[i] >= 0) ex[put[i]] = braw[i];
+            for (int i = 0; i < BP; ++i)
+                if (put[i] >= 0) ex[put[i]] = braw[i];
             wave_fence();
         }
-        if (SUBS > 1 || n + 128 < n1) load(buf ^ 1, n + 128);
+        load(buf ^ 1, n + 128);
         if (id >= 0)
 #pragma unroll
-            for (int j = 0; j < 2; ++j) {
-                const int nl = (col >> 2) * 8 + j * 4 + (col & 3);
+            for (int j = 0; j < 2; ++j)
 #pragma unroll
                 for (int b = 0; b < RB; ++b) {
                     const int kc = b * 2 + (group & 1);
                     Raw<F32> r = {};
-                    if (whole) {
-                        if (kc < m) {
-                            const u32x4* from = ex + b_slot(nl, kc, m) * FR;
-                            r.a = __builtin_bit_cast(decltype(r.a), from[0]);
-                            if constexpr (F32) r.b = __builtin_bit_cast(f32x4, from[1]);
-                        }
-                    } else {
-                        r = load_raw_n<F32>(q.B, ((int64_t)id * q.N + min(n + nl, q.N - 1)) * q.r + kc * 8, min(q.r - kc * 8, 8));
+                    if (kc < m) {
+                        const u32x4* from = ex + b_slot(b_row(col, j), kc, m) * FR;
+                        r.a = __builtin_bit_cast(decltype(r.a), from[0]);
+                        if constexpr (F32) r.b = __builtin_bit_cast(f32x4, from[1]);
                     }
                     sv[j][b] = split_raw<F32>(r);
                 }
-            }
         const int64_t mine = n + (lane & 3) * 8;
         u32x4* sums = ex + BP * 64;
 #pragma unroll
-        for (int t = 0; t < SUBS; ++t) {
+        for (int t = 0; t < 4; ++t) {
+            if (!(pieces >> t & 1)) continue;
             u32x4 out = base[buf][t];
             if (id >= 0) {
                 f32x4 acc[2] = {};
@@ -433,15 +501,8 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int 
 #pragma unroll
                 for (int j = 0; j < 2; ++j) sums[slot<8>(col, group * 2 + j)] = __builtin_bit_cast(u32x4, acc[j]);
                 wave_fence();
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    const f32x4 d = __builtin_bit_cast(f32x4, sums[slot<8>(lane >> 2, (lane & 3) * 2 + j)]);
-#pragma unroll
-                    for (int i = 0; i < 2; ++i) {
-                        const uint32_t two = out[j * 2 + i];
-                        out[j * 2 + i] = pack_bf16x2(bf16_to_f32((bf16_t)two) + d[i * 2], bf16_to_f32((bf16_t)(two >> 16)) + d[i * 2 + 1]);
-                    }
-                }
+                const u32x4 lo = sums[slot<8>(lane >> 2, (lane & 3) * 2)], hi = sums[slot<8>(lane >> 2, (lane & 3) * 2 + 1)];
+                out = add8(out, __builtin_bit_cast(f32x4, lo), __builtin_bit_cast(f32x4, hi));
             }
             if (own[t] >= 0 && mine < n1) *(u32x4*)((bf16_t*)q.out + (int64_t)own[t] * q.ld_out + mine) = out;
         }
@@ -450,7 +511,7 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int 
     load(0, from);
     if (id >= 0) {
         __syncthreads();                                   // (what the tile before left in ts has been read)
-        up_operands<SUBS, RB>(a, q.scaling[id], row, ts);
+        up_operands<4, RB>(a, q.scaling[id], row, ts);
         __syncthreads();
     }
     for (int64_t n = from; n < n1; n += 256) {
@@ -459,23 +520,21 @@ __device__ __forceinline__ void up_tile(const AdapterArgs& a, int id, const int 
     }
 }
 
-template <int SUBS, int RB, bool F32>
+// LEADERS: tiles of rows in any order; otherwise windows of 16 rows, or with SUBS 4 of 64
+template <int SUBS, int RB, bool F32, bool WHOLE>
 __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
-    constexpr int kb = RB * (F32 ? 2 : 1) + 2;
+    constexpr int kb = SUBS > 1 ? RB * (F32 ? 2 : 1) + 2 : 0;
     __shared__ bf16x8 ts[SUBS * RB * 64];
-    __shared__ u32x4 exchange[4 * kb * 64];
-    u32x4* ex = exchange + (threadIdx.x >> 6) * kb * 64;
+    __shared__ u32x4 exchange[4 * kb * 64 + 1];
     const int lane = threadIdx.x & 63;
-    const int64_t chunks = (a.q.N + a.p.cols - 1) / a.p.cols;
-    const int64_t items = a.p.up_tiles * chunks;
+    const int64_t chunks = (a.q.N + a.p.cols - 1) / a.p.cols, items = a.p.up_tiles * chunks;
     for (int64_t b = blockIdx.x; b < items; b += gridDim.x) {
         const int64_t at = a.p.leaders ? b : item_of(b, items);
         const int tile = (int)(at / chunks);
         const int64_t n0 = (at - tile * chunks) * a.p.cols, n1 = min(n0 + a.p.cols, a.q.N);
-        if (a.p.leaders) {
-            int id, row[1];
-            if (!leader_rows(a.q, tile, &id, &row[0])) continue;
-            up_tile<1, RB, F32>(a, id, row, n0, n1, ts, ex);
+        if (SUBS == 1 && a.p.leaders) {
+            int id, row;
+            if (leader_rows(a.q, tile, &id, &row)) up_piece<RB, F32, WHOLE>(a, id, row, n0, n1, ts);
             continue;
         }
         const int64_t row0 = (int64_t)tile * (SUBS * 16);
@@ -489,34 +548,27 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
             int row[SUBS], pieces = 0;
 #pragma unroll
             for (int t = 0; t < SUBS; ++t) {
-                pieces += (same >> (t * 16) & 0xffff) != 0;
+                pieces |= ((same >> (t * 16) & 0xffff) != 0) << t;
                 row[t] = same >> (t * 16 + (lane & 15)) & 1 ? (int)row0 + t * 16 + (lane & 15) : -1;
             }
-            if (SUBS == 1 || pieces > 2) {
-                up_tile<SUBS, RB, F32>(a, id, row, n0, n1, ts, ex);
-            } else {
-#pragma unroll
-                for (int t = 0; t < SUBS; ++t) {
-                    const int one[1] = {row[t]};
-                    if (same >> (t * 16) & 0xffff) up_tile<1, RB, F32>(a, id, one, n0, n1, ts, ex);
-                }
-            }
+            if constexpr (SUBS == 4) up_window<RB, F32>(a, id, row, pieces, n0, n1, ts, exchange + (threadIdx.x >> 6) * kb * 64);
+            else up_piece<RB, F32, WHOLE>(a, id, row[0], n0, n1, ts);
         }
     }
 }
 
-AdapterPlan plan_adapters(int64_t M, int64_t N, int64_t K) {
+AdapterPlan plan_adapters(int64_t M, int64_t N, int64_t K, int r) {
     AdapterPlan p;
     p.leaders = M <= kLeaderRows;
     p.down_subs = p.leaders || M < 8192 ? 1 : 4;
-    p.up_subs = p.leaders ? 1 : 4;
+    p.up_subs = p.leaders || r % 8 != 0 ? 1 : 4;           // (ranks that are no multiple of 8 are read one by one: 16 rows at a time)
     p.down_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.down_subs * 16));
     p.up_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.up_subs * 16));
     // parts that bring two blocks to every compute unit where the tiles do not, of at least two cache lines of x a wave
     const int64_t full = xq_cdiv(M, p.down_subs * 16), units = K / 64;
     p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(full, 1), units / 8, kMostParts}));
     // columns of a block: fewer blocks repeat the reading of t and its roundings less, as long as there are four of them a compute unit
-    p.cols = p.leaders ? 128 : p.up_tiles * xq_cdiv(N, 1024) >= 1024 ? 1024 : 512;
+    p.cols = p.leaders ? 128 : p.up_tiles * xq_cdiv(N, 1024) >= 1024 ? 1024 : p.up_tiles * xq_cdiv(N, 512) >= 1024 ? 512 : 256;
     return p;
 }
 int r_pad(int r) { return (r + 15) / 16 * 16; }
@@ -527,8 +579,9 @@ void launch_adapters(const AdapterArgs& a, hipStream_t st) {
     const dim3 down((unsigned)std::min((int64_t)a.p.down_tiles * a.p.parts, most)), up((unsigned)std::min(a.p.up_tiles * xq_cdiv(a.q.N, a.p.cols), most));
     if (a.p.down_subs == 1) adapter_down_kernel<1, RB, F32><<<down, 256, 0, st>>>(a);
     else adapter_down_kernel<4, RB, F32><<<down, 256, 0, st>>>(a);
-    if (a.p.up_subs == 1) adapter_up_kernel<1, RB, F32><<<up, 256, 0, st>>>(a);
-    else adapter_up_kernel<4, RB, F32><<<up, 256, 0, st>>>(a);
+    if (a.p.up_subs == 4) adapter_up_kernel<4, RB, F32, true><<<up, 256, 0, st>>>(a);
+    else if (a.q.r % 8 == 0) adapter_up_kernel<1, RB, F32, true><<<up, 256, 0, st>>>(a);
+    else adapter_up_kernel<1, RB, F32, false><<<up, 256, 0, st>>>(a);
 }
 template <bool F32>
 void launch_adapters(const AdapterArgs& a, hipStream_t st) {
@@ -551,7 +604,7 @@ using namespace xq;
 
 extern "C" int64_t xq_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r) {
     if (!sizes_fit(M, N, K, r)) return -1;
-    return std::max<int64_t>((int64_t)plan_adapters(M, N, K).parts * M * r_pad(r) * 4, 256);
+    return std::max<int64_t>((int64_t)plan_adapters(M, N, K, r).parts * M * r_pad(r) * 4, 256);
 }
 
 extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -572,7 +625,7 @@ extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t wo
     XQ_REQUIRE(workspace && xq_aligned(workspace, 256) && workspace_bytes >= xq_adapters_workspace_bytes(q->M, q->N, q->K, q->r),
                "xq_adapters_add: a workspace of %lld bytes, 256-byte aligned, is needed", (long long)xq_adapters_workspace_bytes(q->M, q->N, q->K, q->r));
     hipStream_t st = (hipStream_t)stream;
-    const AdapterArgs a = {*q, plan_adapters(q->M, q->N, q->K), (float*)workspace, r_pad(q->r)};
+    const AdapterArgs a = {*q, plan_adapters(q->M, q->N, q->K, q->r), (float*)workspace, r_pad(q->r)};
     q->factor_dtype == XQ_DT_F32 ? launch_adapters<true>(a, st) : launch_adapters<false>(a, st);
     XQ_CHECK_LAUNCH("xq_adapters_add");
     return XQ_OK;
