@@ -30,8 +30,9 @@ struct RouteGradArgs {
     bool wide, wide_dz;
 };
 
-// L lanes have a row (16: four rows a wave, sums and maxima within a quarter of it are register moves), V logits each, four neighbours at a time: lane l has
-// experts (j L + l) 4 + i.  A block is one wave: what goes through LDS needs no barrier.
+// L lanes have a row (16: four rows a wave, sums and maxima within a quarter of it are register moves), V logits each, four neighbours at a time; of 16 lanes each
+// next such round begins four lanes on, so that the experts of a few groups are not all in a few lanes.  A block is one wave: what goes through LDS needs no
+// barrier.
 //
 // Without a bias the order is that of the logits, exactly.  A score with a bias is compared as fp32 where that tells the chosen apart from each other and from the
 // first that is left out: sums whose difference is within their error, of experts that differ in logit or bias, send the row to be done again in 64 bits, which is the definition.
@@ -91,8 +92,41 @@ struct Lanes {
     template <typename T>
     static __device__ __forceinline__ T sum(T v) { return all(v, [](T a, T b) { return a + b; }); }
     static __device__ __forceinline__ int least(int v) { return all(v, [](int a, int b) { return min(a, b); }); }
+    // (L 16) the n-th largest of the lanes' values, and the sum of the lanes before
+    template <typename T>
+    static __device__ __forceinline__ T nth(T v, int n) {
+        int larger = 0;
+        T r = v;
+#pragma unroll
+        for (int i = 1; i < 16; ++i) {
+            r = move<0x121>(r);
+            larger += r > v;
+        }
+        return all(larger < n ? v : (T)INFINITY, [](T a, T b) { return a < b ? a : b; });
+    }
+    // the next lane's value
+    static __device__ __forceinline__ int next(int v) {
+        return L == 16 ? __builtin_amdgcn_update_dpp(0, v, 0x101, 0xf, 0xf, true) : __shfl_down(v, 1, 64);
+    }
+    static __device__ __forceinline__ float next(float v) { return __uint_as_float((uint32_t)next((int)__float_as_uint(v))); }
+    static __device__ __forceinline__ int before(int v) {
+        int u = v;
+        u += __builtin_amdgcn_update_dpp(0, u, 0x111, 0xf, 0xf, true);      // from 1, 2, 4, 8 lanes below in the row, 0 where there is none
+        u += __builtin_amdgcn_update_dpp(0, u, 0x112, 0xf, 0xf, true);
+        u += __builtin_amdgcn_update_dpp(0, u, 0x114, 0xf, 0xf, true);
+        u += __builtin_amdgcn_update_dpp(0, u, 0x118, 0xf, 0xf, true);
+        return u - v;
+    }
+    static __device__ __forceinline__ uint64_t bits(uint64_t v) {
+        auto either = [](int a, int b) { return a | b; };
+        return (uint32_t)all((int)(uint32_t)v, either) | (uint64_t)(uint32_t)all((int)(v >> 32), either) << 32;
+    }
     static __device__ __forceinline__ bool any(bool v) { return all((int)v, [](int a, int b) { return a | b; }) != 0; }
 };
+
+// the first expert of lane l's j-th four
+template <int L>
+__device__ __forceinline__ int first_of(int j, int l) { return (j * L + (L == 16 ? (l - 4 * j) & 15 : l)) * 4; }
 
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -107,7 +141,7 @@ template <typename T, int L, int V>
 __device__ __forceinline__ void load_row(const T* row, int E, bool wide, int l, float none, float (&z)[V]) {
 #pragma unroll
     for (int j = 0; j < V / 4; ++j) {
-        const int e = (j * L + l) * 4;
+        const int e = first_of<L>(j, l);
         if (wide) {                                        // (whole fours at aligned addresses)
             if (e < E) {
                 if constexpr (sizeof(T) == 4) {
@@ -137,21 +171,30 @@ __device__ __forceinline__ void load_row(const T* row, int E, bool wide, int l, 
 }
 
 // e^v for comparisons: 2^t of the hardware and what t leaves of v log2(e), 4 steps of 2^-24 in all; nothing below 2^-126
-__device__ __forceinline__ float exp_of(float v) {
+__device__ __forceinline__ float near_exp(float v) {
     const float t = v * 0x1.715476p+0f, rest = fmaf(v, 0x1.715476p+0f, -t) + v * 0x1.4ae0cp-26f, p = __builtin_amdgcn_exp2f(t);
-    return v < -88.0f ? 0.0f : fmaf(p, rest * 0x1.62e43p-1f, p);
+    return v < -87.0f ? 0.0f : v > 88.0f ? INFINITY : fmaf(p, rest * 0x1.62e43p-1f, p);
 }
-__device__ __forceinline__ double exp_of(double v) { return exp(v); }
-__device__ __forceinline__ float reciprocal(float v) { return __builtin_amdgcn_rcpf(v); }
-__device__ __forceinline__ double reciprocal(double v) { return 1.0 / v; }
 
 // what the steps of a row share in LDS
 template <int L, int V>
 struct RowPlace {
-    double value[L * V];                                   // as R: scores by expert; or the two largest of every four
-    double strength[kMaxGroups];
-    float at[kMaxTopK + 1];                                // what the chosen, and the first left out, were chosen by
-    int e[kMaxTopK + 1];
+    float value[L * V];       // what is compared by expert, the two largest of every four, those that are picked from
+    float strength[kMaxGroups];
+    int who[L == 16 ? 4 * L : 1];
+};
+// a wave's rows, or one row that the whole wave chooses for in 64 bits
+template <int L, int V>
+union WavePlace {
+    RowPlace<L, V> rows[64 / L];
+    struct {
+        double value[L * V], strength[kMaxGroups];
+    } wide;
+};
+// the k-th choice, in lane k
+struct Chosen {
+    int e;                    // or -1
+    float at;                 // what it was chosen by
 };
 
 template <typename R>
@@ -161,85 +204,144 @@ __device__ __forceinline__ void take_in(R c, R& first, R& second) {
     first = first > c ? first : c;
 }
 
-// One choice with R = float or double: false where float cannot tell.  top, total: the row's largest logit and sum of exponentials (softmax)
-template <typename R, typename T, int L, int V>
-__device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const float (&z)[V], const float (&b)[V], float bias_most, R top, R total, int l, RowPlace<L, V>* place) {
+// the largest values and whose they are, equal ones by their index
+template <int L, int V>
+__device__ __forceinline__ Chosen pick(float (&v)[V], const int (&who)[V], int picks, int l) {
+    using A = Lanes<L>;
+    Chosen c = {-1, 0.0f};
+    for (int k = 0; k < picks; ++k) {
+        float best = v[0];
+#pragma unroll
+        for (int i = 1; i < V; ++i) best = fmaxf(best, v[i]);
+        const float m = A::largest(best);
+        if (m == -INFINITY) break;
+        int mine = kMaxExperts;
+#pragma unroll
+        for (int i = 0; i < V; ++i) mine = v[i] == m ? min(mine, who[i]) : mine;
+        const int e = A::least(mine);
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[i] = who[i] == e ? -INFINITY : v[i];
+        if (l == k) c = {e, m};
+    }
+    return c;
+}
+// among the first n of a list in LDS
+template <int L, int V>
+__device__ __forceinline__ Chosen pick_listed(const float* value, const int* who, int n, int picks, int l) {
+    float v[V];
+    int e[V];
+#pragma unroll
+    for (int i = 0; i < V; ++i) {
+        const bool is = i * L + l < n;
+        v[i] = is ? value[i * L + l] : -INFINITY;
+        e[i] = is ? who[i * L + l] : kMaxExperts;
+    }
+    return pick<L, V>(v, e, picks, l);
+}
+
+// among V of every lane in LDS, the i-th of lane l at i L + l: for the rows that have no short list, in few registers
+template <int L, int V>
+__device__ __forceinline__ Chosen pick_stored(float* value, int picks, int l) {
+    using A = Lanes<L>;
+    Chosen c = {-1, 0.0f};
+#pragma unroll 1
+    for (int k = 0; k < picks; ++k) {
+        float best = -INFINITY;
+        int at = -1;
+#pragma unroll 4
+        for (int i = 0; i < V; ++i) {                      // (not in order of the experts only where j turns around: the least of equal ones is looked for)
+            const float v = value[i * L + l];
+            const bool more = v > best || (v == best && at >= 0 && first_of<L>(i >> 2, l) + (i & 3) < first_of<L>(at >> 2, l) + (at & 3));
+            best = more ? v : best;
+            at = more ? i : at;
+        }
+        const float m = A::largest(best);
+        if (m == -INFINITY) break;
+        const int mine = first_of<L>(at >> 2, l) + (at & 3), e = A::least(best == m ? mine : kMaxExperts);
+        if (best == m && mine == e) value[at * L + l] = -INFINITY;
+        if (l == k) c = {e, m};
+    }
+    return c;
+}
+
+// The choice in 32 bits: false where they cannot tell.  top, total: the row's largest logit and sum of exponentials (softmax)
+template <bool SOFT, bool SCORED, typename T, int L, int V>
+__device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const float (&z)[V], const float (&b)[V], float bias_most, float top, float total, int l, RowPlace<L, V>* place, Chosen* chosen) {
     using A = Lanes<L>;
     const xq_moe_route& q = a.q;
-    const R kOut = -INFINITY;
+    const float kOut = -INFINITY;
     const int E = q.num_experts, K = q.top_k;
-    const bool has_bias = q.bias != nullptr, grouped = q.top_groups < q.num_groups, soft = q.scoring == XQ_ROUTE_SOFTMAX;
-    const bool two = grouped && q.group_score == XQ_ROUTE_GROUP_SUM2, scored = has_bias || two;
-    const float error = soft ? kSoftmaxError : kSigmoidError;
+    const bool has_bias = SCORED && q.bias != nullptr, grouped = q.top_groups < q.num_groups, two = SCORED && grouped && q.group_score == XQ_ROUTE_GROUP_SUM2;
+    constexpr float error = SOFT ? kSoftmaxError : kSigmoidError;
     bool sure = true;
-    R v[V];                                                // what is compared
-    R* value = (R*)place->value;
-    R* strength = (R*)place->strength;
+    float v[V];                                            // what is compared
+    float* value = place->value;
+    float* strength = place->strength;
     const int size = E / q.num_groups;
     const bool fours = size % 4 == 0;
-    const R over = scored && soft ? reciprocal(total) : (R)1;
+    const float over = SCORED && SOFT ? __builtin_amdgcn_rcpf(total) : 1.0f;
 #pragma unroll
     for (int j = 0; j < V / 4; ++j) {
-        R c[4];                                            // what counts for a group
+        float c[4];                                        // what counts for a group
 #pragma unroll
         for (int k = 0; k < 4; ++k) {
             const int i = j * 4 + k;
-            R s = 0;
-            if (scored) s = soft ? exp_of((R)z[i] - top) * over : reciprocal((R)1 + exp_of(-(R)z[i]));
-            const bool out = z[i] == -INFINITY || b[i] == -INFINITY;
-            v[i] = out ? kOut : has_bias ? s + (R)b[i] : (R)z[i];
-            c[k] = out || !two || has_bias ? v[i] : s;
+            float s = 0.0f;
+            if (SCORED) s = SOFT ? near_exp(z[i] - top) * over : __builtin_amdgcn_rcpf(1.0f + near_exp(-z[i]));
+            const bool out = z[i] == -INFINITY;
+            // (-inf with such a bias too; without one the bias is 0 here)
+            v[i] = out ? kOut : has_bias ? s + b[i] : z[i];
+            c[k] = !SCORED ? z[i] : out ? kOut : has_bias || two ? s + b[i] : z[i];
         }
         if (grouped && fours) {
-            R first = c[0] > c[1] ? c[0] : c[1], second = c[0] > c[1] ? c[1] : c[0];
+            float first = fmaxf(c[0], c[1]), second = fminf(c[0], c[1]);
             take_in(c[2], first, second);
             take_in(c[3], first, second);
-            value[(j * L + l) * 2] = first;
-            value[(j * L + l) * 2 + 1] = second;
+            value[first_of<L>(j, l) / 2] = first;
+            value[first_of<L>(j, l) / 2 + 1] = second;
         } else if (grouped) {
 #pragma unroll
-            for (int k = 0; k < 4; ++k) value[(j * L + l) * 4 + k] = c[k];
+            for (int k = 0; k < 4; ++k) value[first_of<L>(j, l) + k] = c[k];
         }
     }
     if (grouped) {
         wave_fence();
         const int G = q.num_groups, n = fours ? size / 2 : size;
         for (int g = l; g < G; g += L) {
-            R first = kOut, second = kOut;
+            float first = kOut, second = kOut;
 #pragma unroll 8
             for (int k = 0; k < n; ++k) take_in(value[g * n + k], first, second);
-            strength[g] = first + (two && second != kOut ? second : (R)0);
+            strength[g] = first + (two && second != kOut ? second : 0.0f);
         }
         wave_fence();
-        // a group stays if fewer than top_groups are better; float: the weakest that stays and the strongest that goes have to lie apart
-        R least = INFINITY, most = kOut;
+        // a group stays if fewer than top_groups are better; the weakest that stays and the strongest that goes have to lie apart
+        float least = INFINITY, most = kOut;
         uint64_t kept = 0;
         for (int mine = l; mine < G; mine += L) {
-            const R own = strength[mine];
+            const float own = strength[mine];
             int better = 0;
 #pragma unroll 8
             for (int h = 0; h < G; ++h) {
-                const R other = strength[h];
+                const float other = strength[h];
                 better += other > own || (other == own && h < mine);
             }
             if (better < q.top_groups) {
-                least = least < own ? least : own;
+                least = fminf(least, own);
                 kept |= 1ull << mine;
             } else {
-                most = most > own ? most : own;
+                most = fmaxf(most, own);
             }
         }
-        const int lo = A::all((int)(uint32_t)kept, [](int x, int y) { return x | y; }), hi = G > 32 ? A::all((int)(kept >> 32), [](int x, int y) { return x | y; }) : 0;
-        kept = (uint32_t)lo | (uint64_t)(uint32_t)hi << 32;
-        if (sizeof(R) == 4 && scored) {
+        kept = A::bits(kept);
+        if (SCORED) {
             least = -A::largest(-least);
             most = A::largest(most);
             // (two scores and the sums with the bias on either side)
-            if (most != kOut && !(least - most > (R)(2 * error) * (fabsf((float)least) + fabsf((float)most) + 4 * bias_most))) sure = false;
+            if (most != kOut && !(least - most > 2 * error * (fabsf(least) + fabsf(most) + 4 * bias_most))) sure = false;
         }
 #pragma unroll
         for (int j = 0; j < V / 4; ++j) {
-            const int e = (j * L + l) * 4;
+            const int e = first_of<L>(j, l);
             if (fours) {
                 const bool stays = kept >> (__umulhi((uint32_t)e, a.per_group) & 63) & 1;
 #pragma unroll
@@ -250,124 +352,197 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const f
             }
         }
     }
-    const int picks = K + (sizeof(R) == 4 && has_bias ? 1 : 0);
-    int k = 0;
-    for (; k < picks; ++k) {
-        R best = v[0];
+    const int picks = K + (has_bias ? 1 : 0);              // (at most L)
+    Chosen c;
+    bool listed = false;
+    if constexpr (L == 16 && V > 4) {
+        // Many values a lane: the picks are among those that are at least as large as the picks-th of the lanes' largest, which are not many more
+        // (256 values, 9 picks: 13 on average, 22 where half of the groups are out)
+        float best = v[0];
 #pragma unroll
-        for (int i = 1; i < V; ++i) best = best > v[i] ? best : v[i];
-        const R m = A::largest(best);
-        if (m == kOut) break;                              // none left
-        int at = -1;
+        for (int i = 1; i < V; ++i) best = fmaxf(best, v[i]);
+        const float border = A::nth(best, picks);
+        uint32_t mine = 0;
 #pragma unroll
-        for (int i = V - 1; i >= 0; --i) at = v[i] == m ? i : at;
-        const int mine = at >= 0 ? ((at >> 2) * L + l) * 4 + (at & 3) : kMaxExperts, e = A::least(mine);
-        if (mine != e) at = -1;
+        for (int i = 0; i < V; ++i) mine |= (v[i] >= border && v[i] != kOut ? 1u : 0u) << i;
+        const int n = __popc(mine), before = A::before(n), all = A::sum(n);
+        listed = all <= 4 * L;                             // (values in fewer lanes than there are picks, or many equal ones: not)
+        if (listed) {
+            int to = before;
 #pragma unroll
-        for (int i = 0; i < V; ++i) v[i] = i == at ? kOut : v[i];
-        if (l == 0) {
-            place->at[k] = (float)m;
-            place->e[k] = e;
+            for (int i = 0; i < V; ++i)
+                if (mine >> i & 1) {
+                    value[to] = v[i];
+                    place->who[to++] = first_of<L>(i >> 2, l) + (i & 3);
+                }
+            wave_fence();
+            c = all <= 2 * L ? pick_listed<L, 2>(value, place->who, all, picks, l) : pick_listed<L, 4>(value, place->who, all, picks, l);
         }
     }
-    if (l == 0)
-        for (; k < picks; ++k) place->e[k] = -1;
-    wave_fence();
-    if (sizeof(R) == 4 && has_bias)
-        for (int i = l; i + 1 < picks; i += L) {
-            const int e = place->e[i], f = place->e[i + 1];
-            if (e < 0 || f < 0) continue;
-            const float x = place->at[i], y = place->at[i + 1];
-            if (x - y > error * (fabsf(x) + fabsf(y) + 2 * bias_most)) continue;
-            if (logit(row, e) != logit(row, f) || q.bias[e] != q.bias[f]) sure = false;
+    if (!listed) {
+        if constexpr (L == 16 && V > 4) {
+#pragma unroll
+            for (int i = 0; i < V; ++i) value[i * L + l] = v[i];
+            c = pick_stored<L, V>(value, picks, l);
+        } else {
+            int who[V];
+#pragma unroll
+            for (int i = 0; i < V; ++i) who[i] = first_of<L>(i >> 2, l) + (i & 3);
+            c = pick<L, V>(v, who, picks, l);
         }
+    }
+    if (has_bias) {                                        // each against the next
+        const float y = A::next(c.at);
+        const int f = A::next(c.e);
+        if (l + 1 < picks && c.e >= 0 && f >= 0 && !(c.at - y > error * (fabsf(c.at) + fabsf(y) + 2 * bias_most)) &&
+            (logit(row, c.e) != logit(row, f) || q.bias[c.e] != q.bias[f]))
+            sure = false;
+    }
+    *chosen = c;
     return !A::any(!sure);
 }
 
+// The choice in 64 bits, of one row by the whole wave: few rows come here
 template <typename T, int L, int V>
+__device__ __forceinline__ Chosen choose64(const RouteArgs& a, const T* row, float top, int l, WavePlace<L, V>* wave) {
+    using A = Lanes<64>;
+    auto* place = &wave->wide;
+    const xq_moe_route& q = a.q;
+    const double kOut = -INFINITY;
+    const int E = q.num_experts, size = E / q.num_groups;
+    const bool soft = q.scoring == XQ_ROUTE_SOFTMAX, grouped = q.top_groups < q.num_groups, two = q.group_score == XQ_ROUTE_GROUP_SUM2;
+    double total = 0.0;
+    if (soft) {
+#pragma unroll 1
+        for (int e = l; e < E; e += 64) total += exp((double)logit(row, e) - (double)top);
+        total = A::sum(total);
+    }
+    wave_fence();
+    auto score = [&](int e) {
+        const double z = logit(row, e);
+        return z == kOut ? 0.0 : soft ? exp(z - (double)top) / total : 1.0 / (1.0 + exp(-z));
+    };
+#pragma unroll 1
+    for (int e = l; e < E; e += 64) place->value[e] = logit(row, e) == -INFINITY || (q.bias && q.bias[e] == -INFINITY) ? kOut : q.bias || two ? score(e) + (q.bias ? (double)q.bias[e] : 0.0) : (double)logit(row, e);
+    wave_fence();
+    if (grouped) {
+#pragma unroll 1
+        for (int g = l; g < q.num_groups; g += 64) {
+            double first = kOut, second = kOut;
+#pragma unroll 1
+            for (int e = g * size; e < (g + 1) * size; ++e) take_in(place->value[e], first, second);
+            place->strength[g] = first + (two && second != kOut ? second : 0.0);
+        }
+        wave_fence();
+#pragma unroll 1
+        for (int e = l; e < E; e += 64) {
+            const int g = e / size;
+            const double own = place->strength[g];
+            int better = 0;
+#pragma unroll 1
+            for (int h = 0; h < q.num_groups; ++h) better += place->strength[h] > own || (place->strength[h] == own && h < g);
+            if (better >= q.top_groups) place->value[e] = kOut;
+            else if (!q.bias && place->value[e] != kOut) place->value[e] = logit(row, e);
+        }
+        wave_fence();
+    }
+    Chosen c = {-1, 0.0f};
+#pragma unroll 1
+    for (int k = 0; k < q.top_k; ++k) {
+        double best = kOut;
+        int mine = kMaxExperts;
+#pragma unroll 1
+        for (int e = l; e < E; e += 64)
+            if (place->value[e] > best) { best = place->value[e]; mine = e; }
+        const double m = A::largest(best);
+        if (m == kOut) break;
+        const int e = A::least(best == m ? mine : kMaxExperts);
+        if (l == k) c = {e, (float)m};
+        if (l == 0) place->value[e] = kOut;
+        wave_fence();
+    }
+    return c;
+}
+
+template <typename T, int L, int V, bool SOFT, bool SCORED>
 __global__ void __launch_bounds__(64) moe_route_kernel(RouteArgs a) {
     using A = Lanes<L>;
-    __shared__ RowPlace<L, V> places[64 / L];
+    __shared__ WavePlace<L, V> places;
     const xq_moe_route& q = a.q;
-    const int l = threadIdx.x & (L - 1), E = q.num_experts, K = q.top_k;
-    RowPlace<L, V>* place = places + threadIdx.x / L;
-    const bool soft = q.scoring == XQ_ROUTE_SOFTMAX;
-    for (int64_t row = (int64_t)blockIdx.x * (64 / L) + threadIdx.x / L; row < q.n_tokens; row += (int64_t)gridDim.x * (64 / L)) {
-        float z[V], b[V];
-        const T* from = (const T*)q.logits + row * q.ld;
-        load_row<T, L, V>(from, E, a.wide, l, -INFINITY, z);
-        if (q.bias) {
-            load_row<float, L, V>(q.bias, E, a.wide_bias, l, 0.0f, b);
-        } else {
+    const int lane = threadIdx.x & (L - 1), E = q.num_experts, K = q.top_k;
+    RowPlace<L, V>* place = places.rows + threadIdx.x / L;
+    constexpr bool soft = SOFT;
+    float b[V], most = 0.0f;
+    bool bad_bias = false;
+    if (SCORED && q.bias) {
+        load_row<float, L, V>(q.bias, E, a.wide_bias, lane, 0.0f, b);
 #pragma unroll
-            for (int i = 0; i < V; ++i) b[i] = 0.0f;
-        }
-        float top = -INFINITY, most = 0.0f;
-        bool bad = false;
+        for (int i = 0; i < V; ++i) bad_bias |= b[i] != b[i];
+        bad_bias = A::any(bad_bias);
 #pragma unroll
         for (int i = 0; i < V; ++i) {
-            bad |= z[i] != z[i] || b[i] != b[i];
+            b[i] = bad_bias ? 0.0f : b[i];                 // (then no row's choice matters)
+            most = b[i] != -INFINITY ? fmaxf(most, fabsf(b[i])) : most;
+        }
+        most = A::largest(most);
+    } else {
+#pragma unroll
+        for (int i = 0; i < V; ++i) b[i] = 0.0f;
+    }
+    for (int64_t first = (int64_t)blockIdx.x * (64 / L); first < q.n_tokens; first += (int64_t)gridDim.x * (64 / L)) {
+        int l = lane;
+        asm volatile("" : "+v"(l));                        // (what follows from it is worked out again for every row: kept, it is 90 registers)
+        const int64_t row = first + threadIdx.x / L;
+        const bool real = row < q.n_tokens;                // (lanes behind the last row go along with it)
+        const T* from = (const T*)q.logits + (real ? row : q.n_tokens - 1) * q.ld;
+        float z[V], top = -INFINITY;
+        bool bad = bad_bias;
+        load_row<T, L, V>(from, E, a.wide, l, -INFINITY, z);
+#pragma unroll
+        for (int i = 0; i < V; ++i) {
+            bad |= z[i] != z[i];
             top = fmaxf(top, z[i]);
-            if (b[i] != -INFINITY) most = fmaxf(most, fabsf(b[i]));
         }
         top = A::largest(top);
         bad = A::any(bad || (soft && top == INFINITY));
-        most = q.bias ? A::largest(most) : 0.0f;
         if (bad) {
-            for (int k = l; k < K; k += L) {
-                a.weights[row * K + k] = NAN;
-                a.selected[row * K + k] = k;
-            }
-            continue;
+            top = 0.0f;
+#pragma unroll
+            for (int i = 0; i < V; ++i) z[i] = z[i] == -INFINITY ? -INFINITY : 0.0f;       // (a choice among equals, which is not used)
         }
         // the scores' denominator where anything needs it: chosen by scores, or weights that are not renormalized
         float total = 0.0f;
         const bool sums = soft && top != -INFINITY;
-        if (sums && (q.bias || !q.renormalize || (q.group_score == XQ_ROUTE_GROUP_SUM2 && q.top_groups < q.num_groups))) {
+        if (sums && (SCORED || !q.renormalize)) {
 #pragma unroll
-            for (int i = 0; i < V; ++i) total += q.renormalize ? exp_of(z[i] - top) : expf(z[i] - top);
+            for (int i = 0; i < V; ++i) total += q.renormalize ? near_exp(z[i] - top) : expf(z[i] - top);
             total = A::sum(total);
         }
-        if (!choose<float, T, L, V>(a, from, z, b, most, top, total, l, place)) {
-            double total64 = 0.0;
-            if (sums) {
-#pragma unroll
-                for (int i = 0; i < V; ++i) total64 += exp((double)z[i] - (double)top);
-                total64 = A::sum(total64);
-            }
-            choose<double, T, L, V>(a, from, z, b, most, (double)top, total64, l, place);
+        Chosen c;
+        const bool sure = choose<SOFT, SCORED, T, L, V>(a, from, z, b, most, top, total, l, place, &c);
+        for (uint64_t left = __ballot(!sure && !bad && real); left;) {
+            const int of = __builtin_ctzll(left) / L;
+            left &= L == 64 ? 0 : ~(0xffffull << of * L);
+            wave_fence();
+            const Chosen d = choose64<T, L, V>(a, (const T*)q.logits + (first + of) * q.ld, __shfl(top, of * L, 64), threadIdx.x, &places);
+            const int e = __shfl(d.e, l, 64);
+            const float at = __shfl(d.at, l, 64);
+            if ((int)threadIdx.x / L == of) c = {e, at};
         }
         // the weights.  Renormalized: exp(z - largest chosen) under softmax; under sigmoid e^(z - m) / (1 + e^z) with m the largest chosen if that is negative, so
         // that scores which are no fp32 numbers keep their ratios
-        constexpr int N = (kMaxTopK + L - 1) / L;
-        float x[N], w[N], chosen = -INFINITY, sum = 0.0f;
-        int e[N];
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int k = i * L + l;
-            e[i] = k < K ? place->e[k] : -1;
-            x[i] = e[i] < 0 ? -INFINITY : q.bias ? logit(from, e[i]) : place->at[k];
-            chosen = fmaxf(chosen, x[i]);
+        const bool is = l < K && c.e >= 0;
+        const float x = !is ? -INFINITY : SCORED && q.bias ? logit(from, c.e) : c.at, largest = A::largest(x);
+        float w = 0.0f;
+        if (is) {
+            if (soft) w = q.renormalize ? expf(x - largest) : expf(x - top) / total;
+            else if (x >= 0.0f) w = 1.0f / (1.0f + expf(-x));
+            else w = expf(q.renormalize ? x - fminf(largest, 0.0f) : x) / (1.0f + expf(x));
         }
-        chosen = A::largest(chosen);
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            w[i] = 0.0f;
-            if (e[i] >= 0) {
-                if (soft) w[i] = q.renormalize ? expf(x[i] - chosen) : expf(x[i] - top) / total;
-                else if (x[i] >= 0.0f) w[i] = 1.0f / (1.0f + expf(-x[i]));
-                else w[i] = expf(q.renormalize ? x[i] - fminf(chosen, 0.0f) : x[i]) / (1.0f + expf(x[i]));
-            }
-            sum += w[i];
-        }
-        sum = q.renormalize ? A::sum(sum) : 1.0f;
-#pragma unroll
-        for (int i = 0; i < N; ++i) {
-            const int k = i * L + l;
-            if (k < K) {
-                a.weights[row * K + k] = sum > 0.0f ? q.scale * (w[i] / sum) : 0.0f;
-                a.selected[row * K + k] = e[i];
-            }
+        const float sum = q.renormalize ? A::sum(w) : 1.0f;
+        if (real && l < K) {
+            a.weights[row * K + l] = bad ? NAN : sum > 0.0f ? q.scale * (w / sum) : 0.0f;
+            a.selected[row * K + l] = bad ? l : is ? c.e : -1;
         }
         wave_fence();                                      // (the place is the next row's)
     }
@@ -418,7 +593,7 @@ __global__ void __launch_bounds__(64) moe_route_grad_kernel(RouteGradArgs a) {
             total = A::sum(total);
         }
 #pragma unroll
-        for (int j = 0; j < V / 4; ++j) *(f32x4*)(place + (j * L + l) * 4) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int j = 0; j < V / 4; ++j) *(f32x4*)(place + first_of<L>(j, l)) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         wave_fence();
 #pragma unroll
         for (int i = 0; i < N; ++i)
@@ -437,7 +612,7 @@ __global__ void __launch_bounds__(64) moe_route_grad_kernel(RouteGradArgs a) {
         wave_fence();
 #pragma unroll
         for (int j = 0; j < V / 4; ++j) {
-            const int e = (j * L + l) * 4;
+            const int e = first_of<L>(j, l);
             f32x4 d = *(const f32x4*)(place + e);
 #pragma unroll
             for (int i = 0; i < 4; ++i) {
@@ -471,9 +646,15 @@ constexpr int64_t kFewRows = 2048;
 template <typename T, int L, int V>
 void launch(const RouteArgs* f, const RouteGradArgs* g, hipStream_t st) {
     const xq_moe_route& q = f ? f->q : g->q;
-    const dim3 blocks((unsigned)std::min<int64_t>(xq_cdiv(q.n_tokens, 64 / L), 1 << 24));
-    if (f) moe_route_kernel<T, L, V><<<blocks, 64, 0, st>>>(*f);
-    else moe_route_grad_kernel<T, L, V><<<blocks, 64, 0, st>>>(*g);
+    const dim3 blocks((unsigned)std::min<int64_t>(xq_cdiv(q.n_tokens, 64 / L), 4096));        // (16 waves a compute unit; then several rows each, the bias read once)
+    if (f) {
+        const bool scored = q.bias || (q.group_score == XQ_ROUTE_GROUP_SUM2 && q.top_groups < q.num_groups);
+        if (q.scoring == XQ_ROUTE_SOFTMAX) scored ? moe_route_kernel<T, L, V, true, true><<<blocks, 64, 0, st>>>(*f) : moe_route_kernel<T, L, V, true, false><<<blocks, 64, 0, st>>>(*f);
+        else scored ? moe_route_kernel<T, L, V, false, true><<<blocks, 64, 0, st>>>(*f) : moe_route_kernel<T, L, V, false, false><<<blocks, 64, 0, st>>>(*f);
+    }
+    else {
+        moe_route_grad_kernel<T, L, V><<<blocks, 64, 0, st>>>(*g);
+    }
 }
 template <typename T>
 void launch(const RouteArgs* f, const RouteGradArgs* g, hipStream_t st) {
@@ -481,7 +662,7 @@ void launch(const RouteArgs* f, const RouteGradArgs* g, hipStream_t st) {
     const int E = q.num_experts;
     if (E > 512) launch<T, 64, 16>(f, g, st);
     else if (E > 256) launch<T, 64, 8>(f, g, st);
-    else if (q.n_tokens <= kFewRows) launch<T, 64, 4>(f, g, st);
+    else if (q.n_tokens <= kFewRows || q.top_k > 15) launch<T, 64, 4>(f, g, st);
     else if (E > 128) launch<T, 16, 16>(f, g, st);
     else if (E > 64) launch<T, 16, 8>(f, g, st);
     else launch<T, 16, 4>(f, g, st);
