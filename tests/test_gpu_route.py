@@ -253,6 +253,62 @@ def test_what_is_no_number_stays_in_its_row(hip_device, scoring, renormalize):
     assert moe_route(zg, 5, scoring=scoring, renormalize=renormalize, bias=b)[0].isnan().all()
 
 
+def _kinds(E, dtype, device):
+    """Rows of every kind: ordinary, few left, none, all equal, two values, a run of equal ones, nearly equal, not numbers (the last two, by index)"""
+    z, _ = _inputs(24, E, dtype, E, device, off=0.0)
+    z[1, 3:] = -math.inf
+    z[2] = -math.inf
+    z[3] = 0.25
+    z[4] = torch.where(torch.arange(E, device=device) % 3 == 0, 1.0, 0.5).to(dtype)
+    z[5, E // 2:] = 3.0
+    z[6, :-1] = -math.inf
+    z[7, 20:E - 20] = -math.inf
+    z[8] = torch.linspace(1.0, 1.00001, E, device=device).to(dtype)
+    z[9, ::2] = -math.inf
+    z[10, :90] = 2.0
+    z[22, E - 1], z[23, 0] = math.nan, math.nan
+    return z
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("E, k, groups, top_groups, score", [(100, 15, 1, 1, "sum2"), (128, 8, 8, 4, "max"), (160, 9, 10, 3, "sum2"), (203, 15, 1, 1, "max"), (256, 8, 8, 4, "sum2"),
+                                                            (256, 8, 8, 1, "max"), (64, 15, 2, 1, "sum2"), (240, 12, 60, 7, "sum2")])
+@pytest.mark.parametrize("scoring, with_bias", [("softmax", False), ("sigmoid", True), ("softmax", True)])
+def test_many_rows_of_every_kind(hip_device, E, k, groups, top_groups, score, scoring, with_bias, dtype):
+    """More rows than are done one a wave, in an order in which every kind is next to every other: each has what it has alone"""
+    pool = _kinds(E, dtype, hip_device)
+    bias = 0.1 * torch.randn(E, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(1)) if with_bias else None
+    if with_bias:
+        s = torch.sigmoid(pool[11].double()) if scoring == "sigmoid" else torch.softmax(pool[11].double(), 0)
+        bias[:E // 2] = (0.75 - s[:E // 2]).float()            # half of this row's sums are nearly equal
+    o = dict(top_k=k, scoring=scoring, num_groups=groups, top_groups=top_groups, group_score=score, renormalize=True, scale=2.5)
+    w0, i0, s0 = _reference(pool[:22], o, bias)
+    at = torch.randint(0, 24, (2 * 2048 + 3,), generator=torch.Generator().manual_seed(E))
+    good, bad = (at < 22).nonzero()[:, 0], (at >= 22).nonzero()[:, 0]
+    z = pool[at.to(hip_device)].requires_grad_(True)
+    w, ids = moe_route(z, bias=bias, **o)
+    up = torch.randn(w.shape, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(3))
+    dz, = torch.autograd.grad(w, z, up)
+    want = (w0[at[good]], i0[at[good]], s0[at[good]])
+    _check(z.detach()[good.to(hip_device)], (w.detach()[good.to(hip_device)], ids[good.to(hip_device)]), want)
+    want_dz, mag = gradient(z, up[good.to(hip_device)], *want, scoring, True, 2.5)
+    bound = (2 * 20 + 64 + 40 + 40) * U * mag + (B if dtype == BF else 0.0) * want_dz.abs() + 2.0 ** -120
+    assert ((dz[good.to(hip_device)].double().cpu() - want_dz).abs() <= bound).all()
+    bad = bad.to(hip_device)
+    assert w[bad].isnan().all() and dz[bad].isnan().all() and (ids[bad] == torch.arange(k, device=hip_device)).all()
+
+
+@pytest.mark.parametrize("E", [15, 9, 32])
+def test_all_experts_chosen_beside_rows_that_are_no_numbers(hip_device, E):
+    z, bias = _inputs(7, E, torch.float32, E, hip_device, True)
+    z[2, 1], z[6, E - 1] = math.nan, math.nan
+    w, ids = moe_route(z, E, scoring="sigmoid", bias=bias)
+    good = [0, 1, 3, 4, 5]
+    o = dict(top_k=E, scoring="sigmoid", num_groups=1, top_groups=1, group_score="max", renormalize=True, scale=1.0)
+    _check(z[good], (w[good], ids[good]), _reference(z[good], o, bias))
+    assert w[[2, 6]].isnan().all() and (ids[[2, 6]] == torch.arange(E, device=hip_device)).all()
+
+
 # ---------------------------------------------------------------- layouts, sizes, streams
 def _layouts(z):
     T, E = z.shape

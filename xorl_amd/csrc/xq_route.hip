@@ -30,15 +30,19 @@ struct RouteGradArgs {
     bool wide, wide_dz;
 };
 
+// What bounds it: a row is read once and a few numbers of it written, but a choice is a chain of maxima over lanes, about 1500 instructions for four rows of 256 with
+// groups and a bias.  Their issue is 41 of the 60 us that 65536 such rows take (the reads alone would be 14); 16384 rows of 128 take 8.4 us.  Small calls are one launch:
+// one row 4.5 us, 333 rows of 256 in groups 7.5.
+//
 // L lanes have a row (16: four rows a wave, sums and maxima within a quarter of it are register moves), V logits each, four neighbours at a time; of 16 lanes each
 // next such round begins four lanes on, so that the experts of a few groups are not all in a few lanes.  A block is one wave: what goes through LDS needs no
-// barrier.
+// barrier.  With one row a wave and the same steps 65536 rows in groups took 154 us.
 //
 // Without a bias the order is that of the logits, exactly.  A score with a bias is compared as fp32 where that tells the chosen apart from each other and from the
-// first that is left out: sums whose difference is within their error, of experts that differ in logit or bias, send the row to be done again in 64 bits, which is the definition.
-// Groups by two scores likewise, at the border between those that stay and those that go.  Errors, in steps of 2^-24 of a score: sigmoid 4 for the exponential, 2 for
-// sum and quotient; softmax 88 for the difference in the exponent (below that there is no score), 4, 22 for the sum (16 terms a lane, 6 steps), 1; one
-// more, of itself, for the sum with the bias.
+// first that is left out: sums whose difference is within their error, of experts that differ in logit or bias, send the row to be done again in 64 bits, which is
+// the definition (every score in 64 bits: 524 us).  Groups by two scores likewise, at the border between those that stay and those that go.  Errors, in steps of
+// 2^-24 of a score: sigmoid 4 for the exponential, 2 for sum and quotient; softmax 88 for the difference in the exponent (below that there is no score), 4, 22 for
+// the sum (16 terms a lane, 6 steps), 1; one more, of itself, for the sum with the bias.
 constexpr float kSigmoidError = 0x1p-20f, kSoftmaxError = 0x1p-17f;
 
 template <int L>
@@ -92,7 +96,7 @@ struct Lanes {
     template <typename T>
     static __device__ __forceinline__ T sum(T v) { return all(v, [](T a, T b) { return a + b; }); }
     static __device__ __forceinline__ int least(int v) { return all(v, [](int a, int b) { return min(a, b); }); }
-    // (L 16) the n-th largest of the lanes' values, and the sum of the lanes before
+    // (L 16) the n-th largest of the lanes' values
     template <typename T>
     static __device__ __forceinline__ T nth(T v, int n) {
         int larger = 0;
@@ -109,6 +113,7 @@ struct Lanes {
         return L == 16 ? __builtin_amdgcn_update_dpp(0, v, 0x101, 0xf, 0xf, true) : __shfl_down(v, 1, 64);
     }
     static __device__ __forceinline__ float next(float v) { return __uint_as_float((uint32_t)next((int)__float_as_uint(v))); }
+    // (L 16) the sum of the lanes before
     static __device__ __forceinline__ int before(int v) {
         int u = v;
         u += __builtin_amdgcn_update_dpp(0, u, 0x111, 0xf, 0xf, true);      // from 1, 2, 4, 8 lanes below in the row, 0 where there is none
@@ -408,58 +413,68 @@ __device__ __forceinline__ Chosen choose64(const RouteArgs& a, const T* row, flo
     using A = Lanes<64>;
     auto* place = &wave->wide;
     const xq_moe_route& q = a.q;
+    constexpr int N = L * V / 64, kTogether = N < 4 ? N : 4;          // experts a lane, l, l + 64, ..
     const double kOut = -INFINITY;
     const int E = q.num_experts, size = E / q.num_groups;
-    const bool soft = q.scoring == XQ_ROUTE_SOFTMAX, grouped = q.top_groups < q.num_groups, two = q.group_score == XQ_ROUTE_GROUP_SUM2;
+    const bool soft = q.scoring == XQ_ROUTE_SOFTMAX, grouped = q.top_groups < q.num_groups, two = q.group_score == XQ_ROUTE_GROUP_SUM2, scored = q.bias || (grouped && two);
     double total = 0.0;
-    if (soft) {
-#pragma unroll 1
-        for (int e = l; e < E; e += 64) total += exp((double)logit(row, e) - (double)top);
-        total = A::sum(total);
+    if (scored) {
+#pragma unroll kTogether
+        for (int i = 0; i < N; ++i) {
+            const double z = i * 64 + l < E ? (double)logit(row, i * 64 + l) : kOut;
+            const double x = exp(soft ? z - (double)top : -z);
+            place->value[i * 64 + l] = soft ? x : 1.0 / (1.0 + x);
+            total += x;
+        }
+        total = soft ? A::sum(total) : 1.0;
     }
-    wave_fence();
-    auto score = [&](int e) {
-        const double z = logit(row, e);
-        return z == kOut ? 0.0 : soft ? exp(z - (double)top) / total : 1.0 / (1.0 + exp(-z));
-    };
 #pragma unroll 1
-    for (int e = l; e < E; e += 64) place->value[e] = logit(row, e) == -INFINITY || (q.bias && q.bias[e] == -INFINITY) ? kOut : q.bias || two ? score(e) + (q.bias ? (double)q.bias[e] : 0.0) : (double)logit(row, e);
-    wave_fence();
+    for (int e = l; e < 64 * N; e += 64) {
+        const int at = min(e, E - 1);
+        const double z = logit(row, at), bias = q.bias ? (double)q.bias[at] : 0.0;
+        place->value[e] = e >= E || z == kOut || bias == kOut ? kOut : scored ? place->value[e] / total + bias : z;
+    }
     if (grouped) {
-#pragma unroll 1
-        for (int g = l; g < q.num_groups; g += 64) {
+        wave_fence();
+        if (l < q.num_groups) {
             double first = kOut, second = kOut;
-#pragma unroll 1
-            for (int e = g * size; e < (g + 1) * size; ++e) take_in(place->value[e], first, second);
-            place->strength[g] = first + (two && second != kOut ? second : 0.0);
+#pragma unroll 4
+            for (int e = l * size; e < (l + 1) * size; ++e) take_in(place->value[e], first, second);
+            place->strength[l] = first + (two && second != kOut ? second : 0.0);
         }
         wave_fence();
+        const double own = l < q.num_groups ? place->strength[l] : kOut;
+        int better = 0;
+#pragma unroll 4
+        for (int h = 0; h < q.num_groups; ++h) {
+            const double other = place->strength[h];
+            better += other > own || (other == own && h < l);
+        }
+        const uint64_t kept = __ballot(l < q.num_groups && better < q.top_groups);
 #pragma unroll 1
         for (int e = l; e < E; e += 64) {
-            const int g = e / size;
-            const double own = place->strength[g];
-            int better = 0;
-#pragma unroll 1
-            for (int h = 0; h < q.num_groups; ++h) better += place->strength[h] > own || (place->strength[h] == own && h < g);
-            if (better >= q.top_groups) place->value[e] = kOut;
+            if (!(kept >> (e / size) & 1)) place->value[e] = kOut;
             else if (!q.bias && place->value[e] != kOut) place->value[e] = logit(row, e);
         }
-        wave_fence();
     }
+    double v[N];                                           // (what this lane wrote)
+#pragma unroll
+    for (int i = 0; i < N; ++i) v[i] = place->value[i * 64 + l];
     Chosen c = {-1, 0.0f};
 #pragma unroll 1
     for (int k = 0; k < q.top_k; ++k) {
-        double best = kOut;
-        int mine = kMaxExperts;
-#pragma unroll 1
-        for (int e = l; e < E; e += 64)
-            if (place->value[e] > best) { best = place->value[e]; mine = e; }
+        double best = v[0];
+#pragma unroll
+        for (int i = 1; i < N; ++i) best = v[i] > best ? v[i] : best;
         const double m = A::largest(best);
         if (m == kOut) break;
-        const int e = A::least(best == m ? mine : kMaxExperts);
+        int mine = kMaxExperts;
+#pragma unroll
+        for (int i = N - 1; i >= 0; --i) mine = v[i] == m ? i * 64 + l : mine;
+        const int e = A::least(mine);
+#pragma unroll
+        for (int i = 0; i < N; ++i) v[i] = i * 64 + l == e ? kOut : v[i];
         if (l == k) c = {e, (float)m};
-        if (l == 0) place->value[e] = kOut;
-        wave_fence();
     }
     return c;
 }
@@ -641,12 +656,15 @@ __global__ void __launch_bounds__(64) moe_route_grad_kernel(RouteGradArgs a) {
 // four elements at a time: whole fours, at addresses that are multiples of them
 bool in_fours(const void* p, int dtype, int64_t rows, int64_t ld, int E) { return p && E % 4 == 0 && (rows <= 1 || ld % 4 == 0) && xq_aligned(p, dtype == XQ_DT_F32 ? 16 : 8); }
 
+// From 129 to 256 experts few rows are done by 64 lanes each, whose chain is shorter, many by 16.  Sigmoid with a bias in groups, 64 against 16 lanes: one row 6.6 and
+// 8.9 us, 512 rows 7.2 and 9.4, 4096 17.4 and 16.0, 8192 25 and 17.  Up to 128 experts 16 lanes are never behind (128: one row 4.5 and 4.6, 2048 rows 5.7 and 5.0, 8192 13.1
+// and 5.7).  Rows of more choices than 16 lanes can hold, with the one behind them, take 64.
 constexpr int64_t kFewRows = 2048;
 
 template <typename T, int L, int V>
 void launch(const RouteArgs* f, const RouteGradArgs* g, hipStream_t st) {
     const xq_moe_route& q = f ? f->q : g->q;
-    const dim3 blocks((unsigned)std::min<int64_t>(xq_cdiv(q.n_tokens, 64 / L), 4096));        // (16 waves a compute unit; then several rows each, the bias read once)
+    const dim3 blocks((unsigned)std::min<int64_t>(xq_cdiv(q.n_tokens, 64 / L), 4096));        // (the 16 waves that a compute unit holds at 128 registers; then several rows each, the bias read once)
     if (f) {
         const bool scored = q.bias || (q.group_score == XQ_ROUTE_GROUP_SUM2 && q.top_groups < q.num_groups);
         if (q.scoring == XQ_ROUTE_SOFTMAX) scored ? moe_route_kernel<T, L, V, true, true><<<blocks, 64, 0, st>>>(*f) : moe_route_kernel<T, L, V, true, false><<<blocks, 64, 0, st>>>(*f);
@@ -662,7 +680,7 @@ void launch(const RouteArgs* f, const RouteGradArgs* g, hipStream_t st) {
     const int E = q.num_experts;
     if (E > 512) launch<T, 64, 16>(f, g, st);
     else if (E > 256) launch<T, 64, 8>(f, g, st);
-    else if (q.n_tokens <= kFewRows || q.top_k > 15) launch<T, 64, 4>(f, g, st);
+    else if (q.top_k > 15 || (E > 128 && q.n_tokens <= kFewRows)) launch<T, 64, 4>(f, g, st);
     else if (E > 128) launch<T, 16, 16>(f, g, st);
     else if (E > 64) launch<T, 16, 8>(f, g, st);
     else launch<T, 16, 4>(f, g, st);
