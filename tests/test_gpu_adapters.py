@@ -75,6 +75,19 @@ def test_more_adapters_than_a_launch_has_threads(hip_device):
     _check(lora_adapters(*a), *a)
 
 
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("M", [15, 16, 33, 64, 65, 255, 256, 511, 512, 513, 1024])
+def test_where_rows_change_their_tiles(hip_device, M, dtype):
+    """Each way that rows become tiles, up to its last row: every row its own adapter, all of one, in turn, 16 of each, 17 of each, none and one"""
+    a = list(_inputs(M, 272, 128, 24, M, dtype, M, hip_device, without=0.0))
+    i = torch.arange(M, device=hip_device)
+    for ids in (i, i.flip(0), i * 0, i % 2, i % 5, i // 16, i // 17, i % 17 - 1, torch.where(i == M - 1, 3, -1), torch.where(i < M - 1, 3, -1)):
+        a[4] = ids.to(torch.int64)
+        out = lora_adapters(*a)
+        _check(out, *a)
+        assert torch.equal(lora_adapters(*a), out)
+
+
 def test_no_adapters_and_no_rows(hip_device):
     a = _inputs(20, 32, 64, 4, 3, BF, 2, hip_device)
     none = lora_adapters(a[0], a[1], a[2][:0], a[3][:0], a[4], a[5][:0])

@@ -10,16 +10,23 @@ namespace {
 // Two launches: t = x A_a^T in parts of K, fp32, to the workspace; then out = base + (s t) B_a^T.  Both multiply on 16x16x32 MFMA tiles straight from memory:
 // all four operands have the contraction along their rows, so that a lane's eight elements are one 16-byte load.  t goes into the second product as two bf16
 // numbers (16 bits: one would lose as much of a large update as the result's own rounding), laid out along the contraction: lanes 0-31 hold the high
-// halves of 16 ranks, lanes 32-63 the low ones, and B's 16 ranks stand in both, so that 16 ranks are one MFMA.  fp32 factors are two bf16 numbers in the same way.
+// halves of 16 ranks, lanes 32-63 the low ones, and B's 16 ranks stand in both, so that 16 ranks are one MFMA.  fp32 factors are two bf16 numbers in the same way
+// (an infinity's low half is NaN, and so is what it has a part in).
 //
-// A tile is rows of one adapter.  Up to kLeaderRows rows in any order: tile b belongs to the row b if that is the first, 17th, 33rd .. of its adapter, and its
-// block finds the rows itself among the ids (no launch that sorts them).  More rows are taken in windows of 16 or 64 that follow each other, and a window once for
-// every adapter in it: of prompts' rows, each window has one or two.
-constexpr int kLeaderRows = 1024;
-constexpr int kMostParts = 16;
+// What bounds it: few rows, the latency of two launches that each wait for memory two or three times (one row 8 us, 48 of 8 adapters 9.8 us); many, memory: 16384 rows of
+// prompts, 12288 by 4096, rank 64, read and write 0.68 GB, 139 us at a copy's rate, and take 176 (down 104 us, up 73).  Between them (2049 rows, 46 us against 27) the
+// blocks are too few to keep all of memory busy and the whole is three or four of their lifetimes.
+//
+// A tile is rows of one adapter.  Up to kLeaderRows rows in any order: a tile belongs to the row that is the first, 17th, 33rd .. of its adapter, and the first
+// launch's blocks find the tiles themselves among the ids (no launch that sorts them), and leave them to the second.  Up to 64 rows a block has one row to look at, then
+// four: half of all blocks would do no more than find that their row leads none (1024 rows 81 against 41 us, 64 rows 9.7 against 10.2).  More rows are taken in
+// windows of 16 or 64 that follow each other, and a window once for every adapter in it: of prompts' rows, each window has one or two.  By tiles against by windows, 4096 by
+// 4096, 8 adapters: rank 16, 256 rows in any order 16 and 49 us, 512 27 and 49, 1024 36 and 54; sorted by adapter 17 and 18, 27 and 18, 39 and 17.
+constexpr int kLeaderRows = 512;
+constexpr int kMostParts = 16, kLeadsNone = -2;
 
 struct AdapterPlan {
-    int32_t leaders;      // tiles found by their first row
+    int32_t leaders;      // tiles are found by their first row: how many rows a block looks at, 1 to 16; or 0
     int32_t down_subs, up_subs;      // 16-row pieces of a window: 1 or 4
     int32_t down_tiles, up_tiles;
     int32_t parts;        // of K
@@ -29,6 +36,7 @@ struct AdapterArgs {
     xq_adapters q;
     AdapterPlan p;
     float* t;             // [parts][M][r_pad]
+    int32_t* led;         // [M][16]: the rows of a leader's tile, or -1; kLeadsNone in the first place of a row that leads none
     int32_t r_pad;
 };
 
@@ -47,23 +55,29 @@ __device__ __forceinline__ bool leader_rows(const xq_adapters& q, int lead, int*
     const int mine = uniform(adapter_of(q, lead));
     *id = mine;
     int before = 0, seen = 0, want = lane & 15, found = -1;
-    for (int c = 0; c < M; c += 64) {
-        const int i = c + lane;
-        uint64_t same = __ballot(i < M && adapter_of(q, min(i, M - 1)) == mine);
-        if (lead >= c + 64) { before += __popcll(same); continue; }
-        if (lead > c) {
-            const uint64_t below = (1ull << (lead - c)) - 1;
-            before += __popcll(same & below);
-            same &= ~below;
+    for (int c0 = 0; c0 < M; c0 += 256) {
+        int ids[4];                                        // (four loads on their way)
+#pragma unroll
+        for (int u = 0; u < 4; ++u) ids[u] = adapter_of(q, min(c0 + u * 64 + lane, M - 1));
+#pragma unroll
+        for (int u = 0; u < 4; ++u) {
+            const int c = c0 + u * 64;
+            uint64_t same = __ballot(c + lane < M && ids[u] == mine);
+            if (lead >= c + 64) { before += __popcll(same); continue; }
+            if (lead > c) {
+                const uint64_t below = (1ull << (lead - c)) - 1;
+                before += __popcll(same & below);
+                same &= ~below;
+            }
+            if (before & 15) return false;
+            const int n = __popcll(same);
+            if (want >= seen && want < seen + n) {
+                uint64_t m = same;
+                for (int k = want - seen; k > 0; --k) m &= m - 1;
+                found = c + __ffsll((unsigned long long)m) - 1;
+            }
+            seen += n;
         }
-        if (before & 15) return false;
-        const int n = __popcll(same);
-        if (want >= seen && want < seen + n) {
-            uint64_t m = same;
-            for (int k = want - seen; k > 0; --k) m &= m - 1;
-            found = c + __ffsll((unsigned long long)m) - 1;
-        }
-        seen += n;
         if (seen >= 16) break;
     }
     *row = found;
@@ -118,7 +132,7 @@ __device__ __forceinline__ Raw<F32> load_raw_n(const void* p, int64_t at, int n)
 
 // An MFMA operand has 16 rows in neighbouring lanes; a load that asks for it so touches a cache line a lane.  So rows are loaded whole cache lines at a time, eight
 // lanes on each, and the lanes exchange them through LDS, a wave in a place of its own, pieces of 16 bytes exclusive-ored so that neither side
-// meets a bank twice.  (16384 rows, K 12288, rank 64, us: @DIRECT@)
+// meets a bank twice.  (16384 rows, K 12288, rank 64, us: operands loaded as they lie 133 down and 106 up, exchanged in pieces of 64 bytes 122, in cache lines 104 and 76)
 __device__ __forceinline__ void wave_fence() {
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     __builtin_amdgcn_wave_barrier();
@@ -271,7 +285,7 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const in
 }
 
 // Blocks go to the eight XCDs in turn: neighbouring items, which are of one adapter as a rule, go to one of them, so that each reads few adapters through its L2
-// (16384 rows of 8 adapters whose A have 1.5 MB each: @XCD@)
+// (16384 rows of 8 adapters whose A have 1.5 MB each: down 208 us in turn and 174 so, up 118 and 106)
 __device__ __forceinline__ int64_t item_of(int64_t at, int64_t n) {
     const int64_t each = n / 8, rest = n - each * 8, xcd = at & 7, i = at >> 3;
     return at >= each * 8 + rest ? at : xcd * each + min(xcd, rest) + i;
@@ -281,15 +295,32 @@ template <int SUBS, int RB, bool F32>
 __global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
     __shared__ __attribute__((aligned(16))) float red[4 * kPlaceKb * 256];       // (and the waves' sums: at most 2 * SUBS * RB KB)
     static_assert(2 * SUBS * RB <= 4 * kPlaceKb, "");
-    const int lane = threadIdx.x & 63;
+    __shared__ int found[16][16];
+    const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int64_t items = (int64_t)a.p.down_tiles * a.p.parts;
     for (int64_t b = blockIdx.x; b < items; b += gridDim.x) {
         const int64_t at = a.p.leaders ? b : item_of(b, items);
         const int tile = (int)(at / a.p.parts), part = (int)(at - (int64_t)tile * a.p.parts);
         if (a.p.leaders) {
-            int id, row[1];
-            if (!leader_rows(a.q, tile, &id, &row[0]) || id < 0) continue;
-            down_tile<1, RB, F32>(a, id, row, part, tile, red);
+            // the waves look at the rows in turn, and the block does the tiles of those that lead one after the other
+            const int each = a.p.leaders;
+            __syncthreads();                               // (the rows before have been read)
+            for (int j = wave; j < each; j += 4) {
+                const int lead = tile + j * a.p.down_tiles;
+                int id, row = -1;
+                const bool leads = lead < a.q.M && leader_rows(a.q, lead, &id, &row);
+                if (lane < 16) {
+                    found[j][lane] = leads ? row : kLeadsNone;
+                    if (part == 0 && lead < a.q.M) a.led[lead * 16 + lane] = leads ? row : kLeadsNone;
+                }
+            }
+            __syncthreads();
+            for (int j = 0; j < each; ++j) {
+                const int one[1] = {found[j][lane & 15]}, of = uniform(one[0]);
+                if (of == kLeadsNone) continue;
+                const int id = uniform(adapter_of(a.q, of));
+                if (id >= 0) down_tile<1, RB, F32>(a, id, one, part, tile + j * a.p.down_tiles, red);
+            }
             continue;
         }
         // a window of SUBS * 16 rows: once for every adapter in it
@@ -525,7 +556,7 @@ template <int SUBS, int RB, bool F32, bool WHOLE>
 __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
     constexpr int kb = SUBS > 1 ? RB * (F32 ? 2 : 1) + 2 : 0;
     __shared__ bf16x8 ts[SUBS * RB * 64];
-    __shared__ u32x4 exchange[4 * kb * 64 + 1];
+    __shared__ u32x4 exchange[4 * kb * 64 + 1];           // (SUBS 1 has no use for it, and an array no zero elements)
     const int lane = threadIdx.x & 63;
     const int64_t chunks = (a.q.N + a.p.cols - 1) / a.p.cols, items = a.p.up_tiles * chunks;
     for (int64_t b = blockIdx.x; b < items; b += gridDim.x) {
@@ -533,8 +564,10 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
         const int tile = (int)(at / chunks);
         const int64_t n0 = (at - tile * chunks) * a.p.cols, n1 = min(n0 + a.p.cols, a.q.N);
         if (SUBS == 1 && a.p.leaders) {
-            int id, row;
-            if (leader_rows(a.q, tile, &id, &row)) up_piece<RB, F32, WHOLE>(a, id, row, n0, n1, ts);
+            for (int lead = tile; lead < a.q.M; lead += a.p.up_tiles) {
+                const int row = a.led[lead * 16 + (lane & 15)];
+                if (uniform(row) != kLeadsNone) up_piece<RB, F32, WHOLE>(a, uniform(adapter_of(a.q, lead)), row, n0, n1, ts);
+            }
             continue;
         }
         const int64_t row0 = (int64_t)tile * (SUBS * 16);
@@ -559,16 +592,19 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
 
 AdapterPlan plan_adapters(int64_t M, int64_t N, int64_t K, int r) {
     AdapterPlan p;
-    p.leaders = M <= kLeaderRows;
+    p.leaders = M > kLeaderRows ? 0 : M > 64 ? 4 : 1;
+    // (rank 16 and 64, rows sorted by adapter, 16 against 64 rows: 4096 rows 28 and 48 against 34 and 67 us, 16384 109 and 140 against 110 and 132; in any order 330 and 603 against 288 and 460)
     p.down_subs = p.leaders || M < 8192 ? 1 : 4;
     p.up_subs = p.leaders || r % 8 != 0 ? 1 : 4;           // (ranks that are no multiple of 8 are read one by one: 16 rows at a time)
-    p.down_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.down_subs * 16));
-    p.up_tiles = (int32_t)(p.leaders ? M : xq_cdiv(M, p.up_subs * 16));
+    // (a block's rows lie apart by an odd number: those that lead are often the first ones, or every 16th)
+    const int64_t led = p.leaders > 1 ? xq_cdiv(M, p.leaders) | 1 : M;
+    p.down_tiles = (int32_t)(p.leaders ? led : xq_cdiv(M, p.down_subs * 16));
+    p.up_tiles = (int32_t)(p.leaders ? led : xq_cdiv(M, p.up_subs * 16));
     // parts that bring two blocks to every compute unit where the tiles do not, of at least two cache lines of x a wave
     const int64_t full = xq_cdiv(M, p.down_subs * 16), units = K / 64;
     p.parts = (int32_t)std::max<int64_t>(1, std::min<int64_t>({512 / std::max<int64_t>(full, 1), units / 8, kMostParts}));
     // columns of a block: fewer blocks repeat the reading of t and its roundings less, as long as there are four of them a compute unit
-    p.cols = p.leaders ? 128 : p.up_tiles * xq_cdiv(N, 1024) >= 1024 ? 1024 : p.up_tiles * xq_cdiv(N, 512) >= 1024 ? 512 : 256;
+    p.cols = p.leaders ? (xq_cdiv(M, 16) * xq_cdiv(N, 256) >= 1024 ? 256 : 128) : p.up_tiles * xq_cdiv(N, 1024) >= 1024 ? 1024 : p.up_tiles * xq_cdiv(N, 512) >= 1024 ? 512 : 256;
     return p;
 }
 int r_pad(int r) { return (r + 15) / 16 * 16; }
@@ -604,7 +640,8 @@ using namespace xq;
 
 extern "C" int64_t xq_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r) {
     if (!sizes_fit(M, N, K, r)) return -1;
-    return std::max<int64_t>((int64_t)plan_adapters(M, N, K, r).parts * M * r_pad(r) * 4, 256);
+    const AdapterPlan p = plan_adapters(M, N, K, r);
+    return std::max<int64_t>((int64_t)p.parts * M * r_pad(r) * 4 + (p.leaders ? M * 64 : 0), 256);
 }
 
 extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t workspace_bytes, void* stream) {
@@ -625,7 +662,8 @@ extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t wo
     XQ_REQUIRE(workspace && xq_aligned(workspace, 256) && workspace_bytes >= xq_adapters_workspace_bytes(q->M, q->N, q->K, q->r),
                "xq_adapters_add: a workspace of %lld bytes, 256-byte aligned, is needed", (long long)xq_adapters_workspace_bytes(q->M, q->N, q->K, q->r));
     hipStream_t st = (hipStream_t)stream;
-    const AdapterArgs a = {*q, plan_adapters(q->M, q->N, q->K, q->r), (float*)workspace, r_pad(q->r)};
+    AdapterArgs a = {*q, plan_adapters(q->M, q->N, q->K, q->r), (float*)workspace, nullptr, r_pad(q->r)};
+    a.led = (int32_t*)(a.t + (int64_t)a.p.parts * q->M * a.r_pad);
     q->factor_dtype == XQ_DT_F32 ? launch_adapters<true>(a, st) : launch_adapters<false>(a, st);
     XQ_CHECK_LAUNCH("xq_adapters_add");
     return XQ_OK;
