@@ -63,6 +63,15 @@ def test_refusals(over):
     assert b"xq_adapters_add" in _C.lib().xq_last_error()
 
 
+@pytest.mark.parametrize("over", [dict(K=1 << 23, ldx=1 << 23), dict(N=1 << 24, ld_base=1 << 24, ld_out=1 << 24), dict(M=1 << 24)])
+def test_the_largest_sizes(over):
+    """The first size that is too large is refused as a size, the one before only for the workspace that it does not have"""
+    assert _run(**over) == -1 and b"must be a multiple of 64 below" in _C.lib().xq_last_error()
+    step = {"K": 64, "N": 16, "M": 1}[next(iter(over))]
+    below = {k: v - step if k in "MNK" else v for k, v in over.items()}
+    assert _run(ws=None, **below) == -1 and b"workspace" in _C.lib().xq_last_error()
+
+
 def test_sizes():
     L = _C.lib()
     assert ctypes.sizeof(_C.XqAdapters) == 120
