@@ -6,6 +6,7 @@ import torch
 from tests.test_gpu_moe import _make_experts
 from tests.util_cases import make_dense_module
 from xorl_amd.embedding_functional import embedding
+from xorl_amd.functional import lora_adapters
 from xorl_amd.loss_functional import linear_cross_entropy
 from xorl_amd.moe_functional import moe_route
 from xorl_amd.optim import AdamW
@@ -99,3 +100,40 @@ def test_serving_step(hip_device, fmt, T):
             if T > 1:                                 # each request by itself: other kernels by size, the same formulas
                 alone = torch.cat([_serve(model, ids[i:i + 1], bank_A, bank_B, who[i:i + 1], s) for i in range(T)])
                 assert float((alone.double() - want.double()).norm()) <= 8 * B * float(want.double().norm())
+
+
+def test_calls_on_two_streams_at_once(hip_device):
+    """Each call has a workspace of its own: what two streams do side by side is what each does alone"""
+    g = torch.Generator(device=hip_device).manual_seed(8)
+    w = torch.randn(5000, 512, device=hip_device, generator=g).to(BF).requires_grad_(True)
+    bank_A = (torch.randn(9, 16, 512, device=hip_device, generator=g) / 16).to(BF)
+    bank_B = (torch.randn(9, 256, 16, device=hip_device, generator=g) * 0.1).to(BF)
+    s, bias = torch.rand(9, device=hip_device, generator=g), 0.1 * torch.randn(256, device=hip_device, generator=g)
+
+    def inputs(T):
+        return (torch.randint(0, 5000, (T,), device=hip_device, generator=g), torch.randint(-1, 9, (T,), device=hip_device, generator=g),
+                torch.randn(T, 256, device=hip_device, generator=g), torch.randn(T, 256, device=hip_device, generator=g).to(BF), torch.randn(T, 512, device=hip_device, generator=g).to(BF))
+
+    def work(ids, who, z, base, up):
+        out = embedding(ids, w, scale=2.0)
+        dw, = torch.autograd.grad(out, w, up)
+        with torch.no_grad():
+            y = lora_adapters(base, out.detach(), bank_A, bank_B, who, s)
+            weights, chosen = moe_route(z, 8, scoring="sigmoid", bias=bias, num_groups=8, top_groups=4)
+        return out.detach(), dw, y, weights, chosen
+
+    sets = [inputs(T) for T in (300, 3001)]
+    want = [work(*a) for a in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    for st in streams:
+        st.wait_stream(torch.cuda.current_stream())
+    got = []
+    for _ in range(10):
+        for st, a in zip(streams, sets):
+            with torch.cuda.stream(st):
+                got.append(work(*a))
+    torch.cuda.synchronize()
+    for i, results in enumerate(got):
+        for a, b in zip(results, want[i % 2]):
+            assert torch.equal(a, b)

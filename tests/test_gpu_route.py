@@ -298,6 +298,25 @@ def test_many_rows_of_every_kind(hip_device, E, k, groups, top_groups, score, sc
     assert w[bad].isnan().all() and dz[bad].isnan().all() and (ids[bad] == torch.arange(k, device=hip_device)).all()
 
 
+@pytest.mark.parametrize("E, k, groups, top_groups, scoring, with_bias", [(300, 8, 1, 1, "softmax", False), (512, 17, 8, 3, "sigmoid", True), (1000, 20, 10, 4, "softmax", True),
+                                                                         (120, 31, 1, 1, "sigmoid", True), (256, 16, 4, 2, "softmax", False)])
+def test_more_rows_than_waves_of_one_row_each(hip_device, E, k, groups, top_groups, scoring, with_bias):
+    """Many experts or many choices take a wave a row, and several rows one after the other"""
+    pool = _kinds(E, torch.float32, hip_device)[:22]
+    bias = 0.1 * torch.randn(E, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(1)) if with_bias else None
+    o = dict(top_k=k, scoring=scoring, num_groups=groups, top_groups=top_groups, group_score="sum2", renormalize=True, scale=1.5)
+    w0, i0, s0 = _reference(pool, o, bias)
+    at = torch.randint(0, 22, (2 * 4096 + 5,), generator=torch.Generator().manual_seed(E))
+    z = pool[at.to(hip_device)].requires_grad_(True)
+    w, ids = moe_route(z, bias=bias, **o)
+    up = torch.randn(w.shape, device=hip_device, generator=torch.Generator(device=hip_device).manual_seed(3))
+    dz, = torch.autograd.grad(w, z, up)
+    want = (w0[at], i0[at], s0[at])
+    _check(z.detach(), (w.detach(), ids), want)
+    want_dz, mag = gradient(z, up, *want, scoring, True, 1.5)
+    assert ((dz.double().cpu() - want_dz).abs() <= (2 * 20 + 64 + 40 + 40) * U * mag + 2.0 ** -120).all()
+
+
 @pytest.mark.parametrize("E", [15, 9, 32])
 def test_all_experts_chosen_beside_rows_that_are_no_numbers(hip_device, E):
     z, bias = _inputs(7, E, torch.float32, E, hip_device, True)
