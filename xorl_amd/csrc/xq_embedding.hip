@@ -79,7 +79,7 @@ struct Sorted {
     float* part;              // [n_tokens / kChunk, H]: sums over kChunk tokens in that order, where they are all of one row
     int32_t log_blocks, rows;
 };
-constexpr int kChunk = 16, kSlots = 8, kSortRows = 4096, kSortList = 3072, kSortEach = 8, kSortAtOnce = 256 * kSortEach;      // (list and counters: 35 KB, four blocks a unit)
+constexpr int kChunk = 16, kSlots = 8, kSortRows = 4096, kSortList = 3000, kSortEach = 8, kSortAtOnce = 256 * kSortEach;      // (list and counters: 35 KB, four blocks a unit)
 
 // The tokens of a list go to their places, `next` of their row: 256 at a time, each wave's 64 ranked among themselves (those of one row agree in every bit
 // of it), then the waves take their places in turn.
