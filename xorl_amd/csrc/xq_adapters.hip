@@ -13,12 +13,12 @@ namespace {
 // halves of 16 ranks, lanes 32-63 the low ones, and B's 16 ranks stand in both, so that 16 ranks are one MFMA.  fp32 factors are two bf16 numbers in the same way
 // (an infinity's low half is NaN, and so is what it has a part in).
 //
-// What bounds it: few rows, the latency of two launches that each wait for memory two or three times (one row 8 us, 48 of 8 adapters 9.8 us); many, memory: 16384 rows of
+// What bounds it: few rows, the latency of two launches that each wait for memory two or three times (one row 8.7 us, 48 of 128 adapters 10.2); many, memory: 16384 rows of
 // prompts, 12288 by 4096, rank 64, read and write 0.68 GB, 139 us at a copy's rate, and take 176 (down 104 us, up 73).  Between them (2049 rows, 46 us against 27) the
 // blocks are too few to keep all of memory busy and the whole is three or four of their lifetimes.
 //
 // A tile is rows of one adapter.  Up to kLeaderRows rows in any order: a tile belongs to the row that is the first, 17th, 33rd .. of its adapter, and the first
-// launch's blocks find the tiles themselves among the ids (no launch that sorts them), and leave them to the second.  Up to 64 rows a block has one row to look at, then
+// launch's blocks find the tiles themselves among the ids (no launch that sorts them), and leave them to the second where it has more than 64 rows to look at.  Up to 64 rows a block has one row to look at, then
 // four: half of all blocks would do no more than find that their row leads none (1024 rows 81 against 41 us, 64 rows 9.7 against 10.2).  More rows are taken in
 // windows of 16 or 64 that follow each other, and a window once for every adapter in it: of prompts' rows, each window has one or two.  By tiles against by windows, 4096 by
 // 4096, 8 adapters: rank 16, 256 rows in any order 16 and 49 us, 512 27 and 49, 1024 36 and 54; sorted by adapter 17 and 18, 27 and 18, 39 and 17.
@@ -26,7 +26,7 @@ constexpr int kLeaderRows = 512;
 constexpr int kMostParts = 16, kLeadsNone = -2;
 
 struct AdapterPlan {
-    int32_t leaders;      // tiles are found by their first row: how many rows a block looks at, 1 to 16; or 0
+    int32_t leaders;      // tiles are found by their first row: how many rows a block looks at, 1 or 4; or 0
     int32_t down_subs, up_subs;      // 16-row pieces of a window: 1 or 4
     int32_t down_tiles, up_tiles;
     int32_t parts;        // of K
@@ -50,17 +50,18 @@ __device__ __forceinline__ int adapter_of(const xq_adapters& q, int64_t row) {
 }
 
 // the rows of a leader's tile, in each wave by itself: lane l gets the row of column l % 16, or -1; false: the row leads no tile
+template <int U>
 __device__ __forceinline__ bool leader_rows(const xq_adapters& q, int lead, int* id, int* row) {
     const int lane = threadIdx.x & 63, M = (int)q.M;
     const int mine = uniform(adapter_of(q, lead));
     *id = mine;
     int before = 0, seen = 0, want = lane & 15, found = -1;
-    for (int c0 = 0; c0 < M; c0 += 256) {
-        int ids[4];                                        // (four loads on their way)
+    for (int c0 = 0; c0 < M; c0 += 64 * U) {
+        int ids[U];                                        // (so many loads on their way)
 #pragma unroll
-        for (int u = 0; u < 4; ++u) ids[u] = adapter_of(q, min(c0 + u * 64 + lane, M - 1));
+        for (int u = 0; u < U; ++u) ids[u] = adapter_of(q, min(c0 + u * 64 + lane, M - 1));
 #pragma unroll
-        for (int u = 0; u < 4; ++u) {
+        for (int u = 0; u < U; ++u) {
             const int c = c0 + u * 64;
             uint64_t same = __ballot(c + lane < M && ids[u] == mine);
             if (lead >= c + 64) { before += __popcll(same); continue; }
@@ -295,30 +296,33 @@ template <int SUBS, int RB, bool F32>
 __global__ void __launch_bounds__(256) adapter_down_kernel(AdapterArgs a) {
     __shared__ __attribute__((aligned(16))) float red[4 * kPlaceKb * 256];       // (and the waves' sums: at most 2 * SUBS * RB KB)
     static_assert(2 * SUBS * RB <= 4 * kPlaceKb, "");
-    __shared__ int found[16][16];
+    __shared__ int found[4][16];
     const int lane = threadIdx.x & 63, wave = uniform(threadIdx.x >> 6);
     const int64_t items = (int64_t)a.p.down_tiles * a.p.parts;
     for (int64_t b = blockIdx.x; b < items; b += gridDim.x) {
         const int64_t at = a.p.leaders ? b : item_of(b, items);
         const int tile = (int)(at / a.p.parts), part = (int)(at - (int64_t)tile * a.p.parts);
         if (a.p.leaders) {
-            // the waves look at the rows in turn, and the block does the tiles of those that lead one after the other
-            const int each = a.p.leaders;
+            int id, row = -1;
+            if (a.p.leaders == 1) {                        // (at most 64 rows: one look at them, by each wave for itself)
+                const bool leads = leader_rows<1>(a.q, tile, &id, &row);
+                const int one[1] = {row};
+                if (leads && id >= 0) down_tile<1, RB, F32>(a, id, one, part, tile, red);
+                continue;
+            }
+            // each wave looks at a row, and the block does the tiles of those that lead one after the other
+            const int lead = tile + wave * a.p.down_tiles;
+            const bool leads = lead < a.q.M && leader_rows<4>(a.q, lead, &id, &row);
             __syncthreads();                               // (the rows before have been read)
-            for (int j = wave; j < each; j += 4) {
-                const int lead = tile + j * a.p.down_tiles;
-                int id, row = -1;
-                const bool leads = lead < a.q.M && leader_rows(a.q, lead, &id, &row);
-                if (lane < 16) {
-                    found[j][lane] = leads ? row : kLeadsNone;
-                    if (part == 0 && lead < a.q.M) a.led[lead * 16 + lane] = leads ? row : kLeadsNone;
-                }
+            if (lane < 16) {
+                found[wave][lane] = leads ? row : kLeadsNone;
+                if (part == 0 && lead < a.q.M) a.led[lead * 16 + lane] = leads ? row : kLeadsNone;
             }
             __syncthreads();
-            for (int j = 0; j < each; ++j) {
+            for (int j = 0; j < 4; ++j) {
                 const int one[1] = {found[j][lane & 15]}, of = uniform(one[0]);
                 if (of == kLeadsNone) continue;
-                const int id = uniform(adapter_of(a.q, of));
+                id = uniform(adapter_of(a.q, of));
                 if (id >= 0) down_tile<1, RB, F32>(a, id, one, part, tile + j * a.p.down_tiles, red);
             }
             continue;
@@ -565,8 +569,15 @@ __global__ void __launch_bounds__(256) adapter_up_kernel(AdapterArgs a) {
         const int64_t n0 = (at - tile * chunks) * a.p.cols, n1 = min(n0 + a.p.cols, a.q.N);
         if (SUBS == 1 && a.p.leaders) {
             for (int lead = tile; lead < a.q.M; lead += a.p.up_tiles) {
-                const int row = a.led[lead * 16 + (lane & 15)];
-                if (uniform(row) != kLeadsNone) up_piece<RB, F32, WHOLE>(a, uniform(adapter_of(a.q, lead)), row, n0, n1, ts);
+                int id, row;
+                if (a.p.leaders == 1) {                    // (one look at the ids, which are in the cache, is shorter than reading what was just written: 48 rows 10.2 against 10.5 us)
+                    if (!leader_rows<1>(a.q, lead, &id, &row)) continue;
+                } else {
+                    row = a.led[lead * 16 + (lane & 15)];
+                    id = uniform(adapter_of(a.q, lead));
+                    if (uniform(row) == kLeadsNone) continue;
+                }
+                up_piece<RB, F32, WHOLE>(a, id, row, n0, n1, ts);
             }
             continue;
         }
