@@ -399,9 +399,25 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const f
     if (has_bias) {                                        // each against the next
         const float y = A::next(c.at);
         const int f = A::next(c.e);
-        if (l + 1 < picks && c.e >= 0 && f >= 0 && !(c.at - y > error * (fabsf(c.at) + fabsf(y) + 2 * bias_most)) &&
-            (logit(row, c.e) != logit(row, f) || q.bias[c.e] != q.bias[f]))
-            sure = false;
+        bool tied = false;
+        if (l + 1 < picks && c.e >= 0 && f >= 0 && !(c.at - y > error * (fabsf(c.at) + fabsf(y) + 2 * bias_most))) {
+            const bool same = logit(row, c.e) == logit(row, f) && q.bias[c.e] == q.bias[f];
+            sure &= same;
+            tied = same && l == K - 1;
+        }
+        // The last chosen and the first left out are equal: by their index, if what lies as near as 32 bits tell is equal to them too (all of it is where a router
+        // starts at zero: the row stays here).
+        if (A::any(tied)) {
+            const int last = A::largest(l == K - 1 ? c.e : -1);
+            const float zl = logit(row, last), bl = q.bias[last], at = A::largest(l == K - 1 ? c.at : kOut);
+#pragma unroll 1
+            for (int e = l; e < E; e += L) {
+                const float ze = logit(row, e), be = q.bias[e];
+                if (ze == kOut || be == kOut || (ze == zl && be == bl)) continue;
+                const float x = (SOFT ? near_exp(ze - top) * over : __builtin_amdgcn_rcpf(1.0f + near_exp(-ze))) + be;
+                if (!(fabsf(x - at) > error * (fabsf(x) + fabsf(at) + 2 * bias_most))) sure = false;
+            }
+        }
     }
     *chosen = c;
     return !A::any(!sure);
@@ -479,8 +495,9 @@ __device__ __forceinline__ Chosen choose64(const RouteArgs& a, const T* row, flo
     return c;
 }
 
+// (16 lanes: four waves a SIMD, 128 registers)
 template <typename T, int L, int V, bool SOFT, bool SCORED>
-__global__ void __launch_bounds__(64) moe_route_kernel(RouteArgs a) {
+__global__ void __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(L == 16 ? 4 : 3))) moe_route_kernel(RouteArgs a) {
     using A = Lanes<L>;
     __shared__ WavePlace<L, V> places;
     const xq_moe_route& q = a.q;
