@@ -1,0 +1,54 @@
+"""Host side of experts, adapters and embedding rows: calls that are traced and never run here."""
+
+import pytest
+import torch
+from torch._subclasses.fake_tensor import FakeTensorMode
+
+from xorl_amd import _C
+from xorl_amd.functional import lora_adapters
+
+BF = torch.bfloat16
+
+
+def _traced(monkeypatch, on="cuda", out=None, **elsewhere):
+    """lora_adapters as a compiled program traces it, over tensors without memory"""
+    shapes = {"base": (3, 32), "x": (3, 64), "A": (5, 4, 64), "B": (5, 32, 4), "ids": (3,), "s": (5,)}
+    types = {"base": BF, "x": BF, "A": BF, "B": BF, "ids": torch.int32, "s": torch.float32}
+    monkeypatch.setattr(torch.compiler, "is_compiling", lambda: True)
+    with FakeTensorMode():
+        a = {n: torch.empty(shapes[n], dtype=types[n], device=elsewhere.get(n, on)) for n in shapes}
+        o = None if out is None else torch.empty(out[0], dtype=out[1], device=out[2])
+        return lora_adapters(*a.values(), out=o)
+
+
+def test_a_traced_call_gives_what_an_eager_one_does(monkeypatch):
+    y = _traced(monkeypatch)
+    assert y.shape == (3, 32) and y.dtype == BF and y.device.type == "cuda"
+    assert _traced(monkeypatch, out=((3, 32), BF, "cuda")).dtype == BF
+
+
+@pytest.mark.parametrize("which", ["base", "x", "A", "B", "ids", "s"])
+def test_a_traced_call_refuses_host_memory(monkeypatch, which):
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        _traced(monkeypatch, **{which: "cpu"})
+    with pytest.raises(_C.XqError, match="different devices"):
+        _traced(monkeypatch, **{which: "cuda:1"})
+
+
+@pytest.mark.parametrize("out,match", [(((3, 32), torch.float32, "cuda"), "out must be"), (((2, 3, 32), BF, "cuda"), "out must be"), (((3, 16), BF, "cuda"), "out must be"),
+                                       (((3, 32), BF, "cpu"), "HIP device only"), (((3, 32), BF, "cuda:1"), "different devices")])
+def test_a_traced_call_refuses_an_out_of_another_kind(monkeypatch, out, match):
+    with pytest.raises((_C.XqError, RuntimeError), match=match):
+        _traced(monkeypatch, out=out)
+
+
+@pytest.mark.parametrize("which", range(6))
+def test_the_operator_itself_refuses_host_memory(which):
+    """What a traced call leaves in a program is dispatched by any one of its tensors: without a device that is all of them, and the rest is refused here"""
+    from xorl_amd.functional import _adapters_impl
+
+    with FakeTensorMode():
+        shapes = ((3, 32, BF), (3, 64, BF), (5, 4, 64, BF), (5, 32, 4, BF), (3, torch.int32), (5, torch.float32))
+        a = [torch.empty(s[:-1], dtype=s[-1], device="cpu" if i == which else "cuda") for i, s in enumerate(shapes)]
+        with pytest.raises(RuntimeError, match="HIP device only"):
+            _adapters_impl(*a)

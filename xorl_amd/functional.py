@@ -426,7 +426,14 @@ def _aligned(t: Tensor) -> Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
+def _one_device(*tensors: Optional[Tensor]) -> None:
+    _C.require_hip(*tensors)
+    if any(t is not None and t.device != tensors[0].device for t in tensors):
+        raise _C.XqError("lora_adapters: the tensors are on different devices")
+
+
 def _adapters_impl(base: Tensor, x: Tensor, A: Tensor, B: Tensor, ids: Tensor, scalings: Tensor, out: Optional[Tensor] = None) -> Tensor:
+    _one_device(base, x, A, B, ids, scalings, out)         # (a traced call comes here from the operator's dispatcher, which goes by any one of them)
     dev = x.device
     with torch.cuda.device(dev):
         x2, base2, i1 = _adapters_rows(x), _adapters_rows(base), ids.reshape(-1).contiguous()
@@ -492,16 +499,17 @@ def lora_adapters(base: Tensor, x: Tensor, lora_A: Tensor, lora_B: Tensor, adapt
     if x.shape[-1] < 64 or x.shape[-1] % 64 or base.shape[-1] < 16 or base.shape[-1] % 16 or not 1 <= lora_A.shape[1] <= MAX_FUSED_RANK:
         raise _C.XqError(f"lora_adapters: in_features must be a multiple of 64, out_features of 16 and the rank 1 to {MAX_FUSED_RANK}, got {x.shape[-1]}, {base.shape[-1]} "
                          f"and {lora_A.shape[1]}")
+    if not torch.compiler.is_compiling():
+        refuse_tangents(*tensors, out)
+    _one_device(*tensors, adapter_ids, out)
+    if out is not None and (out.dtype != torch.bfloat16 or out.shape != base.shape):
+        raise _C.XqError(f"lora_adapters: out must be bf16 {tuple(base.shape)}, got {out.dtype} {tuple(out.shape)}")
     if torch.compiler.is_compiling():
         y = _adapters_op(base.detach(), x.detach(), lora_A.detach(), lora_B.detach(), adapter_ids, scalings.detach())
         return y if out is None else out.copy_(y)
-    refuse_tangents(*tensors, out)
-    _C.require_hip(*tensors, adapter_ids, out)
-    if len({t.device for t in (*tensors, adapter_ids, *(() if out is None else (out,)))}) > 1:
-        raise _C.XqError("lora_adapters: the tensors are on different devices")
     if out is not None:
-        if out.dtype != torch.bfloat16 or out.shape != base.shape or _rows_in_place(out) is None:
-            raise _C.XqError(f"lora_adapters: out must be bf16 {tuple(base.shape)} with rows at multiples of 16 bytes, got {out.dtype} {tuple(out.shape)} of strides {out.stride()}")
+        if _rows_in_place(out) is None:
+            raise _C.XqError(f"lora_adapters: out must be made of rows at multiples of 16 bytes, got strides {out.stride()}")
         a, b = _span(out)
         for t in (*tensors, adapter_ids):
             c, d = _span(t)
