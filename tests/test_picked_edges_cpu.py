@@ -6,6 +6,7 @@ from torch._subclasses.fake_tensor import FakeTensorMode
 
 from xorl_amd import _C
 from xorl_amd.functional import lora_adapters
+from xorl_amd.moe_functional import _route_problem
 
 BF = torch.bfloat16
 
@@ -52,3 +53,41 @@ def test_the_operator_itself_refuses_host_memory(which):
         a = [torch.empty(s[:-1], dtype=s[-1], device="cpu" if i == which else "cuda") for i, s in enumerate(shapes)]
         with pytest.raises(RuntimeError, match="HIP device only"):
             _adapters_impl(*a)
+
+
+class _Wrapped(torch.Tensor):
+    """a tensor whose values another one holds, as a distributed tensor's are"""
+
+    @staticmethod
+    def __new__(cls, inner):
+        t = torch.Tensor._make_wrapper_subclass(cls, inner.shape, dtype=inner.dtype, device=inner.device)
+        t.inner = inner
+        return t
+
+    @classmethod
+    def __torch_dispatch__(cls, func, types, args=(), kwargs=None):
+        raise NotImplementedError
+
+
+def test_a_bias_without_memory_of_its_own_is_refused():
+    options = (2, 1, 1, 1, 1, True, 1.0)
+    z, bias = torch.zeros(3, 8), torch.zeros(8)
+    assert _route_problem(z, 3, 8, z.dtype, bias, options).bias == bias.data_ptr()
+    assert _route_problem(z, 3, 8, z.dtype, None, options).bias is None
+    with pytest.raises(_C.XqError, match="no memory"):
+        _route_problem(z, 3, 8, z.dtype, _Wrapped(bias), options)
+    assert _C.ptr(torch.empty(0)) == 0
+
+
+def test_a_distributed_bias_is_refused(tmp_path):
+    import torch.distributed as dist
+    from torch.distributed.device_mesh import init_device_mesh
+    from torch.distributed.tensor import Replicate, distribute_tensor
+
+    dist.init_process_group("gloo", init_method=f"file://{tmp_path / 'store'}", rank=0, world_size=1)
+    try:
+        bias = distribute_tensor(torch.zeros(8), init_device_mesh("cpu", (1,)), [Replicate()])
+        with pytest.raises(_C.XqError, match="no memory"):
+            _route_problem(torch.zeros(3, 8), 3, 8, torch.float32, bias, (2, 1, 1, 1, 1, True, 1.0))
+    finally:
+        dist.destroy_process_group()

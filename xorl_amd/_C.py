@@ -311,7 +311,13 @@ def require_hip(*tensors: Optional[torch.Tensor]) -> None:
 
 
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
-    return None if t is None else t.data_ptr()
+    """The address of an argument that may be absent: a tensor that is there and has none (a distributed one) would count as that."""
+    if t is None:
+        return None
+    p = t.data_ptr()
+    if not p and t.numel():
+        raise XqError(f"{type(t).__name__} {tuple(t.shape)} has no memory of its own on this device: pass the tensor that holds its values")
+    return p
 
 
 def stream_ptr(device: torch.device) -> int:
