@@ -1,11 +1,14 @@
 """GPU: choices of experts (moe_route) that single precision cannot tell, next to the last place and between groups."""
 
+import math
+
 import pytest
 import torch
 
 from xorl_amd.moe_functional import moe_route
 
 pytestmark = pytest.mark.gpu
+LOWEST = torch.finfo(torch.float32).min
 
 
 def _order(z, k, scoring, bias):
@@ -50,3 +53,30 @@ def test_a_router_that_starts_at_zero(hip_device, T, E, scoring):
     z, bias = torch.zeros(T, E, device=hip_device), torch.zeros(E, device=hip_device)
     _, ids = moe_route(z, 8, scoring=scoring, bias=bias)
     assert torch.equal(ids, torch.arange(8, device=hip_device).expand(T, 8))
+
+
+@pytest.mark.parametrize("size", [2, 4, 6])
+@pytest.mark.parametrize("T", [1, 70, 3000])
+@pytest.mark.parametrize("groups", [4, 32])
+def test_groups_of_biases_whose_sum_is_no_fp32_number(hip_device, groups, T, size):
+    """Two scores with a bias near the type's lowest value make a strength below every fp32 number; a group without experts is weaker still"""
+    E = groups * size
+    z = torch.randn(T, E, generator=torch.Generator().manual_seed(T + E)).to(hip_device)
+    bias = torch.full((groups, size), -math.inf)
+    bias[1] = LOWEST
+    bias[2] = 0.75 * LOWEST
+    bias[3] = 0.0
+    at = {g: list(range(g * size, (g + 1) * size)) for g in range(4)}
+    b = bias.view(-1).to(hip_device)
+
+    def rows(order, k):
+        return torch.tensor((order + [-1] * k)[:k], device=hip_device).expand(T, k)
+
+    first = z[:, at[3]].sort(dim=1, descending=True, stable=True)[1] + at[3][0]
+    for top_groups, behind in ((1, []), (2, at[2]), (3, at[2] + at[1]), (4, at[2] + at[1])):
+        k = min(32, top_groups * size)
+        _, ids = moe_route(z, k, scoring="sigmoid", bias=b, num_groups=groups, top_groups=top_groups, group_score="sum2")
+        assert torch.equal(ids, torch.cat([first, rows(behind, k - size)], 1)), top_groups
+    b[at[3][0]:at[3][-1] + 1] = -math.inf
+    _, ids = moe_route(z, size, scoring="sigmoid", bias=b, num_groups=groups, top_groups=1, group_score="sum2")
+    assert torch.equal(ids, rows(at[2], size))

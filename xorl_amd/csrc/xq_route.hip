@@ -316,7 +316,9 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const f
             float first = kOut, second = kOut;
 #pragma unroll 8
             for (int k = 0; k < n; ++k) take_in(value[g * n + k], first, second);
-            strength[g] = first + (two && second != kOut ? second : 0.0f);
+            const float both = first + (two && second != kOut ? second : 0.0f);
+            if (SCORED && both == kOut && first != kOut) sure = false;        // (below every fp32 number, and yet above a group that has no experts)
+            strength[g] = both;
         }
         wave_fence();
         // a group stays if fewer than top_groups are better; the weakest that stays and the strongest that goes have to lie apart
