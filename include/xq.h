@@ -787,8 +787,9 @@ int xq_moe_route_bwd(const xq_moe_route* problem, const float* weights, const in
  * shared projection, base = what xq_linear_fwd leaves for r = 0.  No counterpart in the reference, which serves one adapter at a time.
  * A row whose id lies outside [0, n_adapters) has no adapter: out = base.  Products accumulate in fp32, x . A^T is kept to 16 bits and more.
  * x [M, K], base and out [M, N] bf16, rows at multiples of 16 bytes; out may be base.  A [n_adapters, r, K], B [n_adapters, N, r] dense, in
- * factor_dtype; an adapter of a smaller rank is padded with zeros.  K % 64 == 0, N % 16 == 0, r 1 to 64, M and N < 2^24, K < 2^23.  fp32 factors are
- * taken as two bf16 numbers, so that an infinite one gives NaN.
+ * factor_dtype; an adapter of a smaller rank is padded with zeros.  K % 64 == 0, N % 16 == 0, r 1 to 64, M and N < 2^24, K < 2^23.  fp32 factors, and
+ * scaling x A^T, enter as two bf16 numbers each; what is larger than all bf16 numbers (3.39e38) counts as infinite.  Infinities in x, factors and base give what the formula makes
+ * of them; scaling is finite.
  * workspace: xq_adapters_workspace_bytes(M, N, K, r) bytes, 256-byte aligned. */
 typedef struct xq_adapters {
     const void* x;

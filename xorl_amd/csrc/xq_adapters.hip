@@ -10,8 +10,9 @@ namespace {
 // Two launches: t = x A_a^T in parts of K, fp32, to the workspace; then out = base + (s t) B_a^T.  Both multiply on 16x16x32 MFMA tiles straight from memory:
 // all four operands have the contraction along their rows, so that a lane's eight elements are one 16-byte load.  t goes into the second product as two bf16
 // numbers (16 bits: one would lose as much of a large update as the result's own rounding), laid out along the contraction: lanes 0-31 hold the high
-// halves of 16 ranks, lanes 32-63 the low ones, and B's 16 ranks stand in both, so that 16 ranks are one MFMA.  fp32 factors are two bf16 numbers in the same way
-// (an infinity's low half is NaN, and so is what it has a part in).
+// halves of 16 ranks, lanes 32-63 the low ones, and B's 16 ranks stand in both, so that 16 ranks are one MFMA.  fp32 factors are two bf16 numbers in the same way.
+// Low halves count where the high halves' sum is finite: an infinity times a low half has any sign or is none (the first product keeps them in sums of their own, the
+// second one takes sums that are no numbers again; 0 to 2 % of a call).
 //
 // What bounds it: few rows, the latency of two launches that each wait for memory two or three times (one row 8.7 us, 48 of 128 adapters 10.2); many, memory: 16384 rows of
 // prompts, 12288 by 4096, rank 64, read and write 0.68 GB, 139 us at a copy's rate, and take 176 (down 104 us, up 73).  Between them (2049 rows, 46 us against 27) the
@@ -148,6 +149,7 @@ constexpr int kPlaceKb = 8;           // of a wave
 template <int SUBS, int RB, bool F32, int AHEAD>
 __device__ __forceinline__ void down_units(const bf16_t* const (&x)[SUBS][2], const void* A, const uint32_t (&a_at)[RB][F32 ? 4 : 2], int first, int n, int turn, u32x4* ex,
                                            f32x4 (&acc)[SUBS][RB]) {
+    f32x4 low[F32 ? SUBS : 1][F32 ? RB : 1] = {};          // of A's low halves
     constexpr int FL = F32 ? 4 : 2, AP = F32 ? 16 : 8;    // loads, and pieces a row, of 16 rows of a factor
     constexpr int GROUP = kPlaceKb / FL;                   // blocks of ranks that the place holds
     const int lane = threadIdx.x & 63, col = lane & 15, group = lane >> 4;
@@ -221,12 +223,20 @@ __device__ __forceinline__ void down_units(const bf16_t* const (&x)[SUBS][2], co
 #pragma unroll
                     for (int t = 0; t < SUBS; ++t) {
                         acc[t][b] = mfma(s.hi, xo[u][t][h], acc[t][b]);
-                        if (F32) acc[t][b] = mfma(s.lo, xo[u][t][h], acc[t][b]);
+                        if constexpr (F32) low[t][b] = mfma(s.lo, xo[u][t][h], low[t][b]);
                     }
                 }
             }
         }
     }
+    // (where the high halves' sum is infinite or none, it is the sum: an infinity times a low half has any sign, or is no number)
+    if constexpr (F32)
+#pragma unroll
+        for (int t = 0; t < SUBS; ++t)
+#pragma unroll
+            for (int b = 0; b < RB; ++b)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) acc[t][b][i] += fabsf(acc[t][b][i]) < INFINITY ? low[t][b][i] : 0.0f;
 }
 // units on their way: up to four of x in a wave's place, and 16 loads of factors
 constexpr int ahead_for(int subs, int rb, bool f32) { return subs == 4 ? 1 : std::min(4, std::max(1, 16 / (rb * (f32 ? 8 : 4)))); }
@@ -388,6 +398,30 @@ __device__ __forceinline__ void up_operands(const AdapterArgs& a, float scale, c
         }
 }
 
+__device__ __forceinline__ bool has_nan(const f32x4 (&v)[2]) {
+    bool is = false;
+#pragma unroll
+    for (int j = 0; j < 2; ++j) is |= __builtin_isunordered(v[j][0], v[j][1]) || __builtin_isunordered(v[j][2], v[j][3]);
+    return is;
+}
+// Sums that are no numbers again, of the high halves alone: an infinity in t or B times a low half has any sign, or is none where the sum of the whole
+// numbers is infinite.  factor(j, b): B's operand, as high halves
+template <int RB, typename F>
+__device__ __forceinline__ void sums_again(const bf16x8* ts, F factor, f32x4 (&acc)[2]) {
+    const int lane = threadIdx.x & 63;
+    f32x4 lead[2] = {};
+#pragma unroll
+    for (int b = 0; b < RB; ++b) {
+        const bf16x8 tv = lane < 32 ? ts[b * 64 + lane] : bf16x8{};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) lead[j] = mfma(lane < 32 ? factor(j, b) : bf16x8{}, tv, lead[j]);
+    }
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) acc[j][i] = acc[j][i] != acc[j][i] ? lead[j][i] : acc[j][i];
+}
+
 // eight columns of a row: base and the sums, rounded
 __device__ __forceinline__ u32x4 add8(u32x4 base, const f32x4& lo, const f32x4& hi) {
 #pragma unroll
@@ -446,6 +480,7 @@ __device__ __forceinline__ void up_piece(const AdapterArgs& a, int id, int row, 
                     if (F32) acc[j] = mfma(s.lo, tv, acc[j]);
                 }
             }
+            if (__ballot(has_nan(acc))) sums_again<RB>(ts, [&](int j, int b) { return split_raw<F32>(bv[j][b]).hi; }, acc);
             out = add8(base, acc[0], acc[1]);
         }
         const int64_t mine = n + group * 8;
@@ -532,6 +567,7 @@ __device__ __forceinline__ void up_window(const AdapterArgs& a, int id, const in
                         if (F32) acc[j] = mfma(sv[j][b].lo, tv, acc[j]);
                     }
                 }
+                if (__ballot(has_nan(acc))) sums_again<RB>(ts + t * RB * 64, [&](int j, int b) { return sv[j][b].hi; }, acc);
                 wave_fence();
 #pragma unroll
                 for (int j = 0; j < 2; ++j) sums[slot<8>(col, group * 2 + j)] = __builtin_bit_cast(u32x4, acc[j]);

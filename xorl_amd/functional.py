@@ -474,8 +474,8 @@ def lora_adapters(base: Tensor, x: Tensor, lora_A: Tensor, lora_B: Tensor, adapt
     :func:`~xorl_amd.qlora.qlora_adapters_forward` does both).  A row whose id is negative or no adapter's has none and gets ``base``.
 
     base [.., N] and x [.., K] bf16; lora_A [n, r, K] and lora_B [n, N, r] fp32 or bf16, an adapter of a smaller rank padded with zeros; adapter_ids [..] int32
-    or int64; scalings [n] fp32.  K % 64 == 0, K < 2^23, N % 16 == 0, N and the rows < 2^24, r 1 to 64.  Products accumulate in fp32; factors in fp32 and x @ A.T enter them with 16 bits and more; the sum with base is
-    rounded once.  Any mix of adapters is taken; rows of one adapter that follow each other are the fast order above 512 rows.  The result is a new tensor, or ``out``, which
+    or int64; scalings [n] fp32.  K % 64 == 0, K < 2^23, N % 16 == 0, N and the rows < 2^24, r 1 to 64.  Products accumulate in fp32; factors in fp32 and scalings * x @ A.T enter them with 16 bits and more (larger than
+    3.39e38, the largest bf16 number, they count as infinite); the sum with base is rounded once.  Any mix of adapters is taken; rows of one adapter that follow each other are the fast order above 512 rows.  The result is a new tensor, or ``out``, which
     may be base itself and otherwise shares no memory with what is read."""
     if not torch.compiler.is_compiling() and (out is None or out is base):
         y = native().adapters(base, x, lora_A, lora_B, adapter_ids, scalings, out is not None)
