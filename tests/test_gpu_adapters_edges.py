@@ -1,14 +1,45 @@
-"""GPU: adapters of many requests (lora_adapters) with infinities."""
+"""GPU: adapters of many requests (lora_adapters) where rows are taken 64 at a time, and with infinities."""
 
 import math
 
 import pytest
 import torch
 
-from tests.test_gpu_adapters import BF, _inputs
+from tests.test_gpu_adapters import BF, _check, _inputs
 from xorl_amd.functional import lora_adapters
 
 pytestmark = pytest.mark.gpu
+
+
+def _twice(a):
+    out = lora_adapters(*a)
+    _check(out, *a)
+    assert torch.equal(lora_adapters(*a), out)                    # the same bits on every call
+    return out
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("M,N,K,r", [(8191, 80, 320, 16), (8192, 64, 1088, 64), (8193, 48, 192, 33), (8193, 144, 1600, 8), (9001, 272, 704, 24), (9001, 64, 448, 48), (12345, 528, 64, 40),
+                                     (8200, 1040, 576, 32)])
+def test_many_rows(hip_device, M, N, K, r, dtype):
+    for order, without in (("one", 0.0), ("runs", 0.1), ("mixed", 0.2)):
+        _twice(_inputs(M, N, K, r, 3, dtype, M + r, hip_device, order, without))
+
+
+@pytest.mark.parametrize("dtype", [BF, torch.float32])
+@pytest.mark.parametrize("r", [8, 24, 33, 64])
+def test_pieces_of_a_window(hip_device, r, dtype):
+    """An adapter in every choice of a window's four pieces, alone or beside another one or none, and in one row of a piece"""
+    M = 8192 + 64 * 4 + 21
+    a = list(_inputs(M, 96, 1088, r, 5, dtype, r, hip_device, without=0.0))
+    piece = torch.arange(M, device=hip_device) // 16
+    window, of = piece // 4, piece % 4
+    inside = (window % 16) >> of & 1
+    for rest in (-1, 2):
+        a[4] = torch.where(inside == 1, 1 + 2 * (window % 2), rest).to(torch.int32)
+        _twice(a)
+    a[4] = torch.where((inside == 1) & (torch.arange(M, device=hip_device) % 16 == window % 16), 4, torch.where(of == 0, 0, -1)).to(torch.int32)
+    _twice(a)
 
 
 @pytest.mark.parametrize("dtype", [BF, torch.float32])
