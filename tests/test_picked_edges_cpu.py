@@ -5,8 +5,9 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from xorl_amd import _C
+from xorl_amd.embedding_functional import embedding
 from xorl_amd.functional import lora_adapters
-from xorl_amd.moe_functional import _route_problem
+from xorl_amd.moe_functional import _route_problem, moe_route
 
 BF = torch.bfloat16
 
@@ -91,3 +92,15 @@ def test_a_distributed_bias_is_refused(tmp_path):
             _route_problem(torch.zeros(3, 8), 3, 8, torch.float32, bias, (2, 1, 1, 1, 1, True, 1.0))
     finally:
         dist.destroy_process_group()
+
+
+@pytest.mark.parametrize("kw", [dict(top_k=2.5), dict(num_groups=2.5, top_groups=2), dict(num_groups=4, top_groups=2.5), dict(top_k=float("inf")), dict(top_k=float("nan"))])
+def test_numbers_that_are_not_whole_are_refused(kw):
+    with pytest.raises(_C.XqError, match="moe_route"):
+        moe_route(torch.zeros(3, 20), **{"top_k": 2, **kw})
+
+
+@pytest.mark.parametrize("padding_idx", [0.5, -1.5, float("nan")])
+def test_a_padding_index_that_is_not_whole_is_refused(padding_idx):
+    with pytest.raises(_C.XqError, match="padding_idx"):
+        embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4), padding_idx=padding_idx)

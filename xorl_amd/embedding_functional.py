@@ -119,7 +119,7 @@ def embedding(ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: O
     if ids.dtype not in (torch.int64, torch.int32):
         raise _C.XqError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
     V = weight.shape[0]
-    if padding_idx is not None and not -V <= padding_idx < V:
+    if padding_idx is not None and (not -V <= padding_idx < V or (isinstance(padding_idx, float) and not padding_idx.is_integer())):
         raise _C.XqError(f"embedding: padding_idx {padding_idx} is no row of a weight of {V}")
     if not math.isfinite(scale) or abs(scale) > 3.4e38:
         raise _C.XqError(f"embedding: scale must be finite in fp32, got {scale}")

@@ -174,6 +174,8 @@ def moe_route(router_logits: Tensor, top_k: int, *, scoring: str = "softmax", bi
     # what the native path leaves: traced calls, tensor subclasses, and the errors
     if isinstance(scale, Tensor) or isinstance(top_k, Tensor):
         raise _C.XqError("moe_route: scale and top_k are numbers, not tensors")
+    if any(isinstance(n, float) and not n.is_integer() for n in (top_k, num_groups, top_groups)):
+        raise _C.XqError(f"moe_route: top_k, num_groups and top_groups are whole numbers, got {top_k}, {num_groups} and {top_groups}")
     if options[1] < 0:
         raise _C.XqError(f"moe_route: scoring must be one of {sorted(_C.ROUTE_SCORINGS)}, got {scoring!r}")
     if options[4] < 0:
