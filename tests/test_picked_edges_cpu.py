@@ -104,3 +104,9 @@ def test_numbers_that_are_not_whole_are_refused(kw):
 def test_a_padding_index_that_is_not_whole_is_refused(padding_idx):
     with pytest.raises(_C.XqError, match="padding_idx"):
         embedding(torch.zeros(3, dtype=torch.int64), torch.zeros(5, 4), padding_idx=padding_idx)
+
+
+def test_the_workspace_holds_tiles_only_where_they_are_kept():
+    """[rows][ranks, padded to 16] in fp32, of one part of K; from 65 rows on each row's tile beside it"""
+    need = _C.lib().xq_adapters_workspace_bytes
+    assert [need(M, 32, 64, 5) for M in (4, 64, 65, 512, 513)] == [256, 64 * 64, 65 * 128, 512 * 128, 513 * 64]

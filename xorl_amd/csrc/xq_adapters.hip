@@ -37,7 +37,7 @@ struct AdapterArgs {
     xq_adapters q;
     AdapterPlan p;
     float* t;             // [parts][M][r_pad]
-    int32_t* led;         // [M][16]: the rows of a leader's tile, or -1; kLeadsNone in the first place of a row that leads none
+    int32_t* led;         // (more than 64 rows, tiles by leaders) [M][16]: the rows of a leader's tile, or -1; kLeadsNone in the first place of a row that leads none
     int32_t r_pad;
 };
 
@@ -690,7 +690,7 @@ using namespace xq;
 extern "C" int64_t xq_adapters_workspace_bytes(int64_t M, int64_t N, int64_t K, int r) {
     if (!sizes_fit(M, N, K, r)) return -1;
     const AdapterPlan p = plan_adapters(M, N, K, r);
-    return std::max<int64_t>((int64_t)p.parts * M * r_pad(r) * 4 + (p.leaders ? M * 64 : 0), 256);
+    return std::max<int64_t>((int64_t)p.parts * M * r_pad(r) * 4 + (p.leaders > 1 ? M * 64 : 0), 256);
 }
 
 extern "C" int xq_adapters_add(const xq_adapters* q, void* workspace, int64_t workspace_bytes, void* stream) {
