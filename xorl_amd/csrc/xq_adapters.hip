@@ -299,7 +299,7 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const in
 // (16384 rows of 8 adapters whose A have 1.5 MB each: down 208 us in turn and 174 so, up 118 and 106)
 __device__ __forceinline__ int64_t item_of(int64_t at, int64_t n) {
     const int64_t each = n / 8, rest = n - each * 8, xcd = at & 7, i = at >> 3;
-    return at >= each * 8 + rest ? at : xcd * each + min(xcd, rest) + i;
+    return xcd * each + min(xcd, rest) + i;
 }
 
 template <int SUBS, int RB, bool F32>

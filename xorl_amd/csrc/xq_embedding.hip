@@ -388,7 +388,7 @@ void launch_fwd(const xq_embedding& q, void* out, int64_t ld_out, hipStream_t st
 template <typename T, int W>
 void launch_bwd(const xq_embedding& q, const Sorted& s, const void* grad, int64_t ld_grad, void* dw, int64_t ld_dw, hipStream_t st) {
     const int64_t bytes = q.V * q.H * (int64_t)sizeof(T);
-    const bool filled = W > 1 && q.n_tokens < q.V / 2 && bytes >= kFillBytes && (ld_dw == q.H || q.V == 1);
+    const bool filled = W > 1 && q.n_tokens < q.V / 2 && bytes >= kFillBytes && ld_dw == q.H;
     const unsigned sorts = 1u << s.log_blocks;
     embedding_sort_kernel<<<dim3(sorts + (filled ? (unsigned)std::min<int64_t>(xq_cdiv(bytes, 4096), (1 << 23)) : 0u)), 256, 0, st>>>(q, s, (u32x4*)dw, filled ? bytes / 16 : 0);
     if (q.n_tokens >= kChunk)

@@ -425,7 +425,7 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const f
     return !A::any(!sure);
 }
 
-// The choice in 64 bits, of one row by the whole wave: few rows come here
+// The choice in 64 bits, of one row by the whole wave: rows that are chosen by scores, few of them
 template <typename T, int L, int V>
 __device__ __forceinline__ Chosen choose64(const RouteArgs& a, const T* row, float top, int l, WavePlace<L, V>* wave) {
     using A = Lanes<64>;
@@ -434,23 +434,21 @@ __device__ __forceinline__ Chosen choose64(const RouteArgs& a, const T* row, flo
     constexpr int N = L * V / 64, kTogether = N < 4 ? N : 4;          // experts a lane, l, l + 64, ..
     const double kOut = -INFINITY;
     const int E = q.num_experts, size = E / q.num_groups;
-    const bool soft = q.scoring == XQ_ROUTE_SOFTMAX, grouped = q.top_groups < q.num_groups, two = q.group_score == XQ_ROUTE_GROUP_SUM2, scored = q.bias || (grouped && two);
+    const bool soft = q.scoring == XQ_ROUTE_SOFTMAX, grouped = q.top_groups < q.num_groups, two = q.group_score == XQ_ROUTE_GROUP_SUM2;
     double total = 0.0;
-    if (scored) {
 #pragma unroll kTogether
-        for (int i = 0; i < N; ++i) {
-            const double z = i * 64 + l < E ? (double)logit(row, i * 64 + l) : kOut;
-            const double x = exp(soft ? z - (double)top : -z);
-            place->value[i * 64 + l] = soft ? x : 1.0 / (1.0 + x);
-            total += x;
-        }
-        total = soft ? A::sum(total) : 1.0;
+    for (int i = 0; i < N; ++i) {
+        const double z = i * 64 + l < E ? (double)logit(row, i * 64 + l) : kOut;
+        const double x = exp(soft ? z - (double)top : -z);
+        place->value[i * 64 + l] = soft ? x : 1.0 / (1.0 + x);
+        total += x;
     }
+    total = soft ? A::sum(total) : 1.0;
 #pragma unroll 1
     for (int e = l; e < 64 * N; e += 64) {
         const int at = min(e, E - 1);
         const double z = logit(row, at), bias = q.bias ? (double)q.bias[at] : 0.0;
-        place->value[e] = e >= E || z == kOut || bias == kOut ? kOut : scored ? place->value[e] / total + bias : z;
+        place->value[e] = e >= E || z == kOut || bias == kOut ? kOut : place->value[e] / total + bias;
     }
     if (grouped) {
         wave_fence();
@@ -553,16 +551,17 @@ __global__ void __launch_bounds__(64) __attribute__((amdgpu_waves_per_eu(L == 16
             total = A::sum(total);
         }
         Chosen c;
-        const bool sure = choose<SOFT, SCORED, T, L, V>(a, from, z, b, most, top, total, l, place, &c);
-        for (uint64_t left = __ballot(!sure && !bad && real); left;) {
-            const int of = __builtin_ctzll(left) / L;
-            left &= L == 64 ? 0 : ~(0xffffull << of * L);
-            wave_fence();
-            const Chosen d = choose64<T, L, V>(a, (const T*)q.logits + (first + of) * q.ld, __shfl(top, of * L, 64), threadIdx.x, &places);
-            const int e = __shfl(d.e, l, 64);
-            const float at = __shfl(d.at, l, 64);
-            if ((int)threadIdx.x / L == of) c = {e, at};
-        }
+        [[maybe_unused]] const bool sure = choose<SOFT, SCORED, T, L, V>(a, from, z, b, most, top, total, l, place, &c);
+        if constexpr (SCORED)
+            for (uint64_t left = __ballot(!sure && !bad && real); left;) {
+                const int of = __builtin_ctzll(left) / L;
+                left &= L == 64 ? 0 : ~(0xffffull << of * L);
+                wave_fence();
+                const Chosen d = choose64<T, L, V>(a, (const T*)q.logits + (first + of) * q.ld, __shfl(top, of * L, 64), threadIdx.x, &places);
+                const int e = __shfl(d.e, l, 64);
+                const float at = __shfl(d.at, l, 64);
+                if ((int)threadIdx.x / L == of) c = {e, at};
+            }
         // the weights.  Renormalized: exp(z - largest chosen) under softmax; under sigmoid e^(z - m) / (1 + e^z) with m the largest chosen if that is negative, so
         // that scores which are no fp32 numbers keep their ratios
         const bool is = l < K && c.e >= 0;
