@@ -47,6 +47,29 @@ def test_equal_experts_on_both_sides_of_the_last_place(hip_device, scoring, low,
                 assert torch.equal(ids.cpu(), _order(z, k, scoring, bias)), (equal, k)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("T,E", SHAPES)
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_biases_as_small_as_scores_that_are_no_fp32_numbers(hip_device, scoring, T, E, dtype):
+    g = torch.Generator().manual_seed(E)
+    z = (-94 + 10 * torch.rand(T, E, generator=g)).to(dtype)
+    if scoring == "softmax":
+        z[:, 1] = 0.0
+    bias = 1e-38 * torch.randn(E, generator=g)
+    for k in (1, 2, 8):
+        _, ids = moe_route(z.to(hip_device), k, scoring=scoring, bias=bias.to(hip_device))
+        assert torch.equal(ids.cpu(), _order(z, k, scoring, bias)), k
+    if E % 4 == 0:                                         # groups by the sum of their two best, the best two of four
+        s = torch.sigmoid(z.double()) if scoring == "sigmoid" else torch.softmax(z.double(), 1)
+        c = (s + bias.double()).view(T, 4, E // 4)
+        best = c.sort(dim=2, descending=True)[0]
+        kept = (best[..., 0] + (best[..., 1] if E > 4 else 0.0)).sort(dim=1, descending=True, stable=True)[1][:, :2]
+        out = torch.ones(T, 4, dtype=torch.bool).scatter_(1, kept, False)
+        want = c.masked_fill(out[:, :, None], -math.inf).view(T, E).sort(dim=1, descending=True, stable=True)[1][:, :4]
+        _, ids = moe_route(z.to(hip_device), 4, scoring=scoring, bias=bias.to(hip_device), num_groups=4, top_groups=2, group_score="sum2")
+        assert torch.equal(ids.cpu(), want)
+
+
 @pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
 @pytest.mark.parametrize("T,E", [(4096, 256), (300, 128), (3, 1024)])
 def test_a_router_that_starts_at_zero(hip_device, T, E, scoring):

@@ -43,7 +43,8 @@ struct RouteGradArgs {
 // the definition (every score in 64 bits: 524 us).  Groups by two scores likewise, at the border between those that stay and those that go.  Errors, in steps of
 // 2^-24 of a score: sigmoid 4 for the exponential, 2 for sum and quotient; softmax 88 for the difference in the exponent (below that there is no score), 4, 22 for
 // the sum (16 terms a lane, 6 steps), 1; one more, of itself, for the sum with the bias.
-constexpr float kSigmoidError = 0x1p-20f, kSoftmaxError = 0x1p-17f;
+// Scores below 2^-125 may be 0 here: what lies nearer than kNoScore is told apart in 64 bits too.
+constexpr float kSigmoidError = 0x1p-20f, kSoftmaxError = 0x1p-17f, kNoScore = 0x1p-120f;
 
 template <int L>
 struct Lanes {
@@ -344,7 +345,7 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const f
             least = -A::largest(-least);
             most = A::largest(most);
             // (two scores and the sums with the bias on either side)
-            if (most != kOut && !(least - most > 2 * error * (fabsf(least) + fabsf(most) + 4 * bias_most))) sure = false;
+            if (most != kOut && !(least - most > 2 * error * (fabsf(least) + fabsf(most) + 4 * bias_most) + kNoScore)) sure = false;
         }
 #pragma unroll
         for (int j = 0; j < V / 4; ++j) {
@@ -402,7 +403,7 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const f
         const float y = A::next(c.at);
         const int f = A::next(c.e);
         bool tied = false;
-        if (l + 1 < picks && c.e >= 0 && f >= 0 && !(c.at - y > error * (fabsf(c.at) + fabsf(y) + 2 * bias_most))) {
+        if (l + 1 < picks && c.e >= 0 && f >= 0 && !(c.at - y > error * (fabsf(c.at) + fabsf(y) + 2 * bias_most) + kNoScore)) {
             const bool same = logit(row, c.e) == logit(row, f) && q.bias[c.e] == q.bias[f];
             sure &= same;
             tied = same && l == K - 1;
@@ -417,7 +418,7 @@ __device__ __forceinline__ bool choose(const RouteArgs& a, const T* row, const f
                 const float ze = logit(row, e), be = q.bias[e];
                 if (ze == kOut || be == kOut || (ze == zl && be == bl)) continue;
                 const float x = (SOFT ? near_exp(ze - top) * over : __builtin_amdgcn_rcpf(1.0f + near_exp(-ze))) + be;
-                if (!(fabsf(x - at) > error * (fabsf(x) + fabsf(at) + 2 * bias_most))) sure = false;
+                if (!(fabsf(x - at) > error * (fabsf(x) + fabsf(at) + 2 * bias_most) + kNoScore)) sure = false;
             }
         }
     }
