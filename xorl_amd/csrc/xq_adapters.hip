@@ -15,14 +15,15 @@ namespace {
 // second one takes sums that are no numbers again; 0 to 2 % of a call).
 //
 // What bounds it: few rows, the latency of two launches that each wait for memory two or three times (one row 8.7 us, 48 of 128 adapters 10.2); many, memory: 16384 rows of
-// prompts, 12288 by 4096, rank 64, read and write 0.68 GB, 139 us at a copy's rate, and take 176 (down 104 us, up 73).  Between them (2049 rows, 46 us against 27) the
-// blocks are too few to keep all of memory busy and the whole is three or four of their lifetimes.
+// prompts, 12288 by 4096, rank 64, read and write 0.68 GB, 139 us at a copy's rate, and take 176 (down 104 us, up 73).  Between them (2049 rows, 4096 by 12288, fp32 rank 16: 46 us
+// against 27) the down launch has too few blocks to keep memory busy (12 us against 4 of bytes), the up launch is within a third of its bytes (30 against 23).
 //
-// A tile is rows of one adapter.  Up to kLeaderRows rows in any order: a tile belongs to the row that is the first, 17th, 33rd .. of its adapter, and the first
-// launch's blocks find the tiles themselves among the ids (no launch that sorts them), and leave them to the second where it has more than 64 rows to look at.  Up to 64 rows a block has one row to look at, then
-// four: half of all blocks would do no more than find that their row leads none (1024 rows 81 against 41 us, 64 rows 9.7 against 10.2).  More rows are taken in
+// A tile is rows of one adapter.  Up to kLeaderRows rows in any order: a tile belongs to the row that is the first, 17th, 33rd .. of its adapter, and blocks find the
+// tiles themselves among the ids (no launch that sorts them).  Up to 64 rows each launch does, and a block has one row to look at; from 65 on the first one leaves its tiles to the
+// second, and a block looks at four rows: half of all blocks would do no more than find that their row leads none (1024 rows 81 against 41 us, 64 rows 9.7 against 10.2).  More rows are taken in
 // windows of 16 or 64 that follow each other, and a window once for every adapter in it: of prompts' rows, each window has one or two.  By tiles against by windows, 4096 by
-// 4096, 8 adapters: rank 16, 256 rows in any order 16 and 49 us, 512 27 and 49, 1024 36 and 54; sorted by adapter 17 and 18, 27 and 18, 39 and 17.
+// 4096, 8 adapters: rank 16, 256 rows in any order 16 and 49 us, 512 27 and 49, 1024 36 and 54; sorted by adapter 17 and 18, 27 and 18, 39 and 17.  The order is not known when the
+// launches are made: at 512 rows tiles take 27 us whatever it is, windows 18 or 49; from 1024 on windows cost rows in any order 1.5 times as much and sorted ones less than half.
 constexpr int kLeaderRows = 512;
 constexpr int kMostParts = 16, kLeadsNone = -2;
 
@@ -296,7 +297,8 @@ __device__ __forceinline__ void down_tile(const AdapterArgs& a, int id, const in
 }
 
 // Blocks go to the eight XCDs in turn: neighbouring items, which are of one adapter as a rule, go to one of them, so that each reads few adapters through its L2
-// (16384 rows of 8 adapters whose A have 1.5 MB each: down 208 us in turn and 174 so, up 118 and 106)
+// (4096 by 4096, us so and in the order of launch: 1024 rows of 128 an adapter, rank 16 12.9 and 13.7, 4096 of 512, rank 32 30.7 and 32.0, 16384 of 2048, rank 64 in fp32 179 and
+// 181, rank 16 in fp32 103 and 101; 12288 by 4096, 16384 rows, rank 64 the same; 4096 by 12288, 2049 rows in fp32, rank 16 40.5 and 39.2, rank 64 132 and 119)
 __device__ __forceinline__ int64_t item_of(int64_t at, int64_t n) {
     const int64_t each = n / 8, rest = n - each * 8, xcd = at & 7, i = at >> 3;
     return xcd * each + min(xcd, rest) + i;

@@ -31,16 +31,18 @@ struct RouteGradArgs {
 };
 
 // What bounds it: a row is read once and a few numbers of it written, but a choice is a chain of maxima over lanes, about 1500 instructions for four rows of 256 with
-// groups and a bias.  Their issue is 41 of the 60 us that 65536 such rows take (the reads alone would be 14); 16384 rows of 128 take 8.4 us.  Small calls are one launch:
-// one row 4.5 us, 333 rows of 256 in groups 7.5.
+// groups and a bias.  Their issue is 41 of the 62 us that 65536 such rows take (the reads alone would be 14); 16384 rows of 128 take 7.4 us.  Small calls are one launch:
+// one row 4.2 us, 333 rows of 256 in groups 7.4 of a pass.
 //
 // L lanes have a row (16: four rows a wave, sums and maxima within a quarter of it are register moves), V logits each, four neighbours at a time; of 16 lanes each
 // next such round begins four lanes on, so that the experts of a few groups are not all in a few lanes.  A block is one wave: what goes through LDS needs no
 // barrier.  With one row a wave and the same steps 65536 rows in groups took 154 us.
 //
-// Without a bias the order is that of the logits, exactly.  A score with a bias is compared as fp32 where that tells the chosen apart from each other and from the
-// first that is left out: sums whose difference is within their error, of experts that differ in logit or bias, send the row to be done again in 64 bits, which is
-// the definition (every score in 64 bits: 524 us).  Groups by two scores likewise, at the border between those that stay and those that go.  Errors, in steps of
+// Without a bias the order is that of the logits, exactly.  A score with a bias is compared as fp32 where that tells the chosen apart from each other and from
+// those that are left out: sums whose difference is within their error, of experts that differ in logit or bias, send the row to be done again in 64 bits, which is
+// the definition (every score in 64 bits: 524 us).  Groups by two scores likewise, at the border between those that stay and those that go, equal groups too.  What that makes of
+// 65536 rows of 256 (us, a pass): in groups 57, where all logits and biases are equal 309, with biases of the type's lowest value, in whose error all scores lie, 236; without
+// groups 44, 134 and 166.  Errors, in steps of
 // 2^-24 of a score: sigmoid 4 for the exponential, 2 for sum and quotient; softmax 88 for the difference in the exponent (below that there is no score), 4, 22 for
 // the sum (16 terms a lane, 6 steps), 1; one more, of itself, for the sum with the bias.
 // Scores below 2^-125 may be 0 here: what lies nearer than kNoScore is told apart in 64 bits too.
