@@ -242,7 +242,7 @@ struct Linear {
         PyObject* bias_o = get(params, N.s_bias);
         if (bias_o && bias_o != Py_None) {
             const Tensor* bt = plain(bias_o);
-            if (!bt || bt->numel() != n) return false;
+            if (!bt || bt->numel() != n || !bt->data_ptr()) return false;        // (without memory it would count as absent)
             bias_grad = bt->requires_grad();
             bias = bt->scalar_type() == at::kBFloat16 && bt->is_contiguous() ? *bt : bt->detach().to(at::kBFloat16).contiguous();
         }
@@ -1122,7 +1122,7 @@ PyObject* moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (E < 1 || E > 1024 || scoring < 0 || group_score < 0 || groups < 1 || groups > 64 || E % groups || top_groups < 1 || top_groups > groups || k < 1 || k > 32 ||
             k > E / groups * top_groups || !(scale >= 0x1p-60 && scale <= 0x1p60))
             XQ_NONE;
-        if (bias && (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != E || bias->device() != z->device() || bias->is_neg())) XQ_NONE;
+        if (bias && (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != E || bias->device() != z->device() || bias->is_neg() || !bias->data_ptr())) XQ_NONE;
         const bool grad = at::GradMode::is_enabled() && z->requires_grad();
         c10::DeviceGuard guard(z->device());
         Tensor weights, ids;
