@@ -351,7 +351,10 @@ bool note_decode_forward(const Tensor& x, int64_t M) {
 }
 
 // ---- backward nodes: edges in the order of the inputs named in each
-Tensor cast_to(Tensor g, at::ScalarType dt) { return g.scalar_type() == dt ? g : g.to(dt); }
+Tensor cast_to(Tensor g, at::ScalarType dt) {
+    if (g.is_neg()) g = g.resolve_neg();                 // (a view whose memory holds the other sign)
+    return g.scalar_type() == dt ? g : g.to(dt);
+}
 
 struct QLoRALinearBackward : public Node {
     SavedVariable x_, su_, A_, B_;
@@ -577,11 +580,11 @@ struct AnyRows {
     void* ptr = nullptr;
     int64_t ld = 0, M = 0;
 
-    explicit AnyRows(const Tensor& x) : keep(x), ld(x.size(-1)) {
+    explicit AnyRows(const Tensor& x) : keep(x.is_neg() ? x.resolve_neg() : x), ld(x.size(-1)) {
         M = ld ? x.numel() / ld : 0;
         const int64_t width = ld;
-        if (!x.is_contiguous() && (!Rows::any_pitch(x, &ld) || ld < width)) {
-            keep = x.contiguous();
+        if (!keep.is_contiguous() && (!Rows::any_pitch(keep, &ld) || ld < width)) {
+            keep = keep.contiguous();
             ld = width;
         }
         ptr = keep.data_ptr();

@@ -19,7 +19,7 @@ from .functional import refuse_tangents
 
 
 def _rows(t: Tensor) -> Tensor:
-    t2 = t.reshape(-1, t.shape[-1])
+    t2 = t.resolve_neg().reshape(-1, t.shape[-1])
     return t2 if t2.stride(1) == 1 and (t2.shape[0] <= 1 or t2.stride(0) >= t2.shape[1]) else t2.contiguous()
 
 
@@ -38,7 +38,7 @@ def _problem(ids1: Tensor, V: int, H: int, dtype: torch.dtype, scale: float, pad
 def _fwd_impl(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
     dev = weight.device
     with torch.cuda.device(dev):
-        i1, w2 = ids.reshape(-1).contiguous(), _rows(weight)
+        i1, w2 = ids.reshape(-1).contiguous().resolve_neg(), _rows(weight)
         q = _problem(i1, w2.shape[0], w2.shape[1], weight.dtype, scale, -1)
         q.weight, q.ldw = w2.data_ptr(), _ld(w2)
         out = torch.empty((*ids.shape, weight.shape[1]), dtype=weight.dtype, device=dev)
@@ -49,7 +49,7 @@ def _fwd_impl(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
 def _bwd_impl(grad: Tensor, ids: Tensor, V: int, scale: float, padding_idx: int) -> Tensor:
     dev = grad.device
     with torch.cuda.device(dev):
-        i1, g2 = ids.reshape(-1).contiguous(), _rows(grad)
+        i1, g2 = ids.reshape(-1).contiguous().resolve_neg(), _rows(grad)
         if g2.shape[0] != i1.numel():
             raise _C.XqError("embedding: what the forward kept, or the gradient, is not that of this problem")
         q = _problem(i1, V, g2.shape[1], grad.dtype, scale, padding_idx)

@@ -410,19 +410,19 @@ def _adapters_problem(base2: Tensor, x2: Tensor, A: Tensor, B: Tensor, ids: Tens
 def _rows_in_place(x: Tensor) -> Optional[Tensor]:
     """x as rows at multiples of 16 bytes that share its memory, or None"""
     x2 = x.flatten(0, -2) if x.dim() > 1 and x.is_contiguous() else x if x.dim() == 2 else x.unsqueeze(0) if x.dim() == 1 else None
-    ok = x2 is not None and x2.stride(1) == 1 and (x2.shape[0] <= 1 or (x2.stride(0) % 8 == 0 and x2.stride(0) >= x2.shape[1])) and x2.data_ptr() % 16 == 0
+    ok = x2 is not None and not x2.is_neg() and x2.stride(1) == 1 and (x2.shape[0] <= 1 or (x2.stride(0) % 8 == 0 and x2.stride(0) >= x2.shape[1])) and x2.data_ptr() % 16 == 0
     return x2 if ok else None
 
 
 def _adapters_rows(x: Tensor) -> Tensor:
-    x2 = _as_2d(x)
+    x2 = _as_2d(x.resolve_neg())
     if x2.shape[0] > 1 and x2.stride(0) < x2.shape[1]:           # (an expanded row)
         x2 = x2.contiguous()
     return x2 if x2.data_ptr() % 16 == 0 else x2.clone()
 
 
 def _aligned(t: Tensor) -> Tensor:
-    t = t.contiguous()
+    t = t.contiguous().resolve_neg()
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
@@ -436,8 +436,8 @@ def _adapters_impl(base: Tensor, x: Tensor, A: Tensor, B: Tensor, ids: Tensor, s
     _one_device(base, x, A, B, ids, scalings, out)         # (a traced call comes here from the operator's dispatcher, which goes by any one of them)
     dev = x.device
     with torch.cuda.device(dev):
-        x2, base2, i1 = _adapters_rows(x), _adapters_rows(base), ids.reshape(-1).contiguous()
-        A, B, scalings = _aligned(A), _aligned(B), scalings.contiguous()
+        x2, base2, i1 = _adapters_rows(x), _adapters_rows(base), ids.reshape(-1).contiguous().resolve_neg()
+        A, B, scalings = _aligned(A), _aligned(B), scalings.contiguous().resolve_neg()
         res = torch.empty(base.shape, dtype=torch.bfloat16, device=dev) if out is None else out
         out2 = _rows_in_place(res)
         if out2 is None:
@@ -509,7 +509,7 @@ def lora_adapters(base: Tensor, x: Tensor, lora_A: Tensor, lora_B: Tensor, adapt
         return y if out is None else out.copy_(y)
     if out is not None:
         if _rows_in_place(out) is None:
-            raise _C.XqError(f"lora_adapters: out must be made of rows at multiples of 16 bytes, got strides {out.stride()}")
+            raise _C.XqError(f"lora_adapters: out must be made of rows at multiples of 16 bytes, got strides {out.stride()}{' of a negated view' if out.is_neg() else ''}")
         a, b = _span(out)
         for t in (*tensors, adapter_ids):
             c, d = _span(t)

@@ -53,7 +53,7 @@ def route_build(selected_experts: Tensor, num_experts: int):
 # the choice of experts
 # ---------------------------------------------------------------------------
 def _route_rows(z: Tensor) -> Tensor:
-    z2 = z.reshape(-1, z.shape[-1])
+    z2 = z.resolve_neg().reshape(-1, z.shape[-1])
     return z2 if z2.stride(-1) == 1 and (z2.shape[0] <= 1 or z2.stride(0) >= z2.shape[1]) else z2.contiguous()
 
 
@@ -70,7 +70,7 @@ def _route_fwd_impl(z: Tensor, bias: Optional[Tensor], options) -> Tuple[Tensor,
     dev = z.device
     with torch.cuda.device(dev):
         z2 = _route_rows(z)
-        b = None if bias is None else bias.contiguous()
+        b = None if bias is None else bias.contiguous().resolve_neg()
         shape = (*z.shape[:-1], options[0])
         weights = torch.empty(shape, dtype=torch.float32, device=dev)
         ids = torch.empty(shape, dtype=torch.int64, device=dev)
@@ -84,7 +84,7 @@ def _route_bwd_impl(grad: Tensor, weights: Tensor, ids: Tensor, z: Tensor, num_e
     dev = weights.device
     with torch.cuda.device(dev):
         n = weights.numel() // options[0]
-        g, w, i = grad.to(torch.float32).contiguous(), weights.contiguous(), ids.contiguous()
+        g, w, i = grad.to(torch.float32).contiguous().resolve_neg(), weights.contiguous(), ids.contiguous()
         z2 = _route_rows(z) if _route_keeps_logits(options) else None
         if g.numel() != w.numel() or i.numel() != w.numel() or (z2 is not None and (tuple(z2.shape) != (n, num_experts) or z2.dtype != dtype)):
             raise _C.XqError("moe_route: what the forward kept, or the gradient, is not that of this problem")
