@@ -5,9 +5,9 @@ import torch
 from torch._subclasses.fake_tensor import FakeTensorMode
 
 from xorl_amd import _C
-from xorl_amd.embedding_functional import embedding
-from xorl_amd.functional import lora_adapters
-from xorl_amd.moe_functional import _route_problem, moe_route
+from xorl_amd.embedding_functional import _bwd_impl, _fwd_impl, embedding
+from xorl_amd.functional import _adapters_impl, lora_adapters
+from xorl_amd.moe_functional import _route_bwd_impl, _route_fwd_impl, _route_problem, moe_route
 
 BF = torch.bfloat16
 
@@ -47,8 +47,6 @@ def test_a_traced_call_refuses_an_out_of_another_kind(monkeypatch, out, match):
 @pytest.mark.parametrize("which", range(6))
 def test_the_operator_itself_refuses_host_memory(which):
     """What a traced call leaves in a program is dispatched by any one of its tensors: without a device that is all of them, and the rest is refused here"""
-    from xorl_amd.functional import _adapters_impl
-
     with FakeTensorMode():
         shapes = ((3, 32, BF), (3, 64, BF), (5, 4, 64, BF), (5, 32, 4, BF), (3, torch.int32), (5, torch.float32))
         a = [torch.empty(s[:-1], dtype=s[-1], device="cpu" if i == which else "cuda") for i, s in enumerate(shapes)]
@@ -110,3 +108,53 @@ def test_the_workspace_holds_tiles_only_where_they_are_kept():
     """[rows][ranks, padded to 16] in fp32, of one part of K; from 65 rows on each row's tile beside it"""
     need = _C.lib().xq_adapters_workspace_bytes
     assert [need(M, 32, 64, 5) for M in (4, 64, 65, 512, 513)] == [256, 64 * 64, 65 * 128, 512 * 128, 513 * 64]
+
+
+# ---- the custom operators by themselves: what a kernel would read or write out of bounds, or as another type, is refused before anything runs
+def _z(*shape, dtype=torch.float32):
+    return torch.zeros(*shape, dtype=dtype)
+
+
+OPTIONS = (2, 1, 1, 1, 1, True, 1.0)
+
+
+@pytest.mark.parametrize("z,bias", [(_z(3, 8, dtype=torch.float16), None), (_z(3, 8), _z(7)), (_z(3, 8), _z(8, dtype=torch.float64)), (_z(3, 8), _z(8, dtype=BF)), (_z(3, 0), None),
+                                    (torch.tensor(1.0), None)])
+def test_the_router_operator_refuses(z, bias):
+    with pytest.raises(_C.XqError, match="moe_route"):
+        _route_fwd_impl(z, bias, OPTIONS)
+
+
+def test_the_routers_gradient_operator_refuses():
+    def call(grad=_z(3, 2), w=_z(3, 2), ids=_z(3, 2, dtype=torch.int64), options=OPTIONS):
+        _route_bwd_impl(grad, w, ids, _z(3, 8), 8, torch.float32, options)
+
+    for kw in (dict(w=_z(3, 2, dtype=torch.float64)), dict(ids=_z(3, 2, dtype=torch.int32)), dict(w=_z(3, 4)), dict(ids=_z(2, 2, dtype=torch.int64)), dict(grad=_z(3, 1)), dict(grad=_z(6)),
+               dict(grad=_z(3, 4), w=_z(3, 4), ids=_z(3, 4, dtype=torch.int64)), dict(options=(0, *OPTIONS[1:])), dict(w=_z(6), ids=_z(6, dtype=torch.int64), grad=_z(6))):
+        with pytest.raises(_C.XqError, match="not that of this problem"):
+            call(**kw)
+    with pytest.raises(RuntimeError, match="HIP device only"):
+        call()
+
+
+@pytest.mark.parametrize("i", range(6))
+def test_the_adapters_operator_refuses(i):
+    good = (_z(3, 32, dtype=BF), _z(3, 64, dtype=BF), _z(5, 4, 64), _z(5, 32, 4), _z(3, dtype=torch.int32), _z(5))
+    bad = ((_z(3, 16, dtype=BF), _z(2, 32, dtype=BF), _z(3, 32)), (_z(3, 128, dtype=BF), _z(3, 64)), (_z(5, 4, 32), _z(4, 4, 64), _z(5, 4, 64, dtype=torch.float16)),
+           (_z(5, 32, 3), _z(5, 31, 4), _z(5, 32, 4, dtype=BF)), (_z(2, dtype=torch.int32), _z(3, dtype=torch.int16), _z(3)), (_z(4), _z(5, dtype=torch.float64)))
+    for t in bad[i]:
+        with pytest.raises(_C.XqError, match="lora_adapters"):
+            _adapters_impl(*good[:i], t, *good[i + 1:])
+
+
+def test_the_embedding_operators_refuse():
+    ids = _z(3, dtype=torch.int64)
+    for i, w in ((ids, _z(5, 4, dtype=torch.float16)), (ids, _z(5)), (ids, _z(0, 4)), (ids, _z(5, 0)), (_z(3), _z(5, 4)), (_z(3, dtype=torch.int16), _z(5, 4))):
+        with pytest.raises(_C.XqError, match="embedding"):
+            _fwd_impl(i, w, 1.0)
+    for g, i, V in ((_z(3, 4, dtype=torch.float16), ids, 5), (torch.tensor(1.0), ids, 5), (_z(3, 0), ids, 5), (_z(3, 4), _z(3), 5), (_z(3, 4), ids, 0)):
+        with pytest.raises(_C.XqError, match="not that of this problem"):
+            _bwd_impl(g, i, V, 1.0, -1)
+    for call in (lambda: _fwd_impl(ids, _z(5, 4), 1.0), lambda: _bwd_impl(_z(3, 4), ids, 5, 1.0, -1), lambda: _route_fwd_impl(_z(3, 8), _z(8), OPTIONS)):
+        with pytest.raises(RuntimeError, match="HIP device only"):
+            call()

@@ -35,7 +35,23 @@ def _problem(ids1: Tensor, V: int, H: int, dtype: torch.dtype, scale: float, pad
     return q
 
 
+def _check(ids: Tensor, weight: Tensor) -> None:
+    if weight.dtype not in (torch.bfloat16, torch.float32) or weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
+        raise _C.XqError(f"embedding: the weight [V, H] must be bf16 or fp32 and not empty, got {weight.dtype} {tuple(weight.shape)}")
+    if ids.dtype not in (torch.int64, torch.int32):
+        raise _C.XqError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
+
+
+def _one_device(ids: Tensor, other: Tensor) -> None:
+    _C.require_hip(ids, other)
+    if ids.device != other.device:
+        raise _C.XqError(f"embedding: the tensors are on {ids.device} and {other.device}")
+
+
+# (the operators can be called by themselves: what they read is checked here too)
 def _fwd_impl(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
+    _check(ids, weight)
+    _one_device(ids, weight)
     dev = weight.device
     with torch.cuda.device(dev):
         i1, w2 = ids.reshape(-1).contiguous().resolve_neg(), _rows(weight)
@@ -47,6 +63,9 @@ def _fwd_impl(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
 
 
 def _bwd_impl(grad: Tensor, ids: Tensor, V: int, scale: float, padding_idx: int) -> Tensor:
+    if grad.dtype not in (torch.bfloat16, torch.float32) or grad.dim() < 1 or grad.shape[-1] < 1 or ids.dtype not in (torch.int64, torch.int32) or V < 1:
+        raise _C.XqError("embedding: what the forward kept, or the gradient, is not that of this problem")
+    _one_device(ids, grad)
     dev = grad.device
     with torch.cuda.device(dev):
         i1, g2 = ids.reshape(-1).contiguous().resolve_neg(), _rows(grad)
@@ -114,10 +133,7 @@ def embedding(ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: O
     # what the native path leaves: traced calls, tensor subclasses, and the errors
     if isinstance(scale, Tensor):
         raise _C.XqError("embedding: scale is a number, not a tensor")
-    if weight.dtype not in (torch.bfloat16, torch.float32) or weight.dim() != 2 or weight.shape[0] < 1 or weight.shape[1] < 1:
-        raise _C.XqError(f"embedding: the weight [V, H] must be bf16 or fp32 and not empty, got {weight.dtype} {tuple(weight.shape)}")
-    if ids.dtype not in (torch.int64, torch.int32):
-        raise _C.XqError(f"embedding: ids must be int64 or int32, got {ids.dtype}")
+    _check(ids, weight)
     V = weight.shape[0]
     if padding_idx is not None and (not -V <= padding_idx < V or (isinstance(padding_idx, float) and not padding_idx.is_integer())):
         raise _C.XqError(f"embedding: padding_idx {padding_idx} is no row of a weight of {V}")
@@ -125,9 +141,7 @@ def embedding(ids: Tensor, weight: Tensor, *, scale: float = 1.0, padding_idx: O
         raise _C.XqError(f"embedding: scale must be finite in fp32, got {scale}")
     if not torch.compiler.is_compiling():
         refuse_tangents(weight)
-    _C.require_hip(ids, weight)
-    if ids.device != weight.device:
-        raise _C.XqError(f"embedding: ids and weight are on {ids.device} and {weight.device}")
+    _one_device(ids, weight)
     pad = -1 if padding_idx is None else int(padding_idx) % V
     if torch.is_grad_enabled() and weight.requires_grad:
         return EmbeddingFunction.apply(ids, weight, float(scale), pad)

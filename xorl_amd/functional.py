@@ -426,14 +426,31 @@ def _aligned(t: Tensor) -> Tensor:
     return t if t.data_ptr() % 16 == 0 else t.clone()
 
 
-def _one_device(*tensors: Optional[Tensor]) -> None:
+def _check_adapters(base: Tensor, x: Tensor, lora_A: Tensor, lora_B: Tensor, adapter_ids: Tensor, scalings: Tensor, out: Optional[Tensor] = None) -> None:
+    if base.dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
+        raise _C.XqError(f"lora_adapters: base and x must be bf16, got {base.dtype} and {x.dtype}")
+    if lora_A.dtype != lora_B.dtype or lora_A.dtype not in (torch.float32, torch.bfloat16) or scalings.dtype != torch.float32:
+        raise _C.XqError(f"lora_adapters: the factors must both be fp32 or both bf16 and the scalings fp32, got {lora_A.dtype}, {lora_B.dtype} and {scalings.dtype}")
+    if adapter_ids.dtype not in (torch.int32, torch.int64):
+        raise _C.XqError(f"lora_adapters: adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
+    if (lora_A.dim() != 3 or lora_B.dim() != 3 or x.dim() < 1 or base.dim() < 1 or x.shape[:-1] != base.shape[:-1] or adapter_ids.shape != x.shape[:-1]
+            or tuple(lora_A.shape) != (lora_A.shape[0], lora_B.shape[2], x.shape[-1]) or tuple(lora_B.shape[:2]) != (lora_A.shape[0], base.shape[-1])
+            or tuple(scalings.shape) != (lora_A.shape[0],)):
+        raise _C.XqError(f"lora_adapters: base [.., N], x [.., K], lora_A [n, r, K], lora_B [n, N, r], adapter_ids [..] and scalings [n] do not go together: {tuple(base.shape)}, "
+                         f"{tuple(x.shape)}, {tuple(lora_A.shape)}, {tuple(lora_B.shape)}, {tuple(adapter_ids.shape)}, {tuple(scalings.shape)}")
+    if x.shape[-1] < 64 or x.shape[-1] % 64 or base.shape[-1] < 16 or base.shape[-1] % 16 or not 1 <= lora_A.shape[1] <= MAX_FUSED_RANK:
+        raise _C.XqError(f"lora_adapters: in_features must be a multiple of 64, out_features of 16 and the rank 1 to {MAX_FUSED_RANK}, got {x.shape[-1]}, {base.shape[-1]} "
+                         f"and {lora_A.shape[1]}")
+    tensors = (base, x, lora_A, lora_B, adapter_ids, scalings, out)
     _C.require_hip(*tensors)
-    if any(t is not None and t.device != tensors[0].device for t in tensors):
+    if any(t is not None and t.device != base.device for t in tensors):
         raise _C.XqError("lora_adapters: the tensors are on different devices")
+    if out is not None and (out.dtype != torch.bfloat16 or out.shape != base.shape):
+        raise _C.XqError(f"lora_adapters: out must be bf16 {tuple(base.shape)}, got {out.dtype} {tuple(out.shape)}")
 
 
 def _adapters_impl(base: Tensor, x: Tensor, A: Tensor, B: Tensor, ids: Tensor, scalings: Tensor, out: Optional[Tensor] = None) -> Tensor:
-    _one_device(base, x, A, B, ids, scalings, out)         # (a traced call comes here from the operator's dispatcher, which goes by any one of them)
+    _check_adapters(base, x, A, B, ids, scalings, out)     # (the operator can be called by itself, and its dispatcher goes by any one of the tensors)
     dev = x.device
     with torch.cuda.device(dev):
         x2, base2, i1 = _adapters_rows(x), _adapters_rows(base), ids.reshape(-1).contiguous().resolve_neg()
@@ -485,25 +502,9 @@ def lora_adapters(base: Tensor, x: Tensor, lora_A: Tensor, lora_B: Tensor, adapt
     tensors = (base, x, lora_A, lora_B, scalings)
     if torch.is_grad_enabled() and any(t.requires_grad for t in (*tensors, *(() if out is None else (out,)))):
         raise _C.XqError("lora_adapters is forward-only: call it under torch.no_grad()")
-    if base.dtype != torch.bfloat16 or x.dtype != torch.bfloat16:
-        raise _C.XqError(f"lora_adapters: base and x must be bf16, got {base.dtype} and {x.dtype}")
-    if lora_A.dtype != lora_B.dtype or lora_A.dtype not in (torch.float32, torch.bfloat16) or scalings.dtype != torch.float32:
-        raise _C.XqError(f"lora_adapters: the factors must both be fp32 or both bf16 and the scalings fp32, got {lora_A.dtype}, {lora_B.dtype} and {scalings.dtype}")
-    if adapter_ids.dtype not in (torch.int32, torch.int64):
-        raise _C.XqError(f"lora_adapters: adapter_ids must be int32 or int64, got {adapter_ids.dtype}")
-    if (lora_A.dim() != 3 or lora_B.dim() != 3 or x.dim() < 1 or base.dim() < 1 or x.shape[:-1] != base.shape[:-1] or adapter_ids.shape != x.shape[:-1]
-            or tuple(lora_A.shape) != (lora_A.shape[0], lora_B.shape[2], x.shape[-1]) or tuple(lora_B.shape[:2]) != (lora_A.shape[0], base.shape[-1])
-            or tuple(scalings.shape) != (lora_A.shape[0],)):
-        raise _C.XqError(f"lora_adapters: base [.., N], x [.., K], lora_A [n, r, K], lora_B [n, N, r], adapter_ids [..] and scalings [n] do not go together: {tuple(base.shape)}, "
-                         f"{tuple(x.shape)}, {tuple(lora_A.shape)}, {tuple(lora_B.shape)}, {tuple(adapter_ids.shape)}, {tuple(scalings.shape)}")
-    if x.shape[-1] < 64 or x.shape[-1] % 64 or base.shape[-1] < 16 or base.shape[-1] % 16 or not 1 <= lora_A.shape[1] <= MAX_FUSED_RANK:
-        raise _C.XqError(f"lora_adapters: in_features must be a multiple of 64, out_features of 16 and the rank 1 to {MAX_FUSED_RANK}, got {x.shape[-1]}, {base.shape[-1]} "
-                         f"and {lora_A.shape[1]}")
     if not torch.compiler.is_compiling():
         refuse_tangents(*tensors, out)
-    _one_device(*tensors, adapter_ids, out)
-    if out is not None and (out.dtype != torch.bfloat16 or out.shape != base.shape):
-        raise _C.XqError(f"lora_adapters: out must be bf16 {tuple(base.shape)}, got {out.dtype} {tuple(out.shape)}")
+    _check_adapters(base, x, lora_A, lora_B, adapter_ids, scalings, out)
     if torch.compiler.is_compiling():
         y = _adapters_op(base.detach(), x.detach(), lora_A.detach(), lora_B.detach(), adapter_ids, scalings.detach())
         return y if out is None else out.copy_(y)

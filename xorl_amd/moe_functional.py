@@ -66,7 +66,26 @@ def _route_problem(z2: Optional[Tensor], n_tokens: int, num_experts: int, dtype:
     return q
 
 
+def _check_route(z: Tensor, bias: Optional[Tensor]) -> None:
+    if z.dtype not in (torch.bfloat16, torch.float32) or z.dim() < 1:
+        raise _C.XqError(f"moe_route: logits [.., E] must be bf16 or fp32, got {z.dtype} {tuple(z.shape)}")
+    E = z.shape[-1]
+    if not 1 <= E <= 1024:
+        raise _C.XqError(f"moe_route: 1 to 1024 experts, got {E}")
+    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
+        raise _C.XqError(f"moe_route: the bias must be fp32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
+
+
+def _one_device(*tensors: Optional[Tensor]) -> None:
+    _C.require_hip(*tensors)
+    if any(t is not None and t.device != tensors[0].device for t in tensors):
+        raise _C.XqError(f"moe_route: the tensors are on different devices, {[str(t.device) for t in tensors if t is not None]}")
+
+
+# (the operators can be called by themselves: what they read is checked here too)
 def _route_fwd_impl(z: Tensor, bias: Optional[Tensor], options) -> Tuple[Tensor, Tensor]:
+    _check_route(z, bias)
+    _one_device(z, bias)
     dev = z.device
     with torch.cuda.device(dev):
         z2 = _route_rows(z)
@@ -81,6 +100,10 @@ def _route_fwd_impl(z: Tensor, bias: Optional[Tensor], options) -> Tuple[Tensor,
 
 def _route_bwd_impl(grad: Tensor, weights: Tensor, ids: Tensor, z: Tensor, num_experts: int, dtype: torch.dtype, options) -> Tensor:
     """z without elements: a backward that needs no logits"""
+    if (weights.dtype != torch.float32 or ids.dtype != torch.int64 or weights.dim() < 1 or weights.shape[-1] != options[0] or options[0] < 1 or ids.shape != weights.shape
+            or grad.shape != weights.shape):
+        raise _C.XqError("moe_route: what the forward kept, or the gradient, is not that of this problem")
+    _one_device(weights, ids, grad, z)
     dev = weights.device
     with torch.cuda.device(dev):
         n = weights.numel() // options[0]
@@ -180,13 +203,8 @@ def moe_route(router_logits: Tensor, top_k: int, *, scoring: str = "softmax", bi
         raise _C.XqError(f"moe_route: scoring must be one of {sorted(_C.ROUTE_SCORINGS)}, got {scoring!r}")
     if options[4] < 0:
         raise _C.XqError(f"moe_route: group_score must be one of {sorted(_C.ROUTE_GROUP_SCORES)}, got {group_score!r}")
-    if router_logits.dtype not in (torch.bfloat16, torch.float32) or router_logits.dim() < 1:
-        raise _C.XqError(f"moe_route: logits [.., E] must be bf16 or fp32, got {router_logits.dtype} {tuple(router_logits.shape)}")
+    _check_route(router_logits, bias)
     E = router_logits.shape[-1]
-    if not 1 <= E <= 1024:
-        raise _C.XqError(f"moe_route: 1 to 1024 experts, got {E}")
-    if bias is not None and (bias.dtype != torch.float32 or tuple(bias.shape) != (E,)):
-        raise _C.XqError(f"moe_route: the bias must be fp32 [{E}], got {bias.dtype} {tuple(bias.shape)}")
     if not 1 <= num_groups <= 64 or E % num_groups or not 1 <= top_groups <= num_groups:
         raise _C.XqError(f"moe_route: {E} experts cannot be taken in {num_groups} groups (at most 64, of equal size) of which {top_groups} count")
     if not 1 <= top_k <= min(32, E // num_groups * top_groups):
@@ -195,9 +213,7 @@ def moe_route(router_logits: Tensor, top_k: int, *, scoring: str = "softmax", bi
         raise _C.XqError(f"moe_route: scale must be from 2^-60 to 2^60, got {scale}")
     if not torch.compiler.is_compiling():
         refuse_tangents(router_logits, bias)
-    _C.require_hip(router_logits, bias)
-    if bias is not None and bias.device != router_logits.device:
-        raise _C.XqError(f"moe_route: logits and bias are on {router_logits.device} and {bias.device}")
+    _one_device(router_logits, bias)
     options = (int(top_k), options[1], int(num_groups), int(top_groups), options[4], options[5], float(scale))
     b = None if bias is None else bias.detach()
     if torch.is_grad_enabled() and router_logits.requires_grad:
