@@ -33,6 +33,27 @@ def test_a_linear_whose_bias_was_freed_is_refused(hip_device):
             m(x)
 
 
+def _freed(t):
+    """t behind eight others of a storage that is freed: its address is not 0"""
+    flat = torch.cat([t.new_zeros(8), t.reshape(-1)])
+    view = flat[8:].view(t.shape)
+    flat.untyped_storage().resize_(0)
+    return view
+
+
+def test_views_into_freed_memory_are_refused(hip_device):
+    z, bias = torch.randn(6, 8, device=hip_device), torch.randn(8, device=hip_device)
+    w, ids = torch.randn(10, 16, device=hip_device), torch.tensor([3, 0, 9], device=hip_device)
+    a = [torch.zeros(4, 16, dtype=BF, device=hip_device), torch.zeros(4, 64, dtype=BF, device=hip_device), torch.zeros(2, 4, 64, device=hip_device), torch.zeros(2, 16, 4, device=hip_device),
+         torch.zeros(4, dtype=torch.int32, device=hip_device), torch.ones(2, device=hip_device)]
+    calls = [lambda: moe_route(_freed(z), 2), lambda: moe_route(z, 2, bias=_freed(bias)), lambda: embedding(_freed(ids), w), lambda: embedding(ids, _freed(w)),
+             lambda: embedding(ids, _freed(w).requires_grad_(True))]
+    calls += [lambda i=i: lora_adapters(*a[:i], _freed(a[i]), *a[i + 1:]) for i in range(6)]
+    for call in calls:
+        with pytest.raises(_C.XqError, match="no memory"):
+            call()
+
+
 def _negated(t):
     """a view that stands for t: its memory holds the other sign"""
     return torch._neg_view(t.neg())

@@ -494,6 +494,12 @@ bool in_storage(const Tensor& t) {
     return (last + 1) * (int64_t)t.element_size() <= (int64_t)t.storage().nbytes();
 }
 
+// the tensors of a forward whose memory was freed or cut under them: a view into it has an address all the same
+void check_held(const char* who, std::initializer_list<const Tensor*> ts) {
+    for (const Tensor* t : ts)
+        if (t && !in_storage(*t)) throw ArgError(std::string(who) + ": a tensor has no memory of its own (any more): it was freed or resized");
+}
+
 // whether a stream of torch's is part of this capture (the default stream, which has id 0, never is, and may not be asked while one goes on)
 bool in_capture(const c10::Stream& s, unsigned long long id) {
     if (s.id() == 0) return false;
@@ -1125,7 +1131,8 @@ PyObject* moe_route(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (E < 1 || E > 1024 || scoring < 0 || group_score < 0 || groups < 1 || groups > 64 || E % groups || top_groups < 1 || top_groups > groups || k < 1 || k > 32 ||
             k > E / groups * top_groups || !(scale >= 0x1p-60 && scale <= 0x1p60))
             XQ_NONE;
-        if (bias && (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != E || bias->device() != z->device() || bias->is_neg() || !bias->data_ptr())) XQ_NONE;
+        if (bias && (bias->scalar_type() != at::kFloat || bias->dim() != 1 || bias->size(0) != E || bias->device() != z->device() || bias->is_neg())) XQ_NONE;
+        check_held("moe_route", {z, bias});
         const bool grad = at::GradMode::is_enabled() && z->requires_grad();
         c10::DeviceGuard guard(z->device());
         Tensor weights, ids;
@@ -1185,6 +1192,7 @@ PyObject* adapters(PyObject*, PyObject* const* args, Py_ssize_t n) {
         if (lead != base->sizes().slice(0, base->dim() - 1) || lead != ids->sizes()) XQ_NONE;
         for (const Tensor* t : {base, A, B, ids, s})
             if (t->device() != x->device()) XQ_NONE;
+        check_held("lora_adapters", {base, x, A, B, ids, s});
         auto aligned = [](const Tensor& t) { return (uintptr_t)t.data_ptr() % 16 == 0; };
         // (rows and factors that have to be copied first, and a base that cannot be written, are the Python path's)
         int64_t ldx = K, ldb = N;
@@ -1236,6 +1244,7 @@ PyObject* embedding(PyObject*, PyObject* const* args, Py_ssize_t n) {
             if (pad < 0) pad += V;
         }
         if (!(std::fabs(scale) <= 3.4e38)) XQ_NONE;
+        check_held("embedding", {ids, w});
         const bool grad = at::GradMode::is_enabled() && w->requires_grad();
         c10::DeviceGuard guard(w->device());
         Tensor out;
