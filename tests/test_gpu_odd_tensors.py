@@ -1,5 +1,6 @@
 """GPU: arguments whose memory is not what they stand for: freed, or with the other sign."""
 
+import numpy as np
 import pytest
 import torch
 
@@ -49,6 +50,9 @@ def test_views_into_freed_memory_are_refused(hip_device):
     calls = [lambda: moe_route(_freed(z), 2), lambda: moe_route(z, 2, bias=_freed(bias)), lambda: embedding(_freed(ids), w), lambda: embedding(ids, _freed(w)),
              lambda: embedding(ids, _freed(w).requires_grad_(True))]
     calls += [lambda i=i: lora_adapters(*a[:i], _freed(a[i]), *a[i + 1:]) for i in range(6)]
+    # what the compiled host path leaves to Python
+    calls += [lambda: moe_route(_freed(z), np.int64(2)), lambda: embedding(_freed(ids), w, scale=np.float32(1.0)), lambda: torch.ops.xq.embedding_fwd(ids, _freed(w), 1.0)]
+    calls += [lambda i=i: lora_adapters(*a[:i], _freed(a[i]), *a[i + 1:], out=torch.empty_like(a[0])) for i in range(6)] + [lambda: lora_adapters(*a, out=_freed(a[0]))]
     for call in calls:
         with pytest.raises(_C.XqError, match="no memory"):
             call()

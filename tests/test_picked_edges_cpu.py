@@ -158,3 +158,19 @@ def test_the_embedding_operators_refuse():
     for call in (lambda: _fwd_impl(ids, _z(5, 4), 1.0), lambda: _bwd_impl(_z(3, 4), ids, 5, 1.0, -1), lambda: _route_fwd_impl(_z(3, 8), _z(8), OPTIONS)):
         with pytest.raises(RuntimeError, match="HIP device only"):
             call()
+
+
+def test_memory_that_was_freed_or_cut_is_found():
+    flat = torch.zeros(24)
+    view, rest = flat[8:].view(4, 4), flat[8:].view(4, 4).t()[:, 1:]
+    inside, first, none = view[:, :3], view[:1], view[:0]          # (views of freed memory cannot be made)
+    _C.check_held("x", flat, view, rest, None, flat[:0])
+    flat.untyped_storage().resize_(23 * 4)
+    for t in (flat, view, rest):
+        with pytest.raises(_C.XqError, match="x: .*no memory"):
+            _C.check_held("x", t)
+    _C.check_held("x", inside, first)
+    flat.untyped_storage().resize_(0)
+    with pytest.raises(_C.XqError, match="no memory"):
+        _C.check_held("x", first)
+    _C.check_held("x", none)

@@ -310,6 +310,15 @@ def require_hip(*tensors: Optional[torch.Tensor]) -> None:
             )
 
 
+def check_held(who: str, *tensors: Optional[torch.Tensor]) -> None:
+    """A tensor whose memory was freed or cut under it is refused: a view into it has an address all the same."""
+    for t in tensors:
+        if t is not None and t.numel():
+            last = t.storage_offset() + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))
+            if (last + 1) * t.element_size() > t.untyped_storage().nbytes():
+                raise XqError(f"{who}: a tensor {tuple(t.shape)} has no memory of its own (any more): it was freed or resized")
+
+
 def ptr(t: Optional[torch.Tensor]) -> Optional[int]:
     """The address of an argument that may be absent: a tensor that is there and has none (a distributed one) would count as that."""
     if t is None:

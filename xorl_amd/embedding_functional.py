@@ -52,6 +52,7 @@ def _one_device(ids: Tensor, other: Tensor) -> None:
 def _fwd_impl(ids: Tensor, weight: Tensor, scale: float) -> Tensor:
     _check(ids, weight)
     _one_device(ids, weight)
+    _C.check_held("embedding", ids, weight)
     dev = weight.device
     with torch.cuda.device(dev):
         i1, w2 = ids.reshape(-1).contiguous().resolve_neg(), _rows(weight)
@@ -66,6 +67,7 @@ def _bwd_impl(grad: Tensor, ids: Tensor, V: int, scale: float, padding_idx: int)
     if grad.dtype not in (torch.bfloat16, torch.float32) or grad.dim() < 1 or grad.shape[-1] < 1 or ids.dtype not in (torch.int64, torch.int32) or V < 1:
         raise _C.XqError("embedding: what the forward kept, or the gradient, is not that of this problem")
     _one_device(ids, grad)
+    _C.check_held("embedding", ids, grad)
     dev = grad.device
     with torch.cuda.device(dev):
         i1, g2 = ids.reshape(-1).contiguous().resolve_neg(), _rows(grad)

@@ -451,6 +451,7 @@ def _check_adapters(base: Tensor, x: Tensor, lora_A: Tensor, lora_B: Tensor, ada
 
 def _adapters_impl(base: Tensor, x: Tensor, A: Tensor, B: Tensor, ids: Tensor, scalings: Tensor, out: Optional[Tensor] = None) -> Tensor:
     _check_adapters(base, x, A, B, ids, scalings, out)     # (the operator can be called by itself, and its dispatcher goes by any one of the tensors)
+    _C.check_held("lora_adapters", base, x, A, B, ids, scalings, out)
     dev = x.device
     with torch.cuda.device(dev):
         x2, base2, i1 = _adapters_rows(x), _adapters_rows(base), ids.reshape(-1).contiguous().resolve_neg()

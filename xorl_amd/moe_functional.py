@@ -86,6 +86,7 @@ def _one_device(*tensors: Optional[Tensor]) -> None:
 def _route_fwd_impl(z: Tensor, bias: Optional[Tensor], options) -> Tuple[Tensor, Tensor]:
     _check_route(z, bias)
     _one_device(z, bias)
+    _C.check_held("moe_route", z, bias)
     dev = z.device
     with torch.cuda.device(dev):
         z2 = _route_rows(z)
@@ -104,6 +105,7 @@ def _route_bwd_impl(grad: Tensor, weights: Tensor, ids: Tensor, z: Tensor, num_e
             or grad.shape != weights.shape):
         raise _C.XqError("moe_route: what the forward kept, or the gradient, is not that of this problem")
     _one_device(weights, ids, grad, z)
+    _C.check_held("moe_route", weights, ids, grad, z)
     dev = weights.device
     with torch.cuda.device(dev):
         n = weights.numel() // options[0]
